@@ -83,7 +83,10 @@ int tb_b200_is_device_ptr(const void* p, int* is_device);
 int tb_b200_check_status(void* stream, unsigned int* flags_out);
 #define TB_B200_FLAG_TOKEN_RANGE 0x1u   /* embedding: id < 0 or id >= vocab */
 #define TB_B200_FLAG_WAIT_TIMEOUT 0x2u  /* a kernel's bounded wait gave up (its output is invalid) */
-#define TB_B200_FLAG_POSITION_RANGE 0x4u /* decode attention: position outside [0, max_seq) */
+#define TB_B200_FLAG_POSITION_RANGE 0x4u /* decode attention: position outside [0, max_seq);
+                                           8-bit cache: a sequence past its bounds */
+#define TB_B200_FLAG_PAGE_RANGE 0x8u     /* 8-bit cache: a page number outside [0, n_pages) */
+#define TB_B200_FLAG_NONFINITE 0x10u     /* 8-bit cache: a NaN or infinity was appended */
 
 /* Runs, in a one-warp kernel, the bounded mbarrier wait the staged kernels
  * use for their bulk copies.  supply != 0: one 16-byte copy completes the
@@ -296,6 +299,188 @@ int tb_b200_sparse24_pack(int64_t out_features, int64_t in_features, const float
 int tb_b200_sparse24_linear(int64_t out_features, int64_t in_features, const float* x,
                             const void* vals, const uint8_t* idx, const float* bias, float* y,
                             void* stream);
+
+/* ======================================================================
+ * Rotary positions and head norms of packed Q/K rows; the 8-bit KV cache
+ * (no counterpart in the reference, whose RoPE is one layout over the whole
+ * head, src/ops/rope.c:43-81, and whose cache is f32, ops.hpp:162-204)
+ * ====================================================================== */
+
+/* Which elements of a head make a pair: (2i, 2i + 1), or (i, i + rotary_dim / 2). */
+#define TB_B200_ROTARY_INTERLEAVED 0
+#define TB_B200_ROTARY_HALF 1
+
+/* How the frequencies theta^(-2i / rotary_dim) are stretched for contexts
+ * longer than the model's training:
+ *   NONE
+ *   LINEAR  f / factor (positions interpolated)
+ *   NTK     theta * factor^(r / (r - 2)) in theta's place (r = rotary_dim > 2)
+ *   BANDS   t = trained * f / 2 pi turns over the training length: f / factor
+ *           for t <= low, f for t >= high, between them the linear mix of both
+ *   YARN    (Peng et al., YaRN, section 3.2) with
+ *           at(t) = r ln(trained / (2 pi t)) / (2 ln theta),
+ *           a = max(floor(at(high)), 0), b = min(ceil(at(low)), r - 1):
+ *           f for i <= a, f / factor for i >= b, between them the linear mix
+ *           in i (b = a: a step of 0.001) */
+#define TB_B200_ROTARY_SCALE_NONE 0
+#define TB_B200_ROTARY_SCALE_LINEAR 1
+#define TB_B200_ROTARY_SCALE_NTK 2
+#define TB_B200_ROTARY_SCALE_BANDS 3
+#define TB_B200_ROTARY_SCALE_YARN 4
+typedef struct {
+    int kind;       /* TB_B200_ROTARY_SCALE_* */
+    double theta;   /* > 0, not 1 for YARN */
+    double factor;  /* > 0 */
+    double trained; /* BANDS, YARN: positions the model was trained on, > 0 */
+    double low;     /* BANDS, YARN: turns, 0 < low < high */
+    double high;
+} TbB200RotaryScaling;
+
+/* freqs_dev[i], i < rotary_dim / 2: the angle per position of pair i, in
+ * double.  rotary_dim even, 2 .. 512 (TB_ERR_INVALID_SHAPE); a value outside
+ * the ranges above is TB_ERR_INVALID_ARG.  Computed on the device: a captured
+ * graph replays it, and later launches on `stream` see the new values. */
+int tb_b200_rotary_freqs(int rotary_dim, const TbB200RotaryScaling* scaling, double* freqs_dev,
+                         void* stream);
+
+/* Q and K rows to rotate.  Row r of q holds n_q_heads heads of head_dim
+ * elements at q + r * q_stride (strides in elements, so q and k may be slices
+ * of one packed QKV row); the same for k and the outputs.  An output may be
+ * its input, with the same stride; any other overlap is undefined.
+ *   rotary_dim  even, <= head_dim: elements past it are passed through
+ *   positions   device int32 [rows], any value
+ *   freqs       device double [rotary_dim / 2] (tb_b200_rotary_freqs)
+ *   scale       factor on cos and sin (YaRN's attention factor; 1 otherwise)
+ * Pair (x0, x1) of a row at position p becomes scale * (x0 cos a - x1 sin a,
+ * x1 cos a + x0 sin a), a = p * freqs[i].  The angle is taken in double and
+ * reduced to a fraction of a turn before cos and sin, so far positions are as
+ * exact as near ones; arithmetic on the elements is f32, rounded once.
+ * tb_b200_rope_rows is the engine's f32 arithmetic instead.
+ * q_weight, k_weight [head_dim] (NULL for ones) and eps are read by
+ * tb_b200_qk_norm_rotary only. */
+typedef struct {
+    int dtype; /* of q, k, the outputs and the weights */
+    int64_t rows;
+    int n_q_heads;
+    int n_kv_heads;
+    int head_dim; /* 1 .. 512 */
+    int rotary_dim;
+    int layout; /* TB_B200_ROTARY_INTERLEAVED / _HALF */
+    const void* q;
+    int64_t q_stride;
+    const void* k;
+    int64_t k_stride;
+    void* q_out;
+    int64_t q_out_stride;
+    void* k_out;
+    int64_t k_out_stride;
+    const int32_t* positions;
+    const double* freqs;
+    float scale;
+    const void* q_weight;
+    const void* k_weight;
+    float eps;
+} TbB200Rotary;
+
+int tb_b200_rotary(const TbB200Rotary* rotary, void* stream);
+/* Each head x normalised first, x / sqrt(mean(x^2) + eps) * weight, with the
+ * f32 result rotated.  (tb_b200_rms_norm adds eps to the sum instead, as the
+ * engine does.)  rotary_dim 0: the norm alone, positions and freqs unused. */
+int tb_b200_qk_norm_rotary(const TbB200Rotary* rotary, void* stream);
+
+/* Code formats of the 8-bit KV cache: two's complement in [-127, 127], or
+ * OCP e4m3 (finite up to 448). */
+#define TB_B200_KV_INT8 TB_DTYPE_INT8
+#define TB_B200_KV_E4M3 0x43
+
+/* A paged KV cache of 8-bit codes.  k and v: [n_pages, n_kv_heads, page,
+ * head_dim] codes, 16-byte aligned; k_scale and v_scale: [n_pages,
+ * n_kv_heads], the power of two a page's codes of that head are multiplied
+ * with.  All device memory of the caller's. */
+typedef struct {
+    int format; /* TB_B200_KV_* */
+    int page;   /* tokens per page: 16, 32, 64 or 128 */
+    int n_kv_heads;
+    int head_dim; /* a multiple of 16, at most 256 */
+    int64_t n_pages;
+    void* k;
+    void* v;
+    float* k_scale;
+    float* v_scale;
+} TbB200Kv8;
+
+/* A batch of sequences over such a cache.  Sequence i owns rows
+ * row_start[i] .. row_start[i + 1] - 1 of the call's q, k or v, none or more;
+ * they are its last tokens: after them it has lengths[i] tokens, and its row
+ * t stands at position lengths[i] - (its rows) + t.  A row at a negative
+ * position is padding.  Rows from row_start[n_seqs] on belong to nobody.
+ * Token j of sequence i is in page page_table[i * table_stride + j / page].
+ * row_start, lengths and page_table are device int32, so a captured graph
+ * replays with new ones. */
+typedef struct {
+    int n_seqs;
+    int64_t rows; /* rows in the call's buffers, >= row_start[n_seqs] */
+    const int32_t* row_start; /* [n_seqs + 1], not decreasing, from 0 */
+    const int32_t* lengths;   /* [n_seqs] */
+    const int32_t* page_table;
+    int table_width;          /* pages per sequence at most */
+    int64_t table_stride;     /* elements between sequences, >= table_width */
+} TbB200Kv8Batch;
+
+/* Store the batch's K and V rows ([rows, n_kv_heads, head_dim] f32 or bf16,
+ * rows k_stride and v_stride elements apart) in the cache.  For each page,
+ * head and K or V that gets rows:
+ *   s = max(least power of two with amax <= MAX * s, 2^-100, the page's scale
+ *           if it holds earlier tokens of the sequence)
+ * amax over the new rows, MAX 127 (int8) or 448 (e4m3); where s is above the
+ * earlier scale, the earlier codes c become rne(c * scale / s), rounded to the
+ * format; new codes are rne(x / s).  Scaling by powers of two is exact, so
+ * the only errors are these roundings, and those of a page's rescalings halve
+ * each time: their sum is below one step.  NaN is stored as 0 and an infinity
+ * as the largest code, and TB_B200_FLAG_NONFINITE is raised.  Slots after a
+ * sequence's last token and padding rows change nothing.  A sequence with
+ * lengths[i] > table_width * page raises TB_B200_FLAG_POSITION_RANGE and
+ * loses the tokens past it; a page number outside [0, n_pages) raises
+ * TB_B200_FLAG_PAGE_RANGE and loses that page's.  Two sequences of one call
+ * must not append to the same page. */
+int tb_b200_kv8_append(const TbB200Kv8* cache, const TbB200Kv8Batch* batch, int dtype,
+                       const void* k, int64_t k_stride, const void* v, int64_t v_stride,
+                       void* stream);
+
+/* Attention of the batch's Q rows over the cache (their own keys and values
+ * appended before).  Head h of a row at position p attends keys j of k/v head
+ * h / (n_heads / n_kv_heads) with max(0, p - window + 1) <= j <= p (window 0:
+ * from 0): out = sum_j softmax_j(scale q.k_j) v_j, lse = ln sum_j exp(scale
+ * q.k_j) (f32).  A row without keys (padding) gets out = 0, lse = -inf; rows
+ * of nobody are left as they were.  A sequence whose length is above max_len
+ * or table_width * page, or with more than max_rows rows, raises
+ * TB_B200_FLAG_POSITION_RANGE and its rows are as without keys; keys in a
+ * page outside [0, n_pages) are not attended and raise
+ * TB_B200_FLAG_PAGE_RANGE.  What the cache holds in slots that a row does not
+ * attend never reaches its result. */
+typedef struct {
+    int dtype; /* of q and out: TB_DTYPE_F32 or TB_DTYPE_BF16 */
+    int n_heads; /* a multiple of the cache's n_kv_heads */
+    const void* q; /* [rows, n_heads, head_dim], rows q_stride elements apart */
+    int64_t q_stride;
+    void* out; /* the same, out_stride apart; not q */
+    int64_t out_stride;
+    float* lse; /* [rows, n_heads] dense, or NULL */
+    float scale; /* usually 1 / sqrt(head_dim) */
+    int window; /* >= 0 */
+    int max_rows; /* most rows of one sequence */
+    int max_len; /* most tokens of one sequence */
+    void* workspace; /* 16-byte aligned device memory, at least */
+    size_t workspace_bytes; /* tb_b200_kv8_attention_workspace's bytes */
+} TbB200Kv8Attention;
+
+int tb_b200_kv8_attention(const TbB200Kv8* cache, const TbB200Kv8Batch* batch,
+                          const TbB200Kv8Attention* attention, void* stream);
+/* Bytes of device scratch that call needs on the current device (0 when none):
+ * calls that may overlap on the GPU need scratch of their own.  The pointers
+ * and workspace fields are not read. */
+int tb_b200_kv8_attention_workspace(const TbB200Kv8* cache, const TbB200Kv8Batch* batch,
+                                    const TbB200Kv8Attention* attention, size_t* bytes);
 
 /* ======================================================================
  * Decoder forward on the device (TransformerRunner)

@@ -76,6 +76,11 @@ P = C.POINTER
 INT8, INT4 = 7, 8  # TbDtype codes of quantized weights
 ATTN_REFERENCE, ATTN_STANDARD = 0, 1
 FLAG_POSITION_RANGE = 0x4
+FLAG_PAGE_RANGE = 0x8
+FLAG_NONFINITE = 0x10
+ROTARY_INTERLEAVED, ROTARY_HALF = 0, 1
+ROTARY_SCALING = {"none": 0, "linear": 1, "ntk": 2, "bands": 3, "yarn": 4}
+KV_INT8, KV_E4M3 = 7, 0x43
 PROJECTIONS = ("q", "k", "v", "o", "gate", "up", "down")
 
 
@@ -106,6 +111,36 @@ class TbmTensor(C.Structure):  # TbB200TbmTensor
                 ("nm_n", C.c_uint32), ("nm_m", C.c_uint32), ("num_weights", i64),
                 ("num_mask_bytes", i64), ("scale_count", i64), ("group_size", C.c_uint32),
                 ("weights", vp), ("mask", vp), ("scales", vp), ("weight_bytes", i64)]
+
+
+class Rotary(C.Structure):  # TbB200Rotary
+    _fields_ = [("dtype", i32), ("rows", i64), ("n_q_heads", i32), ("n_kv_heads", i32),
+                ("head_dim", i32), ("rotary_dim", i32), ("layout", i32), ("q", vp),
+                ("q_stride", i64), ("k", vp), ("k_stride", i64), ("q_out", vp),
+                ("q_out_stride", i64), ("k_out", vp), ("k_out_stride", i64), ("positions", vp),
+                ("freqs", vp), ("scale", f32), ("q_weight", vp), ("k_weight", vp), ("eps", f32)]
+
+
+class RotaryScaling(C.Structure):  # TbB200RotaryScaling
+    _fields_ = [("kind", i32)] + [(n, C.c_double) for n in ("theta", "factor", "trained", "low",
+                                                            "high")]
+
+
+class Kv8(C.Structure):  # TbB200Kv8
+    _fields_ = [("format", i32), ("page", i32), ("n_kv_heads", i32), ("head_dim", i32),
+                ("n_pages", i64), ("k", vp), ("v", vp), ("k_scale", vp), ("v_scale", vp)]
+
+
+class Kv8Batch(C.Structure):  # TbB200Kv8Batch
+    _fields_ = [("n_seqs", i32), ("rows", i64), ("row_start", vp), ("lengths", vp),
+                ("page_table", vp), ("table_width", i32), ("table_stride", i64)]
+
+
+class Kv8Attention(C.Structure):  # TbB200Kv8Attention
+    _fields_ = [("dtype", i32), ("n_heads", i32), ("q", vp), ("q_stride", i64), ("out", vp),
+                ("out_stride", i64), ("lse", vp), ("scale", f32), ("window", i32),
+                ("max_rows", i32), ("max_len", i32), ("workspace", vp),
+                ("workspace_bytes", C.c_size_t)]
 
 
 # name -> (restype, argtypes); every entry point of include/tb_b200.h and tb_backend.h.
@@ -154,6 +189,13 @@ SIGNATURES = {
     "tb_b200_sparse24_pack": (i32, [i64, i64, vp, vp, vp, vp, vp, vp]),
     "tb_b200_sparse24_linear": (i32, [i64, i64, vp, vp, vp, vp, vp, vp]),
     "tb_b200_decode_attention": (i32, [i32, i32, i32, i32, i32, vp, vp, vp, vp, vp, vp, vp, vp]),
+    "tb_b200_rotary_freqs": (i32, [i32, P(RotaryScaling), vp, vp]),
+    "tb_b200_rotary": (i32, [P(Rotary), vp]),
+    "tb_b200_qk_norm_rotary": (i32, [P(Rotary), vp]),
+    "tb_b200_kv8_append": (i32, [P(Kv8), P(Kv8Batch), i32, vp, i64, vp, i64, vp]),
+    "tb_b200_kv8_attention": (i32, [P(Kv8), P(Kv8Batch), P(Kv8Attention), vp]),
+    "tb_b200_kv8_attention_workspace": (i32, [P(Kv8), P(Kv8Batch), P(Kv8Attention),
+                                              P(C.c_size_t)]),
     "tb_b200_runner_create": (i32, [P(RunnerDesc), P(vp)]),
     "tb_b200_runner_forward": (i32, [vp, C.c_int32, P(vp)]),
     "tb_b200_runner_logits": (i32, [vp, vp]),
@@ -648,6 +690,214 @@ def embedding_sharded_p2p(ids, shard_addrs, vocab: int, dim: int, dtype, y=None,
                                               arr, len(shard_addrs), ptr(y),
                                               stream or cur_stream()), "embedding_sharded_p2p")
     return y
+
+
+# ------------------------- rotary positions, head norms, the 8-bit KV cache
+def _new(shape, dtype, device, stream):
+    """An uninitialised tensor for a call on `stream`: from that stream's pool, so that the
+    memory's earlier uses are ordered before the call and its later ones after it."""
+    torch = _torch()
+    if stream is None:
+        return torch.empty(shape, dtype=dtype, device=device)
+    s = torch.cuda.ExternalStream(getattr(stream, "value", stream) or 0)
+    with torch.cuda.stream(s):
+        return torch.empty(shape, dtype=dtype, device=device)
+
+
+def _rows3(*ts):
+    """[rows, heads, head_dim] tensors whose heads are dense within a row."""
+    for t in ts:
+        if not t.is_cuda or t.dim() != 3 or (t.shape[2] > 1 and t.stride(2) != 1) or (
+                t.shape[1] > 1 and t.stride(1) != t.shape[2]):
+            raise ValueError("expected CUDA [rows, heads, head_dim] tensors, heads dense in a row")
+
+
+def _here(*ts):
+    """Every tensor on the current device, where the launch goes."""
+    dev = _torch().cuda.current_device()
+    for t in ts:
+        if t is not None and t.device.index != dev:
+            raise ValueError(f"tensor on {t.device}, but the current device is cuda:{dev}")
+
+
+def _typed(what, dtype, *ts):
+    for t in ts:
+        if t is not None and t.dtype != dtype:
+            raise TypeError(f"{what} must be {dtype}, got {t.dtype}")
+
+
+def rotary_freqs(rotary_dim, theta, scaling="none", factor=1.0, trained=0.0, low=0.0, high=0.0,
+                 out=None, stream=None):
+    """Angle per position of each of rotary_dim / 2 pairs (float64, on the
+    device), stretched by `scaling`: "none", "linear", "ntk", "bands" or
+    "yarn" (tb_b200_rotary_freqs)."""
+    torch = _torch()
+    if out is None:
+        out = _new(rotary_dim // 2, torch.float64, "cuda", stream)
+    _dev(out)
+    _here(out)
+    _typed("out", torch.float64, out)
+    if out.numel() != rotary_dim // 2:
+        raise ValueError("out must have rotary_dim / 2 elements")
+    sc = RotaryScaling(ROTARY_SCALING[scaling], theta, factor, trained, low, high)
+    check(lib().tb_b200_rotary_freqs(rotary_dim, C.byref(sc), ptr(out), stream or cur_stream()),
+          "rotary_freqs")
+    return out
+
+
+def _rotary(fn, what, q, k, q_weight, k_weight, eps, positions, freqs, layout, scale, q_out,
+            k_out, stream):
+    torch = _torch()
+    q_out = _new(q.shape, q.dtype, q.device, stream) if q_out is None else q_out
+    k_out = _new(k.shape, k.dtype, k.device, stream) if k_out is None else k_out
+    _rows3(q, k, q_out, k_out)
+    _dev(positions, freqs, q_weight, k_weight)
+    _here(q, k, q_out, k_out, positions, freqs, q_weight, k_weight)
+    _typed("k, the outputs and the weights", q.dtype, k, q_out, k_out, q_weight, k_weight)
+    _typed("positions", torch.int32, positions)
+    _typed("freqs", torch.float64, freqs)
+    rows, hq, d = q.shape
+    if k.shape[0] != rows or k.shape[2] != d or q_out.shape != q.shape or k_out.shape != k.shape:
+        raise ValueError("q, k and the outputs do not agree in rows or head_dim")
+    if freqs is not None and (positions is None or positions.numel() != rows):
+        raise ValueError("positions must have one element per row")
+    if any(w is not None and w.numel() != d for w in (q_weight, k_weight)):
+        raise ValueError("a norm weight must have head_dim elements")
+    t = Rotary(dtype_code(q), rows, hq, k.shape[1], d, 0 if freqs is None else 2 * freqs.numel(),
+               layout, q.data_ptr(), q.stride(0), k.data_ptr(), k.stride(0), q_out.data_ptr(),
+               q_out.stride(0), k_out.data_ptr(), k_out.stride(0),
+               None if positions is None else positions.data_ptr(),
+               None if freqs is None else freqs.data_ptr(), scale,
+               None if q_weight is None else q_weight.data_ptr(),
+               None if k_weight is None else k_weight.data_ptr(), eps)
+    check(getattr(lib(), fn)(C.byref(t), stream or cur_stream()), what)
+    return q_out, k_out
+
+
+def rotary(q, k, positions, freqs, layout=ROTARY_HALF, scale=1.0, q_out=None, k_out=None,
+           stream=None):
+    """Rotary positions of q [R, Hq, d] and k [R, Hkv, d], whose rows may be
+    strided (slices of a packed QKV): the first 2 * freqs.numel() elements of
+    each head, at int32 positions [R] (tb_b200_rotary).  New tensors unless
+    q_out and k_out are given; those may be q and k themselves."""
+    return _rotary("tb_b200_rotary", "rotary", q, k, None, None, 0.0, positions, freqs, layout,
+                   scale, q_out, k_out, stream)
+
+
+def qk_norm_rotary(q, k, q_weight, k_weight, eps, positions=None, freqs=None,
+                   layout=ROTARY_HALF, scale=1.0, q_out=None, k_out=None, stream=None):
+    """RMSNorm of each head of q and k (weights [d] or None), then rotary
+    positions, in one pass (tb_b200_qk_norm_rotary); without freqs the norm
+    alone."""
+    return _rotary("tb_b200_qk_norm_rotary", "qk_norm_rotary", q, k, q_weight, k_weight, eps,
+                   positions, freqs, layout, scale, q_out, k_out, stream)
+
+
+class Kv8Cache:
+    """A paged 8-bit KV cache over the caller's tensors: codes k and v
+    [n_pages, n_kv_heads, page, head_dim], int8 or float8_e4m3fn, and float32
+    k_scale and v_scale [n_pages, n_kv_heads] (TbB200Kv8)."""
+
+    def __init__(self, k, v, k_scale, v_scale):
+        torch = _torch()
+        _dev(k, v, k_scale, v_scale)
+        if k.dtype not in (torch.int8, torch.float8_e4m3fn):
+            raise TypeError(f"codes must be int8 or float8_e4m3fn, got {k.dtype}")
+        _typed("v", k.dtype, v)
+        _typed("scales", torch.float32, k_scale, v_scale)
+        if k.dim() != 4 or v.shape != k.shape or k_scale.shape != k.shape[:2] or (
+                v_scale.shape != k.shape[:2]):
+            raise ValueError("codes are [n_pages, n_kv_heads, page, head_dim], scales their first "
+                             "two dimensions")
+        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self.c = Kv8(KV_INT8 if k.dtype == torch.int8 else KV_E4M3, k.shape[2], k.shape[1],
+                     k.shape[3], k.shape[0], k.data_ptr(), v.data_ptr(), k_scale.data_ptr(),
+                     v_scale.data_ptr())
+
+    @classmethod
+    def empty(cls, n_pages, n_kv_heads, page, head_dim, dtype, device=None):
+        """A cache of its own memory; dtype torch.int8 or torch.float8_e4m3fn."""
+        torch = _torch()
+        device = torch.cuda.current_device() if device is None else device
+        codes = [torch.zeros((n_pages, n_kv_heads, page, head_dim), dtype=torch.uint8,
+                             device=device).view(dtype) for _ in range(2)]
+        scales = [torch.zeros((n_pages, n_kv_heads), dtype=torch.float32, device=device)
+                  for _ in range(2)]
+        return cls(*codes, *scales)
+
+
+def _kv8_batch(cache, rows, row_start, lengths, page_table):
+    torch = _torch()
+    _dev(row_start, lengths)
+    _typed("row_start, lengths and page_table", torch.int32, row_start, lengths, page_table)
+    if not page_table.is_cuda or page_table.dim() != 2 or (
+            page_table.shape[1] > 1 and page_table.stride(1) != 1):
+        raise ValueError("page_table must be a CUDA [n_seqs, pages] tensor, dense in a row")
+    _here(cache.k, row_start, lengths, page_table)
+    n, width = page_table.shape
+    if row_start.numel() != n + 1 or lengths.numel() != n:
+        raise ValueError("row_start has n_seqs + 1 elements, lengths n_seqs")
+    return Kv8Batch(n, rows, row_start.data_ptr(), lengths.data_ptr(), page_table.data_ptr(),
+                    width, max(page_table.stride(0), width))
+
+
+def kv8_append(cache, k, v, row_start, lengths, page_table, stream=None):
+    """Store K and V rows [R, n_kv_heads, head_dim] (rows may be strided) as
+    the last tokens of the sequences of a ragged batch (tb_b200_kv8_append):
+    rows row_start[i] : row_start[i + 1] end sequence i at lengths[i] tokens."""
+    _rows3(k, v)
+    _here(k, v)
+    _typed("v", k.dtype, v)
+    if k.shape != v.shape or k.shape[1:] != (cache.c.n_kv_heads, cache.c.head_dim):
+        raise ValueError("k and v must be [rows, n_kv_heads, head_dim] of the cache")
+    b = _kv8_batch(cache, k.shape[0], row_start, lengths, page_table)
+    check(lib().tb_b200_kv8_append(C.byref(cache.c), C.byref(b), dtype_code(k), k.data_ptr(),
+                                   k.stride(0), v.data_ptr(), v.stride(0),
+                                   stream or cur_stream()), "kv8_append")
+
+
+def kv8_attention(cache, q, row_start, lengths, page_table, max_q=None, max_len=None, scale=None,
+                  window=0, out=None, lse=None, return_lse=False, workspace=None, stream=None):
+    """Causal attention of q rows [R, n_heads, head_dim] over the cache
+    (tb_b200_kv8_attention).  max_q and max_len bound the rows and the tokens
+    of one sequence (as many as q and page_table hold without them); scale is
+    1 / sqrt(head_dim) unless given; window > 0 attends that many last keys.
+    Returns out, or (out, lse) with return_lse or lse."""
+    torch = _torch()
+    if out is None:
+        out = _new(q.shape, q.dtype, q.device, stream)
+    _rows3(q, out)
+    _typed("out", q.dtype, out)
+    rows, heads, d = q.shape
+    if out.shape != q.shape or d != cache.c.head_dim:
+        raise ValueError("q and out must be [rows, n_heads, head_dim] of the cache")
+    if lse is None and return_lse:
+        lse = _new((rows, heads), torch.float32, q.device, stream)
+    if lse is not None:
+        _dev(lse)
+        _typed("lse", torch.float32, lse)
+        if lse.shape != (rows, heads):
+            raise ValueError("lse must be [rows, n_heads]")
+    _here(q, out, lse, workspace)
+    b = _kv8_batch(cache, rows, row_start, lengths, page_table)
+    a = Kv8Attention(dtype_code(q), heads, q.data_ptr(), q.stride(0), out.data_ptr(),
+                     out.stride(0), None if lse is None else lse.data_ptr(),
+                     d ** -0.5 if scale is None else scale, window,
+                     rows if max_q is None else max_q,
+                     b.table_width * cache.c.page if max_len is None else max_len, None, 0)
+    L = lib()
+    need = C.c_size_t()
+    check(L.tb_b200_kv8_attention_workspace(C.byref(cache.c), C.byref(b), C.byref(a),
+                                            C.byref(need)), "kv8_attention_workspace")
+    if workspace is None and need.value:
+        workspace = _new(need.value, torch.uint8, q.device, stream)
+    if workspace is not None:
+        _dev(workspace)
+        a.workspace = workspace.data_ptr()
+        a.workspace_bytes = workspace.numel() * workspace.element_size()
+    check(L.tb_b200_kv8_attention(C.byref(cache.c), C.byref(b), C.byref(a),
+                                  stream or cur_stream()), "kv8_attention")
+    return out if lse is None else (out, lse)
 
 
 # ------------------------------------------------ decoder forward (runner)

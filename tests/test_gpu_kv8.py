@@ -1,0 +1,551 @@
+"""The paged 8-bit KV cache (tb_b200_kv8_append, tb_b200_kv8_attention)
+against its definition in 64 bits.
+
+append: codes and scales are exact -- scaling by a power of two loses nothing,
+so every code is the nearest one of an exact quotient -- and compared for
+equality.
+
+attention, per output element, with A = sum_j p_j |v_j| and, per row,
+S = scale max_j sum_i |q_i k_ij|:
+- a score is off by at most ds = S (d / 16 + 16) 2^-23: one f32 rounding or
+  truncation per group of 16 products, q held to 22 bits, the scalings;
+- p_j is off by 2 ds relative (its own score and the maximum's), 2^-21 for
+  exp2 and its argument, and, for bf16 calls, 2^-11 for p as f16;
+- the sum over n keys is accumulated in f32 by groups of 16: (n / 16 + 16) 2^-23;
+- the output is rounded by 2^-24, or 2^-8 as bf16.
+lse: ds and (n / 16 + 16) 2^-23 for the sum, 2^-21 for exp2 and log.
+"""
+import math
+
+import numpy as np
+import pytest
+
+import tb_b200 as T
+
+pytestmark = pytest.mark.gpu
+MOST = {"int8": 127.0, "e4m3": 448.0}
+
+
+@pytest.fixture(scope="module")
+def dev(cuda):
+    import torch
+    torch.cuda.set_device(cuda)
+    T.check_status()
+    return cuda
+
+
+def nearest(x, fmt):
+    if fmt == "int8":
+        return np.rint(x)
+    e = np.maximum(np.frexp(x)[1] - 1, -6)
+    step = np.ldexp(1.0, e - 3)
+    return np.rint(x / step) * step
+
+
+def scale_for(amax, fmt):
+    s = 2.0 ** -100
+    while amax > MOST[fmt] * s:
+        s *= 2
+    return s
+
+
+class Model:
+    """A cache and its batch in 64 bits, beside the device's."""
+
+    def __init__(self, dev, fmt, page, hkv, d, n_pages, seed=0):
+        import torch
+        self.fmt, self.page, self.hkv, self.d, self.dev = fmt, page, hkv, d, dev
+        self.rng = np.random.default_rng(seed + page + d)
+        dt = torch.int8 if fmt == "int8" else torch.float8_e4m3fn
+        self.cache = T.Kv8Cache.empty(n_pages, hkv, page, d, dt)
+        # what was in the memory before: any codes, NaN ones among them
+        for t in (self.cache.k, self.cache.v):
+            t.view(torch.uint8).copy_(torch.from_numpy(
+                self.rng.integers(0, 256, t.shape, dtype=np.uint8)))
+        self.cache.k_scale.fill_(float("nan"))
+        self.cache.v_scale.fill_(float("nan"))
+        self.codes = [f64(t) for t in (self.cache.k, self.cache.v)]
+        self.scales = [np.full((n_pages, hkv), np.nan) for _ in range(2)]
+
+    def append(self, xs, starts, lengths, table):
+        for x, codes, scales in zip(xs, self.codes, self.scales):
+            for i, total in enumerate(lengths):
+                rows = x[starts[i]:starts[i + 1]]
+                first = total - len(rows)
+                for lp in range(max(first, 0) // self.page, -(-total // self.page)):
+                    a, b = max(first, lp * self.page, 0), min(total, (lp + 1) * self.page)
+                    if a >= b:
+                        continue
+                    at, slot = table[i][lp], a - lp * self.page
+                    part = rows[a - first:b - first]
+                    for h in range(self.hkv):
+                        p = part[:, h]
+                        fin = np.abs(p[np.isfinite(p)])
+                        s = scale_for(fin.max() if fin.size else 0.0, self.fmt)
+                        if slot:
+                            s = max(s, scales[at, h])
+                            old = codes[at, h, :slot]
+                            codes[at, h, :slot] = nearest(old * (scales[at, h] / s), self.fmt)
+                        q = np.clip(np.nan_to_num(p / s, nan=0.0, posinf=1e9, neginf=-1e9),
+                                    -MOST[self.fmt], MOST[self.fmt])
+                        codes[at, h, slot:slot + len(p)] = nearest(q, self.fmt)
+                        scales[at, h] = s
+
+    def same(self):
+        for got, want in zip((self.cache.k, self.cache.v), self.codes):
+            np.testing.assert_array_equal(f64(got), want)
+        for got, want in zip((self.cache.k_scale, self.cache.v_scale), self.scales):
+            np.testing.assert_array_equal(f64(got), want)
+
+    def attention(self, q, starts, lengths, table, window=0, scale=None, bad=()):
+        """(out, lse, tolerance of out, of lse) for f64 q [rows, heads, d]."""
+        rows, heads, d = q.shape
+        scale = d ** -0.5 if scale is None else scale
+        out, lse = np.zeros(q.shape), np.full((rows, heads), -np.inf)
+        A, ds, n = np.zeros(q.shape), np.zeros((rows, heads)), np.zeros(rows)
+        for i, total in enumerate(lengths):
+            m = starts[i + 1] - starts[i]
+            if m <= 0 or total <= 0:
+                continue
+            pages = table[i][:-(-total // self.page)]
+            held = np.repeat([p not in bad for p in pages], self.page)[:total]
+            pages = [0 if p in bad else p for p in pages]
+            k, v = (np.nan_to_num(c[pages] * s[pages][:, :, None, None]).transpose(
+                0, 2, 1, 3).reshape(-1, self.hkv, d)[:total]
+                for c, s in zip(self.codes, self.scales))
+            j = np.arange(total)
+            for t in range(m):
+                row, p = starts[i] + t, total - m + t
+                see = held & (j <= p) & ((j > p - window) if window else True)
+                if not see.any():
+                    continue
+                n[row] = see.sum()
+                for h in range(heads):
+                    g = h // (heads // self.hkv)
+                    s = scale * (k[see, g] @ q[row, h])
+                    top = s.max()
+                    e = np.exp(s - top)
+                    w = e / e.sum()
+                    out[row, h] = w @ v[see, g]
+                    lse[row, h] = top + math.log(e.sum())
+                    A[row, h] = w @ np.abs(v[see, g])
+                    ds[row, h] = abs(scale) * (np.abs(k[see, g]) @ np.abs(q[row, h])).max()
+        ds *= (d / 16 + 16) * 2.0 ** -23
+        acc = (n[:, None] / 16 + 16) * 2.0 ** -23
+        rel = 2 * ds + 2.0 ** -21 + acc
+        return out, lse, A, rel, ds + acc + 2.0 ** -21
+
+
+def f64(t):
+    import torch
+    t = t.detach()
+    if t.dtype == torch.float8_e4m3fn:
+        t = t.float()
+    return t.double().cpu().numpy()
+
+
+def i32(a, dev):
+    import torch
+    return torch.tensor(np.asarray(a), dtype=torch.int32, device=dev)
+
+
+def tables(rng, lengths, page, n_pages, width=None):
+    """Pages of each sequence, at random; unused places name no page."""
+    order = rng.permutation(n_pages)
+    width = width or max(1, max(-(-t // page) for t in lengths))
+    table = np.full((len(lengths), width), -5)
+    at = 0
+    for i, t in enumerate(lengths):
+        n = -(-t // page)
+        table[i, :n] = order[at:at + n]
+        at += n
+    return table
+
+
+def rows_of(rng, n, heads, d, bf16, dev, pad=0, spread=True):
+    import torch
+    x = rng.standard_normal((n, heads * d + pad)).astype(np.float32)
+    if spread:
+        x *= np.exp2(rng.integers(-3, 4, (n, 1))).astype(np.float32)
+    t = torch.from_numpy(x).to(torch.bfloat16 if bf16 else torch.float32).to(dev)
+    return t[:, :heads * d].unflatten(1, (heads, d))
+
+
+def starts_of(counts):
+    return np.concatenate([[0], np.cumsum(counts)]).astype(int)
+
+
+def fill(m, lengths, table, bf16=True, spread=True):
+    """The sequences' tokens appended in one call."""
+    st = starts_of(lengths)
+    k, v = (rows_of(m.rng, int(st[-1]), m.hkv, m.d, bf16, m.dev, spread=spread) for _ in range(2))
+    T.kv8_append(m.cache, k, v, i32(st, m.dev), i32(lengths, m.dev), i32(table, m.dev))
+    m.append([f64(k), f64(v)], st, lengths, table)
+
+
+# ------------------------------------------------------------------ append
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("page,hkv,d", [(16, 1, 16), (32, 3, 80), (64, 8, 128), (128, 2, 256),
+                                        (64, 4, 64)])
+def test_append_prompts_then_tokens(dev, fmt, bf16, page, hkv, d):
+    """Prompts, then tokens one at a time and a few at once, every code equal;
+    pages' scales grow on the way and earlier codes are rescaled."""
+    m = Model(dev, fmt, page, hkv, d, 24)
+    lengths = np.array([page, 1, 3 * page - 1, 2 * page + 5, 0])
+    table = tables(m.rng, lengths + page, page, 24)
+    fill(m, lengths, table, bf16)
+    m.same()
+    for counts in ([1, 1, 1, 1, 1], [0, 5, 3, 0, page - 1], [2, 0, page // 2, 1, 1]):
+        counts = np.array(counts)
+        counts = np.minimum(counts, table.shape[1] * page - lengths)
+        lengths = lengths + counts
+        if any((table[i][-(-t // page) - 1] < 0) for i, t in enumerate(lengths) if t):
+            break
+        st = starts_of(counts)
+        k, v = (rows_of(m.rng, int(st[-1]), hkv, d, bf16, dev, pad=3) for _ in range(2))
+        T.kv8_append(m.cache, k, v, i32(st, dev), i32(lengths, dev), i32(table, dev))
+        m.append([f64(k), f64(v)], st, lengths, table)
+        m.same()
+    assert T.check_status() == (0, 0)
+
+
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+def test_append_scale_borders(dev, fmt):
+    """amax at, just under and just over MAX s; zeros; the smallest and the
+    largest values; ties."""
+    import torch
+    most = MOST[fmt]
+    up = float(np.nextafter(np.float32(most), np.float32(np.inf)))
+    down = float(np.nextafter(np.float32(most), np.float32(0)))
+    peaks = [most, up, down, 0.0, 1e-38, 1e-45, 2.0 ** -100 * most, 2.0 ** -101 * most, 3.4e38,
+             2.0 ** 127, most * 2.0 ** -20, up * 2.0 ** 30]
+    m = Model(dev, fmt, 16, 1, 16, len(peaks))
+    x = np.zeros((len(peaks), 1, 16), np.float32)
+    for i, p in enumerate(peaks):
+        x[i, 0] = np.float32(p) * ((np.arange(16) - 8.0) / 8.0).astype(np.float32)
+        x[i, 0, 9:12] = np.float32(p / (2 * most)) * np.array([1, 3, -5], np.float32)
+    lengths = np.ones(len(peaks), int)
+    table = np.arange(len(peaks))[:, None]
+    t = torch.from_numpy(x).to(dev)
+    T.kv8_append(m.cache, t, -t, i32(starts_of(lengths), dev), i32(lengths, dev), i32(table, dev))
+    m.append([x.astype(np.float64), -x.astype(np.float64)], starts_of(lengths), lengths, table)
+    m.same()
+    assert T.check_status() == (0, 0)
+
+
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+def test_append_nonfinite_is_flagged(dev, fmt):
+    import torch
+    m = Model(dev, fmt, 16, 2, 32, 2)
+    x = m.rng.standard_normal((3, 2, 32)).astype(np.float32)
+    x[0, 0, 3], x[1, 0, 4], x[2, 1, 5] = np.nan, np.inf, -np.inf
+    t = torch.from_numpy(x).to(dev)
+    T.kv8_append(m.cache, t, t, i32([0, 3], dev), i32([3], dev), i32([[1]], dev))
+    m.append([x.astype(np.float64)] * 2, [0, 3], [3], [[1]])
+    m.same()
+    assert T.check_status() == (8, T.FLAG_NONFINITE)
+
+
+def test_append_padding_and_bounds(dev):
+    """Rows before position 0, rows behind the last sequence, pages out of
+    range, a table that is too short, and malformed row_start values."""
+    import torch
+    m = Model(dev, "int8", 16, 2, 64, 6)
+    k, v = (rows_of(m.rng, 40, 2, 64, True, dev) for _ in range(2))
+    # sequence 0: three rows, one token; sequence 1: none; sequence 2: idle slot
+    st, lengths, table = [0, 3, 3, 4], [1, 0, 0], [[2], [0], [1]]
+    T.kv8_append(m.cache, k, v, i32(st, dev), i32(lengths, dev), i32(table, dev))
+    m.append([f64(k), f64(v)], st, lengths, table)
+    m.same()
+    assert T.check_status() == (0, 0)
+    # a bad page between two good ones
+    st, lengths, table = [0, 40], [40], [[3, 6, 4]]
+    T.kv8_append(m.cache, k, v, i32(st, dev), i32(lengths, dev), i32(table, dev))
+    x = [f64(k), f64(v)]
+    m.append([a[:16] for a in x], [0, 16], [16], [[3]])
+    m.append([a[32:] for a in x], [0, 8], [8], [[4]])
+    m.same()
+    assert T.check_status() == (8, T.FLAG_PAGE_RANGE)
+    # 40 tokens, room for 32
+    T.kv8_append(m.cache, k, v, i32([0, 40], dev), i32([40], dev), i32([[0, 5]], dev))
+    m.append([a[:32] for a in x], [0, 32], [32], [[0, 5]])
+    m.same()
+    assert T.check_status() == (8, T.FLAG_POSITION_RANGE)
+    # row_start outside the rows: clamped
+    T.kv8_append(m.cache, k, v, i32([-7, 2 ** 30], dev), i32([40], dev), i32([[0, 5, 1]], dev))
+    m.append(x, [0, 40], [40], [[0, 5, 1]])
+    m.same()
+    T.kv8_append(m.cache, k, v, i32([9, 3], dev), i32([40], dev), i32([[0, 5, 1]], dev))
+    m.same()
+    assert T.check_status() == (0, 0)
+    torch.cuda.synchronize()
+
+
+# --------------------------------------------------------------- attention
+def attend(m, counts, lengths, table, heads, bf16, window=0, scale=None, q=None, bad=(), extra=0,
+           pad=0, **kw):
+    import torch
+    st = starts_of(counts)
+    if q is None:
+        q = rows_of(m.rng, int(st[-1]) + extra, heads, m.d, bf16, m.dev, pad=pad, spread=False)
+    out = torch.full(q.shape, 7.0, dtype=q.dtype, device=m.dev)
+    lse = torch.full(q.shape[:2], 7.0, device=m.dev)
+    T.kv8_attention(m.cache, q, i32(st, m.dev), i32(lengths, m.dev), i32(table, m.dev),
+                    window=window, scale=scale, out=out, lse=lse, **kw)
+    y, z, A, rel, tol = m.attention(f64(q), st, lengths, table, window, scale, bad)
+    n = int(st[-1])
+    half = 2.0 ** -8 if bf16 else 2.0 ** -24
+    if bf16:
+        rel = rel + 2.0 ** -11
+    o, ls = f64(out)[:n], f64(lse)[:n]
+    lim = A[:n] * rel[:n, :, None] + half * np.abs(y[:n]) + 1e-37
+    off = np.abs(o - y[:n])
+    assert (off <= lim).all(), ("out", (off / lim).max(), np.argwhere(off > lim)[:5])
+    np.testing.assert_array_equal(np.isneginf(ls), np.isneginf(z[:n]))
+    fin = np.isfinite(z[:n])
+    off = np.abs(ls[fin] - z[:n][fin])
+    assert (off <= (tol[:n] + 2.0 ** -23 * np.abs(z[:n]))[fin]).all(), ("lse", off.max())
+    if extra:  # rows of nobody
+        assert bool((out[n:] == 7.0).all()) and bool((lse[n:] == 7.0).all())
+    return out, lse
+
+
+SHAPES = [  # page, heads, kv heads, d
+    (16, 4, 4, 64), (64, 64, 8, 128), (32, 7, 1, 80), (128, 2, 2, 256), (64, 12, 4, 96),
+    (16, 3, 3, 16), (64, 40, 2, 128), (64, 6, 2, 208)]
+
+
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("page,heads,hkv,d", SHAPES)
+def test_single_tokens(dev, fmt, bf16, page, heads, hkv, d):
+    """One query per sequence, lengths from none to many pages."""
+    lengths = [1, 2, page - 1, page, page + 1, 0, 3 * page + 7, 517, 16, 17]
+    m = Model(dev, fmt, page, hkv, d, sum(-(-t // page) for t in lengths) + 1)
+    table = tables(m.rng, lengths, page, len(m.scales[0]))
+    fill(m, lengths, table)
+    attend(m, [1] * len(lengths), lengths, table, heads, bf16, extra=2)
+    assert T.check_status() == (0, 0)
+
+
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("window", [0, 1, 37, 1000])
+@pytest.mark.parametrize("page,heads,hkv,d", [(16, 8, 2, 64), (64, 8, 1, 128), (32, 2, 2, 112)])
+def test_ragged_queries(dev, fmt, bf16, page, heads, hkv, d, window):
+    """None to many queries per sequence, more queries than tokens among them."""
+    counts = [1, 0, 5, 17, 70, 33, 4]
+    lengths = [300, 40, 5, 120, 70, 333, 2]
+    m = Model(dev, fmt, page, hkv, d, sum(-(-t // page) for t in lengths), seed=window)
+    table = tables(m.rng, lengths, page, len(m.scales[0]))
+    fill(m, lengths, table)
+    attend(m, counts, lengths, table, heads, bf16, window=window, pad=5, extra=3)
+    assert T.check_status() == (0, 0)
+
+
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("window", [0, 3000])
+def test_long_sequences(dev, fmt, bf16, window):
+    """Rows whose keys are split over the device and joined again."""
+    lengths = [9001, 20, 4097]
+    m = Model(dev, fmt, 64, 2, 128, 300)
+    table = tables(m.rng, lengths, 64, 300, width=200)
+    fill(m, lengths, table, spread=False)
+    attend(m, [1, 1, 1], lengths, table, 8, bf16, window=window)
+    attend(m, [3, 1, 20], lengths, table, 4, bf16, window=window)
+    assert T.check_status() == (0, 0)
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+def test_peaked_tiny_and_huge_scores(dev, bf16):
+    """One key that takes all the weight, scores far apart, a zero and a
+    negative scale, q of very small and very large values."""
+    import torch
+    lengths = [200, 90]
+    m = Model(dev, "int8", 64, 1, 64, 6)
+    table = tables(m.rng, lengths, 64, 6)
+    fill(m, lengths, table)
+    for factor in (50.0, 1e-30, 0.0):
+        q = rows_of(m.rng, 2, 4, 64, bf16, dev, spread=False) * factor
+        attend(m, [1, 1], lengths, table, 4, bf16, q=q)
+    for scale in (0.0, -0.3, 2.0):
+        attend(m, [1, 1], lengths, table, 4, bf16, scale=scale)
+    q = rows_of(m.rng, 2, 4, 64, bf16, dev, spread=False)
+    q[:, :, 5] *= 1e-6  # elements far below their row's largest
+    attend(m, [1, 1], lengths, table, 4, bf16, q=q)
+    big = torch.full((2, 4, 64), 1e30, device=dev).to(q.dtype) * torch.sign(q)
+    attend(m, [1, 1], lengths, table, 4, bf16, q=big, scale=1e-31)
+
+
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+def test_pages_of_very_different_scales(dev, fmt):
+    """Values of pages 2^60 apart: each page's scale is its own."""
+    import torch
+    m = Model(dev, fmt, 16, 1, 32, 8)
+    table = [[3, 1, 7, 0, 5]]
+    x = m.rng.standard_normal((2, 70, 1, 32)).astype(np.float32)
+    for p, e in enumerate([0, -60, 30, -30, 0]):
+        x[1, 16 * p:16 * p + 16] *= np.float32(2.0 ** e)
+        x[0, 16 * p:16 * p + 16] *= np.float32(2.0 ** (e // 30))
+    k, v = (torch.from_numpy(a).to(dev) for a in x)
+    T.kv8_append(m.cache, k, v, i32([0, 70], dev), i32([70], dev), i32(table, dev))
+    m.append([a.astype(np.float64) for a in x], [0, 70], [70], table)
+    m.same()
+    for counts in ([1], [40]):
+        attend(m, counts, [70], table, 2, False)
+    for n in (16, 32):  # the small pages alone
+        attend(m, [1], [n], table, 2, False, window=16)
+
+
+def test_bounds_are_flagged(dev):
+    import torch
+    lengths = [100, 60]
+    m = Model(dev, "int8", 16, 2, 64, 12)
+    table = tables(m.rng, lengths, 16, 12)
+    fill(m, lengths, table)
+    # a page out of range: its keys are not attended
+    broken = table.copy()
+    broken[0, 2], broken[1, 1] = 12, -1
+    attend(m, [1, 2], lengths, broken, 4, True, bad=(12, -1))
+    assert T.check_status() == (8, T.FLAG_PAGE_RANGE)
+    # beyond max_len, max_q and the table: as without keys
+    q = rows_of(m.rng, 5, 4, 64, True, dev)
+    for kw, n in ((dict(max_len=99), 100), (dict(max_q=2), 100), ({}, 113)):
+        out, lse = T.kv8_attention(m.cache, q, i32([0, 3, 5], dev), i32([n, 60], dev),
+                                   i32(table, dev), return_lse=True, **kw)
+        assert bool((out[:3] == 0).all()) and bool(torch.isneginf(lse[:3]).all())
+        assert bool((out[3:] != 0).any()) and bool(torch.isfinite(lse[3:]).all())
+        assert T.check_status() == (8, T.FLAG_POSITION_RANGE)
+
+
+def test_nan_query_stays_its_own(dev):
+    import torch
+    m = Model(dev, "e4m3", 16, 1, 64, 4)
+    table = tables(m.rng, [50], 16, 4)
+    fill(m, [50], table)
+    q = rows_of(m.rng, 3, 2, 64, True, dev)
+    want = T.kv8_attention(m.cache, q, i32([0, 3], dev), i32([50], dev), i32(table, dev))
+    q = q.clone()
+    q[1, 0, 7] = float("nan")
+    got = T.kv8_attention(m.cache, q, i32([0, 3], dev), i32([50], dev), i32(table, dev))
+    assert bool(torch.isnan(got[1, 0]).all())
+    keep = torch.ones(3, 2, dtype=torch.bool, device=dev)
+    keep[1, 0] = False
+    assert torch.equal(got[keep], want[keep])
+
+
+def test_large_page_numbers(dev):
+    """Codes more than 2^31 bytes into the cache."""
+    n, page, d = 9000, 128, 256
+    m = Model.__new__(Model)
+    import torch
+    m.fmt, m.page, m.hkv, m.d, m.dev = "int8", page, 8, d, dev
+    m.rng = np.random.default_rng(3)
+    m.cache = T.Kv8Cache.empty(n, 8, page, d, torch.int8)
+    used = [8998, 8191, 8999]
+    m.codes = [np.zeros((3, 8, page, d)) for _ in range(2)]
+    m.scales = [np.zeros((3, 8)) for _ in range(2)]
+    lengths = [300]
+    st = starts_of(lengths)
+    k, v = (rows_of(m.rng, 300, 8, d, True, dev) for _ in range(2))
+    T.kv8_append(m.cache, k, v, i32(st, dev), i32(lengths, dev), i32([used], dev))
+    m.append([f64(k), f64(v)], st, lengths, [[0, 1, 2]])
+    for got, want in zip((m.cache.k, m.cache.v), m.codes):
+        np.testing.assert_array_equal(f64(got[used]), want)
+    q = rows_of(m.rng, 1, 8, d, True, dev)
+    out = T.kv8_attention(m.cache, q, i32([0, 1], dev), i32(lengths, dev), i32([used], dev))
+    y, _, A, rel, _ = m.attention(f64(q), [0, 1], lengths, [[0, 1, 2]])
+    assert (np.abs(f64(out) - y) <= A * (rel + 2.0 ** -11)[..., None] + 2.0 ** -8 * np.abs(y)).all()
+
+
+# ---------------------------------------------------------------- together
+def test_decode_steps_from_a_graph(dev):
+    """A prompt, then decode steps as one captured graph: head norms with
+    rotary positions, append, attention; lengths and positions advance on the
+    device."""
+    import torch
+    heads, hkv, d, page, seqs = 8, 2, 64, 16, 3
+    m = Model(dev, "int8", page, hkv, d, 40)
+    lengths = np.array([30, 5, 16])
+    table = tables(m.rng, lengths + 20, page, 40)
+    fill(m, lengths, table)
+    qkv = torch.empty(seqs, heads + 2 * hkv, d, dtype=torch.bfloat16, device=dev)
+    q, k, v = qkv[:, :heads], qkv[:, heads:heads + hkv], qkv[:, heads + hkv:]
+    w = torch.ones(d, dtype=torch.bfloat16, device=dev)
+    fr = T.rotary_freqs(d, 1e4)
+    start, length = i32(range(seqs + 1), dev), i32(lengths, dev)
+    pos, tab = i32(lengths - 1, dev), i32(table, dev)
+    qr, kr = torch.empty_like(q), torch.empty_like(k)
+    out = torch.empty_like(qr)
+    ws = torch.empty(64 << 20, dtype=torch.uint8, device=dev)
+
+    def step():
+        length.add_(1)
+        pos.add_(1)
+        T.qk_norm_rotary(q, k, w, w, 1e-6, pos, fr, q_out=qr, k_out=kr)
+        T.kv8_append(m.cache, kr, v, start, length, tab)
+        T.kv8_attention(m.cache, qr, start, length, tab, max_q=1, out=out, workspace=ws)
+
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    for n in range(20):
+        qkv.copy_(torch.from_numpy(m.rng.standard_normal(qkv.shape).astype(np.float32)))
+        graph.replay()
+        lengths = lengths + 1
+        m.append([f64(kr), f64(v)], range(seqs + 1), lengths, table)
+        y, _, A, rel, _ = m.attention(f64(qr), range(seqs + 1), lengths, table)
+        assert (np.abs(f64(out) - y) <= A * (rel + 2.0 ** -11)[..., None]
+                + 2.0 ** -8 * np.abs(y)).all()
+    m.same()
+    assert T.check_status() == (0, 0)
+
+
+def test_two_streams_and_repeats(dev):
+    """Calls at once on two streams, each with its own scratch, and the same
+    call again: the same bits."""
+    import torch
+    lengths = [5000, 3000]
+    m = Model(dev, "e4m3", 64, 2, 128, 130)
+    table = tables(m.rng, lengths, 64, 130)
+    fill(m, lengths, table)
+    q = [rows_of(m.rng, 2, 16, 128, True, dev) for _ in range(2)]
+    args = (i32([0, 1, 2], dev), i32(lengths, dev), i32(table, dev))
+    want = [T.kv8_attention(m.cache, x, *args) for x in q]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = [[], []]
+    for _ in range(20):
+        for i, s in enumerate(streams):
+            got[i].append(T.kv8_attention(m.cache, q[i], *args, stream=s.cuda_stream))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(want[i], g) for g in got[i])
+
+
+def test_python_refusals(dev):
+    import torch
+    m = Model(dev, "int8", 16, 2, 64, 4)
+    q = rows_of(m.rng, 2, 4, 64, True, dev)
+    k = rows_of(m.rng, 2, 2, 64, True, dev)
+    st, ln, tb = i32([0, 1, 2], dev), i32([1, 1], dev), i32([[0], [1]], dev)
+    with pytest.raises(TypeError):
+        T.kv8_append(m.cache, k, k, st.long(), ln, tb)
+    with pytest.raises(TypeError):
+        T.kv8_append(m.cache, k, k.float(), st, ln, tb)
+    with pytest.raises(ValueError):
+        T.kv8_append(m.cache, q, q, st, ln, tb)
+    with pytest.raises(ValueError):
+        T.kv8_append(m.cache, k, k, st[:2], ln, tb)
+    with pytest.raises(ValueError):
+        T.kv8_attention(m.cache, q[:, :, :32], st, ln, tb)
+    with pytest.raises(T.TbError):
+        T.kv8_attention(m.cache, q[:, :3], st, ln, tb)
+    with pytest.raises(T.TbError):
+        T.kv8_attention(m.cache, q, st, ln, tb, out=q)
+    with pytest.raises(TypeError):
+        T.kv8_attention(m.cache, q.half(), st, ln, tb)
+    with pytest.raises(TypeError):
+        T.Kv8Cache(m.cache.k.view(torch.uint8), m.cache.v, m.cache.k_scale, m.cache.v_scale)
