@@ -12,6 +12,10 @@ S = scale max_j sum_i |q_i k_ij|:
 - p_j is off by 2 ds relative (its own score and the maximum's), 2^-21 for
   exp2 and its argument, and, for bf16 calls, 2^-11 for p as f16;
 - the sum over n keys is accumulated in f32 by groups of 16: (n / 16 + 16) 2^-23;
+- the weights p_j scale_j (scale_j the page's for v) are held as f16, or two of
+  them, times 2^11 over a power of two that is at most twice the largest: where
+  that is subnormal its half step 2^-25 is 2^-35 of the largest, so the output
+  is off by 2^-35 max_j(p_j scale_j) sum_j |code_j| however small p_j |v_j| is;
 - the output is rounded by 2^-24, or 2^-8 as bf16.
 lse: ds and (n / 16 + 16) 2^-23 for the sum, 2^-21 for exp2 and log.
 """
@@ -98,11 +102,12 @@ class Model:
             np.testing.assert_array_equal(f64(got), want)
 
     def attention(self, q, starts, lengths, table, window=0, scale=None, bad=()):
-        """(out, lse, tolerance of out, of lse) for f64 q [rows, heads, d]."""
+        """(out, lse, A, tolerance of out, of lse) for f64 q [rows, heads, d]."""
         rows, heads, d = q.shape
         scale = d ** -0.5 if scale is None else scale
         out, lse = np.zeros(q.shape), np.full((rows, heads), -np.inf)
         A, ds, n = np.zeros(q.shape), np.zeros((rows, heads)), np.zeros(rows)
+        floor = np.zeros(q.shape)
         for i, total in enumerate(lengths):
             m = starts[i + 1] - starts[i]
             if m <= 0 or total <= 0:
@@ -113,6 +118,7 @@ class Model:
             k, v = (np.nan_to_num(c[pages] * s[pages][:, :, None, None]).transpose(
                 0, 2, 1, 3).reshape(-1, self.hkv, d)[:total]
                 for c, s in zip(self.codes, self.scales))
+            vs = np.repeat(self.scales[1][pages], self.page, 0)[:total]
             j = np.arange(total)
             for t in range(m):
                 row, p = starts[i] + t, total - m + t
@@ -129,11 +135,14 @@ class Model:
                     out[row, h] = w @ v[see, g]
                     lse[row, h] = top + math.log(e.sum())
                     A[row, h] = w @ np.abs(v[see, g])
+                    floor[row, h] = 2.0 ** -35 * (w * vs[see, g]).max() * (
+                        np.abs(v[see, g]) / vs[see, g][:, None]).sum(0)
                     ds[row, h] = abs(scale) * (np.abs(k[see, g]) @ np.abs(q[row, h])).max()
         ds *= (d / 16 + 16) * 2.0 ** -23
         acc = (n[:, None] / 16 + 16) * 2.0 ** -23
         rel = 2 * ds + 2.0 ** -21 + acc
-        return out, lse, A, rel, ds + acc + 2.0 ** -21
+        # what the output may be off by, but for its rounding and p's as f16
+        return out, lse, A, A * rel[..., None] + floor, ds + acc + 2.0 ** -21
 
 
 def f64(t):
@@ -283,6 +292,10 @@ def test_append_padding_and_bounds(dev):
 
 
 # --------------------------------------------------------------- attention
+def limit(y, A, lim, bf16):
+    return lim + (A * 2.0 ** -11 + 2.0 ** -8 * np.abs(y) if bf16 else 2.0 ** -24 * np.abs(y)) + 1e-37
+
+
 def attend(m, counts, lengths, table, heads, bf16, window=0, scale=None, q=None, bad=(), extra=0,
            pad=0, **kw):
     import torch
@@ -293,13 +306,10 @@ def attend(m, counts, lengths, table, heads, bf16, window=0, scale=None, q=None,
     lse = torch.full(q.shape[:2], 7.0, device=m.dev)
     T.kv8_attention(m.cache, q, i32(st, m.dev), i32(lengths, m.dev), i32(table, m.dev),
                     window=window, scale=scale, out=out, lse=lse, **kw)
-    y, z, A, rel, tol = m.attention(f64(q), st, lengths, table, window, scale, bad)
+    y, z, A, lim, tol = m.attention(f64(q), st, lengths, table, window, scale, bad)
     n = int(st[-1])
-    half = 2.0 ** -8 if bf16 else 2.0 ** -24
-    if bf16:
-        rel = rel + 2.0 ** -11
     o, ls = f64(out)[:n], f64(lse)[:n]
-    lim = A[:n] * rel[:n, :, None] + half * np.abs(y[:n]) + 1e-37
+    lim = limit(y, A, lim, bf16)[:n]
     off = np.abs(o - y[:n])
     assert (off <= lim).all(), ("out", (off / lim).max(), np.argwhere(off > lim)[:5])
     np.testing.assert_array_equal(np.isneginf(ls), np.isneginf(z[:n]))
@@ -456,8 +466,8 @@ def test_large_page_numbers(dev):
         np.testing.assert_array_equal(f64(got[used]), want)
     q = rows_of(m.rng, 1, 8, d, True, dev)
     out = T.kv8_attention(m.cache, q, i32([0, 1], dev), i32(lengths, dev), i32([used], dev))
-    y, _, A, rel, _ = m.attention(f64(q), [0, 1], lengths, [[0, 1, 2]])
-    assert (np.abs(f64(out) - y) <= A * (rel + 2.0 ** -11)[..., None] + 2.0 ** -8 * np.abs(y)).all()
+    y, _, A, lim, _ = m.attention(f64(q), [0, 1], lengths, [[0, 1, 2]])
+    assert (np.abs(f64(out) - y) <= limit(y, A, lim, True)).all()
 
 
 # ---------------------------------------------------------------- together
@@ -496,9 +506,8 @@ def test_decode_steps_from_a_graph(dev):
         graph.replay()
         lengths = lengths + 1
         m.append([f64(kr), f64(v)], range(seqs + 1), lengths, table)
-        y, _, A, rel, _ = m.attention(f64(qr), range(seqs + 1), lengths, table)
-        assert (np.abs(f64(out) - y) <= A * (rel + 2.0 ** -11)[..., None]
-                + 2.0 ** -8 * np.abs(y)).all()
+        y, _, A, lim, _ = m.attention(f64(qr), range(seqs + 1), lengths, table)
+        assert (np.abs(f64(out) - y) <= limit(y, A, lim, True)).all()
     m.same()
     assert T.check_status() == (0, 0)
 
