@@ -2,23 +2,21 @@
 //
 //   s_j = scale q.k_j,  out = sum_j p_j v_j,  p = softmax(s),  k_j = code * page scale
 //
-// A block holds 16 rows of one sequence and k/v head: (query token, head of the
-// group) pairs, token-major.  With a group of 8 heads and one token half of
-// them are empty, which costs nothing while the cache's bytes bound the time.
-// Its keys are split into chunks over CTAs when there are few blocks; a second
-// kernel joins the chunks.
+// A block holds 8 or 16 rows of one sequence and k/v head: (query token, head
+// of the group) pairs, token-major.  Its keys are split into chunks over CTAs
+// when there are few blocks; a second kernel joins the chunks.
 //
 // Within a CTA each of 4 warps takes every fourth step of 16 keys, which lie in
 // one page, through a ring of cp.async stages of its own: no barrier in the
 // loop.  The codes go from shared memory to registers with 16-byte loads and
-// are converted there, each lane having exactly the operands of its m16n8k16
-// instructions:
-//   S = Q K^T: lane (g, t) (g = lane / 4, t = lane % 4) holds key order(g), 16
-//     consecutive elements of it; a word's even and odd bytes are the two
-//     operand registers of one 16-wide step, so the head dimension is summed
-//     in the order that Q's registers are laid out in too;
-//   O = P V: S's registers are P's operands; lane (g, t) holds the elements
-//     16 g .. 16 g + 15 (of 128) of keys order(2t), order(2t + 1).
+// are converted there, as the left operands of m16n8k16 instructions, so that 8
+// rows fill the other side:
+//   S^T = K Q^T: lane (g, t) (g = lane / 4, t = lane % 4) holds keys order(g)
+//     and order(g) + 8, 16 consecutive elements of each; the head dimension is
+//     summed in the order in which that puts it, Q's registers the same;
+//   O^T = V^T P^T: S^T's registers, transposed 8 x 8, are P^T's operands; lane
+//     (g, t) holds elements 16 g .. 16 g + 15 (of 128) of keys order(2t),
+//     order(2t + 1) and those + 8.
 // order() and the two swizzles below put the 8 lanes of each 16-byte access
 // into different banks.
 //
@@ -55,13 +53,13 @@ struct Args {
     const uint8_t *k, *v;
     const float *k_scale, *v_scale;
     unsigned* status;
-    float* part;    // [seq, kv head, block, chunk][16][d] partial outputs
-    float2* state;  // the same [16]: (reference, sum)
+    float* part;    // [seq, kv head, block, chunk][block_rows][d] partial outputs
+    float2* state;  // the same, a row's (reference, sum)
     float scale;
-    int hq, hkv, d, window, max_rows, max_len, chunks, blocks, vec;
+    int hq, hkv, d, window, max_rows, max_len, chunks, blocks, block_rows, vec;
 };
 
-// What a block of 16 rows attends, the same in both kernels.
+// What a block of rows attends, the same in both kernels.
 struct Block {
     kv8::Seq s;
     int rows;       // live rows of the block
@@ -74,8 +72,8 @@ __device__ __forceinline__ Block block_of(const Args& a, int seq, int block, boo
     Block k;
     k.s = kv8::sequence(a.b, seq);
     const int group = a.hq / a.hkv;
-    const int64_t all = (int64_t)k.s.n * group, at = (int64_t)block * 16;
-    k.rows = (int)max((int64_t)0, min((int64_t)16, all - at));
+    const int64_t all = (int64_t)k.s.n * group, at = (int64_t)block * a.block_rows;
+    k.rows = (int)max((int64_t)0, min((int64_t)a.block_rows, all - at));
     k.lo = k.end = 0;
     if (k.rows > 0) {
         if (k.s.len > a.max_len || k.s.n > a.max_rows ||
@@ -96,9 +94,9 @@ __device__ __forceinline__ Block block_of(const Args& a, int seq, int block, boo
     return k;
 }
 
-// The key of a step that column (or lane group) n of 8 stands for.
+// The key (of 8) that row g of an operand stands for.
 __device__ __forceinline__ int order(int n) { return n & 1 ? (n >> 1) ^ 5 : n >> 1; }
-// Where a row's 16-byte piece c lies.
+// Where a key's 16-byte piece c lies.
 __device__ __forceinline__ int k_place(int key, int c, int pieces) {
     return pieces > 4 ? c ^ ((key & 1) << 2) : c;
 }
@@ -106,36 +104,33 @@ __device__ __forceinline__ int v_place(int key, int c, int pieces) {
     return pieces > 4 ? c ^ ((key & 3) << 1) : c ^ (key & 2);
 }
 
-template <int DP>
-constexpr int stages() {
-    return DP == 64 ? 6 : DP == 128 ? 4 : 3;
-}
-template <int DP>
-constexpr int stage_bytes() {
-    return 2 * kStep * DP;
-}
-// Q's operands stay in registers when they are few.
-template <typename T, int DP>
-constexpr bool q_in_registers() {
-    return DP / 16 * 4 * (sizeof(T) == 4 ? 2 : 1) <= 32;
-}
-template <typename T, int DP>
-constexpr int smem_bytes() {
-    const int ring = kWarps * stages<DP>() * (stage_bytes<DP>() + 16);
-    const int q = q_in_registers<T, DP>() ? 0 : DP / 16 * 512 * (sizeof(T) == 4 ? 2 : 1);
-    const int join = kWarps * 16 * (DP + 4) * 4 + kWarps * 16 * 12;
-    return (ring > join ? ring : join) + q;
-}
+// Shapes of a kernel for heads of up to DP elements and blocks of 8 NB rows.
+template <typename T, int DP, int NB>
+struct Shape {
+    static constexpr bool kSplit = sizeof(T) == 4;  // hi + lo operands
+    static constexpr int kStages = DP == 64 ? 5 : 3;
+    static constexpr int kStageBytes = 2 * kStep * DP;
+    static constexpr int kStagePitch = kStageBytes + 16;  // and the page's two scales
+    static constexpr int kSteps = DP / 16;                // 16-wide steps of the head dimension
+    static constexpr int kRows = 8 * NB;
+    // Q's operands stay in registers when they are few
+    static constexpr bool kQReg = kSteps * 2 * NB * (kSplit ? 2 : 1) <= 32;
+    static constexpr int kQBytes = kQReg ? 0 : kSteps * NB * 256 * (kSplit ? 2 : 1);
+    static constexpr int kRing = kWarps * kStages * kStagePitch;
+    static constexpr int kPitch = DP + 4;
+    static constexpr int kJoin = kWarps * kRows * (kPitch + 3) * 4;
+    static constexpr int kBytes = (kRing > kJoin ? kRing : kJoin) + kQBytes;
+    // CTAs per SM: what registers (O: DP NB / 4 a lane) and shared memory allow
+    static constexpr int kCtas = DP * NB >= 512 ? 2 : DP * NB >= 256 ? (DP == 256 ? 2 : 3) : 4;
+};
 
-template <typename T, int FORMAT, int DP>
-__global__ void __launch_bounds__(kThreads, DP == 256 ? 2 : 3)
+template <typename T, int FORMAT, int DP, int NB>
+__global__ void __launch_bounds__(kThreads, Shape<T, DP, NB>::kCtas)
 k_attend(const __grid_constant__ Args a) {
-    constexpr bool kSplit = sizeof(T) == 4;   // hi + lo operands
-    constexpr bool kQReg = q_in_registers<T, DP>();
-    constexpr int kSteps = DP / 16;           // 16-wide steps of the head dimension
-    constexpr int kStages = stages<DP>();
-    constexpr int kPieces = DP / 16;          // 16-byte pieces of a key
-    constexpr int kOut = DP / 8;              // 8-wide output tiles
+    using H = Shape<T, DP, NB>;
+    constexpr bool kSplit = H::kSplit, kQReg = H::kQReg;
+    constexpr int kSteps = H::kSteps, kStages = H::kStages, kPieces = DP / 16, kRows = H::kRows;
+    constexpr int kTiles = DP / 16;  // 16-wide output tiles
     extern __shared__ __align__(16) uint8_t smem[];
 
     const int c = blockIdx.x % a.chunks, block = blockIdx.x / a.chunks;
@@ -145,95 +140,98 @@ k_attend(const __grid_constant__ Args a) {
     if (blk.rows == 0 || c >= blk.used) return;
     const int group = a.hq / a.hkv;
     const int begin = blk.from + c * blk.size, end = min(begin + blk.size, blk.end);
+    const int pieces = a.d / 16;
 
-    // the two rows of this lane: keys [see_lo, see_hi] each
-    int see_lo[2], see_hi[2];
-    float qf[2];  // what a row's scores are multiplied with, but for the page's scale
-    uint32_t qr[kQReg ? kSteps : 1][4], ql[kQReg && kSplit ? kSteps : 1][4];
-    uint4* qs = reinterpret_cast<uint4*>(
-        smem + (smem_bytes<T, DP>() - (kQReg ? 0 : kSteps * 512 * (kSplit ? 2 : 1))));
-    {
-        const T* qp[2];
-        float top[2] = {0.0f, 0.0f};
+    // Q's operands: rows g, g + 8, .. of the block; a row's scores are
+    // multiplied with qf, but for the page's scale
+    uint32_t qr[kQReg ? kSteps : 1][NB][2], ql[kQReg && kSplit ? kSteps : 1][NB][2];
+    uint2* qs = reinterpret_cast<uint2*>(smem + H::kBytes - H::kQBytes);
+    float qf[NB];
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {
-            const int i = g + 8 * r;
-            const bool live = i < blk.rows;
-            const int64_t at = (int64_t)block * 16 + i;
-            const int tok = live ? (int)(at / group) : 0, hh = live ? (int)(at % group) : 0;
-            // rows of the block that are not there see all and are not stored
-            const int p = live ? blk.s.first + tok : INT32_MAX;
-            see_hi[r] = p;
-            see_lo[r] = a.window && live ? max(p - a.window + 1, 0) : 0;
-            qp[r] = live ? static_cast<const T*>(a.q) + (blk.s.lo + tok) * a.q_stride +
-                               (int64_t)(head * group + hh) * a.d
-                         : nullptr;
-            if (live) {
-#pragma unroll
-                for (int h = 0; h < DP / 64; ++h) {
-                    float x[16];
-                    kv8::load16(qp[r] + 64 * h + 16 * t, 64 * h + 16 * t < a.d, a.vec, x);
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) top[r] = fmaxf(top[r], fabsf(x[e]));
-                }
-            }
-            top[r] = fmaxf(top[r], __shfl_xor_sync(tbk::kFull, top[r], 1));
-            top[r] = fmaxf(top[r], __shfl_xor_sync(tbk::kFull, top[r], 2));
-        }
-        float lift[2];
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-            // 2^e with |q| 2^e in [2^14, 2^15); NaN and infinite rows stay that
-            const int e = min(max((int)(__float_as_uint(top[r]) >> 23), 1 + 16), 254);
-            lift[r] = __uint_as_float((uint32_t)(127 + 14 - e + 127) << 23);
-            qf[r] = __uint_as_float((uint32_t)(e - 14) << 23) * (a.scale * kLog2e) *
-                    kv8::kOperandUnit<FORMAT>;
-        }
+    for (int b = 0; b < NB; ++b) {
+        const int i = 8 * b + g;
+        const bool live = i < blk.rows;
+        const int64_t at = (int64_t)block * kRows + i;
+        const int tok = live ? (int)(at / group) : 0, hh = live ? (int)(at % group) : 0;
+        const T* q = static_cast<const T*>(a.q) + (blk.s.lo + tok) * a.q_stride +
+                     (int64_t)(head * group + hh) * a.d;
+        float top = 0.0f;
 #pragma unroll
         for (int h = 0; h < DP / 64; ++h) {
-            float x[2][16];
+            float x[16];
+            kv8::load16(q + 64 * h + 16 * t, live && 64 * h + 16 * t < a.d, a.vec, x);
 #pragma unroll
-            for (int r = 0; r < 2; ++r) {
-                kv8::load16(qp[r] + 64 * h + 16 * t, qp[r] && 64 * h + 16 * t < a.d, a.vec, x[r]);
+            for (int e = 0; e < 16; ++e) top = fmaxf(top, fabsf(x[e]));
+        }
+        top = fmaxf(top, __shfl_xor_sync(tbk::kFull, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(tbk::kFull, top, 2));
+        // 2^e with |q| 2^e in [2^14, 2^15); NaN and infinite rows stay that
+        const int e = min(max((int)(__float_as_uint(top) >> 23), 1 + 16), 254);
+        const float lift = __uint_as_float((uint32_t)(127 + 14 - e + 127) << 23);
+        qf[b] = __uint_as_float((uint32_t)(e - 14) << 23) * (a.scale * kLog2e);
 #pragma unroll
-                for (int e = 0; e < 16; ++e) x[r][e] *= lift[r];
-            }
+        for (int h = 0; h < DP / 64; ++h) {
+            float x[16];
+            kv8::load16(q + 64 * h + 16 * t, live && 64 * h + 16 * t < a.d, a.vec, x);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {  // a word of 4 codes: even ones, odd ones
-                uint32_t hi[4], lo[4];
+            for (int e16 = 0; e16 < 16; ++e16) x[e16] *= lift;
 #pragma unroll
-                for (int e = 0; e < 2; ++e)
+            for (int j = 0; j < 4; ++j) {  // a word of 4 codes
+                uint32_t hi[2], lo[2];
 #pragma unroll
-                    for (int r = 0; r < 2; ++r) {
-                        const float u = x[r][4 * j + e], w = x[r][4 * j + e + 2];
-                        hi[2 * e + r] = kv8::pack_f16x2(u, w);
-                        const __half2 h2 = *reinterpret_cast<const __half2*>(&hi[2 * e + r]);
-                        lo[2 * e + r] =
-                            kv8::pack_f16x2(u - __low2float(h2), w - __high2float(h2));
-                    }
+                for (int r = 0; r < 2; ++r) {
+                    const float u = x[4 * j + kv8::word_element<FORMAT>(r, 0)];
+                    const float w = x[4 * j + kv8::word_element<FORMAT>(r, 1)];
+                    hi[r] = kv8::pack_f16x2(u, w);
+                    const __half2 h2 = *reinterpret_cast<const __half2*>(&hi[r]);
+                    lo[r] = kv8::pack_f16x2(u - __low2float(h2), w - __high2float(h2));
+                }
                 const int s = 4 * h + j;
                 if constexpr (kQReg) {
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        qr[s][e] = hi[e];
-                        if (kSplit) ql[s][e] = lo[e];
+                    for (int r = 0; r < 2; ++r) {
+                        qr[s][b][r] = hi[r];
+                        if (kSplit) ql[s][b][r] = lo[r];
                     }
                 } else if (warp == 0) {
-                    qs[s * 32 + lane] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-                    if (kSplit) qs[(kSteps + s) * 32 + lane] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+                    qs[(s * NB + b) * 32 + lane] = make_uint2(hi[0], hi[1]);
+                    if (kSplit) qs[((kSteps + s) * NB + b) * 32 + lane] = make_uint2(lo[0], lo[1]);
                 }
             }
         }
     }
-    if constexpr (!kQReg) __syncthreads();
+    // S^T's columns: rows 8 b + 2 t + e, keys [see_lo, see_hi] each
+    float qc[NB][2];
+    int see_lo[NB][2], see_hi[NB][2];
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            qc[b][e] = __shfl_sync(tbk::kFull, qf[b], (2 * t + e) * 4);
+            const int i = 8 * b + 2 * t + e;
+            // rows of the block that are not there see all and are not stored
+            const bool live = i < blk.rows;
+            const int p = blk.s.first + (int)(((int64_t)block * kRows + i) / group);
+            see_hi[b][e] = live ? p : INT32_MAX;
+            see_lo[b][e] = a.window && live ? max(p - a.window + 1, 0) : 0;
+        }
 
     // the warp's steps: keys first + 64 n .. + 15
     const int first = begin + warp * kStep;
     const int n_steps = end > first ? (end - first + kWarps * kStep - 1) / (kWarps * kStep) : 0;
-    uint8_t* ring = smem + warp * kStages * (stage_bytes<DP>() + 16);
+    uint8_t* ring = smem + warp * kStages * H::kStagePitch;
     const uint32_t ring_s = tbk::smem_addr(ring);
+    if (pieces < kPieces) {
+        // elements past the head dimension are codes of zero, never written again
+        for (int i = lane; i < kStages * kStep * (kPieces - pieces); i += 32) {
+            const int piece = pieces + i % (kPieces - pieces), key = i / (kPieces - pieces);
+            *reinterpret_cast<uint4*>(ring + (key / kStep) * H::kStagePitch + (key % kStep) * DP +
+                                      k_place(key % kStep, piece, kPieces) * 16) =
+                make_uint4(0, 0, 0, 0);
+        }
+    }
+    __syncthreads();
     const int32_t* table = a.b.table + seq * a.b.table_stride;
-    const int pieces = a.d / 16;
     auto page_of = [&](int n) {  // the page of step n, -1 if it has none
         if (n >= n_steps) return -1;
         const int id = table[(first + n * (kWarps * kStep)) >> a.b.page_shift];
@@ -242,6 +240,8 @@ k_attend(const __grid_constant__ Args a) {
         return -1;
     };
     int ids = page_of(lane), ids_next = page_of(32 + lane);  // of steps [0, 32), [32, 64)
+    constexpr int kKeys = 32 / kPieces;                       // keys per warp access
+    const int my_piece = lane % kPieces, my_key = lane / kPieces;
     auto issue = [&](int n) {
         const int id = __shfl_sync(tbk::kFull, ids, n & 31);
         if ((n & 31) == 31) {
@@ -251,151 +251,183 @@ k_attend(const __grid_constant__ Args a) {
         if (id >= 0) {
             const int64_t unit = (int64_t)id * a.hkv + head;
             const int slot = (first + n * (kWarps * kStep)) & ((1 << a.b.page_shift) - 1);
-            const int64_t at = ((unit << a.b.page_shift) + slot) * a.d;
-            const uint32_t dst = ring_s + (n % kStages) * (stage_bytes<DP>() + 16);
-            constexpr int kRows = 32 / kPieces > 0 ? 32 / kPieces : 1;  // keys per warp access
-            const int piece = lane % kPieces;
-            if (piece < pieces) {
+            const int64_t at =
+                ((unit << a.b.page_shift) + slot + my_key) * a.d + my_piece * 16;
+            const uint8_t *k = a.k + at, *v = a.v + at;
+            const uint32_t dst = ring_s + (n % kStages) * H::kStagePitch;
+            if (my_piece < pieces) {
 #pragma unroll
-                for (int i = 0; i < kStep / kRows; ++i) {
-                    const int key = lane / kPieces + i * kRows;
-                    const int64_t from = at + key * a.d + piece * 16;
-                    const uint32_t row = dst + key * DP;
-                    kv8::cp_async16(row + k_place(key, piece, kPieces) * 16, a.k + from);
-                    kv8::cp_async16(row + kStep * DP + v_place(key, piece, kPieces) * 16,
-                                    a.v + from);
+                for (int i = 0; i < kStep / kKeys; ++i) {
+                    const int key = my_key + i * kKeys;
+                    kv8::cp_async16(dst + key * DP + k_place(key, my_piece, kPieces) * 16,
+                                    k + i * kKeys * a.d);
+                    kv8::cp_async16(
+                        dst + (kStep + key) * DP + v_place(key, my_piece, kPieces) * 16,
+                        v + i * kKeys * a.d);
                 }
             }
             if (lane < 2)
-                kv8::cp_async4(dst + stage_bytes<DP>() + 4 * lane,
+                kv8::cp_async4(dst + H::kStageBytes + 4 * lane,
                                (lane ? a.v_scale : a.k_scale) + unit);
         }
-        const bool there = id >= 0;
         kv8::cp_async_commit();
-        return there;
+        return id >= 0;
     };
     uint32_t there = 0;  // bit i: the step i behind the newest issued one has a page
 #pragma unroll
     for (int n = 0; n < kStages - 1; ++n) there = there << 1 | (uint32_t)issue(n);
 
-    float o[kOut][4];
+    float o[kTiles][NB][4];
 #pragma unroll
-    for (int i = 0; i < kOut; ++i)
+    for (int i = 0; i < kTiles; ++i)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) o[i][e] = 0.0f;
-    float ref[2] = {-INFINITY, -INFINITY}, vref[2] = {-INFINITY, -INFINITY}, sum[2] = {0.0f, 0.0f};
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[i][b][e] = 0.0f;
+    float ref[NB][2], vref[NB][2], sum[NB][2];
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            ref[b][e] = vref[b][e] = -INFINITY;
+            sum[b][e] = 0.0f;
+        }
 
+    const int ka = order(2 * t), kb = order(2 * t + 1), kg = order(g);
     for (int n = 0; n < n_steps; ++n) {
         kv8::cp_async_wait<kStages - 2>();
         __syncwarp();
         there = there << 1 | (uint32_t)issue(n + kStages - 1);
         if (!(there >> (kStages - 1) & 1)) continue;
-        const uint8_t* stage = ring + (n % kStages) * (stage_bytes<DP>() + 16);
-        const float2 scales = *reinterpret_cast<const float2*>(stage + stage_bytes<DP>());
+        uint8_t* stage = ring + (n % kStages) * H::kStagePitch;
+        const float2 scales = *reinterpret_cast<const float2*>(stage + H::kStageBytes);
         const int key0 = first + n * (kWarps * kStep);
+        if (key0 + kStep > blk.s.len) {
+            // slots behind the last token may hold anything, NaN codes too: a
+            // weight of zero needs a finite value beside it
+            for (int i = (blk.s.len - key0) * DP / 16 + lane; i < kStep * DP / 16; i += 32)
+                *reinterpret_cast<uint4*>(stage + kStep * DP + 16 * i) = make_uint4(0, 0, 0, 0);
+            __syncwarp();
+        }
 
-        // S: two tiles of 8 keys
-        float s[2][4];
+        // S^T: 16 keys by the block's rows, two sums of half the steps each
+        float s2[2][NB][4];
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
+        for (int i = 0; i < 2; ++i)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) s[i][e] = 0.0f;
-            const int key = 8 * i + order(g);
+            for (int b = 0; b < NB; ++b)
 #pragma unroll
-            for (int h = 0; h < DP / 64; ++h) {
-                const uint4 w4 = *reinterpret_cast<const uint4*>(
-                    stage + key * DP + k_place(key, 4 * h + t, kPieces) * 16);
-                const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
+                for (int e = 0; e < 4; ++e) s2[i][b][e] = 0.0f;
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    uint32_t b0, b1;
-                    kv8::to_f16<FORMAT>(w[j], b0, b1);
-                    const int k = 4 * h + j;
+        for (int h = 0; h < DP / 64; ++h) {
+            const uint4 x = *reinterpret_cast<const uint4*>(
+                stage + kg * DP + k_place(kg, 4 * h + t, kPieces) * 16);
+            const uint4 y = *reinterpret_cast<const uint4*>(
+                stage + (kg + 8) * DP + k_place(kg + 8, 4 * h + t, kPieces) * 16);
+            const uint32_t wx[4] = {x.x, x.y, x.z, x.w}, wy[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                uint32_t a0, a1, a2, a3;
+                kv8::word<FORMAT>(wx[j], a0, a2);
+                kv8::word<FORMAT>(wy[j], a1, a3);
+                const int k = 4 * h + j;
+#pragma unroll
+                for (int b = 0; b < NB; ++b) {
                     if constexpr (kQReg) {
-                        kv8::mma16816(s[i], qr[k][0], qr[k][1], qr[k][2], qr[k][3], b0, b1);
+                        kv8::mma16816(s2[j & 1][b], a0, a1, a2, a3, qr[k][b][0], qr[k][b][1]);
                         if constexpr (kSplit)
-                            kv8::mma16816(s[i], ql[k][0], ql[k][1], ql[k][2], ql[k][3], b0, b1);
+                            kv8::mma16816(s2[j & 1][b], a0, a1, a2, a3, ql[k][b][0], ql[k][b][1]);
                     } else {
-                        const uint4 x = qs[k * 32 + lane];
-                        kv8::mma16816(s[i], x.x, x.y, x.z, x.w, b0, b1);
+                        const uint2 q = qs[(k * NB + b) * 32 + lane];
+                        kv8::mma16816(s2[j & 1][b], a0, a1, a2, a3, q.x, q.y);
                         if constexpr (kSplit) {
-                            const uint4 y = qs[(kSteps + k) * 32 + lane];
-                            kv8::mma16816(s[i], y.x, y.y, y.z, y.w, b0, b1);
+                            const uint2 r = qs[((kSteps + k) * NB + b) * 32 + lane];
+                            kv8::mma16816(s2[j & 1][b], a0, a1, a2, a3, r.x, r.y);
                         }
                     }
                 }
             }
         }
-        // log2 units; the values' scale as an exponent
+        // log2 units: s[b][2 i + e] is key key0 + kg + 8 i, row 8 b + 2 t + e; the
+        // values' scale as an exponent
         const float lv = (float)((int)(__float_as_uint(scales.y) >> 23) - 127);
-        bool over = false;
+        float s[NB][4];
+        bool inside = true, over = false;
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {
-            const float f = qf[r] * scales.x;
+        for (int b = 0; b < NB; ++b)
 #pragma unroll
-            for (int i = 0; i < 2; ++i)
-#pragma unroll
-                for (int e = 0; e < 2; ++e) s[i][2 * r + e] *= f;
-        }
-        const bool inside = key0 >= see_lo[0] && key0 >= see_lo[1] &&
-                            key0 + kStep - 1 <= see_hi[0] && key0 + kStep - 1 <= see_hi[1];
+            for (int e = 0; e < 2; ++e) {
+                const float f = qc[b][e] * scales.x;
+                s[b][e] = (s2[0][b][e] + s2[1][b][e]) * f;
+                s[b][2 + e] = (s2[0][b][2 + e] + s2[1][b][2 + e]) * f;
+                inside &= key0 >= see_lo[b][e] && key0 + kStep - 1 <= see_hi[b][e];
+            }
         if (!__all_sync(tbk::kFull, inside)) {
 #pragma unroll
-            for (int i = 0; i < 2; ++i)
+            for (int b = 0; b < NB; ++b)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int j = key0 + 8 * i + order(2 * t + (e & 1));
-                    if (j < see_lo[e >> 1] || j > see_hi[e >> 1]) s[i][e] = -INFINITY;
+                for (int i = 0; i < 4; ++i) {
+                    const int j = key0 + kg + 8 * (i >> 1);
+                    if (j < see_lo[b][i & 1] || j > see_hi[b][i & 1]) s[b][i] = -INFINITY;
                 }
         }
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {
-            const float hi = fmaxf(fmaxf(s[0][2 * r], s[0][2 * r + 1]),
-                                   fmaxf(s[1][2 * r], s[1][2 * r + 1]));
-            over |= hi > ref[r] + kSlack || hi + lv > vref[r] + kSlack;
-        }
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const float hi = fmaxf(s[b][e], s[b][2 + e]);
+                over |= hi > ref[b][e] + kSlack || hi + lv > vref[b][e] + kSlack;
+            }
         if (__any_sync(tbk::kFull, over)) {
 #pragma unroll
-            for (int r = 0; r < 2; ++r) {
-                float hi = fmaxf(fmaxf(s[0][2 * r], s[0][2 * r + 1]),
-                                 fmaxf(s[1][2 * r], s[1][2 * r + 1]));
-                hi = fmaxf(hi, __shfl_xor_sync(tbk::kFull, hi, 1));
-                hi = fmaxf(hi, __shfl_xor_sync(tbk::kFull, hi, 2));
-                const float m = fmaxf(ref[r], ceilf(hi)), mv = fmaxf(vref[r], ceilf(hi) + lv);
-                if (m > ref[r]) sum[r] *= kv8::exp2_fast(ref[r] - m);
-                if (mv > vref[r]) {
-                    const float keep = kv8::exp2_fast(vref[r] - mv);
+            for (int b = 0; b < NB; ++b)
 #pragma unroll
-                    for (int i = 0; i < kOut; ++i) {
-                        o[i][2 * r] *= keep;
-                        o[i][2 * r + 1] *= keep;
+                for (int e = 0; e < 2; ++e) {
+                    float hi = fmaxf(s[b][e], s[b][2 + e]);
+#pragma unroll
+                    for (int x = 4; x < 32; x <<= 1)
+                        hi = fmaxf(hi, __shfl_xor_sync(tbk::kFull, hi, x));
+                    const float m = fmaxf(ref[b][e], ceilf(hi));
+                    const float mv = fmaxf(vref[b][e], ceilf(hi) + lv);
+                    if (m > ref[b][e]) sum[b][e] *= kv8::exp2_fast(ref[b][e] - m);
+                    if (mv > vref[b][e]) {
+                        const float keep = kv8::exp2_fast(vref[b][e] - mv);
+#pragma unroll
+                        for (int i = 0; i < kTiles; ++i) {
+                            o[i][b][e] *= keep;
+                            o[i][b][2 + e] *= keep;
+                        }
                     }
+                    ref[b][e] = m;
+                    vref[b][e] = mv;
                 }
-                ref[r] = m;
-                vref[r] = mv;
-            }
         }
-        // weights: for the sum, and times the values' scale as P's operands
-        uint32_t ph[4], pl[4];
+        // weights: for the sum, and times the values' scale as P^T's operands
+        uint32_t ph[NB][2], pl[NB][2];
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {
-            const float m = ref[r] == -INFINITY ? 0.0f : ref[r];
-            const float mv = (vref[r] == -INFINITY ? 0.0f : vref[r]) - lv - kLift;
+        for (int b = 0; b < NB; ++b) {
+            float p[4];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const float m = ref[b][e] == -INFINITY ? 0.0f : ref[b][e];
+                const float mv = (vref[b][e] == -INFINITY ? 0.0f : vref[b][e]) - lv - kLift;
+                sum[b][e] += kv8::exp2_fast(s[b][e] - m) + kv8::exp2_fast(s[b][2 + e] - m);
+                p[e] = kv8::exp2_fast(s[b][e] - mv);
+                p[2 + e] = kv8::exp2_fast(s[b][2 + e] - mv);
+            }
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                const float s0 = s[i][2 * r], s1 = s[i][2 * r + 1];
-                sum[r] += kv8::exp2_fast(s0 - m) + kv8::exp2_fast(s1 - m);
-                const float p0 = kv8::exp2_fast(s0 - mv), p1 = kv8::exp2_fast(s1 - mv);
-                ph[2 * i + r] = kv8::pack_f16x2(p0, p1);
+                const uint32_t hi = kv8::pack_f16x2(p[2 * i], p[2 * i + 1]);
+                ph[b][i] = kv8::transpose8(hi);
                 if constexpr (kSplit) {
-                    const __half2 h2 = *reinterpret_cast<const __half2*>(&ph[2 * i + r]);
-                    pl[2 * i + r] = kv8::pack_f16x2(p0 - __low2float(h2), p1 - __high2float(h2));
+                    const __half2 h2 = *reinterpret_cast<const __half2*>(&hi);
+                    pl[b][i] = kv8::transpose8(kv8::pack_f16x2(p[2 * i] - __low2float(h2),
+                                                               p[2 * i + 1] - __high2float(h2)));
                 }
             }
         }
-        // O += P V
+        // O^T += V^T P^T: tile rows g and g + 8 are two neighbouring elements
         const uint8_t* vs = stage + kStep * DP;
-        const int ka = order(2 * t), kb = order(2 * t + 1);
         constexpr int kWide = DP >= 128 ? 16 : 8;  // bytes a lane takes of a key at once
 #pragma unroll
         for (int h = 0; h < (DP + 127) / 128; ++h) {
@@ -419,48 +451,50 @@ k_attend(const __grid_constant__ Args a) {
                 }
             }
 #pragma unroll
-            for (int j = 0; j < kWide / 4; ++j)
+            for (int j = 0; j < kWide / 4; ++j) {
+                uint32_t lo[4], hi[4];
+                kv8::words<FORMAT>(w[0][j], w[1][j], lo);
+                kv8::words<FORMAT>(w[2][j], w[3][j], hi);
 #pragma unroll
-                for (int half = 0; half < 2; ++half) {
-                    const uint32_t sel = half ? 0x7632 : 0x5410;
-                    uint32_t b0e, b0o, b1e, b1o;
-                    kv8::to_f16<FORMAT>(kv8::prmt(w[0][j], w[1][j], sel), b0e, b0o);
-                    kv8::to_f16<FORMAT>(kv8::prmt(w[2][j], w[3][j], sel), b1e, b1o);
-                    const int tile = h * 16 + 4 * j + 2 * half;
-                    kv8::mma16816(o[tile], ph[0], ph[1], ph[2], ph[3], b0e, b1e);
-                    kv8::mma16816(o[tile + 1], ph[0], ph[1], ph[2], ph[3], b0o, b1o);
-                    if constexpr (kSplit) {
-                        kv8::mma16816(o[tile], pl[0], pl[1], pl[2], pl[3], b0e, b1e);
-                        kv8::mma16816(o[tile + 1], pl[0], pl[1], pl[2], pl[3], b0o, b1o);
+                for (int i = 0; i < 2; ++i)
+#pragma unroll
+                    for (int b = 0; b < NB; ++b) {
+                        float(&d)[4] = o[h * 8 + 2 * j + i][b];
+                        kv8::mma16816(d, lo[2 * i], lo[2 * i + 1], hi[2 * i], hi[2 * i + 1],
+                                      ph[b][0], ph[b][1]);
+                        if constexpr (kSplit)
+                            kv8::mma16816(d, lo[2 * i], lo[2 * i + 1], hi[2 * i], hi[2 * i + 1],
+                                          pl[b][0], pl[b][1]);
                     }
-                }
+            }
         }
     }
     kv8::cp_async_wait<0>();
     __syncthreads();  // the rings are free: the warps' states meet in their place
 
-    // lane (g, t) has columns 2t, 2t + 1 of each tile: element (2t + e) * kWide + tile
-    constexpr int kPitch = DP + 4;
-    float* jo = reinterpret_cast<float*>(smem);
-    float* jm = jo + kWarps * 16 * kPitch;
+    // o[h 8 + u][b][2 r + e]: element 128 h + kWide g + 2 u + r of row 8 b + 2 t + e
     constexpr int kWide = DP >= 128 ? 16 : 8;
+    float* jo = reinterpret_cast<float*>(smem);
+    float* jm = jo + kWarps * kRows * H::kPitch;
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
-        sum[r] += __shfl_xor_sync(tbk::kFull, sum[r], 1);
-        sum[r] += __shfl_xor_sync(tbk::kFull, sum[r], 2);
-        float* row = jo + (warp * 16 + g + 8 * r) * kPitch;
+    for (int b = 0; b < NB; ++b)
 #pragma unroll
-        for (int i = 0; i < kOut; ++i)
+        for (int e = 0; e < 2; ++e) {
+            float z = sum[b][e];
 #pragma unroll
-            for (int e = 0; e < 2; ++e)
-                row[(i / kWide) * 128 + (2 * t + e) * kWide + i % kWide] = o[i][2 * r + e];
-        if (t == 0) {
-            float* st = jm + (warp * 16 + g + 8 * r) * 3;
-            st[0] = ref[r];
-            st[1] = vref[r];
-            st[2] = sum[r];
+            for (int x = 4; x < 32; x <<= 1) z += __shfl_xor_sync(tbk::kFull, z, x);
+            const int i = warp * kRows + 8 * b + 2 * t + e;
+            float* row = jo + i * H::kPitch;
+#pragma unroll
+            for (int u = 0; u < kTiles; ++u)
+                *reinterpret_cast<float2*>(row + (u / 8) * 128 + kWide * g + 2 * (u % 8)) =
+                    make_float2(o[u][b][e], o[u][b][2 + e]);
+            if (g == 0) {
+                jm[i * 3] = ref[b][e];
+                jm[i * 3 + 1] = vref[b][e];
+                jm[i * 3 + 2] = z;
+            }
         }
-    }
     __syncthreads();
     const bool whole = blk.used == 1;
     const int64_t unit =
@@ -469,29 +503,28 @@ k_attend(const __grid_constant__ Args a) {
         float m = -INFINITY, mv = -INFINITY, total = 0.0f, w[kWarps];
 #pragma unroll
         for (int i = 0; i < kWarps; ++i) {
-            m = fmaxf(m, jm[(i * 16 + row) * 3]);
-            mv = fmaxf(mv, jm[(i * 16 + row) * 3 + 1]);
+            m = fmaxf(m, jm[(i * kRows + row) * 3]);
+            mv = fmaxf(mv, jm[(i * kRows + row) * 3 + 1]);
         }
 #pragma unroll
         for (int i = 0; i < kWarps; ++i) {
-            const float* st = jm + (i * 16 + row) * 3;
+            const float* st = jm + (i * kRows + row) * 3;
             total += st[0] == -INFINITY ? st[2] : st[2] * exp2f(st[0] - m);
             w[i] = st[1] == -INFINITY ? 0.0f : exp2f(st[1] - mv);
         }
         const bool none = total == 0.0f;
-        // O is in units of 2^(mv - lift); of the sum's 2^m
-        const float per = none ? 0.0f
-                               : kv8::kOperandUnit<FORMAT> * exp2f(-kLift) / total;
+        // O is in units of 2^(mv - lift), the sum of 2^m
+        const float per = none ? 0.0f : exp2f(-kLift) / total;
         const float unit_v = none ? 0.0f : exp2f(mv - m);
-        const int64_t at = (int64_t)block * 16 + row;
+        const int64_t at = (int64_t)block * kRows + row;
         const int64_t tok = blk.s.lo + at / group;
         const int h = head * group + (int)(at % group);
         T* out = static_cast<T*>(a.out) + tok * a.out_stride + (int64_t)h * a.d;
-        float* part = whole ? nullptr : a.part + (unit * 16 + row) * a.d;
+        float* part = whole ? nullptr : a.part + (unit * kRows + row) * a.d;
         for (int i = lane; i < a.d; i += 32) {
             float y = 0.0f;
 #pragma unroll
-            for (int k = 0; k < kWarps; ++k) y += w[k] * jo[(k * 16 + row) * kPitch + i];
+            for (int k = 0; k < kWarps; ++k) y += w[k] * jo[(k * kRows + row) * H::kPitch + i];
             y = none ? 0.0f : y * per * unit_v;
             if (whole)
                 tbk::Elt<T>::store(out + i, y);
@@ -500,53 +533,65 @@ k_attend(const __grid_constant__ Args a) {
         }
         if (lane == 0) {
             if (!whole)
-                a.state[unit * 16 + row] = make_float2(m, total);
+                a.state[unit * kRows + row] = make_float2(m, total);
             else if (a.lse)
                 a.lse[tok * a.hq + h] = none ? -INFINITY : m * 0.69314718055994531f + logf(total);
         }
     }
 }
 
-// Joins the chunks of each block: out = sum_c w_c out_c / sum_c w_c, w_c the
-// chunk's sum at the largest reference.  A warp per row.
+// Joins the chunks of a row: out = sum_c w_c out_c / sum_c w_c, w_c the chunk's
+// sum at the largest reference.  A CTA per row; its warps take every fourth
+// chunk, so that a long context's hundred chunks are a few loads deep.
 template <typename T>
 __global__ void __launch_bounds__(kThreads) k_join(const __grid_constant__ Args a) {
-    const int block = blockIdx.x, head = blockIdx.y, seq = blockIdx.z;
+    __shared__ float part[kWarps][kv8::kMaxDim];
+    __shared__ float total_s[kWarps];
+    const int block = blockIdx.x / a.block_rows, row = blockIdx.x % a.block_rows;
+    const int head = blockIdx.y, seq = blockIdx.z;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    asm volatile("griddepcontrol.wait;" ::: "memory");
     const Block blk = block_of(a, seq, block, false);
-    if (blk.rows == 0 || blk.used == 1) return;
+    if (row >= blk.rows || blk.used == 1) return;
     const int group = a.hq / a.hkv;
     const int64_t unit = (((int64_t)seq * a.hkv + head) * a.blocks + block) * a.chunks;
-    for (int row = warp; row < blk.rows; row += kWarps) {
-        const float2* st = a.state + unit * 16 + row;
-        float m = -INFINITY;
-        for (int c = lane; c < blk.used; c += 32) m = fmaxf(m, st[c * 16].x);
-        m = tbk::warp_max(m);
-        float total = 0.0f, y[kv8::kMaxDim / 32];
+    const float2* st = a.state + unit * a.block_rows + row;
+    float m = -INFINITY;
+    for (int c = lane; c < blk.used; c += 32) m = fmaxf(m, st[c * a.block_rows].x);
+    m = tbk::warp_max(m);
+    float total = 0.0f, y[kv8::kMaxDim / 32];
 #pragma unroll
-        for (int i = 0; i < kv8::kMaxDim / 32; ++i) y[i] = 0.0f;
-        for (int c = 0; c < blk.used; ++c) {
-            const float2 s = st[c * 16];
-            const float w = s.x == -INFINITY ? s.y : s.y * exp2f(s.x - m);
-            const float* part = a.part + ((unit + c) * 16 + row) * a.d;
-            total += w;
-#pragma unroll
-            for (int i = 0; i < kv8::kMaxDim / 32; ++i)
-                if (lane + 32 * i < a.d) y[i] += w * part[lane + 32 * i];
-        }
-        const bool none = total == 0.0f;
-        const int64_t at = (int64_t)block * 16 + row;
-        const int64_t tok = blk.s.lo + at / group;
-        const int h = head * group + (int)(at % group);
-        T* out = static_cast<T*>(a.out) + tok * a.out_stride + (int64_t)h * a.d;
+    for (int i = 0; i < kv8::kMaxDim / 32; ++i) y[i] = 0.0f;
+#pragma unroll 4
+    for (int c = warp; c < blk.used; c += kWarps) {
+        const float2 s = st[c * a.block_rows];
+        const float w = s.x == -INFINITY ? s.y : s.y * exp2f(s.x - m);
+        const float* p = a.part + ((unit + c) * a.block_rows + row) * a.d;
+        total += w;
 #pragma unroll
         for (int i = 0; i < kv8::kMaxDim / 32; ++i)
-            if (lane + 32 * i < a.d)
-                tbk::Elt<T>::store(out + lane + 32 * i, none ? 0.0f : y[i] / total);
-        if (a.lse && lane == 0)
-            a.lse[tok * a.hq + h] = none ? -INFINITY : m * 0.69314718055994531f + logf(total);
+            if (lane + 32 * i < a.d) y[i] += w * p[lane + 32 * i];
     }
+#pragma unroll
+    for (int i = 0; i < kv8::kMaxDim / 32; ++i)
+        if (lane + 32 * i < a.d) part[warp][lane + 32 * i] = y[i];
+    if (lane == 0) total_s[warp] = total;
+    __syncthreads();
+    total = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kWarps; ++i) total += total_s[i];
+    const bool none = total == 0.0f;
+    const int64_t at = (int64_t)block * a.block_rows + row;
+    const int64_t tok = blk.s.lo + at / group;
+    const int h = head * group + (int)(at % group);
+    T* out = static_cast<T*>(a.out) + tok * a.out_stride + (int64_t)h * a.d;
+    for (int i = threadIdx.x; i < a.d; i += kThreads) {
+        float z = 0.0f;
+#pragma unroll
+        for (int k = 0; k < kWarps; ++k) z += part[k][i];
+        tbk::Elt<T>::store(out + i, none ? 0.0f : z / total);
+    }
+    if (a.lse && threadIdx.x == 0)
+        a.lse[tok * a.hq + h] = none ? -INFINITY : m * 0.69314718055994531f + logf(total);
 }
 
 int check(const TbB200Kv8* cache, const TbB200Kv8Batch* batch, const TbB200Kv8Attention* t,
@@ -567,10 +612,11 @@ int check(const TbB200Kv8* cache, const TbB200Kv8Batch* batch, const TbB200Kv8At
     return TB_OK;
 }
 
-// How a call is cut: blocks of 16 rows per sequence and head, chunks of keys
-// per block, scratch.
+// How a call is cut: blocks of rows per sequence and head, chunks of keys per
+// block, scratch.
 struct Plan {
     int64_t blocks, chunks;
+    int block_rows;
     size_t part_bytes, state_bytes;
 };
 
@@ -578,10 +624,12 @@ Plan plan_of(const TbB200Kv8* cache, const TbB200Kv8Batch* batch, const TbB200Kv
              int sm_count) {
     Plan p;
     const int64_t rows = t->max_rows < batch->rows ? t->max_rows : batch->rows;
-    p.blocks = (rows * (t->n_heads / cache->n_kv_heads) + 15) / 16;
+    const int64_t most_rows = rows * (t->n_heads / cache->n_kv_heads);
+    p.block_rows = most_rows <= 8 ? 8 : 16;
+    p.blocks = (most_rows + p.block_rows - 1) / p.block_rows;
     if (p.blocks < 1) p.blocks = 1;
     const int64_t all = p.blocks * cache->n_kv_heads * batch->n_seqs;
-    const int64_t slots = 3 * (int64_t)sm_count;
+    const int64_t slots = (p.block_rows == 8 ? 4 : 3) * (int64_t)sm_count;
     int64_t keys = t->max_len;
     if (t->window && t->window + rows < keys) keys = t->window + rows;
     const int64_t most = (keys + kLeastChunk - 1) / kLeastChunk;
@@ -589,26 +637,32 @@ Plan plan_of(const TbB200Kv8* cache, const TbB200Kv8Batch* batch, const TbB200Kv
     if (p.chunks > most) p.chunks = most;
     if (p.chunks < 1) p.chunks = 1;
     const size_t units = p.chunks > 1 ? (size_t)(all * p.chunks) : 0;
-    p.part_bytes = units * 16 * cache->head_dim * sizeof(float);
-    p.state_bytes = units * 16 * sizeof(float2);
+    p.part_bytes = units * p.block_rows * cache->head_dim * sizeof(float);
+    p.state_bytes = units * p.block_rows * sizeof(float2);
     return p;
 }
 
-template <typename T, int FORMAT, int DP>
+template <typename T, int FORMAT, int DP, int NB>
 int launch(const Args& a, dim3 grid, cudaStream_t s) {
-    constexpr int bytes = smem_bytes<T, DP>();
-    TB_CUDA_TRY(cudaFuncSetAttribute(k_attend<T, FORMAT, DP>,
+    constexpr int bytes = Shape<T, DP, NB>::kBytes;
+    TB_CUDA_TRY(cudaFuncSetAttribute(k_attend<T, FORMAT, DP, NB>,
                                      cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
-    k_attend<T, FORMAT, DP><<<grid, kThreads, bytes, s>>>(a);
+    k_attend<T, FORMAT, DP, NB><<<grid, kThreads, bytes, s>>>(a);
     TB_LAUNCH_CHECK("8-bit cache attention kernel");
     return TB_OK;
 }
 
-template <typename T, int FORMAT>
+template <typename T, int FORMAT, int NB>
 int launch_dim(const Args& a, dim3 grid, cudaStream_t s) {
-    if (a.d <= 64) return launch<T, FORMAT, 64>(a, grid, s);
-    if (a.d <= 128) return launch<T, FORMAT, 128>(a, grid, s);
-    return launch<T, FORMAT, 256>(a, grid, s);
+    if (a.d <= 64) return launch<T, FORMAT, 64, NB>(a, grid, s);
+    if (a.d <= 128) return launch<T, FORMAT, 128, NB>(a, grid, s);
+    return launch<T, FORMAT, 256, NB>(a, grid, s);
+}
+
+template <typename T, int FORMAT>
+int launch_rows(const Args& a, dim3 grid, cudaStream_t s) {
+    return a.block_rows == 8 ? launch_dim<T, FORMAT, 1>(a, grid, s)
+                             : launch_dim<T, FORMAT, 2>(a, grid, s);
 }
 
 }  // namespace
@@ -638,7 +692,7 @@ extern "C" int tb_b200_kv8_attention(const TbB200Kv8* cache, const TbB200Kv8Batc
     tbh::DeviceState* ds = tbh::current_device_state();
     if (!ds) return TB_ERR_DEVICE;
     const Plan p = plan_of(cache, batch, t, ds->sm_count);
-    if (p.blocks * p.chunks > INT32_MAX) return TB_ERR_INVALID_SHAPE;
+    if (p.blocks * p.chunks > INT32_MAX || p.blocks * p.block_rows > INT32_MAX) return TB_ERR_INVALID_SHAPE;
     const size_t bytes = p.part_bytes + p.state_bytes;
     if (bytes && (!t->workspace || t->workspace_bytes < bytes || !tbh::aligned16(t->workspace))) {
         tbh::set_error_text("8-bit cache attention: workspace missing, small or misaligned");
@@ -668,16 +722,17 @@ extern "C" int tb_b200_kv8_attention(const TbB200Kv8* cache, const TbB200Kv8Batc
     a.max_len = t->max_len;
     a.chunks = (int)p.chunks;
     a.blocks = (int)p.blocks;
+    a.block_rows = p.block_rows;
     a.vec = tbh::aligned16(t->q) && t->q_stride * s % 16 == 0;
     const dim3 grid((unsigned)(p.blocks * p.chunks), (unsigned)a.hkv, (unsigned)batch->n_seqs);
     cudaStream_t st = tbh::stream_of(stream);
     const bool f32 = t->dtype == TB_DTYPE_F32, int8 = cache->format == kv8::kInt8;
-    rc = f32 ? (int8 ? launch_dim<float, kv8::kInt8>(a, grid, st)
-                     : launch_dim<float, kv8::kE4m3>(a, grid, st))
-             : (int8 ? launch_dim<__nv_bfloat16, kv8::kInt8>(a, grid, st)
-                     : launch_dim<__nv_bfloat16, kv8::kE4m3>(a, grid, st));
+    rc = f32 ? (int8 ? launch_rows<float, kv8::kInt8>(a, grid, st)
+                     : launch_rows<float, kv8::kE4m3>(a, grid, st))
+             : (int8 ? launch_rows<__nv_bfloat16, kv8::kInt8>(a, grid, st)
+                     : launch_rows<__nv_bfloat16, kv8::kE4m3>(a, grid, st));
     if (rc != TB_OK || p.chunks == 1) return rc;
-    const dim3 joins((unsigned)p.blocks, (unsigned)a.hkv, (unsigned)batch->n_seqs);
+    const dim3 joins((unsigned)(p.blocks * p.block_rows), (unsigned)a.hkv, (unsigned)batch->n_seqs);
     if (f32)
         k_join<float><<<joins, kThreads, 0, st>>>(a);
     else

@@ -1,18 +1,11 @@
 // kv8_mma.cuh -- 8-bit codes as operands of the f16 matrix instructions.
 //
-// Every code is an f16 value: int8 exactly, e4m3 exactly at 2^-8 of its value
-// (its exponent and mantissa bits moved into f16's places).  Conversion never
-// makes a NaN or an infinity, so what lies in unused slots, multiplied by a
-// weight of zero, adds nothing.
+// Every code is an f16 value exactly, subnormal e4m3 codes among them.
 #pragma once
 
 #include "kv8.cuh"
 
 namespace kv8 {
-
-// What a format's f16 operands are short of the code's value by.
-template <int FORMAT>
-constexpr float kOperandUnit = FORMAT == kE4m3 ? 256.0f : 1.0f;
 
 __device__ __forceinline__ uint32_t prmt(uint32_t a, uint32_t b, uint32_t sel) {
     uint32_t r;
@@ -20,22 +13,60 @@ __device__ __forceinline__ uint32_t prmt(uint32_t a, uint32_t b, uint32_t sel) {
     return r;
 }
 
-// The bytes 0 and 2 (even), and 1 and 3 (odd), of w as two f16.
+// Two codes (the low or high half of w) as two f16.
+__device__ __forceinline__ uint32_t e4m3_pair(uint32_t w, bool high) {
+    uint32_t r;
+    const uint16_t h = (uint16_t)(high ? w >> 16 : w);
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"(h));
+    return r;
+}
+// Bytes 0 and 2 of w (1 and 3: of w >> 8): 1024 + (code + 128) is the f16
+// 0x6400 | (code ^ 0x80); less 1152 it is the code.
+__device__ __forceinline__ uint32_t int8_pair(uint32_t w) {
+    uint32_t e = (w & 0x00ff00ffu) ^ 0x64806480u;
+    const __half2 bias = __halves2half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480));
+    const __half2 h = __hsub2(*reinterpret_cast<__half2*>(&e), bias);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// Which elements of a word of four the two registers of word() hold.
 template <int FORMAT>
-__device__ __forceinline__ void to_f16(uint32_t w, uint32_t& even, uint32_t& odd) {
+__device__ constexpr int word_element(int reg, int i) {
+    return FORMAT == kInt8 ? reg + 2 * i : 2 * reg + i;
+}
+template <int FORMAT>
+__device__ __forceinline__ void word(uint32_t w, uint32_t& r0, uint32_t& r1) {
     if constexpr (FORMAT == kInt8) {
-        // 1024 + (code + 128) is f16 0x6400 | code ^ 0x80; less 1152 the code
-        const __half2 bias = __halves2half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480));
-        uint32_t e = (w & 0x00ff00ffu) ^ 0x64806480u;
-        uint32_t o = ((w >> 8) & 0x00ff00ffu) ^ 0x64806480u;
-        const __half2 he = __hsub2(*reinterpret_cast<__half2*>(&e), bias);
-        const __half2 ho = __hsub2(*reinterpret_cast<__half2*>(&o), bias);
-        even = *reinterpret_cast<const uint32_t*>(&he);
-        odd = *reinterpret_cast<const uint32_t*>(&ho);
+        r0 = int8_pair(w);
+        r1 = int8_pair(w >> 8);
     } else {
-        even = ((w << 8) & 0x80008000u) | ((w << 7) & 0x3f803f80u);
-        odd = (w & 0x80008000u) | ((w >> 1) & 0x3f803f80u);
+        r0 = e4m3_pair(w, false);
+        r1 = e4m3_pair(w, true);
     }
+}
+// Elements 0 .. 3 of two words, each with its partner of the other word.
+template <int FORMAT>
+__device__ __forceinline__ void words(uint32_t a, uint32_t b, uint32_t (&r)[4]) {
+    if constexpr (FORMAT == kInt8) {
+        const uint32_t x = prmt(a, b, 0x5410), y = prmt(a, b, 0x7632);
+        r[0] = int8_pair(x);
+        r[1] = int8_pair(x >> 8);
+        r[2] = int8_pair(y);
+        r[3] = int8_pair(y >> 8);
+    } else {
+        const uint32_t x = prmt(a, b, 0x5140), y = prmt(a, b, 0x7362);
+        r[0] = e4m3_pair(x, false);
+        r[1] = e4m3_pair(x, true);
+        r[2] = e4m3_pair(y, false);
+        r[3] = e4m3_pair(y, true);
+    }
+}
+
+// The transpose of an 8 x 8 tile of f16, two to a lane.
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+    uint32_t y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
 }
 
 __device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
