@@ -7,8 +7,9 @@
 // when there are few blocks; a second kernel joins the chunks.
 //
 // Within a CTA each of 4 warps takes every fourth step of 16 keys, which lie in
-// one page, through a ring of cp.async stages of its own: no barrier in the
-// loop.  The codes go from shared memory to registers with 16-byte loads and
+// one page, through a ring of TMA stages of its own: one lane issues two copies
+// a step, and no barrier of the CTA is in the loop.  The codes go from shared
+// memory to registers with 16-byte loads and
 // are converted there, as the left operands of m16n8k16 instructions, so that 8
 // rows fill the other side:
 //   S^T = K Q^T: lane (g, t) (g = lane / 4, t = lane % 4) holds keys order(g)
@@ -17,8 +18,8 @@
 //   O^T = V^T P^T: S^T's registers, transposed 8 x 8, are P^T's operands; lane
 //     (g, t) holds elements 16 g .. 16 g + 15 (of 128) of keys order(2t),
 //     order(2t + 1) and those + 8.
-// order() and the two swizzles below put the 8 lanes of each 16-byte access
-// into different banks.
+// order() and TMA's swizzle (the 16-byte piece c of key r lies at c ^ (r & 7))
+// put the 8 lanes of each 16-byte access into different banks.
 //
 // Precision.  A code is an f16 exactly.  A row of q is scaled by a power of two
 // to [2^14, 2^15) and held as f16: bf16 elements exactly unless 2^-21 below the
@@ -32,7 +33,6 @@
 // A weight more than 2^-25 below the row's largest is an f16 subnormal, off by
 // at most 2^-36 of the largest.
 #include "kv8_mma.cuh"
-#include "tma.cuh"
 
 namespace {
 
@@ -45,12 +45,12 @@ constexpr float kLift = 11.0f;     // weights are held times 2^11: up to 2^15 in
 constexpr float kLog2e = 1.4426950408889634f;
 
 struct Args {
+    CUtensorMap k_map, v_map;  // [n_pages * n_kv_heads][page][d] codes
     kv8::Batch b;
     const void* q;
     void* out;
     float* lse;
     int64_t q_stride, out_stride;
-    const uint8_t *k, *v;
     const float *k_scale, *v_scale;
     unsigned* status;
     float* part;    // [seq, kv head, block, chunk][block_rows][d] partial outputs
@@ -72,16 +72,16 @@ __device__ __forceinline__ Block block_of(const Args& a, int seq, int block, boo
     Block k;
     k.s = kv8::sequence(a.b, seq);
     const int group = a.hq / a.hkv;
-    const int64_t all = (int64_t)k.s.n * group, at = (int64_t)block * a.block_rows;
-    k.rows = (int)max((int64_t)0, min((int64_t)a.block_rows, all - at));
+    const int at = block * a.block_rows;  // rows * group fits an int
+    k.rows = max(0, min(a.block_rows, k.s.n * group - at));
     k.lo = k.end = 0;
     if (k.rows > 0) {
         if (k.s.len > a.max_len || k.s.n > a.max_rows ||
             k.s.len > ((int64_t)a.b.width << a.b.page_shift)) {
             if (flag) atomicOr(a.status, TB_B200_FLAG_POSITION_RANGE);
         } else {
-            const int p0 = k.s.first + (int)(at / group);
-            const int p1 = k.s.first + (int)((at + k.rows - 1) / group);
+            const int p0 = k.s.first + at / group;
+            const int p1 = k.s.first + (at + k.rows - 1) / group;
             k.end = max(p1 + 1, 0);
             k.lo = a.window ? min(max(p0 - a.window + 1, 0), k.end) : 0;
         }
@@ -95,13 +95,13 @@ __device__ __forceinline__ Block block_of(const Args& a, int seq, int block, boo
 }
 
 // The key (of 8) that row g of an operand stands for.
-__device__ __forceinline__ int order(int n) { return n & 1 ? (n >> 1) ^ 5 : n >> 1; }
-// Where a key's 16-byte piece c lies.
-__device__ __forceinline__ int k_place(int key, int c, int pieces) {
-    return pieces > 4 ? c ^ ((key & 1) << 2) : c;
-}
-__device__ __forceinline__ int v_place(int key, int c, int pieces) {
-    return pieces > 4 ? c ^ ((key & 3) << 1) : c ^ (key & 2);
+__device__ __forceinline__ int order(int n) { return n ^ ((n & 1) << 2); }
+// Where the 16-byte piece c of a stage's key lies: DP = 64 has rows of 64 bytes
+// and that swizzle, DP = 256 two tiles of 128-byte rows.
+template <int DP>
+__device__ __forceinline__ int place(int key, int c) {
+    if constexpr (DP == 64) return key * 64 + (c ^ (key >> 1 & 3)) * 16;
+    return (c >> 3) * kStep * 128 + key * 128 + ((c ^ key) & 7) * 16;
 }
 
 // Shapes of a kernel for heads of up to DP elements and blocks of 8 NB rows.
@@ -110,16 +110,15 @@ struct Shape {
     static constexpr bool kSplit = sizeof(T) == 4;  // hi + lo operands
     static constexpr int kStages = DP == 64 ? 5 : 3;
     static constexpr int kStageBytes = 2 * kStep * DP;
-    static constexpr int kStagePitch = kStageBytes + 16;  // and the page's two scales
     static constexpr int kSteps = DP / 16;                // 16-wide steps of the head dimension
     static constexpr int kRows = 8 * NB;
     // Q's operands stay in registers when they are few
     static constexpr bool kQReg = kSteps * 2 * NB * (kSplit ? 2 : 1) <= 32;
     static constexpr int kQBytes = kQReg ? 0 : kSteps * NB * 256 * (kSplit ? 2 : 1);
-    static constexpr int kRing = kWarps * kStages * kStagePitch;
+    static constexpr int kRing = kWarps * kStages * kStageBytes;  // a multiple of 1024
     static constexpr int kPitch = DP + 4;
     static constexpr int kJoin = kWarps * kRows * (kPitch + 3) * 4;
-    static constexpr int kBytes = (kRing > kJoin ? kRing : kJoin) + kQBytes;
+    static constexpr int kBytes = (kRing > kJoin ? kRing : kJoin) + kQBytes + 1024;  // 1024: to align
     // CTAs per SM: what registers (O: DP NB / 4 a lane) and shared memory allow
     static constexpr int kCtas = DP * NB >= 512 ? 2 : DP * NB >= 256 ? (DP == 256 ? 2 : 3) : 4;
 };
@@ -129,9 +128,12 @@ __global__ void __launch_bounds__(kThreads, Shape<T, DP, NB>::kCtas)
 k_attend(const __grid_constant__ Args a) {
     using H = Shape<T, DP, NB>;
     constexpr bool kSplit = H::kSplit, kQReg = H::kQReg;
-    constexpr int kSteps = H::kSteps, kStages = H::kStages, kPieces = DP / 16, kRows = H::kRows;
+    constexpr int kSteps = H::kSteps, kStages = H::kStages, kRows = H::kRows;
     constexpr int kTiles = DP / 16;  // 16-wide output tiles
-    extern __shared__ __align__(16) uint8_t smem[];
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ uint64_t bars[kWarps * kStages];
+    // TMA's swizzle goes by the address: tiles start on 1024 bytes
+    uint8_t* smem = smem_raw + (-tbk::smem_addr(smem_raw) & 1023u);
 
     const int c = blockIdx.x % a.chunks, block = blockIdx.x / a.chunks;
     const int head = blockIdx.y, seq = blockIdx.z;
@@ -140,19 +142,74 @@ k_attend(const __grid_constant__ Args a) {
     if (blk.rows == 0 || c >= blk.used) return;
     const int group = a.hq / a.hkv;
     const int begin = blk.from + c * blk.size, end = min(begin + blk.size, blk.end);
-    const int pieces = a.d / 16;
+
+    // the warp's steps: keys first + 64 n .. + 15
+    const int first = begin + warp * kStep;
+    const int n_steps = end > first ? (end - first + kWarps * kStep - 1) / (kWarps * kStep) : 0;
+    uint8_t* ring = smem + warp * kStages * H::kStageBytes;
+    uint64_t* bar = bars + warp * kStages;
+    if (lane == 0) {
+#pragma unroll
+        for (int i = 0; i < kStages; ++i) tbk::mbar_init(bar + i, 1);
+        tbk::fence_mbar_init();
+    }
+    __syncwarp();
+    const int32_t* table = a.b.table + seq * a.b.table_stride;
+    auto page_of = [&](int n) {  // the page of step n, -1 if it has none
+        if (n >= n_steps) return -1;
+        const int id = table[(first + n * (kWarps * kStep)) >> a.b.page_shift];
+        if (id >= 0 && id < a.b.n_pages) return id;
+        atomicOr(a.status, TB_B200_FLAG_PAGE_RANGE);
+        return -1;
+    };
+    // Lane i has the page of step 32 m + i and its scales, m the batch that is
+    // being issued; the next batch's pages are on their way.
+    int ids = page_of(lane), ids_next = page_of(32 + lane);
+    float ks_issued = 0.0f, vs_issued = 0.0f, ks = 0.0f, vs = 0.0f;
+    uint32_t pages_issued, pages = 0;  // which steps of the batch have a page
+    auto load_scales = [&] {
+        pages_issued = __ballot_sync(tbk::kFull, ids >= 0);
+        if (ids >= 0) {
+            const int unit = ids * a.hkv + head;
+            ks_issued = a.k_scale[unit];
+            vs_issued = a.v_scale[unit];
+        }
+    };
+    load_scales();
+    auto issue = [&](int n, int stage) {
+        if ((n & 31) == 0 && n > 0) {
+            ids = ids_next;
+            load_scales();
+            ids_next = page_of(n + 32 + lane);
+        }
+        const int id = __shfl_sync(tbk::kFull, ids, n & 31);
+        if (lane == 0 && id >= 0) {
+            uint8_t* dst = ring + stage * H::kStageBytes;
+            const int slot = (first + n * (kWarps * kStep)) & ((1 << a.b.page_shift) - 1);
+            tbk::mbar_expect_tx(bar + stage, H::kStageBytes);
+#pragma unroll
+            for (int h = 0; h < (DP + 127) / 128; ++h) {
+                kv8::tma_load3(dst + h * kStep * 128, &a.k_map, h * 128, slot, id * a.hkv + head,
+                               bar + stage);
+                kv8::tma_load3(dst + kStep * DP + h * kStep * 128, &a.v_map, h * 128, slot,
+                               id * a.hkv + head, bar + stage);
+            }
+        }
+    };
+#pragma unroll
+    for (int n = 0; n < kStages - 1; ++n) issue(n, n);
 
     // Q's operands: rows g, g + 8, .. of the block; a row's scores are
     // multiplied with qf, but for the page's scale
     uint32_t qr[kQReg ? kSteps : 1][NB][2], ql[kQReg && kSplit ? kSteps : 1][NB][2];
-    uint2* qs = reinterpret_cast<uint2*>(smem + H::kBytes - H::kQBytes);
+    uint2* qs = reinterpret_cast<uint2*>(smem + H::kBytes - 1024 - H::kQBytes);
     float qf[NB];
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
         const int i = 8 * b + g;
         const bool live = i < blk.rows;
-        const int64_t at = (int64_t)block * kRows + i;
-        const int tok = live ? (int)(at / group) : 0, hh = live ? (int)(at % group) : 0;
+        const int at = block * kRows + i, tok = live ? at / group : 0;
+        const int hh = live ? at - tok * group : 0;
         const T* q = static_cast<const T*>(a.q) + (blk.s.lo + tok) * a.q_stride +
                      (int64_t)(head * group + hh) * a.d;
         float top = 0.0f;
@@ -211,71 +268,12 @@ k_attend(const __grid_constant__ Args a) {
             const int i = 8 * b + 2 * t + e;
             // rows of the block that are not there see all and are not stored
             const bool live = i < blk.rows;
-            const int p = blk.s.first + (int)(((int64_t)block * kRows + i) / group);
+            const int p = blk.s.first + (block * kRows + i) / group;
             see_hi[b][e] = live ? p : INT32_MAX;
             see_lo[b][e] = a.window && live ? max(p - a.window + 1, 0) : 0;
         }
 
-    // the warp's steps: keys first + 64 n .. + 15
-    const int first = begin + warp * kStep;
-    const int n_steps = end > first ? (end - first + kWarps * kStep - 1) / (kWarps * kStep) : 0;
-    uint8_t* ring = smem + warp * kStages * H::kStagePitch;
-    const uint32_t ring_s = tbk::smem_addr(ring);
-    if (pieces < kPieces) {
-        // elements past the head dimension are codes of zero, never written again
-        for (int i = lane; i < kStages * kStep * (kPieces - pieces); i += 32) {
-            const int piece = pieces + i % (kPieces - pieces), key = i / (kPieces - pieces);
-            *reinterpret_cast<uint4*>(ring + (key / kStep) * H::kStagePitch + (key % kStep) * DP +
-                                      k_place(key % kStep, piece, kPieces) * 16) =
-                make_uint4(0, 0, 0, 0);
-        }
-    }
-    __syncthreads();
-    const int32_t* table = a.b.table + seq * a.b.table_stride;
-    auto page_of = [&](int n) {  // the page of step n, -1 if it has none
-        if (n >= n_steps) return -1;
-        const int id = table[(first + n * (kWarps * kStep)) >> a.b.page_shift];
-        if (id >= 0 && id < a.b.n_pages) return id;
-        atomicOr(a.status, TB_B200_FLAG_PAGE_RANGE);
-        return -1;
-    };
-    int ids = page_of(lane), ids_next = page_of(32 + lane);  // of steps [0, 32), [32, 64)
-    constexpr int kKeys = 32 / kPieces;                       // keys per warp access
-    const int my_piece = lane % kPieces, my_key = lane / kPieces;
-    auto issue = [&](int n) {
-        const int id = __shfl_sync(tbk::kFull, ids, n & 31);
-        if ((n & 31) == 31) {
-            ids = ids_next;
-            ids_next = page_of(n + 33 + lane);
-        }
-        if (id >= 0) {
-            const int64_t unit = (int64_t)id * a.hkv + head;
-            const int slot = (first + n * (kWarps * kStep)) & ((1 << a.b.page_shift) - 1);
-            const int64_t at =
-                ((unit << a.b.page_shift) + slot + my_key) * a.d + my_piece * 16;
-            const uint8_t *k = a.k + at, *v = a.v + at;
-            const uint32_t dst = ring_s + (n % kStages) * H::kStagePitch;
-            if (my_piece < pieces) {
-#pragma unroll
-                for (int i = 0; i < kStep / kKeys; ++i) {
-                    const int key = my_key + i * kKeys;
-                    kv8::cp_async16(dst + key * DP + k_place(key, my_piece, kPieces) * 16,
-                                    k + i * kKeys * a.d);
-                    kv8::cp_async16(
-                        dst + (kStep + key) * DP + v_place(key, my_piece, kPieces) * 16,
-                        v + i * kKeys * a.d);
-                }
-            }
-            if (lane < 2)
-                kv8::cp_async4(dst + H::kStageBytes + 4 * lane,
-                               (lane ? a.v_scale : a.k_scale) + unit);
-        }
-        kv8::cp_async_commit();
-        return id >= 0;
-    };
-    uint32_t there = 0;  // bit i: the step i behind the newest issued one has a page
-#pragma unroll
-    for (int n = 0; n < kStages - 1; ++n) there = there << 1 | (uint32_t)issue(n);
+    if constexpr (!kQReg) __syncthreads();
 
     float o[kTiles][NB][4];
 #pragma unroll
@@ -294,19 +292,45 @@ k_attend(const __grid_constant__ Args a) {
         }
 
     const int ka = order(2 * t), kb = order(2 * t + 1), kg = order(g);
+    uint32_t phases = 0;  // of each stage's barrier: a page out of range has no copy
+    int at_stage = kStages - 1;
     for (int n = 0; n < n_steps; ++n) {
-        kv8::cp_async_wait<kStages - 2>();
-        __syncwarp();
-        there = there << 1 | (uint32_t)issue(n + kStages - 1);
-        if (!(there >> (kStages - 1) & 1)) continue;
-        uint8_t* stage = ring + (n % kStages) * H::kStagePitch;
-        const float2 scales = *reinterpret_cast<const float2*>(stage + H::kStageBytes);
+        if ((n & 31) == 0) {
+            ks = ks_issued;
+            vs = vs_issued;
+            pages = pages_issued;
+        }
+        __syncwarp();  // step n - 1's stage has been read: it is the next to be filled
+        issue(n + kStages - 1, at_stage);
+        at_stage = at_stage == kStages - 1 ? 0 : at_stage + 1;
+        if (!(pages >> (n & 31) & 1)) continue;
+        const float k_scale = __shfl_sync(tbk::kFull, ks, n & 31);
+        const float v_scale = __shfl_sync(tbk::kFull, vs, n & 31);
+        uint8_t* stage = ring + at_stage * H::kStageBytes;
+        const uint32_t phase = phases >> at_stage & 1;
+        phases ^= 1u << at_stage;
+        const bool came = tbk::mbar_wait(bar + at_stage, phase, a.status);
+        if (!__all_sync(tbk::kFull, came)) {
+            // the copy did not come: the output is invalid and flagged.  No copy
+            // may be in flight when the block ends: wait for the others, bounded.
+            for (int i = 1; i < kStages; ++i) {
+                const int m = n + i, x = (at_stage + i) % kStages;
+                const int id = m < n_steps ? table[(first + m * (kWarps * kStep)) >> a.b.page_shift]
+                                           : -1;
+                if (id >= 0 && id < a.b.n_pages)
+                    tbk::mbar_wait(bar + x, phases >> x & 1, a.status);
+            }
+            break;
+        }
         const int key0 = first + n * (kWarps * kStep);
         if (key0 + kStep > blk.s.len) {
             // slots behind the last token may hold anything, NaN codes too: a
             // weight of zero needs a finite value beside it
-            for (int i = (blk.s.len - key0) * DP / 16 + lane; i < kStep * DP / 16; i += 32)
-                *reinterpret_cast<uint4*>(stage + kStep * DP + 16 * i) = make_uint4(0, 0, 0, 0);
+            for (int i = lane; i < kStep * DP / 16; i += 32)
+                if (key0 + i % kStep >= blk.s.len)
+                    *reinterpret_cast<uint4*>(stage + kStep * DP +
+                                              place<DP>(i % kStep, i / kStep)) =
+                        make_uint4(0, 0, 0, 0);
             __syncwarp();
         }
 
@@ -320,10 +344,10 @@ k_attend(const __grid_constant__ Args a) {
                 for (int e = 0; e < 4; ++e) s2[i][b][e] = 0.0f;
 #pragma unroll
         for (int h = 0; h < DP / 64; ++h) {
-            const uint4 x = *reinterpret_cast<const uint4*>(
-                stage + kg * DP + k_place(kg, 4 * h + t, kPieces) * 16);
-            const uint4 y = *reinterpret_cast<const uint4*>(
-                stage + (kg + 8) * DP + k_place(kg + 8, 4 * h + t, kPieces) * 16);
+            const uint4 x =
+                *reinterpret_cast<const uint4*>(stage + place<DP>(kg, 4 * h + t));
+            const uint4 y =
+                *reinterpret_cast<const uint4*>(stage + place<DP>(kg + 8, 4 * h + t));
             const uint32_t wx[4] = {x.x, x.y, x.z, x.w}, wy[4] = {y.x, y.y, y.z, y.w};
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
@@ -350,14 +374,14 @@ k_attend(const __grid_constant__ Args a) {
         }
         // log2 units: s[b][2 i + e] is key key0 + kg + 8 i, row 8 b + 2 t + e; the
         // values' scale as an exponent
-        const float lv = (float)((int)(__float_as_uint(scales.y) >> 23) - 127);
+        const float lv = (float)((int)(__float_as_uint(v_scale) >> 23) - 127);
         float s[NB][4];
         bool inside = true, over = false;
 #pragma unroll
         for (int b = 0; b < NB; ++b)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-                const float f = qc[b][e] * scales.x;
+                const float f = qc[b][e] * k_scale;
                 s[b][e] = (s2[0][b][e] + s2[1][b][e]) * f;
                 s[b][2 + e] = (s2[0][b][2 + e] + s2[1][b][2 + e]) * f;
                 inside &= key0 >= see_lo[b][e] && key0 + kStep - 1 <= see_hi[b][e];
@@ -427,7 +451,7 @@ k_attend(const __grid_constant__ Args a) {
             }
         }
         // O^T += V^T P^T: tile rows g and g + 8 are two neighbouring elements
-        const uint8_t* vs = stage + kStep * DP;
+        const uint8_t* values = stage + kStep * DP;
         constexpr int kWide = DP >= 128 ? 16 : 8;  // bytes a lane takes of a key at once
 #pragma unroll
         for (int h = 0; h < (DP + 127) / 128; ++h) {
@@ -435,17 +459,16 @@ k_attend(const __grid_constant__ Args a) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const int key = (i & 1 ? kb : ka) + (i & 2 ? 8 : 0);
-                const uint8_t* row = vs + key * DP;
                 if constexpr (DP >= 128) {
-                    const uint4 x = *reinterpret_cast<const uint4*>(
-                        row + v_place(key, 8 * h + g, kPieces) * 16);
+                    const uint4 x =
+                        *reinterpret_cast<const uint4*>(values + place<DP>(key, 8 * h + g));
                     w[i][0] = x.x;
                     w[i][1] = x.y;
                     w[i][2] = x.z;
                     w[i][3] = x.w;
                 } else {
                     const uint2 x = *reinterpret_cast<const uint2*>(
-                        row + v_place(key, g >> 1, kPieces) * 16 + (g & 1) * 8);
+                        values + place<DP>(key, g >> 1) + (g & 1) * 8);
                     w[i][0] = x.x;
                     w[i][1] = x.y;
                 }
@@ -469,7 +492,6 @@ k_attend(const __grid_constant__ Args a) {
             }
         }
     }
-    kv8::cp_async_wait<0>();
     __syncthreads();  // the rings are free: the warps' states meet in their place
 
     // o[h 8 + u][b][2 r + e]: element 128 h + kWide g + 2 u + r of row 8 b + 2 t + e
@@ -496,6 +518,7 @@ k_attend(const __grid_constant__ Args a) {
             }
         }
     __syncthreads();
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const bool whole = blk.used == 1;
     const int64_t unit =
         (((int64_t)seq * a.hkv + head) * a.blocks + block) * a.chunks + c;
@@ -516,9 +539,9 @@ k_attend(const __grid_constant__ Args a) {
         // O is in units of 2^(mv - lift), the sum of 2^m
         const float per = none ? 0.0f : exp2f(-kLift) / total;
         const float unit_v = none ? 0.0f : exp2f(mv - m);
-        const int64_t at = (int64_t)block * kRows + row;
+        const int at = block * kRows + row;
         const int64_t tok = blk.s.lo + at / group;
-        const int h = head * group + (int)(at % group);
+        const int h = head * group + at % group;
         T* out = static_cast<T*>(a.out) + tok * a.out_stride + (int64_t)h * a.d;
         float* part = whole ? nullptr : a.part + (unit * kRows + row) * a.d;
         for (int i = lane; i < a.d; i += 32) {
@@ -541,53 +564,74 @@ k_attend(const __grid_constant__ Args a) {
 }
 
 // Joins the chunks of a row: out = sum_c w_c out_c / sum_c w_c, w_c the chunk's
-// sum at the largest reference.  A CTA per row; its warps take every fourth
-// chunk, so that a long context's hundred chunks are a few loads deep.
+// sum at the largest reference.  A CTA per row: the weights first, then a warp
+// takes every eighth chunk, four loads in flight, a lane four elements of 128.
+constexpr int kJoinWarps = 8;
+constexpr int kMostChunks = 1024;
 template <typename T>
-__global__ void __launch_bounds__(kThreads) k_join(const __grid_constant__ Args a) {
-    __shared__ float part[kWarps][kv8::kMaxDim];
-    __shared__ float total_s[kWarps];
+__global__ void __launch_bounds__(32 * kJoinWarps) k_join(const __grid_constant__ Args a) {
+    __shared__ float w_s[kMostChunks];
+    __shared__ float4 part[kJoinWarps][kv8::kMaxDim / 4];
+    __shared__ float red[32];
     const int block = blockIdx.x / a.block_rows, row = blockIdx.x % a.block_rows;
     const int head = blockIdx.y, seq = blockIdx.z;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const Block blk = block_of(a, seq, block, false);
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     if (row >= blk.rows || blk.used == 1) return;
     const int group = a.hq / a.hkv;
     const int64_t unit = (((int64_t)seq * a.hkv + head) * a.blocks + block) * a.chunks;
     const float2* st = a.state + unit * a.block_rows + row;
+    const float4* parts = reinterpret_cast<const float4*>(a.part) + (unit * a.block_rows + row) * (a.d / 4);
+    const int64_t pitch = (int64_t)a.block_rows * (a.d / 4);
     float m = -INFINITY;
-    for (int c = lane; c < blk.used; c += 32) m = fmaxf(m, st[c * a.block_rows].x);
-    m = tbk::warp_max(m);
-    float total = 0.0f, y[kv8::kMaxDim / 32];
-#pragma unroll
-    for (int i = 0; i < kv8::kMaxDim / 32; ++i) y[i] = 0.0f;
-#pragma unroll 4
-    for (int c = warp; c < blk.used; c += kWarps) {
-        const float2 s = st[c * a.block_rows];
+    for (int c = threadIdx.x; c < blk.used; c += 32 * kJoinWarps)
+        m = fmaxf(m, st[(int64_t)c * a.block_rows].x);
+    m = tbk::block_max(m, red);
+    float mine = 0.0f;
+    for (int c = threadIdx.x; c < blk.used; c += 32 * kJoinWarps) {
+        const float2 s = st[(int64_t)c * a.block_rows];
         const float w = s.x == -INFINITY ? s.y : s.y * exp2f(s.x - m);
-        const float* p = a.part + ((unit + c) * a.block_rows + row) * a.d;
-        total += w;
-#pragma unroll
-        for (int i = 0; i < kv8::kMaxDim / 32; ++i)
-            if (lane + 32 * i < a.d) y[i] += w * p[lane + 32 * i];
+        w_s[c] = w;
+        mine += w;
     }
+    const float total = tbk::group_sum(mine, 32 * kJoinWarps, red);  // and w_s is written
 #pragma unroll
-    for (int i = 0; i < kv8::kMaxDim / 32; ++i)
-        if (lane + 32 * i < a.d) part[warp][lane + 32 * i] = y[i];
-    if (lane == 0) total_s[warp] = total;
+    for (int h = 0; h < kv8::kMaxDim / 128; ++h) {
+        const int i = 32 * h + lane;
+        float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (i < a.d / 4) {
+            for (int c0 = warp; c0 < blk.used; c0 += 4 * kJoinWarps) {
+                float4 x[4];
+                float w[4];
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    const int c = c0 + u * kJoinWarps;
+                    const bool there = c < blk.used;
+                    w[u] = there ? w_s[c] : 0.0f;
+                    x[u] = there ? __ldcg(parts + c * pitch + i) : make_float4(0.f, 0.f, 0.f, 0.f);
+                }
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    y.x = fmaf(w[u], x[u].x, y.x);
+                    y.y = fmaf(w[u], x[u].y, y.y);
+                    y.z = fmaf(w[u], x[u].z, y.z);
+                    y.w = fmaf(w[u], x[u].w, y.w);
+                }
+            }
+            part[warp][i] = y;
+        }
+    }
     __syncthreads();
-    total = 0.0f;
-#pragma unroll
-    for (int i = 0; i < kWarps; ++i) total += total_s[i];
     const bool none = total == 0.0f;
-    const int64_t at = (int64_t)block * a.block_rows + row;
+    const int at = block * a.block_rows + row;
     const int64_t tok = blk.s.lo + at / group;
-    const int h = head * group + (int)(at % group);
+    const int h = head * group + at % group;
     T* out = static_cast<T*>(a.out) + tok * a.out_stride + (int64_t)h * a.d;
-    for (int i = threadIdx.x; i < a.d; i += kThreads) {
+    for (int i = threadIdx.x; i < a.d; i += 32 * kJoinWarps) {
         float z = 0.0f;
 #pragma unroll
-        for (int k = 0; k < kWarps; ++k) z += part[k][i];
+        for (int k = 0; k < kJoinWarps; ++k) z += reinterpret_cast<const float*>(part[k])[i];
         tbk::Elt<T>::store(out + i, none ? 0.0f : z / total);
     }
     if (a.lse && threadIdx.x == 0)
@@ -604,6 +648,8 @@ int check(const TbB200Kv8* cache, const TbB200Kv8Batch* batch, const TbB200Kv8At
     if (t->n_heads < 1 || t->n_heads > 65535 || t->n_heads % cache->n_kv_heads ||
         t->window < 0 || t->max_rows < 0 || t->max_len < 0)
         return TB_ERR_INVALID_SHAPE;
+    // a sequence's (token, head of the group) rows are counted in an int
+    if (batch->rows * (t->n_heads / cache->n_kv_heads) > INT32_MAX / 2) return TB_ERR_INVALID_SHAPE;
     const int64_t width = (int64_t)t->n_heads * cache->head_dim;
     if (batch->rows > 1 && pointers && (t->q_stride < width || t->out_stride < width))
         return TB_ERR_INVALID_SHAPE;
@@ -633,8 +679,9 @@ Plan plan_of(const TbB200Kv8* cache, const TbB200Kv8Batch* batch, const TbB200Kv
     int64_t keys = t->max_len;
     if (t->window && t->window + rows < keys) keys = t->window + rows;
     const int64_t most = (keys + kLeastChunk - 1) / kLeastChunk;
-    p.chunks = all >= slots ? (8 * slots + all - 1) / all : slots / all;
+    p.chunks = 2 * all > slots ? (8 * slots + all - 1) / all : slots / all;
     if (p.chunks > most) p.chunks = most;
+    if (p.chunks > kMostChunks) p.chunks = kMostChunks;
     if (p.chunks < 1) p.chunks = 1;
     const size_t units = p.chunks > 1 ? (size_t)(all * p.chunks) : 0;
     p.part_bytes = units * p.block_rows * cache->head_dim * sizeof(float);
@@ -643,26 +690,48 @@ Plan plan_of(const TbB200Kv8* cache, const TbB200Kv8Batch* batch, const TbB200Kv
 }
 
 template <typename T, int FORMAT, int DP, int NB>
-int launch(const Args& a, dim3 grid, cudaStream_t s) {
+int launch(Args& a, const TbB200Kv8* cache, dim3 grid, cudaStream_t s) {
     constexpr int bytes = Shape<T, DP, NB>::kBytes;
-    TB_CUDA_TRY(cudaFuncSetAttribute(k_attend<T, FORMAT, DP, NB>,
-                                     cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+    static std::atomic<uint64_t> granted{0};  // a bit per device
+    int rc = kv8::once_per_device(granted, [&] {
+        return cudaFuncSetAttribute(k_attend<T, FORMAT, DP, NB>,
+                                    cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    });
+    if (rc == TB_OK) rc = kv8::tile_map(&a.k_map, cache, cache->k, DP < 128 ? DP : 128, kStep);
+    if (rc == TB_OK) rc = kv8::tile_map(&a.v_map, cache, cache->v, DP < 128 ? DP : 128, kStep);
+    if (rc != TB_OK) return rc;
     k_attend<T, FORMAT, DP, NB><<<grid, kThreads, bytes, s>>>(a);
     TB_LAUNCH_CHECK("8-bit cache attention kernel");
     return TB_OK;
 }
 
 template <typename T, int FORMAT, int NB>
-int launch_dim(const Args& a, dim3 grid, cudaStream_t s) {
-    if (a.d <= 64) return launch<T, FORMAT, 64, NB>(a, grid, s);
-    if (a.d <= 128) return launch<T, FORMAT, 128, NB>(a, grid, s);
-    return launch<T, FORMAT, 256, NB>(a, grid, s);
+int launch_dim(Args& a, const TbB200Kv8* cache, dim3 grid, cudaStream_t s) {
+    if (a.d <= 64) return launch<T, FORMAT, 64, NB>(a, cache, grid, s);
+    if (a.d <= 128) return launch<T, FORMAT, 128, NB>(a, cache, grid, s);
+    return launch<T, FORMAT, 256, NB>(a, cache, grid, s);
 }
 
 template <typename T, int FORMAT>
-int launch_rows(const Args& a, dim3 grid, cudaStream_t s) {
-    return a.block_rows == 8 ? launch_dim<T, FORMAT, 1>(a, grid, s)
-                             : launch_dim<T, FORMAT, 2>(a, grid, s);
+int launch_rows(Args& a, const TbB200Kv8* cache, dim3 grid, cudaStream_t s) {
+    return a.block_rows == 8 ? launch_dim<T, FORMAT, 1>(a, cache, grid, s)
+                             : launch_dim<T, FORMAT, 2>(a, cache, grid, s);
+}
+
+template <typename T>
+int join(const Args& a, dim3 grid, cudaStream_t s) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(32 * kJoinWarps);
+    cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    TB_CUDA_TRY(cudaLaunchKernelEx(&cfg, k_join<T>, a));
+    TB_LAUNCH_CHECK("8-bit cache attention join kernel");
+    return TB_OK;
 }
 
 }  // namespace
@@ -706,8 +775,6 @@ extern "C" int tb_b200_kv8_attention(const TbB200Kv8* cache, const TbB200Kv8Batc
     a.lse = t->lse;
     a.q_stride = t->q_stride;
     a.out_stride = t->out_stride;
-    a.k = static_cast<const uint8_t*>(cache->k);
-    a.v = static_cast<const uint8_t*>(cache->v);
     a.k_scale = cache->k_scale;
     a.v_scale = cache->v_scale;
     a.status = ds->status;
@@ -727,16 +794,11 @@ extern "C" int tb_b200_kv8_attention(const TbB200Kv8* cache, const TbB200Kv8Batc
     const dim3 grid((unsigned)(p.blocks * p.chunks), (unsigned)a.hkv, (unsigned)batch->n_seqs);
     cudaStream_t st = tbh::stream_of(stream);
     const bool f32 = t->dtype == TB_DTYPE_F32, int8 = cache->format == kv8::kInt8;
-    rc = f32 ? (int8 ? launch_rows<float, kv8::kInt8>(a, grid, st)
-                     : launch_rows<float, kv8::kE4m3>(a, grid, st))
-             : (int8 ? launch_rows<__nv_bfloat16, kv8::kInt8>(a, grid, st)
-                     : launch_rows<__nv_bfloat16, kv8::kE4m3>(a, grid, st));
+    rc = f32 ? (int8 ? launch_rows<float, kv8::kInt8>(a, cache, grid, st)
+                     : launch_rows<float, kv8::kE4m3>(a, cache, grid, st))
+             : (int8 ? launch_rows<__nv_bfloat16, kv8::kInt8>(a, cache, grid, st)
+                     : launch_rows<__nv_bfloat16, kv8::kE4m3>(a, cache, grid, st));
     if (rc != TB_OK || p.chunks == 1) return rc;
     const dim3 joins((unsigned)(p.blocks * p.block_rows), (unsigned)a.hkv, (unsigned)batch->n_seqs);
-    if (f32)
-        k_join<float><<<joins, kThreads, 0, st>>>(a);
-    else
-        k_join<__nv_bfloat16><<<joins, kThreads, 0, st>>>(a);
-    TB_LAUNCH_CHECK("8-bit cache attention join kernel");
-    return TB_OK;
+    return f32 ? join<float>(a, joins, st) : join<__nv_bfloat16>(a, joins, st);
 }

@@ -45,7 +45,8 @@ inline int check_cache(const TbB200Kv8* c, bool pointers) {
     if (c->page != 16 && c->page != 32 && c->page != 64 && c->page != 128)
         return TB_ERR_INVALID_SHAPE;
     if (c->n_kv_heads < 1 || c->n_kv_heads > 65535 || c->head_dim < 16 ||
-        c->head_dim > kMaxDim || c->head_dim % 16 || c->n_pages < 0 || c->n_pages > INT32_MAX)
+        c->head_dim > kMaxDim || c->head_dim % 16 || c->n_pages < 0 ||
+        c->n_pages > INT32_MAX / c->n_kv_heads)
         return TB_ERR_INVALID_SHAPE;
     if (pointers && c->n_pages &&
         (!c->k || !c->v || !c->k_scale || !c->v_scale || !tbh::aligned16(c->k) ||

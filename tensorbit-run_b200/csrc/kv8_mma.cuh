@@ -3,7 +3,11 @@
 // Every code is an f16 value exactly, subnormal e4m3 codes among them.
 #pragma once
 
+#include <atomic>
+
 #include "kv8.cuh"
+#include "tma.cuh"
+#include "tensor_map.h"
 
 namespace kv8 {
 
@@ -90,16 +94,14 @@ __device__ __forceinline__ float exp2_fast(float x) {
     return y;
 }
 
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
-}
-__device__ __forceinline__ void cp_async4(uint32_t dst, const void* src) {
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
-}
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_async_wait() {
-    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+// One tile of a 3-D tensor map into shared memory, its bytes counted on bar.
+__device__ __forceinline__ void tma_load3(void* dst, const CUtensorMap* map, int x, int y, int z,
+                                          uint64_t* bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cta.global.tile.mbarrier::complete_tx::bytes "
+        "[%0], [%1, {%2, %3, %4}], [%5];" ::"r"(tbk::smem_addr(dst)),
+        "l"(map), "r"(x), "r"(y), "r"(z), "r"(tbk::smem_addr(bar))
+        : "memory");
 }
 
 // 16 consecutive elements as f32, the first `n` of them (a multiple of 16: all or none).
@@ -121,6 +123,29 @@ __device__ __forceinline__ void load16(const T* p, bool live, bool vec, float (&
 #pragma unroll
         for (int i = 0; i < 16; ++i) v[i] = tbk::Elt<T>::load(p + i);
     }
+}
+
+// Run `set` (a CUDA call for the current device) unless it has been: `done` has
+// a bit per device.
+template <typename F>
+int once_per_device(std::atomic<uint64_t>& done, F set) {
+    const tbh::DeviceState* ds = tbh::current_device_state();
+    if (!ds) return TB_ERR_DEVICE;
+    const uint64_t bit = 1ull << ds->device;
+    if (done.load() & bit) return TB_OK;
+    TB_CUDA_TRY(set());
+    done.fetch_or(bit);
+    return TB_OK;
+}
+
+// The cache's codes as tiles of `keys` keys of one page by `width` bytes (64 or
+// 128, with the swizzle of that width; past head_dim zeros are loaded).
+inline int tile_map(CUtensorMap* map, const TbB200Kv8* c, const void* codes, int width, int keys) {
+    const uint64_t dims[3] = {(uint64_t)c->head_dim, (uint64_t)c->page,
+                              (uint64_t)(c->n_pages > 0 ? c->n_pages : 1) * c->n_kv_heads};
+    const uint64_t strides[2] = {(uint64_t)c->head_dim, (uint64_t)c->head_dim * c->page};
+    const uint32_t box[3] = {(uint32_t)width, (uint32_t)keys, 1};
+    return tbh::encode_tiles_u8(map, codes, dims, strides, box, width);
 }
 
 }  // namespace kv8
