@@ -3,46 +3,60 @@
 //   s_j = scale q.k_j,  out = sum_j p_j v_j,  p = softmax(s),  k_j = code * page scale
 //
 // A block holds 8 or 16 rows of one sequence and k/v head: (query token, head
-// of the group) pairs, token-major.  Its keys are split into chunks over CTAs
-// when there are few blocks; a second kernel joins the chunks.
+// of the group) pairs, token-major.  The blocks' keys, in tiles of 64 and in
+// one order, are cut into equal shares, one for each CTA that fits on the
+// device: lengths are on the device and often uneven, and equal shares of them
+// leave no CTA waiting for a long sequence and write few partial results (at
+// most two a CTA, whatever the batch).  A CTA walks through its share block by
+// block; a second kernel joins the blocks that a cut went through.
 //
-// Within a CTA each of 4 warps takes every fourth step of 16 keys, which lie in
-// one page, through a ring of TMA stages of its own: one lane issues two copies
-// a step, and no barrier of the CTA is in the loop.  The codes go from shared
-// memory to registers with 16-byte loads and
-// are converted there, as the left operands of m16n8k16 instructions, so that 8
-// rows fill the other side:
-//   S^T = K Q^T: lane (g, t) (g = lane / 4, t = lane % 4) holds keys order(g)
-//     and order(g) + 8, 16 consecutive elements of each; the head dimension is
-//     summed in the order in which that puts it, Q's registers the same;
-//   O^T = V^T P^T: S^T's registers, transposed 8 x 8, are P^T's operands; lane
-//     (g, t) holds elements 16 g .. 16 g + 15 (of 128) of keys order(2t),
-//     order(2t + 1) and those + 8.
+// Within a CTA each of 4 warps takes every fourth step of 32 keys (16 for heads
+// over 128) through a ring of TMA stages of its own: one lane issues the copies,
+// and no barrier of the CTA is in the loop.
+//   S^T = K Q^T, m16n8k32 on the codes as they are: lane (g, t) (g = lane / 4,
+//     t = lane % 4) holds keys order(g) and order(g) + 8, 16 consecutive elements
+//     of each with a 16-byte load; the head dimension is summed in the order in
+//     which that puts it, Q's registers the same.  Q is split into two to six
+//     parts of the format (QParts): matrix instructions on 8-bit operands cost a
+//     half (int8) or an eighth (e4m3) of an f16 one per product, conversions of
+//     the codes more than all of them;
+//   O^T = V^T P^T, m16n8k16 on f16: S^T's registers, transposed 8 x 8, are P^T's
+//     operands; lane (g, t) holds elements 16 g .. 16 g + 15 (of 128) of keys
+//     order(2t), order(2t + 1) and those + 8, and pairs and converts them.
 // order() and TMA's swizzle (the 16-byte piece c of key r lies at c ^ (r & 7))
 // put the 8 lanes of each 16-byte access into different banks.
 //
-// Precision.  A code is an f16 exactly.  A row of q is scaled by a power of two
-// to [2^14, 2^15) and held as f16: bf16 elements exactly unless 2^-21 below the
-// row's largest, where what is lost is 2^-39 of the largest; f32 rows as two f16 (hi + lo), 22 bits.
-// Weights p are f16 relative to a power of two near the row's largest (half a
-// step 2^-12, an eighth of the bf16 output's), for f32 rows hi + lo again.
-// Sums, maxima and the sum of p are f32.  The values' scale joins the exponent,
-// p v_scale = 2^(s + log2 v_scale - r'), with a reference r' of its own per
-// row, so pages of any scales keep their weight.  References are whole numbers
-// and move only when a score passes them by 2^4: rescaling is exact and rare.
-// A weight more than 2^-25 below the row's largest is an f16 subnormal, off by
-// at most 2^-36 of the largest.
+// Precision.  A row of q is held to 2^-22 of its largest element or better,
+// products and their sums are exact (int8) or f32.  Weights p are f16 relative
+// to a power of two near the row's largest (half a step 2^-12, an eighth of the
+// bf16 output's), for f32 rows two f16 (hi + lo).  Sums, maxima and the sum of p
+// are f32.  The values' scale joins the exponent, p v_scale = 2^(s + log2 v_scale
+// - r'), with a reference r' of its own per row, so pages of any scales keep
+// their weight.  References are whole numbers and move only when a score passes
+// them by 2^4: rescaling is exact and rare.  A weight more than 2^-25 below the
+// row's largest is an f16 subnormal, off by at most 2^-36 of the largest.
 #include "kv8_mma.cuh"
 
 namespace {
 
 constexpr int kWarps = 4;
 constexpr int kThreads = 32 * kWarps;
-constexpr int kStep = 16;          // keys a warp takes at once
-constexpr int kLeastChunk = 256;   // keys below which a chunk is not split further
+constexpr int kTileKeys = 128;     // keys that shares are counted in
+constexpr int kLeastTiles = 2;     // tiles below which a share is not cut further
+constexpr int kHeadTiles = 1;      // what a block costs besides its keys, in tiles
+constexpr int kMostCtas = 1024;
 constexpr float kSlack = 4.0f;     // how far (log2) scores may pass a reference
 constexpr float kLift = 11.0f;     // weights are held times 2^11: up to 2^15 in f16
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kNoRef = -3.0e38f;  // the reference of a row that has seen no key
+
+// A cut through a block: what the joining kernel needs.
+struct Cut {
+    int64_t begin, end;  // the block's span, counted over the batch
+    int64_t tiles;       // of the batch
+    int ctas;            // that have a share
+    int seq, head, block;  // seq < 0: the share begins with a block
+};
 
 struct Args {
     CUtensorMap k_map, v_map;  // [n_pages * n_kv_heads][page][d] codes
@@ -53,99 +67,137 @@ struct Args {
     int64_t q_stride, out_stride;
     const float *k_scale, *v_scale;
     unsigned* status;
-    float* part;    // [seq, kv head, block, chunk][block_rows][d] partial outputs
-    float2* state;  // the same, a row's (reference, sum)
+    Cut* cuts;      // [CTA] the block that its share begins inside
+    float* part;    // [CTA][2][block_rows][d] its first and last block's partial outputs
+    float2* state;  // [CTA][2][block_rows] a row's (reference, sum)
     float scale;
-    int hq, hkv, d, window, max_rows, max_len, chunks, blocks, block_rows, vec;
+    int hq, hkv, d, window, max_rows, max_len, block_rows, whole, spread, vec;
 };
 
-// What a block of rows attends, the same in both kernels.
-struct Block {
+// A sequence's blocks and the tiles that its longest one may have.
+struct Load {
     kv8::Seq s;
-    int rows;       // live rows of the block
-    int lo, end;    // keys [lo, end) that some row sees
-    int from, size; // chunk c: keys [from + c size, from + (c + 1) size)
-    int used;       // chunks that are not empty (1 if no key at all)
+    bool ok;  // within the call's bounds
+    int blocks, tiles;
+    // A block spans kHeadTiles, which stand for its fixed cost and are not cut,
+    // and its tiles.
+    __device__ int span() const { return kHeadTiles + tiles; }
+    __device__ int64_t total(const Args& a) const { return (int64_t)blocks * a.hkv * span(); }
 };
 
-__device__ __forceinline__ Block block_of(const Args& a, int seq, int block, bool flag) {
-    Block k;
-    k.s = kv8::sequence(a.b, seq);
+__device__ __forceinline__ Load load_of(const Args& a, int seq) {
+    Load l;
+    l.s = kv8::sequence(a.b, seq);
     const int group = a.hq / a.hkv;
-    const int at = block * a.block_rows;  // rows * group fits an int
-    k.rows = max(0, min(a.block_rows, k.s.n * group - at));
-    k.lo = k.end = 0;
-    if (k.rows > 0) {
-        if (k.s.len > a.max_len || k.s.n > a.max_rows ||
-            k.s.len > ((int64_t)a.b.width << a.b.page_shift)) {
-            if (flag) atomicOr(a.status, TB_B200_FLAG_POSITION_RANGE);
-        } else {
-            const int p0 = k.s.first + at / group;
-            const int p1 = k.s.first + (at + k.rows - 1) / group;
-            k.end = max(p1 + 1, 0);
-            k.lo = a.window ? min(max(p0 - a.window + 1, 0), k.end) : 0;
-        }
+    l.ok = l.s.len <= a.max_len && l.s.n <= a.max_rows &&
+           l.s.len <= ((int64_t)a.b.width << a.b.page_shift);
+    l.blocks = (l.s.n * group + a.block_rows - 1) / a.block_rows;  // rows * group fits an int
+    int64_t keys = l.ok ? l.s.len : 0;
+    // a block's tokens span (block_rows - 1) / group + 1 positions at most, and its
+    // first step begins up to 31 keys early
+    if (a.window) keys = min(keys, (int64_t)a.window + (a.block_rows - 1) / group + 32);
+    l.tiles = a.whole ? 1 : max(1, (int)((keys + kTileKeys - 1) / kTileKeys));
+    return l;
+}
+
+// What a block of rows attends.
+struct Block {
+    int rows;       // live rows of the block
+    int from, end;  // keys [from, end), from a whole step
+};
+
+__device__ __forceinline__ Block block_of(const Args& a, const Load& l, int block) {
+    Block k;
+    const int group = a.hq / a.hkv, at = block * a.block_rows;
+    k.rows = min(a.block_rows, l.s.n * group - at);
+    k.from = k.end = 0;
+    if (l.ok) {
+        const int p0 = l.s.first + at / group, p1 = l.s.first + (at + k.rows - 1) / group;
+        k.end = max(p1 + 1, 0);
+        k.from = a.window ? min(max(p0 - a.window + 1, 0), k.end) & ~31 : 0;
     }
-    k.from = k.lo & ~(kStep - 1);
-    const int keys = k.end - k.from;
-    const int each = (keys + a.chunks - 1) / a.chunks;
-    k.size = max(kLeastChunk, (each + kWarps * kStep - 1) / (kWarps * kStep) * (kWarps * kStep));
-    k.used = max(1, (keys + k.size - 1) / k.size);
     return k;
 }
 
 // The key (of 8) that row g of an operand stands for.
 __device__ __forceinline__ int order(int n) { return n ^ ((n & 1) << 2); }
-// Where the 16-byte piece c of a stage's key lies: DP = 64 has rows of 64 bytes
-// and that swizzle, DP = 256 two tiles of 128-byte rows.
-template <int DP>
+// Where the 16-byte piece c of a key lies in a tile of KEYS keys: DP = 64 has
+// rows of 64 bytes and that swizzle, DP = 256 two tiles of 128-byte rows.
+template <int DP, int KEYS>
 __device__ __forceinline__ int place(int key, int c) {
     if constexpr (DP == 64) return key * 64 + (c ^ (key >> 1 & 3)) * 16;
-    return (c >> 3) * kStep * 128 + key * 128 + ((c ^ key) & 7) * 16;
+    return (c >> 3) * KEYS * 128 + key * 128 + ((c ^ key) & 7) * 16;
+}
+
+// CTAs per SM: what registers (O: DP NB / 4 a lane) and shared memory allow.
+constexpr int ctas_of(int dp, int nb, bool f32) {
+    return dp * nb >= (f32 ? 128 : 256) ? 2 : dp * nb >= (f32 ? 64 : 128) ? 3 : 4;
+}
+inline int ctas_per_sm(int d, int block_rows, bool f32) {
+    return ctas_of(d <= 64 ? 64 : d <= 128 ? 128 : 256, block_rows / 8, f32);
 }
 
 // Shapes of a kernel for heads of up to DP elements and blocks of 8 NB rows.
-template <typename T, int DP, int NB>
+template <typename T, int FORMAT, int DP, int NB>
 struct Shape {
-    static constexpr bool kSplit = sizeof(T) == 4;  // hi + lo operands
-    static constexpr int kStages = DP == 64 ? 5 : 3;
-    static constexpr int kStageBytes = 2 * kStep * DP;
-    static constexpr int kSteps = DP / 16;                // 16-wide steps of the head dimension
+    static constexpr bool kSplit = sizeof(T) == 4;  // hi + lo weights
+    static constexpr int kKeys = DP == 256 ? 16 : 32;  // a warp's step
+    static constexpr int kHalves = kKeys / 16;
+    static constexpr int kStages = DP == 128 ? 2 : 3;
+    static constexpr int kStageBytes = 2 * kKeys * DP;
+    static constexpr int kWords = DP / 16;  // words of four elements a lane has of a row of q
     static constexpr int kRows = 8 * NB;
     // Q's operands stay in registers when they are few
-    static constexpr bool kQReg = kSteps * 2 * NB * (kSplit ? 2 : 1) <= 32;
-    static constexpr int kQBytes = kQReg ? 0 : kSteps * NB * 256 * (kSplit ? 2 : 1);
+    static constexpr int kParts = kv8::QParts<T, FORMAT>::kParts;
+    static constexpr bool kQReg = kParts * kWords * NB <= 32;
+    static constexpr int kQBytes = kQReg ? 0 : kParts * kWords * NB * 128;
     static constexpr int kRing = kWarps * kStages * kStageBytes;  // a multiple of 1024
     static constexpr int kPitch = DP + 4;
     static constexpr int kJoin = kWarps * kRows * (kPitch + 3) * 4;
-    static constexpr int kBytes = (kRing > kJoin ? kRing : kJoin) + kQBytes + 1024;  // 1024: to align
-    // CTAs per SM: what registers (O: DP NB / 4 a lane) and shared memory allow
-    static constexpr int kCtas = DP * NB >= 512 ? 2 : DP * NB >= 256 ? (DP == 256 ? 2 : 3) : 4;
+    static constexpr int kBytes =
+        (kRing > kJoin ? kRing : kJoin) + kQBytes + 1024;  // 1024: to align
+    static constexpr int kCtas = ctas_of(DP, NB, kSplit);
 };
 
+// (sum up to this thread, sum over the block) of v.
+__device__ __forceinline__ longlong2 block_scan(int64_t v, int64_t* warps) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int64_t u = __shfl_up_sync(tbk::kFull, v, o);
+        if (lane >= o) v += u;
+    }
+    __syncthreads();
+    if (lane == 31) warps[warp] = v;
+    __syncthreads();
+    int64_t all = 0, before = 0;
+#pragma unroll
+    for (int i = 0; i < kWarps; ++i) {
+        if (i < warp) before += warps[i];
+        all += warps[i];
+    }
+    return make_longlong2(before + v, all);
+}
+
 template <typename T, int FORMAT, int DP, int NB>
-__global__ void __launch_bounds__(kThreads, Shape<T, DP, NB>::kCtas)
+__global__ void __launch_bounds__(kThreads, Shape<T, FORMAT, DP, NB>::kCtas)
 k_attend(const __grid_constant__ Args a) {
-    using H = Shape<T, DP, NB>;
+    using H = Shape<T, FORMAT, DP, NB>;
+    using Q = kv8::QParts<T, FORMAT>;
     constexpr bool kSplit = H::kSplit, kQReg = H::kQReg;
-    constexpr int kSteps = H::kSteps, kStages = H::kStages, kRows = H::kRows;
-    constexpr int kTiles = DP / 16;  // 16-wide output tiles
+    constexpr int kStages = H::kStages, kRows = H::kRows, kKeys = H::kKeys;
+    constexpr int kHalves = H::kHalves, kParts = H::kParts, kWords = H::kWords;
+    constexpr int kStride = kWarps * kKeys;  // from one of a warp's steps to its next
+    constexpr int kTiles = DP / 16;          // 16-wide output tiles
     extern __shared__ uint8_t smem_raw[];
     __shared__ uint64_t bars[kWarps * kStages];
+    __shared__ int64_t scan[kWarps], found_begin;
+    __shared__ int found_seq;
     // TMA's swizzle goes by the address: tiles start on 1024 bytes
     uint8_t* smem = smem_raw + (-tbk::smem_addr(smem_raw) & 1023u);
 
-    const int c = blockIdx.x % a.chunks, block = blockIdx.x / a.chunks;
-    const int head = blockIdx.y, seq = blockIdx.z;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const Block blk = block_of(a, seq, block, threadIdx.x == 0 && c == 0 && head == 0);
-    if (blk.rows == 0 || c >= blk.used) return;
     const int group = a.hq / a.hkv;
-    const int begin = blk.from + c * blk.size, end = min(begin + blk.size, blk.end);
-
-    // the warp's steps: keys first + 64 n .. + 15
-    const int first = begin + warp * kStep;
-    const int n_steps = end > first ? (end - first + kWarps * kStep - 1) / (kWarps * kStep) : 0;
     uint8_t* ring = smem + warp * kStages * H::kStageBytes;
     uint64_t* bar = bars + warp * kStages;
     if (lane == 0) {
@@ -153,463 +205,592 @@ k_attend(const __grid_constant__ Args a) {
         for (int i = 0; i < kStages; ++i) tbk::mbar_init(bar + i, 1);
         tbk::fence_mbar_init();
     }
-    __syncwarp();
-    const int32_t* table = a.b.table + seq * a.b.table_stride;
-    auto page_of = [&](int n) {  // the page of step n, -1 if it has none
-        if (n >= n_steps) return -1;
-        const int id = table[(first + n * (kWarps * kStep)) >> a.b.page_shift];
-        if (id >= 0 && id < a.b.n_pages) return id;
-        atomicOr(a.status, TB_B200_FLAG_PAGE_RANGE);
-        return -1;
-    };
-    // Lane i has the page of step 32 m + i and its scales, m the batch that is
-    // being issued; the next batch's pages are on their way.
-    int ids = page_of(lane), ids_next = page_of(32 + lane);
-    float ks_issued = 0.0f, vs_issued = 0.0f, ks = 0.0f, vs = 0.0f;
-    uint32_t pages_issued, pages = 0;  // which steps of the batch have a page
-    auto load_scales = [&] {
-        pages_issued = __ballot_sync(tbk::kFull, ids >= 0);
-        if (ids >= 0) {
-            const int unit = ids * a.hkv + head;
-            ks_issued = a.k_scale[unit];
-            vs_issued = a.v_scale[unit];
-        }
-    };
-    load_scales();
-    auto issue = [&](int n, int stage) {
-        if ((n & 31) == 0 && n > 0) {
-            ids = ids_next;
-            load_scales();
-            ids_next = page_of(n + 32 + lane);
-        }
-        const int id = __shfl_sync(tbk::kFull, ids, n & 31);
-        if (lane == 0 && id >= 0) {
-            uint8_t* dst = ring + stage * H::kStageBytes;
-            const int slot = (first + n * (kWarps * kStep)) & ((1 << a.b.page_shift) - 1);
-            tbk::mbar_expect_tx(bar + stage, H::kStageBytes);
-#pragma unroll
-            for (int h = 0; h < (DP + 127) / 128; ++h) {
-                kv8::tma_load3(dst + h * kStep * 128, &a.k_map, h * 128, slot, id * a.hkv + head,
-                               bar + stage);
-                kv8::tma_load3(dst + kStep * DP + h * kStep * 128, &a.v_map, h * 128, slot,
-                               id * a.hkv + head, bar + stage);
-            }
-        }
-    };
-#pragma unroll
-    for (int n = 0; n < kStages - 1; ++n) issue(n, n);
+    uint32_t phases = 0;  // of each stage's barrier: a page out of range has no copy
 
-    // Q's operands: rows g, g + 8, .. of the block; a row's scores are
-    // multiplied with qf, but for the page's scale
-    uint32_t qr[kQReg ? kSteps : 1][NB][2], ql[kQReg && kSplit ? kSteps : 1][NB][2];
-    uint2* qs = reinterpret_cast<uint2*>(smem + H::kBytes - 1024 - H::kQBytes);
-    float qf[NB];
-#pragma unroll
-    for (int b = 0; b < NB; ++b) {
-        const int i = 8 * b + g;
-        const bool live = i < blk.rows;
-        const int at = block * kRows + i, tok = live ? at / group : 0;
-        const int hh = live ? at - tok * group : 0;
-        const T* q = static_cast<const T*>(a.q) + (blk.s.lo + tok) * a.q_stride +
-                     (int64_t)(head * group + hh) * a.d;
-        float top = 0.0f;
-#pragma unroll
-        for (int h = 0; h < DP / 64; ++h) {
-            float x[16];
-            kv8::load16(q + 64 * h + 16 * t, live && 64 * h + 16 * t < a.d, a.vec, x);
-#pragma unroll
-            for (int e = 0; e < 16; ++e) top = fmaxf(top, fabsf(x[e]));
-        }
-        top = fmaxf(top, __shfl_xor_sync(tbk::kFull, top, 1));
-        top = fmaxf(top, __shfl_xor_sync(tbk::kFull, top, 2));
-        // 2^e with |q| 2^e in [2^14, 2^15); NaN and infinite rows stay that
-        const int e = min(max((int)(__float_as_uint(top) >> 23), 1 + 16), 254);
-        const float lift = __uint_as_float((uint32_t)(127 + 14 - e + 127) << 23);
-        qf[b] = __uint_as_float((uint32_t)(e - 14) << 23) * (a.scale * kLog2e);
-#pragma unroll
-        for (int h = 0; h < DP / 64; ++h) {
-            float x[16];
-            kv8::load16(q + 64 * h + 16 * t, live && 64 * h + 16 * t < a.d, a.vec, x);
-#pragma unroll
-            for (int e16 = 0; e16 < 16; ++e16) x[e16] *= lift;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {  // a word of 4 codes
-                uint32_t hi[2], lo[2];
-#pragma unroll
-                for (int r = 0; r < 2; ++r) {
-                    const float u = x[4 * j + kv8::word_element<FORMAT>(r, 0)];
-                    const float w = x[4 * j + kv8::word_element<FORMAT>(r, 1)];
-                    hi[r] = kv8::pack_f16x2(u, w);
-                    const __half2 h2 = *reinterpret_cast<const __half2*>(&hi[r]);
-                    lo[r] = kv8::pack_f16x2(u - __low2float(h2), w - __high2float(h2));
-                }
-                const int s = 4 * h + j;
-                if constexpr (kQReg) {
-#pragma unroll
-                    for (int r = 0; r < 2; ++r) {
-                        qr[s][b][r] = hi[r];
-                        if (kSplit) ql[s][b][r] = lo[r];
-                    }
-                } else if (warp == 0) {
-                    qs[(s * NB + b) * 32 + lane] = make_uint2(hi[0], hi[1]);
-                    if (kSplit) qs[((kSteps + s) * NB + b) * 32 + lane] = make_uint2(lo[0], lo[1]);
-                }
+    // This CTA's share: [tile, stop) of the batch's spans, the first in sequence
+    // seq, whose own begin at seq_begin.
+    int64_t tile, stop, seq_begin, tiles;
+    int seq, ctas;
+    {
+        int64_t mine = 0;
+        for (int i = threadIdx.x; i < a.b.n_seqs; i += kThreads) mine += load_of(a, i).total(a);
+        tiles = block_scan(mine, scan).y;
+        const int64_t want = a.whole ? tiles / (kHeadTiles + 1)
+                                     : (tiles + kLeastTiles - 1) / kLeastTiles;
+        ctas = (int)min((int64_t)gridDim.x, want);
+        if (threadIdx.x == 0 && a.cuts) a.cuts[blockIdx.x].seq = -1;
+        if ((int)blockIdx.x >= ctas) return;
+        tile = blockIdx.x * tiles / ctas;
+        stop = (blockIdx.x + 1) * tiles / ctas;
+        seq_begin = 0;
+        for (int i0 = 0;; i0 += kThreads) {  // ends: the sum over all is above tile
+            const int i = i0 + threadIdx.x;
+            const int64_t w = i < a.b.n_seqs ? load_of(a, i).total(a) : 0;
+            const longlong2 sum = block_scan(w, scan);  // (up to this thread, all)
+            if (tile >= seq_begin + sum.x - w && tile < seq_begin + sum.x) {
+                found_seq = i;
+                found_begin = seq_begin + sum.x - w;
             }
+            __syncthreads();
+            if (tile < seq_begin + sum.y) break;
+            seq_begin += sum.y;
         }
+        seq = found_seq;
+        seq_begin = found_begin;
     }
-    // S^T's columns: rows 8 b + 2 t + e, keys [see_lo, see_hi] each
-    float qc[NB][2];
-    int see_lo[NB][2], see_hi[NB][2];
-#pragma unroll
-    for (int b = 0; b < NB; ++b)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-            qc[b][e] = __shfl_sync(tbk::kFull, qf[b], (2 * t + e) * 4);
-            const int i = 8 * b + 2 * t + e;
-            // rows of the block that are not there see all and are not stored
-            const bool live = i < blk.rows;
-            const int p = blk.s.first + (block * kRows + i) / group;
-            see_hi[b][e] = live ? p : INT32_MAX;
-            see_lo[b][e] = a.window && live ? max(p - a.window + 1, 0) : 0;
+    Load load = load_of(a, seq);
+
+    for (bool first_block = true; tile < stop; first_block = false) {
+        while (tile >= seq_begin + load.total(a)) {
+            seq_begin += load.total(a);
+            load = load_of(a, ++seq);
         }
+        const int in_seq = (int)((tile - seq_begin) / load.span());
+        const int head = in_seq / load.blocks, block = in_seq - head * load.blocks;
+        const int64_t unit_begin = seq_begin + (int64_t)in_seq * load.span();
+        // a share that ends within a block's head leaves it all to the next CTA
+        if (stop - unit_begin <= kHeadTiles) break;
+        const int skip = max(0, (int)(tile - unit_begin) - kHeadTiles);
+        const int till = (int)min((int64_t)load.tiles, stop - unit_begin - kHeadTiles);
+        tile = unit_begin + kHeadTiles + till;
+        const bool whole = skip == 0 && till == load.tiles;
+        const Block blk = block_of(a, load, block);
+        if (threadIdx.x == 0) {
+            if (first_block && skip > 0)
+                a.cuts[blockIdx.x] = {unit_begin, unit_begin + load.span(), tiles, ctas, seq, head,
+                                      block};
+            if (!load.ok) atomicOr(a.status, TB_B200_FLAG_POSITION_RANGE);
+        }
+        const int begin = blk.from + skip * kTileKeys;
+        const int end = a.whole ? blk.end
+                                : (int)min(blk.from + (int64_t)till * kTileKeys, (int64_t)blk.end);
 
-    if constexpr (!kQReg) __syncthreads();
-
-    float o[kTiles][NB][4];
+        // the warp's steps: keys first + kStride n .. + kKeys - 1
+        const int first = begin + warp * kKeys;
+        const int n_steps = end > first ? (end - first + kStride - 1) / kStride : 0;
+        const int32_t* table = a.b.table + seq * a.b.table_stride;
+        // A step's 16-key halves are in one page, or, with pages of 16, in two.
+        const bool one_page = a.b.page_shift >= 5;
+        auto page_of = [&](int i) {  // the page of half-step i, -1 if it has none
+            const int key =
+                first + i / kHalves * kStride + (kHalves == 2 && !one_page ? i % 2 * 16 : 0);
+            if (i / kHalves >= n_steps || key >= end) return -1;
+            const int id = table[key >> a.b.page_shift];
+            if (id >= 0 && id < a.b.n_pages) return id;
+            atomicOr(a.status, TB_B200_FLAG_PAGE_RANGE);
+            return -1;
+        };
+        // Lane i has the page of half-step 32 m + i and its scales, m the batch
+        // that is being issued; the next batch's pages are on their way.
+        constexpr int kBatch = 32 / kHalves;  // steps
+        int ids = page_of(lane), ids_next = page_of(32 + lane);
+        float ks_issued = 0.0f, vs_issued = 0.0f, ks = 0.0f, vs = 0.0f;
+        uint32_t pages_issued, pages = 0;  // which half-steps of the batch have a page
+        auto load_scales = [&] {
+            pages_issued = __ballot_sync(tbk::kFull, ids >= 0);
+            if (ids >= 0) {
+                const int unit = ids * a.hkv + head;
+                ks_issued = a.k_scale[unit];
+                vs_issued = a.v_scale[unit];
+            }
+        };
+        load_scales();
+        auto issue = [&](int n, int stage) {
+            const int i = n % kBatch * kHalves;
+            if (i == 0 && n > 0) {
+                ids = ids_next;
+                load_scales();
+                ids_next = page_of(n * kHalves + 32 + lane);
+            }
+            const int id0 = __shfl_sync(tbk::kFull, ids, i);
+            const int id1 = kHalves == 2 ? __shfl_sync(tbk::kFull, ids, i + 1) : -1;
+            if (lane == 0 && (id0 >= 0 || id1 >= 0)) {
+                uint8_t* dst = ring + stage * H::kStageBytes;
+                const int slot = (first + n * kStride) & ((1 << a.b.page_shift) - 1);
+                auto copy = [&](int id, int at, int slot) {  // a box, from the stage's key `at`
 #pragma unroll
-    for (int i = 0; i < kTiles; ++i)
+                    for (int h = 0; h < (DP + 127) / 128; ++h) {
+                        uint8_t* d = dst + h * kKeys * 128 + at * (DP < 128 ? DP : 128);
+                        kv8::tma_load3(d, &a.k_map, h * 128, slot, id * a.hkv + head, bar + stage);
+                        kv8::tma_load3(d + kKeys * DP, &a.v_map, h * 128, slot, id * a.hkv + head,
+                                       bar + stage);
+                    }
+                };
+                if (kHalves == 1 || one_page) {
+                    tbk::mbar_expect_tx(bar + stage, H::kStageBytes);
+                    copy(id0, 0, slot);
+                } else {
+                    tbk::mbar_expect_tx(bar + stage,
+                                        ((id0 >= 0) + (id1 >= 0)) * (H::kStageBytes / 2));
+                    if (id0 >= 0) copy(id0, 0, slot);
+                    if (id1 >= 0) copy(id1, 16, 0);
+                }
+            }
+        };
+#pragma unroll
+        for (int n = 0; n < kStages - 1; ++n) issue(n, n);
+
+        // Q's operands: row 8 b + g of the block, words of elements 64 h + 16 t +
+        // 4 j .. + 3; its sums of products are multiplied with qf, but for the
+        // page's scale.  A row with a NaN or an infinity is NaN.
+        uint32_t qr[kQReg ? kParts : 1][kQReg ? kWords : 1][NB];
+        uint32_t* qs = reinterpret_cast<uint32_t*>(smem + H::kBytes - 1024 - H::kQBytes);
+        float qf[NB];
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+            const int i = 8 * b + g;
+            const bool live = i < blk.rows;
+            const int at = block * kRows + i, tok = live ? at / group : 0;
+            const int hh = live ? at - tok * group : 0;
+            const T* q = static_cast<const T*>(a.q) + (load.s.lo + tok) * a.q_stride +
+                         (int64_t)(head * group + hh) * a.d;
+            float x[DP / 64][16], top = 0.0f;
+            bool finite = true;
+#pragma unroll
+            for (int h = 0; h < DP / 64; ++h) {
+                kv8::load16(q + 64 * h + 16 * t, live && 64 * h + 16 * t < a.d, a.vec, x[h]);
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    top = fmaxf(top, fabsf(x[h][e]));
+                    finite &= fabsf(x[h][e]) < INFINITY;
+                }
+            }
+            if (!finite) top = INFINITY;
+            top = fmaxf(top, __shfl_xor_sync(tbk::kFull, top, 1));
+            top = fmaxf(top, __shfl_xor_sync(tbk::kFull, top, 2));
+            const Q parts(top < INFINITY ? top : 0.0f);
+            qf[b] = top < INFINITY ? parts.unit * (a.scale * kLog2e) : NAN;
+#pragma unroll
+            for (int h = 0; h < DP / 64; ++h)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    uint32_t w[kParts];
+                    parts.split(x[h] + 4 * j, w);
+#pragma unroll
+                    for (int p = 0; p < kParts; ++p) {
+                        if constexpr (kQReg)
+                            qr[p][4 * h + j][b] = w[p];
+                        else if (warp == 0)
+                            qs[(((p * kWords + 4 * h + j) / 2 * NB + b) * 32 + lane) * 2 + j % 2] =
+                                w[p];
+                    }
+                }
+        }
+        // S^T's columns: rows 8 b + 2 t + e, keys [see_lo, see_hi] each
+        float qc[NB][2];
+        int see_lo[NB][2], see_hi[NB][2];
 #pragma unroll
         for (int b = 0; b < NB; ++b)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) o[i][b][e] = 0.0f;
-    float ref[NB][2], vref[NB][2], sum[NB][2];
-#pragma unroll
-    for (int b = 0; b < NB; ++b)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-            ref[b][e] = vref[b][e] = -INFINITY;
-            sum[b][e] = 0.0f;
-        }
-
-    const int ka = order(2 * t), kb = order(2 * t + 1), kg = order(g);
-    uint32_t phases = 0;  // of each stage's barrier: a page out of range has no copy
-    int at_stage = kStages - 1;
-    for (int n = 0; n < n_steps; ++n) {
-        if ((n & 31) == 0) {
-            ks = ks_issued;
-            vs = vs_issued;
-            pages = pages_issued;
-        }
-        __syncwarp();  // step n - 1's stage has been read: it is the next to be filled
-        issue(n + kStages - 1, at_stage);
-        at_stage = at_stage == kStages - 1 ? 0 : at_stage + 1;
-        if (!(pages >> (n & 31) & 1)) continue;
-        const float k_scale = __shfl_sync(tbk::kFull, ks, n & 31);
-        const float v_scale = __shfl_sync(tbk::kFull, vs, n & 31);
-        uint8_t* stage = ring + at_stage * H::kStageBytes;
-        const uint32_t phase = phases >> at_stage & 1;
-        phases ^= 1u << at_stage;
-        const bool came = tbk::mbar_wait(bar + at_stage, phase, a.status);
-        if (!__all_sync(tbk::kFull, came)) {
-            // the copy did not come: the output is invalid and flagged.  No copy
-            // may be in flight when the block ends: wait for the others, bounded.
-            for (int i = 1; i < kStages; ++i) {
-                const int m = n + i, x = (at_stage + i) % kStages;
-                const int id = m < n_steps ? table[(first + m * (kWarps * kStep)) >> a.b.page_shift]
-                                           : -1;
-                if (id >= 0 && id < a.b.n_pages)
-                    tbk::mbar_wait(bar + x, phases >> x & 1, a.status);
+            for (int e = 0; e < 2; ++e) {
+                qc[b][e] = __shfl_sync(tbk::kFull, qf[b], (2 * t + e) * 4);
+                const int i = 8 * b + 2 * t + e;
+                // rows of the block that are not there see all and are not stored
+                const bool live = i < blk.rows;
+                const int p = load.s.first + (block * kRows + i) / group;
+                see_hi[b][e] = live ? p : INT32_MAX;
+                see_lo[b][e] = a.window && live ? max(p - a.window + 1, 0) : 0;
             }
-            break;
-        }
-        const int key0 = first + n * (kWarps * kStep);
-        if (key0 + kStep > blk.s.len) {
-            // slots behind the last token may hold anything, NaN codes too: a
-            // weight of zero needs a finite value beside it
-            for (int i = lane; i < kStep * DP / 16; i += 32)
-                if (key0 + i % kStep >= blk.s.len)
-                    *reinterpret_cast<uint4*>(stage + kStep * DP +
-                                              place<DP>(i % kStep, i / kStep)) =
-                        make_uint4(0, 0, 0, 0);
-            __syncwarp();
-        }
+        if constexpr (!kQReg) __syncthreads();
 
-        // S^T: 16 keys by the block's rows, two sums of half the steps each
-        float s2[2][NB][4];
+        float o[kTiles][NB][4];
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
+        for (int i = 0; i < kTiles; ++i)
 #pragma unroll
             for (int b = 0; b < NB; ++b)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) s2[i][b][e] = 0.0f;
+                for (int e = 0; e < 4; ++e) o[i][b][e] = 0.0f;
+        float ref[NB][2], vref[NB][2], sum[NB][2];
 #pragma unroll
-        for (int h = 0; h < DP / 64; ++h) {
-            const uint4 x =
-                *reinterpret_cast<const uint4*>(stage + place<DP>(kg, 4 * h + t));
-            const uint4 y =
-                *reinterpret_cast<const uint4*>(stage + place<DP>(kg + 8, 4 * h + t));
-            const uint32_t wx[4] = {x.x, x.y, x.z, x.w}, wy[4] = {y.x, y.y, y.z, y.w};
+        for (int b = 0; b < NB; ++b)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                uint32_t a0, a1, a2, a3;
-                kv8::word<FORMAT>(wx[j], a0, a2);
-                kv8::word<FORMAT>(wy[j], a1, a3);
-                const int k = 4 * h + j;
+            for (int e = 0; e < 2; ++e) {
+                ref[b][e] = vref[b][e] = kNoRef;
+                sum[b][e] = 0.0f;
+            }
+
+        const int ka = order(2 * t), kb = order(2 * t + 1), kg = order(g);
+        int at_stage = kStages - 1;
+        for (int n = 0; n < n_steps; ++n) {
+            const int i0 = n % kBatch * kHalves;
+            if (i0 == 0) {
+                ks = ks_issued;
+                vs = vs_issued;
+                pages = pages_issued;
+            }
+            __syncwarp();  // step n - 1's stage has been read: it is the next to be filled
+            issue(n + kStages - 1, at_stage);
+            at_stage = at_stage == kStages - 1 ? 0 : at_stage + 1;
+            const uint32_t have = pages >> i0 & ((1 << kHalves) - 1);
+            if (have == 0) continue;
+            float k_scale[kHalves], lv[kHalves];  // the values' scale as an exponent
+#pragma unroll
+            for (int f = 0; f < kHalves; ++f) {
+                k_scale[f] = __shfl_sync(tbk::kFull, ks, i0 + f);
+                const float v_scale = __shfl_sync(tbk::kFull, vs, i0 + f);
+                lv[f] = (float)((int)(__float_as_uint(v_scale) >> 23) - 127);
+            }
+            uint8_t* stage = ring + at_stage * H::kStageBytes;
+            const uint32_t phase = phases >> at_stage & 1;
+            phases ^= 1u << at_stage;
+            const bool came = tbk::mbar_wait(bar + at_stage, phase, a.status);
+            if (!__all_sync(tbk::kFull, came)) {
+                // the copy did not come: the output is invalid and flagged.  No copy
+                // may be in flight when the block ends: wait for the others, bounded.
+                for (int i = 1; i < kStages; ++i) {
+                    const int x = (at_stage + i) % kStages;
+                    if (page_of((n + i) * kHalves) >= 0 ||
+                        (kHalves == 2 && page_of((n + i) * kHalves + 1) >= 0))
+                        tbk::mbar_wait(bar + x, phases >> x & 1, a.status);
+                }
+                break;
+            }
+            const int key0 = first + n * kStride;
+            uint8_t* values = stage + kKeys * DP;
+            const bool gaps = key0 + kKeys > load.s.len || have != (1 << kHalves) - 1;
+            if (gaps) {
+                // slots behind the last token, or of no page, may hold anything, NaN
+                // codes too: a weight of zero needs a finite value beside it
+                for (int i = lane; i < kKeys * DP / 16; i += 32) {
+                    const int key = i % kKeys;
+                    if (key0 + key >= load.s.len || !(have >> key / 16 & 1))
+                        *reinterpret_cast<uint4*>(values + place<DP, kKeys>(key, i / kKeys)) =
+                            make_uint4(0, 0, 0, 0);
+                }
+                tbk::fence_proxy_async_shared();  // the stage is filled by TMA again
+                __syncwarp();
+            }
+
+            // S^T in log2 units: s[f][b][2 i + e] is key key0 + 16 f + kg + 8 i, row
+            // 8 b + 2 t + e
+            float s[kHalves][NB][4];
+#pragma unroll
+            for (int f = 0; f < kHalves; ++f) {
+                uint32_t w[DP / 64][2][4];
+#pragma unroll
+                for (int h = 0; h < DP / 64; ++h)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const uint4 x = *reinterpret_cast<const uint4*>(
+                            stage + place<DP, kKeys>(16 * f + 8 * i + kg, 4 * h + t));
+                        w[h][i][0] = x.x;
+                        w[h][i][1] = x.y;
+                        w[h][i][2] = x.z;
+                        w[h][i][3] = x.w;
+                    }
 #pragma unroll
                 for (int b = 0; b < NB; ++b) {
-                    if constexpr (kQReg) {
-                        kv8::mma16816(s2[j & 1][b], a0, a1, a2, a3, qr[k][b][0], qr[k][b][1]);
-                        if constexpr (kSplit)
-                            kv8::mma16816(s2[j & 1][b], a0, a1, a2, a3, ql[k][b][0], ql[k][b][1]);
+                    auto products = [&](auto& d, int p) {
+#pragma unroll
+                        for (int h = 0; h < DP / 64; ++h)
+#pragma unroll
+                            for (int j = 0; j < 4; j += 2) {
+                                uint2 q;
+                                if constexpr (kQReg)
+                                    q = make_uint2(qr[p][4 * h + j][b], qr[p][4 * h + j + 1][b]);
+                                else
+                                    q = reinterpret_cast<const uint2*>(
+                                        qs)[((p * kWords + 4 * h + j) / 2 * NB + b) * 32 + lane];
+                                kv8::mma_codes(d, w[h][0][j], w[h][1][j], w[h][0][j + 1],
+                                               w[h][1][j + 1], q.x, q.y);
+                            }
+                    };
+                    float(&z)[4] = s[f][b];
+                    if constexpr (FORMAT == kv8::kInt8) {
+                        // whole sums below 2^22 over the bits of 1.5 * 2^23 are that
+                        // f32 plus the sum
+                        constexpr int kBits = 0x4b400000;
+                        constexpr float kBase = 12582912.0f;
+                        int d[3][4];
+#pragma unroll
+                        for (int p = 0; p < 3; ++p) {
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) d[p][e] = kBits;
+                            products(d[p], p);
+                        }
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            z[e] = fmaf(__int_as_float(d[0][e]), 16384.0f, -kBase * 16384.0f);
+                            z[e] = fmaf(__int_as_float(d[1][e]) - kBase, 128.0f, z[e]);
+                            z[e] += __int_as_float(d[2][e]) - kBase;
+                        }
                     } else {
-                        const uint2 q = qs[(k * NB + b) * 32 + lane];
-                        kv8::mma16816(s2[j & 1][b], a0, a1, a2, a3, q.x, q.y);
-                        if constexpr (kSplit) {
-                            const uint2 r = qs[((kSteps + k) * NB + b) * 32 + lane];
-                            kv8::mma16816(s2[j & 1][b], a0, a1, a2, a3, r.x, r.y);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) z[e] = 0.0f;
+#pragma unroll
+                        for (int p = kParts - 1; p >= 0; --p) {
+                            float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                            products(d, p);
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) z[e] = fmaf(z[e], 1.0f / Q::kRadix, d[e]);
                         }
                     }
                 }
             }
-        }
-        // log2 units: s[b][2 i + e] is key key0 + kg + 8 i, row 8 b + 2 t + e; the
-        // values' scale as an exponent
-        const float lv = (float)((int)(__float_as_uint(v_scale) >> 23) - 127);
-        float s[NB][4];
-        bool inside = true, over = false;
-#pragma unroll
-        for (int b = 0; b < NB; ++b)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                const float f = qc[b][e] * k_scale;
-                s[b][e] = (s2[0][b][e] + s2[1][b][e]) * f;
-                s[b][2 + e] = (s2[0][b][2 + e] + s2[1][b][2 + e]) * f;
-                inside &= key0 >= see_lo[b][e] && key0 + kStep - 1 <= see_hi[b][e];
-            }
-        if (!__all_sync(tbk::kFull, inside)) {
-#pragma unroll
-            for (int b = 0; b < NB; ++b)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int j = key0 + kg + 8 * (i >> 1);
-                    if (j < see_lo[b][i & 1] || j > see_hi[b][i & 1]) s[b][i] = -INFINITY;
-                }
-        }
-#pragma unroll
-        for (int b = 0; b < NB; ++b)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                const float hi = fmaxf(s[b][e], s[b][2 + e]);
-                over |= hi > ref[b][e] + kSlack || hi + lv > vref[b][e] + kSlack;
-            }
-        if (__any_sync(tbk::kFull, over)) {
+            bool inside = !gaps, over = false;
 #pragma unroll
             for (int b = 0; b < NB; ++b)
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
-                    float hi = fmaxf(s[b][e], s[b][2 + e]);
+                    inside &= key0 >= see_lo[b][e] && key0 + kKeys - 1 <= see_hi[b][e];
 #pragma unroll
-                    for (int x = 4; x < 32; x <<= 1)
-                        hi = fmaxf(hi, __shfl_xor_sync(tbk::kFull, hi, x));
-                    const float m = fmaxf(ref[b][e], ceilf(hi));
-                    const float mv = fmaxf(vref[b][e], ceilf(hi) + lv);
-                    if (m > ref[b][e]) sum[b][e] *= kv8::exp2_fast(ref[b][e] - m);
-                    if (mv > vref[b][e]) {
-                        const float keep = kv8::exp2_fast(vref[b][e] - mv);
+                    for (int f = 0; f < kHalves; ++f) {
+                        const float scale = qc[b][e] * k_scale[f];
+                        s[f][b][e] *= scale;
+                        s[f][b][2 + e] *= scale;
+                    }
+                }
+            if (!__all_sync(tbk::kFull, inside)) {
 #pragma unroll
-                        for (int i = 0; i < kTiles; ++i) {
-                            o[i][b][e] *= keep;
-                            o[i][b][2 + e] *= keep;
+                for (int f = 0; f < kHalves; ++f)
+#pragma unroll
+                    for (int b = 0; b < NB; ++b)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const int j = key0 + 16 * f + kg + 8 * (i >> 1);
+                            if (j < see_lo[b][i & 1] || j > see_hi[b][i & 1] || !(have >> f & 1))
+                                s[f][b][i] = -INFINITY;
+                        }
+            }
+#pragma unroll
+            for (int b = 0; b < NB; ++b)
+#pragma unroll
+                for (int e = 0; e < 2; ++e)
+#pragma unroll
+                    for (int f = 0; f < kHalves; ++f) {
+                        const float hi = fmaxf(s[f][b][e], s[f][b][2 + e]);
+                        over |= hi > ref[b][e] + kSlack || hi + lv[f] > vref[b][e] + kSlack;
+                    }
+            if (__any_sync(tbk::kFull, over)) {
+#pragma unroll
+                for (int b = 0; b < NB; ++b)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        float hi = -INFINITY, hv = -INFINITY;
+#pragma unroll
+                        for (int f = 0; f < kHalves; ++f) {
+                            const float x = fmaxf(s[f][b][e], s[f][b][2 + e]);
+                            hi = fmaxf(hi, x);
+                            hv = fmaxf(hv, ceilf(x) + lv[f]);
+                        }
+#pragma unroll
+                        for (int x = 4; x < 32; x <<= 1) {
+                            hi = fmaxf(hi, __shfl_xor_sync(tbk::kFull, hi, x));
+                            hv = fmaxf(hv, __shfl_xor_sync(tbk::kFull, hv, x));
+                        }
+                        const float m = fmaxf(ref[b][e], ceilf(hi)), mv = fmaxf(vref[b][e], hv);
+                        if (m > ref[b][e]) sum[b][e] *= kv8::exp2_fast(ref[b][e] - m);
+                        if (mv > vref[b][e]) {
+                            const float keep = kv8::exp2_fast(vref[b][e] - mv);
+#pragma unroll
+                            for (int i = 0; i < kTiles; ++i) {
+                                o[i][b][e] *= keep;
+                                o[i][b][2 + e] *= keep;
+                            }
+                        }
+                        ref[b][e] = m;
+                        vref[b][e] = mv;
+                    }
+            }
+#pragma unroll
+            for (int f = 0; f < kHalves; ++f) {
+                // weights: for the sum, and times the values' scale as P^T's operands
+                uint32_t ph[NB][2], pl[NB][2];
+#pragma unroll
+                for (int b = 0; b < NB; ++b) {
+                    float p[4];
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const float m = ref[b][e], mv = vref[b][e] - lv[f] - kLift;
+                        sum[b][e] += kv8::exp2_fast(s[f][b][e] - m) +
+                                     kv8::exp2_fast(s[f][b][2 + e] - m);
+                        p[e] = kv8::exp2_fast(s[f][b][e] - mv);
+                        p[2 + e] = kv8::exp2_fast(s[f][b][2 + e] - mv);
+                    }
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const uint32_t hi = kv8::pack_f16x2(p[2 * i], p[2 * i + 1]);
+                        ph[b][i] = kv8::transpose8(hi);
+                        if constexpr (kSplit) {
+                            const __half2 h2 = *reinterpret_cast<const __half2*>(&hi);
+                            pl[b][i] = kv8::transpose8(
+                                kv8::pack_f16x2(p[2 * i] - __low2float(h2),
+                                                p[2 * i + 1] - __high2float(h2)));
                         }
                     }
-                    ref[b][e] = m;
-                    vref[b][e] = mv;
                 }
-        }
-        // weights: for the sum, and times the values' scale as P^T's operands
-        uint32_t ph[NB][2], pl[NB][2];
+                // O^T += V^T P^T: tile rows g and g + 8 are two neighbouring elements
+                constexpr int kWide = DP >= 128 ? 16 : 8;  // bytes a lane takes of a key at once
 #pragma unroll
-        for (int b = 0; b < NB; ++b) {
-            float p[4];
+                for (int h = 0; h < (DP + 127) / 128; ++h) {
+                    uint32_t w[4][kWide / 4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int key = 16 * f + (i & 1 ? kb : ka) + (i & 2 ? 8 : 0);
+                        if constexpr (DP >= 128) {
+                            const uint4 x = *reinterpret_cast<const uint4*>(
+                                values + place<DP, kKeys>(key, 8 * h + g));
+                            w[i][0] = x.x;
+                            w[i][1] = x.y;
+                            w[i][2] = x.z;
+                            w[i][3] = x.w;
+                        } else {
+                            const uint2 x = *reinterpret_cast<const uint2*>(
+                                values + place<DP, kKeys>(key, g >> 1) + (g & 1) * 8);
+                            w[i][0] = x.x;
+                            w[i][1] = x.y;
+                        }
+                    }
+#pragma unroll
+                    for (int j = 0; j < kWide / 4; ++j) {
+                        uint32_t lo[4], hi[4];
+                        kv8::words<FORMAT>(w[0][j], w[1][j], lo);
+                        kv8::words<FORMAT>(w[2][j], w[3][j], hi);
+#pragma unroll
+                        for (int i = 0; i < 2; ++i)
+#pragma unroll
+                            for (int b = 0; b < NB; ++b) {
+                                float(&d)[4] = o[h * 8 + 2 * j + i][b];
+                                kv8::mma_f16(d, lo[2 * i], lo[2 * i + 1], hi[2 * i], hi[2 * i + 1],
+                                             ph[b][0], ph[b][1]);
+                                if constexpr (kSplit)
+                                    kv8::mma_f16(d, lo[2 * i], lo[2 * i + 1], hi[2 * i],
+                                                 hi[2 * i + 1], pl[b][0], pl[b][1]);
+                            }
+                    }
+                }
+            }
+        }
+        __syncthreads();  // the rings are free: the warps' states meet in their place
+
+        // o[h 8 + u][b][2 r + e]: element 128 h + kWide g + 2 u + r of row 8 b + 2 t + e
+        constexpr int kWide = DP >= 128 ? 16 : 8;
+        float* jo = reinterpret_cast<float*>(smem);
+        float* jm = jo + kWarps * kRows * H::kPitch;
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-                const float m = ref[b][e] == -INFINITY ? 0.0f : ref[b][e];
-                const float mv = (vref[b][e] == -INFINITY ? 0.0f : vref[b][e]) - lv - kLift;
-                sum[b][e] += kv8::exp2_fast(s[b][e] - m) + kv8::exp2_fast(s[b][2 + e] - m);
-                p[e] = kv8::exp2_fast(s[b][e] - mv);
-                p[2 + e] = kv8::exp2_fast(s[b][2 + e] - mv);
-            }
+                float z = sum[b][e];
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const uint32_t hi = kv8::pack_f16x2(p[2 * i], p[2 * i + 1]);
-                ph[b][i] = kv8::transpose8(hi);
-                if constexpr (kSplit) {
-                    const __half2 h2 = *reinterpret_cast<const __half2*>(&hi);
-                    pl[b][i] = kv8::transpose8(kv8::pack_f16x2(p[2 * i] - __low2float(h2),
-                                                               p[2 * i + 1] - __high2float(h2)));
+                for (int x = 4; x < 32; x <<= 1) z += __shfl_xor_sync(tbk::kFull, z, x);
+                const int i = warp * kRows + 8 * b + 2 * t + e;
+                float* row = jo + i * H::kPitch;
+#pragma unroll
+                for (int u = 0; u < kTiles; ++u)
+                    *reinterpret_cast<float2*>(row + (u / 8) * 128 + kWide * g + 2 * (u % 8)) =
+                        make_float2(o[u][b][e], o[u][b][2 + e]);
+                if (g == 0) {
+                    jm[i * 3] = ref[b][e];
+                    jm[i * 3 + 1] = vref[b][e];
+                    jm[i * 3 + 2] = z;
                 }
             }
-        }
-        // O^T += V^T P^T: tile rows g and g + 8 are two neighbouring elements
-        const uint8_t* values = stage + kStep * DP;
-        constexpr int kWide = DP >= 128 ? 16 : 8;  // bytes a lane takes of a key at once
+        __syncthreads();
+        const int64_t unit = 2 * (int64_t)blockIdx.x + !first_block;
+        for (int row = warp; row < blk.rows; row += kWarps) {
+            float m = kNoRef, mv = kNoRef, total = 0.0f, w[kWarps];
 #pragma unroll
-        for (int h = 0; h < (DP + 127) / 128; ++h) {
-            uint32_t w[4][kWide / 4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int key = (i & 1 ? kb : ka) + (i & 2 ? 8 : 0);
-                if constexpr (DP >= 128) {
-                    const uint4 x =
-                        *reinterpret_cast<const uint4*>(values + place<DP>(key, 8 * h + g));
-                    w[i][0] = x.x;
-                    w[i][1] = x.y;
-                    w[i][2] = x.z;
-                    w[i][3] = x.w;
-                } else {
-                    const uint2 x = *reinterpret_cast<const uint2*>(
-                        values + place<DP>(key, g >> 1) + (g & 1) * 8);
-                    w[i][0] = x.x;
-                    w[i][1] = x.y;
-                }
+            for (int i = 0; i < kWarps; ++i) {
+                m = fmaxf(m, jm[(i * kRows + row) * 3]);
+                mv = fmaxf(mv, jm[(i * kRows + row) * 3 + 1]);
             }
 #pragma unroll
-            for (int j = 0; j < kWide / 4; ++j) {
-                uint32_t lo[4], hi[4];
-                kv8::words<FORMAT>(w[0][j], w[1][j], lo);
-                kv8::words<FORMAT>(w[2][j], w[3][j], hi);
+            for (int i = 0; i < kWarps; ++i) {
+                const float* st = jm + (i * kRows + row) * 3;
+                total += st[2] * exp2f(st[0] - m);
+                w[i] = exp2f(st[1] - mv);
+            }
+            const bool none = total == 0.0f;
+            // O is in units of 2^(mv - lift), the sum of 2^m
+            const float per = none ? 0.0f : exp2f(-kLift) / total;
+            const float unit_v = none ? 0.0f : exp2f(mv - m);
+            const int at = block * kRows + row;
+            const int64_t tok = load.s.lo + at / group;
+            const int h = head * group + at % group;
+            T* out = static_cast<T*>(a.out) + tok * a.out_stride + (int64_t)h * a.d;
+            float* part = whole ? nullptr : a.part + (unit * kRows + row) * a.d;
+            for (int i = lane; i < a.d; i += 32) {
+                float y = 0.0f;
 #pragma unroll
-                for (int i = 0; i < 2; ++i)
-#pragma unroll
-                    for (int b = 0; b < NB; ++b) {
-                        float(&d)[4] = o[h * 8 + 2 * j + i][b];
-                        kv8::mma16816(d, lo[2 * i], lo[2 * i + 1], hi[2 * i], hi[2 * i + 1],
-                                      ph[b][0], ph[b][1]);
-                        if constexpr (kSplit)
-                            kv8::mma16816(d, lo[2 * i], lo[2 * i + 1], hi[2 * i], hi[2 * i + 1],
-                                          pl[b][0], pl[b][1]);
-                    }
+                for (int k = 0; k < kWarps; ++k) y += w[k] * jo[(k * kRows + row) * H::kPitch + i];
+                y = none ? 0.0f : y * per * unit_v;
+                if (whole)
+                    tbk::Elt<T>::store(out + i, y);
+                else
+                    part[i] = y;
+            }
+            if (lane == 0) {
+                if (!whole)
+                    a.state[unit * kRows + row] = make_float2(m, total);
+                else if (a.lse)
+                    a.lse[tok * a.hq + h] = none ? -INFINITY : m * 0.69314718055994531f + logf(total);
             }
         }
+        // the next block's copies go where this one's states were read
+        tbk::fence_proxy_async_shared();
+        __syncthreads();
     }
-    __syncthreads();  // the rings are free: the warps' states meet in their place
-
-    // o[h 8 + u][b][2 r + e]: element 128 h + kWide g + 2 u + r of row 8 b + 2 t + e
-    constexpr int kWide = DP >= 128 ? 16 : 8;
-    float* jo = reinterpret_cast<float*>(smem);
-    float* jm = jo + kWarps * kRows * H::kPitch;
-#pragma unroll
-    for (int b = 0; b < NB; ++b)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-            float z = sum[b][e];
-#pragma unroll
-            for (int x = 4; x < 32; x <<= 1) z += __shfl_xor_sync(tbk::kFull, z, x);
-            const int i = warp * kRows + 8 * b + 2 * t + e;
-            float* row = jo + i * H::kPitch;
-#pragma unroll
-            for (int u = 0; u < kTiles; ++u)
-                *reinterpret_cast<float2*>(row + (u / 8) * 128 + kWide * g + 2 * (u % 8)) =
-                    make_float2(o[u][b][e], o[u][b][2 + e]);
-            if (g == 0) {
-                jm[i * 3] = ref[b][e];
-                jm[i * 3 + 1] = vref[b][e];
-                jm[i * 3 + 2] = z;
-            }
-        }
-    __syncthreads();
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    const bool whole = blk.used == 1;
-    const int64_t unit =
-        (((int64_t)seq * a.hkv + head) * a.blocks + block) * a.chunks + c;
-    for (int row = warp; row < blk.rows; row += kWarps) {
-        float m = -INFINITY, mv = -INFINITY, total = 0.0f, w[kWarps];
-#pragma unroll
-        for (int i = 0; i < kWarps; ++i) {
-            m = fmaxf(m, jm[(i * kRows + row) * 3]);
-            mv = fmaxf(mv, jm[(i * kRows + row) * 3 + 1]);
-        }
-#pragma unroll
-        for (int i = 0; i < kWarps; ++i) {
-            const float* st = jm + (i * kRows + row) * 3;
-            total += st[0] == -INFINITY ? st[2] : st[2] * exp2f(st[0] - m);
-            w[i] = st[1] == -INFINITY ? 0.0f : exp2f(st[1] - mv);
-        }
-        const bool none = total == 0.0f;
-        // O is in units of 2^(mv - lift), the sum of 2^m
-        const float per = none ? 0.0f : exp2f(-kLift) / total;
-        const float unit_v = none ? 0.0f : exp2f(mv - m);
-        const int at = block * kRows + row;
-        const int64_t tok = blk.s.lo + at / group;
-        const int h = head * group + at % group;
-        T* out = static_cast<T*>(a.out) + tok * a.out_stride + (int64_t)h * a.d;
-        float* part = whole ? nullptr : a.part + (unit * kRows + row) * a.d;
-        for (int i = lane; i < a.d; i += 32) {
-            float y = 0.0f;
-#pragma unroll
-            for (int k = 0; k < kWarps; ++k) y += w[k] * jo[(k * kRows + row) * H::kPitch + i];
-            y = none ? 0.0f : y * per * unit_v;
-            if (whole)
-                tbk::Elt<T>::store(out + i, y);
-            else
-                part[i] = y;
-        }
-        if (lane == 0) {
-            if (!whole)
-                a.state[unit * kRows + row] = make_float2(m, total);
-            else if (a.lse)
-                a.lse[tok * a.hq + h] = none ? -INFINITY : m * 0.69314718055994531f + logf(total);
-        }
-    }
 }
 
-// Joins the chunks of a row: out = sum_c w_c out_c / sum_c w_c, w_c the chunk's
-// sum at the largest reference.  A CTA per row: the weights first, then a warp
-// takes every eighth chunk, four loads in flight, a lane four elements of 128.
+// Joins the blocks that a cut went through: out = sum_c w_c out_c / sum_c w_c,
+// w_c a part's sum at the largest reference.  The first cut through a block
+// has its CTA; its 8 warps take a row each, or, when there are few blocks (and
+// so many parts of each), all the parts of one row, four loads in flight.
 constexpr int kJoinWarps = 8;
-constexpr int kMostChunks = 1024;
 template <typename T>
 __global__ void __launch_bounds__(32 * kJoinWarps) k_join(const __grid_constant__ Args a) {
-    __shared__ float w_s[kMostChunks];
+    __shared__ float w_s[kJoinWarps][kMostCtas];
     __shared__ float4 part[kJoinWarps][kv8::kMaxDim / 4];
-    __shared__ float red[32];
-    const int block = blockIdx.x / a.block_rows, row = blockIdx.x % a.block_rows;
-    const int head = blockIdx.y, seq = blockIdx.z;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const Block blk = block_of(a, seq, block, false);
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    if (row >= blk.rows || blk.used == 1) return;
-    const int group = a.hq / a.hkv;
-    const int64_t unit = (((int64_t)seq * a.hkv + head) * a.blocks + block) * a.chunks;
-    const float2* st = a.state + unit * a.block_rows + row;
-    const float4* parts = reinterpret_cast<const float4*>(a.part) + (unit * a.block_rows + row) * (a.d / 4);
-    const int64_t pitch = (int64_t)a.block_rows * (a.d / 4);
-    float m = -INFINITY;
-    for (int c = threadIdx.x; c < blk.used; c += 32 * kJoinWarps)
-        m = fmaxf(m, st[(int64_t)c * a.block_rows].x);
-    m = tbk::block_max(m, red);
-    float mine = 0.0f;
-    for (int c = threadIdx.x; c < blk.used; c += 32 * kJoinWarps) {
-        const float2 s = st[(int64_t)c * a.block_rows];
-        const float w = s.x == -INFINITY ? s.y : s.y * exp2f(s.x - m);
-        w_s[c] = w;
-        mine += w;
-    }
-    const float total = tbk::group_sum(mine, 32 * kJoinWarps, red);  // and w_s is written
-#pragma unroll
-    for (int h = 0; h < kv8::kMaxDim / 128; ++h) {
-        const int i = 32 * h + lane;
-        float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        if (i < a.d / 4) {
-            for (int c0 = warp; c0 < blk.used; c0 += 4 * kJoinWarps) {
+    const int c = blockIdx.x + 1;
+    const Cut cut = a.cuts[c];
+    if (cut.seq < 0) return;
+    const int64_t before = (c - 1) * cut.tiles / cut.ctas;
+    if (before > cut.begin + kHeadTiles) return;  // not the first cut
+    // parts: of CTA c - 1 (its first block's, or its last's), c, .. while their
+    // shares begin before the block's end
+    const int last = (int)min((int64_t)cut.ctas - 1, (cut.end * cut.ctas - 1) / cut.tiles);
+    const int parts = last - c + 2;
+    const int64_t lone = 2 * (int64_t)(c - 1) + (before < cut.begin);
+    auto at = [&](int p) { return p == 0 ? lone : 2 * (int64_t)(c - 1 + p); };
+    const Load load = load_of(a, cut.seq);
+    const Block blk = block_of(a, load, cut.block);
+    const int group = a.hq / a.hkv, quads = a.d / 4;
+    const int each = a.spread ? kJoinWarps : 1;  // warps per row
+    for (int row = a.spread ? blockIdx.y : warp; row < blk.rows; row += a.spread ? 1 << 30 : kJoinWarps) {
+        float m = -INFINITY, total = 0.0f;
+        for (int p = lane; p < parts; p += 32)
+            m = fmaxf(m, __ldcg(&a.state[at(p) * a.block_rows + row].x));
+        m = tbk::warp_max(m);
+        __syncwarp();
+        for (int p = lane; p < parts; p += 32) {
+            const float2 s = __ldcg(&a.state[at(p) * a.block_rows + row]);
+            const float w = s.y * exp2f(s.x - m);
+            w_s[warp][p] = w;
+            total += w;
+        }
+        total = tbk::warp_sum(total);
+        __syncwarp();
+        const bool none = total == 0.0f;
+        const int r = cut.block * a.block_rows + row;
+        const int64_t tok = load.s.lo + r / group;
+        const int h = cut.head * group + r % group;
+        T* out = static_cast<T*>(a.out) + tok * a.out_stride + (int64_t)h * a.d;
+        const float4* src = reinterpret_cast<const float4*>(a.part) + row * quads;
+        for (int i = lane; i < quads; i += 32) {
+            float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            for (int p0 = a.spread ? warp : 0; p0 < parts; p0 += 4 * each) {
                 float4 x[4];
                 float w[4];
 #pragma unroll
                 for (int u = 0; u < 4; ++u) {
-                    const int c = c0 + u * kJoinWarps;
-                    const bool there = c < blk.used;
-                    w[u] = there ? w_s[c] : 0.0f;
-                    x[u] = there ? __ldcg(parts + c * pitch + i) : make_float4(0.f, 0.f, 0.f, 0.f);
+                    const int p = p0 + u * each;
+                    w[u] = p < parts ? w_s[warp][p] : 0.0f;
+                    x[u] = p < parts ? __ldcg(src + at(p) * a.block_rows * quads + i)
+                                     : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
                 }
 #pragma unroll
                 for (int u = 0; u < 4; ++u) {
@@ -619,23 +800,28 @@ __global__ void __launch_bounds__(32 * kJoinWarps) k_join(const __grid_constant_
                     y.w = fmaf(w[u], x[u].w, y.w);
                 }
             }
-            part[warp][i] = y;
+            if (a.spread) {
+                part[warp][i] = y;
+            } else {
+                tbk::Elt<T>::store(out + 4 * i, none ? 0.0f : y.x / total);
+                tbk::Elt<T>::store(out + 4 * i + 1, none ? 0.0f : y.y / total);
+                tbk::Elt<T>::store(out + 4 * i + 2, none ? 0.0f : y.z / total);
+                tbk::Elt<T>::store(out + 4 * i + 3, none ? 0.0f : y.w / total);
+            }
         }
-    }
-    __syncthreads();
-    const bool none = total == 0.0f;
-    const int at = block * a.block_rows + row;
-    const int64_t tok = blk.s.lo + at / group;
-    const int h = head * group + at % group;
-    T* out = static_cast<T*>(a.out) + tok * a.out_stride + (int64_t)h * a.d;
-    for (int i = threadIdx.x; i < a.d; i += 32 * kJoinWarps) {
-        float z = 0.0f;
+        if (a.spread) {
+            __syncthreads();
+            for (int i = threadIdx.x; i < a.d; i += 32 * kJoinWarps) {
+                float z = 0.0f;
 #pragma unroll
-        for (int k = 0; k < kJoinWarps; ++k) z += reinterpret_cast<const float*>(part[k])[i];
-        tbk::Elt<T>::store(out + i, none ? 0.0f : z / total);
+                for (int k = 0; k < kJoinWarps; ++k) z += reinterpret_cast<const float*>(part[k])[i];
+                tbk::Elt<T>::store(out + i, none ? 0.0f : z / total);
+            }
+        }
+        if (a.lse && lane == 0 && (!a.spread || warp == 0))
+            a.lse[tok * a.hq + h] = none ? -INFINITY : m * 0.69314718055994531f + logf(total);
+        __syncwarp();
     }
-    if (a.lse && threadIdx.x == 0)
-        a.lse[tok * a.hq + h] = none ? -INFINITY : m * 0.69314718055994531f + logf(total);
 }
 
 int check(const TbB200Kv8* cache, const TbB200Kv8Batch* batch, const TbB200Kv8Attention* t,
@@ -658,47 +844,56 @@ int check(const TbB200Kv8* cache, const TbB200Kv8Batch* batch, const TbB200Kv8At
     return TB_OK;
 }
 
-// How a call is cut: blocks of rows per sequence and head, chunks of keys per
-// block, scratch.
+// How a call is laid out: rows per block, CTAs, scratch.
 struct Plan {
-    int64_t blocks, chunks;
-    int block_rows;
-    size_t part_bytes, state_bytes;
+    int block_rows, ctas, whole, spread;
+    size_t cut_bytes, part_bytes, state_bytes;
+    size_t bytes() const { return cut_bytes + part_bytes + state_bytes; }
 };
 
 Plan plan_of(const TbB200Kv8* cache, const TbB200Kv8Batch* batch, const TbB200Kv8Attention* t,
              int sm_count) {
-    Plan p;
-    const int64_t rows = t->max_rows < batch->rows ? t->max_rows : batch->rows;
-    const int64_t most_rows = rows * (t->n_heads / cache->n_kv_heads);
-    p.block_rows = most_rows <= 8 ? 8 : 16;
-    p.blocks = (most_rows + p.block_rows - 1) / p.block_rows;
-    if (p.blocks < 1) p.blocks = 1;
-    const int64_t all = p.blocks * cache->n_kv_heads * batch->n_seqs;
-    const int64_t slots = (p.block_rows == 8 ? 4 : 3) * (int64_t)sm_count;
+    Plan p = {};
+    const int64_t group = t->n_heads / cache->n_kv_heads;
+    const int64_t rows = (t->max_rows < batch->rows ? t->max_rows : batch->rows) * group;
+    p.block_rows = rows <= 8 ? 8 : 16;
+    // at most so many blocks, of at most so many tiles
+    int64_t blocks = (rows + p.block_rows - 1) / p.block_rows * batch->n_seqs;
+    const int64_t most = batch->rows * group / p.block_rows + batch->n_seqs;
+    blocks = (blocks < most ? blocks : most) * cache->n_kv_heads;
     int64_t keys = t->max_len;
-    if (t->window && t->window + rows < keys) keys = t->window + rows;
-    const int64_t most = (keys + kLeastChunk - 1) / kLeastChunk;
-    p.chunks = 2 * all > slots ? (8 * slots + all - 1) / all : slots / all;
-    if (p.chunks > most) p.chunks = most;
-    if (p.chunks > kMostChunks) p.chunks = kMostChunks;
-    if (p.chunks < 1) p.chunks = 1;
-    const size_t units = p.chunks > 1 ? (size_t)(all * p.chunks) : 0;
-    p.part_bytes = units * p.block_rows * cache->head_dim * sizeof(float);
-    p.state_bytes = units * p.block_rows * sizeof(float2);
+    if (t->window && (int64_t)t->window + p.block_rows + 32 < keys)
+        keys = (int64_t)t->window + p.block_rows + 32;
+    const int64_t tiles = (keys + kTileKeys - 1) / kTileKeys;
+    p.whole = tiles <= kLeastTiles;  // blocks are not cut
+    int64_t ctas =
+        p.whole ? blocks : (blocks * (kHeadTiles + tiles) + kLeastTiles - 1) / kLeastTiles;
+    const int64_t slots = (int64_t)sm_count * ctas_per_sm(cache->head_dim, p.block_rows, t->dtype == TB_DTYPE_F32);
+    if (ctas > slots) ctas = slots;
+    if (ctas > kMostCtas) ctas = kMostCtas;
+    p.ctas = ctas < 1 ? 1 : (int)ctas;
+    if (p.ctas == 1) p.whole = 1;
+    p.spread = 4 * blocks <= p.ctas;
+    if (!p.whole) {
+        p.cut_bytes = (size_t)p.ctas * sizeof(Cut);
+        p.part_bytes = (size_t)p.ctas * 2 * p.block_rows * cache->head_dim * sizeof(float);
+        p.state_bytes = (size_t)p.ctas * 2 * p.block_rows * sizeof(float2);
+    }
     return p;
 }
 
 template <typename T, int FORMAT, int DP, int NB>
 int launch(Args& a, const TbB200Kv8* cache, dim3 grid, cudaStream_t s) {
-    constexpr int bytes = Shape<T, DP, NB>::kBytes;
+    using H = Shape<T, FORMAT, DP, NB>;
+    constexpr int bytes = H::kBytes;
+    const int keys = cache->page < H::kKeys ? cache->page : H::kKeys;
     static std::atomic<uint64_t> granted{0};  // a bit per device
     int rc = kv8::once_per_device(granted, [&] {
         return cudaFuncSetAttribute(k_attend<T, FORMAT, DP, NB>,
                                     cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
     });
-    if (rc == TB_OK) rc = kv8::tile_map(&a.k_map, cache, cache->k, DP < 128 ? DP : 128, kStep);
-    if (rc == TB_OK) rc = kv8::tile_map(&a.v_map, cache, cache->v, DP < 128 ? DP : 128, kStep);
+    if (rc == TB_OK) rc = kv8::tile_map(&a.k_map, cache, cache->k, DP < 128 ? DP : 128, keys);
+    if (rc == TB_OK) rc = kv8::tile_map(&a.v_map, cache, cache->v, DP < 128 ? DP : 128, keys);
     if (rc != TB_OK) return rc;
     k_attend<T, FORMAT, DP, NB><<<grid, kThreads, bytes, s>>>(a);
     TB_LAUNCH_CHECK("8-bit cache attention kernel");
@@ -748,7 +943,7 @@ extern "C" int tb_b200_kv8_attention_workspace(const TbB200Kv8* cache,
     tbh::DeviceState* ds = tbh::current_device_state();
     if (!ds) return TB_ERR_DEVICE;
     const Plan p = plan_of(cache, batch, attention, ds->sm_count);
-    *bytes = p.part_bytes + p.state_bytes;
+    *bytes = p.bytes();
     return TB_OK;
 }
 
@@ -761,8 +956,7 @@ extern "C" int tb_b200_kv8_attention(const TbB200Kv8* cache, const TbB200Kv8Batc
     tbh::DeviceState* ds = tbh::current_device_state();
     if (!ds) return TB_ERR_DEVICE;
     const Plan p = plan_of(cache, batch, t, ds->sm_count);
-    if (p.blocks * p.chunks > INT32_MAX || p.blocks * p.block_rows > INT32_MAX) return TB_ERR_INVALID_SHAPE;
-    const size_t bytes = p.part_bytes + p.state_bytes;
+    const size_t bytes = p.bytes();
     if (bytes && (!t->workspace || t->workspace_bytes < bytes || !tbh::aligned16(t->workspace))) {
         tbh::set_error_text("8-bit cache attention: workspace missing, small or misaligned");
         return TB_ERR_INVALID_ARG;
@@ -778,8 +972,12 @@ extern "C" int tb_b200_kv8_attention(const TbB200Kv8* cache, const TbB200Kv8Batc
     a.k_scale = cache->k_scale;
     a.v_scale = cache->v_scale;
     a.status = ds->status;
-    a.part = static_cast<float*>(t->workspace);
-    a.state = reinterpret_cast<float2*>(static_cast<uint8_t*>(t->workspace) + p.part_bytes);
+    if (bytes) {
+        uint8_t* w = static_cast<uint8_t*>(t->workspace);
+        a.part = reinterpret_cast<float*>(w);
+        a.state = reinterpret_cast<float2*>(w + p.part_bytes);
+        a.cuts = reinterpret_cast<Cut*>(w + p.part_bytes + p.state_bytes);
+    }
     a.scale = t->scale;
     a.hq = t->n_heads;
     a.hkv = cache->n_kv_heads;
@@ -787,18 +985,18 @@ extern "C" int tb_b200_kv8_attention(const TbB200Kv8* cache, const TbB200Kv8Batc
     a.window = t->window;
     a.max_rows = t->max_rows;
     a.max_len = t->max_len;
-    a.chunks = (int)p.chunks;
-    a.blocks = (int)p.blocks;
     a.block_rows = p.block_rows;
+    a.whole = p.whole;
+    a.spread = p.spread;
     a.vec = tbh::aligned16(t->q) && t->q_stride * s % 16 == 0;
-    const dim3 grid((unsigned)(p.blocks * p.chunks), (unsigned)a.hkv, (unsigned)batch->n_seqs);
+    const dim3 grid((unsigned)p.ctas);
     cudaStream_t st = tbh::stream_of(stream);
     const bool f32 = t->dtype == TB_DTYPE_F32, int8 = cache->format == kv8::kInt8;
     rc = f32 ? (int8 ? launch_rows<float, kv8::kInt8>(a, cache, grid, st)
                      : launch_rows<float, kv8::kE4m3>(a, cache, grid, st))
              : (int8 ? launch_rows<__nv_bfloat16, kv8::kInt8>(a, cache, grid, st)
                      : launch_rows<__nv_bfloat16, kv8::kE4m3>(a, cache, grid, st));
-    if (rc != TB_OK || p.chunks == 1) return rc;
-    const dim3 joins((unsigned)(p.blocks * p.block_rows), (unsigned)a.hkv, (unsigned)batch->n_seqs);
+    if (rc != TB_OK || p.whole) return rc;
+    const dim3 joins((unsigned)p.ctas - 1, p.spread ? (unsigned)p.block_rows : 1u);
     return f32 ? join<float>(a, joins, st) : join<__nv_bfloat16>(a, joins, st);
 }

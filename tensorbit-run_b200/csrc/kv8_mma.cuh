@@ -1,6 +1,6 @@
-// kv8_mma.cuh -- 8-bit codes as operands of the f16 matrix instructions.
-//
-// Every code is an f16 value exactly, subnormal e4m3 codes among them.
+// kv8_mma.cuh -- 8-bit codes as operands of the matrix instructions: as they
+// are (int8 x int8, e4m3 x e4m3), or as f16, which holds every code exactly,
+// subnormal e4m3 codes among them.
 #pragma once
 
 #include <atomic>
@@ -33,21 +33,6 @@ __device__ __forceinline__ uint32_t int8_pair(uint32_t w) {
     return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-// Which elements of a word of four the two registers of word() hold.
-template <int FORMAT>
-__device__ constexpr int word_element(int reg, int i) {
-    return FORMAT == kInt8 ? reg + 2 * i : 2 * reg + i;
-}
-template <int FORMAT>
-__device__ __forceinline__ void word(uint32_t w, uint32_t& r0, uint32_t& r1) {
-    if constexpr (FORMAT == kInt8) {
-        r0 = int8_pair(w);
-        r1 = int8_pair(w >> 8);
-    } else {
-        r0 = e4m3_pair(w, false);
-        r1 = e4m3_pair(w, true);
-    }
-}
 // Elements 0 .. 3 of two words, each with its partner of the other word.
 template <int FORMAT>
 __device__ __forceinline__ void words(uint32_t a, uint32_t b, uint32_t (&r)[4]) {
@@ -79,14 +64,84 @@ __device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
 }
 
 // d += a b: a 16 x 16 row-major, b 16 x 8 column-major, f32 sums.
-__device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2,
-                                         uint32_t a3, uint32_t b0, uint32_t b1) {
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+__device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2,
+                                        uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
         "{%8,%9}, {%0,%1,%2,%3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+// The same of codes, 32 elements deep: e4m3 with f32 sums (every bit of them is
+// kept: measured), int8 with exact ones.
+__device__ __forceinline__ void mma_codes(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2,
+                                          uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e4m3.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+        "{%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_codes(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2,
+                                          uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+        "{%8,%9}, {%0,%1,%2,%3};"
+        : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// A row of q, held as the sum of `parts` code operands, each 1 / kRadix of the
+// one before:
+//   int8: the nearest whole number to q * 127 * 2^14 / top as three digits
+//     (2^-22 of top, the row's largest);
+//   e4m3: q * 2^k (top in [128, 256)) four bits at a time: two parts are a bf16
+//     element exactly, six an f32 one, or the nearest multiple of 2^-13 (2^-29)
+//     where that is larger.
+template <typename T, int FORMAT>
+struct QParts {
+    static constexpr int kParts = FORMAT == kInt8 ? 3 : sizeof(T) == 4 ? 6 : 2;
+    static constexpr float kRadix = FORMAT == kInt8 ? 128.0f : 16.0f;
+    float lift, unit;  // q's factor; what a sum of products is to be multiplied with
+
+    __device__ explicit QParts(float top) {
+        if constexpr (FORMAT == kInt8) {
+            lift = 2080768.0f / fmaxf(top, 7.8886090522101181e-31f);
+            unit = fmaxf(top, 7.8886090522101181e-31f) * (1.0f / 2080768.0f);
+        } else {
+            const int e = min(max((int)(__float_as_uint(top) >> 23), 20), 254);
+            lift = __uint_as_float((uint32_t)(127 + 7 - e + 127) << 23);
+            unit = __uint_as_float((uint32_t)(e - 7) << 23);
+        }
+    }
+    // The parts of four elements, one word each.
+    __device__ void split(const float* x, uint32_t (&w)[kParts]) const {
+        if constexpr (FORMAT == kInt8) {
+#pragma unroll
+            for (int p = 0; p < 3; ++p) w[p] = 0;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int v = __float2int_rn(x[i] * lift);
+                const int a = (v + 8192) >> 14, r = v - (a << 14), b = (r + 64) >> 7;
+                w[0] |= (uint32_t)(a & 0xff) << 8 * i;
+                w[1] |= (uint32_t)(b & 0xff) << 8 * i;
+                w[2] |= (uint32_t)((r - (b << 7)) & 0xff) << 8 * i;
+            }
+        } else {
+            float r[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) r[i] = x[i] * lift;
+#pragma unroll
+            for (int p = 0; p < kParts; ++p) {
+                const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(r[0], r[1]),
+                                                             __NV_SATFINITE, __NV_E4M3);
+                const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(r[2], r[3]),
+                                                             __NV_SATFINITE, __NV_E4M3);
+                w[p] = lo | hi << 16;
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    r[i] = (r[i] - decode<kE4m3>((uint8_t)(w[p] >> 8 * i))) * 16.0f;
+            }
+        }
+    }
+};
 
 __device__ __forceinline__ float exp2_fast(float x) {
     float y;

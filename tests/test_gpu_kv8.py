@@ -7,8 +7,9 @@ equality.
 
 attention, per output element, with A = sum_j p_j |v_j| and, per row,
 S = scale max_j sum_i |q_i k_ij|:
-- a score is off by at most ds = S (d / 16 + 16) 2^-23: one f32 rounding or
-  truncation per group of 16 products, q held to 22 bits, the scalings;
+- a score is off by at most ds = S (d / 16 + 16) 2^-23 + R 2^-22: one f32
+  rounding or truncation per group of 16 products and the scalings; and q held
+  to 2^-22 of its row's largest element, so R = scale max_i |q_i| max_j sum_i |k_ij|;
 - p_j is off by 2 ds relative (its own score and the maximum's), 2^-21 for
   exp2 and its argument, and, for bf16 calls, 2^-11 for p as f16;
 - the sum over n keys is accumulated in f32 by groups of 16: (n / 16 + 16) 2^-23;
@@ -137,8 +138,9 @@ class Model:
                     A[row, h] = w @ np.abs(v[see, g])
                     floor[row, h] = 2.0 ** -35 * (w * vs[see, g]).max() * (
                         np.abs(v[see, g]) / vs[see, g][:, None]).sum(0)
-                    ds[row, h] = abs(scale) * (np.abs(k[see, g]) @ np.abs(q[row, h])).max()
-        ds *= (d / 16 + 16) * 2.0 ** -23
+                    ds[row, h] = abs(scale) * (
+                        (np.abs(k[see, g]) @ np.abs(q[row, h])).max() * (d / 16 + 16) * 2.0 ** -23
+                        + np.abs(q[row, h]).max() * np.abs(k[see, g]).sum(1).max() * 2.0 ** -22)
         acc = (n[:, None] / 16 + 16) * 2.0 ** -23
         rel = 2 * ds + 2.0 ** -21 + acc
         # what the output may be off by, but for its rounding and p's as f16
