@@ -13,18 +13,16 @@
 // Within a CTA each of 4 warps takes every fourth step of 32 keys (16 for heads
 // over 128) through a ring of TMA stages of its own: one lane issues the copies,
 // and no barrier of the CTA is in the loop.
-//   S^T = K Q^T, m16n8k32 on the codes as they are: lane (g, t) (g = lane / 4,
-//     t = lane % 4) holds keys order(g) and order(g) + 8, 16 consecutive elements
-//     of each with a 16-byte load; the head dimension is summed in the order in
-//     which that puts it, Q's registers the same.  Q is split into two to six
-//     parts of the format (QParts): matrix instructions on 8-bit operands cost a
-//     half (int8) or an eighth (e4m3) of an f16 one per product, conversions of
-//     the codes more than all of them;
+//   S^T = K Q^T, m16n8k32 on the codes as they are, ldmatrix their registers.  Q
+//     is split into two to six parts of the format (QParts): matrix instructions
+//     on 8-bit operands cost a half (int8) or a quarter (e4m3) of an f16 one per
+//     product, conversions of the codes more than all of them;
 //   O^T = V^T P^T, m16n8k16 on f16: S^T's registers, transposed 8 x 8, are P^T's
-//     operands; lane (g, t) holds elements 16 g .. 16 g + 15 (of 128) of keys
-//     order(2t), order(2t + 1) and those + 8, and pairs and converts them.
-// order() and TMA's swizzle (the 16-byte piece c of key r lies at c ^ (r & 7))
-// put the 8 lanes of each 16-byte access into different banks.
+//     operands; lane (g, t) (g = lane / 4, t = lane % 4) holds elements 16 g ..
+//     16 g + 15 (of 128) of keys 2t, 2t + 1, 2t + 8 and 2t + 9 with 16-byte
+//     loads, and pairs and converts them.
+// TMA's swizzle (the 16-byte piece c of key r lies at c ^ (r & 7)) puts the 8
+// rows of an ldmatrix and the 8 lanes of a 16-byte access into different banks.
 //
 // Precision.  A row of q is held to 2^-22 of its largest element or better,
 // products and their sums are exact (int8) or f32.  Weights p are f16 relative
@@ -43,7 +41,7 @@ constexpr int kWarps = 4;
 constexpr int kThreads = 32 * kWarps;
 constexpr int kTileKeys = 128;     // keys that shares are counted in
 constexpr int kLeastTiles = 2;     // tiles below which a share is not cut further
-constexpr int kHeadTiles = 1;      // what a block costs besides its keys, in tiles
+constexpr int kHeadTiles = 3;      // what a block costs besides its keys, in tiles
 constexpr int kMostCtas = 1024;
 constexpr float kSlack = 4.0f;     // how far (log2) scores may pass a reference
 constexpr float kLift = 11.0f;     // weights are held times 2^11: up to 2^15 in f16
@@ -53,10 +51,19 @@ constexpr float kNoRef = -3.0e38f;  // the reference of a row that has seen no k
 // A cut through a block: what the joining kernel needs.
 struct Cut {
     int64_t begin, end;  // the block's span, counted over the batch
-    int64_t tiles;       // of the batch
-    int ctas;            // that have a share
+    int64_t each;        // a share's length, but for the first `rest` CTAs', one longer
+    int rest;
     int seq, head, block;  // seq < 0: the share begins with a block
 };
+
+// Where CTA c's share begins.
+__device__ __forceinline__ int64_t share(int64_t each, int rest, int c) {
+    return c * each + min(c, rest);
+}
+// a / b of a >= 0, b > 0, in 32 bits where that does.
+__device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {
+    return (a | b) >> 32 ? a / b : (int64_t)((uint32_t)a / (uint32_t)b);
+}
 
 struct Args {
     CUtensorMap k_map, v_map;  // [n_pages * n_kv_heads][page][d] codes
@@ -71,7 +78,7 @@ struct Args {
     float* part;    // [CTA][2][block_rows][d] its first and last block's partial outputs
     float2* state;  // [CTA][2][block_rows] a row's (reference, sum)
     float scale;
-    int hq, hkv, d, window, max_rows, max_len, block_rows, whole, spread, vec;
+    int hq, hkv, d, window, max_rows, max_len, block_rows, whole, vec;
 };
 
 // A sequence's blocks and the tiles that its longest one may have.
@@ -119,8 +126,6 @@ __device__ __forceinline__ Block block_of(const Args& a, const Load& l, int bloc
     return k;
 }
 
-// The key (of 8) that row g of an operand stands for.
-__device__ __forceinline__ int order(int n) { return n ^ ((n & 1) << 2); }
 // Where the 16-byte piece c of a key lies in a tile of KEYS keys: DP = 64 has
 // rows of 64 bytes and that swizzle, DP = 256 two tiles of 128-byte rows.
 template <int DP, int KEYS>
@@ -150,7 +155,7 @@ struct Shape {
     // Q's operands stay in registers when they are few
     static constexpr int kParts = kv8::QParts<T, FORMAT>::kParts;
     static constexpr bool kQReg = kParts * kWords * NB <= 32;
-    static constexpr int kQBytes = kQReg ? 0 : kParts * kWords * NB * 128;
+    static constexpr int kQBytes = kParts * kWords * NB * 128;
     static constexpr int kRing = kWarps * kStages * kStageBytes;  // a multiple of 1024
     static constexpr int kPitch = DP + 4;
     static constexpr int kJoin = kWarps * kRows * (kPitch + 3) * 4;
@@ -209,24 +214,25 @@ k_attend(const __grid_constant__ Args a) {
 
     // This CTA's share: [tile, stop) of the batch's spans, the first in sequence
     // seq, whose own begin at seq_begin.
-    int64_t tile, stop, seq_begin, tiles;
-    int seq, ctas;
+    int64_t tile, stop, seq_begin = 0, each;
+    int seq, rest;
     {
-        int64_t mine = 0;
-        for (int i = threadIdx.x; i < a.b.n_seqs; i += kThreads) mine += load_of(a, i).total(a);
-        tiles = block_scan(mine, scan).y;
-        const int64_t want = a.whole ? tiles / (kHeadTiles + 1)
+        const int tid = threadIdx.x, n_seqs = a.b.n_seqs;
+        int64_t w = tid < n_seqs ? load_of(a, tid).total(a) : 0, tiles = w;
+        for (int i = tid + kThreads; i < n_seqs; i += kThreads) tiles += load_of(a, i).total(a);
+        longlong2 sum = block_scan(tiles, scan);  // (up to this thread, all)
+        tiles = sum.y;
+        const int64_t want = a.whole ? quotient(tiles, kHeadTiles + 1)
                                      : (tiles + kLeastTiles - 1) / kLeastTiles;
-        ctas = (int)min((int64_t)gridDim.x, want);
-        if (threadIdx.x == 0 && a.cuts) a.cuts[blockIdx.x].seq = -1;
+        const int ctas = (int)min((int64_t)gridDim.x, want);
+        if (tid == 0 && a.cuts) a.cuts[blockIdx.x].seq = -1;
         if ((int)blockIdx.x >= ctas) return;
-        tile = blockIdx.x * tiles / ctas;
-        stop = (blockIdx.x + 1) * tiles / ctas;
-        seq_begin = 0;
-        for (int i0 = 0;; i0 += kThreads) {  // ends: the sum over all is above tile
-            const int i = i0 + threadIdx.x;
-            const int64_t w = i < a.b.n_seqs ? load_of(a, i).total(a) : 0;
-            const longlong2 sum = block_scan(w, scan);  // (up to this thread, all)
+        each = quotient(tiles, ctas);
+        rest = (int)(tiles - each * ctas);
+        tile = share(each, rest, blockIdx.x);
+        stop = share(each, rest, blockIdx.x + 1);
+        if (n_seqs > kThreads) sum = block_scan(w, scan);
+        for (int i = tid;;) {  // ends: the sum over all is above tile
             if (tile >= seq_begin + sum.x - w && tile < seq_begin + sum.x) {
                 found_seq = i;
                 found_begin = seq_begin + sum.x - w;
@@ -234,10 +240,15 @@ k_attend(const __grid_constant__ Args a) {
             __syncthreads();
             if (tile < seq_begin + sum.y) break;
             seq_begin += sum.y;
+            i += kThreads;
+            w = i < n_seqs ? load_of(a, i).total(a) : 0;
+            sum = block_scan(w, scan);
         }
         seq = found_seq;
         seq_begin = found_begin;
     }
+    // the joining kernel may take its place on the SMs as CTAs end
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     Load load = load_of(a, seq);
 
     for (bool first_block = true; tile < stop; first_block = false) {
@@ -245,7 +256,7 @@ k_attend(const __grid_constant__ Args a) {
             seq_begin += load.total(a);
             load = load_of(a, ++seq);
         }
-        const int in_seq = (int)((tile - seq_begin) / load.span());
+        const int in_seq = (int)quotient(tile - seq_begin, load.span());
         const int head = in_seq / load.blocks, block = in_seq - head * load.blocks;
         const int64_t unit_begin = seq_begin + (int64_t)in_seq * load.span();
         // a share that ends within a block's head leaves it all to the next CTA
@@ -257,7 +268,7 @@ k_attend(const __grid_constant__ Args a) {
         const Block blk = block_of(a, load, block);
         if (threadIdx.x == 0) {
             if (first_block && skip > 0)
-                a.cuts[blockIdx.x] = {unit_begin, unit_begin + load.span(), tiles, ctas, seq, head,
+                a.cuts[blockIdx.x] = {unit_begin, unit_begin + load.span(), each, rest, seq, head,
                                       block};
             if (!load.ok) atomicOr(a.status, TB_B200_FLAG_POSITION_RANGE);
         }
@@ -330,11 +341,12 @@ k_attend(const __grid_constant__ Args a) {
 #pragma unroll
         for (int n = 0; n < kStages - 1; ++n) issue(n, n);
 
-        // Q's operands: row 8 b + g of the block, words of elements 64 h + 16 t +
-        // 4 j .. + 3; its sums of products are multiplied with qf, but for the
-        // page's scale.  A row with a NaN or an infinity is NaN.
-        uint32_t qr[kQReg ? kParts : 1][kQReg ? kWords : 1][NB];
+        // Q's operands: row 8 b + g of the block, words of elements 16 j +
+        // 4 t .. + 3, a quarter of them each warp's work; a row's sums of products
+        // are multiplied with qf, but for the page's scale.  A row with a NaN or an
+        // infinity is NaN.
         uint32_t* qs = reinterpret_cast<uint32_t*>(smem + H::kBytes - 1024 - H::kQBytes);
+        const uint2* q2 = reinterpret_cast<const uint2*>(qs) + lane;
         float qf[NB];
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
@@ -344,15 +356,15 @@ k_attend(const __grid_constant__ Args a) {
             const int hh = live ? at - tok * group : 0;
             const T* q = static_cast<const T*>(a.q) + (load.s.lo + tok) * a.q_stride +
                          (int64_t)(head * group + hh) * a.d;
-            float x[DP / 64][16], top = 0.0f;
+            float x[kWords][4], top = 0.0f;
             bool finite = true;
 #pragma unroll
-            for (int h = 0; h < DP / 64; ++h) {
-                kv8::load16(q + 64 * h + 16 * t, live && 64 * h + 16 * t < a.d, a.vec, x[h]);
+            for (int j = 0; j < kWords; ++j) {
+                kv8::load4(q + 16 * j + 4 * t, live && 16 * j < a.d, a.vec, x[j]);
 #pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    top = fmaxf(top, fabsf(x[h][e]));
-                    finite &= fabsf(x[h][e]) < INFINITY;
+                for (int e = 0; e < 4; ++e) {
+                    top = fmaxf(top, fabsf(x[j][e]));
+                    finite &= fabsf(x[j][e]) < INFINITY;
                 }
             }
             if (!finite) top = INFINITY;
@@ -361,20 +373,14 @@ k_attend(const __grid_constant__ Args a) {
             const Q parts(top < INFINITY ? top : 0.0f);
             qf[b] = top < INFINITY ? parts.unit * (a.scale * kLog2e) : NAN;
 #pragma unroll
-            for (int h = 0; h < DP / 64; ++h)
+            for (int j = 0; j < kWords; ++j) {
+                if (j % kWarps != warp) continue;
+                uint32_t w[kParts];
+                parts.split(x[j], w);
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    uint32_t w[kParts];
-                    parts.split(x[h] + 4 * j, w);
-#pragma unroll
-                    for (int p = 0; p < kParts; ++p) {
-                        if constexpr (kQReg)
-                            qr[p][4 * h + j][b] = w[p];
-                        else if (warp == 0)
-                            qs[(((p * kWords + 4 * h + j) / 2 * NB + b) * 32 + lane) * 2 + j % 2] =
-                                w[p];
-                    }
-                }
+                for (int p = 0; p < kParts; ++p)
+                    qs[(((p * kWords + j) / 2 * NB + b) * 32 + lane) * 2 + j % 2] = w[p];
+            }
         }
         // S^T's columns: rows 8 b + 2 t + e, keys [see_lo, see_hi] each
         float qc[NB][2];
@@ -391,7 +397,17 @@ k_attend(const __grid_constant__ Args a) {
                 see_hi[b][e] = live ? p : INT32_MAX;
                 see_lo[b][e] = a.window && live ? max(p - a.window + 1, 0) : 0;
             }
-        if constexpr (!kQReg) __syncthreads();
+        __syncthreads();
+        uint2 qr[kQReg ? kParts : 1][kQReg ? kWords / 2 : 1][NB];
+        if constexpr (kQReg) {
+#pragma unroll
+            for (int p = 0; p < kParts; ++p)
+#pragma unroll
+                for (int j = 0; j < kWords / 2; ++j)
+#pragma unroll
+                    for (int b = 0; b < NB; ++b)
+                        qr[p][j][b] = q2[((p * kWords / 2 + j) * NB + b) * 32];
+        }
 
         float o[kTiles][NB][4];
 #pragma unroll
@@ -409,7 +425,6 @@ k_attend(const __grid_constant__ Args a) {
                 sum[b][e] = 0.0f;
             }
 
-        const int ka = order(2 * t), kb = order(2 * t + 1), kg = order(g);
         int at_stage = kStages - 1;
         for (int n = 0; n < n_steps; ++n) {
             const int i0 = n % kBatch * kHalves;
@@ -447,6 +462,7 @@ k_attend(const __grid_constant__ Args a) {
             }
             const int key0 = first + n * kStride;
             uint8_t* values = stage + kKeys * DP;
+            const uint32_t stage_s = tbk::smem_addr(stage);
             const bool gaps = key0 + kKeys > load.s.len || have != (1 << kHalves) - 1;
             if (gaps) {
                 // slots behind the last token, or of no page, may hold anything, NaN
@@ -461,39 +477,32 @@ k_attend(const __grid_constant__ Args a) {
                 __syncwarp();
             }
 
-            // S^T in log2 units: s[f][b][2 i + e] is key key0 + 16 f + kg + 8 i, row
+            // S^T in log2 units: s[f][b][2 i + e] is key key0 + 16 f + g + 8 i, row
             // 8 b + 2 t + e
             float s[kHalves][NB][4];
 #pragma unroll
             for (int f = 0; f < kHalves; ++f) {
-                uint32_t w[DP / 64][2][4];
+                uint32_t w[kWords / 2][4];
 #pragma unroll
-                for (int h = 0; h < DP / 64; ++h)
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        const uint4 x = *reinterpret_cast<const uint4*>(
-                            stage + place<DP, kKeys>(16 * f + 8 * i + kg, 4 * h + t));
-                        w[h][i][0] = x.x;
-                        w[h][i][1] = x.y;
-                        w[h][i][2] = x.z;
-                        w[h][i][3] = x.w;
-                    }
+                for (int j = 0; j < kWords / 2; ++j)
+                    kv8::load_operand(stage_s + place<DP, kKeys>(16 * f + lane % 16, 2 * j + lane / 16),
+                                      w[j]);
 #pragma unroll
                 for (int b = 0; b < NB; ++b) {
-                    auto products = [&](auto& d, int p) {
+                    // d = the products of part p, over c
+                    auto products = [&](auto& d, int p, const auto& c) {
 #pragma unroll
-                        for (int h = 0; h < DP / 64; ++h)
-#pragma unroll
-                            for (int j = 0; j < 4; j += 2) {
-                                uint2 q;
-                                if constexpr (kQReg)
-                                    q = make_uint2(qr[p][4 * h + j][b], qr[p][4 * h + j + 1][b]);
-                                else
-                                    q = reinterpret_cast<const uint2*>(
-                                        qs)[((p * kWords + 4 * h + j) / 2 * NB + b) * 32 + lane];
-                                kv8::mma_codes(d, w[h][0][j], w[h][1][j], w[h][0][j + 1],
-                                               w[h][1][j + 1], q.x, q.y);
-                            }
+                        for (int j = 0; j < kWords / 2; ++j) {
+                            uint2 q;
+                            if constexpr (kQReg)
+                                q = qr[p][j][b];
+                            else
+                                q = q2[((p * kWords / 2 + j) * NB + b) * 32];
+                            if (j == 0)
+                                kv8::mma_codes(d, w[j], q.x, q.y, c);
+                            else
+                                kv8::mma_codes(d, w[j], q.x, q.y, d);
+                        }
                     };
                     float(&z)[4] = s[f][b];
                     if constexpr (FORMAT == kv8::kInt8) {
@@ -501,13 +510,10 @@ k_attend(const __grid_constant__ Args a) {
                         // f32 plus the sum
                         constexpr int kBits = 0x4b400000;
                         constexpr float kBase = 12582912.0f;
+                        const int base[4] = {kBits, kBits, kBits, kBits};
                         int d[3][4];
 #pragma unroll
-                        for (int p = 0; p < 3; ++p) {
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) d[p][e] = kBits;
-                            products(d[p], p);
-                        }
+                        for (int p = 0; p < 3; ++p) products(d[p], p, base);
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
                             z[e] = fmaf(__int_as_float(d[0][e]), 16384.0f, -kBase * 16384.0f);
@@ -515,12 +521,12 @@ k_attend(const __grid_constant__ Args a) {
                             z[e] += __int_as_float(d[2][e]) - kBase;
                         }
                     } else {
+                        const float base[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                        products(z, kParts - 1, base);
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) z[e] = 0.0f;
-#pragma unroll
-                        for (int p = kParts - 1; p >= 0; --p) {
-                            float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                            products(d, p);
+                        for (int p = kParts - 2; p >= 0; --p) {
+                            float d[4];
+                            products(d, p, base);
 #pragma unroll
                             for (int e = 0; e < 4; ++e) z[e] = fmaf(z[e], 1.0f / Q::kRadix, d[e]);
                         }
@@ -547,7 +553,7 @@ k_attend(const __grid_constant__ Args a) {
                     for (int b = 0; b < NB; ++b)
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
-                            const int j = key0 + 16 * f + kg + 8 * (i >> 1);
+                            const int j = key0 + 16 * f + g + 8 * (i >> 1);
                             if (j < see_lo[b][i & 1] || j > see_hi[b][i & 1] || !(have >> f & 1))
                                 s[f][b][i] = -INFINITY;
                         }
@@ -626,7 +632,7 @@ k_attend(const __grid_constant__ Args a) {
                     uint32_t w[4][kWide / 4];
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        const int key = 16 * f + (i & 1 ? kb : ka) + (i & 2 ? 8 : 0);
+                        const int key = 16 * f + 2 * t + (i & 1) + (i & 2) * 4;
                         if constexpr (DP >= 128) {
                             const uint4 x = *reinterpret_cast<const uint4*>(
                                 values + place<DP, kKeys>(key, 8 * h + g));
@@ -731,37 +737,37 @@ k_attend(const __grid_constant__ Args a) {
         tbk::fence_proxy_async_shared();
         __syncthreads();
     }
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 }
 
 // Joins the blocks that a cut went through: out = sum_c w_c out_c / sum_c w_c,
-// w_c a part's sum at the largest reference.  The first cut through a block
-// has its CTA; its 8 warps take a row each, or, when there are few blocks (and
-// so many parts of each), all the parts of one row, four loads in flight.
+// w_c a part's sum at the largest reference.  The first cut through a block has
+// its CTA, a warp per row: the weights first, then the parts, eight loads in
+// flight, a lane four elements of 128.
 constexpr int kJoinWarps = 8;
 template <typename T>
 __global__ void __launch_bounds__(32 * kJoinWarps) k_join(const __grid_constant__ Args a) {
     __shared__ float w_s[kJoinWarps][kMostCtas];
-    __shared__ float4 part[kJoinWarps][kv8::kMaxDim / 4];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const int c = blockIdx.x + 1;
     const Cut cut = a.cuts[c];
     if (cut.seq < 0) return;
-    const int64_t before = (c - 1) * cut.tiles / cut.ctas;
+    const int64_t before = share(cut.each, cut.rest, c - 1);
     if (before > cut.begin + kHeadTiles) return;  // not the first cut
     // parts: of CTA c - 1 (its first block's, or its last's), c, .. while their
     // shares begin before the block's end
-    const int last = (int)min((int64_t)cut.ctas - 1, (cut.end * cut.ctas - 1) / cut.tiles);
-    const int parts = last - c + 2;
+    const int64_t longer = cut.rest * (cut.each + 1);
+    const int last = (int)(cut.end <= longer
+                               ? quotient(cut.end - 1, cut.each + 1)
+                               : cut.rest + quotient(cut.end - 1 - longer, cut.each));
+    const int parts = min(last, (int)gridDim.x) - c + 2;
     const int64_t lone = 2 * (int64_t)(c - 1) + (before < cut.begin);
     auto at = [&](int p) { return p == 0 ? lone : 2 * (int64_t)(c - 1 + p); };
     const Load load = load_of(a, cut.seq);
     const Block blk = block_of(a, load, cut.block);
     const int group = a.hq / a.hkv, quads = a.d / 4;
-    const int each = a.spread ? kJoinWarps : 1;  // warps per row
-    for (int row = a.spread ? blockIdx.y : warp; row < blk.rows; row += a.spread ? 1 << 30 : kJoinWarps) {
-        float m = -INFINITY, total = 0.0f;
+    for (int row = warp; row < blk.rows; row += kJoinWarps) {
+        float m = kNoRef, total = 0.0f;
         for (int p = lane; p < parts; p += 32)
             m = fmaxf(m, __ldcg(&a.state[at(p) * a.block_rows + row].x));
         m = tbk::warp_max(m);
@@ -782,43 +788,30 @@ __global__ void __launch_bounds__(32 * kJoinWarps) k_join(const __grid_constant_
         const float4* src = reinterpret_cast<const float4*>(a.part) + row * quads;
         for (int i = lane; i < quads; i += 32) {
             float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            for (int p0 = a.spread ? warp : 0; p0 < parts; p0 += 4 * each) {
-                float4 x[4];
-                float w[4];
+            for (int p0 = 0; p0 < parts; p0 += 8) {
+                float4 x[8];
+                float w[8];
 #pragma unroll
-                for (int u = 0; u < 4; ++u) {
-                    const int p = p0 + u * each;
+                for (int u = 0; u < 8; ++u) {
+                    const int p = p0 + u;
                     w[u] = p < parts ? w_s[warp][p] : 0.0f;
                     x[u] = p < parts ? __ldcg(src + at(p) * a.block_rows * quads + i)
                                      : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
                 }
 #pragma unroll
-                for (int u = 0; u < 4; ++u) {
+                for (int u = 0; u < 8; ++u) {
                     y.x = fmaf(w[u], x[u].x, y.x);
                     y.y = fmaf(w[u], x[u].y, y.y);
                     y.z = fmaf(w[u], x[u].z, y.z);
                     y.w = fmaf(w[u], x[u].w, y.w);
                 }
             }
-            if (a.spread) {
-                part[warp][i] = y;
-            } else {
-                tbk::Elt<T>::store(out + 4 * i, none ? 0.0f : y.x / total);
-                tbk::Elt<T>::store(out + 4 * i + 1, none ? 0.0f : y.y / total);
-                tbk::Elt<T>::store(out + 4 * i + 2, none ? 0.0f : y.z / total);
-                tbk::Elt<T>::store(out + 4 * i + 3, none ? 0.0f : y.w / total);
-            }
+            tbk::Elt<T>::store(out + 4 * i, none ? 0.0f : y.x / total);
+            tbk::Elt<T>::store(out + 4 * i + 1, none ? 0.0f : y.y / total);
+            tbk::Elt<T>::store(out + 4 * i + 2, none ? 0.0f : y.z / total);
+            tbk::Elt<T>::store(out + 4 * i + 3, none ? 0.0f : y.w / total);
         }
-        if (a.spread) {
-            __syncthreads();
-            for (int i = threadIdx.x; i < a.d; i += 32 * kJoinWarps) {
-                float z = 0.0f;
-#pragma unroll
-                for (int k = 0; k < kJoinWarps; ++k) z += reinterpret_cast<const float*>(part[k])[i];
-                tbk::Elt<T>::store(out + i, none ? 0.0f : z / total);
-            }
-        }
-        if (a.lse && lane == 0 && (!a.spread || warp == 0))
+        if (a.lse && lane == 0)
             a.lse[tok * a.hq + h] = none ? -INFINITY : m * 0.69314718055994531f + logf(total);
         __syncwarp();
     }
@@ -846,7 +839,7 @@ int check(const TbB200Kv8* cache, const TbB200Kv8Batch* batch, const TbB200Kv8At
 
 // How a call is laid out: rows per block, CTAs, scratch.
 struct Plan {
-    int block_rows, ctas, whole, spread;
+    int block_rows, ctas, whole;
     size_t cut_bytes, part_bytes, state_bytes;
     size_t bytes() const { return cut_bytes + part_bytes + state_bytes; }
 };
@@ -873,7 +866,6 @@ Plan plan_of(const TbB200Kv8* cache, const TbB200Kv8Batch* batch, const TbB200Kv
     if (ctas > kMostCtas) ctas = kMostCtas;
     p.ctas = ctas < 1 ? 1 : (int)ctas;
     if (p.ctas == 1) p.whole = 1;
-    p.spread = 4 * blocks <= p.ctas;
     if (!p.whole) {
         p.cut_bytes = (size_t)p.ctas * sizeof(Cut);
         p.part_bytes = (size_t)p.ctas * 2 * p.block_rows * cache->head_dim * sizeof(float);
@@ -987,7 +979,6 @@ extern "C" int tb_b200_kv8_attention(const TbB200Kv8* cache, const TbB200Kv8Batc
     a.max_len = t->max_len;
     a.block_rows = p.block_rows;
     a.whole = p.whole;
-    a.spread = p.spread;
     a.vec = tbh::aligned16(t->q) && t->q_stride * s % 16 == 0;
     const dim3 grid((unsigned)p.ctas);
     cudaStream_t st = tbh::stream_of(stream);
@@ -997,6 +988,6 @@ extern "C" int tb_b200_kv8_attention(const TbB200Kv8* cache, const TbB200Kv8Batc
              : (int8 ? launch_rows<__nv_bfloat16, kv8::kInt8>(a, cache, grid, st)
                      : launch_rows<__nv_bfloat16, kv8::kE4m3>(a, cache, grid, st));
     if (rc != TB_OK || p.whole) return rc;
-    const dim3 joins((unsigned)p.ctas - 1, p.spread ? (unsigned)p.block_rows : 1u);
+    const dim3 joins((unsigned)p.ctas - 1);
     return f32 ? join<float>(a, joins, st) : join<__nv_bfloat16>(a, joins, st);
 }

@@ -51,6 +51,15 @@ __device__ __forceinline__ void words(uint32_t a, uint32_t b, uint32_t (&r)[4]) 
     }
 }
 
+// The left operand of mma_codes from shared memory: lane i gives the address of
+// the 16 bytes of row i % 16 and half i / 16 of 32.
+__device__ __forceinline__ void load_operand(uint32_t addr, uint32_t (&w)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
+                 : "r"(addr)
+                 : "memory");
+}
+
 // The transpose of an 8 x 8 tile of f16, two to a lane.
 __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
     uint32_t y;
@@ -71,21 +80,23 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1,
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-// The same of codes, 32 elements deep: e4m3 with f32 sums (every bit of them is
-// kept: measured), int8 with exact ones.
-__device__ __forceinline__ void mma_codes(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2,
-                                          uint32_t a3, uint32_t b0, uint32_t b1) {
+// d = a b + c of codes, 32 elements deep: e4m3 with f32 sums (every bit of them
+// is kept: measured), int8 with exact ones.
+__device__ __forceinline__ void mma_codes(float (&d)[4], const uint32_t (&a)[4], uint32_t b0,
+                                          uint32_t b1, const float (&c)[4]) {
     asm("mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e4m3.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
-        "{%8,%9}, {%0,%1,%2,%3};"
-        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+        "{%8,%9}, {%10,%11,%12,%13};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]),
+          "f"(c[3]));
 }
-__device__ __forceinline__ void mma_codes(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2,
-                                          uint32_t a3, uint32_t b0, uint32_t b1) {
+__device__ __forceinline__ void mma_codes(int (&d)[4], const uint32_t (&a)[4], uint32_t b0,
+                                          uint32_t b1, const int (&c)[4]) {
     asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
-        "{%8,%9}, {%0,%1,%2,%3};"
-        : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
-        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+        "{%8,%9}, {%10,%11,%12,%13};"
+        : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "r"(c[0]), "r"(c[1]), "r"(c[2]),
+          "r"(c[3]));
 }
 
 // A row of q, held as the sum of `parts` code operands, each 1 / kRadix of the
@@ -159,24 +170,23 @@ __device__ __forceinline__ void tma_load3(void* dst, const CUtensorMap* map, int
         : "memory");
 }
 
-// 16 consecutive elements as f32, the first `n` of them (a multiple of 16: all or none).
+// Four consecutive elements as f32, zeros if not live; vec: aligned to all four.
 template <typename T>
-__device__ __forceinline__ void load16(const T* p, bool live, bool vec, float (&v)[16]) {
+__device__ __forceinline__ void load4(const T* p, bool live, bool vec, float (&v)[4]) {
 #pragma unroll
-    for (int i = 0; i < 16; ++i) v[i] = 0.0f;
+    for (int i = 0; i < 4; ++i) v[i] = 0.0f;
     if (!live) return;
-    if (vec) {
-        constexpr int V = tbk::Elt<T>::kVec;
+    if (!vec) {
 #pragma unroll
-        for (int i = 0; i < 16; i += V) {
-            float x[V];
-            tbk::load_vec<T, V>(p + i, x);
-#pragma unroll
-            for (int e = 0; e < V; ++e) v[i + e] = x[e];
-        }
+        for (int i = 0; i < 4; ++i) v[i] = tbk::Elt<T>::load(p + i);
+    } else if constexpr (sizeof(T) == 4) {
+        tbk::load_vec<T, 4>(p, v);
     } else {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) v[i] = tbk::Elt<T>::load(p + i);
+        const uint2 w = *reinterpret_cast<const uint2*>(p);
+        v[0] = __uint_as_float(w.x << 16);
+        v[1] = __uint_as_float(w.x & 0xffff0000u);
+        v[2] = __uint_as_float(w.y << 16);
+        v[3] = __uint_as_float(w.y & 0xffff0000u);
     }
 }
 
