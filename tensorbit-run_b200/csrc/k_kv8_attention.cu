@@ -41,7 +41,7 @@ constexpr int kWarps = 4;
 constexpr int kThreads = 32 * kWarps;
 constexpr int kTileKeys = 128;     // keys that shares are counted in
 constexpr int kLeastTiles = 2;     // tiles below which a share is not cut further
-constexpr int kHeadTiles = 3;      // what a block costs besides its keys, in tiles
+constexpr int kHeadTiles = 2;      // what a block costs besides its keys, in tiles
 constexpr int kMostCtas = 1024;
 constexpr float kSlack = 4.0f;     // how far (log2) scores may pass a reference
 constexpr float kLift = 11.0f;     // weights are held times 2^11: up to 2^15 in f16
@@ -78,7 +78,7 @@ struct Args {
     float* part;    // [CTA][2][block_rows][d] its first and last block's partial outputs
     float2* state;  // [CTA][2][block_rows] a row's (reference, sum)
     float scale;
-    int hq, hkv, d, window, max_rows, max_len, block_rows, whole, vec;
+    int hq, hkv, d, window, max_rows, max_len, block_rows, whole, vec, vec_out;
 };
 
 // A sequence's blocks and the tiles that its longest one may have.
@@ -157,8 +157,8 @@ struct Shape {
     static constexpr bool kQReg = kParts * kWords * NB <= 32;
     static constexpr int kQBytes = kParts * kWords * NB * 128;
     static constexpr int kRing = kWarps * kStages * kStageBytes;  // a multiple of 1024
-    static constexpr int kPitch = DP + 4;
-    static constexpr int kJoin = kWarps * kRows * (kPitch + 3) * 4;
+    static constexpr int kPitch = DP == 64 ? DP + 2 : DP + 4;  // floats of a row's state
+    static constexpr int kJoin = kWarps * kRows * (kPitch + 4) * 4;
     static constexpr int kBytes =
         (kRing > kJoin ? kRing : kJoin) + kQBytes + 1024;  // 1024: to align
     static constexpr int kCtas = ctas_of(DP, NB, kSplit);
@@ -198,6 +198,7 @@ k_attend(const __grid_constant__ Args a) {
     __shared__ uint64_t bars[kWarps * kStages];
     __shared__ int64_t scan[kWarps], found_begin;
     __shared__ int found_seq;
+    __shared__ uint4 top_s[kRows];
     // TMA's swizzle goes by the address: tiles start on 1024 bytes
     uint8_t* smem = smem_raw + (-tbk::smem_addr(smem_raw) & 1023u);
 
@@ -205,6 +206,10 @@ k_attend(const __grid_constant__ Args a) {
     const int group = a.hq / a.hkv;
     uint8_t* ring = smem + warp * kStages * H::kStageBytes;
     uint64_t* bar = bars + warp * kStages;
+    if (threadIdx.x == 0) {
+        kv8::prefetch_map(&a.k_map);
+        kv8::prefetch_map(&a.v_map);
+    }
     if (lane == 0) {
 #pragma unroll
         for (int i = 0; i < kStages; ++i) tbk::mbar_init(bar + i, 1);
@@ -276,6 +281,25 @@ k_attend(const __grid_constant__ Args a) {
         const int end = a.whole ? blk.end
                                 : (int)min(blk.from + (int64_t)till * kTileKeys, (int64_t)blk.end);
 
+        // Q: row 8 b + g of the block, words of elements 16 j + 4 t .. + 3, those
+        // with j % 4 = warp; asked for first, used when the copies are on their way
+        constexpr int kMine = kWords / kWarps;
+        float x[NB][kMine][4];
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+            const int i = 8 * b + g;
+            const bool live = i < blk.rows;
+            const int at = block * kRows + i, tok = live ? at / group : 0;
+            const int hh = live ? at - tok * group : 0;
+            const T* q = static_cast<const T*>(a.q) + (load.s.lo + tok) * a.q_stride +
+                         (int64_t)(head * group + hh) * a.d;
+#pragma unroll
+            for (int j = 0; j < kMine; ++j) {
+                const int word = 16 * (warp + kWarps * j);
+                kv8::load4(q + word + 4 * t, live && word < a.d, a.vec, x[b][j]);
+            }
+        }
+
         // the warp's steps: keys first + kStride n .. + kKeys - 1
         const int first = begin + warp * kKeys;
         const int n_steps = end > first ? (end - first + kStride - 1) / kStride : 0;
@@ -341,45 +365,38 @@ k_attend(const __grid_constant__ Args a) {
 #pragma unroll
         for (int n = 0; n < kStages - 1; ++n) issue(n, n);
 
-        // Q's operands: row 8 b + g of the block, words of elements 16 j +
-        // 4 t .. + 3, a quarter of them each warp's work; a row's sums of products
-        // are multiplied with qf, but for the page's scale.  A row with a NaN or an
-        // infinity is NaN.
+        // Each warp splits its quarter of Q; a row's sums of products are multiplied
+        // with qf, but for the page's scale.  A row with a NaN or an infinity (whose
+        // bits are the largest) is NaN.
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+            uint32_t top = 0;
+#pragma unroll
+            for (int j = 0; j < kMine; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) top = max(top, __float_as_uint(fabsf(x[b][j][e])));
+            top = max(top, __shfl_xor_sync(tbk::kFull, top, 1));
+            top = max(top, __shfl_xor_sync(tbk::kFull, top, 2));
+            if (t == 0) reinterpret_cast<uint32_t*>(top_s)[(8 * b + g) * 4 + warp] = top;
+        }
+        __syncthreads();
         uint32_t* qs = reinterpret_cast<uint32_t*>(smem + H::kBytes - 1024 - H::kQBytes);
         const uint2* q2 = reinterpret_cast<const uint2*>(qs) + lane;
         float qf[NB];
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
-            const int i = 8 * b + g;
-            const bool live = i < blk.rows;
-            const int at = block * kRows + i, tok = live ? at / group : 0;
-            const int hh = live ? at - tok * group : 0;
-            const T* q = static_cast<const T*>(a.q) + (load.s.lo + tok) * a.q_stride +
-                         (int64_t)(head * group + hh) * a.d;
-            float x[kWords][4], top = 0.0f;
-            bool finite = true;
-#pragma unroll
-            for (int j = 0; j < kWords; ++j) {
-                kv8::load4(q + 16 * j + 4 * t, live && 16 * j < a.d, a.vec, x[j]);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    top = fmaxf(top, fabsf(x[j][e]));
-                    finite &= fabsf(x[j][e]) < INFINITY;
-                }
-            }
-            if (!finite) top = INFINITY;
-            top = fmaxf(top, __shfl_xor_sync(tbk::kFull, top, 1));
-            top = fmaxf(top, __shfl_xor_sync(tbk::kFull, top, 2));
+            const uint4 u = top_s[8 * b + g];
+            const float top = __uint_as_float(max(max(u.x, u.y), max(u.z, u.w)));
             const Q parts(top < INFINITY ? top : 0.0f);
             qf[b] = top < INFINITY ? parts.unit * (a.scale * kLog2e) : NAN;
 #pragma unroll
-            for (int j = 0; j < kWords; ++j) {
-                if (j % kWarps != warp) continue;
+            for (int j = 0; j < kMine; ++j) {
                 uint32_t w[kParts];
-                parts.split(x[j], w);
+                parts.split(x[b][j], w);
+                const int word = warp + kWarps * j;
 #pragma unroll
                 for (int p = 0; p < kParts; ++p)
-                    qs[(((p * kWords + j) / 2 * NB + b) * 32 + lane) * 2 + j % 2] = w[p];
+                    qs[(((p * kWords + word) / 2 * NB + b) * 32 + lane) * 2 + word % 2] = w[p];
             }
         }
         // S^T's columns: rows 8 b + 2 t + e, keys [see_lo, see_hi] each
@@ -669,10 +686,15 @@ k_attend(const __grid_constant__ Args a) {
         }
         __syncthreads();  // the rings are free: the warps' states meet in their place
 
-        // o[h 8 + u][b][2 r + e]: element 128 h + kWide g + 2 u + r of row 8 b + 2 t + e
+        // o[h 8 + u][b][2 r + e]: element 128 h + kWide g + 2 u + r of row 8 b + 2 t
+        // + e.  A row's pairs are stored turned by turn(g) within their kWide, and
+        // kPitch apart, so that the lanes' pairs fall into different banks.
         constexpr int kWide = DP >= 128 ? 16 : 8;
+        auto turned = [](int g, int i) {
+            return kWide * g + ((i + (DP >= 128 ? g >> 1 : g >> 2) * 2) & (kWide - 1));
+        };
         float* jo = reinterpret_cast<float*>(smem);
-        float* jm = jo + kWarps * kRows * H::kPitch;
+        float4* jm = reinterpret_cast<float4*>(smem + kWarps * kRows * H::kPitch * 4);
 #pragma unroll
         for (int b = 0; b < NB; ++b)
 #pragma unroll
@@ -680,57 +702,70 @@ k_attend(const __grid_constant__ Args a) {
                 float z = sum[b][e];
 #pragma unroll
                 for (int x = 4; x < 32; x <<= 1) z += __shfl_xor_sync(tbk::kFull, z, x);
-                const int i = warp * kRows + 8 * b + 2 * t + e;
-                float* row = jo + i * H::kPitch;
+                const int i = 8 * b + 2 * t + e;
+                float* row = jo + (warp * kRows + i) * H::kPitch;
 #pragma unroll
                 for (int u = 0; u < kTiles; ++u)
-                    *reinterpret_cast<float2*>(row + (u / 8) * 128 + kWide * g + 2 * (u % 8)) =
+                    *reinterpret_cast<float2*>(row + (u / 8) * 128 + turned(g, 2 * (u % 8))) =
                         make_float2(o[u][b][e], o[u][b][2 + e]);
-                if (g == 0) {
-                    jm[i * 3] = ref[b][e];
-                    jm[i * 3 + 1] = vref[b][e];
-                    jm[i * 3 + 2] = z;
-                }
+                if (g == 0) jm[i * kWarps + warp] = make_float4(ref[b][e], vref[b][e], z, 0.0f);
             }
         __syncthreads();
         const int64_t unit = 2 * (int64_t)blockIdx.x + !first_block;
-        for (int row = warp; row < blk.rows; row += kWarps) {
+        constexpr int kPerRow = kThreads / kRows;  // threads
+        const int row = threadIdx.x / kPerRow, col = threadIdx.x % kPerRow * 4;
+        if (row < blk.rows) {
+            float4 st[kWarps];
             float m = kNoRef, mv = kNoRef, total = 0.0f, w[kWarps];
 #pragma unroll
             for (int i = 0; i < kWarps; ++i) {
-                m = fmaxf(m, jm[(i * kRows + row) * 3]);
-                mv = fmaxf(mv, jm[(i * kRows + row) * 3 + 1]);
+                st[i] = jm[row * kWarps + i];
+                m = fmaxf(m, st[i].x);
+                mv = fmaxf(mv, st[i].y);
             }
 #pragma unroll
             for (int i = 0; i < kWarps; ++i) {
-                const float* st = jm + (i * kRows + row) * 3;
-                total += st[2] * exp2f(st[0] - m);
-                w[i] = exp2f(st[1] - mv);
+                total += st[i].z * kv8::exp2_fast(st[i].x - m);
+                w[i] = kv8::exp2_fast(st[i].y - mv);
             }
             const bool none = total == 0.0f;
             // O is in units of 2^(mv - lift), the sum of 2^m
-            const float per = none ? 0.0f : exp2f(-kLift) / total;
-            const float unit_v = none ? 0.0f : exp2f(mv - m);
+            const float per = none ? 0.0f : __fdiv_rn(1.0f / 2048.0f, total) * exp2f(mv - m);
+            static_assert(kLift == 11.0f, "per");
             const int at = block * kRows + row;
             const int64_t tok = load.s.lo + at / group;
             const int h = head * group + at % group;
             T* out = static_cast<T*>(a.out) + tok * a.out_stride + (int64_t)h * a.d;
             float* part = whole ? nullptr : a.part + (unit * kRows + row) * a.d;
-            for (int i = lane; i < a.d; i += 32) {
-                float y = 0.0f;
 #pragma unroll
-                for (int k = 0; k < kWarps; ++k) y += w[k] * jo[(k * kRows + row) * H::kPitch + i];
-                y = none ? 0.0f : y * per * unit_v;
+            for (int i = col; i < DP; i += 4 * kPerRow) {
+                if (i >= a.d) break;
+                float y[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int k = 0; k < kWarps; ++k) {
+                    const float* from = jo + (k * kRows + row) * H::kPitch + i / 128 * 128;
+                    const int g = i % 128 / kWide;
+#pragma unroll
+                    for (int e = 0; e < 4; e += 2) {
+                        const float2 v =
+                            *reinterpret_cast<const float2*>(from + turned(g, i % kWide + e));
+                        y[e] = fmaf(w[k], v.x, y[e]);
+                        y[e + 1] = fmaf(w[k], v.y, y[e + 1]);
+                    }
+                }
+#pragma unroll
+                for (int e = 0; e < 4; ++e) y[e] = none ? 0.0f : y[e] * per;
                 if (whole)
-                    tbk::Elt<T>::store(out + i, y);
+                    kv8::store4(out + i, a.vec_out, y);
                 else
-                    part[i] = y;
+                    *reinterpret_cast<float4*>(part + i) = make_float4(y[0], y[1], y[2], y[3]);
             }
-            if (lane == 0) {
+            if (col == 0) {
                 if (!whole)
                     a.state[unit * kRows + row] = make_float2(m, total);
                 else if (a.lse)
-                    a.lse[tok * a.hq + h] = none ? -INFINITY : m * 0.69314718055994531f + logf(total);
+                    a.lse[tok * a.hq + h] =
+                        none ? -INFINITY : m * 0.69314718055994531f + logf(total);
             }
         }
         // the next block's copies go where this one's states were read
@@ -741,13 +776,21 @@ k_attend(const __grid_constant__ Args a) {
 
 // Joins the blocks that a cut went through: out = sum_c w_c out_c / sum_c w_c,
 // w_c a part's sum at the largest reference.  The first cut through a block has
-// its CTA, a warp per row: the weights first, then the parts, eight loads in
-// flight, a lane four elements of 128.
-constexpr int kJoinWarps = 8;
+// the CTAs, each two of the block's rows; a row's four warps take every fourth
+// part, eight loads in flight, a lane four elements of 128.
+constexpr int kJoinWarps = 4;  // per row
+constexpr int kJoinRows = 2;
 template <typename T>
-__global__ void __launch_bounds__(32 * kJoinWarps) k_join(const __grid_constant__ Args a) {
-    __shared__ float w_s[kJoinWarps][kMostCtas];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+__global__ void __launch_bounds__(32 * kJoinWarps * kJoinRows)
+k_join(const __grid_constant__ Args a) {
+    __shared__ float2 st_s[kJoinRows][kMostCtas];
+    __shared__ float4 part_s[kJoinRows][kJoinWarps][kv8::kMaxDim / 4];
+    __shared__ float red[kJoinRows][2][kJoinWarps];
+    const int group_id = threadIdx.x / (32 * kJoinWarps);  // of the four warps of a row
+    const int tid = threadIdx.x % (32 * kJoinWarps), warp = tid >> 5, lane = tid & 31;
+    auto meet = [&] {
+        asm volatile("bar.sync %0, %1;" ::"r"(group_id + 1), "n"(32 * kJoinWarps) : "memory");
+    };
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const int c = blockIdx.x + 1;
     const Cut cut = a.cuts[c];
@@ -765,56 +808,73 @@ __global__ void __launch_bounds__(32 * kJoinWarps) k_join(const __grid_constant_
     auto at = [&](int p) { return p == 0 ? lone : 2 * (int64_t)(c - 1 + p); };
     const Load load = load_of(a, cut.seq);
     const Block blk = block_of(a, load, cut.block);
+    const int row = blockIdx.y * kJoinRows + group_id;
+    if (row >= blk.rows) return;
     const int group = a.hq / a.hkv, quads = a.d / 4;
-    for (int row = warp; row < blk.rows; row += kJoinWarps) {
-        float m = kNoRef, total = 0.0f;
-        for (int p = lane; p < parts; p += 32)
-            m = fmaxf(m, __ldcg(&a.state[at(p) * a.block_rows + row].x));
-        m = tbk::warp_max(m);
-        __syncwarp();
-        for (int p = lane; p < parts; p += 32) {
-            const float2 s = __ldcg(&a.state[at(p) * a.block_rows + row]);
-            const float w = s.y * exp2f(s.x - m);
-            w_s[warp][p] = w;
-            total += w;
-        }
-        total = tbk::warp_sum(total);
-        __syncwarp();
-        const bool none = total == 0.0f;
-        const int r = cut.block * a.block_rows + row;
-        const int64_t tok = load.s.lo + r / group;
-        const int h = cut.head * group + r % group;
-        T* out = static_cast<T*>(a.out) + tok * a.out_stride + (int64_t)h * a.d;
-        const float4* src = reinterpret_cast<const float4*>(a.part) + row * quads;
-        for (int i = lane; i < quads; i += 32) {
-            float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            for (int p0 = 0; p0 < parts; p0 += 8) {
-                float4 x[8];
-                float w[8];
-#pragma unroll
-                for (int u = 0; u < 8; ++u) {
-                    const int p = p0 + u;
-                    w[u] = p < parts ? w_s[warp][p] : 0.0f;
-                    x[u] = p < parts ? __ldcg(src + at(p) * a.block_rows * quads + i)
-                                     : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                }
-#pragma unroll
-                for (int u = 0; u < 8; ++u) {
-                    y.x = fmaf(w[u], x[u].x, y.x);
-                    y.y = fmaf(w[u], x[u].y, y.y);
-                    y.z = fmaf(w[u], x[u].z, y.z);
-                    y.w = fmaf(w[u], x[u].w, y.w);
-                }
-            }
-            tbk::Elt<T>::store(out + 4 * i, none ? 0.0f : y.x / total);
-            tbk::Elt<T>::store(out + 4 * i + 1, none ? 0.0f : y.y / total);
-            tbk::Elt<T>::store(out + 4 * i + 2, none ? 0.0f : y.z / total);
-            tbk::Elt<T>::store(out + 4 * i + 3, none ? 0.0f : y.w / total);
-        }
-        if (a.lse && lane == 0)
-            a.lse[tok * a.hq + h] = none ? -INFINITY : m * 0.69314718055994531f + logf(total);
-        __syncwarp();
+
+    float m = kNoRef;
+    for (int p = tid; p < parts; p += 32 * kJoinWarps) {
+        const float2 s = __ldcg(&a.state[at(p) * a.block_rows + row]);
+        st_s[group_id][p] = s;
+        m = fmaxf(m, s.x);
     }
+    m = tbk::warp_max(m);
+    if (lane == 0) red[group_id][0][warp] = m;
+    meet();
+#pragma unroll
+    for (int i = 0; i < kJoinWarps; ++i) m = fmaxf(m, red[group_id][0][i]);
+    float total = 0.0f;
+    for (int p = tid; p < parts; p += 32 * kJoinWarps) {
+        const float2 s = st_s[group_id][p];
+        const float w = s.y * kv8::exp2_fast(s.x - m);
+        st_s[group_id][p].x = w;
+        total += w;
+    }
+    total = tbk::warp_sum(total);
+    if (lane == 0) red[group_id][1][warp] = total;
+    meet();
+    total = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kJoinWarps; ++i) total += red[group_id][1][i];
+
+    const float4* src = reinterpret_cast<const float4*>(a.part) + row * quads;
+    for (int i = lane; i < quads; i += 32) {
+        float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        for (int p0 = warp; p0 < parts; p0 += 8 * kJoinWarps) {
+            float4 x[8];
+            float w[8];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) {
+                const int p = p0 + u * kJoinWarps;
+                w[u] = p < parts ? st_s[group_id][p].x : 0.0f;
+                x[u] = p < parts ? __ldcg(src + at(p) * a.block_rows * quads + i)
+                                 : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            }
+#pragma unroll
+            for (int u = 0; u < 8; ++u) {
+                y.x = fmaf(w[u], x[u].x, y.x);
+                y.y = fmaf(w[u], x[u].y, y.y);
+                y.z = fmaf(w[u], x[u].z, y.z);
+                y.w = fmaf(w[u], x[u].w, y.w);
+            }
+        }
+        part_s[group_id][warp][i] = y;
+    }
+    meet();
+    const bool none = total == 0.0f;
+    const int r = cut.block * a.block_rows + row;
+    const int64_t tok = load.s.lo + r / group;
+    const int h = cut.head * group + r % group;
+    T* out = static_cast<T*>(a.out) + tok * a.out_stride + (int64_t)h * a.d;
+    for (int i = tid; i < a.d; i += 32 * kJoinWarps) {
+        float z = 0.0f;
+#pragma unroll
+        for (int k = 0; k < kJoinWarps; ++k)
+            z += reinterpret_cast<const float*>(part_s[group_id][k])[i];
+        tbk::Elt<T>::store(out + i, none ? 0.0f : z / total);
+    }
+    if (a.lse && tid == 0)
+        a.lse[tok * a.hq + h] = none ? -INFINITY : m * 0.69314718055994531f + logf(total);
 }
 
 int check(const TbB200Kv8* cache, const TbB200Kv8Batch* batch, const TbB200Kv8Attention* t,
@@ -909,7 +969,7 @@ template <typename T>
 int join(const Args& a, dim3 grid, cudaStream_t s) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = grid;
-    cfg.blockDim = dim3(32 * kJoinWarps);
+    cfg.blockDim = dim3(32 * kJoinWarps * kJoinRows);
     cfg.stream = s;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -980,6 +1040,7 @@ extern "C" int tb_b200_kv8_attention(const TbB200Kv8* cache, const TbB200Kv8Batc
     a.block_rows = p.block_rows;
     a.whole = p.whole;
     a.vec = tbh::aligned16(t->q) && t->q_stride * s % 16 == 0;
+    a.vec_out = tbh::aligned16(t->out) && t->out_stride * s % 16 == 0;
     const dim3 grid((unsigned)p.ctas);
     cudaStream_t st = tbh::stream_of(stream);
     const bool f32 = t->dtype == TB_DTYPE_F32, int8 = cache->format == kv8::kInt8;
@@ -988,6 +1049,6 @@ extern "C" int tb_b200_kv8_attention(const TbB200Kv8* cache, const TbB200Kv8Batc
              : (int8 ? launch_rows<__nv_bfloat16, kv8::kInt8>(a, cache, grid, st)
                      : launch_rows<__nv_bfloat16, kv8::kE4m3>(a, cache, grid, st));
     if (rc != TB_OK || p.whole) return rc;
-    const dim3 joins((unsigned)p.ctas - 1);
+    const dim3 joins((unsigned)p.ctas - 1, (unsigned)(p.block_rows / kJoinRows));
     return f32 ? join<float>(a, joins, st) : join<__nv_bfloat16>(a, joins, st);
 }

@@ -146,9 +146,15 @@ struct QParts {
                 const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(r[2], r[3]),
                                                              __NV_SATFINITE, __NV_E4M3);
                 w[p] = lo | hi << 16;
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    r[i] = (r[i] - decode<kE4m3>((uint8_t)(w[p] >> 8 * i))) * 16.0f;
+                if (p + 1 < kParts) {
+                    const uint32_t a = e4m3_pair(w[p], false), b = e4m3_pair(w[p], true);
+                    const float2 u = __half22float2(*reinterpret_cast<const __half2*>(&a));
+                    const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&b));
+                    r[0] = (r[0] - u.x) * kRadix;
+                    r[1] = (r[1] - u.y) * kRadix;
+                    r[2] = (r[2] - v.x) * kRadix;
+                    r[3] = (r[3] - v.y) * kRadix;
+                }
             }
         }
     }
@@ -158,6 +164,10 @@ __device__ __forceinline__ float exp2_fast(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
+}
+
+__device__ __forceinline__ void prefetch_map(const CUtensorMap* map) {
+    asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
 }
 
 // One tile of a 3-D tensor map into shared memory, its bytes counted on bar.
@@ -187,6 +197,19 @@ __device__ __forceinline__ void load4(const T* p, bool live, bool vec, float (&v
         v[1] = __uint_as_float(w.x & 0xffff0000u);
         v[2] = __uint_as_float(w.y << 16);
         v[3] = __uint_as_float(w.y & 0xffff0000u);
+    }
+}
+
+template <typename T>
+__device__ __forceinline__ void store4(T* p, bool vec, const float (&v)[4]) {
+    if (!vec) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) tbk::Elt<T>::store(p + i, v[i]);
+    } else if constexpr (sizeof(T) == 4) {
+        tbk::store_vec<T, 4>(p, v);
+    } else {
+        *reinterpret_cast<uint2*>(p) =
+            make_uint2(tbk::pack_bf16x2(v[0], v[1]), tbk::pack_bf16x2(v[2], v[3]));
     }
 }
 
