@@ -693,37 +693,67 @@ def embedding_sharded_p2p(ids, shard_addrs, vocab: int, dim: int, dtype, y=None,
 
 
 # ------------------------- rotary positions, head norms, the 8-bit KV cache
-def _new(shape, dtype, device, stream):
-    """An uninitialised tensor for a call on `stream`: from that stream's pool, so that the
-    memory's earlier uses are ordered before the call and its later ones after it."""
+# These calls are a few microseconds of GPU work in a decode step, so their
+# checks are written to cost little: one look at each tensor's device, strides
+# and dtype.
+def _here():
+    """(torch, index of the current device), where a launch goes."""
     torch = _torch()
+    if not torch.cuda.is_initialized():
+        if not torch.cuda.is_available():
+            return torch, None  # no tensor is there
+        torch.cuda.init()
+    return torch, torch._C._cuda_getDevice()
+
+
+def _stream(torch, dev, stream):
+    return torch._C._cuda_getCurrentRawStream(dev) if stream is None else stream
+
+
+def _new(stream, make, *args, **kw):
+    """make(...), an uninitialised tensor for a call on `stream`: from that stream's pool, so
+    that the memory's earlier uses are ordered before the call and its later ones after it."""
     if stream is None:
-        return torch.empty(shape, dtype=dtype, device=device)
-    s = torch.cuda.ExternalStream(getattr(stream, "value", stream) or 0)
-    with torch.cuda.stream(s):
-        return torch.empty(shape, dtype=dtype, device=device)
+        return make(*args, **kw)
+    cuda = _torch().cuda
+    with cuda.stream(cuda.ExternalStream(getattr(stream, "value", stream) or 0)):
+        return make(*args, **kw)
 
 
-def _rows3(*ts):
-    """[rows, heads, head_dim] tensors whose heads are dense within a row."""
-    for t in ts:
-        if not t.is_cuda or t.dim() != 3 or (t.shape[2] > 1 and t.stride(2) != 1) or (
-                t.shape[1] > 1 and t.stride(1) != t.shape[2]):
-            raise ValueError("expected CUDA [rows, heads, head_dim] tensors, heads dense in a row")
+def _device_is(t, dev):
+    if t.get_device() != dev:
+        raise ValueError(f"expected a tensor on the current device cuda:{dev}, got {t.device}")
 
 
-def _here(*ts):
-    """Every tensor on the current device, where the launch goes."""
-    dev = _torch().cuda.current_device()
-    for t in ts:
-        if t is not None and t.device.index != dev:
-            raise ValueError(f"tensor on {t.device}, but the current device is cuda:{dev}")
+def _heads(t, dtype, shape, dev, what):
+    """Row stride of a [rows, heads, head_dim] tensor whose heads are dense
+    within a row."""
+    _device_is(t, dev)
+    if t.dtype is not dtype:
+        raise TypeError(f"{what} must be {dtype}, got {t.dtype}")
+    if t.shape != shape:
+        raise ValueError(f"{what} must be {tuple(shape)}, got {tuple(t.shape)}")
+    s0, s1, s2 = t.stride()
+    if (s2 != 1 and shape[2] > 1) or (s1 != shape[2] and shape[1] > 1):
+        raise ValueError(f"{what} must have its heads dense in a row")
+    return s0
 
 
-def _typed(what, dtype, *ts):
-    for t in ts:
-        if t is not None and t.dtype != dtype:
-            raise TypeError(f"{what} must be {dtype}, got {t.dtype}")
+def _flat(t, dtype, n, dev, what):
+    """Address of a contiguous tensor of n elements."""
+    _device_is(t, dev)
+    if t.dtype is not dtype:
+        raise TypeError(f"{what} must be {dtype}, got {t.dtype}")
+    if t.numel() != n or not t.is_contiguous():
+        raise ValueError(f"{what} must have {n} contiguous elements")
+    return t.data_ptr()
+
+
+def _heads_dtype(t):
+    code = dtype_code(t)
+    if code == I32 or t.dim() != 3:
+        raise ValueError("expected [rows, heads, head_dim] of float32 or bfloat16")
+    return code
 
 
 def rotary_freqs(rotary_dim, theta, scaling="none", factor=1.0, trained=0.0, low=0.0, high=0.0,
@@ -731,46 +761,49 @@ def rotary_freqs(rotary_dim, theta, scaling="none", factor=1.0, trained=0.0, low
     """Angle per position of each of rotary_dim / 2 pairs (float64, on the
     device), stretched by `scaling`: "none", "linear", "ntk", "bands" or
     "yarn" (tb_b200_rotary_freqs)."""
-    torch = _torch()
+    torch, dev = _here()
+    n = rotary_dim // 2
     if out is None:
-        out = _new(rotary_dim // 2, torch.float64, "cuda", stream)
-    _dev(out)
-    _here(out)
-    _typed("out", torch.float64, out)
-    if out.numel() != rotary_dim // 2:
-        raise ValueError("out must have rotary_dim / 2 elements")
+        out = _new(stream, torch.empty, n, dtype=torch.float64, device="cuda")
+    at = _flat(out, torch.float64, n, dev, "out")
     sc = RotaryScaling(ROTARY_SCALING[scaling], theta, factor, trained, low, high)
-    check(lib().tb_b200_rotary_freqs(rotary_dim, C.byref(sc), ptr(out), stream or cur_stream()),
+    check(lib().tb_b200_rotary_freqs(rotary_dim, sc, at, _stream(torch, dev, stream)),
           "rotary_freqs")
     return out
 
 
-def _rotary(fn, what, q, k, q_weight, k_weight, eps, positions, freqs, layout, scale, q_out,
-            k_out, stream):
-    torch = _torch()
-    q_out = _new(q.shape, q.dtype, q.device, stream) if q_out is None else q_out
-    k_out = _new(k.shape, k.dtype, k.device, stream) if k_out is None else k_out
-    _rows3(q, k, q_out, k_out)
-    _dev(positions, freqs, q_weight, k_weight)
-    _here(q, k, q_out, k_out, positions, freqs, q_weight, k_weight)
-    _typed("k, the outputs and the weights", q.dtype, k, q_out, k_out, q_weight, k_weight)
-    _typed("positions", torch.int32, positions)
-    _typed("freqs", torch.float64, freqs)
-    rows, hq, d = q.shape
-    if k.shape[0] != rows or k.shape[2] != d or q_out.shape != q.shape or k_out.shape != k.shape:
-        raise ValueError("q, k and the outputs do not agree in rows or head_dim")
-    if freqs is not None and (positions is None or positions.numel() != rows):
-        raise ValueError("positions must have one element per row")
-    if any(w is not None and w.numel() != d for w in (q_weight, k_weight)):
-        raise ValueError("a norm weight must have head_dim elements")
-    t = Rotary(dtype_code(q), rows, hq, k.shape[1], d, 0 if freqs is None else 2 * freqs.numel(),
-               layout, q.data_ptr(), q.stride(0), k.data_ptr(), k.stride(0), q_out.data_ptr(),
-               q_out.stride(0), k_out.data_ptr(), k_out.stride(0),
-               None if positions is None else positions.data_ptr(),
-               None if freqs is None else freqs.data_ptr(), scale,
-               None if q_weight is None else q_weight.data_ptr(),
-               None if k_weight is None else k_weight.data_ptr(), eps)
-    check(getattr(lib(), fn)(C.byref(t), stream or cur_stream()), what)
+def _rotary(fn, q, k, q_weight, k_weight, eps, positions, freqs, layout, scale, q_out, k_out,
+            stream):
+    torch, dev = _here()
+    dtype, code = q.dtype, _heads_dtype(q)
+    q_shape, k_shape = q.shape, k.shape
+    rows, hq, d = q_shape
+    if len(k_shape) != 3 or k_shape[0] != rows or k_shape[2] != d:
+        raise ValueError("q and k must agree in rows and head_dim")
+    hkv = k_shape[1]
+    qs = _heads(q, dtype, q_shape, dev, "q")
+    ks = _heads(k, dtype, k_shape, dev, "k")
+    dense = torch.contiguous_format
+    if q_out is None:
+        q_out, qos = _new(stream, torch.empty_like, q, memory_format=dense), hq * d
+    else:
+        qos = _heads(q_out, dtype, q_shape, dev, "q_out")
+    if k_out is None:
+        k_out, kos = _new(stream, torch.empty_like, k, memory_format=dense), hkv * d
+    else:
+        kos = _heads(k_out, dtype, k_shape, dev, "k_out")
+    r, at, fr = 0, None, None
+    if freqs is not None:
+        if positions is None:
+            raise ValueError("freqs without positions")
+        r = 2 * freqs.numel()
+        at = _flat(positions, torch.int32, rows, dev, "positions")
+        fr = _flat(freqs, torch.float64, r // 2, dev, "freqs")
+    qw = None if q_weight is None else _flat(q_weight, dtype, d, dev, "q_weight")
+    kw = None if k_weight is None else _flat(k_weight, dtype, d, dev, "k_weight")
+    t = Rotary(code, rows, hq, hkv, d, r, layout, q.data_ptr(), qs, k.data_ptr(), ks,
+               q_out.data_ptr(), qos, k_out.data_ptr(), kos, at, fr, scale, qw, kw, eps)
+    check(fn(t, _stream(torch, dev, stream)), "rotary")
     return q_out, k_out
 
 
@@ -780,8 +813,8 @@ def rotary(q, k, positions, freqs, layout=ROTARY_HALF, scale=1.0, q_out=None, k_
     strided (slices of a packed QKV): the first 2 * freqs.numel() elements of
     each head, at int32 positions [R] (tb_b200_rotary).  New tensors unless
     q_out and k_out are given; those may be q and k themselves."""
-    return _rotary("tb_b200_rotary", "rotary", q, k, None, None, 0.0, positions, freqs, layout,
-                   scale, q_out, k_out, stream)
+    return _rotary(lib().tb_b200_rotary, q, k, None, None, 0.0, positions, freqs, layout, scale,
+                   q_out, k_out, stream)
 
 
 def qk_norm_rotary(q, k, q_weight, k_weight, eps, positions=None, freqs=None,
@@ -789,8 +822,8 @@ def qk_norm_rotary(q, k, q_weight, k_weight, eps, positions=None, freqs=None,
     """RMSNorm of each head of q and k (weights [d] or None), then rotary
     positions, in one pass (tb_b200_qk_norm_rotary); without freqs the norm
     alone."""
-    return _rotary("tb_b200_qk_norm_rotary", "qk_norm_rotary", q, k, q_weight, k_weight, eps,
-                   positions, freqs, layout, scale, q_out, k_out, stream)
+    return _rotary(lib().tb_b200_qk_norm_rotary, q, k, q_weight, k_weight, eps, positions, freqs,
+                   layout, scale, q_out, k_out, stream)
 
 
 class Kv8Cache:
@@ -800,19 +833,20 @@ class Kv8Cache:
 
     def __init__(self, k, v, k_scale, v_scale):
         torch = _torch()
-        _dev(k, v, k_scale, v_scale)
-        if k.dtype not in (torch.int8, torch.float8_e4m3fn):
-            raise TypeError(f"codes must be int8 or float8_e4m3fn, got {k.dtype}")
-        _typed("v", k.dtype, v)
-        _typed("scales", torch.float32, k_scale, v_scale)
-        if k.dim() != 4 or v.shape != k.shape or k_scale.shape != k.shape[:2] or (
-                v_scale.shape != k.shape[:2]):
-            raise ValueError("codes are [n_pages, n_kv_heads, page, head_dim], scales their first "
-                             "two dimensions")
-        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
-        self.c = Kv8(KV_INT8 if k.dtype == torch.int8 else KV_E4M3, k.shape[2], k.shape[1],
-                     k.shape[3], k.shape[0], k.data_ptr(), v.data_ptr(), k_scale.data_ptr(),
-                     v_scale.data_ptr())
+        dtype, shape, dev = k.dtype, k.shape, k.get_device()
+        if dtype is not torch.int8 and dtype is not torch.float8_e4m3fn:
+            raise TypeError(f"codes must be int8 or float8_e4m3fn, got {dtype}")
+        if dev < 0 or len(shape) != 4:
+            raise ValueError("codes are CUDA tensors [n_pages, n_kv_heads, page, head_dim]")
+        pages, heads, page, d = shape
+        n, ns = pages * heads * page * d, pages * heads
+        if v.shape != shape:
+            raise ValueError("k and v must have the same shape")
+        self.k, self.v, self.k_scale, self.v_scale, self.device = k, v, k_scale, v_scale, dev
+        self.c = Kv8(KV_INT8 if dtype is torch.int8 else KV_E4M3, page, heads, d, pages,
+                     _flat(k, dtype, n, dev, "k"), _flat(v, dtype, n, dev, "v"),
+                     _flat(k_scale, torch.float32, ns, dev, "k_scale"),
+                     _flat(v_scale, torch.float32, ns, dev, "v_scale"))
 
     @classmethod
     def empty(cls, n_pages, n_kv_heads, page, head_dim, dtype, device=None):
@@ -826,34 +860,34 @@ class Kv8Cache:
         return cls(*codes, *scales)
 
 
-def _kv8_batch(cache, rows, row_start, lengths, page_table):
-    torch = _torch()
-    _dev(row_start, lengths)
-    _typed("row_start, lengths and page_table", torch.int32, row_start, lengths, page_table)
-    if not page_table.is_cuda or page_table.dim() != 2 or (
-            page_table.shape[1] > 1 and page_table.stride(1) != 1):
-        raise ValueError("page_table must be a CUDA [n_seqs, pages] tensor, dense in a row")
-    _here(cache.k, row_start, lengths, page_table)
+def _kv8_batch(torch, cache, dev, rows, row_start, lengths, page_table):
+    i32_ = torch.int32
+    if cache.device != dev:
+        raise ValueError(f"the cache is on cuda:{cache.device}, the current device is cuda:{dev}")
+    _device_is(page_table, dev)
+    if page_table.dtype is not i32_:
+        raise TypeError(f"page_table must be int32, got {page_table.dtype}")
     n, width = page_table.shape
-    if row_start.numel() != n + 1 or lengths.numel() != n:
-        raise ValueError("row_start has n_seqs + 1 elements, lengths n_seqs")
-    return Kv8Batch(n, rows, row_start.data_ptr(), lengths.data_ptr(), page_table.data_ptr(),
-                    width, max(page_table.stride(0), width))
+    s0, s1 = page_table.stride()
+    if s1 != 1 and width > 1:
+        raise ValueError("page_table must be [n_seqs, pages], dense in a row")
+    return Kv8Batch(n, rows, _flat(row_start, i32_, n + 1, dev, "row_start"),
+                    _flat(lengths, i32_, n, dev, "lengths"), page_table.data_ptr(), width,
+                    s0 if n > 1 else width)
 
 
 def kv8_append(cache, k, v, row_start, lengths, page_table, stream=None):
     """Store K and V rows [R, n_kv_heads, head_dim] (rows may be strided) as
     the last tokens of the sequences of a ragged batch (tb_b200_kv8_append):
     rows row_start[i] : row_start[i + 1] end sequence i at lengths[i] tokens."""
-    _rows3(k, v)
-    _here(k, v)
-    _typed("v", k.dtype, v)
-    if k.shape != v.shape or k.shape[1:] != (cache.c.n_kv_heads, cache.c.head_dim):
+    torch, dev = _here()
+    dtype, code, shape = k.dtype, _heads_dtype(k), k.shape
+    if shape[1] != cache.c.n_kv_heads or shape[2] != cache.c.head_dim:
         raise ValueError("k and v must be [rows, n_kv_heads, head_dim] of the cache")
-    b = _kv8_batch(cache, k.shape[0], row_start, lengths, page_table)
-    check(lib().tb_b200_kv8_append(C.byref(cache.c), C.byref(b), dtype_code(k), k.data_ptr(),
-                                   k.stride(0), v.data_ptr(), v.stride(0),
-                                   stream or cur_stream()), "kv8_append")
+    ks, vs = _heads(k, dtype, shape, dev, "k"), _heads(v, dtype, shape, dev, "v")
+    b = _kv8_batch(torch, cache, dev, shape[0], row_start, lengths, page_table)
+    check(lib().tb_b200_kv8_append(cache.c, b, code, k.data_ptr(), ks, v.data_ptr(), vs,
+                                   _stream(torch, dev, stream)), "kv8_append")
 
 
 def kv8_attention(cache, q, row_start, lengths, page_table, max_q=None, max_len=None, scale=None,
@@ -863,40 +897,43 @@ def kv8_attention(cache, q, row_start, lengths, page_table, max_q=None, max_len=
     of one sequence (as many as q and page_table hold without them); scale is
     1 / sqrt(head_dim) unless given; window > 0 attends that many last keys.
     Returns out, or (out, lse) with return_lse or lse."""
-    torch = _torch()
+    torch, dev = _here()
+    dtype, code, shape = q.dtype, _heads_dtype(q), q.shape
+    rows, heads, d = shape
+    if d != cache.c.head_dim:
+        raise ValueError("q must be [rows, n_heads, head_dim] of the cache")
+    qs = _heads(q, dtype, shape, dev, "q")
+    dense = torch.contiguous_format
     if out is None:
-        out = _new(q.shape, q.dtype, q.device, stream)
-    _rows3(q, out)
-    _typed("out", q.dtype, out)
-    rows, heads, d = q.shape
-    if out.shape != q.shape or d != cache.c.head_dim:
-        raise ValueError("q and out must be [rows, n_heads, head_dim] of the cache")
-    if lse is None and return_lse:
-        lse = _new((rows, heads), torch.float32, q.device, stream)
+        out, os_ = _new(stream, torch.empty_like, q, memory_format=dense), heads * d
+    else:
+        os_ = _heads(out, dtype, shape, dev, "out")
+    ls = None
     if lse is not None:
-        _dev(lse)
-        _typed("lse", torch.float32, lse)
-        if lse.shape != (rows, heads):
+        if lse.shape != shape[:2]:
             raise ValueError("lse must be [rows, n_heads]")
-    _here(q, out, lse, workspace)
-    b = _kv8_batch(cache, rows, row_start, lengths, page_table)
-    a = Kv8Attention(dtype_code(q), heads, q.data_ptr(), q.stride(0), out.data_ptr(),
-                     out.stride(0), None if lse is None else lse.data_ptr(),
+        ls = _flat(lse, torch.float32, rows * heads, dev, "lse")
+    elif return_lse:
+        lse = _new(stream, q.new_empty, (rows, heads), dtype=torch.float32)
+        ls = lse.data_ptr()
+    b = _kv8_batch(torch, cache, dev, rows, row_start, lengths, page_table)
+    a = Kv8Attention(code, heads, q.data_ptr(), qs, out.data_ptr(), os_, ls,
                      d ** -0.5 if scale is None else scale, window,
                      rows if max_q is None else max_q,
                      b.table_width * cache.c.page if max_len is None else max_len, None, 0)
-    L = lib()
-    need = C.c_size_t()
-    check(L.tb_b200_kv8_attention_workspace(C.byref(cache.c), C.byref(b), C.byref(a),
-                                            C.byref(need)), "kv8_attention_workspace")
-    if workspace is None and need.value:
-        workspace = _new(need.value, torch.uint8, q.device, stream)
+    L, need = lib(), C.c_size_t()
+    if workspace is None:
+        check(L.tb_b200_kv8_attention_workspace(cache.c, b, a, need), "kv8_attention_workspace")
+        if need.value:
+            workspace = _new(stream, q.new_empty, need.value, dtype=torch.uint8)
+    else:
+        _device_is(workspace, dev)
+        if not workspace.is_contiguous():
+            raise ValueError("workspace must be contiguous")
     if workspace is not None:
-        _dev(workspace)
         a.workspace = workspace.data_ptr()
         a.workspace_bytes = workspace.numel() * workspace.element_size()
-    check(L.tb_b200_kv8_attention(C.byref(cache.c), C.byref(b), C.byref(a),
-                                  stream or cur_stream()), "kv8_attention")
+    check(L.tb_b200_kv8_attention(cache.c, b, a, _stream(torch, dev, stream)), "kv8_attention")
     return out if lse is None else (out, lse)
 
 
