@@ -9,16 +9,23 @@
 // general scale (amax / MAX) would save up to one bit of int8's range (none of
 // e4m3's) but let each of a page's up to page - 1 rescalings add half a step.
 //
-// HBM bound: the rows read once, one byte an element written.  One CTA per
-// (page that gets rows, head, K or V); which pages those are is on the device,
-// so the grid has a slot for each page that could: a sequence's rows from s to
-// e touch at most e / page - s / page + 2 pages, so sequence i's slots start at
-// row_start[i] / page + 2 i, which a CTA finds its sequence by.
+// HBM bound: the rows read once, one byte an element written.  A unit is (page
+// that gets rows, head, K or V); which pages those are is on the device, so the
+// grid has a slot for each page that could: a sequence's rows from s to e touch at
+// most e / page - s / page + 2 pages, so sequence i's slots start at row_start[i] /
+// page + 2 i, which a warp finds its sequence by, 32 candidates at a time.
+//
+// A unit has a CTA of 8 warps when its page is filled by a prompt, one warp (and a
+// CTA 8 heads) when a call brings few rows a sequence: then the time is the chain
+// of loads that leads to the rows, and a token's 16 vectors of a head need no more
+// lanes.  The rows stay in registers between amax and the codes, up to kHold
+// vectors a thread; what is past that is read again.
 #include "kv8.cuh"
 
 namespace {
 
-constexpr int kThreads = 128;
+constexpr int kThreads = 256;
+constexpr int kHold = 8;
 constexpr float kLeastScale = 7.8886090522101181e-31f;  // 2^-100
 
 template <int FORMAT>
@@ -41,79 +48,213 @@ struct Args {
     int hkv, d;
 };
 
-template <typename T, int FORMAT>
-__global__ void __launch_bounds__(kThreads) k_append(const __grid_constant__ Args a) {
-    __shared__ float red[32];
-    __shared__ int bad;
-    const kv8::Batch& b = a.b;
-    const int slot = blockIdx.x, head = blockIdx.y, page = 1 << b.page_shift;
-    // the last sequence whose slots start at or before this one
-    int lo = 0, hi = b.n_seqs - 1;
-    while (lo < hi) {
-        const int mid = (lo + hi + 1) >> 1;
-        const int start = min(max(b.row_start[mid], 0), b.rows);
-        if ((start >> b.page_shift) + 2 * mid <= slot)
-            lo = mid;
-        else
-            hi = mid - 1;
+// V elements of a row: their largest magnitude (as bits, which order like the
+// values; NaN and infinity are kInf or above) and their codes.
+template <typename T, int V>
+struct Piece {
+    T e[V];
+    static __device__ Piece load(const T* p) {
+        Piece x;
+#pragma unroll
+        for (int i = 0; i < V; ++i) x.e[i] = p[i];
+        return x;
     }
-    const kv8::Seq s = kv8::sequence(b, lo);
+    __device__ float at(int i) const { return tbk::Elt<T>::load(&e[i]); }
+};
+template <>
+struct Piece<float, 4> {
+    uint4 w;
+    static __device__ Piece load(const float* p) {
+        return {__ldcs(reinterpret_cast<const uint4*>(p))};
+    }
+    __device__ float at(int i) const { return __uint_as_float((&w.x)[i]); }
+};
+template <>
+struct Piece<__nv_bfloat16, 8> {
+    uint4 w;
+    static __device__ Piece load(const __nv_bfloat16* p) {
+        return {__ldcs(reinterpret_cast<const uint4*>(p))};
+    }
+    __device__ float at(int i) const {
+        const uint32_t x = (&w.x)[i / 2];
+        return __uint_as_float(i % 2 ? x & 0xffff0000u : x << 16);
+    }
+};
+
+constexpr uint32_t kInf = 0x7f800000u;
+
+template <typename T, int V>
+__device__ __forceinline__ uint32_t top_of(const Piece<T, V>& x) {
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < V; ++i) top = max(top, __float_as_uint(x.at(i)) & 0x7fffffffu);
+    return top;
+}
+
+template <int FORMAT, typename T, int V>
+__device__ __forceinline__ void store_codes(uint8_t* p, const Piece<T, V>& x, float per) {
+    constexpr float most = FORMAT == kv8::kInt8 ? 127.0f : 448.0f;
+    uint32_t w[(V + 3) / 4] = {};
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        float v = x.at(i) * per;
+        v = v != v ? 0.0f : fminf(fmaxf(v, -most), most);
+        w[i / 4] |= (uint32_t)kv8::encode<FORMAT>(v) << 8 * (i % 4);
+    }
+    if constexpr (V == 8)
+        *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
+    else if constexpr (V == 4)
+        *reinterpret_cast<uint32_t*>(p) = w[0];
+    else
+        *p = (uint8_t)w[0];
+}
+
+template <typename T, int FORMAT, int V, int WARPS>  // WARPS of a unit
+__global__ void __launch_bounds__(kThreads) k_append(const __grid_constant__ Args a) {
+    __shared__ uint32_t red[kThreads / 32];
+    constexpr int kUnit = 32 * WARPS;  // threads
+    const kv8::Batch& b = a.b;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, tid = threadIdx.x % kUnit;
+    const int slot = blockIdx.x, page = 1 << b.page_shift;
+    const int head = blockIdx.y * (kThreads / kUnit) + threadIdx.x / kUnit;
+    if (head >= a.hkv) return;  // whole warps of units of one warp
+    // the last sequence whose slots start at or before this one
+    int seq = 0;
+    for (int n = b.n_seqs; n > 1;) {  // it is in [seq, seq + n)
+        const int step = (n + 31) / 32, i = seq + lane * step;
+        const bool before =
+            lane * step < n &&
+            (min(max(b.row_start[i], 0), b.rows) >> b.page_shift) + 2 * i <= slot;
+        const int last = 31 - __clz(__ballot_sync(tbk::kFull, before) | 1);
+        seq += last * step;
+        n = min(step, n - last * step);
+    }
+    const kv8::Seq s = kv8::sequence(b, seq);
     const int first = max(s.first, 0);  // rows before position 0 are padding
-    const int logical = (first >> b.page_shift) + slot - ((s.lo >> b.page_shift) + 2 * lo);
+    const int logical = (first >> b.page_shift) + slot - ((s.lo >> b.page_shift) + 2 * seq);
     const int64_t begin = (int64_t)logical << b.page_shift;
     if (s.n == 0 || logical < 0 || begin >= s.len) return;
     if (logical >= b.width) {
-        if (threadIdx.x == 0) atomicOr(a.status, TB_B200_FLAG_POSITION_RANGE);
+        if (tid == 0) atomicOr(a.status, TB_B200_FLAG_POSITION_RANGE);
         return;
     }
-    const int id = b.table[lo * b.table_stride + logical];
-    if (id < 0 || id >= b.n_pages) {
-        if (threadIdx.x == 0) atomicOr(a.status, TB_B200_FLAG_PAGE_RANGE);
-        return;
-    }
-    const bool is_v = blockIdx.z != 0;
-    const int64_t stride = is_v ? a.v_stride : a.k_stride;
-    const T* x = static_cast<const T*>(is_v ? a.v : a.k) + (int64_t)head * a.d;
-    uint8_t* codes = (is_v ? a.v_codes : a.k_codes) +
-                     (((int64_t)id * a.hkv + head) << b.page_shift) * a.d;
-    float* scale = (is_v ? a.v_scale : a.k_scale) + (int64_t)id * a.hkv + head;
+    const int id = b.table[seq * b.table_stride + logical];
     // slots [from, to) of the page are new; slot from is row `row`
     const int from = max(first - (int)begin, 0);
     const int to = (int)min((int64_t)page, s.len - begin);
     const int row = s.lo + (int)(begin + from - s.first);
-    const int n = (to - from) * a.d;
-    if (threadIdx.x == 0) bad = 0;
-    __syncthreads();
+    const bool is_v = blockIdx.z != 0;
+    const int64_t stride = is_v ? a.v_stride : a.k_stride;
+    const T* x = static_cast<const T*>(is_v ? a.v : a.k) + row * stride + (int64_t)head * a.d;
 
-    float amax = 0.0f;
-    bool finite = true;
-    for (int i = threadIdx.x; i < n; i += kThreads) {
-        const float v = fabsf(tbk::Elt<T>::load(x + (row + i / a.d) * stride + i % a.d));
-        if (v < INFINITY)
-            amax = fmaxf(amax, v);
-        else
-            finite = false;
+    // pieces tid, tid + kUnit, .. of the new rows, `per_row` of them a row
+    const int per_row = a.d / V, n = (to - from) * per_row;
+    const int down = kUnit / per_row, right = kUnit % per_row;
+    const int r0 = tid / per_row, c0 = tid % per_row;
+    Piece<T, V> hold[kHold];
+    uint32_t top = 0;
+    int r = r0, c = c0;
+    auto next = [&] {
+        r += down;
+        c += right;
+        if (c >= per_row) {
+            c -= per_row;
+            ++r;
+        }
+    };
+#pragma unroll
+    for (int u = 0; u < kHold; ++u) {
+        if (tid + u * kUnit < n) hold[u] = Piece<T, V>::load(x + r * stride + c * V);
+        next();
     }
-    if (!finite) bad = 1;
-    amax = tbk::block_max(amax, red);
+    const int r_rest = r, c_rest = c;
+    if (id < 0 || id >= b.n_pages) {
+        if (tid == 0) atomicOr(a.status, TB_B200_FLAG_PAGE_RANGE);
+        return;
+    }
+    uint8_t* codes = (is_v ? a.v_codes : a.k_codes) +
+                     (((int64_t)id * a.hkv + head) << b.page_shift) * a.d;
+    float* scale = (is_v ? a.v_scale : a.k_scale) + (int64_t)id * a.hkv + head;
     const float old = from > 0 ? *scale : 0.0f;
-    const float now = fmaxf(scale_for<FORMAT>(amax), old);
-    const float most = FORMAT == kv8::kInt8 ? 127.0f : 448.0f;
-    if (now > old && from > 0) {
+#pragma unroll
+    for (int u = 0; u < kHold; ++u)
+        if (tid + u * kUnit < n) top = max(top, top_of(hold[u]));
+    for (int i = tid + kHold * kUnit; i < n; i += kUnit) {
+        top = max(top, top_of(Piece<T, V>::load(x + r * stride + c * V)));
+        next();
+    }
+    auto over_unit = [&](uint32_t v) {
+        v = __reduce_max_sync(tbk::kFull, v);
+        if (WARPS == 1) return v;
+        __syncthreads();
+        if (lane == 0) red[warp] = v;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < WARPS; ++i) v = max(v, red[i]);
+        return v;
+    };
+    top = over_unit(top);
+    if (top >= kInf) {  // the largest of the finite ones
+        if (tid == 0) atomicOr(a.status, TB_B200_FLAG_NONFINITE);
+        top = 0;
+        r = r0;
+        c = c0;
+        for (int i = tid; i < n; i += kUnit) {
+            const Piece<T, V> y = Piece<T, V>::load(x + r * stride + c * V);
+            for (int e = 0; e < V; ++e) {
+                const uint32_t bits = __float_as_uint(y.at(e)) & 0x7fffffffu;
+                if (bits < kInf) top = max(top, bits);
+            }
+            next();
+        }
+        top = over_unit(top);
+    }
+    const float now = fmaxf(scale_for<FORMAT>(__uint_as_float(top)), old);
+    if (now > old && from > 0) {  // 16 codes at a time: d is a multiple of 16
         const float ratio = old / now;
-        for (int i = threadIdx.x; i < from * a.d; i += kThreads)
-            codes[i] = kv8::encode<FORMAT>(kv8::decode<FORMAT>(codes[i]) * ratio);
+        for (int i = tid; i < from * a.d / 16; i += kUnit) {
+            uint4 w = reinterpret_cast<uint4*>(codes)[i];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                uint32_t y = 0;
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    y |= (uint32_t)kv8::encode<FORMAT>(
+                             kv8::decode<FORMAT>((uint8_t)((&w.x)[j] >> 8 * e)) * ratio)
+                         << 8 * e;
+                (&w.x)[j] = y;
+            }
+            reinterpret_cast<uint4*>(codes)[i] = w;
+        }
     }
     const float per = 1.0f / now;  // both powers of two: exact
-    for (int i = threadIdx.x; i < n; i += kThreads) {
-        float v = tbk::Elt<T>::load(x + (row + i / a.d) * stride + i % a.d) * per;
-        v = v != v ? 0.0f : fminf(fmaxf(v, -most), most);
-        codes[from * a.d + i] = kv8::encode<FORMAT>(v);
+    r = r0;
+    c = c0;
+#pragma unroll
+    for (int u = 0; u < kHold; ++u) {
+        if (tid + u * kUnit < n)
+            store_codes<FORMAT>(codes + (from + r) * a.d + c * V, hold[u], per);
+        next();
     }
-    __syncthreads();  // every thread has read *scale
-    if (threadIdx.x == 0) {
-        *scale = now;
-        if (bad) atomicOr(a.status, TB_B200_FLAG_NONFINITE);
+    r = r_rest;
+    c = c_rest;
+    for (int i = tid + kHold * kUnit; i < n; i += kUnit) {
+        store_codes<FORMAT>(codes + (from + r) * a.d + c * V,
+                            Piece<T, V>::load(x + r * stride + c * V), per);
+        next();
+    }
+    if (WARPS == 1) __syncwarp();  // every thread has read *scale (else: over_unit's barriers)
+    if (tid == 0) *scale = now;
+}
+
+template <typename T, int FORMAT, int V>
+void launch(const Args& a, bool warps, unsigned slots, cudaStream_t s) {
+    if (warps) {
+        const unsigned heads = (unsigned)(a.hkv + kThreads / 32 - 1) / (kThreads / 32);
+        k_append<T, FORMAT, V, 1><<<dim3(slots, heads, 2), kThreads, 0, s>>>(a);
+    } else {
+        k_append<T, FORMAT, V, kThreads / 32>
+            <<<dim3(slots, (unsigned)a.hkv, 2), kThreads, 0, s>>>(a);
     }
 }
 
@@ -136,18 +277,28 @@ extern "C" int tb_b200_kv8_append(const TbB200Kv8* cache, const TbB200Kv8Batch* 
                     static_cast<uint8_t*>(cache->k), static_cast<uint8_t*>(cache->v),
                     cache->k_scale, cache->v_scale, ds->status, cache->n_kv_heads,
                     cache->head_dim};
-    const dim3 grid((unsigned)(batch->rows / cache->page + 2 * batch->n_seqs),
-                    (unsigned)cache->n_kv_heads, 2);
+    const unsigned slots = (unsigned)(batch->rows / cache->page + 2 * batch->n_seqs);
+    // One warp a unit when a sequence brings so few rows that kHold vectors a lane
+    // hold them (bf16: rows * d <= 2048 elements).
+    const size_t size = dtype == TB_DTYPE_F32 ? 4 : 2;
+    const bool warps = batch->rows * cache->head_dim * (int64_t)size <=
+                       (int64_t)batch->n_seqs * 32 * kHold * 16;
+    const bool vec = tbh::aligned16(k) && tbh::aligned16(v) && k_stride * size % 16 == 0 &&
+                     v_stride * size % 16 == 0;
     cudaStream_t s = tbh::stream_of(stream);
     const bool f32 = dtype == TB_DTYPE_F32, int8 = cache->format == kv8::kInt8;
     if (f32 && int8)
-        k_append<float, kv8::kInt8><<<grid, kThreads, 0, s>>>(a);
+        vec ? launch<float, kv8::kInt8, 4>(a, warps, slots, s)
+            : launch<float, kv8::kInt8, 1>(a, warps, slots, s);
     else if (f32)
-        k_append<float, kv8::kE4m3><<<grid, kThreads, 0, s>>>(a);
+        vec ? launch<float, kv8::kE4m3, 4>(a, warps, slots, s)
+            : launch<float, kv8::kE4m3, 1>(a, warps, slots, s);
     else if (int8)
-        k_append<__nv_bfloat16, kv8::kInt8><<<grid, kThreads, 0, s>>>(a);
+        vec ? launch<__nv_bfloat16, kv8::kInt8, 8>(a, warps, slots, s)
+            : launch<__nv_bfloat16, kv8::kInt8, 1>(a, warps, slots, s);
     else
-        k_append<__nv_bfloat16, kv8::kE4m3><<<grid, kThreads, 0, s>>>(a);
+        vec ? launch<__nv_bfloat16, kv8::kE4m3, 8>(a, warps, slots, s)
+            : launch<__nv_bfloat16, kv8::kE4m3, 1>(a, warps, slots, s);
     TB_LAUNCH_CHECK("8-bit cache append kernel");
     return TB_OK;
 }
