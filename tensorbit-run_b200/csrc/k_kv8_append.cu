@@ -19,13 +19,12 @@
 // CTA 8 heads) when a call brings few rows a sequence: then the time is the chain
 // of loads that leads to the rows, and a token's 16 vectors of a head need no more
 // lanes.  The rows stay in registers between amax and the codes, up to kHold
-// vectors a thread; what is past that is read again.
+// vectors a thread (a page of 64 rows of 128); what is past that is read again.
 #include "kv8.cuh"
 
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kHold = 8;
 constexpr float kLeastScale = 7.8886090522101181e-31f;  // 2^-100
 
 template <int FORMAT>
@@ -83,6 +82,8 @@ struct Piece<__nv_bfloat16, 8> {
 
 constexpr uint32_t kInf = 0x7f800000u;
 
+constexpr int hold_of(size_t size, int warps) { return warps == 1 || size == 4 ? 8 : 4; }
+
 template <typename T, int V>
 __device__ __forceinline__ uint32_t top_of(const Piece<T, V>& x) {
     uint32_t top = 0;
@@ -110,26 +111,33 @@ __device__ __forceinline__ void store_codes(uint8_t* p, const Piece<T, V>& x, fl
 }
 
 template <typename T, int FORMAT, int V, int WARPS>  // WARPS of a unit
-__global__ void __launch_bounds__(kThreads) k_append(const __grid_constant__ Args a) {
+__global__ void __launch_bounds__(kThreads, hold_of(sizeof(T), WARPS) == 4 ? 5 : 3) k_append(const __grid_constant__ Args a) {
     __shared__ uint32_t red[kThreads / 32];
     constexpr int kUnit = 32 * WARPS;  // threads
+    constexpr int kHold = hold_of(sizeof(T), WARPS);
     const kv8::Batch& b = a.b;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, tid = threadIdx.x % kUnit;
     const int slot = blockIdx.x, page = 1 << b.page_shift;
     const int head = blockIdx.y * (kThreads / kUnit) + threadIdx.x / kUnit;
     if (head >= a.hkv) return;  // whole warps of units of one warp
-    // the last sequence whose slots start at or before this one
+    // the last sequence whose slots start at or before this one, in [seq, seq + n)
     int seq = 0;
-    for (int n = b.n_seqs; n > 1;) {  // it is in [seq, seq + n)
-        const int step = (n + 31) / 32, i = seq + lane * step;
+    kv8::Seq s;
+    for (int n = b.n_seqs;;) {
+        const int step = (n + 31) / 32, i = min(seq + lane * step, b.n_seqs - 1);
+        const kv8::Seq mine = kv8::sequence(b, i);  // of the last look, the answer's too
         const bool before =
-            lane * step < n &&
-            (min(max(b.row_start[i], 0), b.rows) >> b.page_shift) + 2 * i <= slot;
+            lane * step < n && (mine.lo >> b.page_shift) + 2 * i <= slot;
         const int last = 31 - __clz(__ballot_sync(tbk::kFull, before) | 1);
         seq += last * step;
         n = min(step, n - last * step);
+        if (step > 1) continue;
+        s.lo = __shfl_sync(tbk::kFull, mine.lo, last);
+        s.n = __shfl_sync(tbk::kFull, mine.n, last);
+        s.len = __shfl_sync(tbk::kFull, mine.len, last);
+        s.first = s.len - s.n;
+        break;
     }
-    const kv8::Seq s = kv8::sequence(b, seq);
     const int first = max(s.first, 0);  // rows before position 0 are padding
     const int logical = (first >> b.page_shift) + slot - ((s.lo >> b.page_shift) + 2 * seq);
     const int64_t begin = (int64_t)logical << b.page_shift;
@@ -278,11 +286,11 @@ extern "C" int tb_b200_kv8_append(const TbB200Kv8* cache, const TbB200Kv8Batch* 
                     cache->k_scale, cache->v_scale, ds->status, cache->n_kv_heads,
                     cache->head_dim};
     const unsigned slots = (unsigned)(batch->rows / cache->page + 2 * batch->n_seqs);
-    // One warp a unit when a sequence brings so few rows that kHold vectors a lane
-    // hold them (bf16: rows * d <= 2048 elements).
+    // One warp a unit when a sequence brings so few rows that 8 vectors a lane hold
+    // them (bf16: rows * d <= 2048 elements).
     const size_t size = dtype == TB_DTYPE_F32 ? 4 : 2;
     const bool warps = batch->rows * cache->head_dim * (int64_t)size <=
-                       (int64_t)batch->n_seqs * 32 * kHold * 16;
+                       (int64_t)batch->n_seqs * 32 * hold_of(size, 1) * 16;
     const bool vec = tbh::aligned16(k) && tbh::aligned16(v) && k_stride * size % 16 == 0 &&
                      v_stride * size % 16 == 0;
     cudaStream_t s = tbh::stream_of(stream);
