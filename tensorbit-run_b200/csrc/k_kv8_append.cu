@@ -87,20 +87,53 @@ constexpr int hold_of(size_t size, int warps) { return warps == 1 || size == 4 ?
 template <typename T, int V>
 __device__ __forceinline__ uint32_t top_of(const Piece<T, V>& x) {
     uint32_t top = 0;
+    if constexpr (sizeof(T) == 2 && V == 8) {  // two magnitudes a word
+        const uint32_t m = 0x7fff7fffu;
+        top = __vmaxu2(__vmaxu2(x.w.x & m, x.w.y & m), __vmaxu2(x.w.z & m, x.w.w & m));
+        return max(top & 0xffff0000u, top << 16);
+    }
 #pragma unroll
     for (int i = 0; i < V; ++i) top = max(top, __float_as_uint(x.at(i)) & 0x7fffffffu);
     return top;
 }
 
-template <int FORMAT, typename T, int V>
+// The codes of x * per; FINITE: of finite values, whose products are within the
+// format's range.
+template <int FORMAT, bool FINITE, typename T, int V>
 __device__ __forceinline__ void store_codes(uint8_t* p, const Piece<T, V>& x, float per) {
     constexpr float most = FORMAT == kv8::kInt8 ? 127.0f : 448.0f;
-    uint32_t w[(V + 3) / 4] = {};
+    float v[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-        float v = x.at(i) * per;
-        v = v != v ? 0.0f : fminf(fmaxf(v, -most), most);
-        w[i / 4] |= (uint32_t)kv8::encode<FORMAT>(v) << 8 * (i % 4);
+        v[i] = x.at(i);
+        if (!FINITE) {
+            v[i] *= per;
+            v[i] = v[i] != v[i] ? 0.0f : fminf(fmaxf(v[i], -most), most);
+        }
+    }
+    const float f = FINITE ? per : 1.0f;
+    uint32_t w[(V + 3) / 4] = {};
+    if constexpr (FORMAT == kv8::kInt8) {
+        // the sum with 1.5 * 2^23 rounds to a whole number, its low byte the code
+        uint32_t u[V];
+#pragma unroll
+        for (int i = 0; i < V; ++i) u[i] = __float_as_uint(fmaf(v[i], f, 12582912.0f));
+        if constexpr (V >= 4) {
+#pragma unroll
+            for (int i = 0; i < V; i += 4)
+                w[i / 4] = __byte_perm(__byte_perm(u[i], u[i + 1], 0x0040),
+                                       __byte_perm(u[i + 2], u[i + 3], 0x0040), 0x5410);
+        } else {
+            w[0] = u[0] & 0xff;
+        }
+    } else if constexpr (V >= 4) {
+#pragma unroll
+        for (int i = 0; i < V; i += 2)
+            w[i / 4] |= (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(v[i] * f, v[i + 1] * f),
+                                                           __NV_SATFINITE, __NV_E4M3)
+                        << 8 * (i % 4);
+    } else {
+        w[0] = kv8::encode<FORMAT>(v[0] * f);
     }
     if constexpr (V == 8)
         *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
@@ -202,7 +235,8 @@ __global__ void __launch_bounds__(kThreads, hold_of(sizeof(T), WARPS) == 4 ? 5 :
         return v;
     };
     top = over_unit(top);
-    if (top >= kInf) {  // the largest of the finite ones
+    const bool finite = top < kInf;
+    if (!finite) {  // the largest of the finite ones
         if (tid == 0) atomicOr(a.status, TB_B200_FLAG_NONFINITE);
         top = 0;
         r = r0;
@@ -236,21 +270,27 @@ __global__ void __launch_bounds__(kThreads, hold_of(sizeof(T), WARPS) == 4 ? 5 :
         }
     }
     const float per = 1.0f / now;  // both powers of two: exact
-    r = r0;
-    c = c0;
+    auto store = [&](auto finite) {
+        r = r0;
+        c = c0;
 #pragma unroll
-    for (int u = 0; u < kHold; ++u) {
-        if (tid + u * kUnit < n)
-            store_codes<FORMAT>(codes + (from + r) * a.d + c * V, hold[u], per);
-        next();
-    }
-    r = r_rest;
-    c = c_rest;
-    for (int i = tid + kHold * kUnit; i < n; i += kUnit) {
-        store_codes<FORMAT>(codes + (from + r) * a.d + c * V,
-                            Piece<T, V>::load(x + r * stride + c * V), per);
-        next();
-    }
+        for (int u = 0; u < kHold; ++u) {
+            if (tid + u * kUnit < n)
+                store_codes<FORMAT, finite.value>(codes + (from + r) * a.d + c * V, hold[u], per);
+            next();
+        }
+        r = r_rest;
+        c = c_rest;
+        for (int i = tid + kHold * kUnit; i < n; i += kUnit) {
+            store_codes<FORMAT, finite.value>(codes + (from + r) * a.d + c * V,
+                                              Piece<T, V>::load(x + r * stride + c * V), per);
+            next();
+        }
+    };
+    if (finite)
+        store(std::true_type{});
+    else
+        store(std::false_type{});
     if (WARPS == 1) __syncwarp();  // every thread has read *scale (else: over_unit's barriers)
     if (tid == 0) *scale = now;
 }
