@@ -10,7 +10,7 @@
 // e4m3's) but let each of a page's up to page - 1 rescalings add half a step.
 //
 // HBM bound: the rows read once, one byte an element written.  A unit is (page
-// that gets rows, head, K or V); which pages those are is on the device, so the
+// that gets rows, head), its K and V; which pages those are is on the device, so the
 // grid has a slot for each page that could: a sequence's rows from s to e touch at
 // most e / page - s / page + 2 pages, so sequence i's slots start at row_start[i] /
 // page + 2 i, which a warp finds its sequence by, 32 candidates at a time.
@@ -25,6 +25,7 @@
 namespace {
 
 constexpr int kThreads = 256;
+constexpr int kHold = 4;
 constexpr float kLeastScale = 7.8886090522101181e-31f;  // 2^-100
 
 template <int FORMAT>
@@ -81,8 +82,6 @@ struct Piece<__nv_bfloat16, 8> {
 };
 
 constexpr uint32_t kInf = 0x7f800000u;
-
-constexpr int hold_of(size_t size, int warps) { return warps == 1 || size == 4 ? 8 : 4; }
 
 template <typename T, int V>
 __device__ __forceinline__ uint32_t top_of(const Piece<T, V>& x) {
@@ -144,10 +143,9 @@ __device__ __forceinline__ void store_codes(uint8_t* p, const Piece<T, V>& x, fl
 }
 
 template <typename T, int FORMAT, int V, int WARPS>  // WARPS of a unit
-__global__ void __launch_bounds__(kThreads, hold_of(sizeof(T), WARPS) == 4 ? 5 : 3) k_append(const __grid_constant__ Args a) {
-    __shared__ uint32_t red[kThreads / 32];
+__global__ void __launch_bounds__(kThreads, 3) k_append(const __grid_constant__ Args a) {
+    __shared__ uint2 red[kThreads / 32];
     constexpr int kUnit = 32 * WARPS;  // threads
-    constexpr int kHold = hold_of(sizeof(T), WARPS);
     const kv8::Batch& b = a.b;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, tid = threadIdx.x % kUnit;
     const int slot = blockIdx.x, page = 1 << b.page_shift;
@@ -184,16 +182,14 @@ __global__ void __launch_bounds__(kThreads, hold_of(sizeof(T), WARPS) == 4 ? 5 :
     const int from = max(first - (int)begin, 0);
     const int to = (int)min((int64_t)page, s.len - begin);
     const int row = s.lo + (int)(begin + from - s.first);
-    const bool is_v = blockIdx.z != 0;
-    const int64_t stride = is_v ? a.v_stride : a.k_stride;
-    const T* x = static_cast<const T*>(is_v ? a.v : a.k) + row * stride + (int64_t)head * a.d;
+    const int64_t strides[2] = {a.k_stride, a.v_stride};
+    const T* x[2] = {static_cast<const T*>(a.k) + row * a.k_stride + (int64_t)head * a.d,
+                     static_cast<const T*>(a.v) + row * a.v_stride + (int64_t)head * a.d};
 
     // pieces tid, tid + kUnit, .. of the new rows, `per_row` of them a row
     const int per_row = a.d / V, n = (to - from) * per_row;
-    const int down = kUnit / per_row, right = kUnit % per_row;
-    const int r0 = tid / per_row, c0 = tid % per_row;
-    Piece<T, V> hold[kHold];
-    uint32_t top = 0;
+    const int down = kUnit / per_row, right = kUnit - down * per_row;
+    const int r0 = tid / per_row, c0 = tid - r0 * per_row;
     int r = r0, c = c0;
     auto next = [&] {
         r += down;
@@ -203,9 +199,14 @@ __global__ void __launch_bounds__(kThreads, hold_of(sizeof(T), WARPS) == 4 ? 5 :
             ++r;
         }
     };
+    auto piece = [&](int kv) { return Piece<T, V>::load(x[kv] + r * strides[kv] + c * V); };
+    Piece<T, V> hold[2][kHold];
 #pragma unroll
     for (int u = 0; u < kHold; ++u) {
-        if (tid + u * kUnit < n) hold[u] = Piece<T, V>::load(x + r * stride + c * V);
+        if (tid + u * kUnit < n) {
+            hold[0][u] = piece(0);
+            hold[1][u] = piece(1);
+        }
         next();
     }
     const int r_rest = r, c_rest = c;
@@ -213,49 +214,64 @@ __global__ void __launch_bounds__(kThreads, hold_of(sizeof(T), WARPS) == 4 ? 5 :
         if (tid == 0) atomicOr(a.status, TB_B200_FLAG_PAGE_RANGE);
         return;
     }
-    uint8_t* codes = (is_v ? a.v_codes : a.k_codes) +
-                     (((int64_t)id * a.hkv + head) << b.page_shift) * a.d;
-    float* scale = (is_v ? a.v_scale : a.k_scale) + (int64_t)id * a.hkv + head;
-    const float old = from > 0 ? *scale : 0.0f;
+    const int64_t unit = (int64_t)id * a.hkv + head;
+    uint8_t* codes[2] = {a.k_codes + (unit << b.page_shift) * a.d,
+                         a.v_codes + (unit << b.page_shift) * a.d};
+    const float old[2] = {from > 0 ? a.k_scale[unit] : 0.0f, from > 0 ? a.v_scale[unit] : 0.0f};
+    uint32_t top[2] = {0, 0};
 #pragma unroll
     for (int u = 0; u < kHold; ++u)
-        if (tid + u * kUnit < n) top = max(top, top_of(hold[u]));
+        if (tid + u * kUnit < n) {
+            top[0] = max(top[0], top_of(hold[0][u]));
+            top[1] = max(top[1], top_of(hold[1][u]));
+        }
     for (int i = tid + kHold * kUnit; i < n; i += kUnit) {
-        top = max(top, top_of(Piece<T, V>::load(x + r * stride + c * V)));
+        top[0] = max(top[0], top_of(piece(0)));
+        top[1] = max(top[1], top_of(piece(1)));
         next();
     }
-    auto over_unit = [&](uint32_t v) {
-        v = __reduce_max_sync(tbk::kFull, v);
-        if (WARPS == 1) return v;
+    auto over_unit = [&] {
+        top[0] = __reduce_max_sync(tbk::kFull, top[0]);
+        top[1] = __reduce_max_sync(tbk::kFull, top[1]);
+        if (WARPS == 1) return;
         __syncthreads();
-        if (lane == 0) red[warp] = v;
+        if (lane == 0) red[warp] = make_uint2(top[0], top[1]);
         __syncthreads();
 #pragma unroll
-        for (int i = 0; i < WARPS; ++i) v = max(v, red[i]);
-        return v;
+        for (int i = 0; i < WARPS; ++i) {
+            top[0] = max(top[0], red[i].x);
+            top[1] = max(top[1], red[i].y);
+        }
     };
-    top = over_unit(top);
-    const bool finite = top < kInf;
+    over_unit();
+    const bool finite = max(top[0], top[1]) < kInf;
     if (!finite) {  // the largest of the finite ones
         if (tid == 0) atomicOr(a.status, TB_B200_FLAG_NONFINITE);
-        top = 0;
+        top[0] = top[1] = 0;
         r = r0;
         c = c0;
         for (int i = tid; i < n; i += kUnit) {
-            const Piece<T, V> y = Piece<T, V>::load(x + r * stride + c * V);
-            for (int e = 0; e < V; ++e) {
-                const uint32_t bits = __float_as_uint(y.at(e)) & 0x7fffffffu;
-                if (bits < kInf) top = max(top, bits);
+            for (int kv = 0; kv < 2; ++kv) {
+                const Piece<T, V> y = piece(kv);
+                for (int e = 0; e < V; ++e) {
+                    const uint32_t bits = __float_as_uint(y.at(e)) & 0x7fffffffu;
+                    if (bits < kInf) top[kv] = max(top[kv], bits);
+                }
             }
             next();
         }
-        top = over_unit(top);
+        over_unit();
     }
-    const float now = fmaxf(scale_for<FORMAT>(__uint_as_float(top)), old);
-    if (now > old && from > 0) {  // 16 codes at a time: d is a multiple of 16
-        const float ratio = old / now;
-        for (int i = tid; i < from * a.d / 16; i += kUnit) {
-            uint4 w = reinterpret_cast<uint4*>(codes)[i];
+    float now[2], per[2];
+#pragma unroll
+    for (int kv = 0; kv < 2; ++kv) {
+        now[kv] = fmaxf(scale_for<FORMAT>(__uint_as_float(top[kv])), old[kv]);
+        per[kv] = 1.0f / now[kv];  // both powers of two: exact
+        if (!(now[kv] > old[kv] && from > 0)) continue;
+        const float ratio = old[kv] * per[kv];
+        uint4* held = reinterpret_cast<uint4*>(codes[kv]);
+        for (int i = tid; i < from * a.d / 16; i += kUnit) {  // d is a multiple of 16
+            uint4 w = held[i];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 uint32_t y = 0;
@@ -266,24 +282,28 @@ __global__ void __launch_bounds__(kThreads, hold_of(sizeof(T), WARPS) == 4 ? 5 :
                          << 8 * e;
                 (&w.x)[j] = y;
             }
-            reinterpret_cast<uint4*>(codes)[i] = w;
+            held[i] = w;
         }
     }
-    const float per = 1.0f / now;  // both powers of two: exact
     auto store = [&](auto finite) {
+        auto put = [&](int kv, const Piece<T, V>& y) {
+            store_codes<FORMAT, finite.value>(codes[kv] + (from + r) * a.d + c * V, y, per[kv]);
+        };
         r = r0;
         c = c0;
 #pragma unroll
         for (int u = 0; u < kHold; ++u) {
-            if (tid + u * kUnit < n)
-                store_codes<FORMAT, finite.value>(codes + (from + r) * a.d + c * V, hold[u], per);
+            if (tid + u * kUnit < n) {
+                put(0, hold[0][u]);
+                put(1, hold[1][u]);
+            }
             next();
         }
         r = r_rest;
         c = c_rest;
         for (int i = tid + kHold * kUnit; i < n; i += kUnit) {
-            store_codes<FORMAT, finite.value>(codes + (from + r) * a.d + c * V,
-                                              Piece<T, V>::load(x + r * stride + c * V), per);
+            put(0, piece(0));
+            put(1, piece(1));
             next();
         }
     };
@@ -291,18 +311,21 @@ __global__ void __launch_bounds__(kThreads, hold_of(sizeof(T), WARPS) == 4 ? 5 :
         store(std::true_type{});
     else
         store(std::false_type{});
-    if (WARPS == 1) __syncwarp();  // every thread has read *scale (else: over_unit's barriers)
-    if (tid == 0) *scale = now;
+    if (WARPS == 1) __syncwarp();  // every thread has read the scales (else: over_unit's barriers)
+    if (tid == 0) {
+        a.k_scale[unit] = now[0];
+        a.v_scale[unit] = now[1];
+    }
 }
 
 template <typename T, int FORMAT, int V>
 void launch(const Args& a, bool warps, unsigned slots, cudaStream_t s) {
     if (warps) {
         const unsigned heads = (unsigned)(a.hkv + kThreads / 32 - 1) / (kThreads / 32);
-        k_append<T, FORMAT, V, 1><<<dim3(slots, heads, 2), kThreads, 0, s>>>(a);
+        k_append<T, FORMAT, V, 1><<<dim3(slots, heads), kThreads, 0, s>>>(a);
     } else {
         k_append<T, FORMAT, V, kThreads / 32>
-            <<<dim3(slots, (unsigned)a.hkv, 2), kThreads, 0, s>>>(a);
+            <<<dim3(slots, (unsigned)a.hkv), kThreads, 0, s>>>(a);
     }
 }
 
@@ -326,11 +349,11 @@ extern "C" int tb_b200_kv8_append(const TbB200Kv8* cache, const TbB200Kv8Batch* 
                     cache->k_scale, cache->v_scale, ds->status, cache->n_kv_heads,
                     cache->head_dim};
     const unsigned slots = (unsigned)(batch->rows / cache->page + 2 * batch->n_seqs);
-    // One warp a unit when a sequence brings so few rows that 8 vectors a lane hold
-    // them (bf16: rows * d <= 2048 elements).
+    // One warp a unit when a sequence brings so few rows that kHold vectors a
+    // lane hold them (bf16: rows * d <= 1024 elements).
     const size_t size = dtype == TB_DTYPE_F32 ? 4 : 2;
     const bool warps = batch->rows * cache->head_dim * (int64_t)size <=
-                       (int64_t)batch->n_seqs * 32 * hold_of(size, 1) * 16;
+                       (int64_t)batch->n_seqs * 32 * kHold * 16;
     const bool vec = tbh::aligned16(k) && tbh::aligned16(v) && k_stride * size % 16 == 0 &&
                      v_stride * size % 16 == 0;
     cudaStream_t s = tbh::stream_of(stream);
