@@ -19,7 +19,10 @@
 // row's angles are computed once and shared; a group of G lanes owns a head,
 // each lane two vectors of it that hold both elements of its pairs, so a
 // head's sum of squares is a shuffle among G lanes and every element is read
-// and written once, in place if asked.
+// and written once, in place if asked.  A lane asks for the vectors of its
+// first U heads before the angles are computed and keeps its pairs' cos and sin
+// and its weights in registers for all of them; the CTA has just the threads
+// that make its passes over the heads full ones.
 #include <math.h>
 
 #include "tb_device.cuh"
@@ -37,6 +40,7 @@ template <typename T, int VEC>
 struct Vec {  // VEC = 1
     T e;
     __device__ static Vec load(const T* p) { return {*p}; }
+    __device__ static Vec load_kept(const T* p) { return {*p}; }
     __device__ void widen(float (&v)[VEC]) const { v[0] = tbk::Elt<T>::load(&e); }
     __device__ static void store(T* p, const float (&v)[VEC]) { tbk::Elt<T>::store(p, v[0]); }
 };
@@ -45,6 +49,7 @@ template <>
 struct Vec<float, 4> {
     uint4 w;
     __device__ static Vec load(const float* p) { return {__ldcs(reinterpret_cast<const uint4*>(p))}; }
+    __device__ static Vec load_kept(const float* p) { return {*reinterpret_cast<const uint4*>(p)}; }
     __device__ void widen(float (&v)[4]) const { tbk::Elt<float>::widen<4>(w, v); }
     __device__ static void store(float* p, const float (&v)[4]) { tbk::store_vec<float, 4>(p, v); }
 };
@@ -54,6 +59,9 @@ struct Vec<__nv_bfloat16, 8> {
     uint4 w;
     __device__ static Vec load(const __nv_bfloat16* p) {
         return {__ldcs(reinterpret_cast<const uint4*>(p))};
+    }
+    __device__ static Vec load_kept(const __nv_bfloat16* p) {
+        return {*reinterpret_cast<const uint4*>(p)};
     }
     __device__ void widen(float (&v)[8]) const { tbk::Elt<__nv_bfloat16>::widen<8>(w, v); }
     __device__ static void store(__nv_bfloat16* p, const float (&v)[8]) {
@@ -66,6 +74,9 @@ struct Vec<__nv_bfloat16, 4> {
     uint2 w;
     __device__ static Vec load(const __nv_bfloat16* p) {
         return {__ldcs(reinterpret_cast<const uint2*>(p))};
+    }
+    __device__ static Vec load_kept(const __nv_bfloat16* p) {
+        return {*reinterpret_cast<const uint2*>(p)};
     }
     __device__ void widen(float (&v)[4]) const {
         v[0] = __uint_as_float(w.x << 16);
@@ -102,117 +113,141 @@ __device__ __forceinline__ float2 turn(double t, float scale) {
 }
 
 template <typename T, int VEC, int NU, bool HALF, bool NORM>
-__global__ void __launch_bounds__(kThreads) k_rotary(const __grid_constant__ Args a) {
+__global__ void __launch_bounds__(kThreads, NU == 1 ? 4 : 1) k_rotary(const __grid_constant__ Args a) {
     __shared__ float2 cs[kMaxDim / 2];
     using V = Vec<T, VEC>;
+    constexpr int U = NU == 1 ? 2 : 1;  // heads a lane holds at once
     const int64_t row = blockIdx.x;
     const int half = a.r / 2;
+    const int lane = threadIdx.x % a.group, slot = threadIdx.x / a.group;
+    const int per_pass = blockDim.x / a.group, heads = a.hq + a.hkv;
+    const int nv = a.d / VEC, units = (nv + 1) / 2, hv = HALF ? half / VEC : 0;
+    const T* q = static_cast<const T*>(a.q) + row * a.q_stride;
+    const T* k = static_cast<const T*>(a.k) + row * a.k_stride - (int64_t)a.hq * a.d;
+    T* q_out = static_cast<T*>(a.q_out) + row * a.q_out_stride;
+    T* k_out = static_cast<T*>(a.k_out) + row * a.k_out_stride - (int64_t)a.hq * a.d;
+
+    int at[NU][2];  // the lane's vectors of a head, nv where there is none
+#pragma unroll
+    for (int n = 0; n < NU; ++n) {
+        const int u = lane + n * a.group;
+        // pairs of halves; past them, and for pairs side by side, two vectors: next
+        // to each other, or half the head apart so that lanes stay next to lanes
+        const bool split = HALF ? u < hv : VEC > 1;
+        at[n][0] = split ? u : 2 * u;
+        at[n][1] = split ? u + (HALF ? hv : units) : 2 * u + 1;
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+            if (u >= units || at[n][b] > nv) at[n][b] = nv;
+    }
+    V held[U][NU][2];
+    auto ask = [&](int h, V (&v)[NU][2]) {
+        const T* in = (h < a.hq ? q : k) + (int64_t)h * a.d;
+#pragma unroll
+        for (int n = 0; n < NU; ++n)
+#pragma unroll
+            for (int b = 0; b < 2; ++b)
+                if (h < heads && at[n][b] < nv) v[n][b] = V::load(in + at[n][b] * VEC);
+    };
+#pragma unroll
+    for (int u = 0; u < U; ++u) ask(slot + u * per_pass, held[u]);
+
     if (half) {
         const double p = (double)a.positions[row];
-        for (int i = threadIdx.x; i < half; i += kThreads)
+        for (int i = threadIdx.x; i < half; i += blockDim.x)
             cs[i] = turn(p * (a.freqs[i] * 0.15915494309189533577), a.scale);
     }
     __syncthreads();
-
-    const int lane = threadIdx.x % a.group, slot = threadIdx.x / a.group;
-    const int per_pass = kThreads / a.group, heads = a.hq + a.hkv;
-    const int nv = a.d / VEC, units = (nv + 1) / 2, hv = HALF ? half / VEC : 0;
-    for (int h0 = 0; h0 < heads; h0 += per_pass) {
-        const int h = h0 + slot;
-        const bool is_q = h < a.hq, live = h < heads;
-        const T* in = is_q ? static_cast<const T*>(a.q) + row * a.q_stride + (int64_t)h * a.d
-                           : static_cast<const T*>(a.k) + row * a.k_stride +
-                                 (int64_t)(h - a.hq) * a.d;
-        T* out = is_q ? static_cast<T*>(a.q_out) + row * a.q_out_stride + (int64_t)h * a.d
-                      : static_cast<T*>(a.k_out) + row * a.k_out_stride +
-                            (int64_t)(h - a.hq) * a.d;
-        const T* w = static_cast<const T*>(is_q ? a.q_weight : a.k_weight);
-        float x[NU][2][VEC];
-        int at[NU][2];  // vector numbers, nv where there is none
-        float ss = 0.0f;
+    // cos and sin of the lane's pairs: VEC of them, of (e, e) of the two vectors or
+    // of (2 e, 2 e + 1) of the first, then the second; turns: whether they are pairs
+    constexpr bool kAcross = HALF || VEC == 1;
+    float2 t[NU][VEC];
+    bool turns[NU][2];
 #pragma unroll
-        for (int n = 0; n < NU; ++n) {
-            const int u = lane + n * a.group;
-            if (HALF && u < hv) {
-                at[n][0] = u;
-                at[n][1] = u + hv;
-            } else if (HALF) {  // past the rotated part
-                at[n][0] = 2 * u;
-                at[n][1] = 2 * u + 1;
-            } else if (VEC == 1) {
-                at[n][0] = 2 * u;
-                at[n][1] = 2 * u + 1;
-            } else {
-                at[n][0] = u;
-                at[n][1] = u + units;
-            }
+    for (int n = 0; n < NU; ++n) {
+        const int u = lane + n * a.group;
 #pragma unroll
-            for (int b = 0; b < 2; ++b) {
-                if (u >= units || at[n][b] >= nv || !live) at[n][b] = nv;
+        for (int b = 0; b < 2; ++b)
+            turns[n][b] = kAcross ? u < (HALF ? hv : half) : at[n][b] * VEC < a.r;
 #pragma unroll
-                for (int e = 0; e < VEC; ++e) x[n][b][e] = 0.0f;
-                if (at[n][b] < nv) V::load(in + at[n][b] * VEC).widen(x[n][b]);
-                if (NORM) {
-#pragma unroll
-                    for (int e = 0; e < VEC; ++e) ss = fmaf(x[n][b][e], x[n][b][e], ss);
-                }
-            }
+        for (int e = 0; e < VEC; ++e) {
+            const int b = kAcross ? 0 : 2 * e / VEC;
+            const int i = kAcross ? u * VEC + e : at[n][b] * VEC / 2 + e % ((VEC + 1) / 2);
+            if (turns[n][b]) t[n][e] = cs[i];
         }
-        if (NORM) {
-            for (int o = a.group >> 1; o > 0; o >>= 1) ss += __shfl_xor_sync(kFull, ss, o);
-            const float inv =
-                __fdiv_rn(1.0f, __fsqrt_rn(__fadd_rn(__fdiv_rn(ss, (float)a.d), a.eps)));
+    }
+
+    for (int h0 = 0; h0 < heads; h0 += U * per_pass) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (h0 + u * per_pass >= heads) break;
+            const int h = h0 + u * per_pass + slot;
+            const bool is_q = h < a.hq, live = h < heads;
+            T* out = (is_q ? q_out : k_out) + (int64_t)h * a.d;
+            float x[NU][2][VEC];
+            float ss = 0.0f;
 #pragma unroll
             for (int n = 0; n < NU; ++n)
 #pragma unroll
                 for (int b = 0; b < 2; ++b) {
-                    float g[VEC];
 #pragma unroll
-                    for (int e = 0; e < VEC; ++e) g[e] = 1.0f;
-                    if (w && at[n][b] < nv) V::load(w + at[n][b] * VEC).widen(g);
+                    for (int e = 0; e < VEC; ++e) x[n][b][e] = 0.0f;
+                    if (live && at[n][b] < nv) held[u][n][b].widen(x[n][b]);
+                    if (NORM) {
 #pragma unroll
-                    for (int e = 0; e < VEC; ++e) x[n][b][e] = x[n][b][e] * inv * g[e];
-                }
-        }
-#pragma unroll
-        for (int n = 0; n < NU; ++n) {
-            const int u = lane + n * a.group;
-            if (HALF || VEC == 1) {
-                if (u < (HALF ? hv : half)) {
-#pragma unroll
-                    for (int e = 0; e < VEC; ++e) {
-                        const float2 t = cs[u * VEC + e];
-                        const float x0 = x[n][0][e], x1 = x[n][1][e];
-                        x[n][0][e] = x0 * t.x - x1 * t.y;
-                        x[n][1][e] = x1 * t.x + x0 * t.y;
+                        for (int e = 0; e < VEC; ++e) ss = fmaf(x[n][b][e], x[n][b][e], ss);
                     }
                 }
-            } else {
+            if (NORM) {
+                for (int o = a.group >> 1; o > 0; o >>= 1) ss += __shfl_xor_sync(kFull, ss, o);
+                const float inv =
+                    __fdiv_rn(1.0f, __fsqrt_rn(__fadd_rn(__fdiv_rn(ss, (float)a.d), a.eps)));
+                const T* w = static_cast<const T*>(is_q ? a.q_weight : a.k_weight);
 #pragma unroll
-                for (int b = 0; b < 2; ++b)
-                    if (at[n][b] * VEC < a.r) {
+                for (int n = 0; n < NU; ++n)
 #pragma unroll
-                        for (int e = 0; e + 1 < VEC; e += 2) {
-                            const float2 t = cs[(at[n][b] * VEC + e) / 2];
-                            const float x0 = x[n][b][e], x1 = x[n][b][e + 1];
-                            x[n][b][e] = x0 * t.x - x1 * t.y;
-                            x[n][b][e + 1] = x1 * t.x + x0 * t.y;
-                        }
+                    for (int b = 0; b < 2; ++b) {
+                        float g[VEC];
+#pragma unroll
+                        for (int e = 0; e < VEC; ++e) g[e] = 1.0f;
+                        if (w && at[n][b] < nv) V::load_kept(w + at[n][b] * VEC).widen(g);
+#pragma unroll
+                        for (int e = 0; e < VEC; ++e) x[n][b][e] = x[n][b][e] * inv * g[e];
                     }
             }
 #pragma unroll
-            for (int b = 0; b < 2; ++b)
-                if (at[n][b] < nv) V::store(out + at[n][b] * VEC, x[n][b]);
+            for (int n = 0; n < NU; ++n) {
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) {
+                    if (!turns[n][kAcross ? 0 : 2 * e / VEC]) continue;
+                    float& x0 = kAcross ? x[n][0][e] : x[n][2 * e / VEC][2 * e % VEC];
+                    float& x1 = kAcross ? x[n][1][e] : x[n][2 * e / VEC][(2 * e + 1) % VEC];
+                    const float y0 = x0 * t[n][e].x - x1 * t[n][e].y;
+                    x1 = x1 * t[n][e].x + x0 * t[n][e].y;
+                    x0 = y0;
+                }
+#pragma unroll
+                for (int b = 0; b < 2; ++b)
+                    if (live && at[n][b] < nv) V::store(out + at[n][b] * VEC, x[n][b]);
+            }
+        }
+        if (h0 + U * per_pass < heads) {
+#pragma unroll
+            for (int u = 0; u < U; ++u) ask(h0 + (U + u) * per_pass + slot, held[u]);
         }
     }
 }
 
 template <typename T, int VEC, int NU, bool NORM>
 void launch_layout(const Args& a, bool half_layout, unsigned rows, cudaStream_t s) {
+    // the fewest passes over the heads, and the fewest threads for as many
+    const int64_t lanes = (int64_t)(a.hq + a.hkv) * a.group;
+    const int64_t passes = (lanes + kThreads - 1) / kThreads;
+    const unsigned threads = (unsigned)((lanes + passes * 32 - 1) / (passes * 32) * 32);
     if (half_layout)
-        k_rotary<T, VEC, NU, true, NORM><<<rows, kThreads, 0, s>>>(a);
+        k_rotary<T, VEC, NU, true, NORM><<<rows, threads, 0, s>>>(a);
     else
-        k_rotary<T, VEC, NU, false, NORM><<<rows, kThreads, 0, s>>>(a);
+        k_rotary<T, VEC, NU, false, NORM><<<rows, threads, 0, s>>>(a);
 }
 
 bool aligned(const void* p, size_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
@@ -245,14 +280,20 @@ void launch(Args& a, int dtype, bool half_layout, unsigned rows, cudaStream_t s)
             launch_layout<__nv_bfloat16, 8, 1, NORM>(a, half_layout, rows, s);
         } else if (vectors_of(4, 2, a, half_layout)) {
             a.group = group_of(a.d, 4);
-            launch_layout<__nv_bfloat16, 4, 2, NORM>(a, half_layout, rows, s);
+            if (a.d <= 256)
+                launch_layout<__nv_bfloat16, 4, 1, NORM>(a, half_layout, rows, s);
+            else
+                launch_layout<__nv_bfloat16, 4, 2, NORM>(a, half_layout, rows, s);
         } else {
             a.group = 32;
             launch_layout<__nv_bfloat16, 1, 8, NORM>(a, half_layout, rows, s);
         }
     } else if (vectors_of(4, 4, a, half_layout)) {
         a.group = group_of(a.d, 4);
-        launch_layout<float, 4, 2, NORM>(a, half_layout, rows, s);
+        if (a.d <= 256)
+            launch_layout<float, 4, 1, NORM>(a, half_layout, rows, s);
+        else
+            launch_layout<float, 4, 2, NORM>(a, half_layout, rows, s);
     } else {
         a.group = 32;
         launch_layout<float, 1, 8, NORM>(a, half_layout, rows, s);

@@ -175,6 +175,25 @@ def test_norm_of_zeros_infinities_and_lone_heads(dev):
     assert bool(torch.isnan(qo[1, 0, 5])) and bool(torch.isnan(qo[2, 1]).all())
 
 
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("layout", [T.ROTARY_INTERLEAVED, T.ROTARY_HALF])
+def test_infinities_stay_in_their_pair(dev, bf16, layout):
+    """What is past the rotated part is passed through, whatever stands beside it."""
+    import torch
+    for d, r in ((80, 32), (64, 16), (17, 6)):
+        q, k, pos, _ = inputs(dev, 5, 3, 2, d, bf16)
+        q, k = q.clone(), k.clone()
+        q[:, :, r + 1::3] = float("inf")
+        q[:, 1, r + 2::5] = float("nan")
+        fr = freqs_of(r)
+        got, _ = T.rotary(q, k, pos.to(dev), torch.from_numpy(fr).to(dev), layout)
+        assert torch.equal(got[:, :, r:].nan_to_num(7.0, 8.0, 9.0),
+                           q[:, :, r:].nan_to_num(7.0, 8.0, 9.0))
+        clean = torch.where(torch.isfinite(q), q, torch.zeros_like(q))
+        y, tol = want(clean, None, 0, pos.numpy(), fr, layout, 1.0, False)
+        check(got[:, :, :r], y[..., :r], tol[..., :r], bf16)
+
+
 SCALINGS = [("none", 1.0, 0, 0, 0), ("linear", 4.0, 0, 0, 0), ("ntk", 8.0, 0, 0, 0),
             ("bands", 8.0, 8192, 1.0, 4.0), ("yarn", 16.0, 4096, 1.0, 32.0)]
 
