@@ -994,8 +994,8 @@ extern "C" int tb_b200_kv8_attention_workspace(const TbB200Kv8* cache,
     if (batch->rows == 0 || batch->n_seqs == 0) return TB_OK;
     tbh::DeviceState* ds = tbh::current_device_state();
     if (!ds) return TB_ERR_DEVICE;
-    const Plan p = plan_of(cache, batch, attention, ds->sm_count);
-    *bytes = p.bytes();
+    if (kv8::chunk_suits(cache, batch, attention, ds->sm_count)) return TB_OK;
+    *bytes = plan_of(cache, batch, attention, ds->sm_count).bytes();
     return TB_OK;
 }
 
@@ -1007,6 +1007,8 @@ extern "C" int tb_b200_kv8_attention(const TbB200Kv8* cache, const TbB200Kv8Batc
     if (batch->rows == 0 || batch->n_seqs == 0) return TB_OK;
     tbh::DeviceState* ds = tbh::current_device_state();
     if (!ds) return TB_ERR_DEVICE;
+    if (kv8::chunk_suits(cache, batch, t, ds->sm_count))
+        return kv8::chunk_attention(cache, batch, t, tbh::stream_of(stream));
     const Plan p = plan_of(cache, batch, t, ds->sm_count);
     const size_t bytes = p.bytes();
     if (bytes && (!t->workspace || t->workspace_bytes < bytes || !tbh::aligned16(t->workspace))) {

@@ -1,0 +1,500 @@
+// k_kv8_chunk.cu -- attention of many query rows (a chunk of a prompt) over the
+// paged 8-bit cache: the mathematics of k_kv8_attention.cu with the products on
+// the fifth-generation tensor cores.
+//
+// A CTA has 256 rows of one sequence and k/v head ((token, head of the group)
+// pairs, token-major), as two tiles of 128, and walks their keys 128 at a time:
+//   S = Q K^T  [128 x 128], operands f16 in shared memory, sums in tensor memory
+//   P = 2^(S f - r), f16, over S's place in tensor memory
+//   O += P V   P from tensor memory, V f16 in shared memory
+// 13 warps: 4 bring codes from global memory and write them as f16 tiles (two
+// stages), 4 for each row tile compute P, a thread a row, and one thread issues
+// the products, so that one tile's softmax runs while the other's products do.
+//
+// What bounds it, per 256 rows and 128 keys: the products, 4 * 128^3 at 4096 a
+// clock, 2050 clocks; the exponentials, 32768 at 16 a clock, as many; converting
+// 32768 codes, 7 % of the products' time an instruction.  Codes are converted
+// once for 256 rows, four times fewer than a block of 16 rows' matrix
+// instructions could share, and the products run at 4 times their rate.
+//
+// Precision as in k_kv8_attention.cu: a row of q is scaled by a power of two to
+// [2^14, 2^15) and held as f16, exact for bf16 elements above 2^-21 of the row's
+// largest; weights are f16 times 2^11 under a reference that moves by whole
+// powers of two; the values' scale joins the weight, p * 2^(log2 v_scale + r - r')
+// with the row's r', in f32 before its rounding.
+#include <math.h>
+
+#include "kv8_mma.cuh"
+#include "tcgen05.cuh"
+
+namespace {
+
+constexpr int kRows = 128;         // of a tile
+constexpr int kTiles = 2;          // of a CTA
+constexpr int kKeys = 128;         // of a step
+constexpr int kGroups = kKeys / 16;  // of keys, each in one page
+constexpr int kStages = 2;
+constexpr int kSoftWarps = 4 * kTiles, kConvWarps = 4;
+constexpr int kIssuer = kSoftWarps + kConvWarps;  // the warp
+constexpr int kThreads = 32 * (kIssuer + 1);
+constexpr float kSlack = 4.0f, kLift = 11.0f, kLog2e = 1.4426950408889634f, kNoRef = -3.0e38f;
+constexpr uint32_t kColumns = 512;  // of tensor memory: S and P at 0, 128, O at 256, 384
+
+struct Args {
+    kv8::Batch b;
+    const void* q;
+    void* out;
+    float* lse;
+    int64_t q_stride, out_stride;
+    const uint8_t *k, *v;
+    const float *k_scale, *v_scale;
+    unsigned* status;
+    float scale;
+    int hq, hkv, d, window, max_rows, max_len, vec, vec_out;
+};
+
+template <int DP>
+struct Shape {
+    static constexpr int kPanels = DP / 64;
+    static constexpr int kPanel = 128 * 128;  // bytes of 128 rows of 64 f16
+    static constexpr int kTile = kPanels * kPanel;
+    static constexpr int kBytes = kTiles * kTile + kStages * 2 * kTile + 1024;  // 1024: to align
+};
+
+struct Shared {
+    uint64_t k_full[kStages], v_full[kStages], kv_free[kStages];
+    uint64_t s_full[kTiles], p_full[kTiles], o_done[kTiles];
+    float2 scales[kStages][kGroups];  // of K (< 0: no page) and log2 of V's
+    uint32_t tmem;
+};
+
+// Where the f16 element e of row r of a tile of 64-element panels lies.
+__device__ __forceinline__ int place(int row, int piece) {  // 16-byte pieces of 8 elements
+    return (piece >> 3) * (128 * 128) + row * 128 + ((piece ^ row) & 7) * 16;
+}
+
+// A bounded wait of a whole warp.
+__device__ __forceinline__ bool wait_all(uint64_t* bar, uint32_t parity, unsigned* status) {
+    const bool came = tbk::mbar_wait(bar, parity, status, 1000000000ull);
+    return __all_sync(tbk::kFull, came);
+}
+
+template <int FORMAT>
+__device__ __forceinline__ void to_f16(const uint4& codes, uint4 (&h)[2]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const uint32_t w = (&codes.x)[i];
+        uint32_t lo, hi;
+        if constexpr (FORMAT == kv8::kInt8) {
+            lo = kv8::int8_pair(kv8::prmt(w, 0, 0x4140));
+            hi = kv8::int8_pair(kv8::prmt(w, 0, 0x4342));
+        } else {
+            lo = kv8::e4m3_pair(w, false);
+            hi = kv8::e4m3_pair(w, true);
+        }
+        (&h[i / 2].x)[i % 2 * 2] = lo;
+        (&h[i / 2].x)[i % 2 * 2 + 1] = hi;
+    }
+}
+
+template <int FORMAT, int DP>
+__global__ void __launch_bounds__(kThreads, 1) k_chunk(const __grid_constant__ Args a) {
+    using H = Shape<DP>;
+    using T = __nv_bfloat16;
+    constexpr int kSteps = DP / 16;
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ Shared sh;
+    uint8_t* smem = smem_raw + (-tbk::smem_addr(smem_raw) & 1023u);
+    uint8_t* q_tiles = smem;
+    uint8_t* kv_tiles = smem + kTiles * H::kTile;  // [stage][K, V]
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int head = blockIdx.x, seq = blockIdx.z;
+    const kv8::Seq s = kv8::sequence(a.b, seq);
+    const int group = a.hq / a.hkv, rows_all = s.n * group;
+    // long blocks first
+    const int block = (int)gridDim.y - 1 - (int)blockIdx.y, at = block * kTiles * kRows;
+    if (at >= rows_all) return;
+    const int rows = min(kTiles * kRows, rows_all - at);
+    const int tiles = rows > kRows ? 2 : 1;
+    const bool ok = s.len <= a.max_len && s.n <= a.max_rows &&
+                    s.len <= ((int64_t)a.b.width << a.b.page_shift);
+    if (!ok && threadIdx.x == 0) atomicOr(a.status, TB_B200_FLAG_POSITION_RANGE);
+    // keys [from, end) that some row sees
+    const int p0 = s.first + at / group, p1 = s.first + (at + rows - 1) / group;
+    const int end = ok ? max(p1 + 1, 0) : 0;
+    const int from = a.window ? min(max(p0 - a.window + 1, 0), end) & ~(kKeys - 1) : 0;
+    const int steps = (end - from + kKeys - 1) / kKeys;
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < kStages; ++i) {
+            tbk::mbar_init(&sh.k_full[i], kConvWarps);
+            tbk::mbar_init(&sh.v_full[i], kConvWarps);
+            tbk::mbar_init(&sh.kv_free[i], 1);
+        }
+        for (int i = 0; i < kTiles; ++i) {
+            tbk::mbar_init(&sh.s_full[i], 1);
+            tbk::mbar_init(&sh.p_full[i], 4);
+            tbk::mbar_init(&sh.o_done[i], 1);
+        }
+        tbk::fence_mbar_init();
+    }
+    if (warp == kIssuer) tc::allocate(&sh.tmem, kColumns);
+
+    // Q: a thread its row.  A row with a NaN or an infinity is NaN.
+    const int tile = warp / 4, row = threadIdx.x & (kRows - 1);
+    const int r = tile * kRows + row;
+    const bool soft = warp < kSoftWarps, live = soft && r < rows;
+    float f = 0.0f;  // what the row's sums of products are multiplied with
+    const int tok = live ? (at + r) / group : 0, hh = live ? (at + r) % group : 0;
+    if (soft && tile < tiles) {
+        const T* q = static_cast<const T*>(a.q) + (s.lo + tok) * a.q_stride +
+                     (int64_t)(head * group + hh) * a.d;
+        uint32_t top = 0;
+        for (int i = 0; i < a.d && live; i += 4) {
+            float x[4];
+            kv8::load4(q + i, true, a.vec, x);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) top = max(top, __float_as_uint(fabsf(x[e])));
+        }
+        const bool finite = top < 0x7f800000u;
+        const int e = min(max((int)(top >> 23), 1 + 16), 254);
+        // a negative scale turns q, so that larger sums are larger scores
+        const float lift = __uint_as_float((uint32_t)(127 + 14 - e + 127) << 23) *
+                           (a.scale < 0.0f ? -1.0f : 1.0f);
+        f = finite ? __uint_as_float((uint32_t)(e - 14) << 23) * (fabsf(a.scale) * kLog2e) : NAN;
+        for (int i = 0; i < DP; i += 8) {
+            float x[4], y[4];
+            kv8::load4(q + i, live && finite && i < a.d, a.vec, x);
+            kv8::load4(q + i + 4, live && finite && i < a.d, a.vec, y);
+            const uint4 h = make_uint4(
+                kv8::pack_f16x2(x[0] * lift, x[1] * lift), kv8::pack_f16x2(x[2] * lift, x[3] * lift),
+                kv8::pack_f16x2(y[0] * lift, y[1] * lift), kv8::pack_f16x2(y[2] * lift, y[3] * lift));
+            *reinterpret_cast<uint4*>(q_tiles + tile * H::kTile + place(row, i / 8)) = h;
+        }
+        tbk::fence_proxy_async_shared();
+    }
+    tc::fence_before();
+    __syncthreads();
+    tc::fence_after();
+    const uint32_t tmem = sh.tmem;
+
+    if (warp == kIssuer) {
+        if (lane == 0 && steps > 0) {
+            const uint32_t instr_s = tc::f16_instruction(kKeys, false);
+            const uint32_t instr_o = tc::f16_instruction(DP, true);
+            const uint32_t q_at = tbk::smem_addr(q_tiles), kv_at = tbk::smem_addr(kv_tiles);
+            auto scores = [&](int t, int j) {  // S of tile t and step j
+                const uint32_t k_at = kv_at + (j % kStages) * 2 * H::kTile;
+#pragma unroll
+                for (int i = 0; i < kSteps; ++i) {
+                    const uint32_t off = i / 4 * H::kPanel + i % 4 * 32;
+                    tc::mma(tmem + t * 128, tc::tile_descriptor(q_at + t * H::kTile + off, 16),
+                            tc::tile_descriptor(k_at + off, 16), instr_s, i > 0);
+                }
+                tc::commit(&sh.s_full[t]);
+            };
+            auto wait = [&](uint64_t* bar, int phase) {
+                return tbk::mbar_wait(bar, phase & 1, a.status, 1000000000ull);
+            };
+            bool fine = wait(&sh.k_full[0], 0);
+            tc::fence_after();
+            for (int t = 0; t < tiles && fine; ++t) scores(t, 0);
+            for (int j = 0; j < steps && fine; ++j) {
+                const int stage = j % kStages;
+                const uint32_t v_at = kv_at + stage * 2 * H::kTile + H::kTile;
+                fine = wait(&sh.v_full[stage], j / kStages);
+                for (int t = 0; t < tiles && fine; ++t) {
+                    fine = wait(&sh.p_full[t], j);
+                    if (!fine) break;
+                    tc::fence_after();
+#pragma unroll
+                    for (int i = 0; i < kKeys / 16; ++i)
+                        tc::mma_tmem(tmem + 256 + t * 128, tmem + t * 128 + i * 8,
+                                     tc::tile_descriptor(v_at + i * 2048, H::kPanel), instr_o,
+                                     j > 0 || i > 0);
+                    tc::commit(&sh.o_done[t]);
+                    if (t == tiles - 1) tc::commit(&sh.kv_free[stage]);
+                    if (j + 1 < steps) {
+                        if (t == 0) {
+                            fine = wait(&sh.k_full[(j + 1) % kStages], (j + 1) / kStages);
+                            if (!fine) break;
+                            tc::fence_after();
+                        }
+                        scores(t, j + 1);
+                    }
+                }
+            }
+        }
+        __syncwarp();
+    } else if (!soft) {
+        // codes to f16: a thread pieces c of keys k, k + 16, ..
+        const int tid = threadIdx.x - 32 * kSoftWarps, c = tid % 8, k0 = tid / 8;
+        const int32_t* table = a.b.table + seq * a.b.table_stride;
+        uint4 held[2][kGroups];
+        float2 scale;  // of group tid (of kGroups), asked for with the codes
+        int ids[kGroups];
+        auto pages = [&](int j) {
+#pragma unroll
+            for (int i = 0; i < kGroups; ++i) {
+                const int key = from + j * kKeys + 16 * i;
+                ids[i] = key < end ? table[key >> a.b.page_shift] : -1;
+            }
+        };
+        auto ask = [&](int j) {
+            scale = make_float2(-1.0f, 0.0f);
+#pragma unroll
+            for (int i = 0; i < kGroups; ++i) {
+                const int key0 = from + j * kKeys + 16 * i, key = key0 + k0;
+                const bool page = ids[i] >= 0 && ids[i] < a.b.n_pages;
+                if (key0 < end && !page) atomicOr(a.status, TB_B200_FLAG_PAGE_RANGE);
+                held[0][i] = held[1][i] = make_uint4(0, 0, 0, 0);
+                if (!page) continue;
+                const int64_t unit = (int64_t)ids[i] * a.hkv + head;
+                if (i == tid) scale = make_float2(a.k_scale[unit], a.v_scale[unit]);
+                if (key >= s.len || c * 16 >= a.d) continue;
+                const int slot = key & ((1 << a.b.page_shift) - 1);
+                const int64_t from_ = ((unit << a.b.page_shift) + slot) * a.d + c * 16;
+                held[0][i] = *reinterpret_cast<const uint4*>(a.k + from_);
+                held[1][i] = *reinterpret_cast<const uint4*>(a.v + from_);
+            }
+        };
+        if (steps > 0) {
+            pages(0);
+            ask(0);
+            if (steps > 1) pages(1);
+        }
+        for (int j = 0; j < steps; ++j) {
+            const int stage = j % kStages;
+            if (j >= kStages && !wait_all(&sh.kv_free[stage], (j / kStages - 1) & 1, a.status))
+                break;
+            uint8_t* to = kv_tiles + stage * 2 * H::kTile;
+            if (tid < kGroups)
+                sh.scales[stage][tid] = make_float2(
+                    scale.x, (float)((int)(__float_as_uint(scale.y) >> 23) - 127));
+#pragma unroll
+            for (int kv = 0; kv < 2; ++kv) {
+                if (c * 16 < DP) {
+#pragma unroll
+                    for (int i = 0; i < kGroups; ++i) {
+                        uint4 h[2];
+                        to_f16<FORMAT>(held[kv][i], h);
+                        // the lanes of a key's second panel write their pieces in
+                        // the other order, into other banks
+                        const int key = k0 + 16 * i, x = c >> 2;
+                        uint8_t* tile_at = to + kv * H::kTile;
+                        *reinterpret_cast<uint4*>(tile_at + place(key, 2 * c + x)) =
+                            x ? h[1] : h[0];
+                        *reinterpret_cast<uint4*>(tile_at + place(key, 2 * c + 1 - x)) =
+                            x ? h[0] : h[1];
+                    }
+                }
+                tbk::fence_proxy_async_shared();
+                __syncwarp();
+                if (lane == 0) tbk::mbar_arrive(kv ? &sh.v_full[stage] : &sh.k_full[stage]);
+            }
+            if (j + 1 < steps) {
+                ask(j + 1);
+                if (j + 2 < steps) pages(j + 2);
+            }
+        }
+    } else if (tile < tiles) {
+        const uint32_t s_at = tmem + tile * 128 + ((uint32_t)(warp % 4) << 21);
+        const uint32_t o_at = s_at + 256;
+        const int see_hi = live ? s.first + tok : INT32_MAX;
+        const int see_lo = live && a.window ? max(see_hi - a.window + 1, 0) : 0;
+        float ref = kNoRef, vref = kNoRef, sum = 0.0f;
+        bool fine = true;
+        for (int j = 0; j < steps; ++j) {
+            fine = wait_all(&sh.k_full[j % kStages], j / kStages & 1, a.status) &&
+                   wait_all(&sh.s_full[tile], j & 1, a.status);
+            if (!fine) break;
+            tc::fence_after();
+            const int key0 = from + j * kKeys;
+            float fs[kGroups], lv[kGroups];
+            uint32_t have = 0;  // groups that have a page
+#pragma unroll
+            for (int i = 0; i < kGroups; ++i) {
+                const float2 x = sh.scales[j % kStages][i];
+                fs[i] = f * x.x;
+                lv[i] = x.y;
+                have |= (uint32_t)(x.x > 0.0f) << i;
+            }
+            const bool inside =
+                __all_sync(tbk::kFull, key0 >= see_lo && key0 + kKeys - 1 <= see_hi &&
+                                           have == (1u << kGroups) - 1);
+            // 32 columns: sums of products, or, of a step with keys that a row does
+            // not see, scores
+            auto columns = [&](int c0, float (&x)[32]) {
+                tc::load32(s_at + c0, x);
+                if (inside) return;
+#pragma unroll
+                for (int e = 0; e < 32; ++e) {
+                    const int key = key0 + c0 + e, i = (c0 + e) / 16;
+                    const bool seen = key >= see_lo && key <= see_hi && (have >> i & 1);
+                    x[e] = seen ? x[e] * fs[i] : -INFINITY;
+                }
+            };
+            // the largest score, and with the values' scale
+            float hi = -INFINITY, hv = -INFINITY;
+#pragma unroll
+            for (int c0 = 0; c0 < kKeys; c0 += 32) {
+                float x[32];
+                columns(c0, x);
+#pragma unroll
+                for (int g = 0; g < 2; ++g) {
+                    float m = x[16 * g];
+#pragma unroll
+                    for (int e = 1; e < 16; ++e) m = fmaxf(m, x[16 * g + e]);
+                    const int i = c0 / 16 + g;
+                    if (inside) m *= fs[i];
+                    hi = fmaxf(hi, m);
+                    hv = fmaxf(hv, m + lv[i]);
+                }
+            }
+            const bool over = hi > ref + kSlack || hv > vref + kSlack;
+            if (__any_sync(tbk::kFull, over)) {
+                const float m = over ? fmaxf(ref, ceilf(hi)) : ref;
+                const float mv = over ? fmaxf(vref, ceilf(hv)) : vref;
+                sum *= exp2f(ref - m);
+                if (__any_sync(tbk::kFull, mv > vref) && j > 0) {
+                    // O is free between its products of two steps
+                    fine = wait_all(&sh.o_done[tile], (j - 1) & 1, a.status);
+                    if (!fine) break;
+                    tc::fence_after();
+                    const float keep = exp2f(vref - mv);
+#pragma unroll 1
+                    for (int c0 = 0; c0 < DP; c0 += 32) {
+                        float x[32];
+                        tc::load32(o_at + c0, x);
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) x[e] *= keep;
+                        tc::store32(o_at + c0, x);
+                    }
+                    tc::wait_store();
+                }
+                ref = m;
+                vref = mv;
+            }
+#pragma unroll
+            for (int c0 = 0; c0 < kKeys; c0 += 32) {
+                float x[32];
+                columns(c0, x);
+                uint32_t p[16];
+#pragma unroll
+                for (int g = 0; g < 2; ++g) {
+                    const int i = c0 / 16 + g;
+                    const float by = kv8::exp2_fast(lv[i] + ref - vref + kLift);
+                    const float fi = inside ? fs[i] : 1.0f;
+#pragma unroll
+                    for (int e = 0; e < 16; e += 2) {
+                        const float y = kv8::exp2_fast(fmaf(x[16 * g + e], fi, -ref));
+                        const float z = kv8::exp2_fast(fmaf(x[16 * g + e + 1], fi, -ref));
+                        sum += y + z;
+                        p[8 * g + e / 2] = kv8::pack_f16x2(y * by, z * by);
+                    }
+                }
+                tc::store16(s_at + c0 / 2, p);
+            }
+            tc::wait_store();
+            tc::fence_before();
+            __syncwarp();
+            if (lane == 0) tbk::mbar_arrive(&sh.p_full[tile]);
+        }
+        if (fine && steps > 0) fine = wait_all(&sh.o_done[tile], (steps - 1) & 1, a.status);
+        tc::fence_after();
+        const bool none = !(sum != 0.0f);
+        const float per = none || !fine ? 0.0f : exp2f(vref - ref - kLift) / sum;
+        T* out = static_cast<T*>(a.out) + (s.lo + tok) * a.out_stride +
+                 (int64_t)(head * group + hh) * a.d;
+#pragma unroll 1
+        for (int c0 = 0; c0 < DP; c0 += 32) {
+            float x[32];
+            if (steps > 0) {
+                tc::load32(o_at + c0, x);
+            }
+            if (!live) continue;
+#pragma unroll
+            for (int e = 0; e < 32; e += 4) {
+                if (c0 + e >= a.d) break;
+                float y[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) y[i] = none || steps == 0 ? 0.0f : x[e + i] * per;
+                kv8::store4(out + c0 + e, a.vec_out, y);
+            }
+        }
+        if (a.lse && live)
+            a.lse[(int64_t)(s.lo + tok) * a.hq + head * group + hh] =
+                none ? -INFINITY : ref * 0.69314718055994531f + logf(sum);
+    }
+    tc::fence_before();
+    __syncthreads();
+    if (warp == kIssuer) tc::release(tmem, kColumns);
+}
+
+template <int FORMAT, int DP>
+int launch(const Args& a, dim3 grid, cudaStream_t s) {
+    constexpr int bytes = Shape<DP>::kBytes;
+    static std::atomic<uint64_t> granted{0};  // a bit per device
+    const int rc = kv8::once_per_device(granted, [&] {
+        return cudaFuncSetAttribute(k_chunk<FORMAT, DP>,
+                                    cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    });
+    if (rc != TB_OK) return rc;
+    k_chunk<FORMAT, DP><<<grid, kThreads, bytes, s>>>(a);
+    TB_LAUNCH_CHECK("8-bit cache chunk attention kernel");
+    return TB_OK;
+}
+
+int64_t blocks_of(const TbB200Kv8* cache, const TbB200Kv8Batch* batch,
+                  const TbB200Kv8Attention* t) {
+    const int64_t rows = t->max_rows < batch->rows ? t->max_rows : batch->rows;
+    return (rows * (t->n_heads / cache->n_kv_heads) + kTiles * kRows - 1) / (kTiles * kRows);
+}
+
+}  // namespace
+
+namespace kv8 {
+
+bool chunk_suits(const TbB200Kv8* cache, const TbB200Kv8Batch* batch, const TbB200Kv8Attention* t,
+                 int sm_count) {
+    if (t->dtype != TB_DTYPE_BF16 || cache->head_dim > 128) return false;
+    const int64_t group = t->n_heads / cache->n_kv_heads;
+    const int64_t each = blocks_of(cache, batch, t);
+    const int64_t all = batch->rows * group / (kTiles * kRows) * cache->n_kv_heads;
+    return each <= 65535 && t->max_rows * group >= kRows && 2 * all >= sm_count;
+}
+
+int chunk_attention(const TbB200Kv8* cache, const TbB200Kv8Batch* batch,
+                    const TbB200Kv8Attention* t, cudaStream_t stream) {
+    tbh::DeviceState* ds = tbh::current_device_state();
+    if (!ds) return TB_ERR_DEVICE;
+    const Args a = {view(cache, batch),
+                    t->q,
+                    t->out,
+                    t->lse,
+                    t->q_stride,
+                    t->out_stride,
+                    static_cast<const uint8_t*>(cache->k),
+                    static_cast<const uint8_t*>(cache->v),
+                    cache->k_scale,
+                    cache->v_scale,
+                    ds->status,
+                    t->scale,
+                    t->n_heads,
+                    cache->n_kv_heads,
+                    cache->head_dim,
+                    t->window,
+                    t->max_rows,
+                    t->max_len,
+                    tbh::aligned16(t->q) && t->q_stride % 8 == 0,
+                    tbh::aligned16(t->out) && t->out_stride % 8 == 0};
+    const dim3 grid((unsigned)a.hkv, (unsigned)blocks_of(cache, batch, t),
+                    (unsigned)batch->n_seqs);
+    const bool int8 = cache->format == kInt8;
+    if (cache->head_dim <= 64)
+        return int8 ? launch<kInt8, 64>(a, grid, stream) : launch<kE4m3, 64>(a, grid, stream);
+    return int8 ? launch<kInt8, 128>(a, grid, stream) : launch<kE4m3, 128>(a, grid, stream);
+}
+
+}  // namespace kv8

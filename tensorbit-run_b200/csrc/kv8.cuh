@@ -73,6 +73,13 @@ inline Batch view(const TbB200Kv8* c, const TbB200Kv8Batch* b) {
             b->table_width, shift, (int)b->rows, c->n_pages};
 }
 
+// Attention of many rows a sequence (k_kv8_chunk.cu): whether a call's bounds
+// suit it, and the call, checked before.
+bool chunk_suits(const TbB200Kv8* cache, const TbB200Kv8Batch* batch, const TbB200Kv8Attention* t,
+                 int sm_count);
+int chunk_attention(const TbB200Kv8* cache, const TbB200Kv8Batch* batch,
+                    const TbB200Kv8Attention* t, cudaStream_t stream);
+
 // ------------------------------------------------------------------ codes
 // A code's value, and the nearest code (ties to even) of a value within
 // the format's range.

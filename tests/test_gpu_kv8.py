@@ -146,6 +146,49 @@ class Model:
         # what the output may be off by, but for its rounding and p's as f16
         return out, lse, A, A * rel[..., None] + floor, ds + acc + 2.0 ** -21
 
+    def attention_by_head(self, q, starts, lengths, table, window=0, scale=None, bad=()):
+        """attention(), a sequence's rows of one k/v head at a time, for many rows."""
+        rows, heads, d = q.shape
+        scale = d ** -0.5 if scale is None else scale
+        group = heads // self.hkv
+        out, lse = np.zeros(q.shape), np.full((rows, heads), -np.inf)
+        A, floor, ds, n = np.zeros(q.shape), np.zeros(q.shape), np.zeros((rows, heads)), np.zeros(rows)
+        for i, total in enumerate(lengths):
+            m = starts[i + 1] - starts[i]
+            if m <= 0 or total <= 0:
+                continue
+            at = slice(starts[i], starts[i + 1])
+            pages = table[i][:-(-total // self.page)]
+            held = np.repeat([p not in bad for p in pages], self.page)[:total]
+            pages = np.array([0 if p in bad else p for p in pages])
+            p, j = total - m + np.arange(m)[:, None], np.arange(total)
+            see = held & (j <= p) & ((j > p - window) if window else True)
+            n[at] = see.sum(1)
+            for g in range(self.hkv):
+                vs = np.repeat(self.scales[1][pages, g], self.page)[:total]
+                c = self.codes[1][pages, g].reshape(-1, d)[:total]
+                k = (self.codes[0][pages, g] * self.scales[0][pages, g][:, None, None]).reshape(
+                    -1, d)[:total]
+                k, c, vs = np.nan_to_num(k), np.nan_to_num(c), np.nan_to_num(vs)
+                for h in range(g * group, (g + 1) * group):
+                    x = q[at, h]
+                    s = np.where(see, scale * (x @ k.T), -np.inf)
+                    top = np.where(see.any(1), s.max(1), 0.0)[:, None]
+                    e = np.exp(s - top)
+                    z = e.sum(1, keepdims=True)
+                    w = e / np.where(z == 0, 1, z)
+                    out[at, h] = (w * vs) @ c
+                    with np.errstate(divide="ignore"):
+                        lse[at, h] = (top + np.log(z))[:, 0]
+                    A[at, h] = (w * vs) @ np.abs(c)
+                    floor[at, h] = 2.0 ** -35 * (w * vs).max(1)[:, None] * (see @ np.abs(c))
+                    ds[at, h] = abs(scale) * (
+                        np.where(see, np.abs(x) @ np.abs(k).T, 0).max(1) * (d / 16 + 16) * 2.0 ** -23
+                        + np.abs(x).max(1) * np.where(see, np.abs(k).sum(1), 0).max(1) * 2.0 ** -22)
+        acc = (n[:, None] / 16 + 16) * 2.0 ** -23
+        rel = 2 * ds + 2.0 ** -21 + acc
+        return out, lse, A, A * rel[..., None] + floor, ds + acc + 2.0 ** -21
+
 
 def f64(t):
     import torch
@@ -299,7 +342,7 @@ def limit(y, A, lim, bf16):
 
 
 def attend(m, counts, lengths, table, heads, bf16, window=0, scale=None, q=None, bad=(), extra=0,
-           pad=0, **kw):
+           pad=0, by_head=False, **kw):
     import torch
     st = starts_of(counts)
     if q is None:
@@ -308,7 +351,8 @@ def attend(m, counts, lengths, table, heads, bf16, window=0, scale=None, q=None,
     lse = torch.full(q.shape[:2], 7.0, device=m.dev)
     T.kv8_attention(m.cache, q, i32(st, m.dev), i32(lengths, m.dev), i32(table, m.dev),
                     window=window, scale=scale, out=out, lse=lse, **kw)
-    y, z, A, lim, tol = m.attention(f64(q), st, lengths, table, window, scale, bad)
+    f = m.attention_by_head if by_head else m.attention
+    y, z, A, lim, tol = f(f64(q), st, lengths, table, window, scale, bad)
     n = int(st[-1])
     o, ls = f64(out)[:n], f64(lse)[:n]
     lim = limit(y, A, lim, bf16)[:n]
@@ -368,6 +412,61 @@ def test_long_sequences(dev, fmt, bf16, window):
     attend(m, [1, 1, 1], lengths, table, 8, bf16, window=window)
     attend(m, [3, 1, 20], lengths, table, 4, bf16, window=window)
     assert T.check_status() == (0, 0)
+
+
+CHUNKS = [  # page, heads, kv heads, d, rows and lengths of the sequences, window
+    (64, 32, 8, 128, [360, 1, 257, 64], [811, 500, 257, 3000], 0),
+    (16, 32, 2, 64, [130, 490, 5], [130, 1000, 20], 0),
+    (128, 28, 4, 80, [700], [1500], 100),
+    (32, 64, 1, 112, [256, 50], [300, 40], 0),
+    (64, 24, 8, 128, [900, 3], [2500, 129], 700),
+    (16, 16, 16, 16, [1300], [1411], 0)]
+
+
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+@pytest.mark.parametrize("page,heads,hkv,d,counts,lengths,window", CHUNKS)
+def test_chunks_of_prompts(dev, fmt, page, heads, hkv, d, counts, lengths, window):
+    """Calls with many rows a sequence, beside ones with few or more than tokens."""
+    m = Model(dev, fmt, page, hkv, d, sum(-(-t // page) for t in lengths) + 1)
+    table = tables(m.rng, lengths, page, len(m.scales[0]))
+    fill(m, lengths, table)
+    attend(m, counts, lengths, table, heads, True, window=window, extra=3, pad=8, by_head=True)
+    assert T.check_status() == (0, 0)
+
+
+def test_chunk_scales_strides_and_bounds(dev):
+    """Many rows: a zero and a negative scale, unaligned rows, pages of very
+    different scales, a page out of range, a NaN row, a sequence past its bounds."""
+    import torch
+    lengths, counts, heads = [500, 300], [400, 250], 32
+    m = Model(dev, "int8", 64, 8, 128, 14)
+    table = tables(m.rng, lengths, 64, 14)
+    fill(m, lengths, table)
+    for scale in (0.0, -0.3, 0.7):
+        attend(m, counts, lengths, table, heads, True, scale=scale, by_head=True, pad=3)
+    broken = table.copy()
+    broken[0, 2], broken[1, 1] = 14, -1
+    attend(m, counts, lengths, broken, heads, True, bad=(14, -1), by_head=True)
+    attend(m, counts, lengths, broken, heads, True, bad=(14, -1), scale=0.0, by_head=True)
+    assert T.check_status() == (8, T.FLAG_PAGE_RANGE)
+    st, ln, tb = i32(starts_of(counts), dev), i32(lengths, dev), i32(table, dev)
+    q = rows_of(m.rng, sum(counts), heads, 128, True, dev, spread=False).clone()
+    want = T.kv8_attention(m.cache, q, st, ln, tb)
+    q[77, 5, 100] = float("nan")
+    got = T.kv8_attention(m.cache, q, st, ln, tb)
+    assert bool(torch.isnan(got[77, 5]).all())
+    got[77, 5] = want[77, 5]
+    assert torch.equal(got, want)
+    out, lse = T.kv8_attention(m.cache, q, st, ln, tb, max_len=499, return_lse=True)
+    assert bool((out[:400] == 0).all()) and bool(torch.isneginf(lse[:400]).all())
+    assert torch.equal(out[400:], want[400:])
+    assert T.check_status() == (8, T.FLAG_POSITION_RANGE)
+    # pages 2^30 apart
+    for p in range(14):
+        e = [0, -30, 12, -5][p % 4]
+        m.cache.v_scale[p] *= 2.0 ** e
+        m.scales[1][p] *= 2.0 ** e
+    attend(m, counts, lengths, table, heads, True, by_head=True)
 
 
 @pytest.mark.parametrize("bf16", [False, True])
