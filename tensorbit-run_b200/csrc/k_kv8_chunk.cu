@@ -7,9 +7,10 @@
 //   S = Q K^T  [128 x 128], operands f16 in shared memory, sums in tensor memory
 //   P = 2^(S f - r), f16, over S's place in tensor memory
 //   O += P V   P from tensor memory, V f16 in shared memory
-// 13 warps: 4 bring codes from global memory and write them as f16 tiles (two
-// stages), 4 for each row tile compute P, a thread a row, and one thread issues
-// the products, so that one tile's softmax runs while the other's products do.
+// 4 warps bring codes by TMA, each its 32 keys, and write them as f16 tiles (two
+// stages), 4 for each row tile compute P, a thread a row with its 128 scores in
+// registers, and one thread issues the products, so that one tile's softmax runs
+// while the other's products do.
 //
 // What bounds it, per 256 rows and 128 keys: the products, 4 * 128^3 at 4096 a
 // clock, 2050 clocks; the exponentials, 32768 at 16 a clock, as many; converting
@@ -19,9 +20,10 @@
 //
 // Precision as in k_kv8_attention.cu: a row of q is scaled by a power of two to
 // [2^14, 2^15) and held as f16, exact for bf16 elements above 2^-21 of the row's
-// largest; weights are f16 times 2^11 under a reference that moves by whole
-// powers of two; the values' scale joins the weight, p * 2^(log2 v_scale + r - r')
-// with the row's r', in f32 before its rounding.
+// largest; weights are f16 times 2^11 under a reference r' that moves by whole
+// powers of two; the values' scale joins the exponent, 2^(S f + log2 v_scale - r'
+// + 11), and the sum of p takes each page's weights back to the row's r.  That
+// holds for pages whose scales are within 2^100 of one another.
 #include <math.h>
 
 #include "kv8_mma.cuh"
@@ -36,17 +38,19 @@ constexpr int kGroups = kKeys / 16;  // of keys, each in one page
 constexpr int kStages = 2;
 constexpr int kSoftWarps = 4 * kTiles, kConvWarps = 4;
 constexpr int kIssuer = kSoftWarps + kConvWarps;  // the warp
-constexpr int kThreads = 32 * (kIssuer + 1);
+constexpr int kThreads = 32 * (kIssuer + 4);  // a whole warpgroup, for its registers
+// Registers a thread of each: 256 * 192 + 128 * 72 + 128 * 56 = 512 * 128.
+constexpr int kSoftRegs = 192, kConvRegs = 72, kIssuerRegs = 56;
 constexpr float kSlack = 4.0f, kLift = 11.0f, kLog2e = 1.4426950408889634f, kNoRef = -3.0e38f;
 constexpr uint32_t kColumns = 512;  // of tensor memory: S and P at 0, 128, O at 256, 384
 
 struct Args {
+    CUtensorMap k_map, v_map;  // [n_pages * n_kv_heads][page][d] codes
     kv8::Batch b;
     const void* q;
     void* out;
     float* lse;
     int64_t q_stride, out_stride;
-    const uint8_t *k, *v;
     const float *k_scale, *v_scale;
     unsigned* status;
     float scale;
@@ -58,12 +62,15 @@ struct Shape {
     static constexpr int kPanels = DP / 64;
     static constexpr int kPanel = 128 * 128;  // bytes of 128 rows of 64 f16
     static constexpr int kTile = kPanels * kPanel;
-    static constexpr int kBytes = kTiles * kTile + kStages * 2 * kTile + 1024;  // 1024: to align
+    static constexpr int kCodes = 2 * kKeys * DP;  // a step's K and V as they are
+    static constexpr int kBytes =
+        kTiles * kTile + kStages * 2 * kTile + kCodes + 1024;  // 1024: to align
 };
 
 struct Shared {
     uint64_t k_full[kStages], v_full[kStages], kv_free[kStages];
     uint64_t s_full[kTiles], p_full[kTiles], o_done[kTiles];
+    uint64_t codes[2][kConvWarps];  // of K, of V: the warp's have come
     float2 scales[kStages][kGroups];  // of K (< 0: no page) and log2 of V's
     uint32_t tmem;
 };
@@ -71,6 +78,29 @@ struct Shared {
 // Where the f16 element e of row r of a tile of 64-element panels lies.
 __device__ __forceinline__ int place(int row, int piece) {  // 16-byte pieces of 8 elements
     return (piece >> 3) * (128 * 128) + row * 128 + ((piece ^ row) & 7) * 16;
+}
+
+// Two f32 at once.
+__device__ __forceinline__ float2 fma2(float2 a, float b, float c) {
+    float2 d;
+    asm("{\n .reg .b64 a, b, c, d;\n mov.b64 a, {%2, %3};\n mov.b64 b, {%4, %4};\n"
+        " mov.b64 c, {%5, %5};\n fma.rn.f32x2 d, a, b, c;\n mov.b64 {%0, %1}, d;\n}"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b), "f"(c));
+    return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    float2 d;
+    asm("{\n .reg .b64 a, b, d;\n mov.b64 a, {%2, %3};\n mov.b64 b, {%4, %5};\n"
+        " add.rn.f32x2 d, a, b;\n mov.b64 {%0, %1}, d;\n}"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
 }
 
 // A bounded wait of a whole warp.
@@ -137,6 +167,10 @@ __global__ void __launch_bounds__(kThreads, 1) k_chunk(const __grid_constant__ A
             tbk::mbar_init(&sh.p_full[i], 4);
             tbk::mbar_init(&sh.o_done[i], 1);
         }
+        for (int i = 0; i < kConvWarps; ++i) {
+            tbk::mbar_init(&sh.codes[0][i], 1);
+            tbk::mbar_init(&sh.codes[1][i], 1);
+        }
         tbk::fence_mbar_init();
     }
     if (warp == kIssuer) tc::allocate(&sh.tmem, kColumns);
@@ -179,8 +213,9 @@ __global__ void __launch_bounds__(kThreads, 1) k_chunk(const __grid_constant__ A
     tc::fence_after();
     const uint32_t tmem = sh.tmem;
 
-    if (warp == kIssuer) {
-        if (lane == 0 && steps > 0) {
+    if (warp >= kIssuer) {
+        tc::fewer_registers<kIssuerRegs>();
+        if (warp == kIssuer && lane == 0 && steps > 0) {
             const uint32_t instr_s = tc::f16_instruction(kKeys, false);
             const uint32_t instr_o = tc::f16_instruction(DP, true);
             const uint32_t q_at = tbk::smem_addr(q_tiles), kv_at = tbk::smem_addr(kv_tiles);
@@ -228,77 +263,105 @@ __global__ void __launch_bounds__(kThreads, 1) k_chunk(const __grid_constant__ A
         }
         __syncwarp();
     } else if (!soft) {
-        // codes to f16: a thread pieces c of keys k, k + 16, ..
-        const int tid = threadIdx.x - 32 * kSoftWarps, c = tid % 8, k0 = tid / 8;
+        tc::fewer_registers<kConvRegs>();
+        // Codes to f16.  The warp has keys 32 w .. 32 w + 31 of each step, two groups
+        // of 16 whose pages lanes 0 and 1 look up, ask for and ring in; a lane has
+        // the 16-byte piece c of every (32 / kPieces)th of them.
+        constexpr int kPieces = DP / 16, kRound = 32 / kPieces;
+        const int w = warp - kSoftWarps, c = lane % kPieces;
+        uint8_t* codes = kv_tiles + kStages * 2 * H::kTile + w * 2 * 32 * DP;  // K, V
         const int32_t* table = a.b.table + seq * a.b.table_stride;
-        uint4 held[2][kGroups];
-        float2 scale;  // of group tid (of kGroups), asked for with the codes
-        int ids[kGroups];
-        auto pages = [&](int j) {
-#pragma unroll
-            for (int i = 0; i < kGroups; ++i) {
-                const int key = from + j * kKeys + 16 * i;
-                ids[i] = key < end ? table[key >> a.b.page_shift] : -1;
-            }
+        const int first = from + 32 * w;  // the warp's first key of step 0
+        auto page_of = [&](int j) {  // lane's group's page of step j, -1 if none
+            const int key = first + j * kKeys + 16 * lane;
+            if (lane > 1 || j >= steps || key >= end) return -1;
+            const int id = table[key >> a.b.page_shift];
+            if ((unsigned)id < (unsigned)a.b.n_pages) return id;
+            atomicOr(a.status, TB_B200_FLAG_PAGE_RANGE);
+            return -1;
         };
-        auto ask = [&](int j) {
+        auto ask = [&](int kv, int j, int id) {  // the groups that have a page
+            const uint32_t have = __ballot_sync(tbk::kFull, id >= 0);
+            if (lane == 0 && have) tbk::mbar_expect_tx(&sh.codes[kv][w], __popc(have) * 16 * DP);
+            __syncwarp();
+            if (id >= 0) {
+                const int slot = (first + j * kKeys + 16 * lane) & ((1 << a.b.page_shift) - 1);
+                kv8::tma_load3(codes + (kv * 32 + 16 * lane) * DP, kv ? &a.v_map : &a.k_map, 0,
+                               slot, id * a.hkv + head, &sh.codes[kv][w]);
+            }
+            return have;
+        };
+        int id = page_of(0), id_next = page_of(1);
+        uint32_t have_k = ask(0, 0, id), have_v = ask(1, 0, id), phases = 0;
+        float2 scale = make_float2(-1.0f, 0.0f);
+        auto ask_scale = [&] {
             scale = make_float2(-1.0f, 0.0f);
-#pragma unroll
-            for (int i = 0; i < kGroups; ++i) {
-                const int key0 = from + j * kKeys + 16 * i, key = key0 + k0;
-                const bool page = ids[i] >= 0 && ids[i] < a.b.n_pages;
-                if (key0 < end && !page) atomicOr(a.status, TB_B200_FLAG_PAGE_RANGE);
-                held[0][i] = held[1][i] = make_uint4(0, 0, 0, 0);
-                if (!page) continue;
-                const int64_t unit = (int64_t)ids[i] * a.hkv + head;
-                if (i == tid) scale = make_float2(a.k_scale[unit], a.v_scale[unit]);
-                if (key >= s.len || c * 16 >= a.d) continue;
-                const int slot = key & ((1 << a.b.page_shift) - 1);
-                const int64_t from_ = ((unit << a.b.page_shift) + slot) * a.d + c * 16;
-                held[0][i] = *reinterpret_cast<const uint4*>(a.k + from_);
-                held[1][i] = *reinterpret_cast<const uint4*>(a.v + from_);
-            }
+            if (id >= 0)
+                scale = make_float2(a.k_scale[id * a.hkv + head], a.v_scale[id * a.hkv + head]);
         };
-        if (steps > 0) {
-            pages(0);
-            ask(0);
-            if (steps > 1) pages(1);
-        }
-        for (int j = 0; j < steps; ++j) {
-            const int stage = j % kStages;
-            if (j >= kStages && !wait_all(&sh.kv_free[stage], (j / kStages - 1) & 1, a.status))
-                break;
+        ask_scale();
+        bool fine = true;
+        for (int j = 0; j < steps && fine; ++j) {
+            const int stage = j % kStages, key0 = first + j * kKeys;
+            fine = j < kStages || wait_all(&sh.kv_free[stage], (j / kStages - 1) & 1, a.status);
+            if (!fine) break;
             uint8_t* to = kv_tiles + stage * 2 * H::kTile;
-            if (tid < kGroups)
-                sh.scales[stage][tid] = make_float2(
+            if (lane < 2)
+                sh.scales[stage][2 * w + lane] = make_float2(
                     scale.x, (float)((int)(__float_as_uint(scale.y) >> 23) - 127));
+            id = id_next;
+            id_next = page_of(j + 2);
 #pragma unroll
             for (int kv = 0; kv < 2; ++kv) {
-                if (c * 16 < DP) {
+                const uint32_t have = kv ? have_v : have_k;
+                if (have) {
+                    fine = wait_all(&sh.codes[kv][w], phases >> kv & 1, a.status);
+                    phases ^= 1u << kv;
+                }
+                if (!fine) break;
+                uint4 x[kPieces];
 #pragma unroll
-                    for (int i = 0; i < kGroups; ++i) {
-                        uint4 h[2];
-                        to_f16<FORMAT>(held[kv][i], h);
-                        // the lanes of a key's second panel write their pieces in
-                        // the other order, into other banks
-                        const int key = k0 + 16 * i, x = c >> 2;
-                        uint8_t* tile_at = to + kv * H::kTile;
-                        *reinterpret_cast<uint4*>(tile_at + place(key, 2 * c + x)) =
-                            x ? h[1] : h[0];
-                        *reinterpret_cast<uint4*>(tile_at + place(key, 2 * c + 1 - x)) =
-                            x ? h[0] : h[1];
+                for (int i = 0; i < kPieces; ++i)
+                    x[i] = *reinterpret_cast<const uint4*>(
+                        codes + (kv * 32 + lane / kPieces + i * kRound) * DP + c * 16);
+                if (have != 3 || key0 + 32 > s.len) {
+                    // slots of no page or behind the last token may hold anything
+#pragma unroll
+                    for (int i = 0; i < kPieces; ++i) {
+                        const int key = lane / kPieces + i * kRound;
+                        if (!(have >> key / 16 & 1) || key0 + key >= s.len)
+                            x[i] = make_uint4(0, 0, 0, 0);
                     }
+                }
+                // all lanes have their codes: the next step's may come
+                tbk::fence_proxy_async_shared();
+                __syncwarp();
+                (kv ? have_v : have_k) = ask(kv, j + 1, id);
+#pragma unroll
+                for (int i = 0; i < kPieces; ++i) {
+                    uint4 h[2];
+                    to_f16<FORMAT>(x[i], h);
+                    // the lanes of a key's second panel write their pieces in the
+                    // other order, into other banks
+                    const int key = 32 * w + lane / kPieces + i * kRound, y = c >> 2;
+                    uint8_t* tile_at = to + kv * H::kTile;
+                    *reinterpret_cast<uint4*>(tile_at + place(key, 2 * c + y)) = y ? h[1] : h[0];
+                    *reinterpret_cast<uint4*>(tile_at + place(key, 2 * c + 1 - y)) =
+                        y ? h[0] : h[1];
                 }
                 tbk::fence_proxy_async_shared();
                 __syncwarp();
                 if (lane == 0) tbk::mbar_arrive(kv ? &sh.v_full[stage] : &sh.k_full[stage]);
             }
-            if (j + 1 < steps) {
-                ask(j + 1);
-                if (j + 2 < steps) pages(j + 2);
-            }
+            ask_scale();
         }
-    } else if (tile < tiles) {
+        if (!fine) {  // no copy may be in flight when the block ends
+            if (have_k) wait_all(&sh.codes[0][w], phases & 1, a.status);
+            if (have_v) wait_all(&sh.codes[1][w], phases >> 1 & 1, a.status);
+        }
+    } else {
+        tc::more_registers<kSoftRegs>();
+        if (tile < tiles) {
         const uint32_t s_at = tmem + tile * 128 + ((uint32_t)(warp % 4) << 21);
         const uint32_t o_at = s_at + 256;
         const int see_hi = live ? s.first + tok : INT32_MAX;
@@ -323,34 +386,27 @@ __global__ void __launch_bounds__(kThreads, 1) k_chunk(const __grid_constant__ A
             const bool inside =
                 __all_sync(tbk::kFull, key0 >= see_lo && key0 + kKeys - 1 <= see_hi &&
                                            have == (1u << kGroups) - 1);
-            // 32 columns: sums of products, or, of a step with keys that a row does
-            // not see, scores
-            auto columns = [&](int c0, float (&x)[32]) {
-                tc::load32(s_at + c0, x);
-                if (inside) return;
+            // sums of products, or, of a step with keys that a row does not see, scores
+            float x[kKeys];
+            tc::load<kKeys>(s_at, x);
+            if (!inside) {
 #pragma unroll
-                for (int e = 0; e < 32; ++e) {
-                    const int key = key0 + c0 + e, i = (c0 + e) / 16;
-                    const bool seen = key >= see_lo && key <= see_hi && (have >> i & 1);
-                    x[e] = seen ? x[e] * fs[i] : -INFINITY;
+                for (int e = 0; e < kKeys; ++e) {
+                    const bool seen = key0 + e >= see_lo && key0 + e <= see_hi && (have >> e / 16 & 1);
+                    x[e] = seen ? x[e] * fs[e / 16] : -INFINITY;
                 }
-            };
+            }
             // the largest score, and with the values' scale
             float hi = -INFINITY, hv = -INFINITY;
 #pragma unroll
-            for (int c0 = 0; c0 < kKeys; c0 += 32) {
-                float x[32];
-                columns(c0, x);
+            for (int i = 0; i < kGroups; ++i) {
+                float m = max3(x[16 * i], x[16 * i + 1], x[16 * i + 2]);
 #pragma unroll
-                for (int g = 0; g < 2; ++g) {
-                    float m = x[16 * g];
-#pragma unroll
-                    for (int e = 1; e < 16; ++e) m = fmaxf(m, x[16 * g + e]);
-                    const int i = c0 / 16 + g;
-                    if (inside) m *= fs[i];
-                    hi = fmaxf(hi, m);
-                    hv = fmaxf(hv, m + lv[i]);
-                }
+                for (int e = 3; e < 15; e += 2) m = max3(m, x[16 * i + e], x[16 * i + e + 1]);
+                m = fmaxf(m, x[16 * i + 15]);
+                if (inside) m *= fs[i];
+                hi = fmaxf(hi, m);
+                hv = fmaxf(hv, m + lv[i]);
             }
             const bool over = hi > ref + kSlack || hv > vref + kSlack;
             if (__any_sync(tbk::kFull, over)) {
@@ -365,34 +421,36 @@ __global__ void __launch_bounds__(kThreads, 1) k_chunk(const __grid_constant__ A
                     const float keep = exp2f(vref - mv);
 #pragma unroll 1
                     for (int c0 = 0; c0 < DP; c0 += 32) {
-                        float x[32];
-                        tc::load32(o_at + c0, x);
+                        float o[32];
+                        tc::load<32>(o_at + c0, o);
 #pragma unroll
-                        for (int e = 0; e < 32; ++e) x[e] *= keep;
-                        tc::store32(o_at + c0, x);
+                        for (int e = 0; e < 32; ++e) o[e] *= keep;
+                        tc::store32(o_at + c0, o);
                     }
                     tc::wait_store();
                 }
                 ref = m;
                 vref = mv;
             }
+            // weights times the values' scale; a group's sum back without it
 #pragma unroll
             for (int c0 = 0; c0 < kKeys; c0 += 32) {
-                float x[32];
-                columns(c0, x);
                 uint32_t p[16];
 #pragma unroll
                 for (int g = 0; g < 2; ++g) {
                     const int i = c0 / 16 + g;
-                    const float by = kv8::exp2_fast(lv[i] + ref - vref + kLift);
+                    const float up = lv[i] - vref + kLift;
                     const float fi = inside ? fs[i] : 1.0f;
+                    float2 part = make_float2(0.0f, 0.0f);
 #pragma unroll
                     for (int e = 0; e < 16; e += 2) {
-                        const float y = kv8::exp2_fast(fmaf(x[16 * g + e], fi, -ref));
-                        const float z = kv8::exp2_fast(fmaf(x[16 * g + e + 1], fi, -ref));
-                        sum += y + z;
-                        p[8 * g + e / 2] = kv8::pack_f16x2(y * by, z * by);
+                        float2 y = fma2(make_float2(x[16 * i + e], x[16 * i + e + 1]), fi, up);
+                        y.x = kv8::exp2_fast(y.x);
+                        y.y = kv8::exp2_fast(y.y);
+                        part = add2(part, y);
+                        p[8 * g + e / 2] = kv8::pack_f16x2(y.x, y.y);
                     }
+                    sum = fmaf(part.x + part.y, kv8::exp2_fast(fminf(-up - ref, 126.0f)), sum);
                 }
                 tc::store16(s_at + c0 / 2, p);
             }
@@ -410,9 +468,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_chunk(const __grid_constant__ A
 #pragma unroll 1
         for (int c0 = 0; c0 < DP; c0 += 32) {
             float x[32];
-            if (steps > 0) {
-                tc::load32(o_at + c0, x);
-            }
+            if (steps > 0) tc::load<32>(o_at + c0, x);
             if (!live) continue;
 #pragma unroll
             for (int e = 0; e < 32; e += 4) {
@@ -426,6 +482,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_chunk(const __grid_constant__ A
         if (a.lse && live)
             a.lse[(int64_t)(s.lo + tok) * a.hq + head * group + hh] =
                 none ? -INFINITY : ref * 0.69314718055994531f + logf(sum);
+        }
     }
     tc::fence_before();
     __syncthreads();
@@ -433,13 +490,15 @@ __global__ void __launch_bounds__(kThreads, 1) k_chunk(const __grid_constant__ A
 }
 
 template <int FORMAT, int DP>
-int launch(const Args& a, dim3 grid, cudaStream_t s) {
+int launch(Args& a, const TbB200Kv8* cache, dim3 grid, cudaStream_t s) {
     constexpr int bytes = Shape<DP>::kBytes;
     static std::atomic<uint64_t> granted{0};  // a bit per device
-    const int rc = kv8::once_per_device(granted, [&] {
+    int rc = kv8::once_per_device(granted, [&] {
         return cudaFuncSetAttribute(k_chunk<FORMAT, DP>,
                                     cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
     });
+    if (rc == TB_OK) rc = kv8::tile_map(&a.k_map, cache, cache->k, DP, 16, false);
+    if (rc == TB_OK) rc = kv8::tile_map(&a.v_map, cache, cache->v, DP, 16, false);
     if (rc != TB_OK) return rc;
     k_chunk<FORMAT, DP><<<grid, kThreads, bytes, s>>>(a);
     TB_LAUNCH_CHECK("8-bit cache chunk attention kernel");
@@ -469,32 +528,33 @@ int chunk_attention(const TbB200Kv8* cache, const TbB200Kv8Batch* batch,
                     const TbB200Kv8Attention* t, cudaStream_t stream) {
     tbh::DeviceState* ds = tbh::current_device_state();
     if (!ds) return TB_ERR_DEVICE;
-    const Args a = {view(cache, batch),
-                    t->q,
-                    t->out,
-                    t->lse,
-                    t->q_stride,
-                    t->out_stride,
-                    static_cast<const uint8_t*>(cache->k),
-                    static_cast<const uint8_t*>(cache->v),
-                    cache->k_scale,
-                    cache->v_scale,
-                    ds->status,
-                    t->scale,
-                    t->n_heads,
-                    cache->n_kv_heads,
-                    cache->head_dim,
-                    t->window,
-                    t->max_rows,
-                    t->max_len,
-                    tbh::aligned16(t->q) && t->q_stride % 8 == 0,
-                    tbh::aligned16(t->out) && t->out_stride % 8 == 0};
+    Args a = {};
+    a.b = view(cache, batch);
+    a.q = t->q;
+    a.out = t->out;
+    a.lse = t->lse;
+    a.q_stride = t->q_stride;
+    a.out_stride = t->out_stride;
+    a.k_scale = cache->k_scale;
+    a.v_scale = cache->v_scale;
+    a.status = ds->status;
+    a.scale = t->scale;
+    a.hq = t->n_heads;
+    a.hkv = cache->n_kv_heads;
+    a.d = cache->head_dim;
+    a.window = t->window;
+    a.max_rows = t->max_rows;
+    a.max_len = t->max_len;
+    a.vec = tbh::aligned16(t->q) && t->q_stride % 8 == 0;
+    a.vec_out = tbh::aligned16(t->out) && t->out_stride % 8 == 0;
     const dim3 grid((unsigned)a.hkv, (unsigned)blocks_of(cache, batch, t),
                     (unsigned)batch->n_seqs);
     const bool int8 = cache->format == kInt8;
     if (cache->head_dim <= 64)
-        return int8 ? launch<kInt8, 64>(a, grid, stream) : launch<kE4m3, 64>(a, grid, stream);
-    return int8 ? launch<kInt8, 128>(a, grid, stream) : launch<kE4m3, 128>(a, grid, stream);
+        return int8 ? launch<kInt8, 64>(a, cache, grid, stream)
+                    : launch<kE4m3, 64>(a, cache, grid, stream);
+    return int8 ? launch<kInt8, 128>(a, cache, grid, stream)
+                : launch<kE4m3, 128>(a, cache, grid, stream);
 }
 
 }  // namespace kv8

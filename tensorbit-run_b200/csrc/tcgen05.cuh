@@ -76,22 +76,34 @@ __device__ __forceinline__ void release(uint32_t address, uint32_t columns) {
                  : "memory");
 }
 
-// 32 columns of the warp's 32 rows, a row a lane.
-__device__ __forceinline__ void load32(uint32_t address, float (&v)[32]) {
-    uint32_t r[32];
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
-        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
-        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
-          "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
-          "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]),
-          "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]),
-          "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-        : "r"(address));
+// COLUMNS columns (a multiple of 32) of the warp's 32 rows, a row a lane: asked
+// for all at once, waited for once.  The values pass through the wait, so that
+// nothing computes with them before it.
+template <int COLUMNS>
+__device__ __forceinline__ void load(uint32_t address, float (&v)[COLUMNS]) {
+#pragma unroll
+    for (int i = 0; i < COLUMNS; i += 32) {
+        float* r = v + i;
+        asm volatile(
+            "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+            "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+            "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+            : "=f"(r[0]), "=f"(r[1]), "=f"(r[2]), "=f"(r[3]), "=f"(r[4]), "=f"(r[5]), "=f"(r[6]),
+              "=f"(r[7]), "=f"(r[8]), "=f"(r[9]), "=f"(r[10]), "=f"(r[11]), "=f"(r[12]),
+              "=f"(r[13]), "=f"(r[14]), "=f"(r[15]), "=f"(r[16]), "=f"(r[17]), "=f"(r[18]),
+              "=f"(r[19]), "=f"(r[20]), "=f"(r[21]), "=f"(r[22]), "=f"(r[23]), "=f"(r[24]),
+              "=f"(r[25]), "=f"(r[26]), "=f"(r[27]), "=f"(r[28]), "=f"(r[29]), "=f"(r[30]),
+              "=f"(r[31])
+            : "r"(address + i));
+    }
     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
-    for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+    for (int i = 0; i < COLUMNS; i += 8) {
+        float* r = v + i;
+        asm volatile(""
+                     : "+f"(r[0]), "+f"(r[1]), "+f"(r[2]), "+f"(r[3]), "+f"(r[4]), "+f"(r[5]),
+                       "+f"(r[6]), "+f"(r[7]));
+    }
 }
 __device__ __forceinline__ void store32(uint32_t address, const float (&v)[32]) {
     uint32_t r[32];
@@ -117,6 +129,16 @@ __device__ __forceinline__ void store16(uint32_t address, const uint32_t (&r)[16
         "r"(r[15])
         : "memory");
 }
+// The warpgroup's registers per thread; the shares add up to the launch's.
+template <int N>
+__device__ __forceinline__ void more_registers() {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void fewer_registers() {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
+
 __device__ __forceinline__ void wait_store() {
     asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
 }

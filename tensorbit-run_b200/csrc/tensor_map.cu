@@ -35,7 +35,8 @@ int encode_tiles_u8(CUtensorMap* map, const void* base, const uint64_t dims[3],
         map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(base),
         reinterpret_cast<const cuuint64_t*>(dims), reinterpret_cast<const cuuint64_t*>(strides),
         box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
-        swizzle == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
+        swizzle == 0 ? CU_TENSOR_MAP_SWIZZLE_NONE
+                     : swizzle == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
         CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (rc != CUDA_SUCCESS) {
         char text[96];
