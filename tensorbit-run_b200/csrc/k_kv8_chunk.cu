@@ -9,7 +9,7 @@
 //   O += P V   P from tensor memory, V f16 in shared memory
 // 4 warps bring codes by TMA, each its 32 keys, and write them as f16 tiles (two
 // stages), 4 for each row tile compute P, a thread a row with its 128 scores in
-// registers, and one thread issues the products, so that one tile's softmax runs
+// registers, and one warp issues the products, so that one tile's softmax runs
 // while the other's products do.
 //
 // What bounds it, per 256 rows and 128 keys: the products, 4 * 128^3 at 4096 a
@@ -215,44 +215,46 @@ __global__ void __launch_bounds__(kThreads, 1) k_chunk(const __grid_constant__ A
 
     if (warp >= kIssuer) {
         tc::fewer_registers<kIssuerRegs>();
-        if (warp == kIssuer && lane == 0 && steps > 0) {
+        if (warp == kIssuer && steps > 0) {
+            const bool leader = lane == 0;
             const uint32_t instr_s = tc::f16_instruction(kKeys, false);
             const uint32_t instr_o = tc::f16_instruction(DP, true);
-            const uint32_t q_at = tbk::smem_addr(q_tiles), kv_at = tbk::smem_addr(kv_tiles);
+            // descriptors count their start in units of 16 bytes
+            const uint64_t q_desc = tc::tile_descriptor(tbk::smem_addr(q_tiles), 16);
+            const uint64_t k_desc = tc::tile_descriptor(tbk::smem_addr(kv_tiles), 16);
+            const uint64_t v_desc =
+                tc::tile_descriptor(tbk::smem_addr(kv_tiles) + H::kTile, H::kPanel);
             auto scores = [&](int t, int j) {  // S of tile t and step j
-                const uint32_t k_at = kv_at + (j % kStages) * 2 * H::kTile;
+                const uint64_t q = q_desc + t * (H::kTile / 16);
+                const uint64_t k = k_desc + (j % kStages) * (2 * H::kTile / 16);
 #pragma unroll
                 for (int i = 0; i < kSteps; ++i) {
-                    const uint32_t off = i / 4 * H::kPanel + i % 4 * 32;
-                    tc::mma(tmem + t * 128, tc::tile_descriptor(q_at + t * H::kTile + off, 16),
-                            tc::tile_descriptor(k_at + off, 16), instr_s, i > 0);
+                    const int off = (i / 4 * H::kPanel + i % 4 * 32) / 16;
+                    tc::mma(tmem + t * 128, q + off, k + off, instr_s, i > 0, leader);
                 }
-                tc::commit(&sh.s_full[t]);
+                tc::commit(&sh.s_full[t], leader);
             };
-            auto wait = [&](uint64_t* bar, int phase) {
-                return tbk::mbar_wait(bar, phase & 1, a.status, 1000000000ull);
-            };
-            bool fine = wait(&sh.k_full[0], 0);
+            bool fine = wait_all(&sh.k_full[0], 0, a.status);
             tc::fence_after();
             for (int t = 0; t < tiles && fine; ++t) scores(t, 0);
             for (int j = 0; j < steps && fine; ++j) {
                 const int stage = j % kStages;
-                const uint32_t v_at = kv_at + stage * 2 * H::kTile + H::kTile;
-                fine = wait(&sh.v_full[stage], j / kStages);
+                const uint64_t v = v_desc + stage * (2 * H::kTile / 16);
+                fine = wait_all(&sh.v_full[stage], j / kStages & 1, a.status);
                 for (int t = 0; t < tiles && fine; ++t) {
-                    fine = wait(&sh.p_full[t], j);
+                    fine = wait_all(&sh.p_full[t], j & 1, a.status);
                     if (!fine) break;
                     tc::fence_after();
 #pragma unroll
                     for (int i = 0; i < kKeys / 16; ++i)
                         tc::mma_tmem(tmem + 256 + t * 128, tmem + t * 128 + i * 8,
-                                     tc::tile_descriptor(v_at + i * 2048, H::kPanel), instr_o,
-                                     j > 0 || i > 0);
-                    tc::commit(&sh.o_done[t]);
-                    if (t == tiles - 1) tc::commit(&sh.kv_free[stage]);
+                                     v + i * (2048 / 16), instr_o, j > 0 || i > 0, leader);
+                    tc::commit(&sh.o_done[t], leader);
+                    if (t == tiles - 1) tc::commit(&sh.kv_free[stage], leader);
                     if (j + 1 < steps) {
                         if (t == 0) {
-                            fine = wait(&sh.k_full[(j + 1) % kStages], (j + 1) / kStages);
+                            fine = wait_all(&sh.k_full[(j + 1) % kStages], (j + 1) / kStages & 1,
+                                            a.status);
                             if (!fine) break;
                             tc::fence_after();
                         }
@@ -261,7 +263,6 @@ __global__ void __launch_bounds__(kThreads, 1) k_chunk(const __grid_constant__ A
                 }
             }
         }
-        __syncwarp();
     } else if (!soft) {
         tc::fewer_registers<kConvRegs>();
         // Codes to f16.  The warp has keys 32 w .. 32 w + 31 of each step, two groups

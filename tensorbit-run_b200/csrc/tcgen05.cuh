@@ -30,29 +30,34 @@ constexpr uint32_t f16_instruction(int n, bool right_mn_major) {
            (uint32_t)(128 / 16) << 24;
 }
 
+// The instructions below are for a whole warp, whose lane `leader` issues them:
+// the operands stay uniform, and no lane waits for another's branch.
+//
 // d (tensor memory) = a b, or += if `add`; a in shared memory.
 __device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t instruction,
-                                    bool add) {
+                                    bool add, bool leader) {
     asm volatile(
-        "{\n .reg .pred p;\n setp.ne.u32 p, %4, 0;\n"
-        " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d),
-        "l"(a), "l"(b), "r"(instruction), "r"((uint32_t)add)
+        "{\n .reg .pred p, q;\n setp.ne.u32 p, %4, 0;\n setp.ne.u32 q, %5, 0;\n"
+        " @q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d),
+        "l"(a), "l"(b), "r"(instruction), "r"((uint32_t)add), "r"((uint32_t)leader)
         : "memory");
 }
 // The same, a in tensor memory (two f16 a column).
 __device__ __forceinline__ void mma_tmem(uint32_t d, uint32_t a, uint64_t b, uint32_t instruction,
-                                         bool add) {
+                                         bool add, bool leader) {
     asm volatile(
-        "{\n .reg .pred p;\n setp.ne.u32 p, %4, 0;\n"
-        " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}" ::"r"(d),
-        "r"(a), "l"(b), "r"(instruction), "r"((uint32_t)add)
+        "{\n .reg .pred p, q;\n setp.ne.u32 p, %4, 0;\n setp.ne.u32 q, %5, 0;\n"
+        " @q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}" ::"r"(d),
+        "r"(a), "l"(b), "r"(instruction), "r"((uint32_t)add), "r"((uint32_t)leader)
         : "memory");
 }
-// Arrive on bar when the products issued so far by this thread are done.
-__device__ __forceinline__ void commit(uint64_t* bar) {
+// Arrive on bar when the products issued so far by the leader are done.
+__device__ __forceinline__ void commit(uint64_t* bar, bool leader) {
     asm volatile(
-        "tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
-            tbk::smem_addr(bar))
+        "{\n .reg .pred q;\n setp.ne.u32 q, %1, 0;\n"
+        " @q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}" ::"r"(
+            tbk::smem_addr(bar)),
+        "r"((uint32_t)leader)
         : "memory");
 }
 __device__ __forceinline__ void fence_before() {
