@@ -13,10 +13,9 @@
 // Within a CTA each of 4 warps takes every fourth step of 32 keys (16 for heads
 // over 128) through a ring of TMA stages of its own: one lane issues the copies,
 // and no barrier of the CTA is in the loop.
-//   S^T = K Q^T, m16n8k32 on the codes as they are, ldmatrix their registers.  Q
-//     is split into two to six parts of the format (QParts): matrix instructions
-//     on 8-bit operands cost a half (int8) or a quarter (e4m3) of an f16 one per
-//     product, conversions of the codes more than all of them;
+//   S^T = K Q^T, ldmatrix the codes' registers: int8 codes as they are
+//     (m16n8k32, Q as three digits: an 8-bit product costs half an f16 one, the
+//     codes' conversion more than all of them), e4m3 codes as f16 (QParts);
 //   O^T = V^T P^T, m16n8k16 on f16: S^T's registers, transposed 8 x 8, are P^T's
 //     operands; lane (g, t) (g = lane / 4, t = lane % 4) holds elements 16 g ..
 //     16 g + 15 (of 128) of keys 2t, 2t + 1, 2t + 8 and 2t + 9 with 16-byte
@@ -153,9 +152,9 @@ struct Shape {
     static constexpr int kWords = DP / 16;  // words of four elements a lane has of a row of q
     static constexpr int kRows = 8 * NB;
     // Q's operands stay in registers when they are few
-    static constexpr int kParts = kv8::QParts<T, FORMAT>::kParts;
-    static constexpr bool kQReg = kParts * kWords * NB <= 32;
-    static constexpr int kQBytes = kParts * kWords * NB * 128;
+    static constexpr int kQPairs = kv8::QParts<T, FORMAT>::kRegs * kWords / 2;
+    static constexpr bool kQReg = kQPairs * NB <= 16;
+    static constexpr int kQBytes = kQPairs * NB * 256;
     static constexpr int kRing = kWarps * kStages * kStageBytes;  // a multiple of 1024
     static constexpr int kPitch = DP == 64 ? DP + 2 : DP + 4;  // floats of a row's state
     static constexpr int kJoin = kWarps * kRows * (kPitch + 4) * 4;
@@ -191,7 +190,7 @@ k_attend(const __grid_constant__ Args a) {
     using Q = kv8::QParts<T, FORMAT>;
     constexpr bool kSplit = H::kSplit, kQReg = H::kQReg;
     constexpr int kStages = H::kStages, kRows = H::kRows, kKeys = H::kKeys;
-    constexpr int kHalves = H::kHalves, kParts = H::kParts, kWords = H::kWords;
+    constexpr int kHalves = H::kHalves, kQPairs = H::kQPairs, kWords = H::kWords;
     constexpr int kStride = kWarps * kKeys;  // from one of a warp's steps to its next
     constexpr int kTiles = DP / 16;          // 16-wide output tiles
     extern __shared__ uint8_t smem_raw[];
@@ -391,12 +390,16 @@ k_attend(const __grid_constant__ Args a) {
             qf[b] = top < INFINITY ? parts.unit * (a.scale * kLog2e) : NAN;
 #pragma unroll
             for (int j = 0; j < kMine; ++j) {
-                uint32_t w[kParts];
+                uint32_t w[Q::kRegs];
                 parts.split(x[b][j], w);
+                // pairs of registers: int8 of two words, e4m3 of one
                 const int word = warp + kWarps * j;
 #pragma unroll
-                for (int p = 0; p < kParts; ++p)
-                    qs[(((p * kWords + word) / 2 * NB + b) * 32 + lane) * 2 + word % 2] = w[p];
+                for (int p = 0; p < Q::kRegs; ++p) {
+                    const int at = FORMAT == kv8::kInt8 ? p * kWords + word
+                                                        : (p / 2 * kWords + word) * 2 + p % 2;
+                    qs[((at / 2 * NB + b) * 32 + lane) * 2 + at % 2] = w[p];
+                }
             }
         }
         // S^T's columns: rows 8 b + 2 t + e, keys [see_lo, see_hi] each
@@ -415,16 +418,19 @@ k_attend(const __grid_constant__ Args a) {
                 see_lo[b][e] = a.window && live ? max(p - a.window + 1, 0) : 0;
             }
         __syncthreads();
-        uint2 qr[kQReg ? kParts : 1][kQReg ? kWords / 2 : 1][NB];
+        uint2 qr[kQReg ? kQPairs : 1][NB];
         if constexpr (kQReg) {
 #pragma unroll
-            for (int p = 0; p < kParts; ++p)
+            for (int i = 0; i < kQPairs; ++i)
 #pragma unroll
-                for (int j = 0; j < kWords / 2; ++j)
-#pragma unroll
-                    for (int b = 0; b < NB; ++b)
-                        qr[p][j][b] = q2[((p * kWords / 2 + j) * NB + b) * 32];
+                for (int b = 0; b < NB; ++b) qr[i][b] = q2[(i * NB + b) * 32];
         }
+        auto q_pair = [&](int i, int b) {
+            if constexpr (kQReg)
+                return qr[i][b];
+            else
+                return q2[(i * NB + b) * 32];
+        };
 
         float o[kTiles][NB][4];
 #pragma unroll
@@ -504,49 +510,52 @@ k_attend(const __grid_constant__ Args a) {
                 for (int j = 0; j < kWords / 2; ++j)
                     kv8::load_operand(stage_s + place<DP, kKeys>(16 * f + lane % 16, 2 * j + lane / 16),
                                       w[j]);
+                if constexpr (FORMAT == kv8::kInt8) {
+                    // whole sums below 2^22 over the bits of 1.5 * 2^23 are that f32
+                    // plus the sum
+                    constexpr int kBits = 0x4b400000;
+                    constexpr float kBase = 12582912.0f;
+                    const int base[4] = {kBits, kBits, kBits, kBits};
 #pragma unroll
-                for (int b = 0; b < NB; ++b) {
-                    // d = the products of part p, over c
-                    auto products = [&](auto& d, int p, const auto& c) {
-#pragma unroll
-                        for (int j = 0; j < kWords / 2; ++j) {
-                            uint2 q;
-                            if constexpr (kQReg)
-                                q = qr[p][j][b];
-                            else
-                                q = q2[((p * kWords / 2 + j) * NB + b) * 32];
-                            if (j == 0)
-                                kv8::mma_codes(d, w[j], q.x, q.y, c);
-                            else
-                                kv8::mma_codes(d, w[j], q.x, q.y, d);
-                        }
-                    };
-                    float(&z)[4] = s[f][b];
-                    if constexpr (FORMAT == kv8::kInt8) {
-                        // whole sums below 2^22 over the bits of 1.5 * 2^23 are that
-                        // f32 plus the sum
-                        constexpr int kBits = 0x4b400000;
-                        constexpr float kBase = 12582912.0f;
-                        const int base[4] = {kBits, kBits, kBits, kBits};
+                    for (int b = 0; b < NB; ++b) {
                         int d[3][4];
 #pragma unroll
-                        for (int p = 0; p < 3; ++p) products(d[p], p, base);
+                        for (int p = 0; p < 3; ++p)
+#pragma unroll
+                            for (int j = 0; j < kWords / 2; ++j) {
+                                const uint2 q = q_pair(p * kWords / 2 + j, b);
+                                if (j == 0)
+                                    kv8::mma_codes(d[p], w[j], q.x, q.y, base);
+                                else
+                                    kv8::mma_codes(d[p], w[j], q.x, q.y, d[p]);
+                            }
+                        float(&z)[4] = s[f][b];
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
                             z[e] = fmaf(__int_as_float(d[0][e]), 16384.0f, -kBase * 16384.0f);
                             z[e] = fmaf(__int_as_float(d[1][e]) - kBase, 128.0f, z[e]);
                             z[e] += __int_as_float(d[2][e]) - kBase;
                         }
-                    } else {
-                        const float base[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                        products(z, kParts - 1, base);
+                    }
+                } else {
+                    // a word's elements 0, 1 are the operand's 2t, 2t + 1 and its 2, 3
+                    // 2t + 8, 2t + 9, as q's pairs have them
 #pragma unroll
-                        for (int p = kParts - 2; p >= 0; --p) {
-                            float d[4];
-                            products(d, p, base);
+                    for (int b = 0; b < NB; ++b)
 #pragma unroll
-                            for (int e = 0; e < 4; ++e) z[e] = fmaf(z[e], 1.0f / Q::kRadix, d[e]);
-                        }
+                        for (int e = 0; e < 4; ++e) s[f][b][e] = 0.0f;
+#pragma unroll
+                    for (int j = 0; j < kWords; ++j) {
+                        const uint32_t k0 = w[j / 2][j % 2 * 2], k1 = w[j / 2][j % 2 * 2 + 1];
+                        const uint32_t a0 = kv8::e4m3_pair(k0, false), a1 = kv8::e4m3_pair(k1, false);
+                        const uint32_t a2 = kv8::e4m3_pair(k0, true), a3 = kv8::e4m3_pair(k1, true);
+#pragma unroll
+                        for (int b = 0; b < NB; ++b)
+#pragma unroll
+                            for (int p = 0; p < Q::kParts; ++p) {
+                                const uint2 q = q_pair(p * kWords + j, b);
+                                kv8::mma_f16(s[f][b], a0, a1, a2, a3, q.x, q.y);
+                            }
                     }
                 }
             }

@@ -1,6 +1,6 @@
 // kv8_mma.cuh -- 8-bit codes as operands of the matrix instructions: as they
-// are (int8 x int8, e4m3 x e4m3), or as f16, which holds every code exactly,
-// subnormal e4m3 codes among them.
+// are (int8 x int8), or as f16, which holds every code exactly, subnormal e4m3
+// codes among them.
 #pragma once
 
 #include <atomic>
@@ -80,16 +80,7 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1,
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-// d = a b + c of codes, 32 elements deep: e4m3 with f32 sums (every bit of them
-// is kept: measured), int8 with exact ones.
-__device__ __forceinline__ void mma_codes(float (&d)[4], const uint32_t (&a)[4], uint32_t b0,
-                                          uint32_t b1, const float (&c)[4]) {
-    asm("mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e4m3.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
-        "{%8,%9}, {%10,%11,%12,%13};"
-        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]),
-          "f"(c[3]));
-}
+// d = a b + c of int8 codes, 32 elements deep, exact.
 __device__ __forceinline__ void mma_codes(int (&d)[4], const uint32_t (&a)[4], uint32_t b0,
                                           uint32_t b1, const int (&c)[4]) {
     asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
@@ -99,17 +90,19 @@ __device__ __forceinline__ void mma_codes(int (&d)[4], const uint32_t (&a)[4], u
           "r"(c[3]));
 }
 
-// A row of q, held as the sum of `parts` code operands, each 1 / kRadix of the
-// one before:
-//   int8: the nearest whole number to q * 127 * 2^14 / top as three digits
-//     (2^-22 of top, the row's largest);
-//   e4m3: q * 2^k (top in [128, 256)) four bits at a time: two parts are a bf16
-//     element exactly, six an f32 one, or the nearest multiple of 2^-13 (2^-29)
-//     where that is larger.
+// A row of q as operands against the codes, kRegs registers for four elements:
+//   int8: the nearest whole number to q * 127 * 2^14 / top as three digits of
+//     radix 128 (2^-22 of top, the row's largest);
+//   e4m3: q * 2^k (top in [2^14, 2^15)) as f16, an f32 row as two (hi + lo): a
+//     bf16 element exactly, an f32 one to 2^-22 of itself, or either to 2^-39 of
+//     top where that is larger.  An e4m3 product of mma.sync costs its operands'
+//     conversions to f16 for each 8 rows and each part of q, and a sum of its
+//     own; f16 products need a key's codes converted once (a step of 32 keys, 16
+//     rows and 64 elements took 644 warp instructions with two e4m3 parts).
 template <typename T, int FORMAT>
 struct QParts {
-    static constexpr int kParts = FORMAT == kInt8 ? 3 : sizeof(T) == 4 ? 6 : 2;
-    static constexpr float kRadix = FORMAT == kInt8 ? 128.0f : 16.0f;
+    static constexpr int kParts = FORMAT == kInt8 ? 3 : sizeof(T) == 4 ? 2 : 1;
+    static constexpr int kRegs = FORMAT == kInt8 ? 3 : 2 * kParts;
     float lift, unit;  // q's factor; what a sum of products is to be multiplied with
 
     __device__ explicit QParts(float top) {
@@ -118,12 +111,12 @@ struct QParts {
             unit = fmaxf(top, 7.8886090522101181e-31f) * (1.0f / 2080768.0f);
         } else {
             const int e = min(max((int)(__float_as_uint(top) >> 23), 20), 254);
-            lift = __uint_as_float((uint32_t)(127 + 7 - e + 127) << 23);
-            unit = __uint_as_float((uint32_t)(e - 7) << 23);
+            lift = __uint_as_float((uint32_t)(127 + 14 - e + 127) << 23);
+            unit = __uint_as_float((uint32_t)(e - 14) << 23);
         }
     }
-    // The parts of four elements, one word each.
-    __device__ void split(const float* x, uint32_t (&w)[kParts]) const {
+    // Four elements: int8 a word of each digit, e4m3 two pairs of each part.
+    __device__ void split(const float* x, uint32_t (&w)[kRegs]) const {
         if constexpr (FORMAT == kInt8) {
 #pragma unroll
             for (int p = 0; p < 3; ++p) w[p] = 0;
@@ -136,24 +129,13 @@ struct QParts {
                 w[2] |= (uint32_t)((r - (b << 7)) & 0xff) << 8 * i;
             }
         } else {
-            float r[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) r[i] = x[i] * lift;
-#pragma unroll
-            for (int p = 0; p < kParts; ++p) {
-                const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(r[0], r[1]),
-                                                             __NV_SATFINITE, __NV_E4M3);
-                const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(r[2], r[3]),
-                                                             __NV_SATFINITE, __NV_E4M3);
-                w[p] = lo | hi << 16;
-                if (p + 1 < kParts) {
-                    const uint32_t a = e4m3_pair(w[p], false), b = e4m3_pair(w[p], true);
-                    const float2 u = __half22float2(*reinterpret_cast<const __half2*>(&a));
-                    const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&b));
-                    r[0] = (r[0] - u.x) * kRadix;
-                    r[1] = (r[1] - u.y) * kRadix;
-                    r[2] = (r[2] - v.x) * kRadix;
-                    r[3] = (r[3] - v.y) * kRadix;
+            for (int i = 0; i < 2; ++i) {
+                const float a = x[2 * i] * lift, b = x[2 * i + 1] * lift;
+                w[i] = pack_f16x2(a, b);
+                if constexpr (kParts == 2) {
+                    const float2 u = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+                    w[2 + i] = pack_f16x2(a - u.x, b - u.y);
                 }
             }
         }
