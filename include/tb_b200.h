@@ -402,7 +402,7 @@ typedef struct {
     int page;   /* tokens per page: 16, 32, 64 or 128 */
     int n_kv_heads;
     int head_dim; /* a multiple of 16, at most 256 */
-    int64_t n_pages;
+    int64_t n_pages; /* at least one */
     void* k;
     void* v;
     float* k_scale;
@@ -413,14 +413,15 @@ typedef struct {
  * row_start[i] .. row_start[i + 1] - 1 of the call's q, k or v, none or more;
  * they are its last tokens: after them it has lengths[i] tokens, and its row
  * t stands at position lengths[i] - (its rows) + t.  A row at a negative
- * position is padding.  Rows from row_start[n_seqs] on belong to nobody.
+ * position is padding.  Rows before row_start[0] and from row_start[n_seqs] on
+ * belong to nobody.
  * Token j of sequence i is in page page_table[i * table_stride + j / page].
  * row_start, lengths and page_table are device int32, so a captured graph
  * replays with new ones. */
 typedef struct {
     int n_seqs;
     int64_t rows; /* rows in the call's buffers, >= row_start[n_seqs] */
-    const int32_t* row_start; /* [n_seqs + 1], not decreasing, from 0 */
+    const int32_t* row_start; /* [n_seqs + 1], not decreasing, >= 0 */
     const int32_t* lengths;   /* [n_seqs] */
     const int32_t* page_table;
     int table_width;          /* pages per sequence at most */
@@ -469,7 +470,7 @@ typedef struct {
     float scale; /* usually 1 / sqrt(head_dim) */
     int window; /* >= 0 */
     int max_rows; /* most rows of one sequence */
-    int max_len; /* most tokens of one sequence */
+    int max_len; /* most tokens of one sequence, at most 2^30 */
     void* workspace; /* 16-byte aligned device memory, at least */
     size_t workspace_bytes; /* tb_b200_kv8_attention_workspace's bytes */
 } TbB200Kv8Attention;

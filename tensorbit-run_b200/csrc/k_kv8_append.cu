@@ -90,10 +90,11 @@ __device__ __forceinline__ uint32_t top_of(const Piece<T, V>& x) {
         const uint32_t m = 0x7fff7fffu;
         top = __vmaxu2(__vmaxu2(x.w.x & m, x.w.y & m), __vmaxu2(x.w.z & m, x.w.w & m));
         return max(top & 0xffff0000u, top << 16);
-    }
+    } else {
 #pragma unroll
-    for (int i = 0; i < V; ++i) top = max(top, __float_as_uint(x.at(i)) & 0x7fffffffu);
-    return top;
+        for (int i = 0; i < V; ++i) top = max(top, __float_as_uint(x.at(i)) & 0x7fffffffu);
+        return top;
+    }
 }
 
 // The codes of x * per; FINITE: of finite values, whose products are within the
@@ -172,7 +173,8 @@ __global__ void __launch_bounds__(kThreads, 3) k_append(const __grid_constant__ 
     const int first = max(s.first, 0);  // rows before position 0 are padding
     const int logical = (first >> b.page_shift) + slot - ((s.lo >> b.page_shift) + 2 * seq);
     const int64_t begin = (int64_t)logical << b.page_shift;
-    if (s.n == 0 || logical < 0 || begin >= s.len) return;
+    // (a slot before the first sequence's, where row_start[0] > 0, has no page)
+    if (s.n == 0 || logical < first >> b.page_shift || begin >= s.len) return;
     if (logical >= b.width) {
         if (tid == 0) atomicOr(a.status, TB_B200_FLAG_POSITION_RANGE);
         return;

@@ -22,8 +22,9 @@
 // [2^14, 2^15) and held as f16, exact for bf16 elements above 2^-21 of the row's
 // largest; weights are f16 times 2^11 under a reference r' that moves by whole
 // powers of two; the values' scale joins the exponent, 2^(S f + log2 v_scale - r'
-// + 11), and the sum of p takes each page's weights back to the row's r.  That
-// holds for pages whose scales are within 2^100 of one another.
+// + 11), and the sum of p takes each page's weights back to the row's r.  A page
+// whose scale makes its weights less than 2^-100 of the row's largest adds to the
+// sum alone: its f16 weights are zeros.
 #include <math.h>
 
 #include "kv8_mma.cuh"
@@ -42,6 +43,7 @@ constexpr int kThreads = 32 * (kIssuer + 4);  // a whole warpgroup, for its regi
 // Registers a thread of each: 256 * 192 + 128 * 72 + 128 * 56 = 512 * 128.
 constexpr int kSoftRegs = 192, kConvRegs = 72, kIssuerRegs = 56;
 constexpr float kSlack = 4.0f, kLift = 11.0f, kLog2e = 1.4426950408889634f, kNoRef = -3.0e38f;
+constexpr float kLeast = -100.0f;  // weights before the sum are at 2^kLeast of the row's or above
 constexpr uint32_t kColumns = 512;  // of tensor memory: S and P at 0, 128, O at 256, 384
 
 struct Args {
@@ -149,11 +151,22 @@ __global__ void __launch_bounds__(kThreads, 1) k_chunk(const __grid_constant__ A
     const int tiles = rows > kRows ? 2 : 1;
     const bool ok = s.len <= a.max_len && s.n <= a.max_rows &&
                     s.len <= ((int64_t)a.b.width << a.b.page_shift);
-    if (!ok && threadIdx.x == 0) atomicOr(a.status, TB_B200_FLAG_POSITION_RANGE);
+    if (!ok) {  // no keys for any row, those behind the grid's last block among them
+        if (threadIdx.x == 0) atomicOr(a.status, TB_B200_FLAG_POSITION_RANGE);
+        for (int lo = at; lo < rows_all; lo += (int)gridDim.y * kTiles * kRows)
+            for (int i = lo + warp; i < min(lo + kTiles * kRows, rows_all); i += kThreads / 32) {
+                const int64_t t = s.lo + i / group;
+                const int h = head * group + i % group;
+                T* out = static_cast<T*>(a.out) + t * a.out_stride + (int64_t)h * a.d;
+                for (int e = lane; e < a.d; e += 32) tbk::Elt<T>::store(out + e, 0.0f);
+                if (a.lse && lane == 0) a.lse[t * a.hq + h] = -INFINITY;
+            }
+        return;
+    }
     // keys [from, end) that some row sees
     const int p0 = s.first + at / group, p1 = s.first + (at + rows - 1) / group;
-    const int end = ok ? max(p1 + 1, 0) : 0;
-    const int from = a.window ? min(max(p0 - a.window + 1, 0), end) & ~(kKeys - 1) : 0;
+    const int end = max(p1 + 1, 0);
+    const int from = min(kv8::first_seen(p0, a.window), end) & ~(kKeys - 1);
     const int steps = (end - from + kKeys - 1) / kKeys;
 
     if (threadIdx.x == 0) {
@@ -366,7 +379,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_chunk(const __grid_constant__ A
         const uint32_t s_at = tmem + tile * 128 + ((uint32_t)(warp % 4) << 21);
         const uint32_t o_at = s_at + 256;
         const int see_hi = live ? s.first + tok : INT32_MAX;
-        const int see_lo = live && a.window ? max(see_hi - a.window + 1, 0) : 0;
+        const int see_lo = live ? kv8::first_seen(see_hi, a.window) : 0;
         float ref = kNoRef, vref = kNoRef, sum = 0.0f;
         bool fine = true;
         for (int j = 0; j < steps; ++j) {
@@ -440,7 +453,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_chunk(const __grid_constant__ A
 #pragma unroll
                 for (int g = 0; g < 2; ++g) {
                     const int i = c0 / 16 + g;
-                    const float up = lv[i] - vref + kLift;
+                    const float up = fmaxf(lv[i] - vref + kLift, kLeast - ref);
                     const float fi = inside ? fs[i] : 1.0f;
                     float2 part = make_float2(0.0f, 0.0f);
 #pragma unroll
@@ -451,7 +464,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_chunk(const __grid_constant__ A
                         part = add2(part, y);
                         p[8 * g + e / 2] = kv8::pack_f16x2(y.x, y.y);
                     }
-                    sum = fmaf(part.x + part.y, kv8::exp2_fast(fminf(-up - ref, 126.0f)), sum);
+                    sum = fmaf(part.x + part.y, kv8::exp2_fast(-up - ref), sum);
                 }
                 tc::store16(s_at + c0 / 2, p);
             }

@@ -38,6 +38,11 @@ __device__ __forceinline__ Seq sequence(const Batch& b, int i) {
     return s;
 }
 
+// The first key that a row at position p attends.
+__device__ __forceinline__ int first_seen(int p, int window) {
+    return window && p >= window ? p - window + 1 : 0;
+}
+
 // The cache's pointers and shapes, checked: TB_OK or the error to return.
 inline int check_cache(const TbB200Kv8* c, bool pointers) {
     if (!c) return TB_ERR_INVALID_ARG;
@@ -45,10 +50,10 @@ inline int check_cache(const TbB200Kv8* c, bool pointers) {
     if (c->page != 16 && c->page != 32 && c->page != 64 && c->page != 128)
         return TB_ERR_INVALID_SHAPE;
     if (c->n_kv_heads < 1 || c->n_kv_heads > 65535 || c->head_dim < 16 ||
-        c->head_dim > kMaxDim || c->head_dim % 16 || c->n_pages < 0 ||
+        c->head_dim > kMaxDim || c->head_dim % 16 || c->n_pages < 1 ||
         c->n_pages > INT32_MAX / c->n_kv_heads)
         return TB_ERR_INVALID_SHAPE;
-    if (pointers && c->n_pages &&
+    if (pointers &&
         (!c->k || !c->v || !c->k_scale || !c->v_scale || !tbh::aligned16(c->k) ||
          !tbh::aligned16(c->v)))
         return TB_ERR_INVALID_ARG;

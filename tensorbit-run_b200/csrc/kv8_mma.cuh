@@ -213,7 +213,7 @@ int once_per_device(std::atomic<uint64_t>& done, F set) {
 inline int tile_map(CUtensorMap* map, const TbB200Kv8* c, const void* codes, int width, int keys,
                     bool swizzled = true) {
     const uint64_t dims[3] = {(uint64_t)c->head_dim, (uint64_t)c->page,
-                              (uint64_t)(c->n_pages > 0 ? c->n_pages : 1) * c->n_kv_heads};
+                              (uint64_t)c->n_pages * c->n_kv_heads};
     const uint64_t strides[2] = {(uint64_t)c->head_dim, (uint64_t)c->head_dim * c->page};
     const uint32_t box[3] = {(uint32_t)width, (uint32_t)keys, 1};
     return tbh::encode_tiles_u8(map, codes, dims, strides, box, swizzled ? width : 0);

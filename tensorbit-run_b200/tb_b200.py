@@ -918,9 +918,10 @@ def kv8_attention(cache, q, row_start, lengths, page_table, max_q=None, max_len=
         ls = lse.data_ptr()
     b = _kv8_batch(torch, cache, dev, rows, row_start, lengths, page_table)
     a = Kv8Attention(code, heads, q.data_ptr(), qs, out.data_ptr(), os_, ls,
-                     d ** -0.5 if scale is None else scale, window,
+                     d ** -0.5 if scale is None else scale, min(window, 0x7fffffff),
                      rows if max_q is None else max_q,
-                     b.table_width * cache.c.page if max_len is None else max_len, None, 0)
+                     min(b.table_width * cache.c.page, 1 << 30) if max_len is None else max_len,
+                     None, 0)
     L, need = lib(), C.c_size_t()
     if workspace is None:
         check(L.tb_b200_kv8_attention_workspace(cache.c, b, a, need), "kv8_attention_workspace")

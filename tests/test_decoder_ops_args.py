@@ -75,10 +75,12 @@ def attention(**kw):
 CACHES = [(dict(format=4), DTYPE), (dict(page=48), SHAPE), (dict(page=256), SHAPE),
           (dict(page=0), SHAPE), (dict(n_kv_heads=0), SHAPE), (dict(head_dim=8), SHAPE),
           (dict(head_dim=72), SHAPE), (dict(head_dim=272), SHAPE), (dict(n_pages=-1), SHAPE),
-          (dict(k=None), ARG), (dict(v_scale=None), ARG), (dict(v=FAKE + 8), ARG)]
+          (dict(n_pages=0), SHAPE), (dict(n_pages=2 ** 31), SHAPE), (dict(k=None), ARG),
+          (dict(v_scale=None), ARG), (dict(v=FAKE + 8), ARG)]
 BATCHES = [(dict(n_seqs=-1), SHAPE), (dict(rows=-1), SHAPE), (dict(table_stride=1), SHAPE),
            (dict(table_width=-1), SHAPE), (dict(row_start=None), ARG), (dict(lengths=None), ARG),
-           (dict(page_table=None), ARG), (dict(rows=0), OK), (dict(n_seqs=0), OK)]
+           (dict(page_table=None), ARG), (dict(n_seqs=65536), SHAPE), (dict(rows=2 ** 31), SHAPE),
+           (dict(rows=0), OK), (dict(n_seqs=0), OK)]
 
 
 @pytest.mark.parametrize("c,want", CACHES)
@@ -110,6 +112,7 @@ def test_append_refusals():
 @pytest.mark.parametrize("change,want", [
     (dict(dtype=T.F16), DTYPE), (dict(n_heads=0), SHAPE), (dict(n_heads=3), SHAPE),
     (dict(window=-1), SHAPE), (dict(max_rows=-1), SHAPE), (dict(max_len=-1), SHAPE),
+    (dict(max_len=2 ** 30 + 1), SHAPE),
     (dict(q_stride=255), SHAPE), (dict(out_stride=255), SHAPE), (dict(q=None), ARG),
     (dict(out=None), ARG), (dict(out=FAKE), ARG)])
 def test_attention_refusals(change, want):

@@ -659,3 +659,216 @@ def test_python_refusals(dev):
         T.kv8_attention(m.cache, q.half(), st, ln, tb)
     with pytest.raises(TypeError):
         T.Kv8Cache(m.cache.k.view(torch.uint8), m.cache.v, m.cache.k_scale, m.cache.v_scale)
+
+
+# ------------------------------------------------ calls at the edges of the rules
+def test_rows_before_the_first_sequence(dev):
+    """row_start[0] > 0: rows of nobody in front, and pages of the sequence that
+    the call does not touch, given back, with no scale or of no number."""
+    m = Model(dev, "int8", 16, 2, 64, 8)
+    for t, s in zip((m.cache.k_scale, m.cache.v_scale), m.scales):
+        t.fill_(0.0)
+        s[:] = 0.0
+    k, v = (rows_of(m.rng, 70, 2, 64, True, dev) for _ in range(2))
+    x = [f64(k), f64(v)]
+    for table in ([[1, 2, 3, 4, 5, 6, 7]], [[-1, -1, 9, -1, -1, 6, 7]]):
+        st, lengths = [40, 70], [110]  # positions 80 .. 109, in its last two pages
+        T.kv8_append(m.cache, k, v, i32(st, dev), i32(lengths, dev), i32(table, dev))
+        m.append(x, st, lengths, table)
+        m.same()
+        assert T.check_status() == (0, 0)
+    q = rows_of(m.rng, 70, 4, 64, True, dev)
+    out, lse = T.kv8_attention(m.cache, q, i32([40, 70], dev), i32([110], dev), i32(table, dev),
+                               window=3, out=q.new_full(q.shape, 7.0), return_lse=True)
+    y, z, A, lim, _ = m.attention(f64(q), [40, 70], [110], table, window=3, bad=(-1, 9))
+    assert (np.abs(f64(out) - y) <= limit(y, A, lim, True))[42:].all()
+    assert bool((out[:40] == 7.0).all())
+    assert T.check_status()[1] in (0, T.FLAG_PAGE_RANGE)  # of rows 40 and 41
+
+
+@pytest.mark.parametrize("n", [129, 1500])
+def test_many_sequences(dev, n):
+    """More sequences than threads of a CTA and than 32 times 32."""
+    m = Model(dev, "e4m3", 16, 1, 32, 3 * n)
+    lengths = m.rng.integers(0, 41, n)
+    table = tables(m.rng, lengths + 3, 16, 3 * n)
+    fill(m, lengths, table)
+    m.same()
+    counts = m.rng.integers(0, 4, n)
+    lengths = lengths + counts
+    st = starts_of(counts)
+    k, v = (rows_of(m.rng, int(st[-1]), 1, 32, True, dev) for _ in range(2))
+    T.kv8_append(m.cache, k, v, i32(st, dev), i32(lengths, dev), i32(table, dev))
+    m.append([f64(k), f64(v)], st, lengths, table)
+    m.same()
+    attend(m, counts, lengths, table, 2, True, extra=1)
+    attend(m, counts, lengths, table, 2, False, max_q=3, max_len=48)
+    assert T.check_status() == (0, 0)
+
+
+@pytest.mark.parametrize("heads,hkv,counts,lengths", [(4, 2, [9, 3], [5, 60]),
+                                                     (32, 8, [700, 20], [300, 60])])
+def test_windows_beyond_every_length(dev, heads, hkv, counts, lengths):
+    """The widest windows are none, for rows before position 0 beside others too."""
+    import torch
+    m = Model(dev, "int8", 16, hkv, 64, 30)
+    table = tables(m.rng, lengths, 16, 30)
+    fill(m, lengths, table)
+    q = rows_of(m.rng, sum(counts), heads, 64, True, dev, spread=False)
+    want = attend(m, counts, lengths, table, heads, True, q=q, by_head=True)
+    for window in (2 ** 31 - 1, 2 ** 31 - 4, 2 ** 40 + 7, max(lengths)):
+        got = attend(m, counts, lengths, table, heads, True, q=q, window=window, by_head=True)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    assert T.check_status() == (0, 0)
+
+
+def test_chunk_rows_past_the_bound(dev):
+    """A sequence with more rows than max_q: all its rows are as without keys."""
+    import torch
+    counts, lengths, heads = [700, 100], [720, 100], 32
+    m = Model(dev, "e4m3", 64, 8, 128, 16)
+    table = tables(m.rng, lengths, 64, 16)
+    fill(m, lengths, table)
+    q = rows_of(m.rng, 800, heads, 128, True, dev, spread=False)
+    args = (i32(starts_of(counts), dev), i32(lengths, dev), i32(table, dev))
+    want = T.kv8_attention(m.cache, q, *args)
+    out, lse = torch.full_like(want, 7.0), torch.full((800, heads), 7.0, device=dev)
+    T.kv8_attention(m.cache, q, *args, max_q=250, out=out, lse=lse)
+    assert bool((out[:700] == 0).all()) and bool(torch.isneginf(lse[:700]).all())
+    assert torch.equal(out[700:], want[700:]) and bool(torch.isfinite(lse[700:]).all())
+    assert T.check_status() == (8, T.FLAG_POSITION_RANGE)
+
+
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+@pytest.mark.parametrize("heads,hkv,counts", [(4, 2, [40, 1]), (32, 8, [600, 30])])
+def test_values_of_zero_beside_huge_ones(dev, fmt, heads, hkv, counts):
+    """Pages of zero values, at the smallest scale, keep their place in the sum."""
+    import torch
+    lengths = [620, 90]
+    m = Model(dev, fmt, 32, hkv, 64, 24)
+    table = tables(m.rng, lengths, 32, 24)
+    st = starts_of(lengths)
+    k, v = (rows_of(m.rng, 710, hkv, 64, False, dev, spread=False) for _ in range(2))
+    v = v * 2.0 ** 100
+    zero = torch.arange(710, device=dev) // 32 % 3 != 1
+    v[zero] = 0.0
+    T.kv8_append(m.cache, k, v, i32(st, dev), i32(lengths, dev), i32(table, dev))
+    m.append([f64(k), f64(v)], st, lengths, table)
+    m.same()
+    attend(m, counts, lengths, table, heads, True, by_head=True)
+    attend(m, counts, lengths, table, heads, False, by_head=True)
+    assert T.check_status() == (0, 0)
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+def test_wide_heads_over_long_sequences(dev, fmt, bf16):
+    """Heads of 256 and of 208, split over the device and joined."""
+    for d, page in ((256, 128), (208, 16)):
+        lengths = [4001, 700]
+        m = Model(dev, fmt, page, 1, d, 320)
+        table = tables(m.rng, lengths, page, 320)
+        fill(m, lengths, table, spread=False)
+        attend(m, [1, 1], lengths, table, 3, bf16)
+        attend(m, [9, 2], lengths, table, 3, bf16, window=2500)
+    assert T.check_status() == (0, 0)
+
+
+@pytest.mark.parametrize("heads,hkv,d,counts,lengths", [
+    (8, 2, 128, [1, 1, 3], [5000, 30, 700]), (32, 8, 64, [600, 30, 1], [620, 50, 90])])
+def test_unaligned_rows_and_strided_tables(dev, heads, hkv, d, counts, lengths):
+    """q and out rows of any start and stride, a page table that is part of a wider
+    one: the bits of the aligned call, and nothing beside them written."""
+    import torch
+    m = Model(dev, "e4m3", 64, hkv, d, 100)
+    table = tables(m.rng, lengths, 64, 100)
+    fill(m, lengths, table)
+    n = sum(counts)
+    q = rows_of(m.rng, n, heads, d, True, dev, spread=False)
+    st, ln = i32(starts_of(counts), dev), i32(lengths, dev)
+    want, lse = T.kv8_attention(m.cache, q, st, ln, i32(table, dev), return_lse=True)
+    wide = torch.full((3, table.shape[1] + 5), -9, dtype=torch.int32, device=dev)
+    wide[:, 2:2 + table.shape[1]] = i32(table, dev)
+    part = wide[:, 2:2 + table.shape[1]]
+    for pad, at in ((1, 1), (8, 3), (8, 8), (3, 0)):
+        w = heads * d
+        qs = torch.zeros(n * (w + pad) + at, dtype=q.dtype, device=dev)
+        os_ = torch.full_like(qs, 7.0)
+        view = [torch.as_strided(t, (n, heads, d), (w + pad, d, 1), at) for t in (qs, os_)]
+        view[0].copy_(q)
+        got, ls = T.kv8_attention(m.cache, view[0], st, ln, part, out=view[1], return_lse=True)
+        assert torch.equal(got, want) and torch.equal(ls, lse)
+        view[1].fill_(7.0)
+        assert bool((os_ == 7.0).all())
+    assert T.check_status() == (0, 0)
+
+
+def test_empty_batches_and_tables(dev):
+    import torch
+    m = Model(dev, "int8", 16, 2, 64, 4)
+    none = i32(np.zeros((2, 0)), dev)
+    q, k = (rows_of(m.rng, 3, h, 64, True, dev) for h in (4, 2))
+    # rows that are padding, or of nobody, need no page
+    T.kv8_append(m.cache, k, k, i32([0, 2, 2], dev), i32([0, 0], dev), none)
+    out, lse = T.kv8_attention(m.cache, q, i32([0, 2, 2], dev), i32([0, 0], dev), none,
+                               out=torch.full_like(q, 7.0), return_lse=True)
+    assert bool((out[:2] == 0).all()) and bool((out[2] == 7.0).all())
+    assert bool(torch.isneginf(lse[:2]).all()) and T.check_status() == (0, 0)
+    # a token and no table
+    T.kv8_append(m.cache, k, k, i32([0, 2, 3], dev), i32([2, 1], dev), none)
+    assert T.check_status() == (8, T.FLAG_POSITION_RANGE)
+    m.same()
+    # no rows, no sequences
+    T.kv8_append(m.cache, k[:0], k[:0], i32([0], dev), i32([], dev), none[:0])
+    assert T.kv8_attention(m.cache, q[:0], i32([0], dev), i32([], dev), none[:0]).shape[0] == 0
+    assert T.check_status() == (0, 0)
+    with pytest.raises(T.TbError):  # a cache of no pages
+        T.kv8_append(T.Kv8Cache.empty(0, 2, 16, 64, torch.int8), k, k, i32([0, 2, 3], dev),
+                     i32([2, 1], dev), i32([[0], [0]], dev))
+
+
+def test_workspace_refusals(dev):
+    import torch
+    m = Model(dev, "int8", 64, 2, 64, 100)
+    table = tables(m.rng, [6000], 64, 100)
+    fill(m, [6000], table)
+    q = rows_of(m.rng, 1, 8, 64, True, dev)
+    args = (i32([0, 1], dev), i32([6000], dev), i32(table, dev))
+    want = T.kv8_attention(m.cache, q, *args)
+    ws = torch.empty(64 << 20, dtype=torch.uint8, device=dev)
+    assert torch.equal(T.kv8_attention(m.cache, q, *args, workspace=ws), want)
+    for bad in (ws[:256], ws[8:]):
+        with pytest.raises(T.TbError):
+            T.kv8_attention(m.cache, q, *args, workspace=bad)
+    with pytest.raises(ValueError):
+        T.kv8_attention(m.cache, q, *args, workspace=ws[::2])
+
+
+@pytest.mark.parametrize("heads,hkv,counts,lengths", [
+    (16, 2, [1, 1], [5000, 3000]), (32, 8, [600, 30], [900, 1000])])
+def test_graphs_at_once(dev, heads, hkv, counts, lengths):
+    """Two captured calls, replayed over and over on two streams beside each other
+    and an eager one: each has scratch of its own."""
+    import torch
+    m = Model(dev, "int8", 64, hkv, 128, 130)
+    table = tables(m.rng, lengths, 64, 130)
+    fill(m, lengths, table)
+    args = (i32(starts_of(counts), dev), i32(lengths, dev), i32(table, dev))
+    q = [rows_of(m.rng, sum(counts), heads, 128, True, dev) for _ in range(3)]
+    want = [T.kv8_attention(m.cache, x, *args, return_lse=True) for x in q]
+    graphs, got, streams = [], [], [torch.cuda.Stream() for _ in range(2)]
+    for x in q[:2]:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            got.append(T.kv8_attention(m.cache, x, *args, return_lse=True))
+        graphs.append(g)
+    torch.cuda.synchronize()
+    for _ in range(10):
+        for s, g in zip(streams, graphs):
+            with torch.cuda.stream(s):
+                g.replay()
+        eager = T.kv8_attention(m.cache, q[2], *args, return_lse=True)
+    torch.cuda.synchronize()
+    for w, g in zip(want, got + [eager]):
+        assert torch.equal(w[0], g[0]) and torch.equal(w[1], g[1])
+    assert T.check_status() == (0, 0)
