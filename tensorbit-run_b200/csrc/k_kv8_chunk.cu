@@ -166,7 +166,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_chunk(const __grid_constant__ A
     // keys [from, end) that some row sees
     const int p0 = s.first + at / group, p1 = s.first + (at + rows - 1) / group;
     const int end = max(p1 + 1, 0);
-    const int from = min(kv8::first_seen(p0, a.window), end) & ~(kKeys - 1);
+    const int from = a.window ? min(kv8::first_seen(p0, a.window), end) & ~(kKeys - 1) : 0;
     const int steps = (end - from + kKeys - 1) / kKeys;
 
     if (threadIdx.x == 0) {
@@ -379,7 +379,9 @@ __global__ void __launch_bounds__(kThreads, 1) k_chunk(const __grid_constant__ A
         const uint32_t s_at = tmem + tile * 128 + ((uint32_t)(warp % 4) << 21);
         const uint32_t o_at = s_at + 256;
         const int see_hi = live ? s.first + tok : INT32_MAX;
-        const int see_lo = live ? kv8::first_seen(see_hi, a.window) : 0;
+        // a row before position 0 sees no key, so that a see_lo that wraps does no harm
+        const int see_lo =
+            live && a.window ? max((int)((unsigned)see_hi - (unsigned)a.window + 1u), 0) : 0;
         float ref = kNoRef, vref = kNoRef, sum = 0.0f;
         bool fine = true;
         for (int j = 0; j < steps; ++j) {
@@ -447,13 +449,14 @@ __global__ void __launch_bounds__(kThreads, 1) k_chunk(const __grid_constant__ A
                 vref = mv;
             }
             // weights times the values' scale; a group's sum back without it
+            const float least = kLeast - ref, shift = kLift - vref;
 #pragma unroll
             for (int c0 = 0; c0 < kKeys; c0 += 32) {
                 uint32_t p[16];
 #pragma unroll
                 for (int g = 0; g < 2; ++g) {
                     const int i = c0 / 16 + g;
-                    const float up = fmaxf(lv[i] - vref + kLift, kLeast - ref);
+                    const float up = fmaxf(lv[i] + shift, least);
                     const float fi = inside ? fs[i] : 1.0f;
                     float2 part = make_float2(0.0f, 0.0f);
 #pragma unroll
