@@ -49,12 +49,13 @@ constexpr float kLift = 11.0f;     // weights are held times 2^11: up to 2^15 in
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kNoRef = -3.0e38f;  // the reference of a row that has seen no key
 
-// A cut through a block: what the joining kernel needs.
-struct Cut {
-    int64_t begin, end;  // the block's span, counted over the batch
-    int64_t each;        // a share's length, but for the first `rest` CTAs', one longer
-    int rest;
-    int seq, head, block;  // seq < 0: the share begins with a block
+// The first cut through a block: what the joining kernel needs.
+struct alignas(16) Cut {
+    int parts;  // 0: the share begins with a block, or the block was cut before
+    int lone;   // where the first part is; the others are the following CTAs' first
+    int rows, at, lo, head;  // the block's live rows, its first one in the sequence's
+                             // (token, head of the group) rows, those' first token
+    int unused[2];
 };
 
 // Where CTA c's share begins.
@@ -231,7 +232,7 @@ k_attend(const __grid_constant__ Args a) {
         const int64_t want = a.whole ? quotient(tiles, kHeadTiles + 1)
                                      : (tiles + kLeastTiles - 1) / kLeastTiles;
         const int ctas = (int)min((int64_t)gridDim.x, want);
-        if (tid == 0 && a.cuts) a.cuts[blockIdx.x].seq = -1;
+        if (tid == 0 && a.cuts) a.cuts[blockIdx.x].parts = 0;
         if ((int)blockIdx.x >= ctas) return;
         each = quotient(tiles, ctas);
         rest = (int)(tiles - each * ctas);
@@ -273,9 +274,16 @@ k_attend(const __grid_constant__ Args a) {
         const bool whole = skip == 0 && till == load.tiles;
         const Block blk = block_of(a, load, block);
         if (threadIdx.x == 0) {
-            if (first_block && skip > 0)
-                a.cuts[blockIdx.x] = {unit_begin, unit_begin + load.span(), each, rest, seq, head,
-                                      block};
+            const int64_t before = share(each, rest, blockIdx.x - 1);
+            if (first_block && skip > 0 && before <= unit_begin + kHeadTiles) {
+                // the last CTA whose share begins before the block's end
+                const int64_t end = unit_begin + load.span() - 1, longer = rest * (each + 1);
+                const int last = (int)(end < longer ? quotient(end, each + 1)
+                                                    : rest + quotient(end - longer, each));
+                a.cuts[blockIdx.x] = {last - (int)blockIdx.x + 2,
+                                      2 * ((int)blockIdx.x - 1) + (before < unit_begin),
+                                      blk.rows, block * kRows, load.s.lo, head, {}};
+            }
             if (!load.ok) atomicOr(a.status, TB_B200_FLAG_POSITION_RANGE);
         }
         const int begin = blk.from + skip * kTileKeys;
@@ -787,105 +795,103 @@ k_attend(const __grid_constant__ Args a) {
 
 // Joins the blocks that a cut went through: out = sum_c w_c out_c / sum_c w_c,
 // w_c a part's sum at the largest reference.  The first cut through a block has
-// the CTAs, each two of the block's rows; a row's four warps take every fourth
-// part, eight loads in flight, a lane four elements of 128.
-constexpr int kJoinWarps = 4;  // per row
-constexpr int kJoinRows = 2;
-template <typename T>
-__global__ void __launch_bounds__(32 * kJoinWarps * kJoinRows)
-k_join(const __grid_constant__ Args a) {
-    __shared__ float2 st_s[kJoinRows][kMostCtas];
-    __shared__ float4 part_s[kJoinRows][kJoinWarps][kv8::kMaxDim / 4];
-    __shared__ float red[kJoinRows][2][kJoinWarps];
-    const int group_id = threadIdx.x / (32 * kJoinWarps);  // of the four warps of a row
-    const int tid = threadIdx.x % (32 * kJoinWarps), warp = tid >> 5, lane = tid & 31;
-    auto meet = [&] {
-        asm volatile("bar.sync %0, %1;" ::"r"(group_id + 1), "n"(32 * kJoinWarps) : "memory");
-    };
+// CTAs for its rows; W warps a row, each with every W-th part, 8 loads in flight
+// before it knows their weights, a lane four elements of 128.  What it takes is
+// the chain cut -> state and part -> output and as few CTAs as do it in one go:
+// a cut's CTA for every two rows and four warps for each took 8 us of 64
+// sequences' 102.
+constexpr int kJoinThreads = 256;
+constexpr int kManyParts = 16;
+template <typename T, int W>
+__global__ void __launch_bounds__(kJoinThreads) k_join(const __grid_constant__ Args a) {
+    constexpr int kRows = kJoinThreads / 32 / W;
+    __shared__ float4 part_s[W > 1 ? kRows : 1][W][kv8::kMaxDim / 4];
+    __shared__ float2 st_s[kRows][W];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int group_id = warp / W, first = warp % W;
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    const int c = blockIdx.x + 1;
-    const Cut cut = a.cuts[c];
-    if (cut.seq < 0) return;
-    const int64_t before = share(cut.each, cut.rest, c - 1);
-    if (before > cut.begin + kHeadTiles) return;  // not the first cut
-    // parts: of CTA c - 1 (its first block's, or its last's), c, .. while their
-    // shares begin before the block's end
-    const int64_t longer = cut.rest * (cut.each + 1);
-    const int last = (int)(cut.end <= longer
-                               ? quotient(cut.end - 1, cut.each + 1)
-                               : cut.rest + quotient(cut.end - 1 - longer, cut.each));
-    const int parts = min(last, (int)gridDim.x) - c + 2;
-    const int64_t lone = 2 * (int64_t)(c - 1) + (before < cut.begin);
-    auto at = [&](int p) { return p == 0 ? lone : 2 * (int64_t)(c - 1 + p); };
-    const Load load = load_of(a, cut.seq);
-    const Block blk = block_of(a, load, cut.block);
-    const int row = blockIdx.y * kJoinRows + group_id;
-    if (row >= blk.rows) return;
+    const Cut cut = a.cuts[blockIdx.x + 1];
+    const int row = blockIdx.y * kRows + group_id;
+    if (row >= cut.rows || cut.parts == 0) return;
     const int group = a.hq / a.hkv, quads = a.d / 4;
-
-    float m = kNoRef;
-    for (int p = tid; p < parts; p += 32 * kJoinWarps) {
-        const float2 s = __ldcg(&a.state[at(p) * a.block_rows + row]);
-        st_s[group_id][p] = s;
-        m = fmaxf(m, s.x);
-    }
-    m = tbk::warp_max(m);
-    if (lane == 0) red[group_id][0][warp] = m;
-    meet();
-#pragma unroll
-    for (int i = 0; i < kJoinWarps; ++i) m = fmaxf(m, red[group_id][0][i]);
-    float total = 0.0f;
-    for (int p = tid; p < parts; p += 32 * kJoinWarps) {
-        const float2 s = st_s[group_id][p];
-        const float w = s.y * kv8::exp2_fast(s.x - m);
-        st_s[group_id][p].x = w;
-        total += w;
-    }
-    total = tbk::warp_sum(total);
-    if (lane == 0) red[group_id][1][warp] = total;
-    meet();
-    total = 0.0f;
-#pragma unroll
-    for (int i = 0; i < kJoinWarps; ++i) total += red[group_id][1][i];
-
-    const float4* src = reinterpret_cast<const float4*>(a.part) + row * quads;
-    for (int i = lane; i < quads; i += 32) {
-        float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        for (int p0 = warp; p0 < parts; p0 += 8 * kJoinWarps) {
-            float4 x[8];
-            float w[8];
-#pragma unroll
-            for (int u = 0; u < 8; ++u) {
-                const int p = p0 + u * kJoinWarps;
-                w[u] = p < parts ? st_s[group_id][p].x : 0.0f;
-                x[u] = p < parts ? __ldcg(src + at(p) * a.block_rows * quads + i)
-                                 : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            }
-#pragma unroll
-            for (int u = 0; u < 8; ++u) {
-                y.x = fmaf(w[u], x[u].x, y.x);
-                y.y = fmaf(w[u], x[u].y, y.y);
-                y.z = fmaf(w[u], x[u].z, y.z);
-                y.w = fmaf(w[u], x[u].w, y.w);
-            }
-        }
-        part_s[group_id][warp][i] = y;
-    }
-    meet();
-    const bool none = total == 0.0f;
-    const int r = cut.block * a.block_rows + row;
-    const int64_t tok = load.s.lo + r / group;
+    const int n = (cut.parts - first + W - 1) / W;  // the warp's parts
+    auto unit = [&](int i) {  // of the warp's part i
+        const int p = first + i * W;
+        return (int64_t)(p == 0 ? cut.lone : 2 * ((int)blockIdx.x + p)) * a.block_rows + row;
+    };
+    const int r = cut.at + row;
+    const int64_t tok = cut.lo + r / group;
     const int h = cut.head * group + r % group;
     T* out = static_cast<T*>(a.out) + tok * a.out_stride + (int64_t)h * a.d;
-    for (int i = tid; i < a.d; i += 32 * kJoinWarps) {
-        float z = 0.0f;
+    const float4* src = reinterpret_cast<const float4*>(a.part);
+    float m = kNoRef, total = 0.0f;
+    for (int q = lane; q < (quads + 31) / 32 * 32; q += 32) {
+        float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        m = kNoRef;
+        total = 0.0f;
+        for (int c = 0; c < n; c += 32) {
+            float4 x[8];
+            auto ask = [&](int i0) {
 #pragma unroll
-        for (int k = 0; k < kJoinWarps; ++k)
-            z += reinterpret_cast<const float*>(part_s[group_id][k])[i];
-        tbk::Elt<T>::store(out + i, none ? 0.0f : z / total);
+                for (int u = 0; u < 8; ++u)
+                    x[u] = i0 + u < min(n, c + 32) && q < quads
+                               ? __ldcg(src + unit(i0 + u) * quads + q)
+                               : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            };
+            ask(c);
+            const float2 s = c + lane < n ? __ldcg(&a.state[unit(c + lane)])
+                                          : make_float2(kNoRef, 0.0f);
+            const float most = fmaxf(m, tbk::warp_max(s.x));
+            const float keep = kv8::exp2_fast(m - most), w = s.y * kv8::exp2_fast(s.x - most);
+            m = most;
+            total = fmaf(total, keep, tbk::warp_sum(w));
+            y = make_float4(y.x * keep, y.y * keep, y.z * keep, y.w * keep);
+            for (int i0 = c; i0 < min(n, c + 32); i0 += 8) {
+                if (i0 > c) ask(i0);
+#pragma unroll
+                for (int u = 0; u < 8; ++u) {
+                    const float wu = __shfl_sync(tbk::kFull, w, (i0 + u - c) & 31);
+                    y.x = fmaf(wu, x[u].x, y.x);
+                    y.y = fmaf(wu, x[u].y, y.y);
+                    y.z = fmaf(wu, x[u].z, y.z);
+                    y.w = fmaf(wu, x[u].w, y.w);
+                }
+            }
+        }
+        if (W > 1) {
+            part_s[group_id][first][q] = y;
+        } else if (q < quads) {
+            const float per[4] = {y.x, y.y, y.z, y.w};
+            float z[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) z[e] = total == 0.0f ? 0.0f : per[e] / total;
+            kv8::store4(out + 4 * q, a.vec_out, z);
+        }
     }
-    if (a.lse && tid == 0)
-        a.lse[tok * a.hq + h] = none ? -INFINITY : m * 0.69314718055994531f + logf(total);
+    if constexpr (W > 1) {
+        if (lane == 0) st_s[group_id][first] = make_float2(m, total);
+        asm volatile("bar.sync %0, %1;" ::"r"(group_id + 1), "n"(32 * W) : "memory");
+        float w[W];
+        total = 0.0f;
+        m = kNoRef;
+#pragma unroll
+        for (int k = 0; k < W; ++k) m = fmaxf(m, st_s[group_id][k].x);
+#pragma unroll
+        for (int k = 0; k < W; ++k) {
+            w[k] = kv8::exp2_fast(st_s[group_id][k].x - m);
+            total = fmaf(w[k], st_s[group_id][k].y, total);
+        }
+        for (int i = threadIdx.x % (32 * W); i < a.d; i += 32 * W) {
+            float z = 0.0f;
+#pragma unroll
+            for (int k = 0; k < W; ++k)
+                z = fmaf(w[k], reinterpret_cast<const float*>(part_s[group_id][k])[i], z);
+            tbk::Elt<T>::store(out + i, total == 0.0f ? 0.0f : z / total);
+        }
+    }
+    if (a.lse && lane == 0 && first == 0)
+        a.lse[tok * a.hq + h] =
+            total == 0.0f ? -INFINITY : m * 0.69314718055994531f + logf(total);
 }
 
 int check(const TbB200Kv8* cache, const TbB200Kv8Batch* batch, const TbB200Kv8Attention* t,
@@ -976,20 +982,27 @@ int launch_rows(Args& a, const TbB200Kv8* cache, dim3 grid, cudaStream_t s) {
                              : launch_dim<T, FORMAT, 2>(a, cache, grid, s);
 }
 
-template <typename T>
-int join(const Args& a, dim3 grid, cudaStream_t s) {
+template <typename T, int W>
+int join_by(const Args& a, int ctas, cudaStream_t s) {
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = grid;
-    cfg.blockDim = dim3(32 * kJoinWarps * kJoinRows);
+    cfg.gridDim = dim3((unsigned)ctas - 1, (unsigned)(a.block_rows * W * 32 / kJoinThreads));
+    cfg.blockDim = dim3(kJoinThreads);
     cfg.stream = s;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    TB_CUDA_TRY(cudaLaunchKernelEx(&cfg, k_join<T>, a));
+    TB_CUDA_TRY(cudaLaunchKernelEx(&cfg, k_join<T, W>, a));
     TB_LAUNCH_CHECK("8-bit cache attention join kernel");
     return TB_OK;
+}
+
+// Four warps a row when few blocks have many parts each.
+template <typename T>
+int join(const Args& a, int ctas, cudaStream_t s) {
+    return ctas > kManyParts * (int64_t)a.hkv * a.b.n_seqs ? join_by<T, 4>(a, ctas, s)
+                                                          : join_by<T, 1>(a, ctas, s);
 }
 
 }  // namespace
@@ -1062,6 +1075,5 @@ extern "C" int tb_b200_kv8_attention(const TbB200Kv8* cache, const TbB200Kv8Batc
              : (int8 ? launch_rows<__nv_bfloat16, kv8::kInt8>(a, cache, grid, st)
                      : launch_rows<__nv_bfloat16, kv8::kE4m3>(a, cache, grid, st));
     if (rc != TB_OK || p.whole) return rc;
-    const dim3 joins((unsigned)p.ctas - 1, (unsigned)(p.block_rows / kJoinRows));
-    return f32 ? join<float>(a, joins, st) : join<__nv_bfloat16>(a, joins, st);
+    return f32 ? join<float>(a, p.ctas, st) : join<__nv_bfloat16>(a, p.ctas, st);
 }
