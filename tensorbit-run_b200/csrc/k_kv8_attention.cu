@@ -3,7 +3,7 @@
 //   s_j = scale q.k_j,  out = sum_j p_j v_j,  p = softmax(s),  k_j = code * page scale
 //
 // A block holds 8 or 16 rows of one sequence and k/v head: (query token, head
-// of the group) pairs, token-major.  The blocks' keys, in tiles of 64 and in
+// of the group) pairs, token-major.  The blocks' keys, in tiles of 128 and in
 // one order, are cut into equal shares, one for each CTA that fits on the
 // device: lengths are on the device and often uneven, and equal shares of them
 // leave no CTA waiting for a long sequence and write few partial results (at
@@ -32,6 +32,14 @@
 // their weight.  References are whole numbers and move only when a score passes
 // them by 2^4: rescaling is exact and rare.  A weight more than 2^-25 below the
 // row's largest is an f16 subnormal, off by at most 2^-36 of the largest.
+//
+// What bounds it and what it measured (8 k/v heads): the codes' bytes where there
+// are many keys a row, 64 sequences of 1 .. 8191 keys, 64 heads of 128, int8, 95 us,
+// 5.7 TB/s (a copy: 6.5), one of 131071, e4m3, 55 us, 4.9 TB/s, of it 14 us above the
+// bytes' time: launch, shares, table -> scale -> codes -> products, join.
+// With 16 rows a block and heads of 64 (48 sequences, 1 .. 8 tokens, 32 heads, a
+// window of 1000) the warps' instructions, about 550 for 32 keys and 1800 a block,
+// issued at half rate by the 12 warps that registers allow: 33 us.
 #include "kv8_mma.cuh"
 
 namespace {
@@ -41,7 +49,7 @@ constexpr int kThreads = 32 * kWarps;
 constexpr int kTileKeys = 128;     // keys that shares are counted in
 constexpr int kLeastTiles = 2;     // tiles below which a share is not cut further
 // What a block costs besides its keys, in tiles (64 sequences of up to 8191 keys
-// at 2: 107 us, 4: 101, 6: 103).
+// at 2: 103 us, 4: 95, 6: 97).
 constexpr int kHeadTiles = 4;
 constexpr int kMostCtas = 1024;
 constexpr float kSlack = 4.0f;     // how far (log2) scores may pass a reference
@@ -798,8 +806,8 @@ k_attend(const __grid_constant__ Args a) {
 // CTAs for its rows; W warps a row, each with every W-th part, 8 loads in flight
 // before it knows their weights, a lane four elements of 128.  What it takes is
 // the chain cut -> state and part -> output and as few CTAs as do it in one go:
-// a cut's CTA for every two rows and four warps for each took 8 us of 64
-// sequences' 102.
+// four warps for every row took 8 us of 64 sequences' 102, and one warp a row 4 of
+// a long sequence's 59, whose blocks have 55 parts.
 constexpr int kJoinThreads = 256;
 constexpr int kManyParts = 16;
 template <typename T, int W>

@@ -18,8 +18,15 @@
 // once for 256 rows, four times fewer than a block of 16 rows' matrix
 // instructions could share, and the products run at 4 times their rate.
 //
+// Measured: 2048 tokens behind 6144, 32 heads of 128 on 8, int8, 342 us, 703 TFLOP/s
+// (0.43 of a library product's rate; blocks of 16 rows: 1634 us).  A step takes 5300
+// clocks: a tile's scores, softmax (2650) and products follow one another, and the
+// products share shared memory's bandwidth with the conversion (3300 clocks where
+// 2050 are the least).  256 CTAs of equal work run on 148 SMs as two waves, 0.86
+// full.
+//
 // Precision as in k_kv8_attention.cu: a row of q is scaled by a power of two to
-// [2^14, 2^15) and held as f16, exact for bf16 elements above 2^-21 of the row's
+// [2^14, 2^15) and held as f16, exact for bf16 elements above 2^-31 of the row's
 // largest; weights are f16 times 2^11 under a reference r' that moves by whole
 // powers of two; the values' scale joins the exponent, 2^(S f + log2 v_scale - r'
 // + 11), and the sum of p takes each page's weights back to the row's r.  A page
@@ -105,6 +112,19 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     return d;
 }
 
+// Eight elements of a row, zeros if not live; vec: aligned to 16 bytes.
+__device__ __forceinline__ uint4 load8(const __nv_bfloat16* p, bool live, bool vec) {
+    uint4 x = make_uint4(0, 0, 0, 0);
+    if (live && vec) {
+        x = *reinterpret_cast<const uint4*>(p);
+    } else if (live) {
+        const uint16_t* u = reinterpret_cast<const uint16_t*>(p);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) (&x.x)[i] = u[2 * i] | (uint32_t)u[2 * i + 1] << 16;
+    }
+    return x;
+}
+
 // A bounded wait of a whole warp.
 __device__ __forceinline__ bool wait_all(uint64_t* bar, uint32_t parity, unsigned* status) {
     const bool came = tbk::mbar_wait(bar, parity, status, 1000000000ull);
@@ -188,7 +208,13 @@ __global__ void __launch_bounds__(kThreads, 1) k_chunk(const __grid_constant__ A
     }
     if (warp == kIssuer) tc::allocate(&sh.tmem, kColumns);
 
-    // Q: a thread its row.  A row with a NaN or an infinity is NaN.
+    tc::fence_before();
+    __syncthreads();
+    tc::fence_after();
+    const uint32_t tmem = sh.tmem;
+
+    // Q: a thread its row, all of it asked for at once, while the first codes come.
+    // A row with a NaN or an infinity is NaN.
     const int tile = warp / 4, row = threadIdx.x & (kRows - 1);
     const int r = tile * kRows + row;
     const bool soft = warp < kSoftWarps, live = soft && r < rows;
@@ -197,34 +223,33 @@ __global__ void __launch_bounds__(kThreads, 1) k_chunk(const __grid_constant__ A
     if (soft && tile < tiles) {
         const T* q = static_cast<const T*>(a.q) + (s.lo + tok) * a.q_stride +
                      (int64_t)(head * group + hh) * a.d;
-        uint32_t top = 0;
-        for (int i = 0; i < a.d && live; i += 4) {
-            float x[4];
-            kv8::load4(q + i, true, a.vec, x);
+        uint4 x[DP / 8];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) top = max(top, __float_as_uint(fabsf(x[e])));
-        }
+        for (int i = 0; i < DP / 8; ++i) x[i] = load8(q + 8 * i, live && 8 * i < a.d, a.vec);
+        uint32_t two = 0;  // the largest magnitudes of the even and of the odd elements
+#pragma unroll
+        for (int i = 0; i < 4 * (DP / 8); ++i)
+            two = __vmaxu2(two, (&x[i / 4].x)[i % 4] & 0x7fff7fffu);
+        const uint32_t top = max(two & 0xffff0000u, two << 16);
         const bool finite = top < 0x7f800000u;
         const int e = min(max((int)(top >> 23), 1 + 16), 254);
         // a negative scale turns q, so that larger sums are larger scores
         const float lift = __uint_as_float((uint32_t)(127 + 14 - e + 127) << 23) *
                            (a.scale < 0.0f ? -1.0f : 1.0f);
         f = finite ? __uint_as_float((uint32_t)(e - 14) << 23) * (fabsf(a.scale) * kLog2e) : NAN;
-        for (int i = 0; i < DP; i += 8) {
-            float x[4], y[4];
-            kv8::load4(q + i, live && finite && i < a.d, a.vec, x);
-            kv8::load4(q + i + 4, live && finite && i < a.d, a.vec, y);
-            const uint4 h = make_uint4(
-                kv8::pack_f16x2(x[0] * lift, x[1] * lift), kv8::pack_f16x2(x[2] * lift, x[3] * lift),
-                kv8::pack_f16x2(y[0] * lift, y[1] * lift), kv8::pack_f16x2(y[2] * lift, y[3] * lift));
-            *reinterpret_cast<uint4*>(q_tiles + tile * H::kTile + place(row, i / 8)) = h;
+#pragma unroll
+        for (int i = 0; i < DP / 8; ++i) {
+            uint4 h;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const uint32_t w = (&x[i].x)[j];
+                const float lo = __uint_as_float(w << 16), hi = __uint_as_float(w & 0xffff0000u);
+                (&h.x)[j] = finite ? kv8::pack_f16x2(lo * lift, hi * lift) : 0u;
+            }
+            *reinterpret_cast<uint4*>(q_tiles + tile * H::kTile + place(row, i)) = h;
         }
         tbk::fence_proxy_async_shared();
     }
-    tc::fence_before();
-    __syncthreads();
-    tc::fence_after();
-    const uint32_t tmem = sh.tmem;
 
     if (warp >= kIssuer) {
         tc::fewer_registers<kIssuerRegs>();
@@ -247,6 +272,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_chunk(const __grid_constant__ A
                 }
                 tc::commit(&sh.s_full[t], leader);
             };
+            asm volatile("bar.sync 1, %0;" ::"n"(32 * (kSoftWarps + 1)) : "memory");  // Q
             bool fine = wait_all(&sh.k_full[0], 0, a.status);
             tc::fence_after();
             for (int t = 0; t < tiles && fine; ++t) scores(t, 0);
@@ -374,6 +400,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_chunk(const __grid_constant__ A
             if (have_v) wait_all(&sh.codes[1][w], phases >> 1 & 1, a.status);
         }
     } else {
+        if (steps > 0) asm volatile("bar.arrive 1, %0;" ::"n"(32 * (kSoftWarps + 1)) : "memory");
         tc::more_registers<kSoftRegs>();
         if (tile < tiles) {
         const uint32_t s_at = tmem + tile * 128 + ((uint32_t)(warp % 4) << 21);
@@ -488,12 +515,17 @@ __global__ void __launch_bounds__(kThreads, 1) k_chunk(const __grid_constant__ A
             if (steps > 0) tc::load<32>(o_at + c0, x);
             if (!live) continue;
 #pragma unroll
-            for (int e = 0; e < 32; e += 4) {
+            for (int e = 0; e < 32; e += 8) {
                 if (c0 + e >= a.d) break;
-                float y[4];
+                float y[8];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) y[i] = none || steps == 0 ? 0.0f : x[e + i] * per;
-                kv8::store4(out + c0 + e, a.vec_out, y);
+                for (int i = 0; i < 8; ++i) y[i] = none || steps == 0 ? 0.0f : x[e + i] * per;
+                if (a.vec_out) {
+                    tbk::store_vec<T, 8>(out + c0 + e, y);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) tbk::Elt<T>::store(out + c0 + e + i, y[i]);
+                }
             }
         }
         if (a.lse && live)

@@ -21,8 +21,14 @@
 // head's sum of squares is a shuffle among G lanes and every element is read
 // and written once, in place if asked.  A lane asks for the vectors of its
 // first U heads before the angles are computed and keeps its pairs' cos and sin
-// and its weights in registers for all of them; the CTA has just the threads
-// that make its passes over the heads full ones.
+// in registers for all of them; the CTA has just the threads that make its passes
+// over the heads full ones.
+//
+// Measured: 16384 rows of 64 + 8 heads of 128, bf16, 101 us, 6.0 TB/s (a copy:
+// 6.5; the first version, a head at a time: 127 us); norm and half the head, 4095
+// rows of 32 + 32 heads of 128, f32, 49.6 us, 5.4 TB/s; 777 rows of 32 + 32 heads
+// of 80, f32, 8.4 us and 256 rows of 32 + 32 heads of 128, bf16, 5.9 us, where a
+// launch and one row's chain of loads are most of the time.
 #include <math.h>
 
 #include "tb_device.cuh"
