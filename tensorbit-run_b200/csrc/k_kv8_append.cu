@@ -356,7 +356,9 @@ extern "C" int tb_b200_kv8_append(const TbB200Kv8* cache, const TbB200Kv8Batch* 
                     cache->head_dim};
     const unsigned slots = (unsigned)(batch->rows / cache->page + 2 * batch->n_seqs);
     // One warp a unit when a sequence brings so few rows that kHold vectors a
-    // lane hold them (bf16: rows * d <= 1024 elements).
+    // lane hold them (bf16: rows * d <= 1024 elements).  A warp and a CTA a unit, 8
+    // heads of 128: 256 sequences' token 4.7 and 15.1 us, 64 of 8 tokens 4.5 and 7.3,
+    // of 16 7.2 and 7.2, of 32 16.7 and 8.4.
     const size_t size = dtype == TB_DTYPE_F32 ? 4 : 2;
     const bool warps = batch->rows * cache->head_dim * (int64_t)size <=
                        (int64_t)batch->n_seqs * 32 * kHold * 16;

@@ -934,6 +934,8 @@ Plan plan_of(const TbB200Kv8* cache, const TbB200Kv8Batch* batch, const TbB200Kv
     Plan p = {};
     const int64_t group = t->n_heads / cache->n_kv_heads;
     const int64_t rows = (t->max_rows < batch->rows ? t->max_rows : batch->rows) * group;
+    // 8 rows a block where they do (64 sequences of 4000 keys, 8 heads a k/v head: 94
+    // us, with blocks of 16 118), 16 where that halves the blocks
     p.block_rows = rows <= 8 ? 8 : 16;
     // at most so many blocks, of at most so many tiles
     int64_t blocks = (rows + p.block_rows - 1) / p.block_rows * batch->n_seqs;

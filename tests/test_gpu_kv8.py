@@ -872,3 +872,19 @@ def test_graphs_at_once(dev, heads, hkv, counts, lengths):
     for w, g in zip(want, got + [eager]):
         assert torch.equal(w[0], g[0]) and torch.equal(w[1], g[1])
     assert T.check_status() == (0, 0)
+
+
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+def test_single_tokens_of_many_heads(dev, fmt):
+    """64 heads on one k/v head: enough rows a sequence and sequences for the kernel
+    of many rows, a token each, empty sequences among them."""
+    m = Model(dev, fmt, 32, 1, 128, 700)
+    lengths = m.rng.integers(0, 200, 130)
+    lengths[[3, 77, 129]] = 0
+    lengths[50] = 513
+    table = tables(m.rng, lengths, 32, 700)
+    fill(m, lengths, table)
+    attend(m, [1] * 130, lengths, table, 64, True, extra=1, by_head=True)
+    counts = m.rng.integers(0, 3, 130)
+    attend(m, counts, lengths, table, 64, True, window=40, by_head=True)
+    assert T.check_status() == (0, 0)
