@@ -18,11 +18,11 @@
 // once for 256 rows, four times fewer than a block of 16 rows' matrix
 // instructions could share, and the products run at 4 times their rate.
 //
-// Measured: 2048 tokens behind 6144, 32 heads of 128 on 8, int8, 342 us, 703 TFLOP/s
-// (0.43 of a library product's rate; blocks of 16 rows: 1634 us).  A step takes 5300
-// clocks: a tile's scores, softmax (2650) and products follow one another, and the
-// products share shared memory's bandwidth with the conversion (3300 clocks where
-// 2050 are the least).  256 CTAs of equal work run on 148 SMs as two waves, 0.86
+// Measured: 2048 tokens behind 6144, 32 heads of 128 on 8, int8, 308 us, 780 TFLOP/s
+// (0.47 of a library product's rate; blocks of 16 rows: 1634 us).  A step takes 2.35
+// us, 4500 clocks: a tile's scores, softmax (2600) and products follow one another,
+// and the products share shared memory's bandwidth with the conversion (3300 clocks
+// where 2050 are the least).  256 CTAs of 62 steps run on 148 SMs as two waves, 0.86
 // full.
 //
 // Precision as in k_kv8_attention.cu: a row of q is scaled by a power of two to
