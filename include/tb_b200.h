@@ -442,8 +442,8 @@ typedef struct {
  * sequence's last token and padding rows change nothing.  A sequence with
  * lengths[i] > table_width * page raises TB_B200_FLAG_POSITION_RANGE and
  * loses the tokens past it; a page number outside [0, n_pages) raises
- * TB_B200_FLAG_PAGE_RANGE and loses that page's.  Two sequences of one call
- * must not append to the same page. */
+ * TB_B200_FLAG_PAGE_RANGE and loses that page's.  One call must not
+ * append to a page from two places of the table. */
 int tb_b200_kv8_append(const TbB200Kv8* cache, const TbB200Kv8Batch* batch, int dtype,
                        const void* k, int64_t k_stride, const void* v, int64_t v_stride,
                        void* stream);

@@ -13,7 +13,7 @@
 // that gets rows, head), its K and V; which pages those are is on the device, so the
 // grid has a slot for each page that could: a sequence's rows from s to e touch at
 // most e / page - s / page + 2 pages, so sequence i's slots start at row_start[i] /
-// page + 2 i, which a warp finds its sequence by, 32 candidates at a time.
+// page + 2 i, which a warp finds its sequence by.
 //
 // A unit has a CTA of 8 warps when its page is filled by a prompt, one warp (and a
 // CTA 8 heads) when a call brings few rows a sequence: then the time is the chain
@@ -156,24 +156,9 @@ __global__ void __launch_bounds__(kThreads, 3) k_append(const __grid_constant__ 
     const int slot = blockIdx.x, page = 1 << b.page_shift;
     const int head = blockIdx.y * (kThreads / kUnit) + threadIdx.x / kUnit;
     if (head >= a.hkv) return;  // whole warps of units of one warp
-    // the last sequence whose slots start at or before this one, in [seq, seq + n)
-    int seq = 0;
     kv8::Seq s;
-    for (int n = b.n_seqs;;) {
-        const int step = (n + 31) / 32, i = min(seq + lane * step, b.n_seqs - 1);
-        const kv8::Seq mine = kv8::sequence(b, i);  // of the last look, the answer's too
-        const bool before =
-            lane * step < n && (mine.lo >> b.page_shift) + 2 * i <= slot;
-        const int last = 31 - __clz(__ballot_sync(tbk::kFull, before) | 1);
-        seq += last * step;
-        n = min(step, n - last * step);
-        if (step > 1) continue;
-        s.lo = __shfl_sync(tbk::kFull, mine.lo, last);
-        s.n = __shfl_sync(tbk::kFull, mine.n, last);
-        s.len = __shfl_sync(tbk::kFull, mine.len, last);
-        s.first = s.len - s.n;
-        break;
-    }
+    const int seq = kv8::find_sequence(
+        b, slot, [&](int lo, int i) { return (lo >> b.page_shift) + 2 * i; }, s);
     const int first = max(s.first, 0);  // rows before position 0 are padding
     const int logical = (first >> b.page_shift) + slot - ((s.lo >> b.page_shift) + 2 * seq);
     const int64_t begin = (int64_t)logical << b.page_shift;

@@ -161,31 +161,24 @@ __global__ void __launch_bounds__(kThreads, 1) k_chunk(const __grid_constant__ A
     uint8_t* kv_tiles = smem + kTiles * H::kTile;  // [stage][K, V]
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int head = blockIdx.x, seq = blockIdx.z;
-    const kv8::Seq s = kv8::sequence(a.b, seq);
-    const int group = a.hq / a.hkv, rows_all = s.n * group;
-    // long blocks first
-    const int block = (int)gridDim.y - 1 - (int)blockIdx.y, at = block * kTiles * kRows;
-    if (at >= rows_all) return;
+    // A slot and head: sequence i's slots start at (its first row) / 256 + i, which is
+    // one for each of its blocks or more; long blocks first.
+    const int head = blockIdx.x % a.hkv, slot = (int)(gridDim.x - 1 - blockIdx.x) / a.hkv;
+    const int group = a.hq / a.hkv;
+    auto start = [&](int lo, int i) { return lo * group / (kTiles * kRows) + i; };
+    kv8::Seq s;
+    const int seq = kv8::find_sequence(a.b, slot, start, s);
+    const int rows_all = s.n * group, block = slot - start(s.lo, seq);
+    const int at = block * kTiles * kRows;
+    if (block < 0 || at >= rows_all) return;
     const int rows = min(kTiles * kRows, rows_all - at);
     const int tiles = rows > kRows ? 2 : 1;
     const bool ok = s.len <= a.max_len && s.n <= a.max_rows &&
                     s.len <= ((int64_t)a.b.width << a.b.page_shift);
-    if (!ok) {  // no keys for any row, those behind the grid's last block among them
-        if (threadIdx.x == 0) atomicOr(a.status, TB_B200_FLAG_POSITION_RANGE);
-        for (int lo = at; lo < rows_all; lo += (int)gridDim.y * kTiles * kRows)
-            for (int i = lo + warp; i < min(lo + kTiles * kRows, rows_all); i += kThreads / 32) {
-                const int64_t t = s.lo + i / group;
-                const int h = head * group + i % group;
-                T* out = static_cast<T*>(a.out) + t * a.out_stride + (int64_t)h * a.d;
-                for (int e = lane; e < a.d; e += 32) tbk::Elt<T>::store(out + e, 0.0f);
-                if (a.lse && lane == 0) a.lse[t * a.hq + h] = -INFINITY;
-            }
-        return;
-    }
+    if (!ok && threadIdx.x == 0) atomicOr(a.status, TB_B200_FLAG_POSITION_RANGE);
     // keys [from, end) that some row sees
     const int p0 = s.first + at / group, p1 = s.first + (at + rows - 1) / group;
-    const int end = max(p1 + 1, 0);
+    const int end = ok ? max(p1 + 1, 0) : 0;
     const int from = a.window ? min(kv8::first_seen(p0, a.window), end) & ~(kKeys - 1) : 0;
     const int steps = (end - from + kKeys - 1) / kKeys;
 
@@ -554,10 +547,13 @@ int launch(Args& a, const TbB200Kv8* cache, dim3 grid, cudaStream_t s) {
     return TB_OK;
 }
 
-int64_t blocks_of(const TbB200Kv8* cache, const TbB200Kv8Batch* batch,
-                  const TbB200Kv8Attention* t) {
-    const int64_t rows = t->max_rows < batch->rows ? t->max_rows : batch->rows;
-    return (rows * (t->n_heads / cache->n_kv_heads) + kTiles * kRows - 1) / (kTiles * kRows);
+// Slots of the grid: a bound on the batch's blocks, whatever max_rows is (64 sequences
+// of 100 rows 253 us; a grid of max_rows for each, 245 with the rows' own bound, 545
+// with the batch's, 6400).
+int64_t slots_of(const TbB200Kv8* cache, const TbB200Kv8Batch* batch,
+                 const TbB200Kv8Attention* t) {
+    const int64_t group = t->n_heads / cache->n_kv_heads;
+    return batch->rows * group / (kTiles * kRows) + batch->n_seqs;
 }
 
 }  // namespace
@@ -575,11 +571,12 @@ bool chunk_suits(const TbB200Kv8* cache, const TbB200Kv8Batch* batch, const TbB2
                  int sm_count) {
     if (t->dtype != TB_DTYPE_BF16 || cache->head_dim > 128) return false;
     const int64_t group = t->n_heads / cache->n_kv_heads, rows = batch->rows * group;
-    const int64_t each = blocks_of(cache, batch, t), n = batch->n_seqs;
-    if (each > 65535) return false;
-    const int64_t most = rows / (kTiles * kRows) + n;
-    const int64_t blocks = (each * n < most ? each * n : most) * cache->n_kv_heads;
-    const int64_t waves = (blocks + sm_count - 1) / sm_count;
+    const int64_t slots = slots_of(cache, batch, t);
+    const int64_t most = t->max_rows < batch->rows ? t->max_rows : batch->rows;
+    const int64_t each = (most * group + kTiles * kRows - 1) / (kTiles * kRows) * batch->n_seqs;
+    const int64_t waves =
+        ((each < slots ? each : slots) * cache->n_kv_heads + sm_count - 1) / sm_count;
+    if (slots * cache->n_kv_heads > INT32_MAX) return false;
     const double small = (double)rows * cache->n_kv_heads / 16;
     return small >= (cache->head_dim <= 64 ? 3.3 : 2.4) * (double)(waves * sm_count);
 }
@@ -607,8 +604,7 @@ int chunk_attention(const TbB200Kv8* cache, const TbB200Kv8Batch* batch,
     a.max_len = t->max_len;
     a.vec = tbh::aligned16(t->q) && t->q_stride % 8 == 0;
     a.vec_out = tbh::aligned16(t->out) && t->out_stride % 8 == 0;
-    const dim3 grid((unsigned)a.hkv, (unsigned)blocks_of(cache, batch, t),
-                    (unsigned)batch->n_seqs);
+    const dim3 grid((unsigned)(slots_of(cache, batch, t) * a.hkv));
     const bool int8 = cache->format == kInt8;
     if (cache->head_dim <= 64)
         return int8 ? launch<kInt8, 64>(a, cache, grid, stream)

@@ -38,6 +38,29 @@ __device__ __forceinline__ Seq sequence(const Batch& b, int i) {
     return s;
 }
 
+// The last sequence whose first slot, start(row_start, i), is at or before `slot`,
+// by a whole warp, 32 candidates at a time; s: its rows.  The first one if there is
+// none.
+template <typename F>
+__device__ __forceinline__ int find_sequence(const Batch& b, int slot, F start, Seq& s) {
+    const int lane = threadIdx.x & 31;
+    int seq = 0;
+    for (int n = b.n_seqs;;) {  // it is in [seq, seq + n)
+        const int step = (n + 31) / 32, i = min(seq + lane * step, b.n_seqs - 1);
+        const Seq mine = sequence(b, i);  // of the last look, the answer's too
+        const bool before = lane * step < n && start(mine.lo, i) <= slot;
+        const int last = 31 - __clz(__ballot_sync(tbk::kFull, before) | 1);
+        seq += last * step;
+        n = min(step, n - last * step);
+        if (step > 1) continue;
+        s.lo = __shfl_sync(tbk::kFull, mine.lo, last);
+        s.n = __shfl_sync(tbk::kFull, mine.n, last);
+        s.len = __shfl_sync(tbk::kFull, mine.len, last);
+        s.first = s.len - s.n;
+        return seq;
+    }
+}
+
 // The first key that a row at position p attends.
 __device__ __forceinline__ int first_seen(int p, int window) {
     return window && p >= window ? p - window + 1 : 0;

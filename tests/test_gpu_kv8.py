@@ -888,3 +888,28 @@ def test_single_tokens_of_many_heads(dev, fmt):
     counts = m.rng.integers(0, 3, 130)
     attend(m, counts, lengths, table, 64, True, window=40, by_head=True)
     assert T.check_status() == (0, 0)
+
+
+def test_chunk_rows_in_front_and_clamped_starts(dev):
+    """Many rows: rows of nobody in front of the first sequence, row_start values
+    outside the rows, and the loosest bounds beside the tightest."""
+    import torch
+    m = Model(dev, "e4m3", 32, 8, 64, 80)
+    lengths = [700, 400, 0, 900]
+    table = tables(m.rng, lengths, 32, 80)
+    fill(m, lengths, table)
+    q = rows_of(m.rng, 1300, 32, 64, True, dev, spread=False)
+    ln, tb = i32(lengths, dev), i32(table, dev)
+    st = np.array([0, 600, 601, 601, 1000])
+    want, lse = T.kv8_attention(m.cache, q[300:], i32(st, dev), ln, tb, max_q=600, max_len=900,
+                                return_lse=True)
+    attend(m, st[1:] - st[:-1], lengths, table, 32, True, q=q[:1000], by_head=True)
+    out, ls = torch.full_like(q, 7.0), torch.full((1300, 32), 7.0, device=dev)
+    T.kv8_attention(m.cache, q, i32(st + 300, dev), ln, tb, out=out, lse=ls)
+    assert torch.equal(out[300:], want) and torch.equal(ls[300:], lse)
+    assert bool((out[:300] == 7.0).all()) and bool((ls[:300] == 7.0).all())
+    one = T.kv8_attention(m.cache, q, i32([0, 1300], dev), ln[3:], tb[3:])
+    out.fill_(7.0)
+    T.kv8_attention(m.cache, q, i32([-9, 2 ** 31 - 1, 40], dev), ln[[3, 0]], tb[[3, 0]], out=out)
+    assert torch.equal(out, one)
+    assert T.check_status() == (0, 0)
