@@ -18,12 +18,13 @@
 // once for 256 rows, four times fewer than a block of 16 rows' matrix
 // instructions could share, and the products run at 4 times their rate.
 //
-// Measured: 2048 tokens behind 6144, 32 heads of 128 on 8, int8, 308 us, 780 TFLOP/s
-// (0.47 of a library product's rate; blocks of 16 rows: 1634 us).  A step takes 2.35
+// Measured: 2048 tokens behind 6144, 32 heads of 128 on 8, int8, 305 us, 789 TFLOP/s
+// (0.48 of a library product's rate; blocks of 16 rows: 1634 us).  A step takes 2.35
 // us, 4500 clocks: a tile's scores, softmax (2600) and products follow one another,
 // and the products share shared memory's bandwidth with the conversion (3300 clocks
 // where 2050 are the least).  256 CTAs of 62 steps run on 148 SMs as two waves, 0.86
-// full.
+// full; a CTA pays some 12 us beside its steps, so 64 sequences of 100 tokens and
+// 1000 keys take 239 us (253 with a thread a row of q and out).
 //
 // Precision as in k_kv8_attention.cu: a row of q is scaled by a power of two to
 // [2^14, 2^15) and held as f16, exact for bf16 elements above 2^-31 of the row's
@@ -125,6 +126,16 @@ __device__ __forceinline__ uint4 load8(const __nv_bfloat16* p, bool live, bool v
     return x;
 }
 
+__device__ __forceinline__ void store8(__nv_bfloat16* p, const uint4& x, bool vec) {
+    if (vec) {
+        *reinterpret_cast<uint4*>(p) = x;
+    } else {
+        uint16_t* u = reinterpret_cast<uint16_t*>(p);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) u[i] = (uint16_t)((&x.x)[i / 2] >> i % 2 * 16);
+    }
+}
+
 // A bounded wait of a whole warp.
 __device__ __forceinline__ bool wait_all(uint64_t* bar, uint32_t parity, unsigned* status) {
     const bool came = tbk::mbar_wait(bar, parity, status, 1000000000ull);
@@ -201,37 +212,63 @@ __global__ void __launch_bounds__(kThreads, 1) k_chunk(const __grid_constant__ A
     }
     if (warp == kIssuer) tc::allocate(&sh.tmem, kColumns);
 
+    // A converting warp has keys 32 w .. 32 w + 31 of each step, two groups of 16 whose
+    // pages lanes 0 and 1 look up, ask for and ring in.
+    const int32_t* table = a.b.table + seq * a.b.table_stride;
+    const int first = from + 32 * (warp - kSoftWarps);  // its first key of step 0
+    auto page_of = [&](int j) {  // lane's group's page of step j, -1 if none
+        const int key = first + j * kKeys + 16 * lane;
+        if (lane > 1 || j >= steps || key >= end) return -1;
+        const int id = table[key >> a.b.page_shift];
+        if ((unsigned)id < (unsigned)a.b.n_pages) return id;
+        atomicOr(a.status, TB_B200_FLAG_PAGE_RANGE);
+        return -1;
+    };
+    const bool converts = warp >= kSoftWarps && warp < kIssuer;
+    int id = converts ? page_of(0) : -1, id_next = converts ? page_of(1) : -1;
+
     tc::fence_before();
     __syncthreads();
     tc::fence_after();
     const uint32_t tmem = sh.tmem;
 
-    // Q: a thread its row, all of it asked for at once, while the first codes come.
-    // A row with a NaN or an infinity is NaN.
-    const int tile = warp / 4, row = threadIdx.x & (kRows - 1);
-    const int r = tile * kRows + row;
+    // Q: a warp its 32 rows, all of them asked for at once, while the first codes
+    // come; a lane has the 16-byte piece `piece` of every kRound-th row.  A row with a
+    // NaN or an infinity is NaN.
+    constexpr int kEach = DP / 8, kRound = 32 / kEach;
+    const int tile = warp / 4, row0 = warp % 4 * 32, row = row0 + lane;
+    const int piece = lane % kEach, r = tile * kRows + row;
     const bool soft = warp < kSoftWarps, live = soft && r < rows;
     float f = 0.0f;  // what the row's sums of products are multiplied with
     const int tok = live ? (at + r) / group : 0, hh = live ? (at + r) % group : 0;
+    const int64_t head_at = (int64_t)(head * group + hh) * a.d;
     if (soft && tile < tiles) {
-        const T* q = static_cast<const T*>(a.q) + (s.lo + tok) * a.q_stride +
-                     (int64_t)(head * group + hh) * a.d;
-        uint4 x[DP / 8];
+        const int64_t mine = live ? (s.lo + tok) * a.q_stride + head_at : -1;
+        uint4 x[kEach];
 #pragma unroll
-        for (int i = 0; i < DP / 8; ++i) x[i] = load8(q + 8 * i, live && 8 * i < a.d, a.vec);
-        uint32_t two = 0;  // the largest magnitudes of the even and of the odd elements
+        for (int i = 0; i < kEach; ++i) {
+            const int64_t there = __shfl_sync(tbk::kFull, mine, i * kRound + lane / kEach);
+            x[i] = load8(static_cast<const T*>(a.q) + there + 8 * piece,
+                         there >= 0 && 8 * piece < a.d, a.vec);
+        }
 #pragma unroll
-        for (int i = 0; i < 4 * (DP / 8); ++i)
-            two = __vmaxu2(two, (&x[i / 4].x)[i % 4] & 0x7fff7fffu);
-        const uint32_t top = max(two & 0xffff0000u, two << 16);
-        const bool finite = top < 0x7f800000u;
-        const int e = min(max((int)(top >> 23), 1 + 16), 254);
-        // a negative scale turns q, so that larger sums are larger scores
-        const float lift = __uint_as_float((uint32_t)(127 + 14 - e + 127) << 23) *
-                           (a.scale < 0.0f ? -1.0f : 1.0f);
-        f = finite ? __uint_as_float((uint32_t)(e - 14) << 23) * (fabsf(a.scale) * kLog2e) : NAN;
+        for (int i = 0; i < kEach; ++i) {
+            uint32_t two = 0;  // the largest magnitudes of the even and of the odd elements
 #pragma unroll
-        for (int i = 0; i < DP / 8; ++i) {
+            for (int j = 0; j < 4; ++j) two = __vmaxu2(two, (&x[i].x)[j] & 0x7fff7fffu);
+#pragma unroll
+            for (int o = 1; o < kEach; o <<= 1)
+                two = __vmaxu2(two, __shfl_xor_sync(tbk::kFull, two, o));
+            const uint32_t top = max(two & 0xffff0000u, two << 16);
+            const bool finite = top < 0x7f800000u;
+            const int e = min(max((int)(top >> 23), 1 + 16), 254);
+            // a negative scale turns q, so that larger sums are larger scores
+            const float lift = __uint_as_float((uint32_t)(127 + 14 - e + 127) << 23) *
+                               (a.scale < 0.0f ? -1.0f : 1.0f);
+            const float unit =
+                finite ? __uint_as_float((uint32_t)(e - 14) << 23) * (fabsf(a.scale) * kLog2e) : NAN;
+            const float own = __shfl_sync(tbk::kFull, unit, lane % kRound * kEach);
+            if (lane / kRound == i) f = own;
             uint4 h;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
@@ -239,7 +276,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_chunk(const __grid_constant__ A
                 const float lo = __uint_as_float(w << 16), hi = __uint_as_float(w & 0xffff0000u);
                 (&h.x)[j] = finite ? kv8::pack_f16x2(lo * lift, hi * lift) : 0u;
             }
-            *reinterpret_cast<uint4*>(q_tiles + tile * H::kTile + place(row, i)) = h;
+            *reinterpret_cast<uint4*>(q_tiles + tile * H::kTile +
+                                      place(row0 + i * kRound + lane / kEach, piece)) = h;
         }
         tbk::fence_proxy_async_shared();
     }
@@ -297,22 +335,10 @@ __global__ void __launch_bounds__(kThreads, 1) k_chunk(const __grid_constant__ A
         }
     } else if (!soft) {
         tc::fewer_registers<kConvRegs>();
-        // Codes to f16.  The warp has keys 32 w .. 32 w + 31 of each step, two groups
-        // of 16 whose pages lanes 0 and 1 look up, ask for and ring in; a lane has
-        // the 16-byte piece c of every (32 / kPieces)th of them.
-        constexpr int kPieces = DP / 16, kRound = 32 / kPieces;
-        const int w = warp - kSoftWarps, c = lane % kPieces;
+        // Codes to f16; a lane has the 16-byte piece c of every (32 / kWide)th key.
+        constexpr int kWide = DP / 16, kStep = 32 / kWide;
+        const int w = warp - kSoftWarps, c = lane % kWide;
         uint8_t* codes = kv_tiles + kStages * 2 * H::kTile + w * 2 * 32 * DP;  // K, V
-        const int32_t* table = a.b.table + seq * a.b.table_stride;
-        const int first = from + 32 * w;  // the warp's first key of step 0
-        auto page_of = [&](int j) {  // lane's group's page of step j, -1 if none
-            const int key = first + j * kKeys + 16 * lane;
-            if (lane > 1 || j >= steps || key >= end) return -1;
-            const int id = table[key >> a.b.page_shift];
-            if ((unsigned)id < (unsigned)a.b.n_pages) return id;
-            atomicOr(a.status, TB_B200_FLAG_PAGE_RANGE);
-            return -1;
-        };
         auto ask = [&](int kv, int j, int id) {  // the groups that have a page
             const uint32_t have = __ballot_sync(tbk::kFull, id >= 0);
             if (lane == 0 && have) tbk::mbar_expect_tx(&sh.codes[kv][w], __popc(have) * 16 * DP);
@@ -324,7 +350,6 @@ __global__ void __launch_bounds__(kThreads, 1) k_chunk(const __grid_constant__ A
             }
             return have;
         };
-        int id = page_of(0), id_next = page_of(1);
         uint32_t have_k = ask(0, 0, id), have_v = ask(1, 0, id), phases = 0;
         float2 scale = make_float2(-1.0f, 0.0f);
         auto ask_scale = [&] {
@@ -352,16 +377,16 @@ __global__ void __launch_bounds__(kThreads, 1) k_chunk(const __grid_constant__ A
                     phases ^= 1u << kv;
                 }
                 if (!fine) break;
-                uint4 x[kPieces];
+                uint4 x[kWide];
 #pragma unroll
-                for (int i = 0; i < kPieces; ++i)
+                for (int i = 0; i < kWide; ++i)
                     x[i] = *reinterpret_cast<const uint4*>(
-                        codes + (kv * 32 + lane / kPieces + i * kRound) * DP + c * 16);
+                        codes + (kv * 32 + lane / kWide + i * kStep) * DP + c * 16);
                 if (have != 3 || key0 + 32 > s.len) {
                     // slots of no page or behind the last token may hold anything
 #pragma unroll
-                    for (int i = 0; i < kPieces; ++i) {
-                        const int key = lane / kPieces + i * kRound;
+                    for (int i = 0; i < kWide; ++i) {
+                        const int key = lane / kWide + i * kStep;
                         if (!(have >> key / 16 & 1) || key0 + key >= s.len)
                             x[i] = make_uint4(0, 0, 0, 0);
                     }
@@ -371,12 +396,12 @@ __global__ void __launch_bounds__(kThreads, 1) k_chunk(const __grid_constant__ A
                 __syncwarp();
                 (kv ? have_v : have_k) = ask(kv, j + 1, id);
 #pragma unroll
-                for (int i = 0; i < kPieces; ++i) {
+                for (int i = 0; i < kWide; ++i) {
                     uint4 h[2];
                     to_f16<FORMAT>(x[i], h);
                     // the lanes of a key's second panel write their pieces in the
                     // other order, into other banks
-                    const int key = 32 * w + lane / kPieces + i * kRound, y = c >> 2;
+                    const int key = 32 * w + lane / kWide + i * kStep, y = c >> 2;
                     uint8_t* tile_at = to + kv * H::kTile;
                     *reinterpret_cast<uint4*>(tile_at + place(key, 2 * c + y)) = y ? h[1] : h[0];
                     *reinterpret_cast<uint4*>(tile_at + place(key, 2 * c + 1 - y)) =
@@ -500,26 +525,31 @@ __global__ void __launch_bounds__(kThreads, 1) k_chunk(const __grid_constant__ A
         tc::fence_after();
         const bool none = !(sum != 0.0f);
         const float per = none || !fine ? 0.0f : exp2f(vref - ref - kLift) / sum;
-        T* out = static_cast<T*>(a.out) + (s.lo + tok) * a.out_stride +
-                 (int64_t)(head * group + hh) * a.d;
+        // through the rows of Q that are its own, for whole rows to be stored at once
+        uint8_t* own = q_tiles + tile * H::kTile;
 #pragma unroll 1
         for (int c0 = 0; c0 < DP; c0 += 32) {
             float x[32];
             if (steps > 0) tc::load<32>(o_at + c0, x);
-            if (!live) continue;
 #pragma unroll
             for (int e = 0; e < 32; e += 8) {
-                if (c0 + e >= a.d) break;
                 float y[8];
 #pragma unroll
                 for (int i = 0; i < 8; ++i) y[i] = none || steps == 0 ? 0.0f : x[e + i] * per;
-                if (a.vec_out) {
-                    tbk::store_vec<T, 8>(out + c0 + e, y);
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) tbk::Elt<T>::store(out + c0 + e + i, y[i]);
-                }
+                *reinterpret_cast<uint4*>(own + place(row, (c0 + e) / 8)) =
+                    make_uint4(tbk::pack_bf16x2(y[0], y[1]), tbk::pack_bf16x2(y[2], y[3]),
+                               tbk::pack_bf16x2(y[4], y[5]), tbk::pack_bf16x2(y[6], y[7]));
             }
+        }
+        __syncwarp();
+        const int64_t mine = live ? (s.lo + tok) * a.out_stride + head_at : -1;
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) {
+            const int other = i * kRound + lane / kEach;
+            const int64_t there = __shfl_sync(tbk::kFull, mine, other);
+            const uint4 y = *reinterpret_cast<const uint4*>(own + place(row0 + other, piece));
+            if (there >= 0 && 8 * piece < a.d)
+                store8(static_cast<T*>(a.out) + there + 8 * piece, y, a.vec_out);
         }
         if (a.lse && live)
             a.lse[(int64_t)(s.lo + tok) * a.hq + head * group + hh] =
@@ -548,8 +578,8 @@ int launch(Args& a, const TbB200Kv8* cache, dim3 grid, cudaStream_t s) {
 }
 
 // Slots of the grid: a bound on the batch's blocks, whatever max_rows is (64 sequences
-// of 100 rows 253 us; a grid of max_rows for each, 245 with the rows' own bound, 545
-// with the batch's, 6400).
+// of 100 rows took 253 us; with a grid of max_rows for each, 245 if that is 100 and
+// 545 if it is the batch's 6400).
 int64_t slots_of(const TbB200Kv8* cache, const TbB200Kv8Batch* batch,
                  const TbB200Kv8Attention* t) {
     const int64_t group = t->n_heads / cache->n_kv_heads;
