@@ -18,13 +18,13 @@
 // once for 256 rows, four times fewer than a block of 16 rows' matrix
 // instructions could share, and the products run at 4 times their rate.
 //
-// Measured: 2048 tokens behind 6144, 32 heads of 128 on 8, int8, 305 us, 789 TFLOP/s
+// Measured: 2048 tokens behind 6144, 32 heads of 128 on 8, int8, 302 us, 796 TFLOP/s
 // (0.48 of a library product's rate; blocks of 16 rows: 1634 us).  A step takes 2.35
 // us, 4500 clocks: a tile's scores, softmax (2600) and products follow one another,
 // and the products share shared memory's bandwidth with the conversion (3300 clocks
 // where 2050 are the least).  256 CTAs of 62 steps run on 148 SMs as two waves, 0.86
-// full; a CTA pays some 12 us beside its steps, so 64 sequences of 100 tokens and
-// 1000 keys take 239 us (253 with a thread a row of q and out).
+// full; a CTA pays some 9 us beside its steps, so 64 sequences of 100 tokens and
+// 1000 keys take 227 us (253 with a thread a row of q and out).
 //
 // Precision as in k_kv8_attention.cu: a row of q is scaled by a power of two to
 // [2^14, 2^15) and held as f16, exact for bf16 elements above 2^-31 of the row's
@@ -240,10 +240,13 @@ __global__ void __launch_bounds__(kThreads, 1) k_chunk(const __grid_constant__ A
     const int piece = lane % kEach, r = tile * kRows + row;
     const bool soft = warp < kSoftWarps, live = soft && r < rows;
     float f = 0.0f;  // what the row's sums of products are multiplied with
-    const int tok = live ? (at + r) / group : 0, hh = live ? (at + r) % group : 0;
-    const int64_t head_at = (int64_t)(head * group + hh) * a.d;
+    // where a row of the block stands in rows of `stride`, -1 if it is not there
+    auto row_at = [&](int i, int64_t stride) {
+        const int tok = i / group, h = head * group + i - tok * group;
+        return live ? (s.lo + tok) * stride + (int64_t)h * a.d : (int64_t)-1;
+    };
     if (soft && tile < tiles) {
-        const int64_t mine = live ? (s.lo + tok) * a.q_stride + head_at : -1;
+        const int64_t mine = row_at(at + r, a.q_stride);
         uint4 x[kEach];
 #pragma unroll
         for (int i = 0; i < kEach; ++i) {
@@ -251,30 +254,41 @@ __global__ void __launch_bounds__(kThreads, 1) k_chunk(const __grid_constant__ A
             x[i] = load8(static_cast<const T*>(a.q) + there + 8 * piece,
                          there >= 0 && 8 * piece < a.d, a.vec);
         }
+        // the largest magnitudes of the even and of the odd elements: of piece i, then,
+        // each lane keeping half of its rows, of all of row `piece` kRound + lane / kEach
+        uint32_t two[kEach];
 #pragma unroll
         for (int i = 0; i < kEach; ++i) {
-            uint32_t two = 0;  // the largest magnitudes of the even and of the odd elements
+            const uint32_t m = 0x7fff7fffu;
+            two[i] = __vmaxu2(__vmaxu2(x[i].x & m, x[i].y & m), __vmaxu2(x[i].z & m, x[i].w & m));
+        }
 #pragma unroll
-            for (int j = 0; j < 4; ++j) two = __vmaxu2(two, (&x[i].x)[j] & 0x7fff7fffu);
+        for (int o = kEach / 2; o > 0; o >>= 1)
 #pragma unroll
-            for (int o = 1; o < kEach; o <<= 1)
-                two = __vmaxu2(two, __shfl_xor_sync(tbk::kFull, two, o));
-            const uint32_t top = max(two & 0xffff0000u, two << 16);
-            const bool finite = top < 0x7f800000u;
-            const int e = min(max((int)(top >> 23), 1 + 16), 254);
-            // a negative scale turns q, so that larger sums are larger scores
-            const float lift = __uint_as_float((uint32_t)(127 + 14 - e + 127) << 23) *
-                               (a.scale < 0.0f ? -1.0f : 1.0f);
-            const float unit =
-                finite ? __uint_as_float((uint32_t)(e - 14) << 23) * (fabsf(a.scale) * kLog2e) : NAN;
-            const float own = __shfl_sync(tbk::kFull, unit, lane % kRound * kEach);
-            if (lane / kRound == i) f = own;
+            for (int i = 0; i < o; ++i) {
+                const bool up = piece & o;
+                const uint32_t other =
+                    __shfl_xor_sync(tbk::kFull, up ? two[i] : two[i + o], o);
+                two[i] = __vmaxu2(up ? two[i + o] : two[i], other);
+            }
+        const uint32_t top = max(two[0] & 0xffff0000u, two[0] << 16);
+        const int e = min(max((int)(top >> 23), 1 + 16), 254);
+        // a negative scale turns q, so that larger sums are larger scores
+        const float lift = __uint_as_float((uint32_t)(127 + 14 - e + 127) << 23) *
+                           (a.scale < 0.0f ? -1.0f : 1.0f);
+        const float unit = top < 0x7f800000u ? __uint_as_float((uint32_t)(e - 14) << 23) *
+                                                   (fabsf(a.scale) * kLog2e)
+                                             : NAN;
+        f = __shfl_sync(tbk::kFull, unit, lane % kRound * kEach + lane / kRound);
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) {
+            const float by = __shfl_sync(tbk::kFull, lift, lane - piece + i);
             uint4 h;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 const uint32_t w = (&x[i].x)[j];
-                const float lo = __uint_as_float(w << 16), hi = __uint_as_float(w & 0xffff0000u);
-                (&h.x)[j] = finite ? kv8::pack_f16x2(lo * lift, hi * lift) : 0u;
+                (&h.x)[j] = kv8::pack_f16x2(__uint_as_float(w << 16) * by,
+                                            __uint_as_float(w & 0xffff0000u) * by);
             }
             *reinterpret_cast<uint4*>(q_tiles + tile * H::kTile +
                                       place(row0 + i * kRound + lane / kEach, piece)) = h;
@@ -423,7 +437,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_chunk(const __grid_constant__ A
         if (tile < tiles) {
         const uint32_t s_at = tmem + tile * 128 + ((uint32_t)(warp % 4) << 21);
         const uint32_t o_at = s_at + 256;
-        const int see_hi = live ? s.first + tok : INT32_MAX;
+        const int see_hi = live ? s.first + (at + r) / group : INT32_MAX;
         // a row before position 0 sees no key, so that a see_lo that wraps does no harm
         const int see_lo =
             live && a.window ? max((int)((unsigned)see_hi - (unsigned)a.window + 1u), 0) : 0;
@@ -542,7 +556,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_chunk(const __grid_constant__ A
             }
         }
         __syncwarp();
-        const int64_t mine = live ? (s.lo + tok) * a.out_stride + head_at : -1;
+        const int64_t mine = row_at(at + r, a.out_stride);
 #pragma unroll
         for (int i = 0; i < kEach; ++i) {
             const int other = i * kRound + lane / kEach;
@@ -552,7 +566,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_chunk(const __grid_constant__ A
                 store8(static_cast<T*>(a.out) + there + 8 * piece, y, a.vec_out);
         }
         if (a.lse && live)
-            a.lse[(int64_t)(s.lo + tok) * a.hq + head * group + hh] =
+            a.lse[(int64_t)(s.lo + (at + r) / group) * a.hq + head * group + (at + r) % group] =
                 none ? -INFINITY : ref * 0.69314718055994531f + logf(sum);
         }
     }
