@@ -18,13 +18,13 @@
 // once for 256 rows, four times fewer than a block of 16 rows' matrix
 // instructions could share, and the products run at 4 times their rate.
 //
-// Measured: 2048 tokens behind 6144, 32 heads of 128 on 8, int8, 302 us, 796 TFLOP/s
-// (0.48 of a library product's rate; blocks of 16 rows: 1634 us).  A step takes 2.35
+// Measured: 2048 tokens behind 6144, 32 heads of 128 on 8, int8, 298 us, 807 TFLOP/s
+// (0.49 of a library product's rate; blocks of 16 rows: 1634 us).  A step takes 2.35
 // us, 4500 clocks: a tile's scores, softmax (2600) and products follow one another,
 // and the products share shared memory's bandwidth with the conversion (3300 clocks
 // where 2050 are the least).  256 CTAs of 62 steps run on 148 SMs as two waves, 0.86
 // full; a CTA pays some 9 us beside its steps, so 64 sequences of 100 tokens and
-// 1000 keys take 227 us (253 with a thread a row of q and out).
+// 1000 keys take 222 us (253 with a thread a row of q and out).
 //
 // Precision as in k_kv8_attention.cu: a row of q is scaled by a power of two to
 // [2^14, 2^15) and held as f16, exact for bf16 elements above 2^-31 of the row's
@@ -48,8 +48,10 @@ constexpr int kStages = 2;
 constexpr int kSoftWarps = 4 * kTiles, kConvWarps = 4;
 constexpr int kIssuer = kSoftWarps + kConvWarps;  // the warp
 constexpr int kThreads = 32 * (kIssuer + 4);  // a whole warpgroup, for its registers
-// Registers a thread of each: 256 * 192 + 128 * 72 + 128 * 56 = 512 * 128.
-constexpr int kSoftRegs = 192, kConvRegs = 72, kIssuerRegs = 56;
+// Registers a thread of each: 256 * 192 + 128 * 96 + 128 * 32 = 512 * 128 (with 184
+// for the first 329 us where 192 took 308, with 72 and 56 for the others 301 where 96
+// and 32 take 298).
+constexpr int kSoftRegs = 192, kConvRegs = 96, kIssuerRegs = 32;
 constexpr float kSlack = 4.0f, kLift = 11.0f, kLog2e = 1.4426950408889634f, kNoRef = -3.0e38f;
 constexpr float kLeast = -100.0f;  // weights before the sum are at 2^kLeast of the row's or above
 constexpr uint32_t kColumns = 512;  // of tensor memory: S and P at 0, 128, O at 256, 384
