@@ -58,14 +58,28 @@ DeviceState* current_device_state() {
         set_error("cudaDeviceGetAttribute", e);
         return nullptr;
     }
-    unsigned int* status = nullptr;
-    if ((e = cudaMalloc(&status, sizeof(unsigned int))) != cudaSuccess) {
-        set_error("cudaMalloc(status)", e);
+    // The first call on a device may be one that a stream is capturing: the status
+    // word is made beside the capture, on a stream of its own.
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    if ((e = cudaThreadExchangeStreamCaptureMode(&mode)) != cudaSuccess) {
+        set_error("cudaThreadExchangeStreamCaptureMode", e);
         return nullptr;
     }
-    if ((e = cudaMemset(status, 0, sizeof(unsigned int))) != cudaSuccess) {
-        set_error("cudaMemset(status)", e);
-        cudaFree(status);
+    unsigned int* status = nullptr;
+    cudaStream_t beside = nullptr;
+    const char* what = "cudaMalloc(status)";
+    e = cudaMalloc(&status, sizeof(unsigned int));
+    if (e == cudaSuccess) {
+        what = "cudaMemsetAsync(status)";
+        e = cudaStreamCreateWithFlags(&beside, cudaStreamNonBlocking);
+        if (e == cudaSuccess) e = cudaMemsetAsync(status, 0, sizeof(unsigned int), beside);
+        if (e == cudaSuccess) e = cudaStreamSynchronize(beside);
+        if (beside) cudaStreamDestroy(beside);
+        if (e != cudaSuccess) cudaFree(status);
+    }
+    cudaThreadExchangeStreamCaptureMode(&mode);
+    if (e != cudaSuccess) {
+        set_error(what, e);
         return nullptr;
     }
     ds->status = status;

@@ -913,3 +913,31 @@ def test_chunk_rows_in_front_and_clamped_starts(dev):
     T.kv8_attention(m.cache, q, i32([-9, 2 ** 31 - 1, 40], dev), ln[[3, 0]], tb[[3, 0]], out=out)
     assert torch.equal(out, one)
     assert T.check_status() == (0, 0)
+
+
+FIRST_CALL = """
+import sys, torch
+sys.path.insert(0, {repo!r})
+import perf.operators as M
+M.own = True
+case = [c for c in M.listed() if c["name"] == {name!r}][0]
+state = M.prepare(case, 1)
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    got = M.run(state)
+graph.replay()
+want = M.run(state)
+for a, b in zip(got, want):
+    assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+"""
+
+
+@pytest.mark.parametrize("name", ["attention long", "attention chunk", "qk_norm decode 256"])
+def test_first_call_is_captured(dev, name):
+    """A process whose first call of the library is captured into a graph."""
+    import os
+    import subprocess
+    import sys
+    repo = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    subprocess.run([sys.executable, "-c", FIRST_CALL.format(repo=repo, name=name)], cwd=repo,
+                   check=True, timeout=300)
