@@ -26,9 +26,10 @@
 //
 // Measured: 16384 rows of 64 + 8 heads of 128, bf16, 101 us, 6.0 TB/s (a copy:
 // 6.5; the first version, a head at a time: 127 us); norm and half the head, 4095
-// rows of 32 + 32 heads of 128, f32, 49.6 us, 5.4 TB/s; 777 rows of 32 + 32 heads
-// of 80, f32, 8.4 us and 256 rows of 32 + 32 heads of 128, bf16, 5.9 us, where a
-// launch and one row's chain of loads are most of the time.
+// rows of 32 + 32 heads of 128, f32, 46.1 us, 5.8 TB/s (49.6 with a division and a
+// root rounded to nearest in rsqrtf's place); 777 rows of 32 + 32 heads of 80, f32,
+// 8.4 us and 256 rows of 32 + 32 heads of 128, bf16, 5.2 us, where a launch and one
+// row's chain of loads are most of the time.
 #include <math.h>
 
 #include "tb_device.cuh"
@@ -104,7 +105,7 @@ struct Args {
     const int32_t* positions;
     const double* freqs;
     const void *q_weight, *k_weight;
-    float scale, eps;
+    float scale, eps, per;  // per: 1 / d
     int hq, hkv, d, r, group;
 };
 
@@ -206,8 +207,7 @@ __global__ void __launch_bounds__(kThreads, NU == 1 ? 4 : 1) k_rotary(const __gr
                 }
             if (NORM) {
                 for (int o = a.group >> 1; o > 0; o >>= 1) ss += __shfl_xor_sync(kFull, ss, o);
-                const float inv =
-                    __fdiv_rn(1.0f, __fsqrt_rn(__fadd_rn(__fdiv_rn(ss, (float)a.d), a.eps)));
+                const float inv = rsqrtf(fmaf(ss, a.per, a.eps));  // 2 ulp
                 const T* w = static_cast<const T*>(is_q ? a.q_weight : a.k_weight);
 #pragma unroll
                 for (int n = 0; n < NU; ++n)
@@ -330,6 +330,7 @@ int run(const TbB200Rotary* t, bool norm, void* stream) {
     Args a = {t->q,         t->k,     t->q_out,    t->k_out,    t->q_stride,    t->k_stride,
               t->q_out_stride, t->k_out_stride, t->positions, t->freqs,
               norm ? t->q_weight : nullptr, norm ? t->k_weight : nullptr, t->scale, t->eps,
+              1.0f / (float)t->head_dim,
               t->n_q_heads, t->n_kv_heads, t->head_dim, t->rotary_dim, 0};
     cudaStream_t s = tbh::stream_of(stream);
     const bool half_layout = t->layout == TB_B200_ROTARY_HALF;

@@ -6,8 +6,8 @@ Tolerances, with u = 2^-24 (half a step of f32, relative):
   2u of the first-order correction and u of the scaling; the two products and
   their sum add 2u of the larger sum: below 6u m (|x0| + |x1|) in all.
 - a norm's sum of squares has at most 16 terms per lane, 5 shuffle steps and
-  the products: 22u, halved by the root; the division, the addition of eps,
-  the root, the reciprocal and two products add 6u: 17u, below 20u.
+  the products: 22u, 1 / d and the product and sum with it 2u, all halved by
+  the root; rsqrtf's 2 ulp are 4u, two products 2u: 18u, below 20u.
 - bf16 outputs are rounded once more, by at most 2^-8 of the value.
 - the frequencies: pow in double within 2 ulp, 3 more operations: 2^-49.
 """
