@@ -24,7 +24,7 @@
 // in registers for all of them; the CTA has just the threads that make its passes
 // over the heads full ones.
 //
-// Measured: 16384 rows of 64 + 8 heads of 128, bf16, 101 us, 6.0 TB/s (a copy:
+// Measured: 16384 rows of 64 + 8 heads of 128, bf16, 94 us, 6.4 TB/s (a copy:
 // 6.5; the first version, a head at a time: 127 us); norm and half the head, 4095
 // rows of 32 + 32 heads of 128, f32, 46.1 us, 5.8 TB/s (49.6 with a division and a
 // root rounded to nearest in rsqrtf's place); 777 rows of 32 + 32 heads of 80, f32,
@@ -41,6 +41,12 @@ using tbk::kFull;
 
 constexpr int kMaxDim = 512;
 constexpr int kThreads = 256;
+
+// Most threads of a CTA.  The rotation of many rows alone streams best in small ones
+// (16384 rows of 72 heads of 128: 94 us with 128, 101 with 256; 8192 of 9 of 256: 18
+// and 24); 64 rows of 72 heads take 3.6 us with 128 and 3.2 with 256, 256 rows with
+// the norm 6.4 and 5.7, 4095 of f32 46.8 and 46.1.
+unsigned threads_of(bool norm, unsigned rows) { return norm || rows <= 4 * 148 ? 256 : 128; }
 
 // ---------------------------------------------------------------- vectors
 template <typename T, int VEC>
@@ -248,7 +254,8 @@ template <typename T, int VEC, int NU, bool NORM>
 void launch_layout(const Args& a, bool half_layout, unsigned rows, cudaStream_t s) {
     // the fewest passes over the heads, and the fewest threads for as many
     const int64_t lanes = (int64_t)(a.hq + a.hkv) * a.group;
-    const int64_t passes = (lanes + kThreads - 1) / kThreads;
+    const unsigned most = threads_of(NORM, rows);
+    const int64_t passes = (lanes + most - 1) / most;
     const unsigned threads = (unsigned)((lanes + passes * 32 - 1) / (passes * 32) * 32);
     if (half_layout)
         k_rotary<T, VEC, NU, true, NORM><<<rows, threads, 0, s>>>(a);
