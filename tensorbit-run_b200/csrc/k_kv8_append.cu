@@ -15,14 +15,14 @@
 // most e / page - s / page + 2 pages, so sequence i's slots start at row_start[i] /
 // page + 2 i, which a warp finds its sequence by.
 //
-// A unit has a CTA of 8 warps when its page is filled by a prompt, one warp (and a
-// CTA 8 heads) when a call brings few rows a sequence: then the time is the chain
-// of loads that leads to the rows, and a token's 16 vectors of a head need no more
-// lanes.  The rows stay in registers between amax and the codes, up to kHold
+// A unit has the warps, up to a CTA's 8, that hold its page's rows when prompts fill
+// it, one warp (and a CTA 8 heads) when a call brings few rows a sequence: then the
+// time is the chain of loads that leads to the rows, and a token's 16 vectors of a
+// head need no more lanes.  The rows stay in registers between amax and the codes, up to kHold
 // vectors a thread (a page of 64 rows of 128); what is past that is read again.
 //
-// Measured, 8 heads of 128, bf16: 14500 tokens of five prompts, e4m3, 18.5 us,
-// 4.8 TB/s; 256 sequences' token, int8, 4.2 us, a launch and the chain row_start ->
+// Measured, 8 heads of 128, bf16: 14476 tokens of five prompts, e4m3, 16.8 us,
+// 5.3 TB/s (18.3 with three CTAs an SM); 256 sequences' token, int8, 4.2 us, a launch and the chain row_start ->
 // page and rows -> scale and code.
 #include "kv8.cuh"
 
@@ -148,7 +148,7 @@ __device__ __forceinline__ void store_codes(uint8_t* p, const Piece<T, V>& x, fl
 }
 
 template <typename T, int FORMAT, int V, int WARPS>  // WARPS of a unit
-__global__ void __launch_bounds__(kThreads, 3) k_append(const __grid_constant__ Args a) {
+__global__ void __launch_bounds__(kThreads, WARPS == 1 ? 3 : 4) k_append(const __grid_constant__ Args a) {
     __shared__ uint2 red[kThreads / 32];
     constexpr int kUnit = 32 * WARPS;  // threads
     const kv8::Batch& b = a.b;
@@ -225,13 +225,17 @@ __global__ void __launch_bounds__(kThreads, 3) k_append(const __grid_constant__ 
         top[0] = __reduce_max_sync(tbk::kFull, top[0]);
         top[1] = __reduce_max_sync(tbk::kFull, top[1]);
         if (WARPS == 1) return;
-        __syncthreads();
+        const int in_cta = warp / WARPS;  // the unit's place in the CTA
+        auto meet = [&] {
+            asm volatile("bar.sync %0, %1;" ::"r"(in_cta + 1), "n"(kUnit) : "memory");
+        };
+        meet();
         if (lane == 0) red[warp] = make_uint2(top[0], top[1]);
-        __syncthreads();
+        meet();
 #pragma unroll
         for (int i = 0; i < WARPS; ++i) {
-            top[0] = max(top[0], red[i].x);
-            top[1] = max(top[1], red[i].y);
+            top[0] = max(top[0], red[in_cta * WARPS + i].x);
+            top[1] = max(top[1], red[in_cta * WARPS + i].y);
         }
     };
     over_unit();
@@ -309,15 +313,23 @@ __global__ void __launch_bounds__(kThreads, 3) k_append(const __grid_constant__ 
     }
 }
 
+template <typename T, int FORMAT, int V, int WARPS>
+void launch_units(const Args& a, unsigned slots, cudaStream_t s) {
+    constexpr int kUnits = kThreads / 32 / WARPS;  // of a CTA
+    const unsigned heads = (unsigned)(a.hkv + kUnits - 1) / kUnits;
+    k_append<T, FORMAT, V, WARPS><<<dim3(slots, heads), kThreads, 0, s>>>(a);
+}
+
 template <typename T, int FORMAT, int V>
-void launch(const Args& a, bool warps, unsigned slots, cudaStream_t s) {
-    if (warps) {
-        const unsigned heads = (unsigned)(a.hkv + kThreads / 32 - 1) / (kThreads / 32);
-        k_append<T, FORMAT, V, 1><<<dim3(slots, heads), kThreads, 0, s>>>(a);
-    } else {
-        k_append<T, FORMAT, V, kThreads / 32>
-            <<<dim3(slots, (unsigned)a.hkv), kThreads, 0, s>>>(a);
-    }
+void launch(const Args& a, int warps, unsigned slots, cudaStream_t s) {
+    if (warps == 1)
+        launch_units<T, FORMAT, V, 1>(a, slots, s);
+    else if (warps == 2)
+        launch_units<T, FORMAT, V, 2>(a, slots, s);
+    else if (warps == 4)
+        launch_units<T, FORMAT, V, 4>(a, slots, s);
+    else
+        launch_units<T, FORMAT, V, 8>(a, slots, s);
 }
 
 }  // namespace
@@ -343,10 +355,14 @@ extern "C" int tb_b200_kv8_append(const TbB200Kv8* cache, const TbB200Kv8Batch* 
     // One warp a unit when a sequence brings so few rows that kHold vectors a
     // lane hold them (bf16: rows * d <= 1024 elements).  A warp and a CTA a unit, 8
     // heads of 128: 256 sequences' token 4.7 and 15.1 us, 64 of 8 tokens 4.5 and 7.3,
-    // of 16 7.2 and 7.2, of 32 16.7 and 8.4.
+    // of 16 7.2 and 7.2, of 32 16.7 and 8.4.  Else as many as hold a page: 14500 tokens
+    // in pages of 16, heads of 128, two warps 21.9 us, eight 36.5; heads of 64, one
+    // 10.6, eight 32.9; pages of 32, four 21.6, eight 23.1.
     const size_t size = dtype == TB_DTYPE_F32 ? 4 : 2;
-    const bool warps = batch->rows * cache->head_dim * (int64_t)size <=
-                       (int64_t)batch->n_seqs * 32 * kHold * 16;
+    const int64_t few = 32 * kHold * 16;  // bytes that a warp's lanes hold
+    int warps = 1;
+    if (batch->rows * cache->head_dim * (int64_t)size > batch->n_seqs * few)
+        while (warps < 8 && cache->page * cache->head_dim * (int64_t)size > warps * few) warps *= 2;
     const bool vec = tbh::aligned16(k) && tbh::aligned16(v) && k_stride * size % 16 == 0 &&
                      v_stride * size % 16 == 0;
     cudaStream_t s = tbh::stream_of(stream);
