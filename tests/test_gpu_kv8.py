@@ -941,3 +941,26 @@ def test_first_call_is_captured(dev, name):
     repo = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
     subprocess.run([sys.executable, "-c", FIRST_CALL.format(repo=repo, name=name)], cwd=repo,
                    check=True, timeout=300)
+
+
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("page,hkv,d", [(16, 5, 128), (32, 3, 64), (16, 9, 96), (32, 5, 128)])
+def test_append_units_that_share_a_cta(dev, fmt, bf16, page, hkv, d):
+    """Small pages, whose heads share CTAs: prompts, then more rows, aligned and not,
+    one head of them with an infinity and a NaN."""
+    m = Model(dev, fmt, page, hkv, d, 40)
+    lengths = np.array([5 * page + 3, page - 1, 0, 2 * page])
+    table = tables(m.rng, lengths + 3 * page, page, 40)
+    fill(m, lengths, table, bf16)
+    m.same()
+    for pad in (0, 3):
+        counts = np.array([page, page + 1, 1, page // 2])
+        lengths = lengths + counts
+        st = starts_of(counts)
+        k, v = (rows_of(m.rng, int(st[-1]), hkv, d, bf16, dev, pad=pad) for _ in range(2))
+        k[2, 1, 5], v[3, 2, 6] = float("inf"), float("nan")
+        T.kv8_append(m.cache, k, v, i32(st, dev), i32(lengths, dev), i32(table, dev))
+        m.append([f64(k), f64(v)], st, lengths, table)
+        m.same()
+        assert T.check_status() == (8, T.FLAG_NONFINITE)
