@@ -36,6 +36,7 @@
 #include <math.h>
 
 #include "kv8_mma.cuh"
+#include "phases.cuh"
 #include "tcgen05.cuh"
 
 namespace {
@@ -45,6 +46,7 @@ constexpr int kTiles = 2;          // of a CTA
 constexpr int kKeys = 128;         // of a step
 constexpr int kGroups = kKeys / 16;  // of keys, each in one page
 constexpr int kStages = 2;
+using Stages = tbk::Ring<kStages>;
 constexpr int kSoftWarps = 4 * kTiles, kConvWarps = 4;
 constexpr int kIssuer = kSoftWarps + kConvWarps;  // the warp
 constexpr int kThreads = 32 * (kIssuer + 4);  // a whole warpgroup, for its registers
@@ -311,7 +313,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_chunk(const __grid_constant__ A
                 tc::tile_descriptor(tbk::smem_addr(kv_tiles) + H::kTile, H::kPanel);
             auto scores = [&](int t, int j) {  // S of tile t and step j
                 const uint64_t q = q_desc + t * (H::kTile / 16);
-                const uint64_t k = k_desc + (j % kStages) * (2 * H::kTile / 16);
+                const uint64_t k = k_desc + Stages::stage(j) * (2 * H::kTile / 16);
 #pragma unroll
                 for (int i = 0; i < kSteps; ++i) {
                     const int off = (i / 4 * H::kPanel + i % 4 * 32) / 16;
@@ -324,9 +326,9 @@ __global__ void __launch_bounds__(kThreads, 1) k_chunk(const __grid_constant__ A
             tc::fence_after();
             for (int t = 0; t < tiles && fine; ++t) scores(t, 0);
             for (int j = 0; j < steps && fine; ++j) {
-                const int stage = j % kStages;
+                const int stage = Stages::stage(j);
                 const uint64_t v = v_desc + stage * (2 * H::kTile / 16);
-                fine = wait_all(&sh.v_full[stage], j / kStages & 1, a.status);
+                fine = wait_all(&sh.v_full[stage], Stages::parity(j), a.status);
                 for (int t = 0; t < tiles && fine; ++t) {
                     fine = wait_all(&sh.p_full[t], j & 1, a.status);
                     if (!fine) break;
@@ -336,11 +338,12 @@ __global__ void __launch_bounds__(kThreads, 1) k_chunk(const __grid_constant__ A
                         tc::mma_tmem(tmem + 256 + t * 128, tmem + t * 128 + i * 8,
                                      v + i * (2048 / 16), instr_o, j > 0 || i > 0, leader);
                     tc::commit(&sh.o_done[t], leader);
-                    if (t == tiles - 1) tc::commit(&sh.kv_free[stage], leader);
+                    if (t == tiles - 1 && Stages::awaited(j, steps))
+                        tc::commit(&sh.kv_free[stage], leader);
                     if (j + 1 < steps) {
                         if (t == 0) {
-                            fine = wait_all(&sh.k_full[(j + 1) % kStages], (j + 1) / kStages & 1,
-                                            a.status);
+                            fine = wait_all(&sh.k_full[Stages::stage(j + 1)],
+                                            Stages::parity(j + 1), a.status);
                             if (!fine) break;
                             tc::fence_after();
                         }
@@ -376,8 +379,9 @@ __global__ void __launch_bounds__(kThreads, 1) k_chunk(const __grid_constant__ A
         ask_scale();
         bool fine = true;
         for (int j = 0; j < steps && fine; ++j) {
-            const int stage = j % kStages, key0 = first + j * kKeys;
-            fine = j < kStages || wait_all(&sh.kv_free[stage], (j / kStages - 1) & 1, a.status);
+            const int stage = Stages::stage(j), key0 = first + j * kKeys;
+            fine = !Stages::reused(j) ||
+                   wait_all(&sh.kv_free[stage], Stages::parity(j - kStages), a.status);
             if (!fine) break;
             uint8_t* to = kv_tiles + stage * 2 * H::kTile;
             if (lane < 2)
@@ -446,7 +450,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_chunk(const __grid_constant__ A
         float ref = kNoRef, vref = kNoRef, sum = 0.0f;
         bool fine = true;
         for (int j = 0; j < steps; ++j) {
-            fine = wait_all(&sh.k_full[j % kStages], j / kStages & 1, a.status) &&
+            fine = wait_all(&sh.k_full[Stages::stage(j)], Stages::parity(j), a.status) &&
                    wait_all(&sh.s_full[tile], j & 1, a.status);
             if (!fine) break;
             tc::fence_after();
@@ -455,7 +459,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_chunk(const __grid_constant__ A
             uint32_t have = 0;  // groups that have a page
 #pragma unroll
             for (int i = 0; i < kGroups; ++i) {
-                const float2 x = sh.scales[j % kStages][i];
+                const float2 x = sh.scales[Stages::stage(j)][i];
                 fs[i] = f * x.x;
                 lv[i] = x.y;
                 have |= (uint32_t)(x.x > 0.0f) << i;

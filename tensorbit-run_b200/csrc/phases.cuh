@@ -1,0 +1,22 @@
+// phases.cuh -- which phase of which barrier the steps of a pipeline wait for.  Plain
+// arithmetic, the same on the host, where tests/test_phases.py runs it.
+#pragma once
+
+#include <stdint.h>
+
+namespace tbk {
+
+// A ring of STAGES barriers: step j uses barrier j % STAGES, each use one completion.
+template <int STAGES>
+struct Ring {
+    static constexpr int stage(int j) { return j % STAGES; }
+    static constexpr uint32_t parity(int j) { return (uint32_t)(j / STAGES) & 1u; }
+    // Whether step j takes a stage that an earlier step, j - STAGES, has to free.
+    static constexpr bool reused(int j) { return j >= STAGES; }
+    // Whether a later step of `steps` waits for step j's stage to be free.  A completion
+    // that nobody waits for may come after the block has ended, when its shared memory
+    // is another's.
+    static constexpr bool awaited(int j, int steps) { return j + STAGES < steps; }
+};
+
+}  // namespace tbk

@@ -1,0 +1,65 @@
+"""The barrier arithmetic of the pipelined kernels (csrc/phases.cuh), on the host: a
+small C++ program runs it against barriers that count their phases."""
+import os
+import subprocess
+
+import pytest
+
+CSRC = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))),
+                    "tensorbit-run_b200", "csrc")
+
+FAKE = """
+#include <cassert>
+#include <cstdio>
+#include "phases.cuh"
+// A barrier of one arrival a phase, and its wait: whether phase `parity` is complete.
+struct Barrier {
+    int completed = 0, awaited = 0;
+    void complete() { ++completed; }
+    bool done(uint32_t parity) const { return (uint32_t)(completed & 1) != parity; }
+    bool wait(uint32_t parity) { return done(parity) ? (awaited = completed, true) : false; }
+};
+"""
+
+
+@pytest.fixture
+def run(tmp_path):
+    def go(body):
+        src, exe = tmp_path / "t.cpp", tmp_path / "t"
+        src.write_text(FAKE + body)
+        subprocess.run(["g++", "-std=c++17", "-O1", "-Wall", "-Werror", "-D__device__=",
+                        "-D__host__=", "-D__forceinline__=inline", "-I", CSRC, str(src), "-o",
+                        str(exe)], check=True, timeout=120)
+        subprocess.run([str(exe)], check=True, timeout=60)
+    return go
+
+
+def test_no_stage_is_freed_for_nobody(run):
+    """A producer that fills a ring, and a consumer that frees each stage when a later
+    step waits for it: each wait is for the phase that the step before completed, and
+    at the end every completion has been waited for."""
+    run("""
+template <int S> void ring(int steps) {
+    using R = tbk::Ring<S>;
+    Barrier full[S], free[S];
+    for (int j = 0; j < steps; ++j) {
+        Barrier& f = free[R::stage(j)];
+        if (R::reused(j)) {
+            assert(f.completed == j / S);  // once by each earlier use
+            assert(f.wait(R::parity(j - S)) && !f.done(R::parity(j)));
+        }
+        Barrier& b = full[R::stage(j)];
+        assert(!b.done(R::parity(j)));
+        b.complete();
+        assert(b.wait(R::parity(j)));
+        if (R::awaited(j, steps)) f.complete();
+    }
+    for (int i = 0; i < S; ++i) {
+        assert(free[i].awaited == free[i].completed);
+        assert(full[i].awaited == full[i].completed);
+    }
+}
+int main() {
+    for (int steps = 0; steps < 20; ++steps) ring<1>(steps), ring<2>(steps), ring<3>(steps);
+}
+""")
