@@ -85,6 +85,7 @@ struct Shared {
     uint64_t k_full[kStages], v_full[kStages], kv_free[kStages];
     uint64_t s_full[kTiles], p_full[kTiles], o_done[kTiles];
     uint64_t codes[2][kConvWarps];  // of K, of V: the warp's have come
+    uint64_t products_done;         // all that the issuer issued
     float2 scales[kStages][kGroups];  // of K (< 0: no page) and log2 of V's
     uint32_t tmem;
 };
@@ -208,6 +209,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_chunk(const __grid_constant__ A
             tbk::mbar_init(&sh.p_full[i], 4);
             tbk::mbar_init(&sh.o_done[i], 1);
         }
+        tbk::mbar_init(&sh.products_done, 1);
         for (int i = 0; i < kConvWarps; ++i) {
             tbk::mbar_init(&sh.codes[0][i], 1);
             tbk::mbar_init(&sh.codes[1][i], 1);
@@ -351,6 +353,9 @@ __global__ void __launch_bounds__(kThreads, 1) k_chunk(const __grid_constant__ A
                     }
                 }
             }
+            // whatever ended the loop, no product may be in flight when tensor memory is freed
+            tc::commit(&sh.products_done, leader);
+            wait_all(&sh.products_done, 0, a.status);
         }
     } else if (!soft) {
         tc::fewer_registers<kConvRegs>();
@@ -369,7 +374,12 @@ __global__ void __launch_bounds__(kThreads, 1) k_chunk(const __grid_constant__ A
             }
             return have;
         };
-        uint32_t have_k = ask(0, 0, id), have_v = ask(1, 0, id), phases = 0;
+        uint32_t have_k = ask(0, 0, id), have_v = ask(1, 0, id);
+        tbk::Phases phases;
+        auto codes_came = [&](int kv) {
+            return phases.wait(
+                kv, [&](uint32_t parity) { return wait_all(&sh.codes[kv][w], parity, a.status); });
+        };
         float2 scale = make_float2(-1.0f, 0.0f);
         auto ask_scale = [&] {
             scale = make_float2(-1.0f, 0.0f);
@@ -392,10 +402,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_chunk(const __grid_constant__ A
 #pragma unroll
             for (int kv = 0; kv < 2; ++kv) {
                 const uint32_t have = kv ? have_v : have_k;
-                if (have) {
-                    fine = wait_all(&sh.codes[kv][w], phases >> kv & 1, a.status);
-                    phases ^= 1u << kv;
-                }
+                fine = !have || codes_came(kv);
                 if (!fine) break;
                 uint4 x[kWide];
 #pragma unroll
@@ -434,8 +441,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_chunk(const __grid_constant__ A
             ask_scale();
         }
         if (!fine) {  // no copy may be in flight when the block ends
-            if (have_k) wait_all(&sh.codes[0][w], phases & 1, a.status);
-            if (have_v) wait_all(&sh.codes[1][w], phases >> 1 & 1, a.status);
+            if (have_k) codes_came(0);
+            if (have_v) codes_came(1);
         }
     } else {
         if (steps > 0) asm volatile("bar.arrive 1, %0;" ::"n"(32 * (kSoftWarps + 1)) : "memory");

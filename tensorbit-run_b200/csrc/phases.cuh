@@ -19,4 +19,19 @@ struct Ring {
     static constexpr bool awaited(int j, int steps) { return j + STAGES < steps; }
 };
 
+// The phases of up to 32 barriers that are waited for when there is something to wait
+// for, a bit each: the one that the next completion of barrier i ends.  A wait that gives
+// up leaves the phase as it is, so that a second one asks for the same completion; past it
+// the barrier would answer for the phase before, at once, with the copy still in flight.
+struct Phases {
+    uint32_t bits = 0;
+    // came(parity): the bounded wait of barrier i
+    template <typename F>
+    __device__ __forceinline__ bool wait(int i, F came) {
+        if (!came(bits >> i & 1u)) return false;
+        bits ^= 1u << i;
+        return true;
+    }
+};
+
 }  // namespace tbk

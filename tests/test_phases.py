@@ -63,3 +63,28 @@ int main() {
     for (int steps = 0; steps < 20; ++steps) ring<1>(steps), ring<2>(steps), ring<3>(steps);
 }
 """)
+
+
+def test_a_wait_that_gave_up_asks_again(run):
+    """A copy that comes after its wait gave up: the clean-up's wait is for that copy,
+    not for the one before, at either parity."""
+    run("""
+int main() {
+    for (int before = 0; before < 5; ++before) {
+        Barrier b[2];
+        tbk::Phases p;
+        auto came = [&](int i) { return p.wait(i, [&](uint32_t parity) { return b[i].wait(parity); }); };
+        for (int j = 0; j < before; ++j) {
+            b[1].complete();
+            assert(came(1));
+            assert(!came(1));  // one wait a completion
+        }
+        assert(!came(1) && !came(1));  // in flight
+        assert(!came(0));
+        b[1].complete();
+        assert(came(1) && !came(0));
+        b[0].complete();
+        assert(came(0) && !came(1));
+    }
+}
+""")
