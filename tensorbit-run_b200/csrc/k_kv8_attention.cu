@@ -41,6 +41,7 @@
 // window of 1000) the warps' instructions, about 550 for 32 keys and 1800 a block,
 // issued at half rate by the 12 warps that registers allow: 33 us.
 #include "kv8_mma.cuh"
+#include "phases.cuh"
 
 namespace {
 
@@ -225,7 +226,7 @@ k_attend(const __grid_constant__ Args a) {
         for (int i = 0; i < kStages; ++i) tbk::mbar_init(bar + i, 1);
         tbk::fence_mbar_init();
     }
-    uint32_t phases = 0;  // of each stage's barrier: a page out of range has no copy
+    tbk::Phases phases;  // of each stage's barrier: a page out of range has no copy
 
     // This CTA's share: [tile, stop) of the batch's spans, the first in sequence
     // seq, whose own begin at seq_begin.
@@ -467,6 +468,12 @@ k_attend(const __grid_constant__ Args a) {
             }
 
         int at_stage = kStages - 1;
+        bool lost = false;  // a copy did not come
+        auto copy_came = [&](int i) {
+            return phases.wait(i, [&](uint32_t parity) {
+                return __all_sync(tbk::kFull, tbk::mbar_wait(bar + i, parity, a.status));
+            });
+        };
         for (int n = 0; n < n_steps; ++n) {
             const int i0 = n % kBatch * kHalves;
             if (i0 == 0) {
@@ -487,18 +494,14 @@ k_attend(const __grid_constant__ Args a) {
                 lv[f] = (float)((int)(__float_as_uint(v_scale) >> 23) - 127);
             }
             uint8_t* stage = ring + at_stage * H::kStageBytes;
-            const uint32_t phase = phases >> at_stage & 1;
-            phases ^= 1u << at_stage;
-            const bool came = tbk::mbar_wait(bar + at_stage, phase, a.status);
-            if (!__all_sync(tbk::kFull, came)) {
-                // the copy did not come: the output is invalid and flagged.  No copy
-                // may be in flight when the block ends: wait for the others, bounded.
-                for (int i = 1; i < kStages; ++i) {
-                    const int x = (at_stage + i) % kStages;
+            if (!copy_came(at_stage)) {
+                // the output is invalid and flagged.  No copy may be in flight when the
+                // CTA ends: wait for this one and those behind it, bounded.
+                for (int i = 0; i < kStages; ++i)
                     if (page_of((n + i) * kHalves) >= 0 ||
                         (kHalves == 2 && page_of((n + i) * kHalves + 1) >= 0))
-                        tbk::mbar_wait(bar + x, phases >> x & 1, a.status);
-                }
+                        copy_came((at_stage + i) % kStages);
+                lost = true;
                 break;
             }
             const int key0 = first + n * kStride;
@@ -711,7 +714,9 @@ k_attend(const __grid_constant__ Args a) {
                 }
             }
         }
-        __syncthreads();  // the rings are free: the warps' states meet in their place
+        // the rings are free: the warps' states meet in their place.  Where a copy was lost
+        // the CTA does no more: a barrier that gave up may be in any phase
+        if (__syncthreads_or(lost)) return;
 
         // o[h 8 + u][b][2 r + e]: element 128 h + kWide g + 2 u + r of row 8 b + 2 t
         // + e.  A row's pairs are stored turned by turn(g) within their kWide, and

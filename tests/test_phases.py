@@ -88,3 +88,45 @@ int main() {
     }
 }
 """)
+
+
+def test_a_lost_copy_leaves_none_in_flight(run):
+    """A ring of stages filled ahead, where the copies from step `late` on come only
+    after a wait gave up on them: waiting for that step's stage again and for those
+    behind it, those of steps without a copy left out, brings all of them in."""
+    run("""
+template <int S> void ring(int steps, int late, unsigned missing) {
+    Barrier b[S];
+    int asked[S] = {}, in_flight = 0;
+    tbk::Phases p;
+    auto has = [&](int n) { return n < steps && !(missing >> n & 1); };
+    auto issue = [&](int n) {
+        if (!has(n)) return;
+        if (n >= late) asked[n % S] = 1, ++in_flight; else b[n % S].complete();
+    };
+    auto came = [&](int i) {
+        return p.wait(i, [&](uint32_t parity) {
+            if (b[i].wait(parity)) return true;
+            if (asked[i] == 1) { asked[i] = 2; return false; }      // gives up
+            if (asked[i] == 2) { b[i].complete(); --in_flight; }    // late, but there
+            return b[i].wait(parity);
+        });
+    };
+    for (int n = 0; n < S - 1; ++n) issue(n);
+    for (int n = 0; n < steps; ++n) {
+        issue(n + S - 1);
+        if (!has(n) || came(n % S)) continue;
+        for (int i = 0; i < S; ++i)
+            if (has(n + i) && !came((n + i) % S)) came((n + i) % S);
+        assert(in_flight == 0);
+        return;
+    }
+    assert(in_flight == 0);
+}
+int main() {
+    for (int steps = 0; steps < 12; ++steps)
+        for (int late = 0; late <= steps; ++late)
+            for (unsigned missing = 0; missing < 4096; missing += 37)
+                ring<2>(steps, late, missing), ring<3>(steps, late, missing);
+}
+""")
