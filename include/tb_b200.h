@@ -457,8 +457,11 @@ int tb_b200_kv8_append(const TbB200Kv8* cache, const TbB200Kv8Batch* batch, int 
  * or table_width * page, or with more than max_rows rows, raises
  * TB_B200_FLAG_POSITION_RANGE and its rows are as without keys; keys in a
  * page outside [0, n_pages) are not attended and raise
- * TB_B200_FLAG_PAGE_RANGE.  What the cache holds in slots that a row does not
- * attend never reaches its result. */
+ * TB_B200_FLAG_PAGE_RANGE.  Slots that no row of the call attends may hold
+ * anything, and a page of only such slots (in front of every window, say) needs
+ * no number: neither reaches a result or raises a flag.  Slots that some row
+ * attends hold numbers, as tb_b200_kv8_append leaves them; an e4m3 NaN code
+ * there may reach other rows of its sequence too. */
 typedef struct {
     int dtype; /* of q and out: TB_DTYPE_F32 or TB_DTYPE_BF16 */
     int n_heads; /* a multiple of the cache's n_kv_heads */

@@ -122,17 +122,19 @@ __device__ __forceinline__ Load load_of(const Args& a, int seq) {
 struct Block {
     int rows;       // live rows of the block
     int from, end;  // keys [from, end), from a whole step
+    int seen;       // the first key that a row attends: those from `from` to it are masked
 };
 
 __device__ __forceinline__ Block block_of(const Args& a, const Load& l, int block) {
     Block k;
     const int group = a.hq / a.hkv, at = block * a.block_rows;
     k.rows = min(a.block_rows, l.s.n * group - at);
-    k.from = k.end = 0;
+    k.from = k.end = k.seen = 0;
     if (l.ok) {
         const int p0 = l.s.first + at / group, p1 = l.s.first + (at + k.rows - 1) / group;
         k.end = max(p1 + 1, 0);
-        k.from = min(kv8::first_seen(p0, a.window), k.end) & ~31;
+        k.seen = min(kv8::first_seen(p0, a.window), k.end);
+        k.from = k.seen & ~31;
     }
     return k;
 }
@@ -324,10 +326,12 @@ k_attend(const __grid_constant__ Args a) {
         const int32_t* table = a.b.table + seq * a.b.table_stride;
         // A step's 16-key halves are in one page, or, with pages of 16, in two.
         const bool one_page = a.b.page_shift >= 5;
+        const int in_page = one_page ? kKeys : 16;  // keys that a lookup is for
         auto page_of = [&](int i) {  // the page of half-step i, -1 if it has none
             const int key =
                 first + i / kHalves * kStride + (kHalves == 2 && !one_page ? i % 2 * 16 : 0);
-            if (i / kHalves >= n_steps || key >= end) return -1;
+            // (a page all in front of a window may be gone)
+            if (i / kHalves >= n_steps || key >= end || key + in_page <= blk.seen) return -1;
             const int id = table[key >> a.b.page_shift];
             if (id >= 0 && id < a.b.n_pages) return id;
             atomicOr(a.status, TB_B200_FLAG_PAGE_RANGE);
@@ -507,13 +511,14 @@ k_attend(const __grid_constant__ Args a) {
             const int key0 = first + n * kStride;
             uint8_t* values = stage + kKeys * DP;
             const uint32_t stage_s = tbk::smem_addr(stage);
-            const bool gaps = key0 + kKeys > load.s.len || have != (1 << kHalves) - 1;
+            const bool gaps = key0 < blk.seen || key0 + kKeys > blk.end ||
+                              have != (1 << kHalves) - 1;
             if (gaps) {
-                // slots behind the last token, or of no page, may hold anything, NaN
-                // codes too: a weight of zero needs a finite value beside it
+                // slots that no row of the block attends, or of no page, may hold anything,
+                // NaN codes too: a weight of zero needs a finite value beside it
                 for (int i = lane; i < kKeys * DP / 16; i += 32) {
                     const int key = i % kKeys;
-                    if (key0 + key >= load.s.len || !(have >> key / 16 & 1))
+                    if (key0 + key < blk.seen || key0 + key >= blk.end || !(have >> key / 16 & 1))
                         *reinterpret_cast<uint4*>(values + place<DP, kKeys>(key, i / kKeys)) =
                             make_uint4(0, 0, 0, 0);
                 }

@@ -964,3 +964,87 @@ def test_append_units_that_share_a_cta(dev, fmt, bf16, page, hkv, d):
         m.append([f64(k), f64(v)], st, lengths, table)
         m.same()
         assert T.check_status() == (8, T.FLAG_NONFINITE)
+
+
+# ---------------------------------------------------------- in front of a window
+def spoil(m, table, keys):
+    """Anything in the slots of sequence 0's `keys`: NaN codes of e4m3 (127 and -1 as
+    int8 codes), beside scales that stay as they were."""
+    import torch
+    for c in (m.cache.k, m.cache.v):
+        c = c.view(torch.uint8)
+        for j in keys:
+            c[int(table[0][j // m.page]), :, j % m.page] = 0x7f if j % 2 else 0xff
+
+
+def front_of_window(dev, fmt, bf16, page, heads, hkv, d, rows, length, window):
+    """A sequence whose rows do not see its first keys: with those spoilt, then their
+    whole pages given back, the same bits and no flag."""
+    import torch
+    m = Model(dev, fmt, page, hkv, d, -(-length // page) + 2)
+    table = tables(m.rng, [length], page, len(m.scales[0]))
+    fill(m, [length], table)
+    q = rows_of(m.rng, rows, heads, d, bf16, dev, spread=False)
+    kw = dict(window=window, q=q, by_head=True)
+    want = attend(m, [rows], [length], table, heads, bf16, **kw)
+    first = max(length - rows - window + 1, 0)  # the first key that a row sees
+    assert first > page
+    spoil(m, table, range(first))
+    st, ln = i32([0, rows], dev), i32([length], dev)
+    for gone in (-1, len(m.scales[0])):
+        got = T.kv8_attention(m.cache, q, st, ln, i32(table, dev), window=window, return_lse=True)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+        assert T.check_status() == (0, 0)
+        table = table.copy()
+        table[0, :first // page] = gone
+    # one page more: the first row sees its last key
+    table[0, first // page] = gone
+    attend(m, [rows], [length], table, heads, bf16, bad=(gone, -1), **kw)
+    assert T.check_status() == (8, T.FLAG_PAGE_RANGE)
+
+
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("page,heads,hkv,d,rows,length,window", [
+    (16, 8, 1, 64, 1, 121, 5),      # a step's first half in front
+    (16, 4, 2, 128, 1, 200, 16), (32, 4, 4, 80, 1, 300, 31),
+    (16, 3, 1, 256, 1, 222, 13),    # a step of 16 in front
+    (64, 3, 1, 208, 2, 333, 40), (128, 2, 2, 128, 5, 400, 77),
+    (16, 4, 2, 64, 30, 177, 1),     # blocks of 8 tokens
+    (64, 8, 8, 128, 1, 9000, 4500)])  # cut into shares
+def test_pages_in_front_of_a_window(dev, fmt, bf16, page, heads, hkv, d, rows, length, window):
+    front_of_window(dev, fmt, bf16, page, heads, hkv, d, rows, length, window)
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+def test_keys_after_a_blocks_rows(dev, bf16):
+    """What rows of later tokens alone attend: NaN codes there leave the rows of
+    earlier blocks as they were."""
+    import torch
+    m = Model(dev, "e4m3", 32, 1, 64, 6)
+    table = tables(m.rng, [150], 32, 6)
+    fill(m, [150], table)
+    q = rows_of(m.rng, 50, 1, 64, bf16, dev, spread=False)  # blocks of 16 tokens, from 100
+    args = (i32([0, 50], dev), i32([150], dev), i32(table, dev))
+    want = T.kv8_attention(m.cache, q, *args)
+    spoil(m, table, range(116, 150))
+    got = T.kv8_attention(m.cache, q, *args)
+    assert torch.equal(got[:16], want[:16]) and bool(torch.isnan(got[-1]).any())
+    assert T.check_status() == (0, 0)
+
+
+def test_attended_bad_page_is_flagged(dev):
+    """Rows whose window ends in a page of number -1 are flagged and attend the rest;
+    rows behind it are not (the calls of test_rows_before_the_first_sequence, apart)."""
+    m = Model(dev, "int8", 16, 2, 64, 8)
+    table = [[-1, -1, 9, -1, 5, 6, 7]]
+    k, v = (rows_of(m.rng, 46, 2, 64, True, dev) for _ in range(2))
+    T.kv8_append(m.cache, k, v, i32([0, 46], dev), i32([110], dev), i32(table, dev))
+    m.append([f64(k), f64(v)], [0, 46], [110], table)
+    broken = [[-1, -1, 9, -1, -1, 6, 7]]
+    attend(m, [30], [110], broken, 4, True, window=3, bad=(-1, 9))  # positions 80 ..
+    assert T.check_status() == (8, T.FLAG_PAGE_RANGE)
+    attend(m, [28], [110], broken, 4, True, window=3, bad=(-1, 9))  # positions 82 ..
+    assert T.check_status() == (0, 0)
+    attend(m, [1], [110], broken, 4, True, window=3, bad=(-1, 9))
+    assert T.check_status() == (0, 0)
