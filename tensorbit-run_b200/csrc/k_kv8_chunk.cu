@@ -192,10 +192,10 @@ __global__ void __launch_bounds__(kThreads, 1) k_chunk(const __grid_constant__ A
     const bool ok = s.len <= a.max_len && s.n <= a.max_rows &&
                     s.len <= ((int64_t)a.b.width << a.b.page_shift);
     if (!ok && threadIdx.x == 0) atomicOr(a.status, TB_B200_FLAG_POSITION_RANGE);
-    // keys [from, end) that some row sees
+    // keys [seen, end) that some row sees, from a whole step
     const int p0 = s.first + at / group, p1 = s.first + (at + rows - 1) / group;
     const int end = ok ? max(p1 + 1, 0) : 0;
-    const int from = a.window ? min(kv8::first_seen(p0, a.window), end) & ~(kKeys - 1) : 0;
+    const int seen = min(kv8::first_seen(p0, a.window), end), from = seen & ~(kKeys - 1);
     const int steps = (end - from + kKeys - 1) / kKeys;
 
     if (threadIdx.x == 0) {
@@ -224,7 +224,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_chunk(const __grid_constant__ A
     const int first = from + 32 * (warp - kSoftWarps);  // its first key of step 0
     auto page_of = [&](int j) {  // lane's group's page of step j, -1 if none
         const int key = first + j * kKeys + 16 * lane;
-        if (lane > 1 || j >= steps || key >= end) return -1;
+        // (a page all in front of a window may be gone)
+        if (lane > 1 || j >= steps || key >= end || key + 16 <= seen) return -1;
         const int id = table[key >> a.b.page_shift];
         if ((unsigned)id < (unsigned)a.b.n_pages) return id;
         atomicOr(a.status, TB_B200_FLAG_PAGE_RANGE);
@@ -409,12 +410,12 @@ __global__ void __launch_bounds__(kThreads, 1) k_chunk(const __grid_constant__ A
                 for (int i = 0; i < kWide; ++i)
                     x[i] = *reinterpret_cast<const uint4*>(
                         codes + (kv * 32 + lane / kWide + i * kStep) * DP + c * 16);
-                if (have != 3 || key0 + 32 > s.len) {
-                    // slots of no page or behind the last token may hold anything
+                if (have != 3 || key0 < seen || key0 + 32 > end) {
+                    // slots of no page or that no row of the block sees may hold anything
 #pragma unroll
                     for (int i = 0; i < kWide; ++i) {
                         const int key = lane / kWide + i * kStep;
-                        if (!(have >> key / 16 & 1) || key0 + key >= s.len)
+                        if (!(have >> key / 16 & 1) || key0 + key < seen || key0 + key >= end)
                             x[i] = make_uint4(0, 0, 0, 0);
                     }
                 }

@@ -1048,3 +1048,29 @@ def test_attended_bad_page_is_flagged(dev):
     assert T.check_status() == (0, 0)
     attend(m, [1], [110], broken, 4, True, window=3, bad=(-1, 9))
     assert T.check_status() == (0, 0)
+
+
+CHUNK_WINDOWS = [  # page, heads, kv heads, d, rows, length, window
+    (16, 32, 8, 128, 300, 700, 40), (64, 32, 8, 64, 400, 1000, 100),
+    (128, 32, 4, 96, 300, 900, 7), (32, 64, 1, 112, 256, 600, 33)]
+
+
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+@pytest.mark.parametrize("page,heads,hkv,d,rows,length,window", CHUNK_WINDOWS)
+def test_chunk_pages_in_front_of_a_window(dev, fmt, page, heads, hkv, d, rows, length, window):
+    """The same with many rows, whose steps begin up to 127 keys early."""
+    front_of_window(dev, fmt, True, page, heads, hkv, d, rows, length, window)
+
+
+def test_keys_after_a_chunks_rows(dev):
+    import torch
+    m = Model(dev, "e4m3", 32, 16, 80, 24)
+    table = tables(m.rng, [700], 32, 24)
+    fill(m, [700], table)
+    q = rows_of(m.rng, 600, 16, 80, True, dev, spread=False)  # blocks of 256 tokens, from 100
+    args = (i32([0, 600], dev), i32([700], dev), i32(table, dev))
+    want = T.kv8_attention(m.cache, q, *args)
+    spoil(m, table, range(356, 700))
+    got = T.kv8_attention(m.cache, q, *args)
+    assert torch.equal(got[:256], want[:256]) and bool(torch.isnan(got[-1]).any())
+    assert T.check_status() == (0, 0)
