@@ -396,7 +396,9 @@ int tb_b200_qk_norm_rotary(const TbB200Rotary* rotary, void* stream);
 /* A paged KV cache of 8-bit codes.  k and v: [n_pages, n_kv_heads, page,
  * head_dim] codes, 16-byte aligned; k_scale and v_scale: [n_pages,
  * n_kv_heads], the power of two a page's codes of that head are multiplied
- * with.  All device memory of the caller's. */
+ * with (any other scale gives wrong results: values take its exponent alone),
+ * or 0 in a page that nobody wrote, whose codes are 0 then.  All device memory
+ * of the caller's. */
 typedef struct {
     int format; /* TB_B200_KV_* */
     int page;   /* tokens per page: 16, 32, 64 or 128 */

@@ -470,7 +470,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_chunk(const __grid_constant__ A
                 const float2 x = sh.scales[Stages::stage(j)][i];
                 fs[i] = f * x.x;
                 lv[i] = x.y;
-                have |= (uint32_t)(x.x > 0.0f) << i;
+                have |= (uint32_t)!(x.x < 0.0f) << i;
             }
             const bool inside =
                 __all_sync(tbk::kFull, key0 >= see_lo && key0 + kKeys - 1 <= see_hi &&

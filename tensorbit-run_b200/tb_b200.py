@@ -829,7 +829,10 @@ def qk_norm_rotary(q, k, q_weight, k_weight, eps, positions=None, freqs=None,
 class Kv8Cache:
     """A paged 8-bit KV cache over the caller's tensors: codes k and v
     [n_pages, n_kv_heads, page, head_dim], int8 or float8_e4m3fn, and float32
-    k_scale and v_scale [n_pages, n_kv_heads] (TbB200Kv8)."""
+    k_scale and v_scale [n_pages, n_kv_heads] (TbB200Kv8).  A scale is a power
+    of two, as kv8_append writes it, or 0 in a page that nobody wrote, whose
+    codes are 0: values take a scale's exponent alone, so any other one gives
+    wrong results."""
 
     def __init__(self, k, v, k_scale, v_scale):
         torch = _torch()

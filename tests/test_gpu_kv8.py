@@ -1074,3 +1074,22 @@ def test_keys_after_a_chunks_rows(dev):
     got = T.kv8_attention(m.cache, q, *args)
     assert torch.equal(got[:256], want[:256]) and bool(torch.isnan(got[-1]).any())
     assert T.check_status() == (0, 0)
+
+
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+@pytest.mark.parametrize("bf16,counts", [(False, [1, 9]), (True, [1, 9]), (True, [300, 80])])
+def test_pages_that_nobody_wrote(dev, fmt, bf16, counts):
+    """Pages as Kv8Cache.empty leaves them, of scale 0 and codes 0, are keys and values
+    of zero: scores of 0, which count, by few rows and by many."""
+    lengths, heads = [500, 200], 32
+    m = Model(dev, fmt, 32, 8, 128, 24)
+    table = tables(m.rng, lengths, 32, 24)
+    fill(m, lengths, table, spread=False)
+    for page in (table[0, 3], table[0, 4], table[1, 0], table[1, 6]):
+        for t, own in zip((m.cache.k, m.cache.v, m.cache.k_scale, m.cache.v_scale),
+                          (*m.codes, *m.scales)):
+            t[int(page)] = 0
+            own[page] = 0.0
+    attend(m, counts, lengths, table, heads, bf16, by_head=True)
+    attend(m, counts, lengths, table, heads, bf16, by_head=True, window=64)
+    assert T.check_status() == (0, 0)
