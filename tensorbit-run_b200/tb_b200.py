@@ -707,16 +707,23 @@ def _here():
 
 
 def _stream(torch, dev, stream):
-    return torch._C._cuda_getCurrentRawStream(dev) if stream is None else stream
+    """The stream that a call given `stream` runs on, as an integer: torch's current one
+    without, and where that is the default stream the one that the library takes for it
+    (tb_b200_set_stream)."""
+    if dev is None:
+        return 0  # no device: the tensors are refused
+    stream = torch._C._cuda_getCurrentRawStream(dev) if stream is None else \
+        getattr(stream, "value", stream)
+    return stream or lib().tb_b200_get_stream() or 0
 
 
-def _new(stream, make, *args, **kw):
-    """make(...), an uninitialised tensor for a call on `stream`: from that stream's pool, so
-    that the memory's earlier uses are ordered before the call and its later ones after it."""
-    if stream is None:
+def _new(torch, dev, stream, make, *args, **kw):
+    """make(...), an uninitialised tensor for a call on `stream` (of _stream): from that
+    stream's pool, so that the memory's earlier uses are ordered before the call and its
+    later ones after it."""
+    if dev is None or stream == torch._C._cuda_getCurrentRawStream(dev):
         return make(*args, **kw)
-    cuda = _torch().cuda
-    with cuda.stream(cuda.ExternalStream(getattr(stream, "value", stream) or 0)):
+    with torch.cuda.stream(torch.cuda.ExternalStream(stream)):
         return make(*args, **kw)
 
 
@@ -762,19 +769,20 @@ def rotary_freqs(rotary_dim, theta, scaling="none", factor=1.0, trained=0.0, low
     device), stretched by `scaling`: "none", "linear", "ntk", "bands" or
     "yarn" (tb_b200_rotary_freqs)."""
     torch, dev = _here()
+    stream = _stream(torch, dev, stream)
     n = rotary_dim // 2
     if out is None:
-        out = _new(stream, torch.empty, n, dtype=torch.float64, device="cuda")
+        out = _new(torch, dev, stream, torch.empty, n, dtype=torch.float64, device="cuda")
     at = _flat(out, torch.float64, n, dev, "out")
     sc = RotaryScaling(ROTARY_SCALING[scaling], theta, factor, trained, low, high)
-    check(lib().tb_b200_rotary_freqs(rotary_dim, sc, at, _stream(torch, dev, stream)),
-          "rotary_freqs")
+    check(lib().tb_b200_rotary_freqs(rotary_dim, sc, at, stream), "rotary_freqs")
     return out
 
 
 def _rotary(fn, q, k, q_weight, k_weight, eps, positions, freqs, layout, scale, q_out, k_out,
             stream):
     torch, dev = _here()
+    stream = _stream(torch, dev, stream)
     dtype, code = q.dtype, _heads_dtype(q)
     q_shape, k_shape = q.shape, k.shape
     rows, hq, d = q_shape
@@ -785,11 +793,11 @@ def _rotary(fn, q, k, q_weight, k_weight, eps, positions, freqs, layout, scale, 
     ks = _heads(k, dtype, k_shape, dev, "k")
     dense = torch.contiguous_format
     if q_out is None:
-        q_out, qos = _new(stream, torch.empty_like, q, memory_format=dense), hq * d
+        q_out, qos = _new(torch, dev, stream, torch.empty_like, q, memory_format=dense), hq * d
     else:
         qos = _heads(q_out, dtype, q_shape, dev, "q_out")
     if k_out is None:
-        k_out, kos = _new(stream, torch.empty_like, k, memory_format=dense), hkv * d
+        k_out, kos = _new(torch, dev, stream, torch.empty_like, k, memory_format=dense), hkv * d
     else:
         kos = _heads(k_out, dtype, k_shape, dev, "k_out")
     r, at, fr = 0, None, None
@@ -803,7 +811,7 @@ def _rotary(fn, q, k, q_weight, k_weight, eps, positions, freqs, layout, scale, 
     kw = None if k_weight is None else _flat(k_weight, dtype, d, dev, "k_weight")
     t = Rotary(code, rows, hq, hkv, d, r, layout, q.data_ptr(), qs, k.data_ptr(), ks,
                q_out.data_ptr(), qos, k_out.data_ptr(), kos, at, fr, scale, qw, kw, eps)
-    check(fn(t, _stream(torch, dev, stream)), "rotary")
+    check(fn(t, stream), "rotary")
     return q_out, k_out
 
 
@@ -901,6 +909,7 @@ def kv8_attention(cache, q, row_start, lengths, page_table, max_q=None, max_len=
     1 / sqrt(head_dim) unless given; window > 0 attends that many last keys.
     Returns out, or (out, lse) with return_lse or lse."""
     torch, dev = _here()
+    stream = _stream(torch, dev, stream)
     dtype, code, shape = q.dtype, _heads_dtype(q), q.shape
     rows, heads, d = shape
     if d != cache.c.head_dim:
@@ -908,7 +917,7 @@ def kv8_attention(cache, q, row_start, lengths, page_table, max_q=None, max_len=
     qs = _heads(q, dtype, shape, dev, "q")
     dense = torch.contiguous_format
     if out is None:
-        out, os_ = _new(stream, torch.empty_like, q, memory_format=dense), heads * d
+        out, os_ = _new(torch, dev, stream, torch.empty_like, q, memory_format=dense), heads * d
     else:
         os_ = _heads(out, dtype, shape, dev, "out")
     ls = None
@@ -917,7 +926,7 @@ def kv8_attention(cache, q, row_start, lengths, page_table, max_q=None, max_len=
             raise ValueError("lse must be [rows, n_heads]")
         ls = _flat(lse, torch.float32, rows * heads, dev, "lse")
     elif return_lse:
-        lse = _new(stream, q.new_empty, (rows, heads), dtype=torch.float32)
+        lse = _new(torch, dev, stream, q.new_empty, (rows, heads), dtype=torch.float32)
         ls = lse.data_ptr()
     b = _kv8_batch(torch, cache, dev, rows, row_start, lengths, page_table)
     a = Kv8Attention(code, heads, q.data_ptr(), qs, out.data_ptr(), os_, ls,
@@ -929,7 +938,7 @@ def kv8_attention(cache, q, row_start, lengths, page_table, max_q=None, max_len=
     if workspace is None:
         check(L.tb_b200_kv8_attention_workspace(cache.c, b, a, need), "kv8_attention_workspace")
         if need.value:
-            workspace = _new(stream, q.new_empty, need.value, dtype=torch.uint8)
+            workspace = _new(torch, dev, stream, q.new_empty, need.value, dtype=torch.uint8)
     else:
         _device_is(workspace, dev)
         if not workspace.is_contiguous():
@@ -937,7 +946,7 @@ def kv8_attention(cache, q, row_start, lengths, page_table, max_q=None, max_len=
     if workspace is not None:
         a.workspace = workspace.data_ptr()
         a.workspace_bytes = workspace.numel() * workspace.element_size()
-    check(L.tb_b200_kv8_attention(cache.c, b, a, _stream(torch, dev, stream)), "kv8_attention")
+    check(L.tb_b200_kv8_attention(cache.c, b, a, stream), "kv8_attention")
     return out if lse is None else (out, lse)
 
 

@@ -1093,3 +1093,56 @@ def test_pages_that_nobody_wrote(dev, fmt, bf16, counts):
     attend(m, counts, lengths, table, heads, bf16, by_head=True)
     attend(m, counts, lengths, table, heads, bf16, by_head=True, window=64)
     assert T.check_status() == (0, 0)
+
+
+def test_scratch_of_the_threads_stream(dev):
+    """Calls on the stream that tb_b200_set_stream chose take their scratch and outputs
+    from that stream's pool, where freed memory waits for the call."""
+    import torch
+    m = Model(dev, "int8", 64, 2, 64, 100)
+    table = tables(m.rng, [6000], 64, 100)
+    fill(m, [6000], table)
+    q = rows_of(m.rng, 1, 8, 64, True, dev)
+    args = (i32([0, 1], dev), i32([6000], dev), i32(table, dev))
+    want = T.kv8_attention(m.cache, q, *args)
+    fr = T.rotary_freqs(64, 1e4)
+    pos = i32([7], dev)
+
+    def taken(call, **kw):
+        """The streams of the memory that a call takes, on a new stream s, and s."""
+        torch.cuda.synchronize()
+        torch.cuda.empty_cache()
+        s = torch.cuda.Stream()
+        before = {x["address"] for x in torch.cuda.memory_snapshot()}
+        T.lib().tb_b200_set_stream(s.cuda_stream)
+        try:
+            got = call(**kw)
+        finally:
+            T.lib().tb_b200_set_stream(None)
+        torch.cuda.synchronize()
+        mine = [x["stream"] for x in torch.cuda.memory_snapshot() if x["stream"] == s.cuda_stream]
+        other = [x for x in torch.cuda.memory_snapshot()
+                 if x["stream"] != s.cuda_stream and x["address"] not in before]
+        assert mine and not other
+        return got
+
+    out = torch.empty_like(want)
+    for kw in ({}, dict(stream=0)):
+        taken(lambda **k: T.kv8_attention(m.cache, q, *args, out=out, **k), **kw)
+        assert torch.equal(out, want)
+        out.zero_()
+        got = taken(lambda **k: T.kv8_attention(m.cache, q, *args, return_lse=True, **k), **kw)
+        assert torch.equal(got[0], want)
+        taken(lambda **k: T.rotary(q, q, pos, fr, **k), **kw)
+        taken(lambda **k: T.rotary_freqs(64, 1e4, **k), **kw)
+    # a call's own stream comes before the thread's
+    s, own = torch.cuda.Stream(), torch.cuda.Stream()
+    T.lib().tb_b200_set_stream(s.cuda_stream)
+    try:
+        got = [T.kv8_attention(m.cache, q, *args, stream=own.cuda_stream)]
+        with torch.cuda.stream(own):
+            got.append(T.kv8_attention(m.cache, q, *args))
+    finally:
+        T.lib().tb_b200_set_stream(None)
+    torch.cuda.synchronize()
+    assert all(torch.equal(g, want) for g in got)
