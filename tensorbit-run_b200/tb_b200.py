@@ -707,23 +707,24 @@ def _here():
 
 
 def _stream(torch, dev, stream):
-    """The stream that a call given `stream` runs on, as an integer: torch's current one
+    """(The stream that a call given `stream` runs on, as an integer: torch's current one
     without, and where that is the default stream the one that the library takes for it
-    (tb_b200_set_stream)."""
+    (tb_b200_set_stream); it as torch's, None where it is the current one.)"""
     if dev is None:
-        return 0  # no device: the tensors are refused
-    stream = torch._C._cuda_getCurrentRawStream(dev) if stream is None else \
-        getattr(stream, "value", stream)
-    return stream or lib().tb_b200_get_stream() or 0
+        return 0, None  # no device: the tensors are refused
+    here = torch._C._cuda_getCurrentRawStream(dev)
+    there = here if stream is None else getattr(stream, "value", stream)
+    there = there or lib().tb_b200_get_stream() or 0
+    return there, None if there == here else torch.cuda.ExternalStream(there)
 
 
-def _new(torch, dev, stream, make, *args, **kw):
-    """make(...), an uninitialised tensor for a call on `stream` (of _stream): from that
-    stream's pool, so that the memory's earlier uses are ordered before the call and its
-    later ones after it."""
-    if dev is None or stream == torch._C._cuda_getCurrentRawStream(dev):
+def _new(other, make, *args, **kw):
+    """make(...), an uninitialised tensor for a call on stream `other` (of _stream): from
+    that stream's pool, so that the memory's earlier uses are ordered before the call and
+    its later ones after it."""
+    if other is None:
         return make(*args, **kw)
-    with torch.cuda.stream(torch.cuda.ExternalStream(stream)):
+    with _torch().cuda.stream(other):
         return make(*args, **kw)
 
 
@@ -769,10 +770,10 @@ def rotary_freqs(rotary_dim, theta, scaling="none", factor=1.0, trained=0.0, low
     device), stretched by `scaling`: "none", "linear", "ntk", "bands" or
     "yarn" (tb_b200_rotary_freqs)."""
     torch, dev = _here()
-    stream = _stream(torch, dev, stream)
+    stream, other = _stream(torch, dev, stream)
     n = rotary_dim // 2
     if out is None:
-        out = _new(torch, dev, stream, torch.empty, n, dtype=torch.float64, device="cuda")
+        out = _new(other, torch.empty, n, dtype=torch.float64, device="cuda")
     at = _flat(out, torch.float64, n, dev, "out")
     sc = RotaryScaling(ROTARY_SCALING[scaling], theta, factor, trained, low, high)
     check(lib().tb_b200_rotary_freqs(rotary_dim, sc, at, stream), "rotary_freqs")
@@ -782,7 +783,7 @@ def rotary_freqs(rotary_dim, theta, scaling="none", factor=1.0, trained=0.0, low
 def _rotary(fn, q, k, q_weight, k_weight, eps, positions, freqs, layout, scale, q_out, k_out,
             stream):
     torch, dev = _here()
-    stream = _stream(torch, dev, stream)
+    stream, other = _stream(torch, dev, stream)
     dtype, code = q.dtype, _heads_dtype(q)
     q_shape, k_shape = q.shape, k.shape
     rows, hq, d = q_shape
@@ -793,11 +794,11 @@ def _rotary(fn, q, k, q_weight, k_weight, eps, positions, freqs, layout, scale, 
     ks = _heads(k, dtype, k_shape, dev, "k")
     dense = torch.contiguous_format
     if q_out is None:
-        q_out, qos = _new(torch, dev, stream, torch.empty_like, q, memory_format=dense), hq * d
+        q_out, qos = _new(other, torch.empty_like, q, memory_format=dense), hq * d
     else:
         qos = _heads(q_out, dtype, q_shape, dev, "q_out")
     if k_out is None:
-        k_out, kos = _new(torch, dev, stream, torch.empty_like, k, memory_format=dense), hkv * d
+        k_out, kos = _new(other, torch.empty_like, k, memory_format=dense), hkv * d
     else:
         kos = _heads(k_out, dtype, k_shape, dev, "k_out")
     r, at, fr = 0, None, None
@@ -898,7 +899,7 @@ def kv8_append(cache, k, v, row_start, lengths, page_table, stream=None):
     ks, vs = _heads(k, dtype, shape, dev, "k"), _heads(v, dtype, shape, dev, "v")
     b = _kv8_batch(torch, cache, dev, shape[0], row_start, lengths, page_table)
     check(lib().tb_b200_kv8_append(cache.c, b, code, k.data_ptr(), ks, v.data_ptr(), vs,
-                                   _stream(torch, dev, stream)), "kv8_append")
+                                   _stream(torch, dev, stream)[0]), "kv8_append")
 
 
 def kv8_attention(cache, q, row_start, lengths, page_table, max_q=None, max_len=None, scale=None,
@@ -909,7 +910,7 @@ def kv8_attention(cache, q, row_start, lengths, page_table, max_q=None, max_len=
     1 / sqrt(head_dim) unless given; window > 0 attends that many last keys.
     Returns out, or (out, lse) with return_lse or lse."""
     torch, dev = _here()
-    stream = _stream(torch, dev, stream)
+    stream, other = _stream(torch, dev, stream)
     dtype, code, shape = q.dtype, _heads_dtype(q), q.shape
     rows, heads, d = shape
     if d != cache.c.head_dim:
@@ -917,7 +918,7 @@ def kv8_attention(cache, q, row_start, lengths, page_table, max_q=None, max_len=
     qs = _heads(q, dtype, shape, dev, "q")
     dense = torch.contiguous_format
     if out is None:
-        out, os_ = _new(torch, dev, stream, torch.empty_like, q, memory_format=dense), heads * d
+        out, os_ = _new(other, torch.empty_like, q, memory_format=dense), heads * d
     else:
         os_ = _heads(out, dtype, shape, dev, "out")
     ls = None
@@ -926,7 +927,7 @@ def kv8_attention(cache, q, row_start, lengths, page_table, max_q=None, max_len=
             raise ValueError("lse must be [rows, n_heads]")
         ls = _flat(lse, torch.float32, rows * heads, dev, "lse")
     elif return_lse:
-        lse = _new(torch, dev, stream, q.new_empty, (rows, heads), dtype=torch.float32)
+        lse = _new(other, q.new_empty, (rows, heads), dtype=torch.float32)
         ls = lse.data_ptr()
     b = _kv8_batch(torch, cache, dev, rows, row_start, lengths, page_table)
     a = Kv8Attention(code, heads, q.data_ptr(), qs, out.data_ptr(), os_, ls,
@@ -938,7 +939,7 @@ def kv8_attention(cache, q, row_start, lengths, page_table, max_q=None, max_len=
     if workspace is None:
         check(L.tb_b200_kv8_attention_workspace(cache.c, b, a, need), "kv8_attention_workspace")
         if need.value:
-            workspace = _new(torch, dev, stream, q.new_empty, need.value, dtype=torch.uint8)
+            workspace = _new(other, q.new_empty, need.value, dtype=torch.uint8)
     else:
         _device_is(workspace, dev)
         if not workspace.is_contiguous():
