@@ -728,6 +728,12 @@ def _new(other, make, *args, **kw):
         return make(*args, **kw)
 
 
+def _c_int(n):
+    """n as the C int that says the same to the library, which refuses what is below 0 and
+    has bounds of its own; ctypes would take the low 32 bits."""
+    return max(-1, min(n, 0x7fffffff))
+
+
 def _device_is(t, dev):
     if t.get_device() != dev:
         raise ValueError(f"expected a tensor on the current device cuda:{dev}, got {t.device}")
@@ -776,7 +782,7 @@ def rotary_freqs(rotary_dim, theta, scaling="none", factor=1.0, trained=0.0, low
         out = _new(other, torch.empty, n, dtype=torch.float64, device="cuda")
     at = _flat(out, torch.float64, n, dev, "out")
     sc = RotaryScaling(ROTARY_SCALING[scaling], theta, factor, trained, low, high)
-    check(lib().tb_b200_rotary_freqs(rotary_dim, sc, at, stream), "rotary_freqs")
+    check(lib().tb_b200_rotary_freqs(_c_int(rotary_dim), sc, at, stream), "rotary_freqs")
     return out
 
 
@@ -810,7 +816,7 @@ def _rotary(fn, q, k, q_weight, k_weight, eps, positions, freqs, layout, scale, 
         fr = _flat(freqs, torch.float64, r // 2, dev, "freqs")
     qw = None if q_weight is None else _flat(q_weight, dtype, d, dev, "q_weight")
     kw = None if k_weight is None else _flat(k_weight, dtype, d, dev, "k_weight")
-    t = Rotary(code, rows, hq, hkv, d, r, layout, q.data_ptr(), qs, k.data_ptr(), ks,
+    t = Rotary(code, rows, hq, hkv, d, r, _c_int(layout), q.data_ptr(), qs, k.data_ptr(), ks,
                q_out.data_ptr(), qos, k_out.data_ptr(), kos, at, fr, scale, qw, kw, eps)
     check(fn(t, stream), "rotary")
     return q_out, k_out
@@ -931,10 +937,10 @@ def kv8_attention(cache, q, row_start, lengths, page_table, max_q=None, max_len=
         ls = lse.data_ptr()
     b = _kv8_batch(torch, cache, dev, rows, row_start, lengths, page_table)
     a = Kv8Attention(code, heads, q.data_ptr(), qs, out.data_ptr(), os_, ls,
-                     d ** -0.5 if scale is None else scale, min(window, 0x7fffffff),
-                     rows if max_q is None else max_q,
-                     min(b.table_width * cache.c.page, 1 << 30) if max_len is None else max_len,
-                     None, 0)
+                     d ** -0.5 if scale is None else scale, _c_int(window),
+                     _c_int(rows if max_q is None else max_q),
+                     min(b.table_width * cache.c.page, 1 << 30) if max_len is None
+                     else _c_int(max_len), None, 0)
     L, need = lib(), C.c_size_t()
     if workspace is None:
         check(L.tb_b200_kv8_attention_workspace(cache.c, b, a, need), "kv8_attention_workspace")

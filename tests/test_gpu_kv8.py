@@ -1146,3 +1146,28 @@ def test_scratch_of_the_threads_stream(dev):
         T.lib().tb_b200_set_stream(None)
     torch.cuda.synchronize()
     assert all(torch.equal(g, want) for g in got)
+
+
+def test_counts_past_an_int(dev):
+    """Bounds that a C int does not hold are what they say, not their low 32 bits."""
+    import torch
+    m = Model(dev, "int8", 16, 2, 64, 8)
+    table = tables(m.rng, [100], 16, 8)
+    fill(m, [100], table)
+    q = rows_of(m.rng, 3, 4, 64, True, dev)
+    args = (i32([0, 3], dev), i32([100], dev), i32(table, dev))
+    want = T.kv8_attention(m.cache, q, *args)
+    for n in (2 ** 31 - 1, 2 ** 31, 2 ** 32, 2 ** 32 + 1, 2 ** 63):
+        assert torch.equal(T.kv8_attention(m.cache, q, *args, max_q=n), want)
+        assert torch.equal(T.kv8_attention(m.cache, q, *args, window=n), want)
+        with pytest.raises(T.TbError):  # more than 2^30
+            T.kv8_attention(m.cache, q, *args, max_len=n)
+    for bad in (-1, -2 ** 31, -2 ** 32, -2 ** 32 + 50, -2 ** 64 + 100):
+        for name in ("max_q", "max_len", "window"):
+            with pytest.raises(T.TbError):
+                T.kv8_attention(m.cache, q, *args, **{name: bad})
+        with pytest.raises(T.TbError):
+            T.rotary(q, q, i32([0, 1, 2], dev), T.rotary_freqs(64, 1e4), layout=bad)
+    with pytest.raises(T.TbError):
+        T.rotary(q, q, i32([0, 1, 2], dev), T.rotary_freqs(64, 1e4), layout=2 ** 32)
+    assert T.check_status() == (0, 0)
