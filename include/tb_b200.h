@@ -362,7 +362,7 @@ typedef struct {
     int dtype; /* of q, k, the outputs and the weights */
     int64_t rows;
     int n_q_heads;
-    int n_kv_heads;
+    int n_kv_heads; /* both together less than 2^30 */
     int head_dim; /* 1 .. 512 */
     int rotary_dim;
     int layout; /* TB_B200_ROTARY_INTERLEAVED / _HALF */

@@ -316,8 +316,8 @@ void launch(Args& a, int dtype, bool half_layout, unsigned rows, cudaStream_t s)
 int run(const TbB200Rotary* t, bool norm, void* stream) {
     if (!t) return TB_ERR_INVALID_ARG;
     if (t->rows < 0 || t->rows > INT32_MAX || t->n_q_heads < 0 || t->n_kv_heads < 0 ||
-        t->n_q_heads > INT32_MAX / 2 || t->n_kv_heads > INT32_MAX / 2 || t->head_dim < 1 ||
-        t->head_dim > kMaxDim || t->rotary_dim < 0 || t->rotary_dim > t->head_dim ||
+        (int64_t)t->n_q_heads + t->n_kv_heads > INT32_MAX / 2 ||  // heads of passes past it too
+        t->head_dim < 1 || t->head_dim > kMaxDim || t->rotary_dim < 0 || t->rotary_dim > t->head_dim ||
         t->rotary_dim % 2)
         return TB_ERR_INVALID_SHAPE;
     if (t->dtype != TB_DTYPE_F32 && t->dtype != TB_DTYPE_BF16) return TB_ERR_UNSUPPORTED_DTYPE;

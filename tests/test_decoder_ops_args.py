@@ -140,3 +140,12 @@ def test_python_refuses_host_tensors():
         T.Kv8Cache(torch.zeros(1, 1, 16, 64, dtype=torch.int8),
                    torch.zeros(1, 1, 16, 64, dtype=torch.int8), torch.zeros(1, 1),
                    torch.zeros(1, 1))
+
+
+@pytest.mark.parametrize("hq,hkv", [(2 ** 30 - 1, 2 ** 30 - 1), (2 ** 30 - 1, 1), (1, 2 ** 30 - 1),
+                                    (2 ** 31 - 1, 0), (2 ** 30, 0)])
+def test_rotary_heads_that_an_index_does_not_hold(hq, hkv):
+    """The kernel counts a row's heads, Q's and K's, in an int, a pass beyond the last."""
+    t = rotary(n_q_heads=hq, n_kv_heads=hkv, head_dim=1, rotary_dim=0, rows=1)
+    assert T.lib().tb_b200_rotary(C.byref(t), None) == SHAPE
+    assert T.lib().tb_b200_qk_norm_rotary(C.byref(t), None) == SHAPE
