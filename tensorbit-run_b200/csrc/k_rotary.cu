@@ -45,8 +45,12 @@ constexpr int kThreads = 256;
 // Most threads of a CTA.  The rotation of many rows alone streams best in small ones
 // (16384 rows of 72 heads of 128: 94 us with 128, 101 with 256; 8192 of 9 of 256: 18
 // and 24); 64 rows of 72 heads take 3.6 us with 128 and 3.2 with 256, 256 rows with
-// the norm 6.4 and 5.7, 4095 of f32 46.8 and 46.1.
-unsigned threads_of(bool norm, unsigned rows) { return norm || rows <= 4 * 148 ? 256 : 128; }
+// the norm 6.4 and 5.7, 4095 of f32 46.8 and 46.1.  Few rows are up to four for every
+// SM, which those of 256 threads hold at once; between 64 rows and 8192 neither side of
+// the rotation alone was measured.
+unsigned threads_of(bool norm, unsigned rows, int sm_count) {
+    return norm || rows <= 4u * sm_count ? 256 : 128;
+}
 
 // ---------------------------------------------------------------- vectors
 template <typename T, int VEC>
@@ -251,10 +255,11 @@ __global__ void __launch_bounds__(kThreads, NU == 1 ? 4 : 1) k_rotary(const __gr
 }
 
 template <typename T, int VEC, int NU, bool NORM>
-void launch_layout(const Args& a, bool half_layout, unsigned rows, cudaStream_t s) {
+void launch_layout(const Args& a, bool half_layout, unsigned rows, int sm_count,
+                   cudaStream_t s) {
     // the fewest passes over the heads, and the fewest threads for as many
     const int64_t lanes = (int64_t)(a.hq + a.hkv) * a.group;
-    const unsigned most = threads_of(NORM, rows);
+    const unsigned most = threads_of(NORM, rows, sm_count);
     const int64_t passes = (lanes + most - 1) / most;
     const unsigned threads = (unsigned)((lanes + passes * 32 - 1) / (passes * 32) * 32);
     if (half_layout)
@@ -286,30 +291,30 @@ int group_of(int d, int vec) {
 }
 
 template <bool NORM>
-void launch(Args& a, int dtype, bool half_layout, unsigned rows, cudaStream_t s) {
+void launch(Args& a, int dtype, bool half_layout, unsigned rows, int sm_count, cudaStream_t s) {
     if (dtype == TB_DTYPE_BF16) {
         if (vectors_of(8, 2, a, half_layout)) {
             a.group = group_of(a.d, 8);
-            launch_layout<__nv_bfloat16, 8, 1, NORM>(a, half_layout, rows, s);
+            launch_layout<__nv_bfloat16, 8, 1, NORM>(a, half_layout, rows, sm_count, s);
         } else if (vectors_of(4, 2, a, half_layout)) {
             a.group = group_of(a.d, 4);
             if (a.d <= 256)
-                launch_layout<__nv_bfloat16, 4, 1, NORM>(a, half_layout, rows, s);
+                launch_layout<__nv_bfloat16, 4, 1, NORM>(a, half_layout, rows, sm_count, s);
             else
-                launch_layout<__nv_bfloat16, 4, 2, NORM>(a, half_layout, rows, s);
+                launch_layout<__nv_bfloat16, 4, 2, NORM>(a, half_layout, rows, sm_count, s);
         } else {
             a.group = 32;
-            launch_layout<__nv_bfloat16, 1, 8, NORM>(a, half_layout, rows, s);
+            launch_layout<__nv_bfloat16, 1, 8, NORM>(a, half_layout, rows, sm_count, s);
         }
     } else if (vectors_of(4, 4, a, half_layout)) {
         a.group = group_of(a.d, 4);
         if (a.d <= 256)
-            launch_layout<float, 4, 1, NORM>(a, half_layout, rows, s);
+            launch_layout<float, 4, 1, NORM>(a, half_layout, rows, sm_count, s);
         else
-            launch_layout<float, 4, 2, NORM>(a, half_layout, rows, s);
+            launch_layout<float, 4, 2, NORM>(a, half_layout, rows, sm_count, s);
     } else {
         a.group = 32;
-        launch_layout<float, 1, 8, NORM>(a, half_layout, rows, s);
+        launch_layout<float, 1, 8, NORM>(a, half_layout, rows, sm_count, s);
     }
 }
 
@@ -339,12 +344,14 @@ int run(const TbB200Rotary* t, bool norm, void* stream) {
               norm ? t->q_weight : nullptr, norm ? t->k_weight : nullptr, t->scale, t->eps,
               1.0f / (float)t->head_dim,
               t->n_q_heads, t->n_kv_heads, t->head_dim, t->rotary_dim, 0};
+    const tbh::DeviceState* ds = tbh::current_device_state();
+    if (!ds) return TB_ERR_DEVICE;
     cudaStream_t s = tbh::stream_of(stream);
     const bool half_layout = t->layout == TB_B200_ROTARY_HALF;
     if (norm)
-        launch<true>(a, t->dtype, half_layout, (unsigned)t->rows, s);
+        launch<true>(a, t->dtype, half_layout, (unsigned)t->rows, ds->sm_count, s);
     else
-        launch<false>(a, t->dtype, half_layout, (unsigned)t->rows, s);
+        launch<false>(a, t->dtype, half_layout, (unsigned)t->rows, ds->sm_count, s);
     TB_LAUNCH_CHECK("rotary kernel");
     return TB_OK;
 }
