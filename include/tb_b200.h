@@ -384,7 +384,7 @@ typedef struct {
 
 int tb_b200_rotary(const TbB200Rotary* rotary, void* stream);
 /* Each head x normalised first, x / sqrt(mean(x^2) + eps) * weight, with the
- * f32 result rotated.  (tb_b200_rms_norm adds eps to the sum instead, as the
+ * f32 result (the root's inverse by rsqrtf, 2 ulp) rotated.  (tb_b200_rms_norm adds eps to the sum instead, as the
  * engine does.)  rotary_dim 0: the norm alone, positions and freqs unused. */
 int tb_b200_qk_norm_rotary(const TbB200Rotary* rotary, void* stream);
 
@@ -463,7 +463,13 @@ int tb_b200_kv8_append(const TbB200Kv8* cache, const TbB200Kv8Batch* batch, int 
  * anything, and a page of only such slots (in front of every window, say) needs
  * no number: neither reaches a result or raises a flag.  Slots that some row
  * attends hold numbers, as tb_b200_kv8_append leaves them; an e4m3 NaN code
- * there may reach other rows of its sequence too. */
+ * there may reach other rows of its sequence too.
+ * Sums, maxima and the softmax's sums are f32 (products with int8 codes exact),
+ * exponentials ex2.approx's (2^-22).  bf16 calls hold q as f16 scaled by a power
+ * of two or in 22 bits, and the weights as f16 (2^-12 of each, an eighth of the
+ * output's half step, so a last place differs from f32 arithmetic's now and
+ * then); f32 calls q in 22 bits of its row's largest element or of each, and
+ * the weights as two f16.  A row of q with a NaN or an infinity gives NaN. */
 typedef struct {
     int dtype; /* of q and out: TB_DTYPE_F32 or TB_DTYPE_BF16 */
     int n_heads; /* a multiple of the cache's n_kv_heads */

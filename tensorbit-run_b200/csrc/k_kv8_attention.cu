@@ -30,16 +30,17 @@
 // are f32.  The values' scale joins the exponent, p v_scale = 2^(s + log2 v_scale
 // - r'), with a reference r' of its own per row, so pages of any scales keep
 // their weight.  References are whole numbers and move only when a score passes
-// them by 2^4: rescaling is exact and rare.  A weight more than 2^-25 below the
-// row's largest is an f16 subnormal, off by at most 2^-36 of the largest.
+// them by 2^4: rescaling is rare, by ex2.approx (2^-22) of a whole number.  A weight
+// more than 2^-25 below the row's largest is an f16 subnormal, off by at most 2^-36 of
+// the largest.
 //
 // What bounds it and what it measured (8 k/v heads): the codes' bytes where there
 // are many keys a row, 64 sequences of 1 .. 8191 keys, 64 heads of 128, int8, 95 us,
-// 5.7 TB/s (a copy: 6.5), one of 131071, e4m3, 55 us, 4.9 TB/s, of it 14 us above the
+// 5.7 TB/s (a copy: 6.5), one of 131071, e4m3, 56 us, 4.8 TB/s, of it 15 us above the
 // bytes' time: launch, shares, table -> scale -> codes -> products, join.
 // With 16 rows a block and heads of 64 (48 sequences, 1 .. 8 tokens, 32 heads, a
 // window of 1000) the warps' instructions, about 550 for 32 keys and 1800 a block,
-// issued at half rate by the 12 warps that registers allow: 33 us.
+// issued at half rate by the 12 warps that registers allow: 34 us.
 #include "kv8_mma.cuh"
 #include "phases.cuh"
 

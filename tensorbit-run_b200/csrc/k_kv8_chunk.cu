@@ -18,13 +18,15 @@
 // once for 256 rows, four times fewer than a block of 16 rows' matrix
 // instructions could share, and the products run at 4 times their rate.
 //
-// Measured: 2048 tokens behind 6144, 32 heads of 128 on 8, int8, 298 us, 807 TFLOP/s
+// Measured: 2048 tokens behind 6144, 32 heads of 128 on 8, int8, 296 us, 812 TFLOP/s
 // (0.49 of a library product's rate; blocks of 16 rows: 1634 us).  A step takes 2.35
 // us, 4500 clocks: a tile's scores, softmax (2600) and products follow one another,
 // and the products share shared memory's bandwidth with the conversion (3300 clocks
-// where 2050 are the least).  256 CTAs of 62 steps run on 148 SMs as two waves, 0.86
-// full; a CTA pays some 9 us beside its steps, so 64 sequences of 100 tokens and
-// 1000 keys take 222 us (253 with a thread a row of q and out).
+// where 2050 are the least).  256 CTAs of 49 to 64 steps, the longest first, give the
+// busiest of 148 SMs 111 steps where 98 would be even shares: 0.88 full.  A CTA pays
+// some 9 us beside its steps, so 64 sequences of 100 tokens and 1000 keys take 222 us
+// (253 with a thread a row of q and out).  Keys are not cut: 100 rows of 64 heads on 8
+// over 131071 keys are 32 CTAs of 1024 steps, 2.3 ms.
 //
 // Precision as in k_kv8_attention.cu: a row of q is scaled by a power of two to
 // [2^14, 2^15) and held as f16, exact for bf16 elements above 2^-31 of the row's
@@ -620,8 +622,12 @@ namespace kv8 {
 
 // A wave of this kernel's CTAs takes a step of 128 keys in about 2.35 us (1.95 with
 // heads of 64) however few of their rows are there, k_attend the same keys in 6.6 ns
-// (3.9) for each block of 16 rows, so one wave is worth 2.4 (3.4) blocks for every
-// SM.  Both sides, this kernel's first, 32 heads of 128 on 8, int8, 2048 keys: one
+// (3.9) for each block of 16 rows, so one wave is worth 356 (500) blocks, 2.4 (3.4, of
+// which the rule takes 3.3) for each of 148 SMs.  The rule is for a whole call, by its
+// bounds, and both sides were measured on equal sequences: a prompt beside single
+// tokens takes this kernel for all of them (2048 rows beside 63 single tokens of up to
+// 8191 keys, 64 heads on 8: 361 us, where a call for each kind takes 120 and 91).
+// Both sides, this kernel's first, 32 heads of 128 on 8, int8, 2048 keys: one
 // sequence of 160 rows 55 and 56 us, 256 55 and 78, 512 55 and 135; 16 of 8 rows 45
 // and 44, 16 of 16 46 and 76; 64 of 8 167 and 136, 64 of 12 169 and 197.  Heads of
 // 64, e4m3: one of 160 46 and 42, 256 44 and 54; 64 of 12 142 and 114, 16 141 and 146.

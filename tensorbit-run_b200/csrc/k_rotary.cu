@@ -28,7 +28,7 @@
 // 6.5; the first version, a head at a time: 127 us); norm and half the head, 4095
 // rows of 32 + 32 heads of 128, f32, 46.1 us, 5.8 TB/s (49.6 with a division and a
 // root rounded to nearest in rsqrtf's place); 777 rows of 32 + 32 heads of 80, f32,
-// 8.4 us and 256 rows of 32 + 32 heads of 128, bf16, 5.2 us, where a launch and one
+// 8.4 us and 256 rows of 32 + 32 heads of 128, bf16, 5.5 us, where a launch and one
 // row's chain of loads are most of the time.
 #include <math.h>
 
