@@ -384,8 +384,8 @@ typedef struct {
 
 int tb_b200_rotary(const TbB200Rotary* rotary, void* stream);
 /* Each head x normalised first, x / sqrt(mean(x^2) + eps) * weight, with the
- * f32 result (the root's inverse by rsqrtf, 2 ulp) rotated.  (tb_b200_rms_norm adds eps to the sum instead, as the
- * engine does.)  rotary_dim 0: the norm alone, positions and freqs unused. */
+ * f32 result (the root's inverse by rsqrtf, 2 ulp) rotated.  (tb_b200_rms_norm
+ * adds eps to the sum instead, as the engine does.)  rotary_dim 0: the norm alone, positions and freqs unused. */
 int tb_b200_qk_norm_rotary(const TbB200Rotary* rotary, void* stream);
 
 /* Code formats of the 8-bit KV cache: two's complement in [-127, 127], or
@@ -465,11 +465,11 @@ int tb_b200_kv8_append(const TbB200Kv8* cache, const TbB200Kv8Batch* batch, int 
  * attends hold numbers, as tb_b200_kv8_append leaves them; an e4m3 NaN code
  * there may reach other rows of its sequence too.
  * Sums, maxima and the softmax's sums are f32 (products with int8 codes exact),
- * exponentials ex2.approx's (2^-22).  bf16 calls hold q as f16 scaled by a power
- * of two or in 22 bits, and the weights as f16 (2^-12 of each, an eighth of the
- * output's half step, so a last place differs from f32 arithmetic's now and
- * then); f32 calls q in 22 bits of its row's largest element or of each, and
- * the weights as two f16.  A row of q with a NaN or an infinity gives NaN. */
+ * exponentials ex2.approx's (2^-22).  q is held to 2^-22 of its row's largest
+ * element or better.  bf16 calls hold the weights as f16 (2^-12 of each, an
+ * eighth of the output's half step, so a last place differs from f32
+ * arithmetic's now and then), f32 calls as two f16.  A row of q with a NaN or an
+ * infinity gives NaN. */
 typedef struct {
     int dtype; /* of q and out: TB_DTYPE_F32 or TB_DTYPE_BF16 */
     int n_heads; /* a multiple of the cache's n_kv_heads */

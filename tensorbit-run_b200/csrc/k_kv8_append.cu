@@ -21,9 +21,9 @@
 // head need no more lanes.  The rows stay in registers between amax and the codes, up
 // to kHold vectors a thread (a page of 64 rows of 128 in bf16); what is past that is
 // read again, a vector at a time: such prompts in pages of 128 take 30 us and in f32,
-// pages of 64, 37 (their bytes: 17 and 23).  The rule goes by the call's mean rows a sequence:
-// 1500 rows beside 255 single tokens, all in one warp a unit, take 21 us, and 4.1 and
-// 4.3 as two calls.
+// pages of 64, 37 (their bytes: 17 and 23).  The rule goes by the call's mean rows a
+// sequence: 1500 rows beside 255 single tokens, all in one warp a unit, take 21 us, and
+// 4.1 and 4.3 as two calls.
 //
 // Measured, 8 heads of 128, bf16: 14476 tokens of five prompts, e4m3, 17.1 us,
 // 5.2 TB/s (18.3 with three CTAs an SM); 256 sequences' token, int8, 4.2 us, a launch

@@ -42,12 +42,12 @@ using tbk::kFull;
 constexpr int kMaxDim = 512;
 constexpr int kThreads = 256;
 
-// Most threads of a CTA.  The rotation of many rows alone streams best in small ones
-// (16384 rows of 72 heads of 128: 94 us with 128, 101 with 256; 8192 of 9 of 256: 18
-// and 24); 64 rows of 72 heads take 3.6 us with 128 and 3.2 with 256, 256 rows with
-// the norm 6.4 and 5.7, 4095 of f32 46.8 and 46.1.  Few rows are up to four for every
-// SM, which those of 256 threads hold at once; between 64 rows and 8192 neither side of
-// the rotation alone was measured.
+// Most threads of a CTA.  The rotation of many rows alone streams best in small ones,
+// that of few in large ones, of which four for every SM run at once: rows of 72 heads of
+// 128 in bf16 with 128 and with 256 threads, 64 rows 3.4 and 3.0 us, 300 5.8 and 5.2, 592
+// 7.4 and 6.9, 1024 9.5 and 10.2, 4096 27.4 and 29.0, 16384 94 and 101; of 9 heads of 256,
+// 592 3.2 and 3.3, 1024 4.6 and 5.6, 8192 18 and 24.  With the norm, 592 9.4 and 8.5, 4095
+// of f32 46.8 and 46.1 (but 1024 of bf16 12.1 and 13.4).
 unsigned threads_of(bool norm, unsigned rows, int sm_count) {
     return norm || rows <= 4u * sm_count ? 256 : 128;
 }
@@ -322,8 +322,8 @@ int run(const TbB200Rotary* t, bool norm, void* stream) {
     if (!t) return TB_ERR_INVALID_ARG;
     if (t->rows < 0 || t->rows > INT32_MAX || t->n_q_heads < 0 || t->n_kv_heads < 0 ||
         (int64_t)t->n_q_heads + t->n_kv_heads > INT32_MAX / 2 ||  // heads of passes past it too
-        t->head_dim < 1 || t->head_dim > kMaxDim || t->rotary_dim < 0 || t->rotary_dim > t->head_dim ||
-        t->rotary_dim % 2)
+        t->head_dim < 1 || t->head_dim > kMaxDim || t->rotary_dim < 0 ||
+        t->rotary_dim > t->head_dim || t->rotary_dim % 2)
         return TB_ERR_INVALID_SHAPE;
     if (t->dtype != TB_DTYPE_F32 && t->dtype != TB_DTYPE_BF16) return TB_ERR_UNSUPPORTED_DTYPE;
     if (t->layout != TB_B200_ROTARY_INTERLEAVED && t->layout != TB_B200_ROTARY_HALF)
