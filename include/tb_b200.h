@@ -495,6 +495,113 @@ int tb_b200_kv8_attention_workspace(const TbB200Kv8* cache, const TbB200Kv8Batch
                                     const TbB200Kv8Attention* attention, size_t* bytes);
 
 /* ======================================================================
+ * Microscaled formats: rows quantised to them, the row ops that end in them,
+ * and the linear layers over them (no counterpart in the reference, whose
+ * linear layers are f32 over one vector, src/ops/linear.c:4-53)
+ * ====================================================================== */
+
+/* Code formats: OCP e4m3 (finite up to 448), a byte each; OCP e2m1 (0, 0.5, 1,
+ * 1.5, 2, 3, 4, 6 and their negatives), two to a byte, element 2i in the low bits. */
+#define TB_B200_MX_E4M3 0x43
+#define TB_B200_MX_E2M1 0x21
+
+/* A [rows, cols] tensor of such codes with a power-of-two scale for every 32
+ * neighbouring elements of a row: element = code * 2^(scale byte - 127); the byte
+ * 0xff is NaN.  Both buffers are the caller's device memory, of
+ * tb_b200_mx_bytes' sizes:
+ *   codes   32-byte aligned; a row is its columns filled up to a multiple of 128
+ *           with zeros, and starts right after the row before
+ *   scales  16-byte aligned; in tiles of 128 rows and 4 blocks, 512 bytes each,
+ *           the tiles of 128 rows one after the other: with
+ *           T = ceil(cols / 128), block b of row r is byte
+ *           512 ((r / 128) T + b / 4) + 16 (r % 32) + 4 (r % 128 / 32) + b % 4
+ * The first n rows of a tensor are a tensor, and so are its rows from any multiple
+ * of 128 on.  What fills up a row belongs to the tensor: codes of zero, with any
+ * scale but 0xff. */
+typedef struct {
+    int format;   /* TB_B200_MX_* */
+    int64_t rows; /* below 2^31 - 128 */
+    int64_t cols; /* 1 .. 2^24 */
+    void* codes;
+    uint8_t* scales;
+} TbB200Mx;
+
+/* Bytes of the codes and the scales of such a tensor. */
+int tb_b200_mx_bytes(int format, int64_t rows, int64_t cols, size_t* codes, size_t* scales);
+
+/* Rows of x (f32 or bf16, x_stride elements apart) to out, every row, fill and scale of
+ * it: the scale of a block is the least 2^e >= 2^-127 with max|x| <= MAX 2^e (MAX 448
+ * or 6), its codes x / 2^e rounded to nearest, ties to even.  A block with a NaN or an
+ * infinity becomes NaN.  Scales of rows behind the last one, up to a multiple of 128,
+ * are written as 0. */
+int tb_b200_mx_quantize(int dtype, const void* x, int64_t x_stride, const TbB200Mx* out,
+                        void* stream);
+/* The values of t, as f32 or bf16 (rounded to nearest even where a value is not a number
+ * of that type: below bf16's least ones only), rows y_stride elements apart. */
+int tb_b200_mx_dequantize(const TbB200Mx* t, int dtype, void* y, int64_t y_stride, void* stream);
+
+/* tb_b200_residual_rms_norm with y in a microscaled format (y->rows rows of y->cols): the
+ * same h and f32 arithmetic, and y's f32 values to codes and scales as tb_b200_mx_quantize
+ * takes them there, without a rounding between.  residual NULL: the norm of x; weight and
+ * h_out may be NULL; h_out may be x or residual. */
+int tb_b200_residual_rms_norm_mx(int dtype, const void* x, const void* residual,
+                                 const void* weight, void* h_out, const TbB200Mx* y, float eps,
+                                 void* stream);
+
+/* tb_b200_swiglu with its f32 result in a microscaled format: out->rows rows of out->cols,
+ * gate and up with rows gate_stride and up_stride elements apart (slices of the joint
+ * product of both, say). */
+int tb_b200_swiglu_mx(int dtype, const void* gate, int64_t gate_stride, const void* up,
+                      int64_t up_stride, const TbB200Mx* out, void* stream);
+
+/* y = x w^T (+ bias): y[r][o] = sum_i x[r][i] w[o][i] + bias[o], x [rows, cols], w
+ * [outs, cols], any two formats; y f32 or bf16 (out_dtype) with rows y_stride elements
+ * apart; bias [outs] f32 or NULL.  Products are exact and their sums f32 (of 32 elements
+ * or 64 at a time, then in the order of i; long sums of few rows as up to 8 parts, in
+ * their order), y rounded once.  A row of x with a NaN gives NaN in its row of y,
+ * a row of w in its column; the others are as without it. */
+int tb_b200_mx_linear(const TbB200Mx* x, const TbB200Mx* w, const float* bias, int out_dtype,
+                      void* y, int64_t y_stride, void* stream);
+
+/* ======================================================================
+ * Sampling with filters
+ * ====================================================================== */
+
+/* One token of each row of logits (f32 or bf16, `stride` elements apart), by the row's own
+ * settings, device arrays of one value per row; NULL is off:
+ *   temperature  w_i = exp((x_i - max x) / temperature); <= 0 or NaN: the first largest
+ *                logit; NULL: 1
+ *   top_k        of the k largest logits (of equal ones the first); <= 0: of all
+ *   top_p        of those, in falling order (equal ones in their order), the ones whose
+ *                predecessors' weights sum to less than top_p of the sum of all of those,
+ *                and the first; >= 1 or NaN: all of them
+ *   min_p        of those, the ones with w_i >= min_p (the largest has 1) and the first;
+ *                <= 0 or NaN: all of them
+ *   uniforms     in [0, 1): the draw is the first i kept, in the order of i, with
+ *                sum_{j <= i} w_j > u * (the sum over all kept)
+ * NaN logits are never kept, -infinity never drawn; where one is +infinity, those are
+ * alike and the others have no weight.  A row with no logit above -infinity draws 0.
+ * Weights are held to 2^-39 of the largest or better (their fixed-point sums do not depend
+ * on an order), so a draw is the definition's unless a border lies about that near to u
+ * times the sum, or to top_p times it.  Unlike tb_b200_sample_temperature this is not
+ * the reference's draw to the last bit, and a NaN does not decide a row. */
+typedef struct {
+    int dtype; /* of the logits */
+    int64_t rows;
+    int64_t vocab; /* 1 .. 2^22 */
+    const void* logits;
+    int64_t stride;
+    const float* temperature;
+    const int32_t* top_k;
+    const float* top_p;
+    const float* min_p;
+    const double* uniforms;
+    int32_t* out; /* [rows] */
+} TbB200Sample;
+
+int tb_b200_sample(const TbB200Sample* sample, void* stream);
+
+/* ======================================================================
  * Decoder forward on the device (TransformerRunner)
  * ====================================================================== */
 

@@ -1,0 +1,470 @@
+// k_mx_rows.cu -- rows to microscaled formats (mx.cuh): quantised as they are, behind
+// SwiGLU, or behind a residual add and RMSNorm; and back to values.
+//
+// A thread has 32 bytes of a row (16 bf16 or 8 f32), so a block of 32 elements is 2 or 4
+// neighbouring lanes, its largest magnitude 1 or 2 shuffles, and the four scales of a tile's
+// row one 32-bit store.  All are HBM bound: the inputs once, codes and scales once.
+#include "bodies.cuh"
+#include "mx.cuh"
+
+namespace {
+
+using tbk::Elt;
+
+constexpr int kThreads = 256;
+
+// 32 bytes of a row as they are.
+template <typename T>
+struct Chunk {
+    static constexpr int E = 32 / sizeof(T);
+    uint4 r[2];
+
+    // Elements [at, at + E) of a row of `cols`, zeros past its end; vec: 16-byte aligned.
+    __device__ __forceinline__ void load(const T* row, int at, int cols, bool vec) {
+        if (vec && at + E <= cols) {
+            const uint4* p = reinterpret_cast<const uint4*>(row + at);
+            r[0] = __ldcs(p);
+            r[1] = __ldcs(p + 1);
+            return;
+        }
+        uint32_t w[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            w[i] = 0;
+            if constexpr (sizeof(T) == 4) {
+                if (at + i < cols) w[i] = reinterpret_cast<const uint32_t*>(row)[at + i];
+            } else {
+                const uint16_t* u = reinterpret_cast<const uint16_t*>(row);
+                if (at + 2 * i < cols) w[i] = u[at + 2 * i];
+                if (at + 2 * i + 1 < cols) w[i] |= (uint32_t)u[at + 2 * i + 1] << 16;
+            }
+        }
+        r[0] = make_uint4(w[0], w[1], w[2], w[3]);
+        r[1] = make_uint4(w[4], w[5], w[6], w[7]);
+    }
+    __device__ __forceinline__ void widen(float (&v)[E]) const {
+        const uint32_t w[8] = {r[0].x, r[0].y, r[0].z, r[0].w, r[1].x, r[1].y, r[1].z, r[1].w};
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            if constexpr (sizeof(T) == 4) {
+                v[i] = __uint_as_float(w[i]);
+            } else {
+                v[2 * i] = __uint_as_float(w[i] << 16);
+                v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+            }
+        }
+    }
+};
+
+// Elements [at, at + E) of a row of `cols` from v.
+template <typename T, int E>
+__device__ __forceinline__ void store_chunk(T* row, int at, int cols, bool vec,
+                                            const float (&v)[E]) {
+    if (vec && at + E <= cols) {
+        constexpr int V = Elt<T>::kVec;
+#pragma unroll
+        for (int i = 0; i < E; i += V) {
+            float part[V];
+#pragma unroll
+            for (int j = 0; j < V; ++j) part[j] = v[i + j];
+            tbk::store_vec<T, V>(row + at + i, part);
+        }
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < E; ++i)
+        if (at + i < cols) Elt<T>::store(row + at + i, v[i]);
+}
+
+// Row and chunk of an item; 32-bit division where the items fit.
+__device__ __forceinline__ void place_of(int64_t i, int chunks, bool small, int64_t& r, int& c) {
+    if (small) {
+        const uint32_t q = (uint32_t)i / (uint32_t)chunks;
+        r = q;
+        c = (int)((uint32_t)i - q * (uint32_t)chunks);
+    } else {
+        r = i / chunks;
+        c = (int)(i - r * chunks);
+    }
+}
+
+// ------------------------------------------------- quantise, SwiGLU
+template <typename T>
+struct Rows {
+    const T *a, *b;  // b: SwiGLU's up rows, a its gate rows
+    int64_t a_stride, b_stride;
+    bool vec;
+};
+
+// A thread an item: chunk c of row r, all rows of whole tiles (behind the last one only the
+// scales are written).
+template <typename T, int FORMAT, bool SWIGLU>
+__global__ void __launch_bounds__(kThreads) k_rows(const Rows<T> in, const mx::View out,
+                                                   int chunks, int64_t items, bool small) {
+    constexpr int E = Chunk<T>::E;
+    const int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x;
+    int64_t r;
+    int c;
+    place_of(min(i, items - 1), chunks, small, r, c);
+    const bool live = i < items && r < out.rows;
+    float v[E];
+    Chunk<T> x, y;
+    if (live) {
+        x.load(in.a + r * in.a_stride, c * E, out.cols, in.vec);
+        if constexpr (SWIGLU) y.load(in.b + r * in.b_stride, c * E, out.cols, in.vec);
+    } else {
+        x.r[0] = x.r[1] = y.r[0] = y.r[1] = make_uint4(0, 0, 0, 0);
+    }
+    x.widen(v);
+    if constexpr (SWIGLU) {
+        float u[E];
+        y.widen(u);
+#pragma unroll
+        for (int e = 0; e < E; ++e) v[e] = tbk::ew_apply<tbk::kSwiglu>(v[e], u[e]);
+    }
+    mx::store_block<FORMAT, E>(out, r, c, live, v);
+    if (!live && i < items && c % (128 / E) == 0)
+        *reinterpret_cast<uint32_t*>(out.scales + mx::scales_at(r, c * E / 128, out.tiles)) = 0;
+}
+
+template <typename T, bool SWIGLU>
+int launch_rows(const Rows<T>& in, const TbB200Mx* out, cudaStream_t s) {
+    const mx::View v = mx::view(out);
+    const int chunks = v.tiles * (128 / Chunk<T>::E);
+    const int64_t items = mx::tiles_of(v.rows) * 128 * chunks;
+    const int64_t grid = (items + kThreads - 1) / kThreads;
+    if (grid > INT32_MAX) return TB_ERR_INVALID_SHAPE;
+    const bool small = items + kThreads <= UINT32_MAX;
+    if (out->format == mx::kE4m3)
+        k_rows<T, mx::kE4m3, SWIGLU><<<(unsigned)grid, kThreads, 0, s>>>(in, v, chunks, items, small);
+    else
+        k_rows<T, mx::kE2m1, SWIGLU><<<(unsigned)grid, kThreads, 0, s>>>(in, v, chunks, items, small);
+    TB_LAUNCH_CHECK("microscaled rows kernel");
+    return TB_OK;
+}
+
+template <typename T>
+bool aligned_rows(const void* p, int64_t stride) {
+    return tbh::aligned16(p) && stride * (int64_t)sizeof(T) % 16 == 0;
+}
+
+template <typename T>
+int quantize(const void* x, int64_t stride, const TbB200Mx* out, cudaStream_t s) {
+    const Rows<T> in = {static_cast<const T*>(x), nullptr, stride, 0, aligned_rows<T>(x, stride)};
+    return launch_rows<T, false>(in, out, s);
+}
+
+template <typename T>
+int swiglu(const void* gate, int64_t gate_stride, const void* up, int64_t up_stride,
+           const TbB200Mx* out, cudaStream_t s) {
+    const Rows<T> in = {static_cast<const T*>(gate), static_cast<const T*>(up), gate_stride,
+                        up_stride,
+                        aligned_rows<T>(gate, gate_stride) && aligned_rows<T>(up, up_stride)};
+    return launch_rows<T, true>(in, out, s);
+}
+
+// ------------------------------------------------- back to values
+// A thread 16 codes.
+template <typename T, int FORMAT>
+__global__ void __launch_bounds__(kThreads) k_values(const mx::View t, T* y, int64_t stride,
+                                                     bool vec, int chunks, int64_t items,
+                                                     bool small) {
+    const int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x;
+    if (i >= items) return;
+    int64_t r;
+    int c;
+    place_of(i, chunks, small, r, c);
+    const uint8_t* from = t.codes + r * t.pitch + (int64_t)c * (FORMAT == mx::kE4m3 ? 16 : 8);
+    const float scale = mx::value_of(t.scales[mx::scales_at(r, c / 8, t.tiles) + c / 2 % 4]);
+    float v[16];
+    if constexpr (FORMAT == mx::kE4m3) {
+        const uint4 w = *reinterpret_cast<const uint4*>(from);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const uint16_t two = (uint16_t)((&w.x)[j / 2] >> j % 2 * 16);
+            const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(two, __NV_E4M3);
+            v[2 * j] = __half2float(__half(__half_raw{h.x}));
+            v[2 * j + 1] = __half2float(__half(__half_raw{h.y}));
+        }
+    } else {
+        const uint2 w = *reinterpret_cast<const uint2*>(from);
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+            // sign, 2 exponent bits and 1 mantissa bit sit in f32's places 126 binades of
+            // bias below their value, the subnormal 0.5 included
+            const uint32_t n = (j < 8 ? w.x : w.y) >> j % 8 * 4;
+            v[j] = __uint_as_float((n & 8) << 28 | (n & 7) << 22) * 8.5070591730234616e37f;
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < 16; ++j) v[j] *= scale;
+    store_chunk<T, 16>(y + r * stride, c * 16, t.cols, vec, v);
+}
+
+template <typename T>
+int dequantize(const TbB200Mx* t, void* y, int64_t stride, cudaStream_t s) {
+    const mx::View v = mx::view(t);
+    const int chunks = (v.cols + 15) / 16;
+    const int64_t items = v.rows * chunks, grid = (items + kThreads - 1) / kThreads;
+    if (grid > INT32_MAX) return TB_ERR_INVALID_SHAPE;
+    const bool vec = aligned_rows<T>(y, stride), small = items + kThreads <= UINT32_MAX;
+    if (t->format == mx::kE4m3)
+        k_values<T, mx::kE4m3><<<(unsigned)grid, kThreads, 0, s>>>(v, static_cast<T*>(y), stride,
+                                                                   vec, chunks, items, small);
+    else
+        k_values<T, mx::kE2m1><<<(unsigned)grid, kThreads, 0, s>>>(v, static_cast<T*>(y), stride,
+                                                                   vec, chunks, items, small);
+    TB_LAUNCH_CHECK("microscaled values kernel");
+    return TB_OK;
+}
+
+// ------------------------------------------------- residual + RMSNorm
+template <typename T>
+struct Norm {
+    const T *x, *res, *w;
+    T* h;
+    bool vec, vec_w;
+    float eps;
+};
+
+// h of a chunk: x + residual in f32, the same bits each time.
+template <typename T>
+__device__ __forceinline__ void sum_of(const Norm<T>& in, const Chunk<T>& x, const Chunk<T>& res,
+                                       float (&h)[Chunk<T>::E]) {
+    x.widen(h);
+    if (in.res) {
+        float r[Chunk<T>::E];
+        res.widen(r);
+#pragma unroll
+        for (int e = 0; e < Chunk<T>::E; ++e) h[e] = __fadd_rn(h[e], r[e]);
+    }
+}
+
+// h and the norm of chunk c of row r, stored.
+template <typename T, int FORMAT>
+__device__ __forceinline__ void finish(const Norm<T>& in, const mx::View& out, int64_t r, int c,
+                                       bool live, float scale, float (&h)[Chunk<T>::E]) {
+    constexpr int E = Chunk<T>::E;
+    if (live && in.h) store_chunk<T, E>(in.h + r * out.cols, c * E, out.cols, in.vec, h);
+    float w[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) h[e] = __fmul_rn(h[e], scale);
+    if (in.w && live) {
+        if (in.vec_w && c * E + E <= out.cols) {
+            const uint4* p = reinterpret_cast<const uint4*>(in.w + c * E);
+            Chunk<T> raw;
+            raw.r[0] = p[0];
+            raw.r[1] = p[1];
+            raw.widen(w);
+        } else {
+#pragma unroll
+            for (int e = 0; e < E; ++e)
+                w[e] = c * E + e < out.cols ? Elt<T>::load(in.w + c * E + e) : 0.0f;
+        }
+#pragma unroll
+        for (int e = 0; e < E; ++e) h[e] = __fmul_rn(h[e], w[e]);
+    }
+    // (a row whose scale is NaN or an infinity has fill of zeros all the same)
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+        if (c * E + e >= out.cols) h[e] = 0.0f;
+    mx::store_block<FORMAT, E>(out, r, c, live, h);
+}
+
+__device__ __forceinline__ float scale_of(float ss, float eps, int cols) {
+    return __fdiv_rn(1.0f, __fsqrt_rn(__fdiv_rn(__fadd_rn(ss, eps), (float)cols)));
+}
+
+// G threads a row, ITEMS chunks a thread, kept in registers as they were loaded.
+template <typename T, int FORMAT, int ITEMS, int MAXT>
+__global__ void __launch_bounds__(MAXT) k_norm(const Norm<T> in, const mx::View out, int G) {
+    constexpr int E = Chunk<T>::E;
+    __shared__ float red[32];
+    const int lane = threadIdx.x & (G - 1);
+    const int64_t r = (int64_t)blockIdx.x * (blockDim.x / G) + threadIdx.x / G;
+    const bool active = r < out.rows;
+    const int chunks = out.tiles * (128 / E);
+    Chunk<T> x[ITEMS], res[ITEMS];
+    float ss = 0.0f;
+    if (active) {
+#pragma unroll
+        for (int i = 0; i < ITEMS; ++i) {
+            const int c = lane + i * G;
+            if (c < chunks) {
+                x[i].load(in.x + r * out.cols, c * E, out.cols, in.vec);
+                if (in.res) res[i].load(in.res + r * out.cols, c * E, out.cols, in.vec);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < ITEMS; ++i) {
+            if (lane + i * G < chunks) {
+                float h[E];
+                sum_of(in, x[i], res[i], h);
+#pragma unroll
+                for (int e = 0; e < E; ++e) ss = __fmaf_rn(h[e], h[e], ss);
+            }
+        }
+    }
+    ss = tbk::group_sum(ss, G, red);
+    const float scale = scale_of(ss, in.eps, out.cols);
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i) {
+        const int c = lane + i * G;
+        const bool live = active && c < chunks;
+        float h[E];
+        if (live) {
+            sum_of(in, x[i], res[i], h);
+        } else {
+#pragma unroll
+            for (int e = 0; e < E; ++e) h[e] = 0.0f;
+        }
+        finish<T, FORMAT>(in, out, r, c, live, scale, h);
+        if (!active && c < chunks && r < (out.rows + 127) / 128 * 128 && c % (128 / E) == 0)
+            *reinterpret_cast<uint32_t*>(out.scales + mx::scales_at(r, c * E / 128, out.tiles)) = 0;
+    }
+}
+
+// Rows wider than that: a CTA a row, read twice, the second time from L2.
+template <typename T, int FORMAT>
+__global__ void __launch_bounds__(1024) k_norm_wide(const Norm<T> in, const mx::View out) {
+    constexpr int E = Chunk<T>::E;
+    __shared__ float red[32];
+    const int64_t r = blockIdx.x;
+    const int chunks = out.tiles * (128 / E);
+    const bool active = r < out.rows;
+    float ss = 0.0f;
+    Chunk<T> x, res;
+    float h[E];
+    for (int c = threadIdx.x; active && c < chunks; c += blockDim.x) {
+        x.load(in.x + r * out.cols, c * E, out.cols, in.vec);
+        if (in.res) res.load(in.res + r * out.cols, c * E, out.cols, in.vec);
+        sum_of(in, x, res, h);
+#pragma unroll
+        for (int e = 0; e < E; ++e) ss = __fmaf_rn(h[e], h[e], ss);
+    }
+    ss = tbk::group_sum(ss, blockDim.x, red);
+    const float scale = scale_of(ss, in.eps, out.cols);
+    for (int c0 = 0; c0 < chunks; c0 += blockDim.x) {
+        const int c = c0 + threadIdx.x;
+        const bool live = active && c < chunks;
+#pragma unroll
+        for (int e = 0; e < E; ++e) h[e] = 0.0f;
+        if (live) {
+            x.load(in.x + r * out.cols, c * E, out.cols, in.vec);
+            if (in.res) res.load(in.res + r * out.cols, c * E, out.cols, in.vec);
+            sum_of(in, x, res, h);
+        }
+        finish<T, FORMAT>(in, out, r, c, live, scale, h);
+        if (!active && c < chunks && c % (128 / E) == 0)
+            *reinterpret_cast<uint32_t*>(out.scales + mx::scales_at(r, c * E / 128, out.tiles)) = 0;
+    }
+}
+
+template <typename T, int FORMAT>
+int launch_norm(const Norm<T>& in, const TbB200Mx* y, cudaStream_t s) {
+    const mx::View out = mx::view(y);
+    const int64_t rows = mx::tiles_of(out.rows) * 128;
+    const tbh::NormCfg c = tbh::norm_cfg((int64_t)out.tiles * (128 / Chunk<T>::E), 1024);
+    const int per = c.threads / c.G;
+    const unsigned grid = (unsigned)((rows + per - 1) / per);
+    if (c.items == 0) {
+        k_norm_wide<T, FORMAT><<<(unsigned)rows, 1024, 0, s>>>(in, out);
+    } else if (c.threads <= 256) {
+        switch (c.items) {
+            case 1: k_norm<T, FORMAT, 1, 256><<<grid, c.threads, 0, s>>>(in, out, c.G); break;
+            case 2: k_norm<T, FORMAT, 2, 256><<<grid, c.threads, 0, s>>>(in, out, c.G); break;
+            default: k_norm<T, FORMAT, 4, 256><<<grid, c.threads, 0, s>>>(in, out, c.G); break;
+        }
+    } else {
+        switch (c.items) {
+            case 1: k_norm<T, FORMAT, 1, 1024><<<grid, c.threads, 0, s>>>(in, out, c.G); break;
+            case 2: k_norm<T, FORMAT, 2, 1024><<<grid, c.threads, 0, s>>>(in, out, c.G); break;
+            default: k_norm<T, FORMAT, 4, 1024><<<grid, c.threads, 0, s>>>(in, out, c.G); break;
+        }
+    }
+    TB_LAUNCH_CHECK("residual_rms_norm_mx kernel");
+    return TB_OK;
+}
+
+template <typename T>
+int norm(const void* x, const void* res, const void* w, void* h, const TbB200Mx* y, float eps,
+         cudaStream_t s) {
+    const bool vec = aligned_rows<T>(x, y->cols) && (!res || tbh::aligned16(res)) &&
+                     (!h || tbh::aligned16(h));
+    const Norm<T> in = {static_cast<const T*>(x), static_cast<const T*>(res),
+                        static_cast<const T*>(w), static_cast<T*>(h), vec, tbh::aligned16(w), eps};
+    return y->format == mx::kE4m3 ? launch_norm<T, mx::kE4m3>(in, y, s)
+                                  : launch_norm<T, mx::kE2m1>(in, y, s);
+}
+
+bool is_float(int dtype) { return dtype == TB_DTYPE_F32 || dtype == TB_DTYPE_BF16; }
+
+// Rows of cols elements that are `stride` apart.
+bool strided(int64_t rows, int64_t cols, int64_t stride) { return rows <= 1 || stride >= cols; }
+
+}  // namespace
+
+extern "C" int tb_b200_mx_bytes(int format, int64_t rows, int64_t cols, size_t* codes,
+                                size_t* scales) {
+    const TbB200Mx t = {format, rows, cols, nullptr, nullptr};
+    const int rc = mx::check(&t, false);
+    if (rc != TB_OK) return rc;
+    if (!codes || !scales) return TB_ERR_INVALID_ARG;
+    *codes = (size_t)(rows * mx::pitch_of(format, cols));
+    *scales = (size_t)(mx::tiles_of(rows) * mx::tiles_of(cols) * mx::kTileBytes);
+    return TB_OK;
+}
+
+extern "C" int tb_b200_mx_quantize(int dtype, const void* x, int64_t x_stride,
+                                   const TbB200Mx* out, void* stream) {
+    const int rc = mx::check(out, true);
+    if (rc != TB_OK) return rc;
+    if (!is_float(dtype)) return TB_ERR_UNSUPPORTED_DTYPE;
+    if (!strided(out->rows, out->cols, x_stride)) return TB_ERR_INVALID_SHAPE;
+    if (out->rows == 0) return TB_OK;
+    if (!x) return TB_ERR_INVALID_ARG;
+    cudaStream_t s = tbh::stream_of(stream);
+    return dtype == TB_DTYPE_F32 ? quantize<float>(x, x_stride, out, s)
+                                 : quantize<__nv_bfloat16>(x, x_stride, out, s);
+}
+
+extern "C" int tb_b200_mx_dequantize(const TbB200Mx* t, int dtype, void* y, int64_t y_stride,
+                                     void* stream) {
+    const int rc = mx::check(t, true);
+    if (rc != TB_OK) return rc;
+    if (!is_float(dtype)) return TB_ERR_UNSUPPORTED_DTYPE;
+    if (!strided(t->rows, t->cols, y_stride)) return TB_ERR_INVALID_SHAPE;
+    if (t->rows == 0) return TB_OK;
+    if (!y) return TB_ERR_INVALID_ARG;
+    cudaStream_t s = tbh::stream_of(stream);
+    return dtype == TB_DTYPE_F32 ? dequantize<float>(t, y, y_stride, s)
+                                 : dequantize<__nv_bfloat16>(t, y, y_stride, s);
+}
+
+extern "C" int tb_b200_residual_rms_norm_mx(int dtype, const void* x, const void* residual,
+                                            const void* weight, void* h_out, const TbB200Mx* y,
+                                            float eps, void* stream) {
+    const int rc = mx::check(y, true);
+    if (rc != TB_OK) return rc;
+    if (!is_float(dtype)) return TB_ERR_UNSUPPORTED_DTYPE;
+    if (y->rows == 0) return TB_OK;
+    if (!x) return TB_ERR_INVALID_ARG;
+    cudaStream_t s = tbh::stream_of(stream);
+    return dtype == TB_DTYPE_F32 ? norm<float>(x, residual, weight, h_out, y, eps, s)
+                                 : norm<__nv_bfloat16>(x, residual, weight, h_out, y, eps, s);
+}
+
+extern "C" int tb_b200_swiglu_mx(int dtype, const void* gate, int64_t gate_stride, const void* up,
+                                 int64_t up_stride, const TbB200Mx* out, void* stream) {
+    const int rc = mx::check(out, true);
+    if (rc != TB_OK) return rc;
+    if (!is_float(dtype)) return TB_ERR_UNSUPPORTED_DTYPE;
+    if (!strided(out->rows, out->cols, gate_stride) || !strided(out->rows, out->cols, up_stride))
+        return TB_ERR_INVALID_SHAPE;
+    if (out->rows == 0) return TB_OK;
+    if (!gate || !up) return TB_ERR_INVALID_ARG;
+    cudaStream_t s = tbh::stream_of(stream);
+    return dtype == TB_DTYPE_F32
+               ? swiglu<float>(gate, gate_stride, up, up_stride, out, s)
+               : swiglu<__nv_bfloat16>(gate, gate_stride, up, up_stride, out, s);
+}

@@ -1,6 +1,7 @@
 // tcgen05.cuh -- the fifth-generation tensor core instructions that the kernels
 // use: f16 products with f32 sums in tensor memory, issued by one thread, their
-// right operand in shared memory, the left one there or in tensor memory.
+// right operand in shared memory, the left one there or in tensor memory; and products
+// of 8- and 4-bit floats with a scale for every 32 elements of K, in tensor memory too.
 //
 // Operand tiles in shared memory have rows of 128 bytes (64 f16), the 16-byte
 // piece c of row r at c ^ (r & 7), on 1024-byte boundaries:
@@ -134,6 +135,63 @@ __device__ __forceinline__ void store16(uint32_t address, const uint32_t (&r)[16
         "r"(r[15])
         : "memory");
 }
+
+// Products with scales.  Operands are K-major, 128 bytes a row: 128 8-bit elements, 4-bit
+// ones among them (16 in 8 bytes and 8 bytes of fill), or, both operands 4-bit, 256 elements.
+// 32 bytes further is the next instruction's K, 32 or 64 elements.  The scales of 128 rows
+// and 4 blocks of 32 elements have 4 columns of tensor memory: row r in lane r % 32 of every
+// 32, column r / 32, a byte a block.
+enum Element { kE4m3 = 0, kE2m1 = 5 };
+// M = 128, f32 sums, E8M0 scales; less the number of columns and the block (of 4) that the
+// instruction starts with.
+constexpr uint32_t scaled_instruction(Element a, Element b) {
+    return (uint32_t)a << 7 | (uint32_t)b << 10 | 1u << 23 | (uint32_t)(128 / 16) << 24;
+}
+constexpr uint32_t scaled_instruction_4bit() {
+    return 1u << 7 | 1u << 10 | 1u << 23 | (uint32_t)(128 / 16) << 24;
+}
+__device__ __forceinline__ uint32_t with_columns(uint32_t instruction, int n) {
+    return instruction | (uint32_t)(n / 8) << 17;
+}
+__device__ __forceinline__ uint32_t with_block(uint32_t instruction, int block) {
+    return instruction | (uint32_t)block << 4 | (uint32_t)block << 29;
+}
+// d (tensor memory) = a b, or += if `add`; the scales of a and b in tensor memory.
+template <bool BOTH4>
+__device__ __forceinline__ void mma_scaled(uint32_t d, uint64_t a, uint64_t b, uint32_t instruction,
+                                           uint32_t a_scales, uint32_t b_scales, bool add,
+                                           bool leader) {
+    if constexpr (BOTH4)
+        asm volatile(
+            "{\n .reg .pred p, q;\n setp.ne.u32 p, %6, 0;\n setp.ne.u32 q, %7, 0;\n"
+            " @q tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X "
+            "[%0], %1, %2, %3, [%4], [%5], p;\n}" ::"r"(d),
+            "l"(a), "l"(b), "r"(instruction), "r"(a_scales), "r"(b_scales), "r"((uint32_t)add),
+            "r"((uint32_t)leader)
+            : "memory");
+    else
+        asm volatile(
+            "{\n .reg .pred p, q;\n setp.ne.u32 p, %6, 0;\n setp.ne.u32 q, %7, 0;\n"
+            " @q tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X "
+            "[%0], %1, %2, %3, [%4], [%5], p;\n}" ::"r"(d),
+            "l"(a), "l"(b), "r"(instruction), "r"(a_scales), "r"(b_scales), "r"((uint32_t)add),
+            "r"((uint32_t)leader)
+            : "memory");
+}
+// 512 bytes of scales in shared memory (32 rows of 16 bytes, on 16 bytes) to 4 columns of
+// tensor memory, in every 32 lanes; products issued after it by the same thread see them.
+__device__ __forceinline__ void copy_scales(uint32_t to, uint32_t smem, bool leader) {
+    const uint64_t from = (uint64_t)((smem >> 4) & 0x3fff) |  // start
+                          (uint64_t)(128 >> 4) << 16 |        // leading dimension: one wide
+                          (uint64_t)(128 >> 4) << 32 |        // 8 rows further
+                          1ull << 46;                         // the version; no swizzle
+    asm volatile(
+        "{\n .reg .pred q;\n setp.ne.u32 q, %2, 0;\n"
+        " @q tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;\n}" ::"r"(to),
+        "l"(from), "r"((uint32_t)leader)
+        : "memory");
+}
+
 // The warpgroup's registers per thread; the shares add up to the launch's.
 template <int N>
 __device__ __forceinline__ void more_registers() {

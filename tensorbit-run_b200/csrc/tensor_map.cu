@@ -17,8 +17,10 @@ std::atomic<void*> g_encode{nullptr};
 
 namespace tbh {
 
-int encode_tiles_u8(CUtensorMap* map, const void* base, const uint64_t dims[3],
-                    const uint64_t strides[2], const uint32_t box[3], int swizzle) {
+namespace {
+int encode_tiles(CUtensorMap* map, CUtensorMapDataType type, const void* base,
+                 const uint64_t dims[3], const uint64_t strides[2], const uint32_t box[3],
+                 int swizzle) {
     void* fn = g_encode.load();
     if (!fn) {
         cudaDriverEntryPointQueryResult found;
@@ -32,7 +34,7 @@ int encode_tiles_u8(CUtensorMap* map, const void* base, const uint64_t dims[3],
     }
     const cuuint32_t steps[3] = {1, 1, 1};
     const CUresult rc = reinterpret_cast<Encode>(fn)(
-        map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(base),
+        map, type, 3, const_cast<void*>(base),
         reinterpret_cast<const cuuint64_t*>(dims), reinterpret_cast<const cuuint64_t*>(strides),
         box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
         swizzle == 0 ? CU_TENSOR_MAP_SWIZZLE_NONE
@@ -45,6 +47,18 @@ int encode_tiles_u8(CUtensorMap* map, const void* base, const uint64_t dims[3],
         return TB_ERR_DEVICE;
     }
     return TB_OK;
+}
+}  // namespace
+
+int encode_tiles_u8(CUtensorMap* map, const void* base, const uint64_t dims[3],
+                    const uint64_t strides[2], const uint32_t box[3], int swizzle) {
+    return encode_tiles(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, base, dims, strides, box, swizzle);
+}
+
+int encode_tiles_u4(CUtensorMap* map, const void* base, const uint64_t dims[3],
+                    const uint64_t strides[2], const uint32_t box[3], int swizzle) {
+    return encode_tiles(map, CU_TENSOR_MAP_DATA_TYPE_16U4_ALIGN16B, base, dims, strides, box,
+                        swizzle);
 }
 
 }  // namespace tbh

@@ -81,6 +81,7 @@ FLAG_NONFINITE = 0x10
 ROTARY_INTERLEAVED, ROTARY_HALF = 0, 1
 ROTARY_SCALING = {"none": 0, "linear": 1, "ntk": 2, "bands": 3, "yarn": 4}
 KV_INT8, KV_E4M3 = 7, 0x43
+MX_FORMATS = {"e4m3": 0x43, "e2m1": 0x21}
 PROJECTIONS = ("q", "k", "v", "o", "gate", "up", "down")
 
 
@@ -143,6 +144,16 @@ class Kv8Attention(C.Structure):  # TbB200Kv8Attention
                 ("workspace_bytes", C.c_size_t)]
 
 
+class Mx(C.Structure):  # TbB200Mx
+    _fields_ = [("format", i32), ("rows", i64), ("cols", i64), ("codes", vp), ("scales", vp)]
+
+
+class Sample(C.Structure):  # TbB200Sample
+    _fields_ = [("dtype", i32), ("rows", i64), ("vocab", i64), ("logits", vp), ("stride", i64),
+                ("temperature", vp), ("top_k", vp), ("top_p", vp), ("min_p", vp),
+                ("uniforms", vp), ("out", vp)]
+
+
 # name -> (restype, argtypes); every entry point of include/tb_b200.h and tb_backend.h.
 SIGNATURES = {
     "tb_b200_version": (i32, []),
@@ -196,6 +207,13 @@ SIGNATURES = {
     "tb_b200_kv8_attention": (i32, [P(Kv8), P(Kv8Batch), P(Kv8Attention), vp]),
     "tb_b200_kv8_attention_workspace": (i32, [P(Kv8), P(Kv8Batch), P(Kv8Attention),
                                               P(C.c_size_t)]),
+    "tb_b200_mx_bytes": (i32, [i32, i64, i64, P(C.c_size_t), P(C.c_size_t)]),
+    "tb_b200_mx_quantize": (i32, [i32, vp, i64, P(Mx), vp]),
+    "tb_b200_mx_dequantize": (i32, [P(Mx), i32, vp, i64, vp]),
+    "tb_b200_residual_rms_norm_mx": (i32, [i32, vp, vp, vp, vp, P(Mx), f32, vp]),
+    "tb_b200_swiglu_mx": (i32, [i32, vp, i64, vp, i64, P(Mx), vp]),
+    "tb_b200_mx_linear": (i32, [P(Mx), P(Mx), vp, i32, vp, i64, vp]),
+    "tb_b200_sample": (i32, [P(Sample), vp]),
     "tb_b200_runner_create": (i32, [P(RunnerDesc), P(vp)]),
     "tb_b200_runner_forward": (i32, [vp, C.c_int32, P(vp)]),
     "tb_b200_runner_logits": (i32, [vp, vp]),
@@ -955,6 +973,175 @@ def kv8_attention(cache, q, row_start, lengths, page_table, max_q=None, max_len=
         a.workspace_bytes = workspace.numel() * workspace.element_size()
     check(L.tb_b200_kv8_attention(cache.c, b, a, stream), "kv8_attention")
     return out if lse is None else (out, lse)
+
+
+# ------------------------- microscaled formats, their product, filtered sampling
+class MxTensor:
+    """[rows, cols] in a microscaled format ("e4m3" or "e2m1") over the caller's uint8
+    tensors: codes [rows, bytes of a row], whose columns are filled up to a multiple of 128,
+    and the tiled scales (TbB200Mx)."""
+
+    def __init__(self, codes, scales, cols, format):
+        torch = _torch()
+        dev = codes.get_device()
+        if dev < 0 or codes.dim() != 2:
+            raise ValueError("codes are a CUDA tensor [rows, bytes of a row]")
+        rows = codes.shape[0]
+        tiles = -(-cols // 128)
+        pitch = tiles * (64 if format == "e2m1" else 128)
+        self.c = Mx(MX_FORMATS[format], rows, cols,
+                    _flat(codes, torch.uint8, rows * pitch, dev, "codes"),
+                    _flat(scales, torch.uint8, -(-rows // 128) * tiles * 512, dev, "scales"))
+        self.codes, self.scales, self.format, self.device = codes, scales, format, dev
+        self.rows, self.cols = rows, cols
+
+    @classmethod
+    def empty(cls, rows, cols, format="e4m3", device=None):
+        """A tensor of its own, uninitialised memory."""
+        torch = _torch()
+        device = torch.cuda.current_device() if device is None else device
+        tiles = -(-cols // 128)
+        return cls(torch.empty((rows, tiles * (64 if format == "e2m1" else 128)),
+                               dtype=torch.uint8, device=device),
+                   torch.empty(-(-rows // 128) * tiles * 512, dtype=torch.uint8, device=device),
+                   cols, format)
+
+
+def _mx(t, dev, what):
+    if t.device != dev:
+        raise ValueError(f"{what} is on cuda:{t.device}, the current device is cuda:{dev}")
+    return t.c
+
+
+def _mx_out(other, dev, out, rows, cols, format):
+    if out is None:
+        return _new(other, MxTensor.empty, rows, cols, format, dev)
+    if (out.rows, out.cols) != (rows, cols):
+        raise ValueError(f"out must be [{rows}, {cols}]")
+    _mx(out, dev, "out")
+    return out
+
+
+def _rows(t, dev, what, dtype=None):
+    """(dtype code, row stride) of a [rows, cols] tensor of f32 or bf16 that is dense in a
+    row."""
+    _device_is(t, dev)
+    code = dtype_code(t)
+    if code == I32 or t.dim() != 2:
+        raise ValueError(f"{what} must be [rows, cols] of float32 or bfloat16")
+    if dtype is not None and t.dtype is not dtype:
+        raise TypeError(f"{what} must be {dtype}, got {t.dtype}")
+    s0, s1 = t.stride()
+    if s1 != 1 and t.shape[1] > 1:
+        raise ValueError(f"{what} must be dense in a row")
+    return code, s0
+
+
+def mx_quantize(x, format="e4m3", out=None, stream=None):
+    """x [rows, cols], whose rows may be strided, in a microscaled format
+    (tb_b200_mx_quantize)."""
+    torch, dev = _here()
+    stream, other = _stream(torch, dev, stream)
+    code, stride = _rows(x, dev, "x")
+    out = _mx_out(other, dev, out, x.shape[0], x.shape[1], format)
+    check(lib().tb_b200_mx_quantize(code, x.data_ptr(), stride, out.c, stream), "mx_quantize")
+    return out
+
+
+def mx_dequantize(t, dtype=None, out=None, stream=None):
+    """The values of an MxTensor, [rows, cols] of float32 or bfloat16 (`dtype`, or out's)
+    (tb_b200_mx_dequantize)."""
+    torch, dev = _here()
+    stream, other = _stream(torch, dev, stream)
+    c = _mx(t, dev, "t")
+    if out is None:
+        out = _new(other, torch.empty, (t.rows, t.cols),
+                   dtype=torch.float32 if dtype is None else dtype, device=dev)
+    elif out.shape != (t.rows, t.cols):
+        raise ValueError(f"out must be [{t.rows}, {t.cols}]")
+    code, stride = _rows(out, dev, "out", dtype)
+    check(lib().tb_b200_mx_dequantize(c, code, out.data_ptr(), stride, stream), "mx_dequantize")
+    return out
+
+
+def residual_rms_norm_mx(x, residual, weight, eps, h_out=None, format="e4m3", out=None,
+                         stream=None):
+    """(h, y): residual_rms_norm of [rows, cols] with y in a microscaled format
+    (tb_b200_residual_rms_norm_mx).  residual None: the norm of x, with no h; h is a new
+    tensor unless h_out is given (x or residual may be)."""
+    torch, dev = _here()
+    stream, other = _stream(torch, dev, stream)
+    code, _ = _rows(x, dev, "x")
+    (rows, cols), dtype = x.shape, x.dtype
+    n = rows * cols
+    at = [_flat(x, dtype, n, dev, "x"),
+          None if residual is None else _flat(residual, dtype, n, dev, "residual"),
+          None if weight is None else _flat(weight, dtype, cols, dev, "weight")]
+    if h_out is None and residual is not None:
+        h_out = _new(other, torch.empty_like, x)
+    h = None if h_out is None else _flat(h_out, dtype, n, dev, "h_out")
+    out = _mx_out(other, dev, out, rows, cols, format)
+    check(lib().tb_b200_residual_rms_norm_mx(code, *at, h, out.c, eps, stream),
+          "residual_rms_norm_mx")
+    return h_out, out
+
+
+def swiglu_mx(gate, up, format="e4m3", out=None, stream=None):
+    """silu(gate) * up of [rows, cols], whose rows may be strided, in a microscaled format
+    (tb_b200_swiglu_mx)."""
+    torch, dev = _here()
+    stream, other = _stream(torch, dev, stream)
+    code, gs = _rows(gate, dev, "gate")
+    _, us = _rows(up, dev, "up", gate.dtype)
+    if up.shape != gate.shape:
+        raise ValueError("gate and up must have the same shape")
+    out = _mx_out(other, dev, out, gate.shape[0], gate.shape[1], format)
+    check(lib().tb_b200_swiglu_mx(code, gate.data_ptr(), gs, up.data_ptr(), us, out.c, stream),
+          "swiglu_mx")
+    return out
+
+
+def mx_linear(x, w, bias=None, dtype=None, y=None, stream=None):
+    """y = x w^T (+ bias) of MxTensors x [rows, cols] and w [outs, cols]: [rows, outs] of
+    float32 or bfloat16 (`dtype`, or y's; bfloat16 without both), bias float32 [outs]
+    (tb_b200_mx_linear)."""
+    torch, dev = _here()
+    stream, other = _stream(torch, dev, stream)
+    xc, wc = _mx(x, dev, "x"), _mx(w, dev, "w")
+    if y is None:
+        y = _new(other, torch.empty, (x.rows, w.rows),
+                 dtype=torch.bfloat16 if dtype is None else dtype, device=dev)
+    elif y.shape != (x.rows, w.rows):
+        raise ValueError(f"y must be [{x.rows}, {w.rows}]")
+    code, stride = _rows(y, dev, "y", dtype)
+    b = None if bias is None else _flat(bias, torch.float32, w.rows, dev, "bias")
+    check(lib().tb_b200_mx_linear(xc, wc, b, code, y.data_ptr(), stride, stream), "mx_linear")
+    return y
+
+
+def sample(logits, uniforms, temperature=None, top_k=None, top_p=None, min_p=None, out=None,
+           stream=None):
+    """A token of each row of logits [rows, vocab] (rows may be strided), drawn by its
+    uniform (float64 in [0, 1)) after its temperature, top_k (int32), top_p and min_p
+    (float32), device tensors [rows] or None for off (tb_b200_sample).  int32 [rows]."""
+    torch, dev = _here()
+    stream, other = _stream(torch, dev, stream)
+    code, stride = _rows(logits, dev, "logits")
+    rows, vocab = logits.shape
+    f = torch.float32
+
+    def setting(t, dtype, what):
+        return None if t is None else _flat(t, dtype, rows, dev, what)
+
+    if out is None:
+        out = _new(other, torch.empty, rows, dtype=torch.int32, device=dev)
+    t = Sample(code, rows, vocab, logits.data_ptr(), stride,
+               setting(temperature, f, "temperature"), setting(top_k, torch.int32, "top_k"),
+               setting(top_p, f, "top_p"), setting(min_p, f, "min_p"),
+               _flat(uniforms, torch.float64, rows, dev, "uniforms"),
+               _flat(out, torch.int32, rows, dev, "out"))
+    check(lib().tb_b200_sample(t, stream), "sample")
+    return out
 
 
 # ------------------------------------------------ decoder forward (runner)
