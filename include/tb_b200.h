@@ -581,14 +581,14 @@ int tb_b200_mx_linear(const TbB200Mx* x, const TbB200Mx* w, const float* bias, i
  *                sum_{j <= i} w_j > u * (the sum over all kept)
  * NaN logits are never kept, -infinity never drawn; where one is +infinity, those are
  * alike and the others have no weight.  A row with no logit above -infinity draws 0.
- * Weights are held to 2^-39 of the largest or better (their fixed-point sums do not depend
+ * Weights are held to 2^-44 of the largest or better (their fixed-point sums do not depend
  * on an order), so a draw is the definition's unless a border lies about that near to u
  * times the sum, or to top_p times it.  Unlike tb_b200_sample_temperature this is not
  * the reference's draw to the last bit, and a NaN does not decide a row. */
 typedef struct {
     int dtype; /* of the logits */
     int64_t rows;
-    int64_t vocab; /* 1 .. 2^22 */
+    int64_t vocab; /* 1 .. 376832 */
     const void* logits;
     int64_t stride;
     const float* temperature;

@@ -57,8 +57,7 @@ __device__ __forceinline__ void tma_tile(void* dst, const CUtensorMap* map, int 
 }
 
 __device__ __forceinline__ void cluster_sync() {
-    asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;"
-                 ::: "memory");
+    asm volatile("barrier.cluster.arrive.release;\nbarrier.cluster.wait.acquire;" ::: "memory");
 }
 __device__ __forceinline__ float load_of(uint32_t smem, int rank) {
     uint32_t at;
@@ -254,7 +253,6 @@ __global__ void __launch_bounds__(kThreads) k_linear(const __grid_constant__ Arg
                 }
             }
         }
-        __syncwarp();
         cluster_sync();  // the others have read this CTA's part
     }
 }
