@@ -4,8 +4,9 @@
 // w is the left operand: a tile is 128 outs by up to 256 rows of x, its sums in tensor memory
 // as [out][row].  So a single row of x is as good a tile as many (the instruction takes 16
 // columns at least), and w, the larger side in serving, is read once for up to 256 rows.
-// One warp asks for operands and scales by TMA, one copies the scales to tensor memory and
-// issues the products, four bring a tile's sums to y, a lane an out.  Where the tiles do not
+// One warp asks for operands by TMA, four bring scales from global memory through registers
+// to tensor memory (a lane 16 bytes, no step of their way through shared memory or the tensor
+// pipe), one issues the products, four bring a tile's sums to y, a lane an out.  Where the tiles do not
 // fill the SMs, the CTAs of a cluster take parts of cols and add them up, in order, through
 // one another's shared memory.
 #include <atomic>
@@ -17,10 +18,11 @@
 
 namespace {
 
-constexpr int kThreads = 192;
-constexpr int kLoader = 0, kIssuer = 1, kStoreWarps = 4;  // warps; the others store
-constexpr int kTileOuts = 128, kMostRows = 256, kMostStages = 12, kMostSplit = 8;
-constexpr int kStepBytes = 128;  // of a row of codes
+// warps; of the others kStoreWarps store and 4 bring scales
+constexpr int kLoader = 0, kIssuer = 1, kStorers = 2;
+constexpr int kOuts = 128, kMostStages = 12, kMostSplit = 8;  // kOuts: of a CTA's tile
+constexpr int kPieceBytes = 128;  // of a row of codes; a step has one or two such pieces
+constexpr uint64_t kLimit = 1000000000ull;  // ns, of a wait
 
 struct Args {
     CUtensorMap w_map, x_map;
@@ -31,223 +33,424 @@ struct Args {
     unsigned* status;
     int rows, outs, tiles128;  // cols in tiles of 128
     int tile_rows, row_tiles, n_tiles;
-    int steps, split, stages, stage_bytes, scales_off;
-    int code_bytes;  // that a step's copies of codes count, fill left out
+    int steps, split, stages, stage_bytes, x_off, x_piece;
+    int y_vec;       // rows of y start on 16 bytes
+    int code_bytes;  // that a step's copies count, fill left out
     uint32_t columns, scales_column, instruction;
 };
 
 struct Shared {
-    uint64_t full[kMostStages], empty[kMostStages], sums, drained, products_done;
+    uint64_t full[kMostStages], scaled[kMostStages], empty[kMostStages];
+    uint64_t sums, drained, products_done;
     uint32_t tmem;
-    int consumed;  // steps whose operands the issuer has waited for
+    int consumed;  // steps whose copies the issuer has waited for
 };
 
+// A bounded wait.  The clock is read once in kTries tries (%globaltimer takes about a
+// microsecond, as long as a step's products).
+__device__ __forceinline__ bool wait_one(uint64_t* bar, uint32_t parity, unsigned* status) {
+    constexpr int kTries = 256;
+    uint64_t t0 = 0;
+    for (;;) {
+        for (int i = 0; i < kTries; ++i)
+            if (tbk::mbar_try_wait(bar, parity)) return true;
+        const uint64_t now = tbk::global_ns();
+        if (t0 == 0) t0 = now;
+        if (now - t0 > kLimit) break;
+    }
+    atomicOr(status, tbk::kFlagTimeout);
+    return false;
+}
 __device__ __forceinline__ bool wait_all(uint64_t* bar, uint32_t parity, unsigned* status) {
-    const bool came = tbk::mbar_wait(bar, parity, status, 1000000000ull);
+    const bool came = wait_one(bar, parity, status);
     return __all_sync(tbk::kFull, came);
 }
 
+// `mine` in the shared memory of CTA `rank` of the cluster.
+__device__ __forceinline__ uint32_t peer(const void* mine, int rank) {
+    uint32_t at;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;"
+                 : "=r"(at)
+                 : "r"(tbk::smem_addr(mine)), "r"(rank));
+    return at;
+}
+// Arrive on the first CTA's barrier, with what this thread did before.
+__device__ __forceinline__ void arrive_first(uint64_t* bar) {
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(peer(bar, 0))
+                 : "memory");
+}
+// A tile to this CTA's shared memory; PAIR: counted on the first CTA's barrier.
+template <bool PAIR>
 __device__ __forceinline__ void tma_tile(void* dst, const CUtensorMap* map, int x, int y,
                                          uint64_t* bar) {
-    asm volatile(
-        "cp.async.bulk.tensor.3d.shared::cta.global.tile.mbarrier::complete_tx::bytes "
-        "[%0], [%1, {%2, %3, %4}], [%5];" ::"r"(tbk::smem_addr(dst)),
-        "l"(map), "r"(x), "r"(y), "r"(0), "r"(tbk::smem_addr(bar))
-        : "memory");
+    if constexpr (PAIR)
+        asm volatile(
+            "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.tile"
+            ".mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
+                tbk::smem_addr(dst)),
+            "l"(map), "r"(x), "r"(y), "r"(0), "r"(peer(bar, 0))
+            : "memory");
+    else
+        asm volatile(
+            "cp.async.bulk.tensor.3d.shared::cta.global.tile.mbarrier::complete_tx::bytes "
+            "[%0], [%1, {%2, %3, %4}], [%5];" ::"r"(tbk::smem_addr(dst)),
+            "l"(map), "r"(x), "r"(y), "r"(0), "r"(tbk::smem_addr(bar))
+            : "memory");
 }
 
 __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.release;\nbarrier.cluster.wait.acquire;" ::: "memory");
 }
-__device__ __forceinline__ float load_of(uint32_t smem, int rank) {
-    uint32_t at;
+__device__ __forceinline__ float load_of(const float* mine, int rank) {
     float v;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem), "r"(rank));
-    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(peer(mine, rank)) : "memory");
     return v;
 }
 
-// A tile of rows [row, row + n) and outs [out, out + 128).
+// A tile of n rows from `row` on and of outs from `out` on: the CTA's 128, or the pair's 256.
 struct Tile {
-    int out, row, n, scale_tiles;
+    int out, row, n;
 };
+template <bool PAIR>
 __device__ __forceinline__ Tile tile_of(const Args& a, int i) {
+    constexpr int kUnit = PAIR ? 32 : 16;  // the instruction's, half of it in each CTA
     Tile t;
-    t.out = i / a.row_tiles * kTileOuts;
+    t.out = i / a.row_tiles * (PAIR ? 2 * kOuts : kOuts);
     t.row = i % a.row_tiles * a.tile_rows;
-    t.n = min(a.tile_rows, (a.rows - t.row + 15) / 16 * 16);
-    t.scale_tiles = (t.n + 127) / 128;
+    t.n = min(a.tile_rows, (a.rows - t.row + kUnit - 1) / kUnit * kUnit);
     return t;
 }
 
-// BOTH4: both operands 4-bit, a step 256 columns; else 128.
-template <typename T, bool BOTH4>
-__global__ void __launch_bounds__(kThreads) k_linear(const __grid_constant__ Args a) {
-    constexpr int kScaleTiles = BOTH4 ? 2 : 1;  // of 4 blocks, a step
+template <typename T, int N>
+__device__ __forceinline__ void store_column(T* y, int64_t stride, int n, const float (&v)[N],
+                                             float bias) {
+#pragma unroll
+    for (int e = 0; e < N; ++e)
+        if (e < n) tbk::Elt<T>::store(y + e * stride, v[e] + bias);
+}
+
+// PAIR: two CTAs on a tile of 256 outs by up to 256 rows, one an SM; else up to 128 rows.
+template <bool BOTH4, bool PAIR>
+struct Shape {
+    static constexpr int kPieces = PAIR ? 2 : 1;
+    static constexpr int kStoreWarps = PAIR ? 8 : 4;
+    static constexpr int kScalers = kStorers + kStoreWarps;
+    static constexpr int kThreads = 32 * (kScalers + 4);
+    static constexpr int kTiles = (BOTH4 ? 2 : 1) * kPieces;  // of 128 columns, a step
+    static constexpr int kMostX = PAIR ? 2 : 1;               // x's tiles of 128 rows
+    static constexpr int kEach = (1 + kMostX) * kTiles;       // a step's tiles of scales
+    static constexpr int kScaleColumns = 4 * kEach;
+    static constexpr int kAhead = BOTH4 ? 4 : 8;  // steps' scales in shared memory
+    static constexpr int kScaleBytes = kAhead * kEach * mx::kTileBytes;
+    static constexpr int kStaged = PAIR ? 8192 : 0;  // bytes of y on their way
+};
+
+// BOTH4: both operands 4-bit, a piece 256 columns; else 128.
+template <typename T, bool BOTH4, bool PAIR>
+__global__ void __launch_bounds__(Shape<BOTH4, PAIR>::kThreads, PAIR ? 1 : 3)
+k_linear(const __grid_constant__ Args a) {
+    using H = Shape<BOTH4, PAIR>;
+    constexpr int kTiles = H::kTiles, kMostX = H::kMostX, kEach = H::kEach, kPieces = H::kPieces;
     extern __shared__ uint8_t smem_raw[];
     __shared__ Shared sh;
     uint8_t* smem = smem_raw + (-tbk::smem_addr(smem_raw) & 1023u);
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int rank = blockIdx.x % a.split;
-    const int first = (int)((int64_t)a.steps * rank / a.split);
-    const int last = (int)((int64_t)a.steps * (rank + 1) / a.split);
-    const int tile0 = blockIdx.x / a.split, tile_step = gridDim.x / a.split;
+    // (the same in all lanes, and known to be)
+    const int warp = __shfl_sync(tbk::kFull, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+    const int ctas = PAIR ? 2 : a.split, rank = blockIdx.x % ctas;
+    const int first = PAIR ? 0 : (int)((int64_t)a.steps * rank / ctas);
+    const int last = PAIR ? a.steps : (int)((int64_t)a.steps * (rank + 1) / ctas);
+    const int tile0 = blockIdx.x / ctas, tile_step = gridDim.x / ctas;
     const int mine = tile0 < a.n_tiles ? (a.n_tiles - 1 - tile0) / tile_step + 1 : 0;
     const int total = mine * (last - first);  // steps of this CTA
-    auto stage_at = [&](int stage) { return smem + stage * a.stage_bytes; };
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < a.stages; ++i) {
             tbk::mbar_init(&sh.full[i], 1);
+            tbk::mbar_init(&sh.scaled[i], PAIR ? 8 : 4);
             tbk::mbar_init(&sh.empty[i], 1);
         }
         tbk::mbar_init(&sh.sums, 1);
-        tbk::mbar_init(&sh.drained, kStoreWarps);
+        tbk::mbar_init(&sh.drained, (PAIR ? 2 : 1) * H::kStoreWarps);
         tbk::mbar_init(&sh.products_done, 1);
+        sh.consumed = 0;
         tbk::fence_mbar_init();
     }
-    if (warp == kIssuer) tc::allocate(&sh.tmem, a.columns);
+    if (warp == kIssuer) {
+        if constexpr (PAIR)
+            tc::allocate_pair(&sh.tmem, a.columns);
+        else
+            tc::allocate(&sh.tmem, a.columns);
+    }
     tc::fence_before();
     __syncthreads();
+    if (PAIR) cluster_sync();  // the other CTA's barriers are there
     tc::fence_after();
     const uint32_t tmem = sh.tmem;
 
     int issued = 0;
     bool fine = true;
     if (warp == kLoader) {
-        int stage = 0;
-        uint32_t parity = 1;  // of the round before
-        for (int i = 0; i < mine && fine; ++i) {
-            const Tile t = tile_of(a, tile0 + i * tile_step);
-            for (int j = first; j < last; ++j) {
-                if (issued >= a.stages) fine = wait_all(&sh.empty[stage], parity, a.status);
-                if (!fine) break;
-                if (lane == 0) {
-                    uint8_t* to = stage_at(stage);
+        if (lane == 0) {
+            int stage = 0;
+            uint32_t parity = 1;  // of the round before
+            for (int i = 0; i < mine && fine; ++i) {
+                const Tile t = tile_of<PAIR>(a, tile0 + i * tile_step);
+                const int out = t.out + (PAIR ? kOuts * rank : 0);
+                const int row = t.row + (PAIR ? t.n / 2 * rank : 0);
+                for (int j = first; j < last; ++j) {
+                    if (issued >= a.stages) fine = wait_one(&sh.empty[stage], parity, a.status);
+                    if (!fine) break;
+                    uint8_t* to = smem + stage * a.stage_bytes;
                     uint64_t* bar = &sh.full[stage];
-                    // (the last step of 256 columns may have 128)
-                    const int at = j * kScaleTiles;
-                    const int bytes = min(kScaleTiles, a.tiles128 - at) * mx::kTileBytes;
-                    tbk::mbar_expect_tx(bar, a.code_bytes + (1 + t.scale_tiles) * bytes);
-                    tma_tile(to, &a.w_map, j * 128, t.out, bar);
-                    tma_tile(to + kTileOuts * kStepBytes, &a.x_map, j * 128, t.row, bar);
-                    uint8_t* s = to + a.scales_off;
-                    tbk::bulk_g2s(s, a.w_scales + mx::scales_at(t.out, at, a.tiles128), bytes, bar);
-                    for (int k = 0; k < t.scale_tiles; ++k)
-                        tbk::bulk_g2s(s + (1 + k) * kScaleTiles * mx::kTileBytes,
-                                      a.x_scales + mx::scales_at(t.row + 128 * k, at, a.tiles128),
-                                      bytes, bar);
-                }
-                __syncwarp();
-                ++issued;
-                if (++stage == a.stages) {
-                    stage = 0;
-                    parity ^= 1;
-                }
-            }
-        }
-    } else if (warp == kIssuer) {
-        const bool leader = lane == 0;
-        const uint64_t w_desc = tc::tile_descriptor(tbk::smem_addr(smem), 16);
-        const uint64_t x_desc = w_desc + kTileOuts * kStepBytes / 16;
-        const uint32_t scales_s = tbk::smem_addr(smem) + a.scales_off;
-        const int scale_columns = (1 + (a.tile_rows + 127) / 128) * kScaleTiles * 4;
-        int stage = 0, done = 0;
-        uint32_t parity = 0;
-        for (int i = 0; i < mine && fine; ++i) {
-            const Tile t = tile_of(a, tile0 + i * tile_step);
-            const uint32_t instruction = tc::with_columns(a.instruction, t.n);
-            if (i > 0) fine = wait_all(&sh.drained, (i - 1) & 1, a.status);
-            tc::fence_after();
-            for (int j = first; j < last && fine; ++j) {
-                fine = wait_all(&sh.full[stage], parity, a.status);
-                if (!fine) break;
-                const uint32_t s = scales_s + stage * a.stage_bytes;
-                const uint32_t w_to = tmem + a.scales_column + stage * scale_columns;
-                const uint32_t x_to = w_to + kScaleTiles * 4;
-                const int have = min(kScaleTiles, a.tiles128 - j * kScaleTiles);
-                for (int h = 0; h < have; ++h) {
-                    tc::copy_scales(w_to + 4 * h, s + h * mx::kTileBytes, leader);
-                    // rows' tiles one after the other for each 4 blocks
-                    for (int k = 0; k < t.scale_tiles; ++k)
-                        tc::copy_scales(x_to + (h * t.scale_tiles + k) * 4,
-                                        s + ((1 + k) * kScaleTiles + h) * mx::kTileBytes, leader);
-                }
-                const uint64_t off = stage * (a.stage_bytes / 16);
+                    if (!PAIR || rank == 0)
+                        tbk::mbar_expect_tx(bar, (PAIR ? 2 : 1) * a.code_bytes);
 #pragma unroll
-                for (int m = 0; m < 4; ++m) {
-                    const int h = BOTH4 ? m / 2 : 0, block = BOTH4 ? m % 2 * 2 : m;
-                    if (h < have)
-                        tc::mma_scaled<BOTH4>(tmem, w_desc + off + 2 * m, x_desc + off + 2 * m,
-                                              tc::with_block(instruction, block), w_to + 4 * h,
-                                              x_to + h * t.scale_tiles * 4, j > first || m > 0,
-                                              leader);
-                }
-                if (done + a.stages < total) tc::commit(&sh.empty[stage], leader);
-                ++done;
-                if (++stage == a.stages) {
-                    stage = 0;
-                    parity ^= 1;
+                    for (int p = 0; p < kPieces; ++p) {
+                        const int x = (j * kPieces + p) * 128;  // (bytes, or 4-bit elements)
+                        tma_tile<PAIR>(to + p * kOuts * kPieceBytes, &a.w_map, x, out, bar);
+                        tma_tile<PAIR>(to + a.x_off + p * a.x_piece, &a.x_map, x, row, bar);
+                    }
+                    ++issued;
+                    if (++stage == a.stages) {
+                        stage = 0;
+                        parity ^= 1;
+                    }
                 }
             }
-            if (fine) tc::commit(&sh.sums, leader);
         }
-        if (lane == 0) sh.consumed = done;
-        // whatever ended the loop, no product may be in flight when tensor memory is freed
-        tc::commit(&sh.products_done, leader);
-        wait_all(&sh.products_done, 0, a.status);
+        __syncwarp();
+    } else if (warp == kIssuer) {
+        // A whole warp, one lane of which issues: operands stay in uniform registers (by one
+        // lane's branch a step took twice the time).
+        if (!PAIR || rank == 0) {
+            const bool leader = lane == 0;
+            auto commit = [&](uint64_t* bar) {
+                if constexpr (PAIR)
+                    tc::commit_pair(bar, leader);
+                else
+                    tc::commit(bar, leader);
+            };
+            const uint64_t w_desc = tc::tile_descriptor(tbk::smem_addr(smem), 16);
+            const uint32_t x_off = a.x_off / 16, x_piece = a.x_piece / 16;
+            int stage = 0, done = 0, consumed = 0;
+            uint32_t parity = 0;
+            for (int i = 0; i < mine && fine; ++i) {
+                const Tile t = tile_of<PAIR>(a, tile0 + i * tile_step);
+                const uint32_t instruction = tc::with_columns(a.instruction, t.n);
+                if (i > 0) fine = wait_all(&sh.drained, (i - 1) & 1, a.status);
+                tc::fence_after();
+                for (int j = first; j < last && fine; ++j) {
+                    fine = wait_all(&sh.full[stage], parity, a.status);
+                    if (fine) ++consumed;
+                    fine = fine && wait_all(&sh.scaled[stage], parity, a.status);
+                    if (!fine) break;
+                    tc::fence_after();
+                    const uint32_t w_scales = tmem + a.scales_column + stage * H::kScaleColumns;
+                    const uint32_t x_scales = w_scales + 4 * kTiles;
+                    const uint64_t w = w_desc + (uint32_t)(stage * (a.stage_bytes / 16));
+                    const int have = a.tiles128 - j * kTiles;  // the last step may have less
+#pragma unroll
+                    for (int p = 0; p < kPieces; ++p)
+#pragma unroll
+                        for (int m = 0; m < 4; ++m) {
+                            const int h = BOTH4 ? 2 * p + m / 2 : p, block = BOTH4 ? m % 2 * 2 : m;
+                            if (h == 0 || h < have)
+                                tc::mma_scaled<BOTH4, PAIR>(
+                                    tmem, w + p * (kOuts * kPieceBytes / 16) + 2 * m,
+                                    w + x_off + p * x_piece + 2 * m,
+                                    tc::with_block(instruction, block), w_scales + 4 * h,
+                                    x_scales + 4 * kMostX * h, j > first || p + m > 0, leader);
+                        }
+                    if (done + a.stages < total) commit(&sh.empty[stage]);
+                    ++done;
+                    if (++stage == a.stages) {
+                        stage = 0;
+                        parity ^= 1;
+                    }
+                }
+                if (fine) commit(&sh.sums);
+            }
+            if (leader) sh.consumed = consumed;
+            // whatever ended the loop, no product may be in flight when tensor memory is freed
+            commit(&sh.products_done);
+            wait_all(&sh.products_done, 0, a.status);
+        }
+    } else if (warp >= H::kScalers) {
+        // Scales to shared memory, kAhead - 1 steps ahead, by all four warps; from there each
+        // brings all of them to its quarter of the rows of tensor memory, a lane the words of
+        // rows l, l + 32, l + 64 and l + 96.
+        constexpr int kAhead = H::kAhead, kChunks = kEach * 32;
+        const uint32_t to = tmem + a.scales_column + ((uint32_t)(warp % 4) << 21);
+        const int thread = threadIdx.x - 32 * H::kScalers;
+        uint4* ring = reinterpret_cast<uint4*>(smem + a.stages * a.stage_bytes);
+        int ask_tile = 0, ask_step = first, ask_slot = 0;  // the next step that is asked for
+        auto ask = [&] {
+            if (ask_tile < mine) {
+                const Tile t = tile_of<PAIR>(a, tile0 + ask_tile * tile_step);
+                const int out = t.out + (PAIR ? kOuts * rank : 0);
+#pragma unroll
+                for (int i = 0; i < (kChunks + 127) / 128; ++i) {
+                    const int c = thread + 128 * i, tile = c / 32, x = tile - kTiles;
+                    const int h = x < 0 ? tile : x / kMostX, at = ask_step * kTiles + h;
+                    const int row = x < 0 ? out : t.row + 128 * (x % kMostX);
+                    if (c < kChunks && at < a.tiles128 && row < (x < 0 ? a.outs : a.rows)) {
+                        const uint8_t* from = (x < 0 ? a.w_scales : a.x_scales) +
+                                              mx::scales_at(row, at, a.tiles128) + c % 32 * 16;
+                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(
+                                         tbk::smem_addr(ring + ask_slot * kChunks + c)),
+                                     "l"(from)
+                                     : "memory");
+                    }
+                }
+                if (++ask_step == last) {
+                    ask_step = first;
+                    ++ask_tile;
+                }
+            }
+            asm volatile("cp.async.commit_group;" ::: "memory");
+            if (++ask_slot == kAhead) ask_slot = 0;
+        };
+#pragma unroll 1
+        for (int i = 0; i < kAhead - 1; ++i) ask();
+        int stage = 0, slot = 0;
+        uint32_t parity = 1;  // of the round before
+        for (int done = 0; done < total; ++done) {
+            asm volatile("cp.async.wait_group %0;" ::"n"(kAhead - 2) : "memory");
+            // this step's are there, and the step before's have been taken by all
+            asm volatile("bar.sync 1, 128;" ::: "memory");
+            ask();
+            uint4 r[kEach];
+#pragma unroll
+            for (int i = 0; i < kEach; ++i) r[i] = ring[slot * kChunks + i * 32 + lane];
+            if (done >= a.stages) {
+                if (fine) fine = wait_all(&sh.empty[stage], parity, a.status);
+            }
+            if (fine) {  // (a warp that gave up still comes to the barrier above)
+                tc::fence_after();
+                const uint32_t at = to + stage * H::kScaleColumns;
+#pragma unroll
+                for (int i = 0; i < kEach; ++i) tc::store_scales(at + 4 * i, r[i]);
+                tc::wait_store();
+                tc::fence_before();
+                __syncwarp();
+                if (lane == 0) {
+                    if (PAIR)
+                        arrive_first(&sh.scaled[stage]);
+                    else
+                        tbk::mbar_arrive(&sh.scaled[stage]);
+                }
+            }
+            if (++slot == kAhead) slot = 0;
+            if (++stage == a.stages) {
+                stage = 0;
+                parity ^= 1;
+            }
+        }
+        asm volatile("cp.async.wait_all;" ::: "memory");
     } else {
         const int quarter = warp % 4;
         const uint32_t sums = tmem + ((uint32_t)quarter << 21);
         float* part = reinterpret_cast<float*>(smem);  // split: [row][out]
         for (int i = 0; i < mine; ++i) {
-            const Tile t = tile_of(a, tile0 + i * tile_step);
-            fine = wait_all(&sh.sums, i & 1, a.status);
-            if (!fine) break;
+            const Tile t = tile_of<PAIR>(a, tile0 + i * tile_step);
+            if (fine) fine = wait_all(&sh.sums, i & 1, a.status);
+            if (!fine && !PAIR) break;  // (a pair's warps still come to the barriers below)
             tc::fence_after();
-            const int out = t.out + 32 * quarter + lane;
+            const int out = t.out + (PAIR ? kOuts * rank : 0) + 32 * quarter + lane;
             const float bias = a.bias && out < a.outs ? a.bias[out] : 0.0f;
+            const int n = out < a.outs ? min(a.rows - t.row, t.n) : 0;
             T* y = static_cast<T*>(a.y) + (int64_t)t.row * a.y_stride + out;
-            for (int c = 0; c < t.n; c += 32) {
-                float v[32];
-                tc::load<32>(sums + c, v);
-                if (a.split > 1) {
-#pragma unroll
-                    for (int e = 0; e < 32; ++e)
-                        if (c + e < t.n) part[(c + e) * kTileOuts + 32 * quarter + lane] = v[e];
-                } else if (out < a.outs) {
-                    const int n = min(a.rows - t.row, t.n) - c;
-#pragma unroll
-                    for (int e = 0; e < 32; ++e)
-                        if (e < n) tbk::Elt<T>::store(y + (c + e) * a.y_stride, v[e] + bias);
+            auto release = [&] {  // tensor memory may take the next tile's sums
+                tc::fence_before();
+                __syncwarp();
+                if (lane == 0 && i + 1 < mine) {
+                    if (PAIR)
+                        arrive_first(&sh.drained);
+                    else
+                        tbk::mbar_arrive(&sh.drained);
                 }
+            };
+            if constexpr (PAIR) {
+                // half of the rows each of two warps, in registers before any is stored; then
+                // through shared memory, for whole rows of the CTA's outs to be stored at once
+                constexpr int kRows = H::kStaged / 2 / (kOuts * sizeof(T));  // of each half
+                constexpr int kVec = 16 / sizeof(T), kPer = kOuts / kVec;    // pieces of a row
+                const int half = (warp - kStorers) / 4, c = half * 128;
+                const int thread = threadIdx.x - 32 * kStorers;
+                T* staged = reinterpret_cast<T*>(smem + a.stages * a.stage_bytes + H::kScaleBytes);
+                T* y0 = static_cast<T*>(a.y) + (int64_t)t.row * a.y_stride + t.out + kOuts * rank;
+                const int outs = a.outs - t.out - kOuts * rank, rows = min(a.rows - t.row, t.n);
+                float v[128];
+                if (c < t.n) tc::load<128>(sums + c, v);
+                if (fine) release();
+#pragma unroll
+                for (int g = 0; g < 128; g += kRows) {
+                    if (g >= t.n) break;
+#pragma unroll
+                    for (int e = 0; e < kRows; ++e)
+                        tbk::Elt<T>::store(staged + (half * kRows + e) * kOuts + 32 * quarter + lane,
+                                           v[g + e] + bias);
+                    asm volatile("bar.sync 2, 256;" ::: "memory");
+#pragma unroll
+                    for (int k = 0; k < 2 * kRows * kPer / 256; ++k) {
+                        const int i = thread + 256 * k, r = i / kPer, o = i % kPer * kVec;
+                        const int row = r / kRows * 128 + g + r % kRows;
+                        if (row >= rows || o >= outs) continue;
+                        const T* from = staged + r * kOuts + o;
+                        T* to = y0 + (int64_t)row * a.y_stride + o;
+                        if (a.y_vec && o + kVec <= outs) {
+                            *reinterpret_cast<uint4*>(to) = *reinterpret_cast<const uint4*>(from);
+                        } else {
+                            for (int e = 0; e < kVec && o + e < outs; ++e) to[e] = from[e];
+                        }
+                    }
+                    asm volatile("bar.sync 2, 256;" ::: "memory");
+                }
+            } else {
+                for (int c = 0; c < t.n; c += 32) {
+                    float v[32];
+                    tc::load<32>(sums + c, v);
+                    if (a.split > 1) {
+#pragma unroll
+                        for (int e = 0; e < 32; ++e)
+                            if (c + e < t.n) part[(c + e) * kOuts + 32 * quarter + lane] = v[e];
+                    } else {
+                        store_column(y + c * a.y_stride, a.y_stride, n - c, v, bias);
+                    }
+                }
+                release();
             }
-            tc::fence_before();
-            __syncwarp();
-            if (lane == 0 && i + 1 < mine) tbk::mbar_arrive(&sh.drained);
         }
     }
     tc::fence_before();
     const bool lost = __syncthreads_or(!fine);
-    if (warp == kLoader && lost) {
-        // no copy may be in flight when the CTA ends: those that nobody waited for
+    if (warp == kLoader && lane == 0 && lost && (!PAIR || rank == 0)) {
+        // no copy may be in flight when the CTA ends: those that nobody waited for (a pair's
+        // other CTA is behind the barrier below until then)
         for (int j = sh.consumed; j < issued; ++j)
-            wait_all(&sh.full[j % a.stages], (uint32_t)(j / a.stages) & 1u, a.status);
+            wait_one(&sh.full[j % a.stages], (uint32_t)(j / a.stages) & 1u, a.status);
+    }
+    __syncwarp();
+    if constexpr (PAIR) {
+        // (the first CTA's last arrival comes here too)
+        if (warp == kIssuer && rank == 1) wait_all(&sh.products_done, 0, a.status);
+        cluster_sync();  // no product reads the other's shared memory any more
+        if (warp == kIssuer) tc::release_pair(tmem, a.columns);
+        return;
     }
     if (warp == kIssuer) tc::release(tmem, a.columns);
     if (a.split > 1) {
         cluster_sync();
-        if (warp >= 2) {
-            const Tile t = tile_of(a, tile0);
-            const int quarter = warp % 4, out = t.out + 32 * quarter + lane;
+        if (warp >= kStorers && warp < H::kScalers) {
+            const Tile t = tile_of<PAIR>(a, tile0);
+            const int at = warp % 4 * 32 + lane, out = t.out + at;
             if (out < a.outs) {
                 const float bias = a.bias ? a.bias[out] : 0.0f;
                 const int n = min(a.rows - t.row, t.n);
+                const float* part = reinterpret_cast<const float*>(smem) + at;
                 for (int c = rank; c < n; c += a.split) {
-                    const uint32_t at =
-                        tbk::smem_addr(smem) + (c * kTileOuts + 32 * quarter + lane) * 4;
                     float sum = 0.0f;
-                    for (int k = 0; k < a.split; ++k) sum += load_of(at, k);
+                    for (int k = 0; k < a.split; ++k) sum += load_of(part + c * kOuts, k);
                     tbk::Elt<T>::store(static_cast<T*>(a.y) + (t.row + c) * a.y_stride + out,
                                        sum + bias);
                 }
@@ -258,52 +461,52 @@ __global__ void __launch_bounds__(kThreads) k_linear(const __grid_constant__ Arg
 }
 
 struct Plan {
-    int tile_rows, row_tiles, n_tiles, steps, split, stages, stage_bytes, scales_off, bytes, ctas;
+    bool pair;
+    int tile_rows, row_tiles, n_tiles, steps, split, stages, stage_bytes, bytes, ctas;
+    int x_rows;  // that a CTA loads
     uint32_t columns, scales_column;
 };
 
 int plan_of(Plan& p, const TbB200Mx* x, const TbB200Mx* w, bool both4, int sm_count) {
     const int64_t tiles128 = mx::tiles_of(x->cols);
-    p.tile_rows = x->rows >= kMostRows ? kMostRows : (int)((x->rows + 15) / 16 * 16);
+    p.pair = x->rows > 128;
+    const int pieces = p.pair ? 2 : 1, step_tiles = (both4 ? 2 : 1) * pieces;
+    p.steps = (int)((tiles128 + step_tiles - 1) / step_tiles);
+    p.tile_rows = p.pair ? 256 : (int)((x->rows + 15) / 16 * 16);
+    p.x_rows = p.pair ? 128 : p.tile_rows;
     p.row_tiles = (int)((x->rows + p.tile_rows - 1) / p.tile_rows);
-    const int64_t n_tiles = (w->rows + kTileOuts - 1) / kTileOuts * p.row_tiles;
+    const int outs = p.pair ? 2 * kOuts : kOuts;
+    const int64_t n_tiles = (w->rows + outs - 1) / outs * p.row_tiles;
     if (n_tiles * kMostSplit > INT32_MAX) return TB_ERR_INVALID_SHAPE;
     p.n_tiles = (int)n_tiles;
-    p.steps = (int)(both4 ? (tiles128 + 1) / 2 : tiles128);
-    const int scale_tiles = (1 + (p.tile_rows + 127) / 128) * (both4 ? 2 : 1);
-    p.scales_off = (kTileOuts + p.tile_rows) * kStepBytes;
-    p.stage_bytes = p.scales_off + (scale_tiles * mx::kTileBytes + 1023) / 1024 * 1024;
-    const int per_sm = p.tile_rows <= 64 ? 2 : 1;
-    const int budget = (per_sm == 2 ? 112 : 224) * 1024;
-    p.stages = (budget - 1024) / p.stage_bytes;
+    p.stage_bytes = pieces * (kOuts + p.x_rows) * kPieceBytes;
+    // as many CTAs an SM as keep four stages each
+    const int beside = (p.pair ? Shape<false, true>::kScaleBytes + Shape<false, true>::kStaged
+                               : Shape<false, false>::kScaleBytes) + 1024;
+    const int per_sm = p.pair ? 1 : p.tile_rows <= 32 ? 3 : p.tile_rows <= 64 ? 2 : 1;
+    p.stages = (226 * 1024 / per_sm - 1024 - beside) / p.stage_bytes;
     if (p.stages > kMostStages) p.stages = kMostStages;
     p.scales_column = (uint32_t)(p.tile_rows + 31) / 32 * 32;
-    const uint32_t need = p.scales_column + p.stages * scale_tiles * 4;
+    const int scale_columns = (p.pair ? 12 : 8) * step_tiles;
+    const uint32_t need = p.scales_column + p.stages * scale_columns;
     for (p.columns = 32; p.columns < need;) p.columns *= 2;
-    const int slots = sm_count * per_sm;
-    // parts of cols: rounds of CTAs by what each takes, a tile's fixed cost as 8 steps
+    const int slots = p.pair ? sm_count / 2 : sm_count * per_sm;
+    // parts of cols where the tiles leave SMs idle, 4 steps each at least
     p.split = 1;
-    int64_t best = INT64_MAX;
-    for (int s = 1; s <= kMostSplit; s *= 2) {
-        if (s > 1 && (p.steps < 2 * s || p.tile_rows * kTileOuts * 4 > p.stages * p.stage_bytes))
-            break;
-        const int64_t rounds = (n_tiles * s + slots - 1) / slots;
-        const int64_t cost = rounds * ((p.steps + s - 1) / s + 8);
-        if (cost < best) {
-            best = cost;
-            p.split = s;
-        }
-    }
+    while (!p.pair && p.split < kMostSplit && n_tiles * p.split * 2 <= slots &&
+           p.steps >= 8 * p.split && p.tile_rows * kOuts * 4 <= p.stages * p.stage_bytes)
+        p.split *= 2;
     p.ctas = p.split > 1 ? p.n_tiles * p.split : p.n_tiles < slots ? p.n_tiles : slots;
-    p.bytes = p.stages * p.stage_bytes + 1024;
+    if (p.pair) p.ctas *= 2;
+    p.bytes = p.stages * p.stage_bytes + beside;
     return TB_OK;
 }
 
-// Rows of 128 bytes of codes a step: packed, or with fill beside 8-bit codes.
+// Pieces of `rows` rows, 128 bytes of codes each: packed, or with fill beside 8-bit codes.
 int map_of(CUtensorMap* map, const TbB200Mx* t, int rows, bool packed) {
     const uint64_t pitch = (uint64_t)mx::pitch_of(t->format, t->cols);
     const uint64_t strides[2] = {pitch, pitch * (uint64_t)t->rows};
-    const uint32_t box[3] = {128, (uint32_t)rows, 1};
+    const uint32_t box[3] = {kPieceBytes, (uint32_t)rows, 1};
     if (t->format == mx::kE2m1 && !packed) {
         const uint64_t dims[3] = {2 * pitch, (uint64_t)t->rows, 1};
         return tbh::encode_tiles_u4(map, t->codes, dims, strides, box, 128);
@@ -312,30 +515,36 @@ int map_of(CUtensorMap* map, const TbB200Mx* t, int rows, bool packed) {
     return tbh::encode_tiles_u8(map, t->codes, dims, strides, box, 128);
 }
 
-template <typename T, bool BOTH4>
+template <typename T, bool BOTH4, bool PAIR>
 int launch(const Args& a, const Plan& p, cudaStream_t s) {
     static std::atomic<uint64_t> granted{0};  // a bit per device
     const tbh::DeviceState* ds = tbh::current_device_state();
     if (!ds) return TB_ERR_DEVICE;
     if (!(granted.load() >> ds->device & 1)) {
-        TB_CUDA_TRY(cudaFuncSetAttribute(k_linear<T, BOTH4>,
-                                         cudaFuncAttributeMaxDynamicSharedMemorySize, 224 * 1024));
+        TB_CUDA_TRY(cudaFuncSetAttribute(k_linear<T, BOTH4, PAIR>,
+                                         cudaFuncAttributeMaxDynamicSharedMemorySize, 226 * 1024));
         granted.fetch_or(1ull << ds->device);
     }
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)p.ctas);
-    cfg.blockDim = dim3(kThreads);
+    cfg.blockDim = dim3(Shape<BOTH4, PAIR>::kThreads);
     cfg.dynamicSmemBytes = (size_t)p.bytes;
     cfg.stream = s;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = (unsigned)p.split;
+    attr[0].val.clusterDim.x = (unsigned)(PAIR ? 2 : p.split);
     attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    TB_CUDA_TRY(cudaLaunchKernelEx(&cfg, k_linear<T, BOTH4>, a));
+    TB_CUDA_TRY(cudaLaunchKernelEx(&cfg, k_linear<T, BOTH4, PAIR>, a));
     TB_LAUNCH_CHECK("microscaled product kernel");
     return TB_OK;
+}
+
+template <typename T>
+int launch_by(const Args& a, const Plan& p, bool both4, cudaStream_t s) {
+    if (p.pair) return both4 ? launch<T, true, true>(a, p, s) : launch<T, false, true>(a, p, s);
+    return both4 ? launch<T, true, false>(a, p, s) : launch<T, false, false>(a, p, s);
 }
 
 tc::Element element(int format) { return format == mx::kE4m3 ? tc::kE4m3 : tc::kE2m1; }
@@ -358,14 +567,15 @@ extern "C" int tb_b200_mx_linear(const TbB200Mx* x, const TbB200Mx* w, const flo
     rc = plan_of(p, x, w, both4, ds->sm_count);
     if (rc != TB_OK) return rc;
     Args a = {};
-    rc = map_of(&a.w_map, w, kTileOuts, both4);
-    if (rc == TB_OK) rc = map_of(&a.x_map, x, p.tile_rows, both4);
+    rc = map_of(&a.w_map, w, kOuts, both4);
+    if (rc == TB_OK) rc = map_of(&a.x_map, x, p.x_rows, both4);
     if (rc != TB_OK) return rc;
     a.w_scales = w->scales;
     a.x_scales = x->scales;
     a.bias = bias;
     a.y = y;
     a.y_stride = y_stride;
+    a.y_vec = tbh::aligned16(y) && y_stride * (out_dtype == TB_DTYPE_F32 ? 4 : 2) % 16 == 0;
     a.status = ds->status;
     a.rows = (int)x->rows;
     a.outs = (int)w->rows;
@@ -377,15 +587,17 @@ extern "C" int tb_b200_mx_linear(const TbB200Mx* x, const TbB200Mx* w, const flo
     a.split = p.split;
     a.stages = p.stages;
     a.stage_bytes = p.stage_bytes;
-    a.scales_off = p.scales_off;
-    a.code_bytes = (kTileOuts >> (w->format == mx::kE2m1 && !both4)) * kStepBytes +
-                   (p.tile_rows * kStepBytes >> (x->format == mx::kE2m1 && !both4));
+    const int pieces = p.pair ? 2 : 1;
+    a.x_off = pieces * kOuts * kPieceBytes;
+    a.x_piece = p.x_rows * kPieceBytes;
+    a.code_bytes = pieces * ((kOuts * kPieceBytes >> (w->format == mx::kE2m1 && !both4)) +
+                              (p.x_rows * kPieceBytes >> (x->format == mx::kE2m1 && !both4)));
     a.columns = p.columns;
     a.scales_column = p.scales_column;
-    a.instruction = both4 ? tc::scaled_instruction_4bit()
-                          : tc::scaled_instruction(element(w->format), element(x->format));
+    const int m = p.pair ? 2 * kOuts : kOuts;
+    a.instruction = both4 ? tc::scaled_instruction_4bit(m)
+                          : tc::scaled_instruction(element(w->format), element(x->format), m);
     cudaStream_t s = tbh::stream_of(stream);
-    if (out_dtype == TB_DTYPE_F32)
-        return both4 ? launch<float, true>(a, p, s) : launch<float, false>(a, p, s);
-    return both4 ? launch<__nv_bfloat16, true>(a, p, s) : launch<__nv_bfloat16, false>(a, p, s);
+    return out_dtype == TB_DTYPE_F32 ? launch_by<float>(a, p, both4, s)
+                                     : launch_by<__nv_bfloat16>(a, p, both4, s);
 }

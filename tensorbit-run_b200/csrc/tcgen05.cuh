@@ -142,13 +142,13 @@ __device__ __forceinline__ void store16(uint32_t address, const uint32_t (&r)[16
 // and 4 blocks of 32 elements have 4 columns of tensor memory: row r in lane r % 32 of every
 // 32, column r / 32, a byte a block.
 enum Element { kE4m3 = 0, kE2m1 = 5 };
-// M = 128, f32 sums, E8M0 scales; less the number of columns and the block (of 4) that the
-// instruction starts with.
-constexpr uint32_t scaled_instruction(Element a, Element b) {
-    return (uint32_t)a << 7 | (uint32_t)b << 10 | 1u << 23 | (uint32_t)(128 / 16) << 24;
+// M = 128, or 256 of a pair of CTAs; f32 sums, E8M0 scales; less the number of columns and the
+// block (of 4) that the instruction starts with.
+constexpr uint32_t scaled_instruction(Element a, Element b, int m) {
+    return (uint32_t)a << 7 | (uint32_t)b << 10 | 1u << 23 | (uint32_t)(m / 16) << 24;
 }
-constexpr uint32_t scaled_instruction_4bit() {
-    return 1u << 7 | 1u << 10 | 1u << 23 | (uint32_t)(128 / 16) << 24;
+constexpr uint32_t scaled_instruction_4bit(int m) {
+    return 1u << 7 | 1u << 10 | 1u << 23 | (uint32_t)(m / 16) << 24;
 }
 __device__ __forceinline__ uint32_t with_columns(uint32_t instruction, int n) {
     return instruction | (uint32_t)(n / 8) << 17;
@@ -156,40 +156,59 @@ __device__ __forceinline__ uint32_t with_columns(uint32_t instruction, int n) {
 __device__ __forceinline__ uint32_t with_block(uint32_t instruction, int block) {
     return instruction | (uint32_t)block << 4 | (uint32_t)block << 29;
 }
-// d (tensor memory) = a b, or += if `add`; the scales of a and b in tensor memory.
-template <bool BOTH4>
+// d (tensor memory) = a b, or += if `add`; the scales of a and b in tensor memory.  PAIR: by
+// the first CTA of two, for both: each has half of a's rows, their scales and sums, half of
+// b's rows, and the scales of all of those, at the same addresses.
+#define TC_MMA_SCALED(group, kind)                                                          \
+    asm volatile("{\n .reg .pred p, q;\n setp.ne.u32 p, %6, 0;\n setp.ne.u32 q, %7, 0;\n" \
+                 " @q tcgen05.mma.cta_group::" group ".kind::" kind                         \
+                 " [%0], %1, %2, %3, [%4], [%5], p;\n}" ::"r"(d),                           \
+                 "l"(a), "l"(b), "r"(instruction), "r"(a_scales), "r"(b_scales),            \
+                 "r"((uint32_t)add), "r"((uint32_t)leader)                                  \
+                 : "memory")
+template <bool BOTH4, bool PAIR>
 __device__ __forceinline__ void mma_scaled(uint32_t d, uint64_t a, uint64_t b, uint32_t instruction,
                                            uint32_t a_scales, uint32_t b_scales, bool add,
                                            bool leader) {
-    if constexpr (BOTH4)
-        asm volatile(
-            "{\n .reg .pred p, q;\n setp.ne.u32 p, %6, 0;\n setp.ne.u32 q, %7, 0;\n"
-            " @q tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X "
-            "[%0], %1, %2, %3, [%4], [%5], p;\n}" ::"r"(d),
-            "l"(a), "l"(b), "r"(instruction), "r"(a_scales), "r"(b_scales), "r"((uint32_t)add),
-            "r"((uint32_t)leader)
-            : "memory");
+    if constexpr (BOTH4 && PAIR)
+        TC_MMA_SCALED("2", "mxf4.block_scale.scale_vec::2X");
+    else if constexpr (BOTH4)
+        TC_MMA_SCALED("1", "mxf4.block_scale.scale_vec::2X");
+    else if constexpr (PAIR)
+        TC_MMA_SCALED("2", "mxf8f6f4.block_scale.scale_vec::1X");
     else
-        asm volatile(
-            "{\n .reg .pred p, q;\n setp.ne.u32 p, %6, 0;\n setp.ne.u32 q, %7, 0;\n"
-            " @q tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X "
-            "[%0], %1, %2, %3, [%4], [%5], p;\n}" ::"r"(d),
-            "l"(a), "l"(b), "r"(instruction), "r"(a_scales), "r"(b_scales), "r"((uint32_t)add),
-            "r"((uint32_t)leader)
-            : "memory");
+        TC_MMA_SCALED("1", "mxf8f6f4.block_scale.scale_vec::1X");
 }
-// 512 bytes of scales in shared memory (32 rows of 16 bytes, on 16 bytes) to 4 columns of
-// tensor memory, in every 32 lanes; products issued after it by the same thread see them.
-__device__ __forceinline__ void copy_scales(uint32_t to, uint32_t smem, bool leader) {
-    const uint64_t from = (uint64_t)((smem >> 4) & 0x3fff) |  // start
-                          (uint64_t)(128 >> 4) << 16 |        // leading dimension: one wide
-                          (uint64_t)(128 >> 4) << 32 |        // 8 rows further
-                          1ull << 46;                         // the version; no swizzle
+#undef TC_MMA_SCALED
+// Arrive on bar of both CTAs of a pair when the products issued so far are done.
+__device__ __forceinline__ void commit_pair(uint64_t* bar, bool leader) {
     asm volatile(
         "{\n .reg .pred q;\n setp.ne.u32 q, %2, 0;\n"
-        " @q tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;\n}" ::"r"(to),
-        "l"(from), "r"((uint32_t)leader)
+        " @q tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster"
+        ".multicast::cluster.b64 [%0], %1;\n}" ::"r"(tbk::smem_addr(bar)),
+        "h"((uint16_t)3), "r"((uint32_t)leader)
         : "memory");
+}
+// Tensor memory of a pair of CTAs: allocate and release for both, a warp of each.
+__device__ __forceinline__ void allocate_pair(uint32_t* smem_out, uint32_t columns) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                     tbk::smem_addr(smem_out)),
+                 "r"(columns)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void release_pair(uint32_t address, uint32_t columns) {
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(address),
+                 "r"(columns)
+                 : "memory");
+}
+// Four columns of the warp's 32 rows, a row a lane: the scales of 128 rows and 4 blocks, of
+// which lane l has the words of rows l, l + 32, l + 64 and l + 96 (every quarter of the rows
+// has them all).
+__device__ __forceinline__ void store_scales(uint32_t address, const uint4& r) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1,%2,%3,%4};" ::"r"(address),
+                 "r"(r.x), "r"(r.y), "r"(r.z), "r"(r.w)
+                 : "memory");
 }
 
 // The warpgroup's registers per thread; the shares add up to the launch's.
