@@ -4,9 +4,9 @@
 // w is the left operand: a tile is 128 outs by up to 256 rows of x, its sums in tensor memory
 // as [out][row].  So a single row of x is as good a tile as many (the instruction takes 16
 // columns at least), and w, the larger side in serving, is read once for up to 256 rows.
-// One warp asks for operands by TMA, four bring scales from global memory through registers
-// to tensor memory (a lane 16 bytes, no step of their way through shared memory or the tensor
-// pipe), one issues the products, four bring a tile's sums to y, a lane an out.  Where the tiles do not
+// One warp asks for operands by TMA, one for scales, further ahead, and copies them to tensor
+// memory (stores from registers to there waited for the products: 1700 clocks a step), one
+// issues the products, four or eight bring a tile's sums to y, a lane an out.  Where the tiles do not
 // fill the SMs, the CTAs of a cluster take parts of cols and add them up, in order, through
 // one another's shared memory.
 #include <atomic>
@@ -18,9 +18,9 @@
 
 namespace {
 
-// warps; of the others kStoreWarps store and 4 bring scales
-constexpr int kLoader = 0, kIssuer = 1, kStorers = 2;
-constexpr int kOuts = 128, kMostStages = 12, kMostSplit = 8;  // kOuts: of a CTA's tile
+// warps; the others store
+constexpr int kLoader = 0, kIssuer = 1, kScaler = 2, kStorers = 3;
+constexpr int kOuts = 128, kMostStages = 8, kMostAhead = 8, kMostSplit = 8;  // kOuts: of a CTA's tile
 constexpr int kPieceBytes = 128;  // of a row of codes; a step has one or two such pieces
 constexpr uint64_t kLimit = 1000000000ull;  // ns, of a wait
 
@@ -41,7 +41,9 @@ struct Args {
 
 struct Shared {
     uint64_t full[kMostStages], scaled[kMostStages], empty[kMostStages];
-    uint64_t sums, drained, products_done;
+    uint64_t other[kMostStages];  // the pair's other CTA has the step's scales
+    uint64_t asked[kMostAhead];   // a step's scales, to shared memory
+    uint64_t sums, drained, products_done, scales_done;
     uint32_t tmem;
     int consumed;  // steps whose copies the issuer has waited for
 };
@@ -134,13 +136,13 @@ template <bool BOTH4, bool PAIR>
 struct Shape {
     static constexpr int kPieces = PAIR ? 2 : 1;
     static constexpr int kStoreWarps = PAIR ? 8 : 4;
-    static constexpr int kScalers = kStorers + kStoreWarps;
-    static constexpr int kThreads = 32 * (kScalers + 4);
+    static constexpr int kThreads = 32 * (kStorers + kStoreWarps);
     static constexpr int kTiles = (BOTH4 ? 2 : 1) * kPieces;  // of 128 columns, a step
     static constexpr int kMostX = PAIR ? 2 : 1;               // x's tiles of 128 rows
     static constexpr int kEach = (1 + kMostX) * kTiles;       // a step's tiles of scales
     static constexpr int kScaleColumns = 4 * kEach;
-    static constexpr int kAhead = BOTH4 ? 4 : 8;  // steps' scales in shared memory
+    static constexpr int kAhead = PAIR && BOTH4 ? 4 : 8;  // steps' scales asked for
+    static_assert(kAhead >= (PAIR ? 3 : kMostStages), "a stage's scales are asked for before it is taken");
     static constexpr int kScaleBytes = kAhead * kEach * mx::kTileBytes;
     static constexpr int kStaged = PAIR ? 8192 : 0;  // bytes of y on their way
 };
@@ -166,9 +168,12 @@ k_linear(const __grid_constant__ Args a) {
     if (threadIdx.x == 0) {
         for (int i = 0; i < a.stages; ++i) {
             tbk::mbar_init(&sh.full[i], 1);
-            tbk::mbar_init(&sh.scaled[i], PAIR ? 8 : 4);
+            tbk::mbar_init(&sh.scaled[i], 1);
             tbk::mbar_init(&sh.empty[i], 1);
+            tbk::mbar_init(&sh.other[i], 1);
         }
+        for (int i = 0; i < H::kAhead; ++i) tbk::mbar_init(&sh.asked[i], 1);
+        tbk::mbar_init(&sh.scales_done, 1);
         tbk::mbar_init(&sh.sums, 1);
         tbk::mbar_init(&sh.drained, (PAIR ? 2 : 1) * H::kStoreWarps);
         tbk::mbar_init(&sh.products_done, 1);
@@ -187,7 +192,13 @@ k_linear(const __grid_constant__ Args a) {
     tc::fence_after();
     const uint32_t tmem = sh.tmem;
 
-    int issued = 0;
+    auto commit = [&](uint64_t* bar, bool leader) {
+        if constexpr (PAIR)
+            tc::commit_pair(bar, leader);
+        else
+            tc::commit(bar, leader);
+    };
+    int issued = 0, taken = 0;  // the loader's steps; the scaler's, asked for and taken
     bool fine = true;
     if (warp == kLoader) {
         if (lane == 0) {
@@ -224,12 +235,6 @@ k_linear(const __grid_constant__ Args a) {
         // lane's branch a step took twice the time).
         if (!PAIR || rank == 0) {
             const bool leader = lane == 0;
-            auto commit = [&](uint64_t* bar) {
-                if constexpr (PAIR)
-                    tc::commit_pair(bar, leader);
-                else
-                    tc::commit(bar, leader);
-            };
             const uint64_t w_desc = tc::tile_descriptor(tbk::smem_addr(smem), 16);
             const uint32_t x_off = a.x_off / 16, x_piece = a.x_piece / 16;
             int stage = 0, done = 0, consumed = 0;
@@ -261,92 +266,102 @@ k_linear(const __grid_constant__ Args a) {
                                     tc::with_block(instruction, block), w_scales + 4 * h,
                                     x_scales + 4 * kMostX * h, j > first || p + m > 0, leader);
                         }
-                    if (done + a.stages < total) commit(&sh.empty[stage]);
+                    if (done + a.stages < total) commit(&sh.empty[stage], leader);
                     ++done;
                     if (++stage == a.stages) {
                         stage = 0;
                         parity ^= 1;
                     }
                 }
-                if (fine) commit(&sh.sums);
+                if (fine) commit(&sh.sums, leader);
             }
             if (leader) sh.consumed = consumed;
             // whatever ended the loop, no product may be in flight when tensor memory is freed
-            commit(&sh.products_done);
+            commit(&sh.products_done, leader);
             wait_all(&sh.products_done, 0, a.status);
         }
-    } else if (warp >= H::kScalers) {
-        // Scales to shared memory, kAhead - 1 steps ahead, by all four warps; from there each
-        // brings all of them to its quarter of the rows of tensor memory, a lane the words of
-        // rows l, l + 32, l + 64 and l + 96.
-        constexpr int kAhead = H::kAhead, kChunks = kEach * 32;
-        const uint32_t to = tmem + a.scales_column + ((uint32_t)(warp % 4) << 21);
-        const int thread = threadIdx.x - 32 * H::kScalers;
-        uint4* ring = reinterpret_cast<uint4*>(smem + a.stages * a.stage_bytes);
+    } else if (warp == kScaler) {
+        constexpr int kAhead = H::kAhead;
+        const bool leader = lane == 0;
+        uint8_t* ring = smem + a.stages * a.stage_bytes;
         int ask_tile = 0, ask_step = first, ask_slot = 0;  // the next step that is asked for
         auto ask = [&] {
-            if (ask_tile < mine) {
-                const Tile t = tile_of<PAIR>(a, tile0 + ask_tile * tile_step);
-                const int out = t.out + (PAIR ? kOuts * rank : 0);
+            const Tile t = tile_of<PAIR>(a, tile0 + ask_tile * tile_step);
+            const int out = t.out + (PAIR ? kOuts * rank : 0), at = ask_step * kTiles;
+            const int bytes = min(kTiles, a.tiles128 - at) * mx::kTileBytes;
+            const bool has_w = out < a.outs, has_x1 = kMostX > 1 && t.n > 128;
+            if (leader) {
+                uint8_t* to = ring + ask_slot * kEach * mx::kTileBytes;
+                uint64_t* bar = &sh.asked[ask_slot];
+                tbk::mbar_expect_tx(bar, (1 + has_w + has_x1) * bytes);
+                if (has_w)
+                    tbk::bulk_g2s(to, a.w_scales + mx::scales_at(out, at, a.tiles128), bytes, bar);
 #pragma unroll
-                for (int i = 0; i < (kChunks + 127) / 128; ++i) {
-                    const int c = thread + 128 * i, tile = c / 32, x = tile - kTiles;
-                    const int h = x < 0 ? tile : x / kMostX, at = ask_step * kTiles + h;
-                    const int row = x < 0 ? out : t.row + 128 * (x % kMostX);
-                    if (c < kChunks && at < a.tiles128 && row < (x < 0 ? a.outs : a.rows)) {
-                        const uint8_t* from = (x < 0 ? a.w_scales : a.x_scales) +
-                                              mx::scales_at(row, at, a.tiles128) + c % 32 * 16;
-                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(
-                                         tbk::smem_addr(ring + ask_slot * kChunks + c)),
-                                     "l"(from)
-                                     : "memory");
-                    }
-                }
-                if (++ask_step == last) {
-                    ask_step = first;
-                    ++ask_tile;
-                }
+                for (int k = 0; k < kMostX; ++k)
+                    if (k == 0 || has_x1)
+                        tbk::bulk_g2s(to + (1 + k) * kTiles * mx::kTileBytes,
+                                      a.x_scales + mx::scales_at(t.row + 128 * k, at, a.tiles128),
+                                      bytes, bar);
             }
-            asm volatile("cp.async.commit_group;" ::: "memory");
+            __syncwarp();
+            ++issued;
             if (++ask_slot == kAhead) ask_slot = 0;
+            if (++ask_step == last) {
+                ask_step = first;
+                ++ask_tile;
+            }
         };
-#pragma unroll 1
-        for (int i = 0; i < kAhead - 1; ++i) ask();
-        int stage = 0, slot = 0;
-        uint32_t parity = 1;  // of the round before
+        while (issued < min(kAhead, total)) ask();
+        int stage = 0, slot = 0, step = first;
+        uint32_t parity = 0, slot_parity = 0;
         for (int done = 0; done < total; ++done) {
-            asm volatile("cp.async.wait_group %0;" ::"n"(kAhead - 2) : "memory");
-            // this step's are there, and the step before's have been taken by all
-            asm volatile("bar.sync 1, 128;" ::: "memory");
-            ask();
-            uint4 r[kEach];
-#pragma unroll
-            for (int i = 0; i < kEach; ++i) r[i] = ring[slot * kChunks + i * 32 + lane];
             if (done >= a.stages) {
-                if (fine) fine = wait_all(&sh.empty[stage], parity, a.status);
+                // the products of step done - stages, and so the copies of its scales, are done
+                fine = wait_all(&sh.empty[stage], parity ^ 1, a.status);
+                if (!fine) break;
+                if (issued < total && issued - kAhead <= done - a.stages) ask();
             }
-            if (fine) {  // (a warp that gave up still comes to the barrier above)
+            fine = wait_all(&sh.asked[slot], slot_parity, a.status);
+            if (!fine) break;
+            ++taken;
+            if (!PAIR || rank == 0) {
+                if (PAIR) fine = wait_all(&sh.other[stage], parity, a.status);
+                if (!fine) break;
                 tc::fence_after();
-                const uint32_t at = to + stage * H::kScaleColumns;
+                const uint32_t from = tbk::smem_addr(ring) + slot * kEach * mx::kTileBytes;
+                const uint32_t w_to = tmem + a.scales_column + stage * H::kScaleColumns;
+                const uint32_t x_to = w_to + 4 * kTiles;
+                const int have = a.tiles128 - step * kTiles;
 #pragma unroll
-                for (int i = 0; i < kEach; ++i) tc::store_scales(at + 4 * i, r[i]);
-                tc::wait_store();
-                tc::fence_before();
-                __syncwarp();
-                if (lane == 0) {
-                    if (PAIR)
-                        arrive_first(&sh.scaled[stage]);
-                    else
-                        tbk::mbar_arrive(&sh.scaled[stage]);
+                for (int h = 0; h < kTiles; ++h) {
+                    if (h > 0 && h >= have) break;
+                    tc::copy_scales<PAIR>(w_to + 4 * h, from + h * mx::kTileBytes, leader);
+#pragma unroll
+                    for (int k = 0; k < kMostX; ++k)
+                        tc::copy_scales<PAIR>(x_to + 4 * (kMostX * h + k),
+                                              from + ((1 + k) * kTiles + h) * mx::kTileBytes,
+                                              leader);
                 }
+                // (by the first CTA alone: the other's issuer does not wait)
+                tc::commit(&sh.scaled[stage], leader, PAIR);
+            } else if (lane == 0) {
+                arrive_first(&sh.other[stage]);
             }
-            if (++slot == kAhead) slot = 0;
+            if (++step == last) step = first;
+            if (++slot == kAhead) {
+                slot = 0;
+                slot_parity ^= 1;
+            }
             if (++stage == a.stages) {
                 stage = 0;
                 parity ^= 1;
             }
         }
-        asm volatile("cp.async.wait_all;" ::: "memory");
+        if (!PAIR || rank == 0) {
+            // no copy to tensor memory may be in flight when that is freed
+            tc::commit(&sh.scales_done, leader, PAIR);
+            wait_all(&sh.scales_done, 0, a.status);
+        }
     } else {
         const int quarter = warp % 4;
         const uint32_t sums = tmem + ((uint32_t)quarter << 21);
@@ -430,6 +445,10 @@ k_linear(const __grid_constant__ Args a) {
         for (int j = sh.consumed; j < issued; ++j)
             wait_one(&sh.full[j % a.stages], (uint32_t)(j / a.stages) & 1u, a.status);
     }
+    if (warp == kScaler && lane == 0 && lost) {
+        for (int j = taken; j < issued; ++j)
+            wait_one(&sh.asked[j % H::kAhead], (uint32_t)(j / H::kAhead) & 1u, a.status);
+    }
     __syncwarp();
     if constexpr (PAIR) {
         // (the first CTA's last arrival comes here too)
@@ -441,7 +460,7 @@ k_linear(const __grid_constant__ Args a) {
     if (warp == kIssuer) tc::release(tmem, a.columns);
     if (a.split > 1) {
         cluster_sync();
-        if (warp >= kStorers && warp < H::kScalers) {
+        if (warp >= kStorers) {
             const Tile t = tile_of<PAIR>(a, tile0);
             const int at = warp % 4 * 32 + lane, out = t.out + at;
             if (out < a.outs) {
@@ -481,8 +500,10 @@ int plan_of(Plan& p, const TbB200Mx* x, const TbB200Mx* w, bool both4, int sm_co
     p.n_tiles = (int)n_tiles;
     p.stage_bytes = pieces * (kOuts + p.x_rows) * kPieceBytes;
     // as many CTAs an SM as keep four stages each
-    const int beside = (p.pair ? Shape<false, true>::kScaleBytes + Shape<false, true>::kStaged
-                               : Shape<false, false>::kScaleBytes) + 1024;
+    const int scales = p.pair ? Shape<false, true>::kScaleBytes
+                       : both4 ? Shape<true, false>::kScaleBytes : Shape<false, false>::kScaleBytes;
+    static_assert(Shape<false, true>::kScaleBytes == Shape<true, true>::kScaleBytes, "scales");
+    const int beside = scales + (p.pair ? Shape<false, true>::kStaged : 0) + 1024;
     const int per_sm = p.pair ? 1 : p.tile_rows <= 32 ? 3 : p.tile_rows <= 64 ? 2 : 1;
     p.stages = (226 * 1024 / per_sm - 1024 - beside) / p.stage_bytes;
     if (p.stages > kMostStages) p.stages = kMostStages;
