@@ -18,8 +18,8 @@
 
 namespace {
 
-// warps; the others store
-constexpr int kLoader = 0, kIssuer = 1, kScaler = 2, kStorers = 3;
+// warps
+constexpr int kLoader = 0, kIssuer = 1;
 constexpr int kOuts = 128, kMostStages = 8, kMostAhead = 8, kMostSplit = 8;  // kOuts: of a CTA's tile
 constexpr int kPieceBytes = 128;  // of a row of codes; a step has one or two such pieces
 constexpr uint64_t kLimit = 1000000000ull;  // ns, of a wait
@@ -136,6 +136,8 @@ template <bool BOTH4, bool PAIR>
 struct Shape {
     static constexpr int kPieces = PAIR ? 2 : 1;
     static constexpr int kStoreWarps = PAIR ? 8 : 4;
+    // warps: one that brings scales or four, and those that store
+    static constexpr int kScalers = 2, kScaleWarps = PAIR ? 1 : 4, kStorers = 2 + kScaleWarps;
     static constexpr int kThreads = 32 * (kStorers + kStoreWarps);
     static constexpr int kTiles = (BOTH4 ? 2 : 1) * kPieces;  // of 128 columns, a step
     static constexpr int kMostX = PAIR ? 2 : 1;               // x's tiles of 128 rows
@@ -168,7 +170,7 @@ k_linear(const __grid_constant__ Args a) {
     if (threadIdx.x == 0) {
         for (int i = 0; i < a.stages; ++i) {
             tbk::mbar_init(&sh.full[i], 1);
-            tbk::mbar_init(&sh.scaled[i], 1);
+            tbk::mbar_init(&sh.scaled[i], H::kScaleWarps);
             tbk::mbar_init(&sh.empty[i], 1);
             tbk::mbar_init(&sh.other[i], 1);
         }
@@ -280,87 +282,158 @@ k_linear(const __grid_constant__ Args a) {
             commit(&sh.products_done, leader);
             wait_all(&sh.products_done, 0, a.status);
         }
-    } else if (warp == kScaler) {
-        constexpr int kAhead = H::kAhead;
-        const bool leader = lane == 0;
-        uint8_t* ring = smem + a.stages * a.stage_bytes;
-        int ask_tile = 0, ask_step = first, ask_slot = 0;  // the next step that is asked for
-        auto ask = [&] {
-            const Tile t = tile_of<PAIR>(a, tile0 + ask_tile * tile_step);
-            const int out = t.out + (PAIR ? kOuts * rank : 0), at = ask_step * kTiles;
-            const int bytes = min(kTiles, a.tiles128 - at) * mx::kTileBytes;
-            const bool has_w = out < a.outs, has_x1 = kMostX > 1 && t.n > 128;
-            if (leader) {
-                uint8_t* to = ring + ask_slot * kEach * mx::kTileBytes;
-                uint64_t* bar = &sh.asked[ask_slot];
-                tbk::mbar_expect_tx(bar, (1 + has_w + has_x1) * bytes);
-                if (has_w)
-                    tbk::bulk_g2s(to, a.w_scales + mx::scales_at(out, at, a.tiles128), bytes, bar);
-#pragma unroll
-                for (int k = 0; k < kMostX; ++k)
-                    if (k == 0 || has_x1)
-                        tbk::bulk_g2s(to + (1 + k) * kTiles * mx::kTileBytes,
-                                      a.x_scales + mx::scales_at(t.row + 128 * k, at, a.tiles128),
-                                      bytes, bar);
-            }
-            __syncwarp();
-            ++issued;
-            if (++ask_slot == kAhead) ask_slot = 0;
-            if (++ask_step == last) {
-                ask_step = first;
-                ++ask_tile;
-            }
-        };
-        while (issued < min(kAhead, total)) ask();
-        int stage = 0, slot = 0, step = first;
-        uint32_t parity = 0, slot_parity = 0;
-        for (int done = 0; done < total; ++done) {
-            if (done >= a.stages) {
-                // the products of step done - stages, and so the copies of its scales, are done
-                fine = wait_all(&sh.empty[stage], parity ^ 1, a.status);
-                if (!fine) break;
-                if (issued < total && issued - kAhead <= done - a.stages) ask();
-            }
-            fine = wait_all(&sh.asked[slot], slot_parity, a.status);
-            if (!fine) break;
-            ++taken;
-            if (!PAIR || rank == 0) {
-                if (PAIR) fine = wait_all(&sh.other[stage], parity, a.status);
-                if (!fine) break;
-                tc::fence_after();
-                const uint32_t from = tbk::smem_addr(ring) + slot * kEach * mx::kTileBytes;
-                const uint32_t w_to = tmem + a.scales_column + stage * H::kScaleColumns;
-                const uint32_t x_to = w_to + 4 * kTiles;
-                const int have = a.tiles128 - step * kTiles;
-#pragma unroll
-                for (int h = 0; h < kTiles; ++h) {
-                    if (h > 0 && h >= have) break;
-                    tc::copy_scales<PAIR>(w_to + 4 * h, from + h * mx::kTileBytes, leader);
+    } else if (warp < H::kStorers) {
+        if constexpr (PAIR) {
+            // One warp: scales to shared memory, kAhead steps ahead, and from there by the tensor
+            // pipe.  Stores from registers wait for the pair's products, 1700 clocks a step.
+            constexpr int kAhead = H::kAhead;
+            const bool leader = lane == 0;
+            uint8_t* ring = smem + a.stages * a.stage_bytes;
+            int ask_tile = 0, ask_step = first, ask_slot = 0;  // the next step that is asked for
+            auto ask = [&] {
+                const Tile t = tile_of<PAIR>(a, tile0 + ask_tile * tile_step);
+                const int out = t.out + (PAIR ? kOuts * rank : 0), at = ask_step * kTiles;
+                const int bytes = min(kTiles, a.tiles128 - at) * mx::kTileBytes;
+                const bool has_w = out < a.outs, has_x1 = kMostX > 1 && t.n > 128;
+                if (leader) {
+                    uint8_t* to = ring + ask_slot * kEach * mx::kTileBytes;
+                    uint64_t* bar = &sh.asked[ask_slot];
+                    tbk::mbar_expect_tx(bar, (1 + has_w + has_x1) * bytes);
+                    if (has_w)
+                        tbk::bulk_g2s(to, a.w_scales + mx::scales_at(out, at, a.tiles128), bytes, bar);
 #pragma unroll
                     for (int k = 0; k < kMostX; ++k)
-                        tc::copy_scales<PAIR>(x_to + 4 * (kMostX * h + k),
-                                              from + ((1 + k) * kTiles + h) * mx::kTileBytes,
-                                              leader);
+                        if (k == 0 || has_x1)
+                            tbk::bulk_g2s(to + (1 + k) * kTiles * mx::kTileBytes,
+                                          a.x_scales + mx::scales_at(t.row + 128 * k, at, a.tiles128),
+                                          bytes, bar);
                 }
-                // (by the first CTA alone: the other's issuer does not wait)
-                tc::commit(&sh.scaled[stage], leader, PAIR);
-            } else if (lane == 0) {
-                arrive_first(&sh.other[stage]);
+                __syncwarp();
+                ++issued;
+                if (++ask_slot == kAhead) ask_slot = 0;
+                if (++ask_step == last) {
+                    ask_step = first;
+                    ++ask_tile;
+                }
+            };
+            while (issued < min(kAhead, total)) ask();
+            int stage = 0, slot = 0, step = first;
+            uint32_t parity = 0, slot_parity = 0;
+            for (int done = 0; done < total; ++done) {
+                if (done >= a.stages) {
+                    // the products of step done - stages, and so the copies of its scales, are done
+                    fine = wait_all(&sh.empty[stage], parity ^ 1, a.status);
+                    if (!fine) break;
+                    if (issued < total && issued - kAhead <= done - a.stages) ask();
+                }
+                fine = wait_all(&sh.asked[slot], slot_parity, a.status);
+                if (!fine) break;
+                ++taken;
+                if (rank == 0) {
+                    fine = wait_all(&sh.other[stage], parity, a.status);
+                    if (!fine) break;
+                    tc::fence_after();
+                    const uint32_t from = tbk::smem_addr(ring) + slot * kEach * mx::kTileBytes;
+                    const uint32_t w_to = tmem + a.scales_column + stage * H::kScaleColumns;
+                    const uint32_t x_to = w_to + 4 * kTiles;
+                    const int have = a.tiles128 - step * kTiles;
+#pragma unroll
+                    for (int h = 0; h < kTiles; ++h) {
+                        if (h > 0 && h >= have) break;
+                        tc::copy_scales<PAIR>(w_to + 4 * h, from + h * mx::kTileBytes, leader);
+#pragma unroll
+                        for (int k = 0; k < kMostX; ++k)
+                            tc::copy_scales<PAIR>(x_to + 4 * (kMostX * h + k),
+                                                  from + ((1 + k) * kTiles + h) * mx::kTileBytes,
+                                                  leader);
+                    }
+                    // (by the first CTA alone: the other's issuer does not wait)
+                    tc::commit(&sh.scaled[stage], leader, PAIR);
+                } else if (lane == 0) {
+                    arrive_first(&sh.other[stage]);
+                }
+                if (++step == last) step = first;
+                if (++slot == kAhead) {
+                    slot = 0;
+                    slot_parity ^= 1;
+                }
+                if (++stage == a.stages) {
+                    stage = 0;
+                    parity ^= 1;
+                }
             }
-            if (++step == last) step = first;
-            if (++slot == kAhead) {
-                slot = 0;
-                slot_parity ^= 1;
+            if (rank == 0) {
+                // no copy to tensor memory may be in flight when that is freed
+                tc::commit(&sh.scales_done, leader, PAIR);
+                wait_all(&sh.scales_done, 0, a.status);
             }
-            if (++stage == a.stages) {
-                stage = 0;
-                parity ^= 1;
+        } else {
+            // Four warps: scales to shared memory, kAhead - 1 steps ahead, by all of them; from
+            // there through registers, each to its quarter of the rows of tensor memory, a lane the words
+            // of rows l, l + 32, l + 64 and l + 96.
+            constexpr int kAhead = H::kAhead, kChunks = kEach * 32;
+            const uint32_t to = tmem + a.scales_column + ((uint32_t)(warp % 4) << 21);
+            const int thread = threadIdx.x - 32 * H::kScalers;
+            uint4* ring = reinterpret_cast<uint4*>(smem + a.stages * a.stage_bytes);
+            int ask_tile = 0, ask_step = first, ask_slot = 0;  // the next step that is asked for
+            auto ask = [&] {
+                if (ask_tile < mine) {
+                    const Tile t = tile_of<PAIR>(a, tile0 + ask_tile * tile_step);
+                    const int out = t.out;
+#pragma unroll
+                    for (int i = 0; i < (kChunks + 127) / 128; ++i) {
+                        const int c = thread + 128 * i, tile = c / 32, x = tile - kTiles;
+                        const int h = x < 0 ? tile : x / kMostX, at = ask_step * kTiles + h;
+                        const int row = x < 0 ? out : t.row + 128 * (x % kMostX);
+                        if (c < kChunks && at < a.tiles128 && row < (x < 0 ? a.outs : a.rows)) {
+                            const uint8_t* from = (x < 0 ? a.w_scales : a.x_scales) +
+                                                  mx::scales_at(row, at, a.tiles128) + c % 32 * 16;
+                            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(
+                                             tbk::smem_addr(ring + ask_slot * kChunks + c)),
+                                         "l"(from)
+                                         : "memory");
+                        }
+                    }
+                    if (++ask_step == last) {
+                        ask_step = first;
+                        ++ask_tile;
+                    }
+                }
+                asm volatile("cp.async.commit_group;" ::: "memory");
+                if (++ask_slot == kAhead) ask_slot = 0;
+            };
+#pragma unroll 1
+            for (int i = 0; i < kAhead - 1; ++i) ask();
+            int stage = 0, slot = 0;
+            uint32_t parity = 1;  // of the round before
+            for (int done = 0; done < total; ++done) {
+                asm volatile("cp.async.wait_group %0;" ::"n"(kAhead - 2) : "memory");
+                // this step's are there, and the step before's have been taken by all
+                asm volatile("bar.sync 1, 128;" ::: "memory");
+                ask();
+                uint4 r[kEach];
+#pragma unroll
+                for (int i = 0; i < kEach; ++i) r[i] = ring[slot * kChunks + i * 32 + lane];
+                if (done >= a.stages) {
+                    if (fine) fine = wait_all(&sh.empty[stage], parity, a.status);
+                }
+                if (fine) {  // (a warp that gave up still comes to the barrier above)
+                    tc::fence_after();
+                    const uint32_t at = to + stage * H::kScaleColumns;
+#pragma unroll
+                    for (int i = 0; i < kEach; ++i) tc::store_scales(at + 4 * i, r[i]);
+                    tc::wait_store();
+                    tc::fence_before();
+                    __syncwarp();
+                    if (lane == 0) tbk::mbar_arrive(&sh.scaled[stage]);
+                }
+                if (++slot == kAhead) slot = 0;
+                if (++stage == a.stages) {
+                    stage = 0;
+                    parity ^= 1;
+                }
             }
-        }
-        if (!PAIR || rank == 0) {
-            // no copy to tensor memory may be in flight when that is freed
-            tc::commit(&sh.scales_done, leader, PAIR);
-            wait_all(&sh.scales_done, 0, a.status);
+            asm volatile("cp.async.wait_all;" ::: "memory");
         }
     } else {
         const int quarter = warp % 4;
@@ -390,8 +463,8 @@ k_linear(const __grid_constant__ Args a) {
                 // through shared memory, for whole rows of the CTA's outs to be stored at once
                 constexpr int kRows = H::kStaged / 2 / (kOuts * sizeof(T));  // of each half
                 constexpr int kVec = 16 / sizeof(T), kPer = kOuts / kVec;    // pieces of a row
-                const int half = (warp - kStorers) / 4, c = half * 128;
-                const int thread = threadIdx.x - 32 * kStorers;
+                const int half = (warp - H::kStorers) / 4, c = half * 128;
+                const int thread = threadIdx.x - 32 * H::kStorers;
                 T* staged = reinterpret_cast<T*>(smem + a.stages * a.stage_bytes + H::kScaleBytes);
                 T* y0 = static_cast<T*>(a.y) + (int64_t)t.row * a.y_stride + t.out + kOuts * rank;
                 const int outs = a.outs - t.out - kOuts * rank, rows = min(a.rows - t.row, t.n);
@@ -445,7 +518,7 @@ k_linear(const __grid_constant__ Args a) {
         for (int j = sh.consumed; j < issued; ++j)
             wait_one(&sh.full[j % a.stages], (uint32_t)(j / a.stages) & 1u, a.status);
     }
-    if (warp == kScaler && lane == 0 && lost) {
+    if (PAIR && warp == H::kScalers && lane == 0 && lost) {
         for (int j = taken; j < issued; ++j)
             wait_one(&sh.asked[j % H::kAhead], (uint32_t)(j / H::kAhead) & 1u, a.status);
     }
@@ -460,7 +533,7 @@ k_linear(const __grid_constant__ Args a) {
     if (warp == kIssuer) tc::release(tmem, a.columns);
     if (a.split > 1) {
         cluster_sync();
-        if (warp >= kStorers) {
+        if (warp >= H::kStorers) {
             const Tile t = tile_of<PAIR>(a, tile0);
             const int at = warp % 4 * 32 + lane, out = t.out + at;
             if (out < a.outs) {
@@ -499,12 +572,12 @@ int plan_of(Plan& p, const TbB200Mx* x, const TbB200Mx* w, bool both4, int sm_co
     if (n_tiles * kMostSplit > INT32_MAX) return TB_ERR_INVALID_SHAPE;
     p.n_tiles = (int)n_tiles;
     p.stage_bytes = pieces * (kOuts + p.x_rows) * kPieceBytes;
-    // as many CTAs an SM as keep four stages each
+    // two CTAs an SM (64 rows of 8192 to 128256: one 419 us, two 135, three 152)
     const int scales = p.pair ? Shape<false, true>::kScaleBytes
                        : both4 ? Shape<true, false>::kScaleBytes : Shape<false, false>::kScaleBytes;
     static_assert(Shape<false, true>::kScaleBytes == Shape<true, true>::kScaleBytes, "scales");
     const int beside = scales + (p.pair ? Shape<false, true>::kStaged : 0) + 1024;
-    const int per_sm = p.pair ? 1 : p.tile_rows <= 32 ? 3 : p.tile_rows <= 64 ? 2 : 1;
+    const int per_sm = p.pair ? 1 : 2;
     p.stages = (226 * 1024 / per_sm - 1024 - beside) / p.stage_bytes;
     if (p.stages > kMostStages) p.stages = kMostStages;
     p.scales_column = (uint32_t)(p.tile_rows + 31) / 32 * 32;

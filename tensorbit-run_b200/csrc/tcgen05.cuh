@@ -235,6 +235,15 @@ __device__ __forceinline__ void copy_scales(uint32_t to, uint32_t smem, bool lea
             : "memory");
 }
 
+// Four columns of the warp's 32 rows, a row a lane: the scales of 128 rows and 4 blocks, of
+// which lane l has the words of rows l, l + 32, l + 64 and l + 96 (every quarter of the rows
+// has them all).
+__device__ __forceinline__ void store_scales(uint32_t address, const uint4& r) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1,%2,%3,%4};" ::"r"(address),
+                 "r"(r.x), "r"(r.y), "r"(r.z), "r"(r.w)
+                 : "memory");
+}
+
 // The warpgroup's registers per thread; the shares add up to the launch's.
 template <int N>
 __device__ __forceinline__ void more_registers() {
