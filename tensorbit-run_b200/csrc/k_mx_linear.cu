@@ -45,7 +45,7 @@ struct Shared {
     uint64_t asked[kMostAhead];   // a step's scales, to shared memory
     uint64_t sums, drained, products_done, scales_done;
     uint32_t tmem;
-    int consumed;  // steps whose copies the issuer has waited for
+    int consumed, taken;  // steps whose codes, and whose scales, have been waited for
 };
 
 // A bounded wait.  The clock is read once in kTries tries (%globaltimer takes about a
@@ -136,8 +136,8 @@ template <bool BOTH4, bool PAIR>
 struct Shape {
     static constexpr int kPieces = PAIR ? 2 : 1;
     static constexpr int kStoreWarps = PAIR ? 8 : 4;
-    // warps: one that brings scales or four, and those that store
-    static constexpr int kScalers = 2, kScaleWarps = PAIR ? 1 : 4, kStorers = 2 + kScaleWarps;
+    // warps: those that bring scales, and those that store
+    static constexpr int kScalers = 2, kScaleWarps = PAIR ? 2 : 4, kStorers = 2 + kScaleWarps;
     static constexpr int kThreads = 32 * (kStorers + kStoreWarps);
     static constexpr int kTiles = (BOTH4 ? 2 : 1) * kPieces;  // of 128 columns, a step
     static constexpr int kMostX = PAIR ? 2 : 1;               // x's tiles of 128 rows
@@ -175,11 +175,11 @@ k_linear(const __grid_constant__ Args a) {
             tbk::mbar_init(&sh.other[i], 1);
         }
         for (int i = 0; i < H::kAhead; ++i) tbk::mbar_init(&sh.asked[i], 1);
-        tbk::mbar_init(&sh.scales_done, 1);
+        tbk::mbar_init(&sh.scales_done, H::kScaleWarps);
         tbk::mbar_init(&sh.sums, 1);
         tbk::mbar_init(&sh.drained, (PAIR ? 2 : 1) * H::kStoreWarps);
         tbk::mbar_init(&sh.products_done, 1);
-        sh.consumed = 0;
+        sh.consumed = sh.taken = 0;
         tbk::fence_mbar_init();
     }
     if (warp == kIssuer) {
@@ -200,10 +200,39 @@ k_linear(const __grid_constant__ Args a) {
         else
             tc::commit(bar, leader);
     };
-    int issued = 0, taken = 0;  // the loader's steps; the scaler's, asked for and taken
+    int issued = 0, asked = 0;  // the loader's steps of codes and of scales
     bool fine = true;
     if (warp == kLoader) {
         if (lane == 0) {
+            // PAIR: a step's scales too, to a ring of their own, kAhead steps before they are
+            // taken
+            constexpr int kAhead = H::kAhead;
+            uint8_t* ring = smem + a.stages * a.stage_bytes;
+            int ask_tile = 0, ask_step = first, ask_slot = 0;  // the next that are asked for
+            Tile ask_t = tile_of<PAIR>(a, tile0);
+            auto ask = [&] {
+                const int out = ask_t.out + kOuts * rank, at = ask_step * kTiles;
+                const int bytes = min(kTiles, a.tiles128 - at) * mx::kTileBytes;
+                const bool has_w = out < a.outs, has_x1 = kMostX > 1 && ask_t.n > 128;
+                uint8_t* to = ring + ask_slot * kEach * mx::kTileBytes;
+                uint64_t* bar = &sh.asked[ask_slot];
+                tbk::mbar_expect_tx(bar, (1 + has_w + has_x1) * bytes);
+                if (has_w)
+                    tbk::bulk_g2s(to, a.w_scales + mx::scales_at(out, at, a.tiles128), bytes, bar);
+#pragma unroll
+                for (int k = 0; k < kMostX; ++k)
+                    if (k == 0 || has_x1)
+                        tbk::bulk_g2s(to + (1 + k) * kTiles * mx::kTileBytes,
+                                      a.x_scales + mx::scales_at(ask_t.row + 128 * k, at,
+                                                                 a.tiles128),
+                                      bytes, bar);
+                ++asked;
+                if (++ask_slot == kAhead) ask_slot = 0;
+                if (++ask_step == last) {
+                    ask_step = first;
+                    if (++ask_tile < mine) ask_t = tile_of<PAIR>(a, tile0 + ask_tile * tile_step);
+                }
+            };
             int stage = 0;
             uint32_t parity = 1;  // of the round before
             for (int i = 0; i < mine && fine; ++i) {
@@ -211,6 +240,8 @@ k_linear(const __grid_constant__ Args a) {
                 const int out = t.out + (PAIR ? kOuts * rank : 0);
                 const int row = t.row + (PAIR ? t.n / 2 * rank : 0);
                 for (int j = first; j < last; ++j) {
+                    // the products of step issued - stages are done, and so are the copies of
+                    // its scales
                     if (issued >= a.stages) fine = wait_one(&sh.empty[stage], parity, a.status);
                     if (!fine) break;
                     uint8_t* to = smem + stage * a.stage_bytes;
@@ -222,6 +253,9 @@ k_linear(const __grid_constant__ Args a) {
                         const int x = (j * kPieces + p) * 128;  // (bytes, or 4-bit elements)
                         tma_tile<PAIR>(to + p * kOuts * kPieceBytes, &a.w_map, x, out, bar);
                         tma_tile<PAIR>(to + a.x_off + p * a.x_piece, &a.x_map, x, row, bar);
+                    }
+                    if constexpr (PAIR) {
+                        while (asked < total && asked < kAhead + max(0, issued - a.stages + 1)) ask();
                     }
                     ++issued;
                     if (++stage == a.stages) {
@@ -284,53 +318,22 @@ k_linear(const __grid_constant__ Args a) {
         }
     } else if (warp < H::kStorers) {
         if constexpr (PAIR) {
-            // One warp: scales to shared memory, kAhead steps ahead, and from there by the tensor
-            // pipe.  Stores from registers wait for the pair's products, 1700 clocks a step.
+            // Two warps, half of a step's copies of scales to tensor memory each, by the tensor
+            // pipe (stores from registers wait for the pair's products, 1700 clocks a step; one
+            // warp, that asked for them too, took 2000 clocks a step).
             constexpr int kAhead = H::kAhead;
+            const int part = warp - H::kScalers;
             const bool leader = lane == 0;
-            uint8_t* ring = smem + a.stages * a.stage_bytes;
-            int ask_tile = 0, ask_step = first, ask_slot = 0;  // the next step that is asked for
-            auto ask = [&] {
-                const Tile t = tile_of<PAIR>(a, tile0 + ask_tile * tile_step);
-                const int out = t.out + (PAIR ? kOuts * rank : 0), at = ask_step * kTiles;
-                const int bytes = min(kTiles, a.tiles128 - at) * mx::kTileBytes;
-                const bool has_w = out < a.outs, has_x1 = kMostX > 1 && t.n > 128;
-                if (leader) {
-                    uint8_t* to = ring + ask_slot * kEach * mx::kTileBytes;
-                    uint64_t* bar = &sh.asked[ask_slot];
-                    tbk::mbar_expect_tx(bar, (1 + has_w + has_x1) * bytes);
-                    if (has_w)
-                        tbk::bulk_g2s(to, a.w_scales + mx::scales_at(out, at, a.tiles128), bytes, bar);
-#pragma unroll
-                    for (int k = 0; k < kMostX; ++k)
-                        if (k == 0 || has_x1)
-                            tbk::bulk_g2s(to + (1 + k) * kTiles * mx::kTileBytes,
-                                          a.x_scales + mx::scales_at(t.row + 128 * k, at, a.tiles128),
-                                          bytes, bar);
-                }
-                __syncwarp();
-                ++issued;
-                if (++ask_slot == kAhead) ask_slot = 0;
-                if (++ask_step == last) {
-                    ask_step = first;
-                    ++ask_tile;
-                }
-            };
-            while (issued < min(kAhead, total)) ask();
+            const uint8_t* ring = smem + a.stages * a.stage_bytes;
             int stage = 0, slot = 0, step = first;
             uint32_t parity = 0, slot_parity = 0;
-            for (int done = 0; done < total; ++done) {
-                if (done >= a.stages) {
-                    // the products of step done - stages, and so the copies of its scales, are done
-                    fine = wait_all(&sh.empty[stage], parity ^ 1, a.status);
-                    if (!fine) break;
-                    if (issued < total && issued - kAhead <= done - a.stages) ask();
-                }
+            for (int done = 0; done < total && (rank == 0 || part == 0); ++done) {
                 fine = wait_all(&sh.asked[slot], slot_parity, a.status);
                 if (!fine) break;
-                ++taken;
+                if (part == 0 && lane == 0) sh.taken = done + 1;
                 if (rank == 0) {
-                    fine = wait_all(&sh.other[stage], parity, a.status);
+                    fine = done < a.stages || wait_all(&sh.empty[stage], parity ^ 1, a.status);
+                    fine = fine && wait_all(&sh.other[stage], parity, a.status);
                     if (!fine) break;
                     tc::fence_after();
                     const uint32_t from = tbk::smem_addr(ring) + slot * kEach * mx::kTileBytes;
@@ -338,8 +341,9 @@ k_linear(const __grid_constant__ Args a) {
                     const uint32_t x_to = w_to + 4 * kTiles;
                     const int have = a.tiles128 - step * kTiles;
 #pragma unroll
-                    for (int h = 0; h < kTiles; ++h) {
-                        if (h > 0 && h >= have) break;
+                    for (int i = 0; i < kTiles / 2; ++i) {
+                        const int h = 2 * i + part;
+                        if (h >= have) break;
                         tc::copy_scales<PAIR>(w_to + 4 * h, from + h * mx::kTileBytes, leader);
 #pragma unroll
                         for (int k = 0; k < kMostX; ++k)
@@ -518,8 +522,8 @@ k_linear(const __grid_constant__ Args a) {
         for (int j = sh.consumed; j < issued; ++j)
             wait_one(&sh.full[j % a.stages], (uint32_t)(j / a.stages) & 1u, a.status);
     }
-    if (PAIR && warp == H::kScalers && lane == 0 && lost) {
-        for (int j = taken; j < issued; ++j)
+    if (PAIR && warp == kLoader && lane == 0 && lost) {
+        for (int j = sh.taken; j < asked; ++j)
             wait_one(&sh.asked[j % H::kAhead], (uint32_t)(j / H::kAhead) & 1u, a.status);
     }
     __syncwarp();
