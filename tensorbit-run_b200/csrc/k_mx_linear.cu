@@ -35,14 +35,15 @@ struct Args {
     int tile_rows, row_tiles, n_tiles;
     int steps, split, stages, stage_bytes, x_off, x_piece;
     int y_vec;       // rows of y start on 16 bytes
+    int flat;        // a copy takes one piece, by its x
     int code_bytes;  // that a step's copies count, fill left out
     uint32_t columns, scales_column, instruction;
 };
 
 struct Shared {
     uint64_t full[kMostStages], scaled[kMostStages], empty[kMostStages];
-    uint64_t other[kMostStages];  // the pair's other CTA has the step's scales
-    uint64_t asked[kMostAhead];   // a step's scales, to shared memory
+    uint64_t asked[kMostAhead];  // a step's scales, to shared memory
+    uint64_t other[kMostAhead];  // the pair's other CTA has them
     uint64_t sums, drained, products_done, scales_done;
     uint32_t tmem;
     int consumed, taken;  // steps whose codes, and whose scales, have been waited for
@@ -83,20 +84,20 @@ __device__ __forceinline__ void arrive_first(uint64_t* bar) {
 }
 // A tile to this CTA's shared memory; PAIR: counted on the first CTA's barrier.
 template <bool PAIR>
-__device__ __forceinline__ void tma_tile(void* dst, const CUtensorMap* map, int x, int y,
-                                         uint64_t* bar) {
+__device__ __forceinline__ void tma_tile(void* dst, const CUtensorMap* map, int x, int row,
+                                         int piece, uint64_t* bar) {
     if constexpr (PAIR)
         asm volatile(
             "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.tile"
             ".mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
                 tbk::smem_addr(dst)),
-            "l"(map), "r"(x), "r"(y), "r"(0), "r"(peer(bar, 0))
+            "l"(map), "r"(x), "r"(row), "r"(piece), "r"(peer(bar, 0))
             : "memory");
     else
         asm volatile(
             "cp.async.bulk.tensor.3d.shared::cta.global.tile.mbarrier::complete_tx::bytes "
             "[%0], [%1, {%2, %3, %4}], [%5];" ::"r"(tbk::smem_addr(dst)),
-            "l"(map), "r"(x), "r"(y), "r"(0), "r"(tbk::smem_addr(bar))
+            "l"(map), "r"(x), "r"(row), "r"(piece), "r"(tbk::smem_addr(bar))
             : "memory");
 }
 
@@ -172,9 +173,11 @@ k_linear(const __grid_constant__ Args a) {
             tbk::mbar_init(&sh.full[i], 1);
             tbk::mbar_init(&sh.scaled[i], H::kScaleWarps);
             tbk::mbar_init(&sh.empty[i], 1);
+        }
+        for (int i = 0; i < H::kAhead; ++i) {
+            tbk::mbar_init(&sh.asked[i], 1);
             tbk::mbar_init(&sh.other[i], 1);
         }
-        for (int i = 0; i < H::kAhead; ++i) tbk::mbar_init(&sh.asked[i], 1);
         tbk::mbar_init(&sh.scales_done, H::kScaleWarps);
         tbk::mbar_init(&sh.sums, 1);
         tbk::mbar_init(&sh.drained, (PAIR ? 2 : 1) * H::kStoreWarps);
@@ -248,11 +251,16 @@ k_linear(const __grid_constant__ Args a) {
                     uint64_t* bar = &sh.full[stage];
                     if (!PAIR || rank == 0)
                         tbk::mbar_expect_tx(bar, (PAIR ? 2 : 1) * a.code_bytes);
+                    if (PAIR && !a.flat) {
+                        tma_tile<PAIR>(to, &a.w_map, 0, out, j * kPieces, bar);
+                        tma_tile<PAIR>(to + a.x_off, &a.x_map, 0, row, j * kPieces, bar);
+                    } else {
 #pragma unroll
-                    for (int p = 0; p < kPieces; ++p) {
-                        const int x = (j * kPieces + p) * 128;  // (bytes, or 4-bit elements)
-                        tma_tile<PAIR>(to + p * kOuts * kPieceBytes, &a.w_map, x, out, bar);
-                        tma_tile<PAIR>(to + a.x_off + p * a.x_piece, &a.x_map, x, row, bar);
+                        for (int p = 0; p < kPieces; ++p) {
+                            const int x = (j * kPieces + p) * 128;  // (bytes, or 4-bit elements)
+                            tma_tile<PAIR>(to + p * kOuts * kPieceBytes, &a.w_map, x, out, 0, bar);
+                            tma_tile<PAIR>(to + a.x_off + p * a.x_piece, &a.x_map, x, row, 0, bar);
+                        }
                     }
                     if constexpr (PAIR) {
                         while (asked < total && asked < kAhead + max(0, issued - a.stages + 1)) ask();
@@ -332,8 +340,9 @@ k_linear(const __grid_constant__ Args a) {
                 if (!fine) break;
                 if (part == 0 && lane == 0) sh.taken = done + 1;
                 if (rank == 0) {
-                    fine = done < a.stages || wait_all(&sh.empty[stage], parity ^ 1, a.status);
-                    fine = fine && wait_all(&sh.other[stage], parity, a.status);
+                    fine = wait_all(&sh.other[slot], slot_parity, a.status);
+                    if (fine && done >= a.stages)
+                        fine = wait_all(&sh.empty[stage], parity ^ 1, a.status);
                     if (!fine) break;
                     tc::fence_after();
                     const uint32_t from = tbk::smem_addr(ring) + slot * kEach * mx::kTileBytes;
@@ -354,7 +363,8 @@ k_linear(const __grid_constant__ Args a) {
                     // (by the first CTA alone: the other's issuer does not wait)
                     tc::commit(&sh.scaled[stage], leader, PAIR);
                 } else if (lane == 0) {
-                    arrive_first(&sh.other[stage]);
+                    // (the slot is asked for again when this step's products are done)
+                    arrive_first(&sh.other[slot]);
                 }
                 if (++step == last) step = first;
                 if (++slot == kAhead) {
@@ -600,17 +610,18 @@ int plan_of(Plan& p, const TbB200Mx* x, const TbB200Mx* w, bool both4, int sm_co
     return TB_OK;
 }
 
-// Pieces of `rows` rows, 128 bytes of codes each: packed, or with fill beside 8-bit codes.
-int map_of(CUtensorMap* map, const TbB200Mx* t, int rows, bool packed) {
+// Tiles of `rows` rows and one piece of 128 bytes, or (not flat) two pieces, one after the
+// other in shared memory: codes packed, or with fill beside 8-bit codes.
+int map_of(CUtensorMap* map, const TbB200Mx* t, int rows, bool flat, bool packed) {
     const uint64_t pitch = (uint64_t)mx::pitch_of(t->format, t->cols);
-    const uint64_t strides[2] = {pitch, pitch * (uint64_t)t->rows};
-    const uint32_t box[3] = {kPieceBytes, (uint32_t)rows, 1};
-    if (t->format == mx::kE2m1 && !packed) {
-        const uint64_t dims[3] = {2 * pitch, (uint64_t)t->rows, 1};
-        return tbh::encode_tiles_u4(map, t->codes, dims, strides, box, 128);
-    }
-    const uint64_t dims[3] = {pitch, (uint64_t)t->rows, 1};
-    return tbh::encode_tiles_u8(map, t->codes, dims, strides, box, 128);
+    const bool fill = t->format == mx::kE2m1 && !packed;
+    const uint64_t wide = fill ? kPieceBytes / 2 : kPieceBytes;  // a piece's bytes in memory
+    const uint64_t dims[3] = {flat ? pitch * kPieceBytes / wide : kPieceBytes, (uint64_t)t->rows,
+                              flat ? 1 : pitch / wide};
+    const uint64_t strides[2] = {pitch, flat ? pitch * (uint64_t)t->rows : wide};
+    const uint32_t box[3] = {kPieceBytes, (uint32_t)rows, flat ? 1u : 2u};
+    return fill ? tbh::encode_tiles_u4(map, t->codes, dims, strides, box, 128)
+                : tbh::encode_tiles_u8(map, t->codes, dims, strides, box, 128);
 }
 
 template <typename T, bool BOTH4, bool PAIR>
@@ -665,8 +676,11 @@ extern "C" int tb_b200_mx_linear(const TbB200Mx* x, const TbB200Mx* w, const flo
     rc = plan_of(p, x, w, both4, ds->sm_count);
     if (rc != TB_OK) return rc;
     Args a = {};
-    rc = map_of(&a.w_map, w, kOuts, both4);
-    if (rc == TB_OK) rc = map_of(&a.x_map, x, p.x_rows, both4);
+    // (rows that end within a piece of packed codes are not whole pieces)
+    const int pieces = p.pair ? 2 : 1;
+    a.flat = !p.pair || (both4 && mx::tiles_of(x->cols) % 2);
+    rc = map_of(&a.w_map, w, kOuts, a.flat, both4);
+    if (rc == TB_OK) rc = map_of(&a.x_map, x, p.x_rows, a.flat, both4);
     if (rc != TB_OK) return rc;
     a.w_scales = w->scales;
     a.x_scales = x->scales;
@@ -685,7 +699,6 @@ extern "C" int tb_b200_mx_linear(const TbB200Mx* x, const TbB200Mx* w, const flo
     a.split = p.split;
     a.stages = p.stages;
     a.stage_bytes = p.stage_bytes;
-    const int pieces = p.pair ? 2 : 1;
     a.x_off = pieces * kOuts * kPieceBytes;
     a.x_piece = p.x_rows * kPieceBytes;
     a.code_bytes = pieces * ((kOuts * kPieceBytes >> (w->format == mx::kE2m1 && !both4)) +
