@@ -541,8 +541,8 @@ int tb_b200_mx_quantize(int dtype, const void* x, int64_t x_stride, const TbB200
 int tb_b200_mx_dequantize(const TbB200Mx* t, int dtype, void* y, int64_t y_stride, void* stream);
 
 /* tb_b200_residual_rms_norm with y in a microscaled format (y->rows rows of y->cols): the
- * same h and f32 arithmetic, and y's f32 values to codes and scales as tb_b200_mx_quantize
- * takes them there, without a rounding between.  residual NULL: the norm of x; weight and
+ * same h; y's f32 values (from sums of squares in double, with one rounding and little more)
+ * go to codes and scales as tb_b200_mx_quantize takes them there.  residual NULL: the norm of x; weight and
  * h_out may be NULL; h_out may be x or residual. */
 int tb_b200_residual_rms_norm_mx(int dtype, const void* x, const void* residual,
                                  const void* weight, void* h_out, const TbB200Mx* y, float eps,

@@ -1,9 +1,10 @@
 // k_mx_rows.cu -- rows to microscaled formats (mx.cuh): quantised as they are, behind
 // SwiGLU, or behind a residual add and RMSNorm; and back to values.
 //
-// A thread has 32 bytes of a row (16 bf16 or 8 f32), so a block of 32 elements is 2 or 4
-// neighbouring lanes, its largest magnitude 1 or 2 shuffles, and the four scales of a tile's
-// row one 32-bit store.  All are HBM bound: the inputs once, codes and scales once.
+// A thread has 32 bytes of a row (16 where rows are reduced first: the norm), so a block of 32
+// elements is 2 to 8 neighbouring lanes, its largest magnitude 1 to 3 shuffles, and the four
+// scales of a tile's row one 32-bit store.  All are HBM bound: the inputs once, codes and
+// scales once.
 #include "bodies.cuh"
 #include "mx.cuh"
 
@@ -13,45 +14,45 @@ using tbk::Elt;
 
 constexpr int kThreads = 256;
 
-// 32 bytes of a row as they are.
-template <typename T>
+// W times 16 bytes of a row as they are.
+template <typename T, int W>
 struct Chunk {
-    static constexpr int E = 32 / sizeof(T);
-    uint4 r[2];
+    static constexpr int V = Elt<T>::kVec, E = W * V;
+    uint4 r[W];
 
     // Elements [at, at + E) of a row of `cols`, zeros past its end; vec: 16-byte aligned.
     __device__ __forceinline__ void load(const T* row, int at, int cols, bool vec) {
         if (vec && at + E <= cols) {
-            const uint4* p = reinterpret_cast<const uint4*>(row + at);
-            r[0] = __ldcs(p);
-            r[1] = __ldcs(p + 1);
+#pragma unroll
+            for (int j = 0; j < W; ++j) r[j] = __ldcs(reinterpret_cast<const uint4*>(row + at) + j);
             return;
         }
-        uint32_t w[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            w[i] = 0;
-            if constexpr (sizeof(T) == 4) {
-                if (at + i < cols) w[i] = reinterpret_cast<const uint32_t*>(row)[at + i];
-            } else {
-                const uint16_t* u = reinterpret_cast<const uint16_t*>(row);
-                if (at + 2 * i < cols) w[i] = u[at + 2 * i];
-                if (at + 2 * i + 1 < cols) w[i] |= (uint32_t)u[at + 2 * i + 1] << 16;
+        for (int j = 0; j < W; ++j) {
+            uint32_t w[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                w[i] = 0;
+                if constexpr (sizeof(T) == 4) {
+                    const int k = at + j * V + i;
+                    if (k < cols) w[i] = reinterpret_cast<const uint32_t*>(row)[k];
+                } else {
+                    const uint16_t* u = reinterpret_cast<const uint16_t*>(row);
+                    const int k = at + j * V + 2 * i;
+                    if (k < cols) w[i] = u[k];
+                    if (k + 1 < cols) w[i] |= (uint32_t)u[k + 1] << 16;
+                }
             }
+            r[j] = make_uint4(w[0], w[1], w[2], w[3]);
         }
-        r[0] = make_uint4(w[0], w[1], w[2], w[3]);
-        r[1] = make_uint4(w[4], w[5], w[6], w[7]);
     }
     __device__ __forceinline__ void widen(float (&v)[E]) const {
-        const uint32_t w[8] = {r[0].x, r[0].y, r[0].z, r[0].w, r[1].x, r[1].y, r[1].z, r[1].w};
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            if constexpr (sizeof(T) == 4) {
-                v[i] = __uint_as_float(w[i]);
-            } else {
-                v[2 * i] = __uint_as_float(w[i] << 16);
-                v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-            }
+        for (int j = 0; j < W; ++j) {
+            float part[V];
+            Elt<T>::template widen<V>(r[j], part);
+#pragma unroll
+            for (int i = 0; i < V; ++i) v[j * V + i] = part[i];
         }
     }
 };
@@ -96,31 +97,63 @@ struct Rows {
     bool vec;
 };
 
+// tbk::silu_f of E elements, the same bits with a shorter division: q = g r, r an approximate
+// reciprocal of d = 1 + e^-g after one of Newton's steps, and q + r (g - q d) is the quotient
+// rounded to nearest (Markstein's theorem), where nothing leaves f32's normal numbers.  (4096
+// rows of 28672 in bf16: 153 us with the exact division's own checks; what bounds the kernel is
+// the instructions.)
+template <int E>
+__device__ __forceinline__ void silu(float (&v)[E]) {
+    float most = 0.0f, least = INFINITY;
+#pragma unroll
+    for (int i = 0; i < E; i += 2) {
+        const float x = fabsf(v[i]), y = fabsf(v[i + 1]);
+        asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(most) : "f"(most), "f"(x), "f"(y));
+        asm("min.f32 %0, %1, %2, %3;" : "=f"(least) : "f"(least), "f"(x), "f"(y));
+    }
+    if (!(most < 80.0f) || least < 1e-20f) {
+#pragma unroll
+        for (int i = 0; i < E; ++i) v[i] = tbk::silu_f(v[i]);
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+        const float d = __fadd_rn(1.0f, expf(-v[i]));
+        float r;
+        asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(d));
+        r = fmaf(r, fmaf(-d, r, 1.0f), r);
+        const float q = v[i] * r;
+        v[i] = fmaf(r, fmaf(-q, d, v[i]), q);
+    }
+}
+
 // A thread an item: chunk c of row r, all rows of whole tiles (behind the last one only the
 // scales are written).
 template <typename T, int FORMAT, bool SWIGLU>
 __global__ void __launch_bounds__(kThreads) k_rows(const Rows<T> in, const mx::View out,
                                                    int chunks, int64_t items, bool small) {
-    constexpr int E = Chunk<T>::E;
+    using C = Chunk<T, 2>;
+    constexpr int E = C::E;
     const int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x;
     int64_t r;
     int c;
     place_of(min(i, items - 1), chunks, small, r, c);
     const bool live = i < items && r < out.rows;
-    float v[E];
-    Chunk<T> x, y;
+    C x, y;
     if (live) {
         x.load(in.a + r * in.a_stride, c * E, out.cols, in.vec);
         if constexpr (SWIGLU) y.load(in.b + r * in.b_stride, c * E, out.cols, in.vec);
     } else {
         x.r[0] = x.r[1] = y.r[0] = y.r[1] = make_uint4(0, 0, 0, 0);
     }
+    float v[E];
     x.widen(v);
     if constexpr (SWIGLU) {
         float u[E];
         y.widen(u);
+        silu<E>(v);
 #pragma unroll
-        for (int e = 0; e < E; ++e) v[e] = tbk::ew_apply<tbk::kSwiglu>(v[e], u[e]);
+        for (int e = 0; e < E; ++e) v[e] = __fmul_rn(v[e], u[e]);
     }
     mx::store_block<FORMAT, E>(out, r, c, live, v);
     if (!live && i < items && c % (128 / E) == 0)
@@ -130,7 +163,7 @@ __global__ void __launch_bounds__(kThreads) k_rows(const Rows<T> in, const mx::V
 template <typename T, bool SWIGLU>
 int launch_rows(const Rows<T>& in, const TbB200Mx* out, cudaStream_t s) {
     const mx::View v = mx::view(out);
-    const int chunks = v.tiles * (128 / Chunk<T>::E);
+    const int chunks = v.tiles * (128 / Chunk<T, 2>::E);
     const int64_t items = mx::tiles_of(v.rows) * 128 * chunks;
     const int64_t grid = (items + kThreads - 1) / kThreads;
     if (grid > INT32_MAX) return TB_ERR_INVALID_SHAPE;
@@ -229,64 +262,99 @@ struct Norm {
 
 // h of a chunk: x + residual in f32, the same bits each time.
 template <typename T>
-__device__ __forceinline__ void sum_of(const Norm<T>& in, const Chunk<T>& x, const Chunk<T>& res,
-                                       float (&h)[Chunk<T>::E]) {
+__device__ __forceinline__ void sum_of(const Norm<T>& in, const Chunk<T, 1>& x, const Chunk<T, 1>& res,
+                                       float (&h)[Chunk<T, 1>::E]) {
     x.widen(h);
     if (in.res) {
-        float r[Chunk<T>::E];
+        float r[Chunk<T, 1>::E];
         res.widen(r);
 #pragma unroll
-        for (int e = 0; e < Chunk<T>::E; ++e) h[e] = __fadd_rn(h[e], r[e]);
+        for (int e = 0; e < Chunk<T, 1>::E; ++e) h[e] = __fadd_rn(h[e], r[e]);
     }
 }
 
 // h and the norm of chunk c of row r, stored.
 template <typename T, int FORMAT>
 __device__ __forceinline__ void finish(const Norm<T>& in, const mx::View& out, int64_t r, int c,
-                                       bool live, float scale, float (&h)[Chunk<T>::E]) {
-    constexpr int E = Chunk<T>::E;
+                                       bool live, float2 scale, float (&h)[Chunk<T, 1>::E]) {
+    constexpr int E = Chunk<T, 1>::E;
     if (live && in.h) store_chunk<T, E>(in.h + r * out.cols, c * E, out.cols, in.vec, h);
+    // h times the factor's two parts times w, to half an ulp and a little: what a product's
+    // rounding leaves out goes on with it
     float w[E];
 #pragma unroll
-    for (int e = 0; e < E; ++e) h[e] = __fmul_rn(h[e], scale);
+    for (int e = 0; e < E; ++e) w[e] = 1.0f;
     if (in.w && live) {
         if (in.vec_w && c * E + E <= out.cols) {
-            const uint4* p = reinterpret_cast<const uint4*>(in.w + c * E);
-            Chunk<T> raw;
-            raw.r[0] = p[0];
-            raw.r[1] = p[1];
+            Chunk<T, 1> raw;
+            raw.r[0] = *reinterpret_cast<const uint4*>(in.w + c * E);
             raw.widen(w);
         } else {
 #pragma unroll
             for (int e = 0; e < E; ++e)
                 w[e] = c * E + e < out.cols ? Elt<T>::load(in.w + c * E + e) : 0.0f;
         }
-#pragma unroll
-        for (int e = 0; e < E; ++e) h[e] = __fmul_rn(h[e], w[e]);
     }
-    // (a row whose scale is NaN or an infinity has fill of zeros all the same)
 #pragma unroll
-    for (int e = 0; e < E; ++e)
-        if (c * E + e >= out.cols) h[e] = 0.0f;
+    for (int e = 0; e < E; ++e) {
+        const float t = h[e] * scale.x, left = fmaf(h[e], scale.y, fmaf(h[e], scale.x, -t));
+        const float y = t * w[e];
+        h[e] = y + fmaf(left, w[e], fmaf(t, w[e], -y));
+    }
+    if (c * E + E > out.cols) {  // (a row whose scale is NaN has fill of zeros all the same)
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+            if (c * E + e >= out.cols) h[e] = 0.0f;
+    }
     mx::store_block<FORMAT, E>(out, r, c, live, h);
 }
 
-__device__ __forceinline__ float scale_of(float ss, float eps, int cols) {
-    return __fdiv_rn(1.0f, __fsqrt_rn(__fdiv_rn(__fadd_rn(ss, eps), (float)cols)));
+// The norm's factor from the sum of squares, as two f32: an error of it moves a whole row's
+// codes the same way, over the same rounding borders.
+__device__ __forceinline__ float2 scale_of(double ss, float eps, int cols) {
+    const double s = 1.0 / sqrt((ss + (double)eps) / (double)cols);
+    const float hi = (float)s;
+    return make_float2(hi, hi < INFINITY ? (float)(s - (double)hi) : 0.0f);
+}
+// The sum over a row's G threads (tbk::group_sum's), in double.
+__device__ __forceinline__ double row_sum(double v, int G, double* red) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(tbk::kFull, v, o);
+    if (G <= 32) return v;
+    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
+    __syncthreads();
+    const int first = threadIdx.x / G * (G >> 5);
+    double s = red[first];
+    for (int w = 1; w < (G >> 5); ++w) s += red[first + w];
+    return s;
+}
+// The squares of a chunk, f32 sums of four each.
+template <int E>
+__device__ __forceinline__ float squares(const float (&h)[E]) {
+    float part[E / 4], sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < E / 4; ++i) {
+        part[i] = __fmul_rn(h[4 * i], h[4 * i]);
+#pragma unroll
+        for (int e = 1; e < 4; ++e) part[i] = __fmaf_rn(h[4 * i + e], h[4 * i + e], part[i]);
+        sum = __fadd_rn(sum, part[i]);
+    }
+    return sum;
 }
 
-// G threads a row, ITEMS chunks a thread, kept in registers as they were loaded.
+// G threads a row, ITEMS chunks a thread, whose sums stay in registers.
 template <typename T, int FORMAT, int ITEMS, int MAXT>
 __global__ void __launch_bounds__(MAXT) k_norm(const Norm<T> in, const mx::View out, int G) {
-    constexpr int E = Chunk<T>::E;
-    __shared__ float red[32];
+    constexpr int E = Chunk<T, 1>::E;
+    __shared__ double red[32];
     const int lane = threadIdx.x & (G - 1);
     const int64_t r = (int64_t)blockIdx.x * (blockDim.x / G) + threadIdx.x / G;
     const bool active = r < out.rows;
     const int chunks = out.tiles * (128 / E);
-    Chunk<T> x[ITEMS], res[ITEMS];
-    float ss = 0.0f;
+    float h[ITEMS][E];
+    double ss = 0.0;
     if (active) {
+        Chunk<T, 1> x[ITEMS], res[ITEMS];
 #pragma unroll
         for (int i = 0; i < ITEMS; ++i) {
             const int c = lane + i * G;
@@ -298,27 +366,22 @@ __global__ void __launch_bounds__(MAXT) k_norm(const Norm<T> in, const mx::View 
 #pragma unroll
         for (int i = 0; i < ITEMS; ++i) {
             if (lane + i * G < chunks) {
-                float h[E];
-                sum_of(in, x[i], res[i], h);
-#pragma unroll
-                for (int e = 0; e < E; ++e) ss = __fmaf_rn(h[e], h[e], ss);
+                sum_of(in, x[i], res[i], h[i]);
+                ss += (double)squares<E>(h[i]);
             }
         }
     }
-    ss = tbk::group_sum(ss, G, red);
-    const float scale = scale_of(ss, in.eps, out.cols);
+    ss = row_sum(ss, G, red);
+    const float2 scale = scale_of(ss, in.eps, out.cols);
 #pragma unroll
     for (int i = 0; i < ITEMS; ++i) {
         const int c = lane + i * G;
         const bool live = active && c < chunks;
-        float h[E];
-        if (live) {
-            sum_of(in, x[i], res[i], h);
-        } else {
+        if (!live) {
 #pragma unroll
-            for (int e = 0; e < E; ++e) h[e] = 0.0f;
+            for (int e = 0; e < E; ++e) h[i][e] = 0.0f;
         }
-        finish<T, FORMAT>(in, out, r, c, live, scale, h);
+        finish<T, FORMAT>(in, out, r, c, live, scale, h[i]);
         if (!active && c < chunks && r < (out.rows + 127) / 128 * 128 && c % (128 / E) == 0)
             *reinterpret_cast<uint32_t*>(out.scales + mx::scales_at(r, c * E / 128, out.tiles)) = 0;
     }
@@ -327,23 +390,22 @@ __global__ void __launch_bounds__(MAXT) k_norm(const Norm<T> in, const mx::View 
 // Rows wider than that: a CTA a row, read twice, the second time from L2.
 template <typename T, int FORMAT>
 __global__ void __launch_bounds__(1024) k_norm_wide(const Norm<T> in, const mx::View out) {
-    constexpr int E = Chunk<T>::E;
-    __shared__ float red[32];
+    constexpr int E = Chunk<T, 1>::E;
+    __shared__ double red[32];
     const int64_t r = blockIdx.x;
     const int chunks = out.tiles * (128 / E);
     const bool active = r < out.rows;
-    float ss = 0.0f;
-    Chunk<T> x, res;
+    double ss = 0.0;
+    Chunk<T, 1> x, res;
     float h[E];
     for (int c = threadIdx.x; active && c < chunks; c += blockDim.x) {
         x.load(in.x + r * out.cols, c * E, out.cols, in.vec);
         if (in.res) res.load(in.res + r * out.cols, c * E, out.cols, in.vec);
         sum_of(in, x, res, h);
-#pragma unroll
-        for (int e = 0; e < E; ++e) ss = __fmaf_rn(h[e], h[e], ss);
+        ss += (double)squares<E>(h);
     }
-    ss = tbk::group_sum(ss, blockDim.x, red);
-    const float scale = scale_of(ss, in.eps, out.cols);
+    ss = row_sum(ss, blockDim.x, red);
+    const float2 scale = scale_of(ss, in.eps, out.cols);
     for (int c0 = 0; c0 < chunks; c0 += blockDim.x) {
         const int c = c0 + threadIdx.x;
         const bool live = active && c < chunks;
@@ -364,7 +426,7 @@ template <typename T, int FORMAT>
 int launch_norm(const Norm<T>& in, const TbB200Mx* y, cudaStream_t s) {
     const mx::View out = mx::view(y);
     const int64_t rows = mx::tiles_of(out.rows) * 128;
-    const tbh::NormCfg c = tbh::norm_cfg((int64_t)out.tiles * (128 / Chunk<T>::E), 1024);
+    const tbh::NormCfg c = tbh::norm_cfg((int64_t)out.tiles * (128 / Chunk<T, 1>::E), 1024);
     const int per = c.threads / c.G;
     const unsigned grid = (unsigned)((rows + per - 1) / per);
     if (c.items == 0) {

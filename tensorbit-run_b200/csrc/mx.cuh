@@ -100,16 +100,30 @@ __device__ __forceinline__ uint32_t e2m1x8(const float* v) {
     return w;
 }
 
-// E neighbouring elements of a row, E = 8 or 16, to codes and scales: the 32 / E lanes of a
+// Four elements as e2m1 codes.
+__device__ __forceinline__ uint16_t e2m1x4(const float* v) {
+    uint16_t w;
+    asm("{\n .reg .b8 a, b;\n cvt.rn.satfinite.e2m1x2.f32 a, %2, %1;\n"
+        " cvt.rn.satfinite.e2m1x2.f32 b, %4, %3;\n mov.b16 %0, {a, b};\n}"
+        : "=h"(w)
+        : "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]));
+    return w;
+}
+
+// E neighbouring elements of a row, E = 4, 8 or 16, to codes and scales: the 32 / E lanes of a
 // block and the 128 / E lanes of a tile are neighbours in a warp.  Chunk c of row r; every
 // lane of the warp calls it, `live` or not.
 template <int FORMAT, int E>
 __device__ __forceinline__ void store_block(const View& out, int64_t r, int c, bool live,
                                             float (&v)[E]) {
     constexpr int kBlock = 32 / E, kLanes = 128 / E;
-    uint32_t top = 0;
+    float most = 0.0f;  // a NaN stays one, and its bits are the largest
 #pragma unroll
-    for (int i = 0; i < E; ++i) top = max(top, __float_as_uint(v[i]) & 0x7fffffffu);
+    for (int i = 0; i < E; i += 2)
+        asm("max.NaN.f32 %0, %1, %2, %3;"
+            : "=f"(most)
+            : "f"(most), "f"(fabsf(v[i])), "f"(fabsf(v[i + 1])));
+    uint32_t top = __float_as_uint(most);
 #pragma unroll
     for (int o = 1; o < kBlock; o <<= 1) top = max(top, __shfl_xor_sync(tbk::kFull, top, o));
     const uint32_t byte = scale_byte<FORMAT>(top);
@@ -122,19 +136,19 @@ __device__ __forceinline__ void store_block(const View& out, int64_t r, int c, b
 #pragma unroll
     for (int i = 0; i < E; ++i) v[i] *= by;
     uint8_t* to = out.codes + r * out.pitch + (int64_t)c * (FORMAT == kE4m3 ? E : E / 2);
-    if constexpr (FORMAT == kE4m3) {
-        uint32_t w[E / 4];
-#pragma unroll
-        for (int i = 0; i < E / 4; ++i) w[i] = e4m3x4(v + 4 * i);
-        if constexpr (E == 16)
-            *reinterpret_cast<uint4*>(to) = make_uint4(w[0], w[1], w[2], w[3]);
-        else
-            *reinterpret_cast<uint2*>(to) = make_uint2(w[0], w[1]);
-    } else if constexpr (E == 16) {
+    if constexpr (FORMAT == kE4m3 && E == 16)
+        *reinterpret_cast<uint4*>(to) =
+            make_uint4(e4m3x4(v), e4m3x4(v + 4), e4m3x4(v + 8), e4m3x4(v + 12));
+    else if constexpr (FORMAT == kE4m3 && E == 8)
+        *reinterpret_cast<uint2*>(to) = make_uint2(e4m3x4(v), e4m3x4(v + 4));
+    else if constexpr (FORMAT == kE4m3)
+        *reinterpret_cast<uint32_t*>(to) = e4m3x4(v);
+    else if constexpr (E == 16)
         *reinterpret_cast<uint2*>(to) = make_uint2(e2m1x8(v), e2m1x8(v + 8));
-    } else {
+    else if constexpr (E == 8)
         *reinterpret_cast<uint32_t*>(to) = e2m1x8(v);
-    }
+    else
+        *reinterpret_cast<uint16_t*>(to) = e2m1x4(v);
     if (lane % kLanes == 0)
         *reinterpret_cast<uint32_t*>(out.scales + scales_at(r, c / kLanes, out.tiles)) = four;
 }

@@ -1000,11 +1000,22 @@ class MxTensor:
         """A tensor of its own, uninitialised memory."""
         torch = _torch()
         device = torch.cuda.current_device() if device is None else device
+        return cls._like(torch.empty(0, dtype=torch.uint8, device=device), rows, cols, format)
+
+    @classmethod
+    def _like(cls, t, rows, cols, format):
+        """empty() on tensor t's device, past the checks of the caller's tensors."""
+        if cols < 1:
+            raise ValueError("an MxTensor has columns")
+        u8 = _torch().uint8
         tiles = -(-cols // 128)
-        return cls(torch.empty((rows, tiles * (64 if format == "e2m1" else 128)),
-                               dtype=torch.uint8, device=device),
-                   torch.empty(-(-rows // 128) * tiles * 512, dtype=torch.uint8, device=device),
-                   cols, format)
+        self = cls.__new__(cls)
+        self.codes = codes = t.new_empty((rows, tiles * (64 if format == "e2m1" else 128)),
+                                         dtype=u8)
+        self.scales = scales = t.new_empty(-(-rows // 128) * tiles * 512, dtype=u8)
+        self.c = Mx(MX_FORMATS[format], rows, cols, codes.data_ptr(), scales.data_ptr())
+        self.format, self.device, self.rows, self.cols = format, t.get_device(), rows, cols
+        return self
 
 
 def _mx(t, dev, what):
@@ -1013,9 +1024,9 @@ def _mx(t, dev, what):
     return t.c
 
 
-def _mx_out(other, dev, out, rows, cols, format):
+def _mx_out(other, dev, out, like, rows, cols, format):
     if out is None:
-        return _new(other, MxTensor.empty, rows, cols, format, dev)
+        return _new(other, MxTensor._like, like, rows, cols, format)
     if (out.rows, out.cols) != (rows, cols):
         raise ValueError(f"out must be [{rows}, {cols}]")
     _mx(out, dev, "out")
@@ -1043,7 +1054,7 @@ def mx_quantize(x, format="e4m3", out=None, stream=None):
     torch, dev = _here()
     stream, other = _stream(torch, dev, stream)
     code, stride = _rows(x, dev, "x")
-    out = _mx_out(other, dev, out, x.shape[0], x.shape[1], format)
+    out = _mx_out(other, dev, out, x, x.shape[0], x.shape[1], format)
     check(lib().tb_b200_mx_quantize(code, x.data_ptr(), stride, out.c, stream), "mx_quantize")
     return out
 
@@ -1055,8 +1066,8 @@ def mx_dequantize(t, dtype=None, out=None, stream=None):
     stream, other = _stream(torch, dev, stream)
     c = _mx(t, dev, "t")
     if out is None:
-        out = _new(other, torch.empty, (t.rows, t.cols),
-                   dtype=torch.float32 if dtype is None else dtype, device=dev)
+        out = _new(other, t.codes.new_empty, (t.rows, t.cols),
+                   dtype=torch.float32 if dtype is None else dtype)
     elif out.shape != (t.rows, t.cols):
         raise ValueError(f"out must be [{t.rows}, {t.cols}]")
     code, stride = _rows(out, dev, "out", dtype)
@@ -1080,7 +1091,7 @@ def residual_rms_norm_mx(x, residual, weight, eps, h_out=None, format="e4m3", ou
     if h_out is None and residual is not None:
         h_out = _new(other, torch.empty_like, x)
     h = None if h_out is None else _flat(h_out, dtype, n, dev, "h_out")
-    out = _mx_out(other, dev, out, rows, cols, format)
+    out = _mx_out(other, dev, out, x, rows, cols, format)
     check(lib().tb_b200_residual_rms_norm_mx(code, *at, h, out.c, eps, stream),
           "residual_rms_norm_mx")
     return h_out, out
@@ -1095,7 +1106,7 @@ def swiglu_mx(gate, up, format="e4m3", out=None, stream=None):
     _, us = _rows(up, dev, "up", gate.dtype)
     if up.shape != gate.shape:
         raise ValueError("gate and up must have the same shape")
-    out = _mx_out(other, dev, out, gate.shape[0], gate.shape[1], format)
+    out = _mx_out(other, dev, out, gate, gate.shape[0], gate.shape[1], format)
     check(lib().tb_b200_swiglu_mx(code, gate.data_ptr(), gs, up.data_ptr(), us, out.c, stream),
           "swiglu_mx")
     return out
@@ -1109,8 +1120,8 @@ def mx_linear(x, w, bias=None, dtype=None, y=None, stream=None):
     stream, other = _stream(torch, dev, stream)
     xc, wc = _mx(x, dev, "x"), _mx(w, dev, "w")
     if y is None:
-        y = _new(other, torch.empty, (x.rows, w.rows),
-                 dtype=torch.bfloat16 if dtype is None else dtype, device=dev)
+        y = _new(other, x.codes.new_empty, (x.rows, w.rows),
+                 dtype=torch.bfloat16 if dtype is None else dtype)
     elif y.shape != (x.rows, w.rows):
         raise ValueError(f"y must be [{x.rows}, {w.rows}]")
     code, stride = _rows(y, dev, "y", dtype)
@@ -1134,7 +1145,7 @@ def sample(logits, uniforms, temperature=None, top_k=None, top_p=None, min_p=Non
         return None if t is None else _flat(t, dtype, rows, dev, what)
 
     if out is None:
-        out = _new(other, torch.empty, rows, dtype=torch.int32, device=dev)
+        out = _new(other, logits.new_empty, rows, dtype=torch.int32)
     t = Sample(code, rows, vocab, logits.data_ptr(), stride,
                setting(temperature, f, "temperature"), setting(top_k, torch.int32, "top_k"),
                setting(top_p, f, "top_p"), setting(min_p, f, "min_p"),
