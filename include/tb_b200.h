@@ -542,8 +542,8 @@ int tb_b200_mx_dequantize(const TbB200Mx* t, int dtype, void* y, int64_t y_strid
 
 /* tb_b200_residual_rms_norm with y in a microscaled format (y->rows rows of y->cols): the
  * same h; y's f32 values (from sums of squares in double, with one rounding and little more)
- * go to codes and scales as tb_b200_mx_quantize takes them there.  residual NULL: the norm of x; weight and
- * h_out may be NULL; h_out may be x or residual. */
+ * go to codes and scales as tb_b200_mx_quantize takes them there.  residual NULL: the norm
+ * of x; weight and h_out may be NULL; h_out may be x or residual. */
 int tb_b200_residual_rms_norm_mx(int dtype, const void* x, const void* residual,
                                  const void* weight, void* h_out, const TbB200Mx* y, float eps,
                                  void* stream);
@@ -569,8 +569,8 @@ int tb_b200_mx_linear(const TbB200Mx* x, const TbB200Mx* w, const float* bias, i
 
 /* One token of each row of logits (f32 or bf16, `stride` elements apart), by the row's own
  * settings, device arrays of one value per row; NULL is off:
- *   temperature  w_i = exp((x_i - max x) / temperature); <= 0 or NaN: the first largest
- *                logit; NULL: 1
+ *   temperature  w_i = exp((x_i - max x) / temperature); below 2^-126 or NaN: the first
+ *                largest logit; NULL: 1
  *   top_k        of the k largest logits (of equal ones the first); <= 0: of all
  *   top_p        of those, in falling order (equal ones in their order), the ones whose
  *                predecessors' weights sum to less than top_p of the sum of all of those,

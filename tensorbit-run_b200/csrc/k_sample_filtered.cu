@@ -66,11 +66,12 @@ struct Weights {
     double top, scale;          // y = (x - top) scale
     const double* table;
     int shift;
-    // (a temperature above 1 takes half of each logit, whose difference is within f32)
+    // (a temperature above 1 takes half of each logit, whose difference is within f32; one
+    // below f32's normal numbers, whose reciprocal is not, does not come here)
     __device__ Weights(float top_, float t, const double* table, int shift)
         : part(t > 1.0f ? 0.5f : 1.0f), part_top(top_ * part), top(top_),
           scale(1.4426950408889634074 / (double)t), table(table), shift(shift) {
-        per = (float)fmin(scale / part, 3e38);
+        per = (float)(scale / part);
     }
     // How far a logit lies below the top, in halvings of its weight; NaN stays NaN.
     __device__ __forceinline__ float fall(float x) const { return fmaf(-part, x, part_top) * per; }
@@ -504,7 +505,7 @@ struct Row {
         int b0, b1, t = 0;
         bool few;  // all that is above and in the bins
         if constexpr (BY_WEIGHT) {
-            const double mass = (double)set.p * (double)whole;
+            const double mass = fmax((double)set.p, 0.0) * (double)whole;
             reach(h, before, max((u64)(mass * (1 - 0x1p-13)), 1ull),
                   (u64)(mass * (1 + 0x1p-13)) + 1, b0, b1);
             // exact: the sum of all, of what is above the bins, and how many there are
@@ -707,7 +708,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample(const Args a) {
         if (row.rank == 0 && threadIdx.x == 0) a.out[at] = 0;
         return;
     }
-    if (!(t > 0.0f) || min_p > 1.0f) {
+    if (!(t >= 0x1p-126f) || min_p > 1.0f) {
         v[0] = 0;
         row.each([&](float x, int i) {
             if (x == top) v[0] = max(v[0], (u64)~(uint32_t)i);

@@ -73,7 +73,7 @@ def draw(x, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     if not ok.any():
         return 0
     top = x[ok].max()
-    if not temperature > 0:
+    if not temperature >= 2.0 ** -126:
         return int(np.flatnonzero(x == top)[0])
     with np.errstate(invalid="ignore"):
         w = np.where(x == top, 1.0, np.exp((x - top) / temperature))

@@ -103,6 +103,24 @@ def test_ends_of_temperature(temperature):
     check(x, r.random(50), temperature=np.full(50, temperature))
 
 
+def test_least_temperatures():
+    """Equal logits, and ones a least number apart, either side of 2^-126."""
+    x = torch.zeros(40, 300, device="cuda")
+    x[:, 100:] = 2.0 ** -149
+    x[:, 200:250] = 2.0 ** -130
+    r = np.random.default_rng(19)
+    t = np.tile([2.0 ** -126, 2.0 ** -127, 2.0 ** -149, 2.0 ** -125], 10)
+    check(x, r.random(40), temperature=t)
+    check(x, r.random(40), temperature=t, top_p=np.full(40, 0.7), min_p=np.full(40, 0.9))
+
+
+def test_negative_top_p_keeps_one():
+    r = np.random.default_rng(20)
+    x = torch.from_numpy(r.standard_normal((12, 3000))).float().cuda()
+    got = check(x, r.random(12), top_p=np.tile([-1.0, -np.inf, 0.0], 4))
+    assert torch.equal(torch.from_numpy(got).long(), x.argmax(-1).cpu())
+
+
 def test_nan_settings_are_off():
     r = np.random.default_rng(12)
     x = torch.from_numpy(r.standard_normal((30, 100))).float().cuda()
