@@ -1,14 +1,29 @@
 // k_mx_linear.cu -- y = x w^T (+ bias) of microscaled x [rows, cols] and w [outs, cols], on
 // the block-scaled matrix instructions.
 //
-// w is the left operand: a tile is 128 outs by up to 256 rows of x, its sums in tensor memory
-// as [out][row].  So a single row of x is as good a tile as many (the instruction takes 16
-// columns at least), and w, the larger side in serving, is read once for up to 256 rows.
-// One warp asks for operands by TMA, one for scales, further ahead, and copies them to tensor
-// memory (stores from registers to there waited for the products: 1700 clocks a step), one
-// issues the products, four or eight bring a tile's sums to y, a lane an out.  Where the tiles do not
-// fill the SMs, the CTAs of a cluster take parts of cols and add them up, in order, through
-// one another's shared memory.
+// w is the left operand: a tile is 128 outs by some rows of x, its sums in tensor memory as
+// [out][row].  So a single row of x is as good a tile as many (the instruction takes 16 columns
+// at least), and w, the larger side in serving, is read once for up to 256 rows.  Two shapes:
+//
+// Above 128 rows of x, two CTAs (a pair of SMs) have a tile of 256 outs by 256 rows together:
+// each loads half of either operand, and the first one's products read both halves.  The
+// scales of 128 rows and 128 columns are 512 bytes that one copy of the tensor pipe brings from
+// shared to tensor memory; two warps share those of a step.  What bounds it: a step's chain of
+// loads (about 3000 clocks from far memory), copies of scales and products over the three
+// stages that fit; the tensor pipe is busy for 56 % of the time by the profiler's count.
+//   4096 x 8192 x 28672: 8-bit rows and 4-bit weights 835 us (2.3 PFLOP/s), both 8 bits 905
+//   us, both 4 bits 420 us (4.6 PFLOP/s); bf16 products of that size take 1150 us at the
+//   fastest.  Stores of scales from registers waited for the products in flight, 1700 clocks a
+//   step (806 us for 4 bits); copies by one warp, that asked for them too, took 543 us.
+//
+// Up to 128 rows it is w's bytes that count, and then latency: one tile of 128 outs a CTA, two
+// CTAs an SM, one's loads under the other's epilogue, scales through registers (products are
+// few, nothing waits for them).  Where the tiles leave SMs idle, the CTAs of a cluster take
+// parts of cols and add them up, in order, through one another's shared memory.
+//   64 x 8192 x 128256, 4-bit weights to f32: 134 us (4.4 TB/s of the bytes there have to be);
+//   one CTA an SM 419 us, three 152.  1 x 4096 x 4096: 9.5 us, of which a launch and the first
+//   loads are the most.  Asking for w ahead into L2 made it slower (72 -> 85 us for 57344
+//   outs), as did a K split in rounds.
 #include <atomic>
 
 #include "mx.cuh"
@@ -20,7 +35,8 @@ namespace {
 
 // warps
 constexpr int kLoader = 0, kIssuer = 1;
-constexpr int kOuts = 128, kMostStages = 8, kMostAhead = 8, kMostSplit = 8;  // kOuts: of a CTA's tile
+constexpr int kOuts = 128;  // of a CTA's tile
+constexpr int kMostStages = 8, kMostAhead = 8, kMostSplit = 8;
 constexpr int kPieceBytes = 128;  // of a row of codes; a step has one or two such pieces
 constexpr uint64_t kLimit = 1000000000ull;  // ns, of a wait
 
@@ -145,7 +161,6 @@ struct Shape {
     static constexpr int kEach = (1 + kMostX) * kTiles;       // a step's tiles of scales
     static constexpr int kScaleColumns = 4 * kEach;
     static constexpr int kAhead = PAIR && BOTH4 ? 4 : 8;  // steps' scales asked for
-    static_assert(kAhead >= (PAIR ? 3 : kMostStages), "a stage's scales are asked for before it is taken");
     static constexpr int kScaleBytes = kAhead * kEach * mx::kTileBytes;
     static constexpr int kStaged = PAIR ? 8192 : 0;  // bytes of y on their way
 };
@@ -326,9 +341,7 @@ k_linear(const __grid_constant__ Args a) {
         }
     } else if (warp < H::kStorers) {
         if constexpr (PAIR) {
-            // Two warps, half of a step's copies of scales to tensor memory each, by the tensor
-            // pipe (stores from registers wait for the pair's products, 1700 clocks a step; one
-            // warp, that asked for them too, took 2000 clocks a step).
+            // Two warps, half of a step's copies of scales to tensor memory each.
             constexpr int kAhead = H::kAhead;
             const int part = warp - H::kScalers;
             const bool leader = lane == 0;
@@ -353,15 +366,15 @@ k_linear(const __grid_constant__ Args a) {
                     for (int i = 0; i < kTiles / 2; ++i) {
                         const int h = 2 * i + part;
                         if (h >= have) break;
-                        tc::copy_scales<PAIR>(w_to + 4 * h, from + h * mx::kTileBytes, leader);
+                        tc::copy_scales(w_to + 4 * h, from + h * mx::kTileBytes, leader);
 #pragma unroll
                         for (int k = 0; k < kMostX; ++k)
-                            tc::copy_scales<PAIR>(x_to + 4 * (kMostX * h + k),
-                                                  from + ((1 + k) * kTiles + h) * mx::kTileBytes,
-                                                  leader);
+                            tc::copy_scales(x_to + 4 * (kMostX * h + k),
+                                            from + ((1 + k) * kTiles + h) * mx::kTileBytes,
+                                            leader);
                     }
                     // (by the first CTA alone: the other's issuer does not wait)
-                    tc::commit(&sh.scaled[stage], leader, PAIR);
+                    tc::commit_of_pair(&sh.scaled[stage], leader);
                 } else if (lane == 0) {
                     // (the slot is asked for again when this step's products are done)
                     arrive_first(&sh.other[slot]);
@@ -378,13 +391,13 @@ k_linear(const __grid_constant__ Args a) {
             }
             if (rank == 0) {
                 // no copy to tensor memory may be in flight when that is freed
-                tc::commit(&sh.scales_done, leader, PAIR);
+                tc::commit_of_pair(&sh.scales_done, leader);
                 wait_all(&sh.scales_done, 0, a.status);
             }
         } else {
             // Four warps: scales to shared memory, kAhead - 1 steps ahead, by all of them; from
-            // there through registers, each to its quarter of the rows of tensor memory, a lane the words
-            // of rows l, l + 32, l + 64 and l + 96.
+            // there through registers, each to its quarter of the rows of tensor memory, a lane
+            // the words of rows l, l + 32, l + 64 and l + 96.
             constexpr int kAhead = H::kAhead, kChunks = kEach * 32;
             const uint32_t to = tmem + a.scales_column + ((uint32_t)(warp % 4) << 21);
             const int thread = threadIdx.x - 32 * H::kScalers;
@@ -586,7 +599,6 @@ int plan_of(Plan& p, const TbB200Mx* x, const TbB200Mx* w, bool both4, int sm_co
     if (n_tiles * kMostSplit > INT32_MAX) return TB_ERR_INVALID_SHAPE;
     p.n_tiles = (int)n_tiles;
     p.stage_bytes = pieces * (kOuts + p.x_rows) * kPieceBytes;
-    // two CTAs an SM (64 rows of 8192 to 128256: one 419 us, two 135, three 152)
     const int scales = p.pair ? Shape<false, true>::kScaleBytes
                        : both4 ? Shape<true, false>::kScaleBytes : Shape<false, false>::kScaleBytes;
     static_assert(Shape<false, true>::kScaleBytes == Shape<true, true>::kScaleBytes, "scales");

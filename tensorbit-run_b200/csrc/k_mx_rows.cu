@@ -3,8 +3,13 @@
 //
 // A thread has 32 bytes of a row (16 where rows are reduced first: the norm), so a block of 32
 // elements is 2 to 8 neighbouring lanes, its largest magnitude 1 to 3 shuffles, and the four
-// scales of a tile's row one 32-bit store.  All are HBM bound: the inputs once, codes and
-// scales once.
+// scales of a tile's row one 32-bit store.  Bytes are the inputs once, codes and scales once;
+// what bounds the kernels now is their instructions (issue slots are 65 to 73 % busy, DRAM 40 to
+// 51 %), most of which widen, scale and round:
+//   28672 x 8192 bf16 to 4 bits 230 us (5.1 TB/s); 283 with 16 bytes a thread, more with two
+//   or four pieces of work a thread
+//   SwiGLU 4096 x 28672 bf16 140 us (4.2 TB/s)
+//   norm 16384 x 8192 bf16 with the residual 198 us (4.8 TB/s); 188 with products rounded twice
 #include "bodies.cuh"
 #include "mx.cuh"
 
@@ -99,9 +104,11 @@ struct Rows {
 
 // tbk::silu_f of E elements, the same bits with a shorter division: q = g r, r an approximate
 // reciprocal of d = 1 + e^-g after one of Newton's steps, and q + r (g - q d) is the quotient
-// rounded to nearest (Markstein's theorem), where nothing leaves f32's normal numbers.  (4096
-// rows of 28672 in bf16: 153 us with the exact division's own checks; what bounds the kernel is
-// the instructions.)
+// rounded to nearest (Markstein's theorems) where nothing leaves f32's normal numbers and d's
+// mantissa is not all ones, r then being the nearest to 1 / d.  With all ones r may be 2^-k in
+// place of 2^-k (1 + 2^-23), and the quotient comes out wrong only for g = 2^j: of those, 2^-23
+// alone has such a d.  (4096 rows of 28672 in bf16: 153 us with the exact division's own checks,
+// 140 so.)
 template <int E>
 __device__ __forceinline__ void silu(float (&v)[E]) {
     float most = 0.0f, least = INFINITY;
@@ -111,7 +118,7 @@ __device__ __forceinline__ void silu(float (&v)[E]) {
         asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(most) : "f"(most), "f"(x), "f"(y));
         asm("min.f32 %0, %1, %2, %3;" : "=f"(least) : "f"(least), "f"(x), "f"(y));
     }
-    if (!(most < 80.0f) || least < 1e-20f) {
+    if (!(most < 80.0f) || least < 0x1p-22f) {
 #pragma unroll
         for (int i = 0; i < E; ++i) v[i] = tbk::silu_f(v[i]);
         return;

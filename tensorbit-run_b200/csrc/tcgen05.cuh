@@ -62,15 +62,12 @@ __device__ __forceinline__ void commit(uint64_t* bar, bool leader) {
         : "memory");
 }
 // The same for products or copies of a pair of CTAs, on this CTA's bar alone.
-__device__ __forceinline__ void commit(uint64_t* bar, bool leader, bool pair) {
-    if (!pair)
-        commit(bar, leader);
-    else
-        asm volatile(
-            "{\n .reg .pred q;\n setp.ne.u32 q, %1, 0;\n @q tcgen05.commit.cta_group::2"
-            ".mbarrier::arrive::one.shared::cluster.b64 [%0];\n}" ::"r"(tbk::smem_addr(bar)),
-            "r"((uint32_t)leader)
-            : "memory");
+__device__ __forceinline__ void commit_of_pair(uint64_t* bar, bool leader) {
+    asm volatile(
+        "{\n .reg .pred q;\n setp.ne.u32 q, %1, 0;\n @q tcgen05.commit.cta_group::2"
+        ".mbarrier::arrive::one.shared::cluster.b64 [%0];\n}" ::"r"(tbk::smem_addr(bar)),
+        "r"((uint32_t)leader)
+        : "memory");
 }
 __device__ __forceinline__ void fence_before() {
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -214,27 +211,18 @@ __device__ __forceinline__ void release_pair(uint32_t address, uint32_t columns)
                  : "memory");
 }
 // 512 bytes of scales in shared memory (32 rows of 16 bytes, on 16 bytes) to 4 columns of
-// tensor memory, in every 32 lanes; PAIR: of both CTAs, from their own shared memory.
-template <bool PAIR>
+// tensor memory, in every 32 lanes, of both CTAs of a pair, from their own shared memory.
 __device__ __forceinline__ void copy_scales(uint32_t to, uint32_t smem, bool leader) {
     const uint64_t from = (uint64_t)((smem >> 4) & 0x3fff) |  // start
                           (uint64_t)(128 >> 4) << 16 |        // leading dimension: one wide
                           (uint64_t)(128 >> 4) << 32 |        // 8 rows further
                           1ull << 46;                         // the version; no swizzle
-    if constexpr (PAIR)
-        asm volatile(
-            "{\n .reg .pred q;\n setp.ne.u32 q, %2, 0;\n"
-            " @q tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;\n}" ::"r"(to),
-            "l"(from), "r"((uint32_t)leader)
-            : "memory");
-    else
-        asm volatile(
-            "{\n .reg .pred q;\n setp.ne.u32 q, %2, 0;\n"
-            " @q tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;\n}" ::"r"(to),
-            "l"(from), "r"((uint32_t)leader)
-            : "memory");
+    asm volatile(
+        "{\n .reg .pred q;\n setp.ne.u32 q, %2, 0;\n"
+        " @q tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;\n}" ::"r"(to),
+        "l"(from), "r"((uint32_t)leader)
+        : "memory");
 }
-
 // Four columns of the warp's 32 rows, a row a lane: the scales of 128 rows and 4 blocks, of
 // which lane l has the words of rows l, l + 32, l + 64 and l + 96 (every quarter of the rows
 // has them all).

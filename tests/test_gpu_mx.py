@@ -2,9 +2,11 @@
 
 Quantising is exact by definition (a power-of-two scale, one rounding), so its values and
 scales are equal.  Where a row op comes first, its f32 result y is off by at most REL |y|:
-RMSNorm's sum of squares is a chain of at most 64 terms a thread (128 in the wide form) and
-10 levels of a tree, 138 * 2^-24 of the sum and half of that of its root, 6 more roundings:
-75 * 2^-24 < 2^-17; SwiGLU has expf (2 ulp) and 4 roundings, less where -x cancels nothing.
+RMSNorm's squares are summed in f32 8 at a time, each with 8 roundings, then in double; half of
+that of the root, and 4 more of h and its product with the factor and the weight: 8 * 2^-24;
+residual_rms_norm, whose rows are compared with it, sums in f32: a chain of at most 128 terms a
+thread and 10 levels of a tree, 138 * 2^-24 of the sum and half of that of its root, 6 more
+roundings: 75 * 2^-24 < 2^-17.  SwiGLU has expf (2 ulp) and 4 roundings.
 A code is then off by half a step of y + its error, with a scale that may be the next one
 where the block's largest is within REL of a border.
 
@@ -234,6 +236,21 @@ def test_swiglu_mx(rows, cols, dtype, fmt):
     assert torch.equal(t.codes, t2.codes) and torch.equal(t.scales, t2.scales)
 
 
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_swiglu_mx_is_the_row_op(fmt):
+    """swiglu's f32 rows, bit for bit, at gates of all sizes and next to its branches."""
+    g = normal(54, 300, 4096) * torch.exp2(
+        torch.randint(-60, 12, (300, 4096), generator=gen(55), device="cuda") / 2.0)
+    one = torch.ldexp(torch.ones(4096, device="cuda"), torch.arange(4096, device="cuda") % 200 - 140)
+    near = torch.nextafter(one, 2 * one)
+    g[:4] = torch.stack([one, -one, near, -near])
+    g[4] = torch.linspace(79.9, 80.1, 4096, device="cuda")
+    g[5] = -torch.linspace(79.9, 110, 4096, device="cuda")
+    u = normal(56, 300, 4096)
+    t, want = T.swiglu_mx(g, u, fmt), T.mx_quantize(T.swiglu(g, u), fmt)
+    assert torch.equal(t.scales, want.scales) and torch.equal(t.codes, want.codes)
+
+
 # ---------------------------------------------------------------- the product
 def linear_of(x, w, bias=None):
     """(x w^T + bias, the bound on sum |x w|'s error) in float64."""
@@ -265,6 +282,39 @@ def test_linear(rows, cols, outs, xf, wf):
     bias = normal(22, outs)
     check_linear(x, w, None, T.mx_linear(x, w))
     check_linear(x, w, bias, T.mx_linear(x, w, bias, torch.float32))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("off", [0, 3])
+@pytest.mark.parametrize("xf,rows,cols,outs", [
+    ("e4m3", 1290, 300, 4100), ("e2m1", 1290, 640, 4100), ("e2m1", 1290, 200, 4100),
+    ("e4m3", 100, 300, 40007), ("e2m1", 100, 300, 40007)])
+def test_linear_of_several_tiles_a_cta(xf, rows, cols, outs, off, dtype):
+    """More tiles than CTAs, the last of them ragged; rows of y aligned or not."""
+    x, w = T.mx_quantize(normal(57, rows, cols), xf), T.mx_quantize(normal(58, outs, cols), "e2m1")
+    stride = (outs + 15) // 8 * 8 + off % 2
+    y = torch.full((rows, stride), 7.0, dtype=DTYPES[dtype], device="cuda")
+    bias = normal(59, outs)
+    T.mx_linear(x, w, bias, y=y[:, off:off + outs])
+    check_linear(x, w, bias, y[:, off:off + outs])
+    assert (y[:, :off] == 7.0).all() and (y[:, off + outs:] == 7.0).all()
+
+
+@pytest.mark.parametrize("rows", [2, 200])
+def test_linear_of_far_larger_codes_and_scales(rows):
+    """Codes and scales that did not come from mx_quantize: every code but NaN, any scale."""
+    def raw(seed, rows, cols, fmt):
+        t = T.MxTensor.empty(rows, cols, fmt)
+        c = torch.randint(0, 256, t.codes.shape, generator=gen(seed), device="cuda")
+        if fmt == "e4m3":
+            c = torch.where((c & 127) == 127, c - 1, c)
+        t.codes.copy_(c)
+        t.scales.copy_(torch.randint(90, 160, t.scales.shape, generator=gen(seed), device="cuda"))
+        return t
+    for xf in FORMATS:
+        for wf in FORMATS:
+            x, w = raw(60, rows, 384, xf), raw(61, 140, 384, wf)
+            check_linear(x, w, None, T.mx_linear(x, w, dtype=torch.float32))
 
 
 @pytest.mark.parametrize("xf,wf", [("e4m3", "e2m1"), ("e2m1", "e2m1")])
