@@ -19,6 +19,7 @@
 // search in the order of the index.  That search, by exact sums of CTA, warp, slab and lane,
 // makes the draw too.  Where all that is above the border is as few, the last steps are one
 // CTA's, on that list.
+#include <float.h>
 #include <math.h>
 
 #include <atomic>
@@ -75,6 +76,7 @@ struct Weights {
     }
     // How far a logit lies below the top, in halvings of its weight; NaN stays NaN.
     __device__ __forceinline__ float fall(float x) const { return fmaf(-part, x, part_top) * per; }
+    __device__ __forceinline__ float logit_at(float y) const { return (part_top - y / per) / part; }
     __device__ __forceinline__ u64 operator()(float x) const {
         if (!(fall(x) < 64.0f)) return 0;
         constexpr double kLn2 = 0.69314718055994530942;
@@ -134,6 +136,7 @@ struct alignas(16) Shared {
     float x;
     int index;
     uint32_t listed;
+    int over;  // the list is longer than it may be
 };
 
 // (lanes may come from different branches: not the aligned form)
@@ -454,6 +457,7 @@ struct Row {
         float p, least;
         double u;
         int32_t* out;
+        float most;  // the thread's largest logit
     };
 
     // in: to the last element of those inside it, in falling order, whose predecessors sum to
@@ -472,6 +476,46 @@ struct Row {
         };
         sh.bins[threadIdx.x] = 0;
         __syncthreads();
+        if constexpr (!BY_WEIGHT) {
+            // The n-th of the threads' largest is not above the n-th of all, and little below
+            // it where threads are many: what is from its bin on is listed at once, if it fits.
+            if (limit <= kFew * 3 / 4 && 2 * (int)limit <= min(kThreads * a.ctas, a.vocab / V)) {
+                if (set.most > in.x) atomicAdd(&sh.bins[bin_of(w.fall(set.most))], 1u);
+                __syncthreads();
+                u64 n, h = push([&](int b) -> u64 { return sh.bins[b]; });
+                const u64 before = scan(h, n);
+                int b0, b1;
+                reach(h, before, limit, limit, b0, b1);
+                if (n >= limit && b0 < kBins - 1) {
+                    // (any logit does that n of the largest are not below: the bin's lower end)
+                    const float from = fmaxf(w.logit_at((b0 + 0.51f) / kPerHalving), -FLT_MAX);
+                    u64 v[4] = {0, 0, 0, 0};
+                    each([&](float x, int i) {
+                        if (!(x >= from)) return;
+                        ++v[0];
+                        if (*(volatile int*)&sh.over) return;
+                        const uint32_t at = add_to(peer(&sh.listed, 0), 1);
+                        if (at >= kFew) {
+                            sh.over = 1;
+                            return;
+                        }
+                        store_to(peer(sh.members + at, 0),
+                                 (u64)(uint32_t)i << 32 | __float_as_uint(x), 1ull);
+                    });
+                    all<1, 1>(v);
+                    if (v[0] <= kFew) {
+                        if (rank == 0)
+                            draw_few(w, (int)v[0], limit, 0, set.p, set.least, set.u, set.out);
+                        return kDrawn;
+                    }
+                    if (threadIdx.x == 0) sh.listed = 0;
+                } else {
+                    cluster_sync();  // the pushed bins have been read
+                }
+                sh.bins[threadIdx.x] = 0;
+                __syncthreads();
+            }
+        }
         uint32_t rest = 0;  // the last bin's: many rows have most of their elements there
         each([&](float x, int i) {
             if (!in.inside(x, i)) return;
@@ -688,11 +732,11 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample(const Args a) {
     using R = Row<T>;
     extern __shared__ uint4 held[];
     __shared__ Shared sh;
-    if (threadIdx.x == 0) sh.listed = 0;
+    if (threadIdx.x == 0) sh.listed = sh.over = 0;
     cluster_arrive();
     R row(a, sh, held, blockIdx.x % a.ctas);
     const int64_t at = blockIdx.x / a.ctas;
-    const float mine_top = row.load(static_cast<const T*>(a.logits) + at * a.stride);
+    float mine_top = row.load(static_cast<const T*>(a.logits) + at * a.stride);
     u64 v[4] = {key_of(mine_top), 0, 0, 0};
     const float t = a.temperature ? a.temperature[at] : 1.0f;
     const float min_p = a.min_p ? a.min_p[at] : 0.0f, p = a.top_p ? a.top_p[at] : 1.0f;
@@ -728,10 +772,11 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample(const Args a) {
                 tbk::Elt<T>::store(to + e, x[e] == top ? 0.0f : -INFINITY);
         }
         top = 0.0f;
+        mine_top = mine_top == INFINITY ? 0.0f : -INFINITY;
     }
     const Weights w(top, t, sh.table, a.shift);
     const float least = min_p > 0.0f ? least_of((double)min_p, top, (double)t) : -INFINITY;
-    const typename R::Setting set = {p, least, u, a.out + at};
+    const typename R::Setting set = {p, least, u, a.out + at, mine_top};
 
     // everything above -infinity at first
     Border in = {-INFINITY, -1};
