@@ -99,6 +99,11 @@ struct Weights {
     }
 };
 
+// Whether a logit's weight is min_p or more.
+__device__ __forceinline__ bool reaches(float x, double top, double t, double min_p) {
+    return exp(((double)x - top) / t) >= min_p;
+}
+
 struct Border {
     float x;
     int index;  // the last inside of the logits that are x
@@ -424,10 +429,19 @@ struct Row {
         return scaled(sum, q, 53, cut);
     }
 
+    // What a search for a border came to.
+    enum Found { kBorder, kSums, kDrawn };
+    struct Setting {
+        float p;
+        double min_p, t, u;
+        int32_t* out;
+        float most;  // the thread's largest logit
+    };
+
     // The draw from the list, n members: the k first of them, then top-p (whose limit is
-    // p_limit, or, 0, p's share of those k), then min_p (logits of `least` or more).
-    __device__ __forceinline__ void draw_few(const Weights& w, int n, u64 k, u64 p_limit, float p,
-                                             float least, double u, int32_t* out) {
+    // p_limit, or, 0, p's share of those k), then min_p.
+    __device__ __forceinline__ void draw_few(const Weights& w, int n, u64 k, u64 p_limit,
+                                             const Setting& set) {
         Member mine = member_of(n);
         const bool writes = (threadIdx.x & 1) == 0 && (int)(threadIdx.x >> 1) < n;
         const u64 weight = w(mine.x);
@@ -440,25 +454,17 @@ struct Row {
         // (members come with a measure of 1; every lane takes part in the sums)
         u64 sum = sum_before<true>(n, mine);
         hold(mine.measure && sum < k);
-        if (p < 1.0f) {
-            const u64 limit = p_limit ? p_limit : share(block_sum(writes ? mine.measure : 0), p);
+        if (set.p < 1.0f) {
+            const u64 limit =
+                p_limit ? p_limit : share(block_sum(writes ? mine.measure : 0), set.p);
             sum = sum_before<true>(n, mine);
             hold(mine.measure && sum < limit);
         }
-        hold(mine.measure && mine.x >= least);
-        const u64 target = target_of(block_sum(writes ? mine.measure : 0), u);
+        if (set.min_p > 0.0) hold(mine.measure && reaches(mine.x, w.top, set.t, set.min_p));
+        const u64 target = target_of(block_sum(writes ? mine.measure : 0), set.u);
         const u64 before = sum_before<false>(n, mine);
-        if (writes && before <= target && target < before + mine.measure) *out = mine.index;
+        if (writes && before <= target && target < before + mine.measure) *set.out = mine.index;
     }
-
-    // What a search for a border came to.
-    enum Found { kBorder, kSums, kDrawn };
-    struct Setting {
-        float p, least;
-        double u;
-        int32_t* out;
-        float most;  // the thread's largest logit
-    };
 
     // in: to the last element of those inside it, in falling order, whose predecessors sum to
     // less than a limit: of counts, limit; of weights, p times the sum of all.  kSums: and
@@ -505,7 +511,7 @@ struct Row {
                     all<1, 1>(v);
                     if (v[0] <= kFew) {
                         if (rank == 0)
-                            draw_few(w, (int)v[0], limit, 0, set.p, set.least, set.u, set.out);
+                            draw_few(w, (int)v[0], limit, 0, set);
                         return kDrawn;
                     }
                     if (threadIdx.x == 0) sh.listed = 0;
@@ -654,8 +660,7 @@ struct Row {
         cluster_sync();
         if (few) {
             if (rank == 0)
-                draw_few(w, n, BY_WEIGHT ? (u64)kFew : limit, BY_WEIGHT ? limit : 0, set.p,
-                         set.least, set.u, set.out);
+                draw_few(w, n, BY_WEIGHT ? (u64)kFew : limit, BY_WEIGHT ? limit : 0, set);
             return kDrawn;
         }
         if (threadIdx.x == 0) sh.listed = 0;
@@ -713,10 +718,7 @@ __device__ __forceinline__ float least_of(double min_p, float top, double t) {
     while (hi - lo > 1) {  // a round leaves a 33rd
         const uint32_t key = from + lane * step;
         bool reached = key >= hi;
-        if (key > lo && key < hi) {
-            const double d = ((double)logit_of(key) - (double)top) / t;
-            reached = exp(d) >= min_p;
-        }
+        if (key > lo && key < hi) reached = reaches(logit_of(key), (double)top, t, min_p);
         const uint32_t yes = __ballot_sync(tbk::kFull, reached);
         const int first = yes ? __ffs(yes) - 1 : 32;
         if (first < 32) hi = min(hi, from + first * step);
@@ -775,8 +777,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample(const Args a) {
         mine_top = mine_top == INFINITY ? 0.0f : -INFINITY;
     }
     const Weights w(top, t, sh.table, a.shift);
-    const float least = min_p > 0.0f ? least_of((double)min_p, top, (double)t) : -INFINITY;
-    const typename R::Setting set = {p, least, u, a.out + at, mine_top};
+    const typename R::Setting set = {p, (double)min_p, (double)t, u, a.out + at, mine_top};
 
     // everything above -infinity at first
     Border in = {-INFINITY, -1};
@@ -784,6 +785,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample(const Args a) {
     if (k > 0 && k < a.vocab) found = row.template border<false>(w, in, k, set);
     if (found == R::kBorder && p < 1.0f) found = row.template border<true>(w, in, 0, set);
     if (found == R::kDrawn) return;
+    const float least = min_p > 0.0f ? least_of(set.min_p, top, set.t) : -INFINITY;
     if (least > in.x) {
         in = {least, INT32_MAX};
         found = R::kBorder;
