@@ -49,7 +49,8 @@ struct Args {
     unsigned* status;
     int rows, outs, tiles128;  // cols in tiles of 128
     int tile_rows, row_tiles, n_tiles;
-    int steps, split, stages, stage_bytes, x_off, x_piece;
+    int steps, stages, stage_bytes, x_off, x_piece;
+    int split, whole;  // CTAs that share a tile's steps; each one's tiles before, if split > 1
     int y_vec;       // rows of y start on 16 bytes
     int flat;        // a copy takes one piece, by its x
     int code_bytes;  // that a step's copies count, fill left out
@@ -140,6 +141,12 @@ __device__ __forceinline__ Tile tile_of(const Args& a, int i) {
     return t;
 }
 
+// Steps [first, last) of a tile.
+struct Work {
+    Tile t;
+    int first, last;
+};
+
 template <typename T, int N>
 __device__ __forceinline__ void store_column(T* y, int64_t stride, int n, const float (&v)[N],
                                              float bias) {
@@ -177,11 +184,23 @@ k_linear(const __grid_constant__ Args a) {
     // (the same in all lanes, and known to be)
     const int warp = __shfl_sync(tbk::kFull, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     const int ctas = PAIR ? 2 : a.split, rank = blockIdx.x % ctas;
-    const int first = PAIR ? 0 : (int)((int64_t)a.steps * rank / ctas);
-    const int last = PAIR ? a.steps : (int)((int64_t)a.steps * (rank + 1) / ctas);
-    const int tile0 = blockIdx.x / ctas, tile_step = gridDim.x / ctas;
-    const int mine = tile0 < a.n_tiles ? (a.n_tiles - 1 - tile0) / tile_step + 1 : 0;
-    const int total = mine * (last - first);  // steps of this CTA
+    // whole tiles, then, split > 1, a part of one that the cluster shares
+    const int tile0 = PAIR ? blockIdx.x / 2 : blockIdx.x, tile_step = PAIR ? gridDim.x / 2 : gridDim.x;
+    const int shared = a.whole * gridDim.x + blockIdx.x / ctas;
+    const bool shares = !PAIR && a.split > 1 && shared < a.n_tiles;
+    const int part_first = (int)((int64_t)a.steps * rank / ctas);
+    const int part_last = (int)((int64_t)a.steps * (rank + 1) / ctas);
+    const int whole = PAIR || a.split == 1 ? (a.n_tiles - 1 - tile0) / tile_step + 1 : a.whole;
+    const int mine = whole + shares;
+    const int total = whole * a.steps + (shares ? part_last - part_first : 0);  // this CTA's steps
+    auto work_of = [&](int i) {
+        Work w;
+        const bool part = !PAIR && i == whole;
+        w.t = tile_of<PAIR>(a, part ? shared : tile0 + i * tile_step);
+        w.first = part ? part_first : 0;
+        w.last = part ? part_last : a.steps;
+        return w;
+    };
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < a.stages; ++i) {
@@ -226,7 +245,7 @@ k_linear(const __grid_constant__ Args a) {
             // taken
             constexpr int kAhead = H::kAhead;
             uint8_t* ring = smem + a.stages * a.stage_bytes;
-            int ask_tile = 0, ask_step = first, ask_slot = 0;  // the next that are asked for
+            int ask_tile = 0, ask_step = 0, ask_slot = 0;  // the next that are asked for
             Tile ask_t = tile_of<PAIR>(a, tile0);
             auto ask = [&] {
                 const int out = ask_t.out + kOuts * rank, at = ask_step * kTiles;
@@ -246,18 +265,18 @@ k_linear(const __grid_constant__ Args a) {
                                       bytes, bar);
                 ++asked;
                 if (++ask_slot == kAhead) ask_slot = 0;
-                if (++ask_step == last) {
-                    ask_step = first;
+                if (++ask_step == a.steps) {
+                    ask_step = 0;
                     if (++ask_tile < mine) ask_t = tile_of<PAIR>(a, tile0 + ask_tile * tile_step);
                 }
             };
             int stage = 0;
             uint32_t parity = 1;  // of the round before
             for (int i = 0; i < mine && fine; ++i) {
-                const Tile t = tile_of<PAIR>(a, tile0 + i * tile_step);
-                const int out = t.out + (PAIR ? kOuts * rank : 0);
-                const int row = t.row + (PAIR ? t.n / 2 * rank : 0);
-                for (int j = first; j < last; ++j) {
+                const Work k = work_of(i);
+                const int out = k.t.out + (PAIR ? kOuts * rank : 0);
+                const int row = k.t.row + (PAIR ? k.t.n / 2 * rank : 0);
+                for (int j = k.first; j < k.last; ++j) {
                     // the products of step issued - stages are done, and so are the copies of
                     // its scales
                     if (issued >= a.stages) fine = wait_one(&sh.empty[stage], parity, a.status);
@@ -299,11 +318,11 @@ k_linear(const __grid_constant__ Args a) {
             int stage = 0, done = 0, consumed = 0;
             uint32_t parity = 0;
             for (int i = 0; i < mine && fine; ++i) {
-                const Tile t = tile_of<PAIR>(a, tile0 + i * tile_step);
-                const uint32_t instruction = tc::with_columns(a.instruction, t.n);
+                const Work k = work_of(i);
+                const uint32_t instruction = tc::with_columns(a.instruction, k.t.n);
                 if (i > 0) fine = wait_all(&sh.drained, (i - 1) & 1, a.status);
                 tc::fence_after();
-                for (int j = first; j < last && fine; ++j) {
+                for (int j = k.first; j < k.last && fine; ++j) {
                     fine = wait_all(&sh.full[stage], parity, a.status);
                     if (fine) ++consumed;
                     fine = fine && wait_all(&sh.scaled[stage], parity, a.status);
@@ -323,7 +342,7 @@ k_linear(const __grid_constant__ Args a) {
                                     tmem, w + p * (kOuts * kPieceBytes / 16) + 2 * m,
                                     w + x_off + p * x_piece + 2 * m,
                                     tc::with_block(instruction, block), w_scales + 4 * h,
-                                    x_scales + 4 * kMostX * h, j > first || p + m > 0, leader);
+                                    x_scales + 4 * kMostX * h, j > k.first || p + m > 0, leader);
                         }
                     if (done + a.stages < total) commit(&sh.empty[stage], leader);
                     ++done;
@@ -346,7 +365,7 @@ k_linear(const __grid_constant__ Args a) {
             const int part = warp - H::kScalers;
             const bool leader = lane == 0;
             const uint8_t* ring = smem + a.stages * a.stage_bytes;
-            int stage = 0, slot = 0, step = first;
+            int stage = 0, slot = 0, step = 0;
             uint32_t parity = 0, slot_parity = 0;
             for (int done = 0; done < total && (rank == 0 || part == 0); ++done) {
                 fine = wait_all(&sh.asked[slot], slot_parity, a.status);
@@ -379,7 +398,7 @@ k_linear(const __grid_constant__ Args a) {
                     // (the slot is asked for again when this step's products are done)
                     arrive_first(&sh.other[slot]);
                 }
-                if (++step == last) step = first;
+                if (++step == a.steps) step = 0;
                 if (++slot == kAhead) {
                     slot = 0;
                     slot_parity ^= 1;
@@ -402,16 +421,16 @@ k_linear(const __grid_constant__ Args a) {
             const uint32_t to = tmem + a.scales_column + ((uint32_t)(warp % 4) << 21);
             const int thread = threadIdx.x - 32 * H::kScalers;
             uint4* ring = reinterpret_cast<uint4*>(smem + a.stages * a.stage_bytes);
-            int ask_tile = 0, ask_step = first, ask_slot = 0;  // the next step that is asked for
+            int ask_tile = 0, ask_slot = 0;
+            Work next = work_of(0);  // the next step that is asked for is its first
             auto ask = [&] {
                 if (ask_tile < mine) {
-                    const Tile t = tile_of<PAIR>(a, tile0 + ask_tile * tile_step);
-                    const int out = t.out;
+                    const Tile t = next.t;
 #pragma unroll
                     for (int i = 0; i < (kChunks + 127) / 128; ++i) {
                         const int c = thread + 128 * i, tile = c / 32, x = tile - kTiles;
-                        const int h = x < 0 ? tile : x / kMostX, at = ask_step * kTiles + h;
-                        const int row = x < 0 ? out : t.row + 128 * (x % kMostX);
+                        const int h = x < 0 ? tile : x / kMostX, at = next.first * kTiles + h;
+                        const int row = x < 0 ? t.out : t.row + 128 * (x % kMostX);
                         if (c < kChunks && at < a.tiles128 && row < (x < 0 ? a.outs : a.rows)) {
                             const uint8_t* from = (x < 0 ? a.w_scales : a.x_scales) +
                                                   mx::scales_at(row, at, a.tiles128) + c % 32 * 16;
@@ -421,10 +440,7 @@ k_linear(const __grid_constant__ Args a) {
                                          : "memory");
                         }
                     }
-                    if (++ask_step == last) {
-                        ask_step = first;
-                        ++ask_tile;
-                    }
+                    if (++next.first == next.last && ++ask_tile < mine) next = work_of(ask_tile);
                 }
                 asm volatile("cp.async.commit_group;" ::: "memory");
                 if (++ask_slot == kAhead) ask_slot = 0;
@@ -465,9 +481,9 @@ k_linear(const __grid_constant__ Args a) {
     } else {
         const int quarter = warp % 4;
         const uint32_t sums = tmem + ((uint32_t)quarter << 21);
-        float* part = reinterpret_cast<float*>(smem);  // split: [row][out]
+        float* part = reinterpret_cast<float*>(smem);  // of a shared tile: [row][out]
         for (int i = 0; i < mine; ++i) {
-            const Tile t = tile_of<PAIR>(a, tile0 + i * tile_step);
+            const Tile t = work_of(i).t;
             if (fine) fine = wait_all(&sh.sums, i & 1, a.status);
             if (!fine && !PAIR) break;  // (a pair's warps still come to the barriers below)
             tc::fence_after();
@@ -525,7 +541,7 @@ k_linear(const __grid_constant__ Args a) {
                 for (int c = 0; c < t.n; c += 32) {
                     float v[32];
                     tc::load<32>(sums + c, v);
-                    if (a.split > 1) {
+                    if (i == whole) {
 #pragma unroll
                         for (int e = 0; e < 32; ++e)
                             if (c + e < t.n) part[(c + e) * kOuts + 32 * quarter + lane] = v[e];
@@ -558,10 +574,10 @@ k_linear(const __grid_constant__ Args a) {
         return;
     }
     if (warp == kIssuer) tc::release(tmem, a.columns);
-    if (a.split > 1) {
+    if (shares) {
         cluster_sync();
         if (warp >= H::kStorers) {
-            const Tile t = tile_of<PAIR>(a, tile0);
+            const Tile t = tile_of<PAIR>(a, shared);
             const int at = warp % 4 * 32 + lane, out = t.out + at;
             if (out < a.outs) {
                 const float bias = a.bias ? a.bias[out] : 0.0f;
@@ -581,7 +597,7 @@ k_linear(const __grid_constant__ Args a) {
 
 struct Plan {
     bool pair;
-    int tile_rows, row_tiles, n_tiles, steps, split, stages, stage_bytes, bytes, ctas;
+    int tile_rows, row_tiles, n_tiles, steps, split, whole, stages, stage_bytes, bytes, ctas;
     int x_rows;  // that a CTA loads
     uint32_t columns, scales_column;
 };
@@ -611,12 +627,23 @@ int plan_of(Plan& p, const TbB200Mx* x, const TbB200Mx* w, bool both4, int sm_co
     const uint32_t need = p.scales_column + p.stages * scale_columns;
     for (p.columns = 32; p.columns < need;) p.columns *= 2;
     const int slots = p.pair ? sm_count / 2 : sm_count * per_sm;
-    // parts of cols where the tiles leave SMs idle, 4 steps each at least
+    // parts of cols, 4 steps each at least: where the tiles leave SMs idle, and of the last
+    // round's tiles where they are for half of the CTAs or fewer
+    const int rest = (int)(n_tiles % slots);
+    const bool can = !p.pair && p.tile_rows * kOuts * 4 <= p.stages * p.stage_bytes;
     p.split = 1;
-    while (!p.pair && p.split < kMostSplit && n_tiles * p.split * 2 <= slots &&
-           p.steps >= 8 * p.split && p.tile_rows * kOuts * 4 <= p.stages * p.stage_bytes)
-        p.split *= 2;
-    p.ctas = p.split > 1 ? p.n_tiles * p.split : p.n_tiles < slots ? p.n_tiles : slots;
+    p.whole = 0;
+    if (n_tiles > slots) {
+        if (can && rest && 2 * rest <= slots && p.steps >= 8) {
+            p.split = 2;
+            p.whole = (int)(n_tiles / slots);
+        }
+    } else {
+        while (can && p.split < kMostSplit && n_tiles * p.split * 2 <= slots &&
+               p.steps >= 8 * p.split)
+            p.split *= 2;
+    }
+    p.ctas = n_tiles > slots ? slots : p.n_tiles * p.split;
     if (p.pair) p.ctas *= 2;
     p.bytes = p.stages * p.stage_bytes + beside;
     return TB_OK;
@@ -709,6 +736,7 @@ extern "C" int tb_b200_mx_linear(const TbB200Mx* x, const TbB200Mx* w, const flo
     a.n_tiles = p.n_tiles;
     a.steps = p.steps;
     a.split = p.split;
+    a.whole = p.whole;
     a.stages = p.stages;
     a.stage_bytes = p.stage_bytes;
     a.x_off = pieces * kOuts * kPieceBytes;

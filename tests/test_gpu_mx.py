@@ -288,7 +288,8 @@ def test_linear(rows, cols, outs, xf, wf):
 @pytest.mark.parametrize("off", [0, 3])
 @pytest.mark.parametrize("xf,rows,cols,outs", [
     ("e4m3", 1290, 300, 4100), ("e2m1", 1290, 640, 4100), ("e2m1", 1290, 200, 4100),
-    ("e4m3", 100, 300, 40007), ("e2m1", 100, 300, 40007)])
+    ("e4m3", 100, 300, 40007), ("e2m1", 100, 300, 40007), ("e4m3", 30, 1100, 40007),
+    ("e2m1", 30, 2100, 40007), ("e4m3", 1, 1024, 57000), ("e4m3", 128, 1024, 40007)])
 def test_linear_of_several_tiles_a_cta(xf, rows, cols, outs, off, dtype):
     """More tiles than CTAs, the last of them ragged; rows of y aligned or not."""
     x, w = T.mx_quantize(normal(57, rows, cols), xf), T.mx_quantize(normal(58, outs, cols), "e2m1")
