@@ -42,6 +42,7 @@ constexpr uint64_t kLimit = 1000000000ull;  // ns, of a wait
 
 struct Args {
     CUtensorMap w_map, x_map;
+    CUtensorMap w_scale_map, x_scale_map;  // a pair's
     const uint8_t *w_scales, *x_scales;
     const float* bias;
     void* y;
@@ -60,7 +61,6 @@ struct Args {
 struct Shared {
     uint64_t full[kMostStages], scaled[kMostStages], empty[kMostStages];
     uint64_t asked[kMostAhead];  // a step's scales, to shared memory
-    uint64_t other[kMostAhead];  // the pair's other CTA has them
     uint64_t sums, drained, products_done, scales_done;
     uint32_t tmem;
     int consumed, taken;  // steps whose codes, and whose scales, have been waited for
@@ -208,10 +208,7 @@ k_linear(const __grid_constant__ Args a) {
             tbk::mbar_init(&sh.scaled[i], H::kScaleWarps);
             tbk::mbar_init(&sh.empty[i], 1);
         }
-        for (int i = 0; i < H::kAhead; ++i) {
-            tbk::mbar_init(&sh.asked[i], 1);
-            tbk::mbar_init(&sh.other[i], 1);
-        }
+        for (int i = 0; i < H::kAhead; ++i) tbk::mbar_init(&sh.asked[i], 1);
         tbk::mbar_init(&sh.scales_done, H::kScaleWarps);
         tbk::mbar_init(&sh.sums, 1);
         tbk::mbar_init(&sh.drained, (PAIR ? 2 : 1) * H::kStoreWarps);
@@ -248,21 +245,13 @@ k_linear(const __grid_constant__ Args a) {
             int ask_tile = 0, ask_step = 0, ask_slot = 0;  // the next that are asked for
             Tile ask_t = tile_of<PAIR>(a, tile0);
             auto ask = [&] {
-                const int out = ask_t.out + kOuts * rank, at = ask_step * kTiles;
-                const int bytes = min(kTiles, a.tiles128 - at) * mx::kTileBytes;
-                const bool has_w = out < a.outs, has_x1 = kMostX > 1 && ask_t.n > 128;
                 uint8_t* to = ring + ask_slot * kEach * mx::kTileBytes;
                 uint64_t* bar = &sh.asked[ask_slot];
-                tbk::mbar_expect_tx(bar, (1 + has_w + has_x1) * bytes);
-                if (has_w)
-                    tbk::bulk_g2s(to, a.w_scales + mx::scales_at(out, at, a.tiles128), bytes, bar);
-#pragma unroll
-                for (int k = 0; k < kMostX; ++k)
-                    if (k == 0 || has_x1)
-                        tbk::bulk_g2s(to + (1 + k) * kTiles * mx::kTileBytes,
-                                      a.x_scales + mx::scales_at(ask_t.row + 128 * k, at,
-                                                                 a.tiles128),
-                                      bytes, bar);
+                const int at = ask_step * 2 * kTiles;  // (halves of a tile's scales)
+                if (rank == 0) tbk::mbar_expect_tx(bar, 2 * kEach * mx::kTileBytes);
+                tma_tile<PAIR>(to, &a.w_scale_map, 0, at, ask_t.out / kOuts + rank, bar);
+                tma_tile<PAIR>(to + kTiles * mx::kTileBytes, &a.x_scale_map, 0, at,
+                               ask_t.row / 128, bar);
                 ++asked;
                 if (++ask_slot == kAhead) ask_slot = 0;
                 if (++ask_step == a.steps) {
@@ -367,37 +356,29 @@ k_linear(const __grid_constant__ Args a) {
             const uint8_t* ring = smem + a.stages * a.stage_bytes;
             int stage = 0, slot = 0, step = 0;
             uint32_t parity = 0, slot_parity = 0;
-            for (int done = 0; done < total && (rank == 0 || part == 0); ++done) {
+            for (int done = 0; done < total && rank == 0; ++done) {
                 fine = wait_all(&sh.asked[slot], slot_parity, a.status);
                 if (!fine) break;
                 if (part == 0 && lane == 0) sh.taken = done + 1;
-                if (rank == 0) {
-                    fine = wait_all(&sh.other[slot], slot_parity, a.status);
-                    if (fine && done >= a.stages)
-                        fine = wait_all(&sh.empty[stage], parity ^ 1, a.status);
-                    if (!fine) break;
-                    tc::fence_after();
-                    const uint32_t from = tbk::smem_addr(ring) + slot * kEach * mx::kTileBytes;
-                    const uint32_t w_to = tmem + a.scales_column + stage * H::kScaleColumns;
-                    const uint32_t x_to = w_to + 4 * kTiles;
-                    const int have = a.tiles128 - step * kTiles;
+                if (done >= a.stages) fine = wait_all(&sh.empty[stage], parity ^ 1, a.status);
+                if (!fine) break;
+                tc::fence_after();
+                const uint32_t from = tbk::smem_addr(ring) + slot * kEach * mx::kTileBytes;
+                const uint32_t w_to = tmem + a.scales_column + stage * H::kScaleColumns;
+                const uint32_t x_to = w_to + 4 * kTiles;
+                const int have = a.tiles128 - step * kTiles;
 #pragma unroll
-                    for (int i = 0; i < kTiles / 2; ++i) {
-                        const int h = 2 * i + part;
-                        if (h >= have) break;
-                        tc::copy_scales(w_to + 4 * h, from + h * mx::kTileBytes, leader);
+                for (int i = 0; i < kTiles / 2; ++i) {
+                    const int h = 2 * i + part;
+                    if (h >= have) break;
+                    tc::copy_scales(w_to + 4 * h, from + h * mx::kTileBytes, leader);
 #pragma unroll
-                        for (int k = 0; k < kMostX; ++k)
-                            tc::copy_scales(x_to + 4 * (kMostX * h + k),
-                                            from + ((1 + k) * kTiles + h) * mx::kTileBytes,
-                                            leader);
-                    }
-                    // (by the first CTA alone: the other's issuer does not wait)
-                    tc::commit_of_pair(&sh.scaled[stage], leader);
-                } else if (lane == 0) {
-                    // (the slot is asked for again when this step's products are done)
-                    arrive_first(&sh.other[slot]);
+                    for (int k = 0; k < kMostX; ++k)
+                        tc::copy_scales(x_to + 4 * (kMostX * h + k),
+                                        from + ((1 + k) * kTiles + h) * mx::kTileBytes, leader);
                 }
+                // (by the first CTA alone: the other's issuer does not wait)
+                tc::commit_of_pair(&sh.scaled[stage], leader);
                 if (++step == a.steps) step = 0;
                 if (++slot == kAhead) {
                     slot = 0;
@@ -561,7 +542,7 @@ k_linear(const __grid_constant__ Args a) {
         for (int j = sh.consumed; j < issued; ++j)
             wait_one(&sh.full[j % a.stages], (uint32_t)(j / a.stages) & 1u, a.status);
     }
-    if (PAIR && warp == kLoader && lane == 0 && lost) {
+    if (PAIR && rank == 0 && warp == kLoader && lane == 0 && lost) {
         for (int j = sh.taken; j < asked; ++j)
             wait_one(&sh.asked[j % H::kAhead], (uint32_t)(j / H::kAhead) & 1u, a.status);
     }
@@ -663,6 +644,16 @@ int map_of(CUtensorMap* map, const TbB200Mx* t, int rows, bool flat, bool packed
                 : tbh::encode_tiles_u8(map, t->codes, dims, strides, box, 128);
 }
 
+// The scales of a step's `tiles` tiles of 128 columns and of 128 or 256 rows: whole boxes, with
+// zeros where the tensor has ended.
+int scale_map_of(CUtensorMap* map, const TbB200Mx* t, int tiles, int row_tiles) {
+    const uint64_t n = (uint64_t)mx::tiles_of(t->cols);
+    const uint64_t dims[3] = {mx::kTileBytes / 2, 2 * n, (uint64_t)mx::tiles_of(t->rows)};
+    const uint64_t strides[2] = {mx::kTileBytes / 2, n * mx::kTileBytes};
+    const uint32_t box[3] = {mx::kTileBytes / 2, 2u * tiles, (uint32_t)row_tiles};
+    return tbh::encode_tiles_u8(map, t->scales, dims, strides, box, 0);
+}
+
 template <typename T, bool BOTH4, bool PAIR>
 int launch(const Args& a, const Plan& p, cudaStream_t s) {
     static std::atomic<uint64_t> granted{0};  // a bit per device
@@ -720,6 +711,11 @@ extern "C" int tb_b200_mx_linear(const TbB200Mx* x, const TbB200Mx* w, const flo
     a.flat = !p.pair || (both4 && mx::tiles_of(x->cols) % 2);
     rc = map_of(&a.w_map, w, kOuts, a.flat, both4);
     if (rc == TB_OK) rc = map_of(&a.x_map, x, p.x_rows, a.flat, both4);
+    if (p.pair) {
+        const int tiles = both4 ? 4 : 2;
+        if (rc == TB_OK) rc = scale_map_of(&a.w_scale_map, w, tiles, 1);
+        if (rc == TB_OK) rc = scale_map_of(&a.x_scale_map, x, tiles, 2);
+    }
     if (rc != TB_OK) return rc;
     a.w_scales = w->scales;
     a.x_scales = x->scales;
