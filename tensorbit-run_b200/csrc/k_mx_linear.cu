@@ -86,6 +86,18 @@ __device__ __forceinline__ bool wait_all(uint64_t* bar, uint32_t parity, unsigne
     return __all_sync(tbk::kFull, came);
 }
 
+// Whether a wait would be over.
+__device__ __forceinline__ bool is_over(uint64_t* bar, uint32_t parity) {
+    uint32_t over;
+    asm volatile(
+        "{\n .reg .pred p;\n mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n"
+        " selp.u32 %0, 1, 0, p;\n}"
+        : "=r"(over)
+        : "r"(tbk::smem_addr(bar)), "r"(parity)
+        : "memory");
+    return over;
+}
+
 // `mine` in the shared memory of CTA `rank` of the cluster.
 __device__ __forceinline__ uint32_t peer(const void* mine, int rank) {
     uint32_t at;
@@ -308,17 +320,24 @@ k_linear(const __grid_constant__ Args a) {
             const uint32_t x_off = a.x_off / 16, x_piece = a.x_piece / 16;
             int stage = 0, done = 0, consumed = 0;
             uint32_t parity = 0;
+            // whether a step's operands are there is asked before the products of the step
+            // before are issued: a wait that is over takes 220 clocks, a step's issue 340 to 600
+            bool there = false;
             for (int i = 0; i < mine && fine; ++i) {
                 const Work k = work_of(i);
                 const uint32_t instruction = tc::with_columns(a.instruction, k.t.n);
                 if (i > 0) fine = wait_all(&sh.drained, (i - 1) & 1, a.status);
                 tc::fence_after();
                 for (int j = k.first; j < k.last && fine; ++j) {
-                    fine = wait_all(&sh.full[stage], parity, a.status);
+                    if (!there) fine = wait_all(&sh.full[stage], parity, a.status);
                     if (fine) ++consumed;
-                    fine = fine && wait_all(&sh.scaled[stage], parity, a.status);
+                    if (!there) fine = fine && wait_all(&sh.scaled[stage], parity, a.status);
                     if (!fine) break;
                     tc::fence_after();
+                    const int next = stage + 1 == a.stages ? 0 : stage + 1;
+                    const uint32_t next_parity = next ? parity : parity ^ 1;
+                    const bool full = is_over(&sh.full[next], next_parity),
+                               scaled = is_over(&sh.scaled[next], next_parity);
                     const uint32_t w_scales = tmem + a.scales_column + stage * H::kScaleColumns;
                     const uint32_t x_scales = w_scales + 4 * kTiles;
                     const uint64_t w = w_desc + (uint32_t)(stage * (a.stage_bytes / 16));
@@ -337,10 +356,9 @@ k_linear(const __grid_constant__ Args a) {
                         }
                     if (done + a.stages < total) commit(&sh.empty[stage], leader);
                     ++done;
-                    if (++stage == a.stages) {
-                        stage = 0;
-                        parity ^= 1;
-                    }
+                    stage = next;
+                    parity = next_parity;
+                    there = __all_sync(tbk::kFull, full && scaled);
                 }
                 if (fine) commit(&sh.sums, leader);
             }
