@@ -6,24 +6,31 @@
 // at least), and w, the larger side in serving, is read once for up to 256 rows.  Two shapes:
 //
 // Above 128 rows of x, two CTAs (a pair of SMs) have a tile of 256 outs by 256 rows together:
-// each loads half of either operand, and the first one's products read both halves.  The
-// scales of 128 rows and 128 columns are 512 bytes that one copy of the tensor pipe brings from
-// shared to tensor memory; two warps share those of a step.  What bounds it: a step's chain of
-// loads (about 3000 clocks from far memory), copies of scales and products over the three
-// stages that fit; the tensor pipe is busy for 56 % of the time by the profiler's count.
-//   4096 x 8192 x 28672: 8-bit rows and 4-bit weights 835 us (2.3 PFLOP/s), both 8 bits 905
-//   us, both 4 bits 420 us (4.6 PFLOP/s); bf16 products of that size take 1150 us at the
-//   fastest.  Stores of scales from registers waited for the products in flight, 1700 clocks a
-//   step (806 us for 4 bits); copies by one warp, that asked for them too, took 543 us.
+// each loads half of either operand, and the first one's products read both halves.  Codes and
+// scales come by tensor copies of both CTAs that count on the first one's barriers: an arrival of
+// the other CTA's own would release its shared memory first, 1500 clocks a step.  The scales of 128
+// rows and 128 columns are 512 bytes that one copy of the tensor pipe brings from shared to tensor
+// memory; two warps share those of a step.  A step of 256 columns (512 of 4 bits) takes 1170
+// clocks, 1024 of them its products at the instruction's nominal rate; then it is the power limit
+// that bounds long calls, by the clock.
+//   4096 x 8192 x 28672: 8-bit rows and 4-bit weights 639 us (3.0 PFLOP/s), both 8 bits 690 us,
+//   both 4 bits 330 us (5.8 PFLOP/s); bf16 products of that size take 1150 us at the fastest.
+//   Stores of scales from registers waited for the products in flight (4 bits: 806 us), copies by
+//   one warp that asked for them too took 543, the other CTA's arrivals 420.  Steps of half the
+//   columns, twice the stages: 1318 us for 639's case with those arrivals, 835 then.
 //
-// Up to 128 rows it is w's bytes that count, and then latency: one tile of 128 outs a CTA, two
-// CTAs an SM, one's loads under the other's epilogue, scales through registers (products are
-// few, nothing waits for them).  Where the tiles leave SMs idle, the CTAs of a cluster take
-// parts of cols and add them up, in order, through one another's shared memory.
-//   64 x 8192 x 128256, 4-bit weights to f32: 134 us (4.4 TB/s of the bytes there have to be);
-//   one CTA an SM 419 us, three 152.  1 x 4096 x 4096: 9.5 us, of which a launch and the first
-//   loads are the most.  Asking for w ahead into L2 made it slower (72 -> 85 us for 57344
-//   outs), as did a K split in rounds.
+// Up to 128 rows it is w's bytes that count, and the issuing warp's chain of waits, products and
+// commits (1000 clocks a step of 128 columns): one tile of 128 outs a CTA, two CTAs an SM, one's
+// loads under the other's epilogue, scales through registers (products are few, nothing waits for
+// them).  Where the tiles leave SMs idle, the CTAs of a cluster take parts of cols and add them
+// up, in order, through one another's shared memory; so do two of them in a last round that has
+// tiles for half of the CTAs.
+//   64 x 8192 x 128256, 4-bit weights to f32: 128 us (4.6 TB/s of the bytes there have to be);
+//   one CTA an SM 419 us, three 152 against 135 then; last round whole 135 -> 130.
+//   1 x 8192 x 57344: 57 us (4.4 TB/s); 64 with waits for a step that is there already.
+//   1 x 4096 x 4096: 8.7 us, of which a launch and the first loads are the most.
+//   Asking for w ahead into L2 made it slower (72 -> 85 us for 57344 outs), as did parts of cols
+//   in every round.
 #include <atomic>
 
 #include "mx.cuh"

@@ -18,7 +18,17 @@
 // them are first thinned by exact histograms of their bits, and equal ones are told apart by a
 // search in the order of the index.  That search, by exact sums of CTA, warp, slab and lane,
 // makes the draw too.  Where all that is above the border is as few, the last steps are one
-// CTA's, on that list.
+// CTA's, on that list; and few of many (top-k up to 192) need no histogram of all: the k-th of
+// the threads' largest is a bound that few others are above.
+//
+// What bounds it: a row's chain of exchanges, its bytes cross HBM once.  256 rows of 128256 f32
+// are 2048 CTAs, two an SM by shared memory and registers, so 7 rounds of them:
+//   first largest 62 us; no filter 121; the 50 first 105 (138 by the histogram of all, whose
+//   atomics are 30), and 0.9 of those 110; min_p 88; the 1000 first 203; 0.9 of all 324, of
+//   which the exact sums in double and their search are half; 20 us are the bytes alone.
+//   1 row of 32000: first largest 4.4 us, no filter 7.5, the 50 first 10, 0.9 of all 17.5.
+// Histograms that each CTA pulled from the others took 15000 to 54000 clocks where they read the
+// same bins at once: they are pushed.  Radix passes over the bits with exact sums: 1553 us.
 #include <float.h>
 #include <math.h>
 
