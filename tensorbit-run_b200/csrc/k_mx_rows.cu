@@ -4,7 +4,7 @@
 // A thread has 32 bytes of a row (16 where rows are reduced first: the norm), so a block of 32
 // elements is 2 to 8 neighbouring lanes, its largest magnitude 1 to 3 shuffles, and the four
 // scales of a tile's row one 32-bit store.  Bytes are the inputs once, codes and scales once;
-// what bounds the kernels now is their instructions (issue slots are 65 to 73 % busy, DRAM 40 to
+// what bounds the kernels now is their instructions (issue slots are 75 % busy, DRAM 41 to
 // 51 %), most of which widen, scale and round:
 //   28672 x 8192 bf16 to 4 bits 230 us (5.1 TB/s); 283 with 16 bytes a thread, more with two
 //   or four pieces of work a thread
