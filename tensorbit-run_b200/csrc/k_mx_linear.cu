@@ -31,6 +31,7 @@
 //   1 x 4096 x 4096: 8.7 us, of which a launch and the first loads are the most.
 //   Asking for w ahead into L2 made it slower (72 -> 85 us for 57344 outs), as did parts of cols
 //   in every round.
+#include <algorithm>
 #include <atomic>
 
 #include "mx.cuh"
@@ -646,10 +647,13 @@ int plan_of(Plan& p, const TbB200Mx* x, const TbB200Mx* w, bool both4, int sm_co
             p.split = 2;
             p.whole = (int)(n_tiles / slots);
         }
-    } else {
-        while (can && p.split < kMostSplit && n_tiles * p.split * 2 <= slots &&
-               p.steps >= 8 * p.split)
-            p.split *= 2;
+    } else if (can) {
+        // clusters of 3, 5, 6 or 7 leave places of a GPC over, up to one less than their CTAs:
+        // those of 3 that fit take 10.4 us for 11.9 (1 x 4096 x 11008), ones too many 25 for 18
+        constexpr int kGpcs = 8;
+        p.split = (int)std::min<int64_t>({kMostSplit, slots / n_tiles, std::max(p.steps / 4, 1)});
+        while ((p.split & (p.split - 1)) && n_tiles * p.split > slots - kGpcs * (p.split - 1))
+            --p.split;
     }
     p.ctas = n_tiles > slots ? slots : p.n_tiles * p.split;
     if (p.pair) p.ctas *= 2;

@@ -301,6 +301,18 @@ def test_linear_of_several_tiles_a_cta(xf, rows, cols, outs, off, dtype):
     assert (y[:, :off] == 7.0).all() and (y[:, off + outs:] == 7.0).all()
 
 
+@pytest.mark.parametrize("cols,outs", [(1600, 10240), (2600, 6100), (3200, 5100), (3600, 300),
+                                       (4200, 700), (1100, 300)])
+@pytest.mark.parametrize("xf", FORMATS)
+def test_linear_in_parts_of_cols(xf, cols, outs):
+    """2 to 8 CTAs a tile, by the number of tiles and of steps."""
+    x, w = T.mx_quantize(normal(62, 5, cols), xf), T.mx_quantize(normal(63, outs, cols), "e2m1")
+    bias = normal(64, outs)
+    y = T.mx_linear(x, w, bias, torch.float32)
+    check_linear(x, w, bias, y)
+    assert torch.equal(T.mx_linear(x, w, bias, torch.float32), y)
+
+
 @pytest.mark.parametrize("rows", [2, 200])
 def test_linear_of_far_larger_codes_and_scales(rows):
     """Codes and scales that did not come from mx_quantize: every code but NaN, any scale."""
