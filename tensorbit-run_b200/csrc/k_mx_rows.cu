@@ -10,6 +10,8 @@
 //   or four pieces of work a thread
 //   SwiGLU 4096 x 28672 bf16 140 us (4.2 TB/s)
 //   norm 16384 x 8192 bf16 with the residual 198 us (4.8 TB/s); 188 with products rounded twice
+#include <cmath>
+
 #include "bodies.cuh"
 #include "mx.cuh"
 
@@ -265,6 +267,7 @@ struct Norm {
     T* h;
     bool vec, vec_w;
     float eps;
+    double root;  // of the number of columns
 };
 
 // h of a chunk: x + residual in f32, the same bits each time.
@@ -280,12 +283,17 @@ __device__ __forceinline__ void sum_of(const Norm<T>& in, const Chunk<T, 1>& x, 
     }
 }
 
-// h and the norm of chunk c of row r, stored.
+// The norm's factor: (hi + lo) by, by a power of two that keeps hi and its products with h
+// within f32's normal numbers for rows of any size.
+struct Factor {
+    float hi, lo, by;
+};
+
+// The norm of chunk c of row r, stored; h comes scaled by the factor's power of two.
 template <typename T, int FORMAT>
 __device__ __forceinline__ void finish(const Norm<T>& in, const mx::View& out, int64_t r, int c,
-                                       bool live, float2 scale, float (&h)[Chunk<T, 1>::E]) {
+                                       bool live, Factor scale, float (&h)[Chunk<T, 1>::E]) {
     constexpr int E = Chunk<T, 1>::E;
-    if (live && in.h) store_chunk<T, E>(in.h + r * out.cols, c * E, out.cols, in.vec, h);
     // h times the factor's two parts times w, to half an ulp and a little: what a product's
     // rounding leaves out goes on with it
     float w[E];
@@ -304,7 +312,7 @@ __device__ __forceinline__ void finish(const Norm<T>& in, const mx::View& out, i
     }
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-        const float t = h[e] * scale.x, left = fmaf(h[e], scale.y, fmaf(h[e], scale.x, -t));
+        const float t = h[e] * scale.hi, left = fmaf(h[e], scale.lo, fmaf(h[e], scale.hi, -t));
         const float y = t * w[e];
         h[e] = y + fmaf(left, w[e], fmaf(t, w[e], -y));
     }
@@ -318,10 +326,13 @@ __device__ __forceinline__ void finish(const Norm<T>& in, const mx::View& out, i
 
 // The norm's factor from the sum of squares, as two f32: an error of it moves a whole row's
 // codes the same way, over the same rounding borders.
-__device__ __forceinline__ float2 scale_of(double ss, float eps, int cols) {
-    const double s = 1.0 / sqrt((ss + (double)eps) / (double)cols);
-    const float hi = (float)s;
-    return make_float2(hi, hi < INFINITY ? (float)(s - (double)hi) : 0.0f);
+__device__ __forceinline__ Factor scale_of(double ss, float eps, double root) {
+    const double s = rsqrt(ss + (double)eps) * root;  // off by less than 2^-51
+    const bool great = s > 0x1p64, small = s < 0x1p-64;
+    const float by = great ? 0x1p64f : small ? 0x1p-64f : 1.0f;
+    const double rest = s * (great ? 0x1p-64 : small ? 0x1p64 : 1.0);
+    const float hi = (float)rest;
+    return {hi, hi < INFINITY ? (float)(rest - (double)hi) : 0.0f, by};
 }
 // The sum over a row's G threads (tbk::group_sum's), in double.
 __device__ __forceinline__ double row_sum(double v, int G, double* red) {
@@ -335,17 +346,14 @@ __device__ __forceinline__ double row_sum(double v, int G, double* red) {
     for (int w = 1; w < (G >> 5); ++w) s += red[first + w];
     return s;
 }
-// The squares of a chunk, f32 sums of four each.
+// The sum of a chunk's squares.  Double holds each exactly whatever the row's size; f32's overflow
+// above 1.8e19 and vanish below 1e-23, and a narrow row's sum of them is off by more than the
+// factor's second part says.  (16384 rows of 8192 bf16: 198 us with either.)
 template <int E>
-__device__ __forceinline__ float squares(const float (&h)[E]) {
-    float part[E / 4], sum = 0.0f;
+__device__ __forceinline__ double squares(const float (&h)[E]) {
+    double sum = 0.0;
 #pragma unroll
-    for (int i = 0; i < E / 4; ++i) {
-        part[i] = __fmul_rn(h[4 * i], h[4 * i]);
-#pragma unroll
-        for (int e = 1; e < 4; ++e) part[i] = __fmaf_rn(h[4 * i + e], h[4 * i + e], part[i]);
-        sum = __fadd_rn(sum, part[i]);
-    }
+    for (int e = 0; e < E; ++e) sum = fma((double)h[e], (double)h[e], sum);
     return sum;
 }
 
@@ -374,12 +382,20 @@ __global__ void __launch_bounds__(MAXT) k_norm(const Norm<T> in, const mx::View 
         for (int i = 0; i < ITEMS; ++i) {
             if (lane + i * G < chunks) {
                 sum_of(in, x[i], res[i], h[i]);
-                ss += (double)squares<E>(h[i]);
+                if (in.h)
+                    store_chunk<T, E>(in.h + r * out.cols, (lane + i * G) * E, out.cols, in.vec, h[i]);
+                ss += squares<E>(h[i]);
             }
         }
     }
     ss = row_sum(ss, G, red);
-    const float2 scale = scale_of(ss, in.eps, out.cols);
+    const Factor scale = scale_of(ss, in.eps, in.root);
+    if (scale.by != 1.0f) {
+#pragma unroll
+        for (int i = 0; i < ITEMS; ++i)
+#pragma unroll
+            for (int e = 0; e < E; ++e) h[i][e] *= scale.by;
+    }
 #pragma unroll
     for (int i = 0; i < ITEMS; ++i) {
         const int c = lane + i * G;
@@ -409,10 +425,10 @@ __global__ void __launch_bounds__(1024) k_norm_wide(const Norm<T> in, const mx::
         x.load(in.x + r * out.cols, c * E, out.cols, in.vec);
         if (in.res) res.load(in.res + r * out.cols, c * E, out.cols, in.vec);
         sum_of(in, x, res, h);
-        ss += (double)squares<E>(h);
+        ss += squares<E>(h);
     }
     ss = row_sum(ss, blockDim.x, red);
-    const float2 scale = scale_of(ss, in.eps, out.cols);
+    const Factor scale = scale_of(ss, in.eps, in.root);
     for (int c0 = 0; c0 < chunks; c0 += blockDim.x) {
         const int c = c0 + threadIdx.x;
         const bool live = active && c < chunks;
@@ -422,6 +438,9 @@ __global__ void __launch_bounds__(1024) k_norm_wide(const Norm<T> in, const mx::
             x.load(in.x + r * out.cols, c * E, out.cols, in.vec);
             if (in.res) res.load(in.res + r * out.cols, c * E, out.cols, in.vec);
             sum_of(in, x, res, h);
+            if (in.h) store_chunk<T, E>(in.h + r * out.cols, c * E, out.cols, in.vec, h);
+#pragma unroll
+            for (int e = 0; e < E; ++e) h[e] *= scale.by;
         }
         finish<T, FORMAT>(in, out, r, c, live, scale, h);
         if (!active && c < chunks && c % (128 / E) == 0)
@@ -461,7 +480,8 @@ int norm(const void* x, const void* res, const void* w, void* h, const TbB200Mx*
     const bool vec = aligned_rows<T>(x, y->cols) && (!res || tbh::aligned16(res)) &&
                      (!h || tbh::aligned16(h));
     const Norm<T> in = {static_cast<const T*>(x), static_cast<const T*>(res),
-                        static_cast<const T*>(w), static_cast<T*>(h), vec, tbh::aligned16(w), eps};
+                        static_cast<const T*>(w), static_cast<T*>(h), vec, tbh::aligned16(w), eps,
+                        std::sqrt((double)y->cols)};
     return y->format == mx::kE4m3 ? launch_norm<T, mx::kE4m3>(in, y, s)
                                   : launch_norm<T, mx::kE2m1>(in, y, s);
 }
