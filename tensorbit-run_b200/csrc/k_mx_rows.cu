@@ -295,7 +295,8 @@ __device__ __forceinline__ void finish(const Norm<T>& in, const mx::View& out, i
                                        bool live, Factor scale, float (&h)[Chunk<T, 1>::E]) {
     constexpr int E = Chunk<T, 1>::E;
     // h times the factor's two parts times w, to half an ulp and a little: what a product's
-    // rounding leaves out goes on with it
+    // rounding leaves out goes on with it (each step as it is written: a sum that took the last
+    // product unrounded would count what that left out twice)
     float w[E];
 #pragma unroll
     for (int e = 0; e < E; ++e) w[e] = 1.0f;
@@ -312,9 +313,9 @@ __device__ __forceinline__ void finish(const Norm<T>& in, const mx::View& out, i
     }
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-        const float t = h[e] * scale.hi, left = fmaf(h[e], scale.lo, fmaf(h[e], scale.hi, -t));
-        const float y = t * w[e];
-        h[e] = y + fmaf(left, w[e], fmaf(t, w[e], -y));
+        const float t = __fmul_rn(h[e], scale.hi), y = __fmul_rn(t, w[e]);
+        const float left = fmaf(h[e], scale.lo, fmaf(h[e], scale.hi, -t));
+        h[e] = __fadd_rn(y, fmaf(left, w[e], fmaf(t, w[e], -y)));
     }
     if (c * E + E > out.cols) {  // (a row whose scale is NaN has fill of zeros all the same)
 #pragma unroll
