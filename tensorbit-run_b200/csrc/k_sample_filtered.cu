@@ -85,15 +85,20 @@ struct Weights {
         per = (float)(scale / part);
     }
     // How far a logit lies below the top, in halvings of its weight; NaN stays NaN.
-    __device__ __forceinline__ float fall(float x) const { return fmaf(-part, x, part_top) * per; }
+    __device__ __forceinline__ float fall(float x) const {
+        return __fmul_rn(fmaf(-part, x, part_top), per);
+    }
     __device__ __forceinline__ float logit_at(float y) const { return (part_top - y / per) / part; }
+    // (no product here that the compiler may or may not fuse with a sum, or a weight could come
+    // out a unit more in one place than in another: what is summed in one pass is searched by the
+    // sums of a later one)
     __device__ __forceinline__ u64 operator()(float x) const {
         if (!(fall(x) < 64.0f)) return 0;
         constexpr double kLn2 = 0.69314718055994530942;
         constexpr double c2 = kLn2 * kLn2 / 2, c3 = c2 * kLn2 / 3, c4 = c3 * kLn2 / 4,
                          c5 = c4 * kLn2 / 5, c6 = c5 * kLn2 / 6;
         const double magic = 0x1.8p48;  // a unit of 2^-4
-        const double y = ((double)x - top) * scale, z = y + magic, f = y - (z - magic);
+        const double d = (double)x - top, z = fma(d, scale, magic), f = fma(d, scale, magic - z);
         const int n = __double2loint(z);
         double p = fma(f, c6, c5);
         p = fma(f, p, c4);
