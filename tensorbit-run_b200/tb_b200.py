@@ -1026,9 +1026,11 @@ def _mx(t, dev, what):
 
 def _mx_out(other, dev, out, like, rows, cols, format):
     if out is None:
-        return _new(other, MxTensor._like, like, rows, cols, format)
+        return _new(other, MxTensor._like, like, rows, cols, format or "e4m3")
     if (out.rows, out.cols) != (rows, cols):
         raise ValueError(f"out must be [{rows}, {cols}]")
+    if format is not None and format != out.format:
+        raise TypeError(f"out must be in {format}, got {out.format}")
     _mx(out, dev, "out")
     return out
 
@@ -1048,9 +1050,9 @@ def _rows(t, dev, what, dtype=None):
     return code, s0
 
 
-def mx_quantize(x, format="e4m3", out=None, stream=None):
-    """x [rows, cols], whose rows may be strided, in a microscaled format
-    (tb_b200_mx_quantize)."""
+def mx_quantize(x, format=None, out=None, stream=None):
+    """x [rows, cols], whose rows may be strided, in a microscaled format (`format`, or out's;
+    e4m3 without both) (tb_b200_mx_quantize)."""
     torch, dev = _here()
     stream, other = _stream(torch, dev, stream)
     code, stride = _rows(x, dev, "x")
@@ -1075,10 +1077,10 @@ def mx_dequantize(t, dtype=None, out=None, stream=None):
     return out
 
 
-def residual_rms_norm_mx(x, residual, weight, eps, h_out=None, format="e4m3", out=None,
+def residual_rms_norm_mx(x, residual, weight, eps, h_out=None, format=None, out=None,
                          stream=None):
-    """(h, y): residual_rms_norm of [rows, cols] with y in a microscaled format
-    (tb_b200_residual_rms_norm_mx).  residual None: the norm of x, with no h; h is a new
+    """(h, y): residual_rms_norm of [rows, cols] with y in a microscaled format (`format`, or
+    out's; e4m3 without both) (tb_b200_residual_rms_norm_mx).  residual None: the norm of x, with no h; h is a new
     tensor unless h_out is given (x or residual may be)."""
     torch, dev = _here()
     stream, other = _stream(torch, dev, stream)
@@ -1097,9 +1099,9 @@ def residual_rms_norm_mx(x, residual, weight, eps, h_out=None, format="e4m3", ou
     return h_out, out
 
 
-def swiglu_mx(gate, up, format="e4m3", out=None, stream=None):
+def swiglu_mx(gate, up, format=None, out=None, stream=None):
     """silu(gate) * up of [rows, cols], whose rows may be strided, in a microscaled format
-    (tb_b200_swiglu_mx)."""
+    (`format`, or out's; e4m3 without both) (tb_b200_swiglu_mx)."""
     torch, dev = _here()
     stream, other = _stream(torch, dev, stream)
     code, gs = _rows(gate, dev, "gate")
