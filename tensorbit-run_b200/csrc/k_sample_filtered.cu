@@ -151,6 +151,9 @@ struct alignas(16) Shared {
     u64 warps[4][kWarps];
     u64 ranks[kMostCtas], kept[kWarps];  // a search's sums, of the CTAs and of this one's warps
     double table[16];
+    double uniform;  // the row's settings, the first CTA's words to all
+    float temperature, min_p, top_p;  // (told as pairs)
+    int top_k;
     int bin[2];
     u64 before, in_bin;
     float x;
@@ -187,6 +190,14 @@ __device__ __forceinline__ uint32_t add_to(uint32_t at, uint32_t v) {
     uint32_t old;
     asm volatile("atom.shared::cluster.add.u32 %0, [%1], %2;" : "=r"(old) : "r"(at), "r"(v) : "memory");
     return old;
+}
+// BYTES of a setting to shared memory, some time until cp.async.wait_all.
+template <int BYTES>
+__device__ __forceinline__ void fetch_to(void* smem, const void* from) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(
+                     (uint32_t)__cvta_generic_to_shared(smem)),
+                 "l"(from), "n"(BYTES)
+                 : "memory");
 }
 __device__ __forceinline__ u64 warp_scan(u64 v) {
 #pragma unroll
@@ -447,8 +458,6 @@ struct Row {
     // What a search for a border came to.
     enum Found { kBorder, kSums, kDrawn };
     struct Setting {
-        float p;
-        double min_p, t, u;
         int32_t* out;
         float most;  // the thread's largest logit
     };
@@ -469,14 +478,16 @@ struct Row {
         // (members come with a measure of 1; every lane takes part in the sums)
         u64 sum = sum_before<true>(n, mine);
         hold(mine.measure && sum < k);
-        if (set.p < 1.0f) {
+        if (sh.top_p < 1.0f) {
             const u64 limit =
-                p_limit ? p_limit : share(block_sum(writes ? mine.measure : 0), set.p);
+                p_limit ? p_limit : share(block_sum(writes ? mine.measure : 0), sh.top_p);
             sum = sum_before<true>(n, mine);
             hold(mine.measure && sum < limit);
         }
-        if (set.min_p > 0.0) hold(mine.measure && reaches(mine.x, w.top, set.t, set.min_p));
-        const u64 target = target_of(block_sum(writes ? mine.measure : 0), set.u);
+        if (sh.min_p > 0.0f)
+            hold(mine.measure &&
+                 reaches(mine.x, w.top, (double)sh.temperature, (double)sh.min_p));
+        const u64 target = target_of(block_sum(writes ? mine.measure : 0), sh.uniform);
         const u64 before = sum_before<false>(n, mine);
         if (writes && before <= target && target < before + mine.measure) *set.out = mine.index;
     }
@@ -570,7 +581,7 @@ struct Row {
         int b0, b1, t = 0;
         bool few;  // all that is above and in the bins
         if constexpr (BY_WEIGHT) {
-            const double mass = fmax((double)set.p, 0.0) * (double)whole;
+            const double mass = fmax((double)sh.top_p, 0.0) * (double)whole;
             reach(h, before, max((u64)(mass * (1 - 0x1p-13)), 1ull),
                   (u64)(mass * (1 + 0x1p-13)) + 1, b0, b1);
             // exact: the sum of all, of what is above the bins, and how many there are
@@ -588,7 +599,7 @@ struct Row {
             const u64 above = v[2] >> 32;
             v[2] &= 0xffffffffu;
             few = above + v[2] <= kFew;
-            limit = share(v[0], set.p);
+            limit = share(v[0], sh.top_p);
             if (few)
                 v[2] += above;
             else
@@ -744,6 +755,41 @@ __device__ __forceinline__ float least_of(double min_p, float top, double t) {
     return logit_of(hi);
 }
 
+// The settings of row `at`.  One thread of a cluster reads them, once: its CTAs wait for one another
+// on every branch that they decide, and a program that writes them during the call (from a stream
+// that nothing orders) gets some draw, not CTAs that wait for ever on different branches.
+__device__ __forceinline__ void fetch_settings(const Args& a, Shared& sh, int64_t at) {
+    fetch_to<8>(&sh.uniform, a.uniforms + at);
+    if (a.temperature)
+        fetch_to<4>(&sh.temperature, a.temperature + at);
+    else
+        sh.temperature = 1.0f;
+    if (a.min_p)
+        fetch_to<4>(&sh.min_p, a.min_p + at);
+    else
+        sh.min_p = 0.0f;
+    if (a.top_p)
+        fetch_to<4>(&sh.top_p, a.top_p + at);
+    else
+        sh.top_p = 1.0f;
+    if (a.top_k)
+        fetch_to<4>(&sh.top_k, a.top_k + at);
+    else
+        sh.top_k = 0;
+}
+// They to the cluster's other CTAs, by that thread; the next cluster_sync makes them seen.
+__device__ __forceinline__ void tell_settings(const Args& a, Shared& sh) {
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    const u64 u = (u64)__double_as_longlong(sh.uniform);
+    const u64 v = (u64)__float_as_uint(sh.min_p) << 32 | __float_as_uint(sh.temperature);
+    const u64 w = (u64)(uint32_t)sh.top_k << 32 | __float_as_uint(sh.top_p);
+    for (int c = 1; c < a.ctas; ++c) {
+        store_to(peer(&sh.uniform, c), u);
+        store_to(peer(&sh.temperature, c), v);
+        store_to(peer(&sh.top_p, c), w);
+    }
+}
+
 template <typename T>
 __global__ void __launch_bounds__(kThreads, 2) k_sample(const Args a) {
     using R = Row<T>;
@@ -753,23 +799,24 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample(const Args a) {
     cluster_arrive();
     R row(a, sh, held, blockIdx.x % a.ctas);
     const int64_t at = blockIdx.x / a.ctas;
+    const bool tells = row.rank == 0 && threadIdx.x == 0;
+    if (tells) fetch_settings(a, sh, at);
     float mine_top = row.load(static_cast<const T*>(a.logits) + at * a.stride);
     u64 v[4] = {key_of(mine_top), 0, 0, 0};
-    const float t = a.temperature ? a.temperature[at] : 1.0f;
-    const float min_p = a.min_p ? a.min_p[at] : 0.0f, p = a.top_p ? a.top_p[at] : 1.0f;
-    const int k = a.top_k ? a.top_k[at] : 0;
-    const double u = a.uniforms[at];
     if (threadIdx.x < 16) sh.table[threadIdx.x] = exp2((double)threadIdx.x / 16);
 
     cluster_wait();  // every CTA is there to be written to
+    if (tells) tell_settings(a, sh);
     // the largest logit, and the first of the largest
     row.template all<1, 0>(v);
+    const float t = sh.temperature;
+    const int k = sh.top_k;
     float top = logit_of((uint32_t)v[0]);
     if (top == -INFINITY) {
         if (row.rank == 0 && threadIdx.x == 0) a.out[at] = 0;
         return;
     }
-    if (!(t >= 0x1p-126f) || min_p > 1.0f) {
+    if (!(t >= 0x1p-126f) || sh.min_p > 1.0f) {
         v[0] = 0;
         row.each([&](float x, int i) {
             if (x == top) v[0] = max(v[0], (u64)~(uint32_t)i);
@@ -792,15 +839,16 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample(const Args a) {
         mine_top = mine_top == INFINITY ? 0.0f : -INFINITY;
     }
     const Weights w(top, t, sh.table, a.shift);
-    const typename R::Setting set = {p, (double)min_p, (double)t, u, a.out + at, mine_top};
+    const typename R::Setting set = {a.out + at, mine_top};
 
     // everything above -infinity at first
     Border in = {-INFINITY, -1};
     auto found = R::kBorder;
     if (k > 0 && k < a.vocab) found = row.template border<false>(w, in, k, set);
-    if (found == R::kBorder && p < 1.0f) found = row.template border<true>(w, in, 0, set);
+    if (found == R::kBorder && sh.top_p < 1.0f) found = row.template border<true>(w, in, 0, set);
     if (found == R::kDrawn) return;
-    const float least = min_p > 0.0f ? least_of(set.min_p, top, set.t) : -INFINITY;
+    const float least =
+        sh.min_p > 0.0f ? least_of((double)sh.min_p, top, (double)sh.temperature) : -INFINITY;
     if (least > in.x) {
         in = {least, INT32_MAX};
         found = R::kBorder;
@@ -814,7 +862,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample(const Args a) {
     u64 sum = 0;
     for (int c = 0; c < a.ctas; ++c) sum += sh.ranks[c];
     // the first with a running sum above u * all
-    const int drawn = row.locate(R::target_of(sum, u), weight);
+    const int drawn = row.locate(R::target_of(sum, sh.uniform), weight);
     if (drawn >= 0) *set.out = drawn;
 }
 
