@@ -581,10 +581,13 @@ int tb_b200_mx_linear(const TbB200Mx* x, const TbB200Mx* w, const float* bias, i
  *                sum_{j <= i} w_j > u * (the sum over all kept)
  * NaN logits are never kept, -infinity never drawn; where one is +infinity, those are
  * alike and the others have no weight.  A row with no logit above -infinity draws 0.
- * Weights are held to 2^-44 of the largest or better (their fixed-point sums do not depend
- * on an order), so a draw is the definition's unless a border lies about that near to u
- * times the sum, or to top_p times it.  Unlike tb_b200_sample_temperature this is not
- * the reference's draw to the last bit, and a NaN does not decide a row. */
+ * Weights are whole numbers of a fraction of the largest, so their sums do not depend on an
+ * order.  Each is off by up to 2^-44 of the largest (2^-46 at 128256 words, 2^-48 at 32000),
+ * equal ones to the same side, and a sum of n by n times that.  So a draw is the definition's
+ * unless a border lies nearer to u times the sum, or to top_p times it, than 2 vocab times
+ * that: 2^-24.5 of the largest weight at the largest vocabulary, 2^-28 at 128256 words, 2^-32
+ * at 32000.  Unlike tb_b200_sample_temperature this is not the reference's draw to the last
+ * bit, and a NaN does not decide a row. */
 typedef struct {
     int dtype; /* of the logits */
     int64_t rows;
