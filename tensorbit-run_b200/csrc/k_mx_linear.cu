@@ -44,7 +44,7 @@ namespace {
 // warps
 constexpr int kLoader = 0, kIssuer = 1;
 constexpr int kOuts = 128;  // of a CTA's tile
-constexpr int kMostStages = 8, kMostAhead = 8, kMostSplit = 8;
+constexpr int kMostStages = 5, kMostAhead = 8, kMostSplit = 8;
 constexpr int kPieceBytes = 128;  // of a row of codes; a step has one or two such pieces
 constexpr uint64_t kLimit = 1000000000ull;  // ns, of a wait
 
@@ -196,7 +196,7 @@ struct Shape {
 
 // BOTH4: both operands 4-bit, a piece 256 columns; else 128.
 template <typename T, bool BOTH4, bool PAIR>
-__global__ void __launch_bounds__(Shape<BOTH4, PAIR>::kThreads, PAIR ? 1 : 3)
+__global__ void __launch_bounds__(Shape<BOTH4, PAIR>::kThreads, PAIR ? 1 : 2)
 k_linear(const __grid_constant__ Args a) {
     using H = Shape<BOTH4, PAIR>;
     constexpr int kTiles = H::kTiles, kMostX = H::kMostX, kEach = H::kEach, kPieces = H::kPieces;
@@ -630,7 +630,8 @@ int plan_of(Plan& p, const TbB200Mx* x, const TbB200Mx* w, bool both4, int sm_co
     const int beside = scales + (p.pair ? Shape<false, true>::kStaged : 0) + 1024;
     const int per_sm = p.pair ? 1 : 2;
     p.stages = (226 * 1024 / per_sm - 1024 - beside) / p.stage_bytes;
-    if (p.stages > kMostStages) p.stages = kMostStages;
+    static_assert((226 * 1024 / 2 - 2048 - Shape<false, false>::kScaleBytes) /
+                          ((kOuts + 16) * kPieceBytes) <= kMostStages, "the smallest tiles' stages");
     p.scales_column = (uint32_t)(p.tile_rows + 31) / 32 * 32;
     const int scale_columns = (p.pair ? 12 : 8) * step_tiles;
     const uint32_t need = p.scales_column + p.stages * scale_columns;
