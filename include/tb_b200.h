@@ -540,10 +540,13 @@ int tb_b200_mx_quantize(int dtype, const void* x, int64_t x_stride, const TbB200
  * of that type: below bf16's least ones only), rows y_stride elements apart. */
 int tb_b200_mx_dequantize(const TbB200Mx* t, int dtype, void* y, int64_t y_stride, void* stream);
 
-/* tb_b200_residual_rms_norm with y in a microscaled format (y->rows rows of y->cols): the
- * same h; y's f32 values (from sums of squares in double, with one rounding and little more)
- * go to codes and scales as tb_b200_mx_quantize takes them there.  residual NULL: the norm
- * of x; weight and h_out may be NULL; h_out may be x or residual. */
+/* tb_b200_residual_rms_norm with y in a microscaled format (y->rows rows of y->cols):
+ *   h = x + residual (f32, stored in dtype),  y = h / sqrt((eps + sum h^2) / cols) * weight
+ * eps is added to the sum, as the engine has it: for a model whose norm divides by
+ * sqrt(mean(h^2) + eps), give cols * eps.  y is f32 with one rounding (squares, their sum and
+ * the factor are held in double, for rows of any size) and goes to codes and scales as
+ * tb_b200_mx_quantize takes it there.  residual NULL: the norm of x; weight and h_out may be
+ * NULL; h_out may be x or residual. */
 int tb_b200_residual_rms_norm_mx(int dtype, const void* x, const void* residual,
                                  const void* weight, void* h_out, const TbB200Mx* y, float eps,
                                  void* stream);

@@ -13,11 +13,12 @@
 // memory; two warps share those of a step.  A step of 256 columns (512 of 4 bits) takes 1170
 // clocks, 1024 of them its products at the instruction's nominal rate; then it is the power limit
 // that bounds long calls, by the clock.
-//   4096 x 8192 x 28672: 8-bit rows and 4-bit weights 639 us (3.0 PFLOP/s), both 8 bits 690 us,
-//   both 4 bits 330 us (5.8 PFLOP/s); bf16 products of that size take 1150 us at the fastest.
+//   4096 x 8192 x 28672, a few calls from a graph: 8-bit rows and 4-bit weights 632 us (3.0
+//   PFLOP/s), both 8 bits 680, both 4 bits 325 (5.9 PFLOP/s); one after another for seconds 740 and
+//   380 us (1432 MHz at 990 W); bf16 products of that size take 1150 us at the fastest.
 //   Stores of scales from registers waited for the products in flight (4 bits: 806 us), copies by
 //   one warp that asked for them too took 543, the other CTA's arrivals 420.  Steps of half the
-//   columns, twice the stages: 1318 us for 639's case with those arrivals, 835 then.
+//   columns, twice the stages: 1318 us for 632's case with those arrivals, 835 then.
 //
 // Up to 128 rows it is w's bytes that count, and the issuing warp's chain of waits, products and
 // commits (1000 clocks a step of 128 columns): one tile of 128 outs a CTA, two CTAs an SM, one's
@@ -613,6 +614,17 @@ struct Plan {
 
 int plan_of(Plan& p, const TbB200Mx* x, const TbB200Mx* w, bool both4, int sm_count) {
     const int64_t tiles128 = mx::tiles_of(x->cols);
+    // In us, single CTAs and pairs at 64, 96, 128, 129 and 256 rows (above 128 single ones read w
+    // again for each 128), 8-bit rows and 4-bit weights:
+    //   8192 x 8192    18 24   21 24   24 25   37 26   38 28
+    //   8192 x 28672   34 43   40 44   43 46   72 47   75 55
+    //   8192 x 57344   66 81   78 83   82 86  144 89  147 106
+    //   28672 x 8192   38 67   44 68   47 71   76 73   78 82
+    //   4096 x 4096    13 13   15 14   17 14   19 15   20 16
+    //   4096 x 11008   20 15   25 15   29 15   24 16   24 18
+    //   8192 x 28672, both 4 bits  29 30, 36 32 at 128, 55 32, 59 35
+    // 128 is where pairs take over for the larger of these; of short cols they are ahead from 32
+    // to 96 rows on, which the rule leaves.
     p.pair = x->rows > 128;
     const int pieces = p.pair ? 2 : 1, step_tiles = (both4 ? 2 : 1) * pieces;
     p.steps = (int)((tiles128 + step_tiles - 1) / step_tiles);

@@ -23,10 +23,10 @@
 //
 // What bounds it: a row's chain of exchanges, its bytes cross HBM once.  256 rows of 128256 f32
 // are 2048 CTAs, two an SM by shared memory and registers, so 7 rounds of them:
-//   first largest 62 us; no filter 121; the 50 first 105 (138 by the histogram of all, whose
-//   atomics are 30), and 0.9 of those 110; min_p 88; the 1000 first 203; 0.9 of all 324, of
+//   first largest 61 us; no filter 119; the 50 first 104 (138 by the histogram of all, whose
+//   atomics are 30), and 0.9 of those 109; min_p 87; the 1000 first 200; 0.9 of all 322, of
 //   which the exact sums in double and their search are half; 20 us are the bytes alone.
-//   1 row of 32000: first largest 4.4 us, no filter 7.5, the 50 first 10, 0.9 of all 17.5.
+//   1 row of 32000: first largest 4.2 us, no filter 7.5, the 50 first 10, 0.9 of all 17.5.
 // Histograms that each CTA pulled from the others took 15000 to 54000 clocks where they read the
 // same bins at once: they are pushed.  Radix passes over the bits with exact sums: 1553 us.
 #include <float.h>
@@ -869,7 +869,12 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample(const Args a) {
 template <typename T>
 int run(Args& a, int64_t rows, int sm_count, cudaStream_t s) {
     // as many CTAs a row as hold it in 64 KB each (two an SM), and more while the SMs have
-    // room for them and there is something to share
+    // room for them and there is something to share.  In us, top-k 50 and 0.9 (0.9 alone):
+    //   256 rows of 32000: 64 KB each 45 (106), 32 KB 49 (103), 128 KB 57 (159); 128 rows 23
+    //   (83), 26 (70), 23 (83); 512 rows of 128256, 8 CTAs each: 217 (676), 128 KB 208 (814)
+    //   1 row of 32000 by 8 CTAs 13.8 (22), by the 2 that hold it 17 (33); 32 rows 18.5 (40), 20
+    //   (75); 64 rows by 4, for which there is room, 19 (53), by 2 20.5 (78), by 8 27 (57); 256
+    //   rows by 2 45 (106), by 8 86 (164)
     constexpr int kSlab = kThreads * 16 / sizeof(T);
     const int64_t slots = 2ll * sm_count;
     a.ctas = 1;

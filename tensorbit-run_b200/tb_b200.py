@@ -1080,8 +1080,9 @@ def mx_dequantize(t, dtype=None, out=None, stream=None):
 def residual_rms_norm_mx(x, residual, weight, eps, h_out=None, format=None, out=None,
                          stream=None):
     """(h, y): residual_rms_norm of [rows, cols] with y in a microscaled format (`format`, or
-    out's; e4m3 without both) (tb_b200_residual_rms_norm_mx).  residual None: the norm of x, with no h; h is a new
-    tensor unless h_out is given (x or residual may be)."""
+    out's; e4m3 without both) (tb_b200_residual_rms_norm_mx): h / sqrt((eps + sum h^2) / cols),
+    so a model whose norm has mean(h^2) + eps gives cols * eps.  residual None: the norm of x,
+    with no h; h is a new tensor unless h_out is given (x or residual may be)."""
     torch, dev = _here()
     stream, other = _stream(torch, dev, stream)
     code, _ = _rows(x, dev, "x")
